@@ -319,6 +319,42 @@ int gdn2_attn_decode(const void *qkv, const float *cos, const float *sin, int ro
                      void *stream);
 
 /*
+ * Softmax attention over whole sequences and its gradient: the multi-token
+ * path of the hybrid host's attention layers (CausalSelfAttention.forward,
+ * reference src/qwendopamine/models/gdn2_gpt/model.py:89-173) in training and
+ * prefill, grouped heads read in place (no repeated k, v).
+ *   q [B, Tq, H, D], k, v [B, Tk, G, D] io_dtype, H a multiple of G: `strides`
+ *            is a host array of nine element strides (batch, token, head of q,
+ *            then of k, then of v), channels contiguous, rows 16-byte aligned
+ *   o        [B, Tq, H, D], contiguous: softmax(scale q k^T) v
+ *   o_lo     like o: what rounding o to io_dtype left out, for the backward (NULL
+ *            in a forward without one)
+ *   lse      [B, H, Tq] fp32: base-2 logarithm of sum exp(scale q k^T)
+ * Query i sees key j < kv_lengths[b] (device int64 [B], clamped to [0, Tk]; NULL:
+ * all Tk keys); with causal != 0 only j <= i + Tk - Tq (the queries are the last
+ * Tq positions).  With cu_seqlens (device int64 [num_seqs + 1], and its host
+ * copy; B = 1, Tq = Tk, no kv_lengths) sequences are packed along the tokens,
+ * each attending within itself.  A query that sees no key gets zeros (and
+ * lse = +inf), and gradients of zero.  Keys outside a row's length or sequence
+ * are not read; a hidden key inside it must be finite (0 * inf is NaN).
+ * gdn2_attn_bwd writes dq (like o) and dk, dv [B, Tk, G, D] contiguous, summed
+ * over the query heads of a group, from o, o_lo and lse of the forward and dout
+ * [B, Tq, H, D] contiguous; the probabilities are recomputed.  Every output has
+ * the same bits in every run.  bf16 / fp16, D in {64, 128}, scale > 0; else
+ * GDN2_ERR_UNSUPPORTED.
+ */
+int gdn2_attn_fwd(const void *q, const void *k, const void *v, const int64_t *strides, void *o, void *o_lo, float *lse,
+                  int io_dtype, const int64_t *kv_lengths, const int64_t *cu_seqlens,
+                  const int64_t *cu_seqlens_host, int num_seqs, int B, int Tq, int Tk, int H, int G, int D,
+                  float scale, int causal, void *stream);
+size_t gdn2_attn_bwd_workspace_size(int B, int Tq, int H, int G);
+int gdn2_attn_bwd(const void *q, const void *k, const void *v, const int64_t *strides, const void *o,
+                  const void *o_lo, const float *lse, const void *dout, void *dq, void *dk, void *dv, int io_dtype,
+                  const int64_t *kv_lengths, const int64_t *cu_seqlens, const int64_t *cu_seqlens_host,
+                  int num_seqs, int B, int Tq, int Tk, int H, int G, int D, float scale, int causal,
+                  void *workspace, size_t workspace_bytes, void *stream);
+
+/*
  * Greedy decoding's argmax over the LM head's logits (the logits of reference
  * src/qwendopamine/models/gdn2_gpt/model.py:304-380, GPT.forward; the
  * reference has no decoding loop, the hybrid host's greedy decoder calls this

@@ -445,6 +445,103 @@ int gdn2_attn_decode(const void *qkv, const float *cos, const float *sin, int ro
     return err == hipSuccess ? GDN2_OK : GDN2_ERR_LAUNCH;
 }
 
+// Shared by gdn2_attn_fwd and gdn2_attn_bwd: checks, and the parameters both take.
+static int fill_attn_args(AttnTrainParams &p, const void *q, const void *k, const void *v, const int64_t *strides,
+                          int io_dtype, const int64_t *kv_lengths, const int64_t *cu, const int64_t *cu_host,
+                          int num_seqs, int B, int Tq, int Tk, int H, int G, int D, float scale, int causal)
+{
+    if (!valid_dtype(io_dtype) || B < 0 || Tq < 0 || Tk < 0 || H < 1 || G < 1 || D < 1 || H % G != 0)
+        return GDN2_ERR_INVALID;
+    if (!strides || (cu == nullptr) != (cu_host == nullptr)) return GDN2_ERR_INVALID;
+    if (!attn_train_supported(io_dtype, D)) return GDN2_ERR_UNSUPPORTED;
+    if (!(scale > 0.0f) || scale > 1e30f) return GDN2_ERR_UNSUPPORTED;
+    p.max_q = Tq;
+    if (cu) {
+        if (B != 1 || Tq != Tk || kv_lengths || num_seqs < 0) return GDN2_ERR_INVALID;
+        if (cu_host[0] != 0 || cu_host[num_seqs] != Tq) return GDN2_ERR_INVALID;
+        p.max_q = 0;
+        for (int i = 0; i < num_seqs; ++i) {
+            const int64_t n = cu_host[i + 1] - cu_host[i];
+            if (n < 0 || n > Tq) return GDN2_ERR_INVALID;
+            if (n > p.max_q) p.max_q = static_cast<int>(n);
+        }
+    }
+    if ((B > 0 && Tq > 0 && !q) || (B > 0 && Tk > 0 && (!k || !v))) return GDN2_ERR_INVALID;
+    if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15)
+        return GDN2_ERR_INVALID;
+    const int size[9] = {B, Tq, H, B, Tk, G, B, Tk, G};
+    for (int i = 0; i < 9; ++i) {
+        if (strides[i] < 0 || (size[i] > 1 && strides[i] % 8 != 0)) return GDN2_ERR_INVALID;
+        (i < 3 ? p.qs : i < 6 ? p.ks : p.vs)[i % 3] = strides[i];
+    }
+    p.nseq = cu ? num_seqs : B;
+    // One launch of at most 2^31 - 1 workgroups, the smallest of them 32 rows.
+    const int64_t longest = p.max_q > Tk ? p.max_q : Tk;
+    if (Tq > (1 << 30) || Tk > (1 << 30) || (longest / 32 + 1) * static_cast<int64_t>(p.nseq) * H > 2147483647LL ||
+        static_cast<int64_t>(B) * Tq * H > (static_cast<int64_t>(1) << 34))
+        return GDN2_ERR_UNSUPPORTED;
+    p.q = q; p.k = k; p.v = v;
+    p.kv_len = kv_lengths;
+    p.cu = cu;
+    p.B = B; p.Tq = Tq; p.Tk = Tk; p.H = H; p.G = G; p.D = D;
+    p.causal = causal != 0;
+    p.scale = scale;
+    return GDN2_OK;
+}
+
+int gdn2_attn_fwd(const void *q, const void *k, const void *v, const int64_t *strides, void *o, void *o_lo, float *lse,
+                  int io_dtype, const int64_t *kv_lengths, const int64_t *cu_seqlens,
+                  const int64_t *cu_seqlens_host, int num_seqs, int B, int Tq, int Tk, int H, int G, int D,
+                  float scale, int causal, void *stream)
+{
+    AttnTrainParams p = {};
+    const int st = fill_attn_args(p, q, k, v, strides, io_dtype, kv_lengths, cu_seqlens, cu_seqlens_host, num_seqs, B,
+                                  Tq, Tk, H, G, D, scale, causal);
+    if (st != GDN2_OK) return st;
+    if (B == 0 || Tq == 0 || p.nseq == 0) return GDN2_OK;
+    if (!o || !lse || ((reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(o_lo)) & 15)) return GDN2_ERR_INVALID;
+    p.o = o;
+    p.o_lo = o_lo;
+    p.lse = lse;
+    return launch_attn_fwd(p, io_dtype, static_cast<hipStream_t>(stream)) == hipSuccess ? GDN2_OK : GDN2_ERR_LAUNCH;
+}
+
+size_t gdn2_attn_bwd_workspace_size(int B, int Tq, int H, int G)
+{
+    if (B < 0 || Tq < 0 || H < 1 || G < 1) return 0;
+    return attn_bwd_workspace_bytes(B, Tq, H, G);
+}
+
+int gdn2_attn_bwd(const void *q, const void *k, const void *v, const int64_t *strides, const void *o,
+                  const void *o_lo, const float *lse, const void *dout, void *dq, void *dk, void *dv, int io_dtype,
+                  const int64_t *kv_lengths, const int64_t *cu_seqlens, const int64_t *cu_seqlens_host,
+                  int num_seqs, int B, int Tq, int Tk, int H, int G, int D, float scale, int causal,
+                  void *workspace, size_t workspace_bytes, void *stream)
+{
+    AttnTrainParams p = {};
+    const int st = fill_attn_args(p, q, k, v, strides, io_dtype, kv_lengths, cu_seqlens, cu_seqlens_host, num_seqs, B,
+                                  Tq, Tk, H, G, D, scale, causal);
+    if (st != GDN2_OK) return st;
+    if (B == 0 || p.nseq == 0 || (Tq == 0 && Tk == 0)) return GDN2_OK;
+    if ((Tq > 0 && (!o || !o_lo || !lse || !dout || !dq)) || (Tk > 0 && (!dk || !dv))) return GDN2_ERR_INVALID;
+    if ((reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(o_lo) | reinterpret_cast<uintptr_t>(dout) | reinterpret_cast<uintptr_t>(dq) |
+         reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv)) & 15)
+        return GDN2_ERR_INVALID;
+    if (!workspace || workspace_bytes < attn_bwd_workspace_bytes(B, Tq, H, G) ||
+        (reinterpret_cast<uintptr_t>(workspace) & 15))
+        return GDN2_ERR_WORKSPACE;
+    p.o = const_cast<void *>(o);
+    p.o_lo = const_cast<void *>(o_lo);
+    p.lse = const_cast<float *>(lse);
+    p.dout = dout;
+    p.dq = dq; p.dk = dk; p.dv = dv;
+    p.delta = static_cast<float *>(workspace);
+    p.mx_do = reinterpret_cast<unsigned *>(static_cast<char *>(workspace) +
+                                           ((static_cast<size_t>(B) * H * Tq * sizeof(float) + 15) & ~static_cast<size_t>(15)));
+    p.mx_v = p.mx_do + static_cast<size_t>(B) * H;
+    return launch_attn_bwd(p, io_dtype, static_cast<hipStream_t>(stream)) == hipSuccess ? GDN2_OK : GDN2_ERR_LAUNCH;
+}
+
 size_t gdn2_gate_bwd_workspace_size(int64_t tokens, int H, int K, int has_dt_bias)
 {
     if (tokens < 0 || H <= 0 || K <= 0 || K > 256) return 0;

@@ -1,0 +1,744 @@
+// Softmax attention over whole sequences with its gradient, gfx950: the
+// training and prefill side of the hybrid decoder host's attention layers.
+//
+//   S = scale Q K^T, hidden keys at -inf, P = softmax(S), O = P V
+//   L = log sum exp(S) (kept per query), D = dO . O
+//   dV = P^T dO,  dS = P (dO V^T - D),  dQ = scale dS K,  dK = scale dS^T Q
+//
+// The probabilities are never stored: the forward makes one pass over the keys
+// with a running maximum and sum, the backward recomputes P = exp(S - L) tile
+// by tile, once with the queries resident (dQ) and once with the keys resident
+// (dK, dV, summed over the query heads of a group in registers).  Every output
+// element is summed by one wave in a fixed order: no atomics on values, the
+// same bits in every run.
+//
+// Layout of the products (v_mfma_f32_32x32x16): lane l = n + 32 h (n < 32,
+// h < 2) supplies contraction indices 8 h + j (j < 8) of row / column n, and
+// the accumulator element i holds row 8 (i / 4) + 4 h + i % 4 of column n.
+// The resident side (32 queries, or 32 keys, per wave) is always the column:
+// softmax statistics are then per-lane scalars, and an accumulator feeds the
+// next product as its B operand unmoved, since elements 8 t .. 8 t + 7 of half
+// h are the contraction indices 16 t + {4 h + 0..3, 8 + 4 h + 0..3} and the
+// A operand is read with the same assignment.  The streamed side lies in LDS
+// row-major and serves both products: rows by 16-byte reads, columns by
+// ds_read_b64_tr_b16 (a 16-lane group reads 4 rows x 16 columns and each lane
+// receives one column's 4 rows).
+#include "gdn2_common.h"
+#include "gdn2_internal.h"
+#include "gdn2_mfma.h"
+
+namespace gdn2 {
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+// Reference maximum before any key has been seen: finite, so that the
+// exponent of a hidden score (-inf) is -inf and never inf - inf.
+constexpr float kNoMax = -3.0e38f;
+// The running maximum moves only when a score exceeds it by 2^kLazy: until
+// then the probabilities are at most 2^kLazy, exact in the same number of
+// bits, and the accumulators need no rescaling.
+constexpr float kLazy = 8.0f;
+constexpr int kTile = 64;  // rows of the streamed side per LDS tile
+
+template <PrecKind PK>
+__device__ __forceinline__ f32x16 mma32(f32x16 acc, uint4 a, uint4 b)
+{
+    if constexpr (PK == PrecKind::BF16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b),
+                                                       acc, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b),
+                                                      acc, 0, 0, 0);
+}
+
+__device__ __forceinline__ f32x16 zero16()
+{
+    f32x16 z;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) z[i] = 0.0f;
+    return z;
+}
+
+// Elements 8 t .. 8 t + 7 of an accumulator, rounded to the operand type: the
+// B operand of the next product.
+template <PrecKind PK>
+__device__ __forceinline__ uint4 pack8(const f32x16 &x, int t)
+{
+    const Q4<PK> lo = pack4<PK>(x[8 * t], x[8 * t + 1], x[8 * t + 2], x[8 * t + 3]);
+    const Q4<PK> hi = pack4<PK>(x[8 * t + 4], x[8 * t + 5], x[8 * t + 6], x[8 * t + 7]);
+    return make_uint4(lo.u.x, lo.u.y, hi.u.x, hi.u.y);
+}
+
+// The other half's value (lane l ^ 32) combined with this lane's.
+__device__ __forceinline__ float half_max(float x)
+{
+    const unsigned u = __float_as_uint(x);
+    const auto s = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+
+__device__ __forceinline__ float half_add(float x)
+{
+    const unsigned u = __float_as_uint(x);
+    const auto s = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+
+// LDS tile [rows][D]: a row's 16-byte pieces are permuted by XOR with
+// swz(row), which differs in its upper bits over 4 consecutive rows (a column
+// read touches 4 rows x 2 pieces) and in all of its bits over 8 (a row read
+// touches 8 rows x 1 piece per LDS cycle).
+template <int D>
+__device__ __forceinline__ int swz(int row)
+{
+    return (((row & 3) << 1) | ((row >> 2) & 1) | (row & 8)) & (D / 8 - 1);
+}
+
+// One tile, row0 .. row0 + kTile - 1 of nrows rows ts elements apart, requested
+// into LDS.  Rows past the end repeat the last row (never out of bounds, never
+// another sequence's row); the scores of such rows are hidden.
+template <int D, int NW>
+__device__ __forceinline__ void stage(const uint16_t *base, int64_t ts, int row0, int nrows, uint16_t *lds, int wave,
+                                      int lane)
+{
+    constexpr int P = D / 8, R = 64 / P, IT = kTile / R;  // pieces per row, rows per request, requests
+#pragma unroll
+    for (int it = 0; it < (IT + NW - 1) / NW; ++it) {
+        const int c = it * NW + wave;
+        if (IT % NW != 0 && c >= IT) break;
+        const int r = c * R + lane / P;
+        const int piece = (lane % P) ^ swz<D>(r);
+        const int gr = row0 + r < nrows ? row0 + r : nrows - 1;
+        __builtin_amdgcn_global_load_lds(reinterpret_cast<const char *>(base + gr * ts + piece * 8), lds + c * R * D, 16,
+                                         0, 0);
+    }
+}
+
+// A operand, rows r0 + (l & 31), contraction step s of the row (16 channels).
+template <int D>
+__device__ __forceinline__ uint4 row_frag(const uint16_t *lds, int r0, int s, int lane)
+{
+    const int row = r0 + (lane & 31);
+    return *reinterpret_cast<const uint4 *>(lds + row * D + (((2 * s + (lane >> 5)) ^ swz<D>(row)) * 8));
+}
+
+// A operand of the transposed tile: channels 32 dt + (l & 31), contraction
+// over rows r0 + {4 h + 0..3, 8 + 4 h + 0..3}.
+template <int D>
+__device__ __forceinline__ uint4 col_frag(const uint16_t *lds, int r0, int dt, int lane)
+{
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s4 *lds_s4;
+    const int i = lane & 15, grp = (lane >> 4) & 1, h = lane >> 5;
+    uint2 r[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int row = r0 + 8 * u + 4 * h + (i >> 2);
+        const int piece = (dt * 4 + grp * 2 + ((i & 3) >> 1)) ^ swz<D>(8 * u + 4 * h + (i >> 2));
+        r[u] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                             (lds_s4)(lds + row * D + piece * 8 + (i & 1) * 4)));
+    }
+    return make_uint4(r[0].x, r[0].y, r[1].x, r[1].y);
+}
+
+// What a workgroup works on: head h of sequence s, its rows and their extent.
+struct Where {
+    int s, h, g, tile;
+    int64_t q0, k0;  // first query / key token within the batch row
+    int bq, bk;      // batch row of q and k
+    int nq, nk;      // queries, visible keys
+    int shift;       // causal: query i sees keys j <= i + shift
+};
+
+__device__ __forceinline__ void where_rows(const AttnTrainParams &p, Where &w)
+{
+    if (p.cu) {
+        const int64_t a = p.cu[w.s], b = p.cu[w.s + 1];
+        w.q0 = w.k0 = a;
+        w.bq = w.bk = 0;
+        w.nq = w.nk = static_cast<int>(b - a);
+        w.shift = 0;
+    } else {
+        w.q0 = w.k0 = 0;
+        w.bq = w.bk = w.s;
+        w.nq = p.Tq;
+        w.nk = p.Tk;
+        w.shift = p.Tk - p.Tq;
+        if (p.kv_len) {
+            const int64_t n = p.kv_len[w.s];
+            w.nk = n < 0 ? 0 : (n < p.Tk ? static_cast<int>(n) : p.Tk);
+        }
+    }
+}
+
+// Query-resident kernels: heads of a group next to each other in the order of
+// workgroups modulo 8 (the XCDs), long causal tiles first.
+__device__ __forceinline__ Where where_q(const AttnTrainParams &p)
+{
+    Where w;
+    const int nbh = p.nseq * p.H;
+    const int t = blockIdx.x / nbh, j = blockIdx.x - t * nbh;
+    w.s = j / p.H;
+    const int jh = j - w.s * p.H;
+    w.g = jh % p.G;
+    w.h = w.g * (p.H / p.G) + jh / p.G;
+    w.tile = p.tiles - 1 - t;
+    where_rows(p, w);
+    return w;
+}
+
+// exp2 of a tile's scaled scores relative to ref, hidden keys to 0.  keys of
+// the accumulator: j0 + 8 (i / 4) + 4 h + i % 4.
+template <bool MASK>
+__device__ __forceinline__ void hide(f32x16 &s, int j0, int h, int limit)
+{
+    if constexpr (MASK) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int j = j0 + 8 * (i >> 2) + 4 * h + (i & 3);
+            s[i] = j < limit ? s[i] : -INFINITY;
+        }
+    }
+}
+
+// ---------------------------------------------------------------- forward
+
+template <PrecKind PK, int D, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(AttnTrainParams p)
+{
+    constexpr int KS = D / 16, DT = D / 32, BM = 32 * NW;
+    __shared__ __align__(16) uint16_t sk[2][kTile * D];
+    __shared__ __align__(16) uint16_t sv[2][kTile * D];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 31, h = lane >> 5;
+    const Where w = where_q(p);
+    const int m0 = w.tile * BM;
+    if (m0 >= w.nq) return;
+    const int qi = m0 + 32 * wave + n;  // this lane's query
+    const int qc = qi < w.nq ? qi : w.nq - 1;
+    const uint16_t *kb = static_cast<const uint16_t *>(p.k) + w.bk * p.ks[0] + w.k0 * p.ks[1] + w.g * p.ks[2];
+    const uint16_t *vb = static_cast<const uint16_t *>(p.v) + w.bk * p.vs[0] + w.k0 * p.vs[1] + w.g * p.vs[2];
+    const uint16_t *qr = static_cast<const uint16_t *>(p.q) + w.bq * p.qs[0] + (w.q0 + qc) * p.qs[1] + w.h * p.qs[2];
+    uint4 qf[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const uint4 *>(qr + 16 * s + 8 * h);
+
+    // Keys of the workgroup, of this wave and of this lane.
+    int kend = w.nk;
+    if (p.causal) {
+        const int last = (m0 + BM < w.nq ? m0 + BM : w.nq) + w.shift;
+        kend = last < kend ? last : kend;
+    }
+    const int lim = p.causal && qi + w.shift + 1 < w.nk ? qi + w.shift + 1 : w.nk;
+    const int wmin = m0 + 32 * wave, wmax = wmin + 31;
+    const int wlim = p.causal && wmin + w.shift + 1 < w.nk ? wmin + w.shift + 1 : w.nk;  // all of the wave see these
+    const int wend = p.causal && wmax + w.shift + 1 < w.nk ? wmax + w.shift + 1 : w.nk;  // none sees more
+    const float c = p.scale * kLog2e;
+
+    float m = kNoMax, l = 0.0f;
+    f32x16 acc[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d) acc[d] = zero16();
+
+    const int nt = kend > 0 ? (kend + kTile - 1) / kTile : 0;
+    if (nt > 0) {
+        stage<D, NW>(kb, p.ks[1], 0, w.nk, sk[0], wave, lane);
+        stage<D, NW>(vb, p.vs[1], 0, w.nk, sv[0], wave, lane);
+    }
+    for (int t = 0; t < nt; ++t) {
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();  // tile t has landed, and every wave is done with tile t - 1
+        if (t + 1 < nt) {
+            stage<D, NW>(kb, p.ks[1], (t + 1) * kTile, w.nk, sk[(t + 1) & 1], wave, lane);
+            stage<D, NW>(vb, p.vs[1], (t + 1) * kTile, w.nk, sv[(t + 1) & 1], wave, lane);
+        }
+        const int j0 = t * kTile;
+        if (j0 >= wend) continue;
+        const uint16_t *kt = sk[t & 1], *vt = sv[t & 1];
+        f32x16 s[2];
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+            s[a] = zero16();
+#pragma unroll
+            for (int st = 0; st < KS; ++st) s[a] = mma32<PK>(s[a], row_frag<D>(kt, 32 * a, st, lane), qf[st]);
+        }
+        if (j0 + kTile > wlim) {
+            hide<true>(s[0], j0, h, lim);
+            hide<true>(s[1], j0 + 32, h, lim);
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, fmaxf(s[0][i], s[1][i]));
+        mx = half_max(mx) * c;
+        if (__any(mx > m + kLazy)) {
+            const float mn = fmaxf(m, mx);
+            const float r = __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= r;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[d][i] *= r;
+        }
+        float sum = 0.0f;
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[a][i] = __builtin_amdgcn_exp2f(fmaf(s[a][i], c, -m));
+                sum += s[a][i];
+            }
+        l += sum;
+        // The probabilities are rounded to the operand type for this product
+        // (their sum l is not): a relative error of half a step each, as large
+        // as the rounding of V itself and averaged over the keys.
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const uint4 pf = pack8<PK>(s[a], u);
+#pragma unroll
+                for (int d = 0; d < DT; ++d) acc[d] = mma32<PK>(acc[d], col_frag<D>(vt, 32 * a + 16 * u, d, lane), pf);
+            }
+    }
+    l = half_add(l);
+    if (qi >= w.nq) return;
+    // A query that sees no key: zeros, and L = +inf, which makes its recomputed P zero.
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    if (h == 0)
+        p.lse[(static_cast<int64_t>(w.bq) * p.H + w.h) * p.Tq + w.q0 + qi] =
+            l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
+    const int64_t row = ((w.bq * static_cast<int64_t>(p.Tq) + w.q0 + qi) * p.H + w.h) * D;
+    uint16_t *o = static_cast<uint16_t *>(p.o) + row, *ol = static_cast<uint16_t *>(p.o_lo) + row;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float y[4] = {acc[d][4 * i] * inv, acc[d][4 * i + 1] * inv, acc[d][4 * i + 2] * inv,
+                                acc[d][4 * i + 3] * inv};
+            const Q4<PK> r = pack4<PK>(y[0], y[1], y[2], y[3]);
+            st_q4<PK>(o + 32 * d + 8 * i + 4 * h, r);
+            if (p.o_lo) {
+                // What the rounding left out, for D = dO . O: without it D is
+                // off by half a step of O, which shows in dS where few keys
+                // carry the weight and dP - D cancels.
+                float z[4];
+                unpack4<PK>(r, z);
+                st_q4<PK>(ol + 32 * d + 8 * i + 4 * h, pack4<PK>(y[0] - z[0], y[1] - z[1], y[2] - z[2], y[3] - z[3]));
+            }
+        }
+}
+
+// ---------------------------------------------------------------- backward
+
+// D = dO . O per query (fp32), one 16-byte piece per lane.  fp16 also leaves
+// the largest squared row norm of dO per (row of the batch, head), from which
+// and from V's the kernels below scale dS into fp16's range (norm_max_kernel).
+template <PrecKind PK, int D>
+__global__ __launch_bounds__(256) void attn_delta_kernel(AttnTrainParams p)
+{
+    constexpr int P = D / 8;
+    const int64_t row = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / P;  // (b * Tq + t) * H + h
+    const int piece = threadIdx.x % P;
+    const int64_t rows = static_cast<int64_t>(p.B) * p.Tq * p.H;
+    if (row >= rows) return;  // whole groups of P lanes
+    const int hh = static_cast<int>(row % p.H);
+    const int64_t bt = row / p.H;
+    const int b = static_cast<int>(bt / p.Tq), t = static_cast<int>(bt % p.Tq);
+    typename Prec<PK>::frag fo, fl, fd;
+    fo.u = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.o) + row * D + piece * 8);
+    fl.u = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.o_lo) + row * D + piece * 8);
+    fd.u = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.dout) + row * D + piece * 8);
+    float xo[8], xl[8], xd[8];
+    unpack_frag<PK>(fo, xo);
+    unpack_frag<PK>(fl, xl);
+    unpack_frag<PK>(fd, xd);
+    float s = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s = fmaf(xo[e] + xl[e], xd[e], s);
+#pragma unroll
+    for (int k = 1; k < P; k <<= 1) s += __shfl_xor(s, k, 64);
+    if (piece == 0) p.delta[(static_cast<int64_t>(b) * p.H + hh) * p.Tq + t] = s;
+}
+
+// fp16 only: the largest squared row norm of x [B, T, heads, D] per (b, head)
+// into mx [B][heads] (cleared before), by integer maxima of the float bits
+// (non-negative floats order as integers, so the order of arrival does not
+// matter).  Rows that are not finite, or past len[b], do not count.
+constexpr int kNormParts = 4;  // workgroups per (b, head)
+template <int D>
+__global__ __launch_bounds__(256) void norm_max_kernel(const uint16_t *x, int64_t sb, int64_t st, int64_t sh, int T,
+                                                       const int64_t *len, int heads, unsigned *mx)
+{
+    constexpr int P = D / 8, R = 256 / P;
+    const int bh = blockIdx.x % (gridDim.x / kNormParts), part = blockIdx.x / (gridDim.x / kNormParts);
+    const int b = bh / heads, hh = bh - b * heads;
+    if (len && len[b] < T) T = static_cast<int>(len[b] < 0 ? 0 : len[b]);
+    const int piece = threadIdx.x % P;
+    float best = 0.0f;
+    for (int t = part * R + threadIdx.x / P; t < T; t += kNormParts * R) {
+        typename Prec<PrecKind::F16>::frag f;
+        f.u = *reinterpret_cast<const uint4 *>(x + b * sb + t * st + hh * sh + piece * 8);
+        float v[8];
+        unpack_frag<PrecKind::F16>(f, v);
+        float s = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s = fmaf(v[e], v[e], s);
+#pragma unroll
+        for (int k = 1; k < P; k <<= 1) s += __shfl_xor(s, k, 64);
+        best = s < INFINITY ? fmaxf(best, s) : best;
+    }
+#pragma unroll
+    for (int k = 32; k > 0; k >>= 1) best = fmaxf(best, __shfl_xor(best, k, 64));
+    if ((threadIdx.x & 63) == 0) atomicMax(mx + bh, __float_as_uint(best));
+}
+
+__global__ __launch_bounds__(256) void clear_kernel(unsigned *x, int n)
+{
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i < n) x[i] = 0u;
+}
+
+// fp16: P is held scaled by 2^kP16 (P = 1 / T of long rows stays a normal
+// number), dS by a power of two that brings 2 max |dO_i| max |v_j|, its bound,
+// to 2^14.  Exact scalings, undone in fp32.
+constexpr float kP16 = 14.0f;
+
+template <PrecKind PK>
+__device__ __forceinline__ float ds_scale(const AttnTrainParams &p, const Where &w)
+{
+    if constexpr (PK != PrecKind::F16) return 1.0f;
+    const float a = __uint_as_float(p.mx_do[w.bq * p.H + w.h]), b = __uint_as_float(p.mx_v[w.bk * p.G + w.g]);
+    const float bound = 2.0f * sqrtf(a) * sqrtf(b);
+    if (!(bound > 0.0f)) return 1.0f;
+    int e = 13 - ilogbf(bound);
+    e = e < -60 ? -60 : (e > 100 ? 100 : e);
+    return ldexpf(1.0f, e);
+}
+
+// dQ: queries resident, one pass over the keys.
+template <PrecKind PK, int D, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void attn_dq_kernel(AttnTrainParams p)
+{
+    constexpr int KS = D / 16, DT = D / 32, BM = 32 * NW;
+    __shared__ __align__(16) uint16_t sk[2][kTile * D];
+    __shared__ __align__(16) uint16_t sv[2][kTile * D];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 31, h = lane >> 5;
+    const Where w = where_q(p);
+    const int m0 = w.tile * BM;
+    if (m0 >= w.nq) return;
+    const int qi = m0 + 32 * wave + n;
+    const int qc = qi < w.nq ? qi : w.nq - 1;
+    const uint16_t *kb = static_cast<const uint16_t *>(p.k) + w.bk * p.ks[0] + w.k0 * p.ks[1] + w.g * p.ks[2];
+    const uint16_t *vb = static_cast<const uint16_t *>(p.v) + w.bk * p.vs[0] + w.k0 * p.vs[1] + w.g * p.vs[2];
+    const uint16_t *qr = static_cast<const uint16_t *>(p.q) + w.bq * p.qs[0] + (w.q0 + qc) * p.qs[1] + w.h * p.qs[2];
+    const int64_t orow = ((w.bq * static_cast<int64_t>(p.Tq) + w.q0 + qc) * p.H + w.h) * D;
+    const uint16_t *dr = static_cast<const uint16_t *>(p.dout) + orow;
+    const int64_t srow = (static_cast<int64_t>(w.bq) * p.H + w.h) * p.Tq + w.q0 + qc;
+    uint4 qf[KS], df[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+        qf[s] = *reinterpret_cast<const uint4 *>(qr + 16 * s + 8 * h);
+        df[s] = *reinterpret_cast<const uint4 *>(dr + 16 * s + 8 * h);
+    }
+    const float sc = ds_scale<PK>(p, w);
+    const float lse = p.lse[srow], dl = p.delta[srow] * sc;
+
+    int kend = w.nk;
+    if (p.causal) {
+        const int last = (m0 + BM < w.nq ? m0 + BM : w.nq) + w.shift;
+        kend = last < kend ? last : kend;
+    }
+    const int lim = p.causal && qi + w.shift + 1 < w.nk ? qi + w.shift + 1 : w.nk;
+    const int wmin = m0 + 32 * wave, wmax = wmin + 31;
+    const int wlim = p.causal && wmin + w.shift + 1 < w.nk ? wmin + w.shift + 1 : w.nk;
+    const int wend = p.causal && wmax + w.shift + 1 < w.nk ? wmax + w.shift + 1 : w.nk;
+    const float c = p.scale * kLog2e;
+
+    f32x16 acc[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d) acc[d] = zero16();
+    const int nt = kend > 0 ? (kend + kTile - 1) / kTile : 0;
+    if (nt > 0) {
+        stage<D, NW>(kb, p.ks[1], 0, w.nk, sk[0], wave, lane);
+        stage<D, NW>(vb, p.vs[1], 0, w.nk, sv[0], wave, lane);
+    }
+    for (int t = 0; t < nt; ++t) {
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        if (t + 1 < nt) {
+            stage<D, NW>(kb, p.ks[1], (t + 1) * kTile, w.nk, sk[(t + 1) & 1], wave, lane);
+            stage<D, NW>(vb, p.vs[1], (t + 1) * kTile, w.nk, sv[(t + 1) & 1], wave, lane);
+        }
+        const int j0 = t * kTile;
+        if (j0 >= wend) continue;
+        const uint16_t *kt = sk[t & 1], *vt = sv[t & 1];
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+            f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+            for (int st = 0; st < KS; ++st) s = mma32<PK>(s, row_frag<D>(kt, 32 * a, st, lane), qf[st]);
+#pragma unroll
+            for (int st = 0; st < KS; ++st) dp = mma32<PK>(dp, row_frag<D>(vt, 32 * a, st, lane), df[st]);
+            if (j0 + kTile > wlim) hide<true>(s, j0 + 32 * a, h, lim);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float pr = __builtin_amdgcn_exp2f(fmaf(s[i], c, -lse));
+                s[i] = pr * fmaf(dp[i], sc, -dl);
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const uint4 pf = pack8<PK>(s, u);
+#pragma unroll
+                for (int d = 0; d < DT; ++d) acc[d] = mma32<PK>(acc[d], col_frag<D>(kt, 32 * a + 16 * u, d, lane), pf);
+            }
+        }
+    }
+    if (qi >= w.nq) return;
+    const float f = p.scale / sc;
+    uint16_t *dq = static_cast<uint16_t *>(p.dq) + orow;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            st_q4<PK>(dq + 32 * d + 8 * i + 4 * h, pack4<PK>(acc[d][4 * i] * f, acc[d][4 * i + 1] * f,
+                                                             acc[d][4 * i + 2] * f, acc[d][4 * i + 3] * f));
+}
+
+// dK, dV: keys resident, one pass over the queries of every head of the group.
+template <PrecKind PK, int D, int NW>
+__global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : 1) void attn_dkv_kernel(AttnTrainParams p)
+{
+    constexpr int KS = D / 16, DT = D / 32, BN = 32 * NW;
+    __shared__ __align__(16) uint16_t sq[2][kTile * D];
+    __shared__ __align__(16) uint16_t sd[2][kTile * D];
+    __shared__ __align__(16) float sl[2][2][kTile];  // L and scaled D of the tile's queries
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 31, h = lane >> 5;
+    Where w;
+    const int nbg = p.nseq * p.G, qpk = p.H / p.G;
+    w.tile = blockIdx.x / nbg;
+    const int jg = blockIdx.x - w.tile * nbg;
+    w.s = jg / p.G;
+    w.g = jg - w.s * p.G;
+    w.h = w.g * qpk;
+    where_rows(p, w);
+    const int n0 = w.tile * BN;
+    const int kall = p.cu ? w.nk : p.Tk;  // rows that dk and dv have (hidden ones get zeros)
+    if (n0 >= kall) return;
+    const int kj = n0 + 32 * wave + n;  // this lane's key
+    const int kc = kj < w.nk ? kj : (w.nk > 0 ? w.nk - 1 : 0);
+    const uint16_t *kr = static_cast<const uint16_t *>(p.k) + w.bk * p.ks[0] + (w.k0 + kc) * p.ks[1] + w.g * p.ks[2];
+    const uint16_t *vr = static_cast<const uint16_t *>(p.v) + w.bk * p.vs[0] + (w.k0 + kc) * p.vs[1] + w.g * p.vs[2];
+    uint4 kf[KS], vf[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+        kf[s] = *reinterpret_cast<const uint4 *>(kr + 16 * s + 8 * h);
+        vf[s] = *reinterpret_cast<const uint4 *>(vr + 16 * s + 8 * h);
+    }
+    // First query that sees this lane's key, any of the wave's, all of the wave's.
+    const int big = 0x7fffffff;
+    const int first = kj >= w.nk ? big : (p.causal ? kj - w.shift : 0);
+    const int wk0 = n0 + 32 * wave;
+    const int wfirst = wk0 >= w.nk ? big : (p.causal ? wk0 - w.shift : 0);
+    const int wall = wk0 + 31 >= w.nk ? big : (p.causal ? wk0 + 31 - w.shift : 0);
+    int gfirst = n0 >= w.nk ? big : (p.causal ? n0 - w.shift : 0);
+    gfirst = gfirst < 0 ? 0 : gfirst;
+    const int t0 = gfirst / kTile;
+    const int nt = gfirst >= w.nq ? 0 : (w.nq + kTile - 1) / kTile - t0;
+    const float c = p.scale * kLog2e;
+    const float p16 = PK == PrecKind::F16 ? kP16 : 0.0f;
+
+    f32x16 dk[DT], dv[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+        dk[d] = zero16();
+        dv[d] = zero16();
+    }
+    // fp16: one scale for every head of the group, the smallest of theirs.
+    float sc = 1.0f;
+    if constexpr (PK == PrecKind::F16) {
+        sc = ds_scale<PK>(p, w);
+        for (int r = 1; r < qpk; ++r) {
+            Where o = w;
+            o.h = w.h + r;
+            sc = fminf(sc, ds_scale<PK>(p, o));
+        }
+    }
+    const float ds_mul = PK == PrecKind::F16 ? sc * ldexpf(1.0f, -14) : 1.0f;
+
+    const int steps = nt * qpk;
+    const uint16_t *qb = static_cast<const uint16_t *>(p.q) + w.bq * p.qs[0] + w.q0 * p.qs[1];
+    const uint16_t *db = static_cast<const uint16_t *>(p.dout) + (w.bq * static_cast<int64_t>(p.Tq) + w.q0) * p.H * D;
+    const int64_t sb = static_cast<int64_t>(w.bq) * p.H * p.Tq + w.q0;
+    // Step x: head x / nt of the group, query tile t0 + x % nt.
+    int rh = 0, rt = 0;  // of the step requested next
+    auto request = [&](int buf) __attribute__((always_inline)) {
+        const int hh = w.h + rh, row0 = (t0 + rt) * kTile;
+        stage<D, NW>(qb + hh * p.qs[2], p.qs[1], row0, w.nq, sq[buf], wave, lane);
+        stage<D, NW>(db + hh * D, static_cast<int64_t>(p.H) * D, row0, w.nq, sd[buf], wave, lane);
+        if (tid < 2 * kTile) {
+            const int r = row0 + (tid & (kTile - 1));
+            const float *src = (tid < kTile ? p.lse : p.delta) + sb + static_cast<int64_t>(hh) * p.Tq;
+            // Queries past the end: L = +inf hides them.
+            const float x = r < w.nq ? src[r] : (tid < kTile ? INFINITY : 0.0f);
+            sl[buf][tid < kTile ? 0 : 1][tid & (kTile - 1)] = tid < kTile ? x - p16 : x * ds_mul;
+        }
+        if (++rt == nt) {
+            rt = 0;
+            ++rh;
+        }
+    };
+    if (steps > 0) request(0);
+    int ct = 0;  // query tile of the current step
+    for (int x = 0; x < steps; ++x) {
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        if (x + 1 < steps) request((x + 1) & 1);
+        const int i0 = (t0 + ct) * kTile;
+        if (++ct == nt) ct = 0;
+        if (i0 + kTile <= wfirst) continue;
+        const uint16_t *qt = sq[x & 1], *dt = sd[x & 1];
+        const float *lt = sl[x & 1][0], *et = sl[x & 1][1];
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+            f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+            for (int st = 0; st < KS; ++st) s = mma32<PK>(s, row_frag<D>(qt, 32 * a, st, lane), kf[st]);
+            if (i0 < wall) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int qi = i0 + 32 * a + 8 * (i >> 2) + 4 * h + (i & 3);
+                    s[i] = qi >= first ? s[i] : -INFINITY;
+                }
+            }
+#pragma unroll
+            for (int st = 0; st < KS; ++st) dp = mma32<PK>(dp, row_frag<D>(dt, 32 * a, st, lane), vf[st]);
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const float4 lv = *reinterpret_cast<const float4 *>(lt + 32 * a + 8 * b + 4 * h);
+                const float ls[4] = {lv.x, lv.y, lv.z, lv.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[4 * b + i] = __builtin_amdgcn_exp2f(fmaf(s[4 * b + i], c, -ls[i]));
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const uint4 pf = pack8<PK>(s, u);
+#pragma unroll
+                for (int d = 0; d < DT; ++d) dv[d] = mma32<PK>(dv[d], col_frag<D>(dt, 32 * a + 16 * u, d, lane), pf);
+            }
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const float4 ev = *reinterpret_cast<const float4 *>(et + 32 * a + 8 * b + 4 * h);
+                const float es[4] = {ev.x, ev.y, ev.z, ev.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    s[4 * b + i] *= PK == PrecKind::F16 ? fmaf(dp[4 * b + i], ds_mul, -es[i]) : dp[4 * b + i] - es[i];
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const uint4 pf = pack8<PK>(s, u);
+#pragma unroll
+                for (int d = 0; d < DT; ++d) dk[d] = mma32<PK>(dk[d], col_frag<D>(qt, 32 * a + 16 * u, d, lane), pf);
+            }
+        }
+    }
+    if (kj >= kall) return;
+    const float fk = p.scale / sc, fv = PK == PrecKind::F16 ? ldexpf(1.0f, -14) : 1.0f;
+    const int64_t krow = ((w.bk * static_cast<int64_t>(p.Tk) + w.k0 + kj) * p.G + w.g) * D;
+    uint16_t *ok = static_cast<uint16_t *>(p.dk) + krow, *ov = static_cast<uint16_t *>(p.dv) + krow;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            st_q4<PK>(ok + 32 * d + 8 * i + 4 * h, pack4<PK>(dk[d][4 * i] * fk, dk[d][4 * i + 1] * fk,
+                                                             dk[d][4 * i + 2] * fk, dk[d][4 * i + 3] * fk));
+            st_q4<PK>(ov + 32 * d + 8 * i + 4 * h, pack4<PK>(dv[d][4 * i] * fv, dv[d][4 * i + 1] * fv,
+                                                             dv[d][4 * i + 2] * fv, dv[d][4 * i + 3] * fv));
+        }
+}
+
+template <PrecKind PK, int D>
+hipError_t fwd_d(AttnTrainParams p, hipStream_t s)
+{
+    constexpr int NW = 8;
+    p.tiles = (p.max_q + 32 * NW - 1) / (32 * NW);
+    hipLaunchKernelGGL((attn_fwd_kernel<PK, D, NW>), dim3(static_cast<unsigned>(p.tiles) * p.nseq * p.H), dim3(64 * NW),
+                       0, s, p);
+    return hipGetLastError();
+}
+
+template <PrecKind PK, int D>
+hipError_t bwd_d(AttnTrainParams p, hipStream_t s)
+{
+    constexpr int NW = 8;
+    hipError_t e;
+    if (p.Tq > 0) {
+        const int64_t rows = static_cast<int64_t>(p.B) * p.Tq * p.H;
+        hipLaunchKernelGGL((attn_delta_kernel<PK, D>), dim3(static_cast<unsigned>((rows * (D / 8) + 255) / 256)),
+                           dim3(256), 0, s, p);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
+    if constexpr (PK == PrecKind::F16) {
+        const int n = p.B * (p.H + p.G);
+        hipLaunchKernelGGL(clear_kernel, dim3((n + 255) / 256), dim3(256), 0, s, p.mx_do, n);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+        const int64_t HD = static_cast<int64_t>(p.H) * D;
+        if (p.Tq > 0) {
+            hipLaunchKernelGGL((norm_max_kernel<D>), dim3(kNormParts * p.B * p.H), dim3(256), 0, s,
+                               static_cast<const uint16_t *>(p.dout), p.Tq * HD, HD, static_cast<int64_t>(D), p.Tq,
+                               static_cast<const int64_t *>(nullptr), p.H, p.mx_do);
+            if ((e = hipGetLastError()) != hipSuccess) return e;
+        }
+        if (p.Tk > 0) {
+            hipLaunchKernelGGL((norm_max_kernel<D>), dim3(kNormParts * p.B * p.G), dim3(256), 0, s,
+                               static_cast<const uint16_t *>(p.v), p.vs[0], p.vs[1], p.vs[2], p.Tk, p.kv_len, p.G,
+                               p.mx_v);
+            if ((e = hipGetLastError()) != hipSuccess) return e;
+        }
+    }
+    if (p.Tk > 0) {
+        const int tiles = ((p.cu ? p.max_q : p.Tk) + 32 * NW - 1) / (32 * NW);
+        hipLaunchKernelGGL((attn_dkv_kernel<PK, D, NW>), dim3(static_cast<unsigned>(tiles) * p.nseq * p.G),
+                           dim3(64 * NW), 0, s, p);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
+    if (p.Tq > 0) {
+        p.tiles = (p.max_q + 32 * NW - 1) / (32 * NW);
+        hipLaunchKernelGGL((attn_dq_kernel<PK, D, NW>), dim3(static_cast<unsigned>(p.tiles) * p.nseq * p.H),
+                           dim3(64 * NW), 0, s, p);
+    }
+    return hipGetLastError();
+}
+
+}  // namespace
+
+bool attn_train_supported(int io_dtype, int D)
+{
+    return (io_dtype == GDN2_DTYPE_BF16 || io_dtype == GDN2_DTYPE_F16) && (D == 64 || D == 128);
+}
+
+size_t attn_bwd_workspace_bytes(int B, int Tq, int H, int G)
+{
+    const size_t delta = (static_cast<size_t>(B) * H * Tq * sizeof(float) + 15) & ~static_cast<size_t>(15);
+    return delta + static_cast<size_t>(B) * (H + G) * sizeof(unsigned);
+}
+
+hipError_t launch_attn_fwd(const AttnTrainParams &p, int io_dtype, hipStream_t s)
+{
+    if (io_dtype == GDN2_DTYPE_BF16)
+        return p.D == 64 ? fwd_d<PrecKind::BF16, 64>(p, s) : fwd_d<PrecKind::BF16, 128>(p, s);
+    return p.D == 64 ? fwd_d<PrecKind::F16, 64>(p, s) : fwd_d<PrecKind::F16, 128>(p, s);
+}
+
+hipError_t launch_attn_bwd(const AttnTrainParams &p, int io_dtype, hipStream_t s)
+{
+    if (io_dtype == GDN2_DTYPE_BF16)
+        return p.D == 64 ? bwd_d<PrecKind::BF16, 64>(p, s) : bwd_d<PrecKind::BF16, 128>(p, s);
+    return p.D == 64 ? bwd_d<PrecKind::F16, 64>(p, s) : bwd_d<PrecKind::F16, 128>(p, s);
+}
+
+}  // namespace gdn2

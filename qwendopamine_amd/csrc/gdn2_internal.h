@@ -302,6 +302,36 @@ int argmax_splits(int64_t n, int io_dtype);
 hipError_t launch_argmax_rows(const ArgmaxParams &p, int io_dtype, hipStream_t stream);
 hipError_t launch_attn_decode(const AttnDecodeParams &p, int io_dtype, hipStream_t stream);
 
+// Softmax attention over whole sequences and its gradient (the hybrid host's
+// attention layers in training and prefill).  q [B, Tq, H, D], k and v
+// [B, Tk, G, D] by strides (batch, token, head; elements, unit channel stride,
+// 16-byte aligned rows); o, dout, dq [B, Tq, H, D] and dk, dv [B, Tk, G, D]
+// contiguous; lse, delta [B, H, Tq] (lse: base-2 log of the softmax sum).
+// Query i sees key j < kv_len[b] (or Tk), with causal only j <= i + Tk - Tq; or,
+// with cu (B = 1, Tq = Tk), the keys of its own packed sequence, causal within it.
+struct AttnTrainParams {
+    const void *q, *k, *v;
+    int64_t qs[3], ks[3], vs[3];
+    void *o, *o_lo;  // o_lo: what rounding o left out (NULL in a forward without a backward)
+    float *lse;
+    const void *dout;
+    void *dq, *dk, *dv;
+    float *delta;
+    unsigned *mx_do, *mx_v;  // fp16: squared row norm maxima [B][H], [B][G]
+    const int64_t *kv_len;   // [B] or NULL
+    const int64_t *cu;       // [nseq + 1] or NULL
+    int nseq;                // B without cu
+    int max_q;               // longest sequence's queries
+    int tiles;               // set by the launcher
+    int B, Tq, Tk, H, G, D;
+    int causal;
+    float scale;
+};
+bool attn_train_supported(int io_dtype, int D);
+size_t attn_bwd_workspace_bytes(int B, int Tq, int H, int G);
+hipError_t launch_attn_fwd(const AttnTrainParams &p, int io_dtype, hipStream_t stream);
+hipError_t launch_attn_bwd(const AttnTrainParams &p, int io_dtype, hipStream_t stream);
+
 // Backward of the short convolution on a prefill call (no cache).
 struct ConvBwdParams {
     const void *x;      // [B, T, D] input rows: row (b, t) at x + (b * T + t) * ldx

@@ -23,6 +23,7 @@ from __future__ import annotations
 
 from typing import Any
 
+import contextlib
 import ctypes
 
 import torch
@@ -48,6 +49,8 @@ __all__ = [
     "linear_pair",
     "argmax_rows",
     "attention_decode",
+    "attention",
+    "AttentionFunction",
     "decode_step_fused",
 ]
 
@@ -1499,6 +1502,140 @@ def attention_decode(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, in
     )
     nat.check(st, name)
     return out
+
+
+def _on_device(device: torch.device):
+    """Context in which ``device`` is the current one (launches go to the current device);
+    free where it already is."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _head_rows(x: torch.Tensor) -> torch.Tensor:
+    """``x [B, T, heads, D]`` as the attention kernels read it: in place where its channels are
+    contiguous and every row starts on 16 bytes, else a contiguous copy."""
+    per = 16 // x.element_size()
+    if x.stride(3) == 1 and x.data_ptr() % 16 == 0 and all(
+            x.stride(i) % per == 0 for i in range(3) if x.shape[i] > 1):
+        return x
+    x = x.contiguous()
+    return x if x.data_ptr() % 16 == 0 else x.clone()
+
+
+def attention_supported(q: torch.Tensor, head_dim: int) -> bool:
+    """Whether :func:`attention` takes this dtype and head size."""
+    return q.is_cuda and q.dtype in (torch.bfloat16, torch.float16) and head_dim in (64, 128)
+
+
+class AttentionFunction(torch.autograd.Function):
+    """:func:`attention` with the HIP forward and backward (``gdn2_attn_fwd`` / ``gdn2_attn_bwd``):
+    the output (with what its rounding left out) and the softmax's log sums are kept, the
+    probabilities are recomputed."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, scale: float, causal: bool, kv_len, cu_dev, cu_host):
+        q, k, v = _head_rows(q), _head_rows(k), _head_rows(v)
+        B, Tq, H, D = q.shape
+        Tk, G = k.shape[1], k.shape[2]
+        o = torch.empty(B, Tq, H, D, dtype=q.dtype, device=q.device)
+        o_lo = torch.empty_like(o) if any(ctx.needs_input_grad) else None
+        lse = torch.empty(B, H, Tq, dtype=torch.float32, device=q.device)
+        strides = (ctypes.c_int64 * 9)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
+        n = 0 if cu_host is None else cu_host.numel() - 1
+        with _on_device(q.device):
+            st = nat.load().gdn2_attn_fwd(
+                nat.ptr(q), nat.ptr(k), nat.ptr(v), ctypes.addressof(strides), nat.ptr(o), nat.ptr(o_lo),
+                nat.ptr(lse), nat.dtype_code(q.dtype), nat.ptr(kv_len), nat.ptr(cu_dev), nat.ptr(cu_host), n, B, Tq, Tk, H, G, D,
+                scale, int(causal), nat.stream_handle(q.device))
+        nat.check(st, "attention")
+        ctx.save_for_backward(q, k, v, o, o_lo, lse, kv_len, cu_dev)
+        ctx.scale, ctx.causal, ctx.cu_host = scale, causal, cu_host
+        return o
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do):
+        q, k, v, o, o_lo, lse, kv_len, cu_dev = ctx.saved_tensors
+        cu_host = ctx.cu_host
+        B, Tq, H, D = q.shape
+        Tk, G = k.shape[1], k.shape[2]
+        do = _io(do, q.dtype)
+        dq = torch.empty(B, Tq, H, D, dtype=q.dtype, device=q.device)
+        dk, dv = (torch.empty(B, Tk, G, D, dtype=q.dtype, device=q.device) for _ in range(2))
+        strides = (ctypes.c_int64 * 9)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
+        n = 0 if cu_host is None else cu_host.numel() - 1
+        lib = nat.load()
+        ws = torch.empty(max(lib.gdn2_attn_bwd_workspace_size(B, Tq, H, G), 16), dtype=torch.uint8, device=q.device)
+        with _on_device(q.device):
+            st = lib.gdn2_attn_bwd(
+                nat.ptr(q), nat.ptr(k), nat.ptr(v), ctypes.addressof(strides), nat.ptr(o), nat.ptr(o_lo),
+                nat.ptr(lse), nat.ptr(do), nat.ptr(dq), nat.ptr(dk), nat.ptr(dv), nat.dtype_code(q.dtype), nat.ptr(kv_len), nat.ptr(cu_dev),
+                nat.ptr(cu_host), n, B, Tq, Tk, H, G, D, ctx.scale, int(ctx.causal), nat.ptr(ws), ws.numel(),
+                nat.stream_handle(q.device))
+        nat.check(st, "attention backward")
+        return dq, dk, dv, None, None, None, None, None
+
+
+@torch.compiler.disable
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float | None = None, causal: bool = True,
+              kv_lengths: torch.Tensor | None = None, cu_seqlens: torch.Tensor | None = None) -> torch.Tensor:
+    """Differentiable softmax attention with grouped heads on the HIP kernels: the multi-token
+    path of reference ``CausalSelfAttention.forward`` (``gdn2_gpt/model.py:89-173``) without the
+    repeated k and v.
+
+    ``q`` ``[B, Tq, H, D]``, ``k`` / ``v`` ``[B, Tk, G, D]`` (``H`` a multiple of ``G``; bf16 or
+    fp16, ``D`` 64 or 128; any strides, read in place where the channels are contiguous and rows
+    16-byte aligned).  Returns ``[B, Tq, H, D]``, ``softmax(scale q k^T) v`` with
+    ``scale = D**-0.5`` unless given (> 0).
+
+    Query ``i`` of a row sees key ``j`` if
+
+    * ``causal``: ``j <= i + Tk - Tq`` (the queries are the last ``Tq`` positions);
+    * ``kv_lengths`` (int32 / int64 ``[B]`` on the device): ``j < kv_lengths[b]``; keys from there on
+      are not read, and their gradients are zero;
+    * ``cu_seqlens`` (``[N + 1]`` offsets, one row, ``Tq = Tk``, without ``kv_lengths``): both belong to
+      the same packed sequence.  The offsets are checked on the host: pass them as a CPU tensor
+      to avoid a device synchronisation (a captured graph needs that).
+
+    A query that sees no key gives zeros and passes no gradient.  A key hidden from some queries of
+    its row by ``causal`` must be finite (0 times infinity is NaN, as in any attention by
+    products).  Scores, softmax statistics and sums are float32; the probabilities, and in the
+    backward their gradients, are rounded to the io dtype for the products.  The gradients have
+    the same bits in every run.  In a HIP graph, capture the forward and backward together with no
+    eager autograd graph of the same leaves alive, as torch asks of any captured backward.
+    """
+    name = "attention"
+    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape:
+        raise ValueError(f"{name}: q must be [B, Tq, H, D] and k, v [B, Tk, G, D]; got {tuple(q.shape)}, "
+                         f"{tuple(k.shape)}, {tuple(v.shape)}")
+    B, Tq, H, D = q.shape
+    Tk, G = k.shape[1], k.shape[2]
+    if k.shape[0] != B or k.shape[3] != D or G < 1 or H < 1 or H % G != 0:
+        raise ValueError(f"{name}: q {tuple(q.shape)} and k {tuple(k.shape)} do not agree (H a multiple of G)")
+    if not (q.dtype == k.dtype == v.dtype):
+        raise ValueError(f"{name}: q, k, v must have one dtype; got {q.dtype}, {k.dtype}, {v.dtype}")
+    if q.dtype not in (torch.bfloat16, torch.float16) or D not in (64, 128):
+        raise NotImplementedError(f"{name}: bfloat16 / float16 heads of 64 or 128 channels; got {q.dtype}, {D}")
+    scale = float(D) ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale <= 1e30:
+        raise NotImplementedError(f"{name}: scale must be positive and at most 1e30, got {scale}")
+    if kv_lengths is not None:
+        if cu_seqlens is not None:
+            raise ValueError(f"{name}: kv_lengths and cu_seqlens exclude each other")
+        if kv_lengths.shape != (B,) or kv_lengths.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"{name}: kv_lengths must be {B} int32 / int64 lengths; got {tuple(kv_lengths.shape)} "
+                             f"{kv_lengths.dtype}")
+    if cu_seqlens is not None and (B != 1 or Tq != Tk):
+        raise ValueError(f"{name}: packed sequences (cu_seqlens) go in a single row with as many keys as queries; "
+                         f"got batch {B}, {Tq} queries, {Tk} keys")
+    _require_gpu(name, q, k, v, kv_lengths)
+    for t in (k, v, kv_lengths):
+        if t is not None and t.device != q.device:
+            raise ValueError(f"{name}: tensors on {q.device} and {t.device}")
+    kv_len = None if kv_lengths is None else kv_lengths.detach().to(torch.int64).contiguous()
+    cu_dev, cu_host = _cu(cu_seqlens, q.device, Tq)
+    return AttentionFunction.apply(q, k, v, scale, bool(causal), kv_len, cu_dev, cu_host)
 
 
 def _rows2d(name: str, x: torch.Tensor, dt: torch.dtype, width: int) -> int:
