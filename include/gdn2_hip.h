@@ -319,6 +319,36 @@ int gdn2_attn_decode(const void *qkv, const float *cos, const float *sin, int ro
                      void *stream);
 
 /*
+ * Log probabilities of given tokens over the LM head's logits (the logits of
+ * reference src/qwendopamine/models/gdn2_gpt/model.py:304-380, GPT.forward),
+ * the rows' entropies and their top_k most probable tokens, and the gradient:
+ * a training loss, a scorer, or what a decoder reports beside its tokens.
+ *   x        rows of n logits (io_dtype f32 / bf16 / fp16): row r starts
+ *            (r / inner_rows) * outer_stride + (r % inner_rows) * row_stride
+ *            elements after x (any element alignment)
+ *   targets  int64 [rows]: logp[r] = x[r][t] - logsumexp(x[r]); a target equal to
+ *            ignore_index gives 0 and passes no gradient, any other outside
+ *            [0, n) gives NaN
+ *   logp, entropy  fp32 [rows], entropy = -sum p ln p
+ *   lse      fp32 [rows][2], what the backward needs of the sums; NULL without one
+ *   top_logp fp32, top_ids int64 [rows][top_k], 0 <= top_k <= 32, top_k <= n: in
+ *            descending order, equal logits by the lower index, NaN first
+ * A row with a NaN or +inf, or of -inf alone, gives NaN (as log_softmax).
+ * gdn2_token_logprobs_bwd writes dx [rows][n] (contiguous, io_dtype) from dlogp and
+ * dentropy (fp32 [rows]; either may be NULL), x, lse and entropy; a row to which no gradient
+ * arrives gets zeros.  Deterministic.
+ */
+size_t gdn2_token_logprobs_workspace_size(int64_t rows, int64_t n, int top_k, int io_dtype);
+int gdn2_token_logprobs_fwd(const void *x, int64_t inner_rows, int64_t outer_stride, int64_t row_stride, int io_dtype,
+                            int64_t rows, int64_t n, const int64_t *targets, int64_t ignore_index, float *logp,
+                            float *entropy, float *lse, int top_k, float *top_logp, int64_t *top_ids, void *workspace,
+                            size_t workspace_bytes, void *stream);
+int gdn2_token_logprobs_bwd(const void *x, int64_t inner_rows, int64_t outer_stride, int64_t row_stride, int io_dtype,
+                            int64_t rows, int64_t n, const int64_t *targets, int64_t ignore_index,
+                            const float *entropy, const float *lse, const float *dlogp, const float *dentropy,
+                            void *dx, void *stream);
+
+/*
  * Softmax attention over whole sequences and its gradient: the multi-token
  * path of the hybrid host's attention layers (CausalSelfAttention.forward,
  * reference src/qwendopamine/models/gdn2_gpt/model.py:89-173) in training and

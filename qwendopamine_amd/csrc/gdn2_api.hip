@@ -445,6 +445,75 @@ int gdn2_attn_decode(const void *qkv, const float *cos, const float *sin, int ro
     return err == hipSuccess ? GDN2_OK : GDN2_ERR_LAUNCH;
 }
 
+static int fill_logprob_args(LogprobParams &p, const void *x, int64_t inner, int64_t outer_stride, int64_t row_stride,
+                             int io_dtype, int64_t rows, int64_t n, const int64_t *targets, int64_t ignore)
+{
+    if (!valid_dtype(io_dtype) || rows < 0 || n < 1 || inner < 1 || outer_stride < 0 || row_stride < 0)
+        return GDN2_ERR_INVALID;
+    if (rows > 0 && (!x || !targets)) return GDN2_ERR_INVALID;
+    if (reinterpret_cast<uintptr_t>(x) % (io_dtype == GDN2_DTYPE_F32 ? 4 : 2) != 0) return GDN2_ERR_INVALID;
+    // One launch of rows * parts workgroups; indices of a row in 32 bits.
+    if (rows > (1 << 27) || n > (1 << 30)) return GDN2_ERR_UNSUPPORTED;
+    p.x = x;
+    p.inner = inner; p.outer_stride = outer_stride; p.row_stride = row_stride;
+    p.rows = rows; p.n = n;
+    p.targets = targets;
+    p.ignore = ignore;
+    return GDN2_OK;
+}
+
+size_t gdn2_token_logprobs_workspace_size(int64_t rows, int64_t n, int top_k, int io_dtype)
+{
+    if (!valid_dtype(io_dtype) || rows < 1 || n < 1 || rows > (1 << 27) || n > (1 << 30) || top_k < 0 || top_k > 32)
+        return 0;
+    const int parts = logprob_parts(rows, n, io_dtype);
+    return parts == 1 ? 0 : static_cast<size_t>(rows) * parts * (4 * sizeof(float) + static_cast<size_t>(top_k) * 8);
+}
+
+int gdn2_token_logprobs_fwd(const void *x, int64_t inner_rows, int64_t outer_stride, int64_t row_stride, int io_dtype,
+                            int64_t rows, int64_t n, const int64_t *targets, int64_t ignore_index, float *logp,
+                            float *entropy, float *lse, int top_k, float *top_logp, int64_t *top_ids, void *workspace,
+                            size_t workspace_bytes, void *stream)
+{
+    LogprobParams p = {};
+    const int st = fill_logprob_args(p, x, inner_rows, outer_stride, row_stride, io_dtype, rows, n, targets,
+                                     ignore_index);
+    if (st != GDN2_OK) return st;
+    if (top_k < 0 || top_k > n) return GDN2_ERR_INVALID;
+    if (top_k > 32) return GDN2_ERR_UNSUPPORTED;
+    if (rows == 0) return GDN2_OK;
+    if (!logp || !entropy || (top_k > 0 && (!top_logp || !top_ids))) return GDN2_ERR_INVALID;
+    const size_t need = gdn2_token_logprobs_workspace_size(rows, n, top_k, io_dtype);
+    if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15)))
+        return GDN2_ERR_WORKSPACE;
+    p.logp = logp; p.entropy = entropy; p.lse = lse;
+    p.top = top_k; p.top_logp = top_logp; p.top_ids = top_ids;
+    p.parts = logprob_parts(rows, n, io_dtype);
+    p.part_stat = static_cast<float *>(workspace);
+    p.part_top = reinterpret_cast<unsigned long long *>(p.part_stat + rows * p.parts * 4);
+    return launch_logprobs(p, io_dtype, static_cast<hipStream_t>(stream)) == hipSuccess ? GDN2_OK : GDN2_ERR_LAUNCH;
+}
+
+int gdn2_token_logprobs_bwd(const void *x, int64_t inner_rows, int64_t outer_stride, int64_t row_stride, int io_dtype,
+                            int64_t rows, int64_t n, const int64_t *targets, int64_t ignore_index,
+                            const float *entropy, const float *lse, const float *dlogp, const float *dentropy,
+                            void *dx, void *stream)
+{
+    LogprobParams p = {};
+    const int st = fill_logprob_args(p, x, inner_rows, outer_stride, row_stride, io_dtype, rows, n, targets,
+                                     ignore_index);
+    if (st != GDN2_OK) return st;
+    if (rows == 0) return GDN2_OK;
+    if (!entropy || !lse || !dx || reinterpret_cast<uintptr_t>(dx) % (io_dtype == GDN2_DTYPE_F32 ? 4 : 2) != 0)
+        return GDN2_ERR_INVALID;
+    if ((n / 8192 + 1) * rows > 2147483647LL) return GDN2_ERR_UNSUPPORTED;
+    p.entropy = const_cast<float *>(entropy);
+    p.lse = const_cast<float *>(lse);
+    p.dlogp = dlogp; p.dent = dentropy;
+    p.dx = dx;
+    return launch_logprobs_bwd(p, io_dtype, static_cast<hipStream_t>(stream)) == hipSuccess ? GDN2_OK : GDN2_ERR_LAUNCH;
+}
+
 // Shared by gdn2_attn_fwd and gdn2_attn_bwd: checks, and the parameters both take.
 static int fill_attn_args(AttnTrainParams &p, const void *q, const void *k, const void *v, const int64_t *strides,
                           int io_dtype, const int64_t *kv_lengths, const int64_t *cu, const int64_t *cu_host,

@@ -332,6 +332,30 @@ size_t attn_bwd_workspace_bytes(int B, int Tq, int H, int G);
 hipError_t launch_attn_fwd(const AttnTrainParams &p, int io_dtype, hipStream_t stream);
 hipError_t launch_attn_bwd(const AttnTrainParams &p, int io_dtype, hipStream_t stream);
 
+// Log probabilities of given tokens with entropy and top alternatives, and
+// their gradient.  Row r of the logits at x + (r / inner) * outer_stride +
+// (r % inner) * row_stride (elements; any alignment of an element), n values.
+struct LogprobParams {
+    const void *x;
+    int64_t inner, outer_stride, row_stride, rows, n;
+    const int64_t *targets;   // [rows]
+    int64_t ignore;
+    float *logp, *entropy;    // [rows]
+    float *lse;               // [rows][2]: maximum and ln of the scaled sum (NULL without a backward)
+    int top;                  // alternatives per row, 0 .. 32
+    float *top_logp;          // [rows][top]
+    int64_t *top_ids;
+    const float *dlogp, *dent;  // backward: [rows] or NULL
+    void *dx;                   // [rows][n], contiguous
+    int parts;                  // per row (logprob_parts; the backward sets its own)
+    int64_t pieces_per_part;    // set by the launchers
+    float *part_stat;           // [rows][parts][4]
+    unsigned long long *part_top;  // [rows][parts][top]
+};
+int logprob_parts(int64_t rows, int64_t n, int io_dtype);
+hipError_t launch_logprobs(LogprobParams p, int io_dtype, hipStream_t stream);
+hipError_t launch_logprobs_bwd(const LogprobParams &p, int io_dtype, hipStream_t stream);
+
 // Backward of the short convolution on a prefill call (no cache).
 struct ConvBwdParams {
     const void *x;      // [B, T, D] input rows: row (b, t) at x + (b * T + t) * ldx

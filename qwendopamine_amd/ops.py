@@ -21,7 +21,7 @@ float32 (as the reference's accelerated ops return it).
 
 from __future__ import annotations
 
-from typing import Any
+from typing import Any, NamedTuple
 
 import contextlib
 import ctypes
@@ -51,6 +51,9 @@ __all__ = [
     "attention_decode",
     "attention",
     "AttentionFunction",
+    "token_logprobs",
+    "TokenLogprobs",
+    "TokenLogprobsFunction",
     "decode_step_fused",
 ]
 
@@ -1636,6 +1639,110 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float | 
     kv_len = None if kv_lengths is None else kv_lengths.detach().to(torch.int64).contiguous()
     cu_dev, cu_host = _cu(cu_seqlens, q.device, Tq)
     return AttentionFunction.apply(q, k, v, scale, bool(causal), kv_len, cu_dev, cu_host)
+
+
+class TokenLogprobs(NamedTuple):
+    """What :func:`token_logprobs` returns; the last two are None without ``top_k``."""
+
+    logprobs: torch.Tensor
+    entropy: torch.Tensor
+    top_logprobs: torch.Tensor | None
+    top_ids: torch.Tensor | None
+
+
+def _logit_rows(x: torch.Tensor) -> tuple[torch.Tensor, int, int, int, int]:
+    """``(x, inner, outer stride, row stride, rows)`` of logits ``[..., V]``: up to two leading axes
+    are read in place by their strides, more only where they collapse without a copy."""
+    if x.stride(-1) != 1 and x.shape[-1] > 1:
+        x = x.contiguous()
+    if x.dim() > 3:
+        x = x.reshape(-1, x.shape[-1])
+    if x.dim() == 3:
+        B, T, _ = x.shape
+        return x, max(T, 1), x.stride(0), x.stride(1), B * T
+    rows = x.shape[0] if x.dim() == 2 else 1
+    return x, max(rows, 1), 0, x.stride(0) if x.dim() == 2 else x.shape[-1], rows
+
+
+class TokenLogprobsFunction(torch.autograd.Function):
+    """:func:`token_logprobs` with the HIP forward and backward (``gdn2_token_logprobs_fwd`` /
+    ``gdn2_token_logprobs_bwd``): each row's maximum and log sum are kept, nothing of its size."""
+
+    @staticmethod
+    def forward(ctx, logits, targets, top_k: int, ignore_index: int):
+        x, inner, so, sr, rows = _logit_rows(logits)
+        V, dev, shape = x.shape[-1], x.device, tuple(targets.shape)
+        logp, ent = (torch.empty(shape, dtype=torch.float32, device=dev) for _ in range(2))
+        lse = torch.empty(rows, 2, dtype=torch.float32, device=dev) if ctx.needs_input_grad[0] else None
+        top_lp = torch.empty(*shape, top_k, dtype=torch.float32, device=dev) if top_k else None
+        top_ids = torch.empty(*shape, top_k, dtype=torch.int64, device=dev) if top_k else None
+        lib, dt = nat.load(), nat.dtype_code(x.dtype)
+        nbytes = lib.gdn2_token_logprobs_workspace_size(rows, V, top_k, dt)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        with _on_device(dev):
+            st = lib.gdn2_token_logprobs_fwd(
+                nat.ptr(x), inner, so, sr, dt, rows, V, nat.ptr(targets), ignore_index, nat.ptr(logp), nat.ptr(ent),
+                nat.ptr(lse), top_k, nat.ptr(top_lp), nat.ptr(top_ids), nat.ptr(ws), nbytes, nat.stream_handle(dev))
+        nat.check(st, "token_logprobs")
+        ctx.save_for_backward(x, targets, ent, lse)
+        ctx.shape, ctx.ignore_index = logits.shape, ignore_index
+        ctx.set_materialize_grads(False)
+        if top_k:
+            ctx.mark_non_differentiable(top_lp, top_ids)
+        return logp, ent, top_lp, top_ids
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dlogp, dent, *_):
+        if dlogp is None and dent is None:
+            return None, None, None, None
+        x, targets, ent, lse = ctx.saved_tensors
+        x, inner, so, sr, rows = _logit_rows(x)
+        V, dev = x.shape[-1], x.device
+        dlogp, dent = (None if d is None else d.float().contiguous() for d in (dlogp, dent))
+        dx = torch.empty(ctx.shape, dtype=x.dtype, device=dev)
+        with _on_device(dev):
+            st = nat.load().gdn2_token_logprobs_bwd(
+                nat.ptr(x), inner, so, sr, nat.dtype_code(x.dtype), rows, V, nat.ptr(targets), ctx.ignore_index,
+                nat.ptr(ent), nat.ptr(lse), nat.ptr(dlogp), nat.ptr(dent), nat.ptr(dx), nat.stream_handle(dev))
+        nat.check(st, "token_logprobs backward")
+        return dx, None, None, None
+
+
+@torch.compiler.disable
+def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0,
+                   ignore_index: int = -100) -> TokenLogprobs:
+    """Log probability of each row's target token, the row's entropy and its ``top_k`` most probable
+    tokens, in one pass over the logits (of reference ``GPT.forward``,
+    ``gdn2_gpt/model.py:304-380``); differentiable in the logits through the log probabilities and
+    the entropies.
+
+    ``logits`` ``[..., V]`` (bf16, fp16 or float32; rows read in place at any alignment, up to two
+    leading axes at any strides), ``targets`` int64 ``[...]``.  Returns :class:`TokenLogprobs`:
+    ``logprobs`` and ``entropy`` float32 ``[...]``, ``top_logprobs`` float32 and ``top_ids`` int64
+    ``[..., top_k]`` (descending, equal logits by the lower index, NaN first; at most 32; not
+    differentiable), or None without ``top_k``.
+
+    A target equal to ``ignore_index`` gives 0 and passes no gradient; any other target outside
+    ``[0, V)`` gives NaN.  A row with a NaN or +inf, or of -inf alone, gives NaN, as ``log_softmax``
+    does; single -inf logits have probability 0 and pass no gradient.  Sums are float32, the
+    gradient is rounded once to the logits' dtype; everything has the same bits in every run.
+    """
+    name = "token_logprobs"
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"{name}: logits must be [..., V] with V >= 1; got {tuple(logits.shape)}")
+    if tuple(targets.shape) != tuple(logits.shape[:-1]) or targets.dtype != torch.int64:
+        raise ValueError(f"{name}: targets must be int64 {tuple(logits.shape[:-1])}; got {targets.dtype} "
+                         f"{tuple(targets.shape)}")
+    if not 0 <= int(top_k) <= logits.shape[-1]:
+        raise ValueError(f"{name}: top_k must be within 0 .. {logits.shape[-1]}, got {top_k}")
+    if top_k > 32:
+        raise NotImplementedError(f"{name}: at most 32 alternatives, got {top_k}")
+    nat.dtype_code(logits.dtype)
+    _require_gpu(name, logits, targets)
+    if targets.device != logits.device:
+        raise ValueError(f"{name}: tensors on {logits.device} and {targets.device}")
+    return TokenLogprobs(*TokenLogprobsFunction.apply(logits, targets.contiguous(), int(top_k), int(ignore_index)))
 
 
 def _rows2d(name: str, x: torch.Tensor, dt: torch.dtype, width: int) -> int:

@@ -85,3 +85,42 @@ def _attn_call(lib, **over):
 ])
 def test_attention_entry_point_checks(lib, want, over):
     assert _attn_call(lib, **over) == want
+
+
+@pytest.mark.parametrize("err,x,t,kw", [
+    (ValueError, torch.zeros(3, 0), torch.zeros(3, dtype=torch.int64), {}),
+    (ValueError, torch.zeros(3, 5), torch.zeros(4, dtype=torch.int64), {}),
+    (ValueError, torch.zeros(3, 5), torch.zeros(3, dtype=torch.int32), {}),
+    (ValueError, torch.zeros(3, 5), torch.zeros(3, dtype=torch.int64), dict(top_k=6)),
+    (ValueError, torch.zeros(3, 5), torch.zeros(3, dtype=torch.int64), dict(top_k=-1)),
+    (NotImplementedError, torch.zeros(3, 50), torch.zeros(3, dtype=torch.int64), dict(top_k=33)),
+    (NotImplementedError, torch.zeros(3, 50, dtype=torch.float64), torch.zeros(3, dtype=torch.int64), {}),
+    (RuntimeError, torch.zeros(3, 50), torch.zeros(3, dtype=torch.int64), {}),
+])
+def test_token_logprobs_refuses(err, x, t, kw):
+    with pytest.raises(err):
+        ops.token_logprobs(x, t, **kw)
+
+
+@pytest.mark.parametrize("want,over", [
+    (nat.ERR_INVALID, dict(dt=nat.DTYPE_I32)),
+    (nat.ERR_INVALID, dict(n=0)),
+    (nat.ERR_INVALID, dict(inner=0)),
+    (nat.ERR_INVALID, dict(sr=-1)),
+    (nat.ERR_INVALID, dict(x=4097)),
+    (nat.ERR_INVALID, dict(x=None)),
+    (nat.ERR_INVALID, dict(t=None)),
+    (nat.ERR_INVALID, dict(logp=None)),
+    (nat.ERR_INVALID, dict(top=101)),
+    (nat.ERR_INVALID, dict(top=5)),  # without outputs for them
+    (nat.ERR_UNSUPPORTED, dict(top=33)),
+    (nat.ERR_UNSUPPORTED, dict(n=1 << 31)),
+    (nat.ERR_UNSUPPORTED, dict(rows=1 << 28)),
+    (nat.ERR_WORKSPACE, dict(n=100000)),
+    (nat.OK, dict(rows=0)),
+])
+def test_token_logprobs_entry_point_checks(lib, want, over):
+    a = dict(x=4096, inner=4, so=0, sr=100, dt=nat.DTYPE_BF16, rows=4, n=100, t=4096, logp=4096, top=0)
+    a.update(over)
+    assert lib.gdn2_token_logprobs_fwd(a["x"], a["inner"], a["so"], a["sr"], a["dt"], a["rows"], a["n"], a["t"], -100,
+                                       a["logp"], 4096, None, a["top"], None, None, None, 0, None) == want
