@@ -319,6 +319,47 @@ int gdn2_attn_decode(const void *qkv, const float *cos, const float *sin, int ro
                      void *stream);
 
 /*
+ * gdn2_attn_decode over caches held in 4 bits (the same reference path; the
+ * cache format is this library's).  A position's 64-channel group is held as 64
+ * codes 0 .. 15 and two bf16 numbers:
+ *   minimum = bf16(min x), scale = bf16(max((max x - minimum) / 15, 0)),
+ *   code = clamp(rint((x - minimum) * (1 / scale)), 0, 15)   (0 if scale is 0)
+ * in fp32, every operation rounded by itself; it stands for scale * code +
+ * minimum.  A group with a value that is not finite gets NaN for both.
+ *   k_codes, v_codes  [B, G, max_len, D / 2] bytes, 16-byte aligned: channel 2 i
+ *            in the low, 2 i + 1 in the high nibble of byte i
+ *   k_meta, v_meta    [B, G, max_len, D / 64, 2] bf16 (scale, minimum)
+ *   pos      device int64: sequence b's position is pos[pos_stride * b]
+ *            (pos_stride 0: one position for all)
+ *   cos, sin with rope_row_stride > 0 the tables' row of the sequence's position is read; 0:
+ *            one row for all
+ * The token's k (rotated, rounded to io_dtype) and v are stored as codes at the
+ * position, and every q head attends positions 0 .. pos as the cache then holds
+ * them, its own included.  A position outside [0, max_len) leaves its
+ * sequence's caches alone and writes zeros.  bf16 / fp16, D in {64, 128}, qpk in
+ * 1 .. 16; else GDN2_ERR_UNSUPPORTED.  workspace: gdn2_attn_decode_q4_workspace_size()
+ * bytes, 16-byte aligned (may be 0), of which concurrent calls need one each.
+ *
+ * gdn2_kv_cache_q4_store stores k, v [B, T, G, D] (io_dtype f32 / bf16 / fp16;
+ * `strides`: host array of six element strides, batch, token, head of k, then of
+ * v; channels contiguous, rows 16-byte aligned) at positions start[start_stride
+ * * b] .. (start NULL: from 0); gdn2_kv_cache_q4_load writes what positions
+ * start .. start + T - 1 stand for into k, v [B, T, G, D] (contiguous, io_dtype, rounded
+ * once).  Positions outside the cache are not stored, and load as zeros.
+ */
+size_t gdn2_attn_decode_q4_workspace_size(int B, int G, int qpk, int D, int64_t max_len);
+int gdn2_attn_decode_q4(const void *qkv, const float *cos, const float *sin, int rope_pairs, int64_t rope_row_stride,
+                        const int64_t *pos, int64_t pos_stride, void *k_codes, void *k_meta, void *v_codes,
+                        void *v_meta, void *out, int io_dtype, int B, int G, int qpk, int D, int64_t max_len,
+                        float scale, void *workspace, size_t workspace_bytes, void *stream);
+int gdn2_kv_cache_q4_store(const void *k, const void *v, const int64_t *strides, int io_dtype, const int64_t *start,
+                           int64_t start_stride, void *k_codes, void *k_meta, void *v_codes, void *v_meta, int B,
+                           int64_t T, int G, int D, int64_t max_len, void *stream);
+int gdn2_kv_cache_q4_load(const void *k_codes, const void *k_meta, const void *v_codes, const void *v_meta,
+                          const int64_t *start, int64_t start_stride, void *k, void *v, int io_dtype, int B, int64_t T,
+                          int G, int D, int64_t max_len, void *stream);
+
+/*
  * Log probabilities of given tokens over the LM head's logits (the logits of
  * reference src/qwendopamine/models/gdn2_gpt/model.py:304-380, GPT.forward),
  * the rows' entropies and their top_k most probable tokens, and the gradient:

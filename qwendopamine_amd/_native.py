@@ -82,6 +82,13 @@ SIGNATURES: dict[str, tuple] = {
     "gdn2_argmax_rows": (_i, [_vp, _i64, _i, _i64, _i64, _vp, _i64, _vp, _sz, _vp]),
     "gdn2_attn_decode_workspace_size": (_sz, [_i, _i, _i, _i, _i64]),
     "gdn2_attn_decode": (_i, [_vp, _vp, _vp, _i, _i64, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i64, _f, _vp, _sz, _vp]),
+    "gdn2_attn_decode_q4_workspace_size": (_sz, [_i, _i, _i, _i, _i64]),
+    "gdn2_attn_decode_q4": (
+        _i,
+        [_vp, _vp, _vp, _i, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i64, _f, _vp, _sz, _vp],
+    ),
+    "gdn2_kv_cache_q4_store": (_i, [_vp, _vp, _vp, _i, _vp, _i64, _vp, _vp, _vp, _vp, _i, _i64, _i, _i, _i64, _vp]),
+    "gdn2_kv_cache_q4_load": (_i, [_vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _i, _i, _i64, _i, _i, _i64, _vp]),
     "gdn2_token_logprobs_workspace_size": (_sz, [_i64, _i64, _i, _i]),
     "gdn2_token_logprobs_fwd": (_i, [_vp, _i64, _i64, _i64, _i, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _i, _vp, _vp, _vp,
                                      _sz, _vp]),

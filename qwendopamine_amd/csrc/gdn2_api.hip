@@ -445,6 +445,100 @@ int gdn2_attn_decode(const void *qkv, const float *cos, const float *sin, int ro
     return err == hipSuccess ? GDN2_OK : GDN2_ERR_LAUNCH;
 }
 
+static int check_q4_cache(const void *kc, const void *km, const void *vc, const void *vm, int B, int G, int D,
+                          int64_t max_len)
+{
+    if (B < 0 || G < 1 || D < 1 || max_len < 1) return GDN2_ERR_INVALID;
+    if (D % 64 != 0 || D > 1024) return GDN2_ERR_UNSUPPORTED;
+    if (max_len > (1 << 30) || static_cast<int64_t>(B) * G > 2147483647LL) return GDN2_ERR_UNSUPPORTED;
+    if (B > 0 && (!kc || !km || !vc || !vm)) return GDN2_ERR_INVALID;
+    if ((reinterpret_cast<uintptr_t>(kc) | reinterpret_cast<uintptr_t>(vc)) & 15) return GDN2_ERR_INVALID;
+    if ((reinterpret_cast<uintptr_t>(km) | reinterpret_cast<uintptr_t>(vm)) & 3) return GDN2_ERR_INVALID;
+    return GDN2_OK;
+}
+
+size_t gdn2_attn_decode_q4_workspace_size(int B, int G, int qpk, int D, int64_t max_len)
+{
+    if (B < 1 || G < 1 || qpk < 1 || D < 1 || max_len < 1) return 0;
+    return attn_q4_workspace_floats(B, G, qpk, D, max_len) * sizeof(float);
+}
+
+int gdn2_attn_decode_q4(const void *qkv, const float *cos, const float *sin, int rope_pairs, int64_t rope_row_stride,
+                        const int64_t *pos, int64_t pos_stride, void *k_codes, void *k_meta, void *v_codes,
+                        void *v_meta, void *out, int io_dtype, int B, int G, int qpk, int D, int64_t max_len,
+                        float scale, void *workspace, size_t workspace_bytes, void *stream)
+{
+    if (!valid_dtype(io_dtype) || qpk < 1 || pos_stride < 0) return GDN2_ERR_INVALID;
+    const int st = check_q4_cache(k_codes, k_meta, v_codes, v_meta, B, G, D, max_len);
+    if (st != GDN2_OK) return st;
+    if (rope_pairs < 0 || 2 * rope_pairs > D || (rope_pairs > 0 && (!cos || !sin))) return GDN2_ERR_INVALID;
+    if (rope_row_stride < 0 || (rope_row_stride > 0 && rope_row_stride < rope_pairs)) return GDN2_ERR_INVALID;
+    if (!attn_q4_supported(io_dtype, qpk, D) || !(scale > 0.0f) || scale > 1e30f) return GDN2_ERR_UNSUPPORTED;
+    if (static_cast<int64_t>(B) * G * qpk > 2147483647LL) return GDN2_ERR_UNSUPPORTED;
+    if (B == 0) return GDN2_OK;
+    if (!qkv || !pos || !out) return GDN2_ERR_INVALID;
+    AttnQ4Params p = {};
+    p.qkv = qkv; p.cos = cos; p.sin = sin;
+    p.rope_pairs = rope_pairs;
+    p.rope_stride = rope_row_stride;
+    p.pos = pos; p.pos_stride = pos_stride;
+    p.k_codes = static_cast<uint8_t *>(k_codes); p.v_codes = static_cast<uint8_t *>(v_codes);
+    p.k_meta = static_cast<unsigned *>(k_meta); p.v_meta = static_cast<unsigned *>(v_meta);
+    p.out = out;
+    p.max_len = max_len; p.B = B; p.G = G; p.qpk = qpk; p.D = D; p.scale = scale;
+    p.splits = attn_q4_splits(B, G, max_len);
+    p.part = static_cast<float *>(workspace);
+    if (p.splits > 1 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) ||
+                         workspace_bytes < gdn2_attn_decode_q4_workspace_size(B, G, qpk, D, max_len)))
+        return GDN2_ERR_WORKSPACE;
+    return launch_attn_q4(p, io_dtype, static_cast<hipStream_t>(stream)) == hipSuccess ? GDN2_OK : GDN2_ERR_LAUNCH;
+}
+
+int gdn2_kv_cache_q4_store(const void *k, const void *v, const int64_t *strides, int io_dtype, const int64_t *start,
+                           int64_t start_stride, void *k_codes, void *k_meta, void *v_codes, void *v_meta, int B,
+                           int64_t T, int G, int D, int64_t max_len, void *stream)
+{
+    if (!valid_dtype(io_dtype) || T < 0 || start_stride < 0 || !strides) return GDN2_ERR_INVALID;
+    const int st = check_q4_cache(k_codes, k_meta, v_codes, v_meta, B, G, D, max_len);
+    if (st != GDN2_OK) return st;
+    if (B == 0 || T == 0) return GDN2_OK;
+    if (!k || !v || ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15)) return GDN2_ERR_INVALID;
+    if (T > (1 << 30) || ((T + 7) / 8) * (D / 64) * static_cast<int64_t>(G) * B > 2147483647LL)
+        return GDN2_ERR_UNSUPPORTED;
+    Q4StoreParams p = {};
+    const int64_t size[6] = {B, T, G, B, T, G};
+    const int per = io_dtype == GDN2_DTYPE_F32 ? 4 : 8;
+    for (int i = 0; i < 6; ++i) {
+        if (strides[i] < 0 || (size[i] > 1 && strides[i] % per != 0)) return GDN2_ERR_INVALID;
+        (i < 3 ? p.ks : p.vs)[i % 3] = strides[i];
+    }
+    p.k = k; p.v = v;
+    p.start = start; p.start_stride = start_stride;
+    p.k_codes = static_cast<uint8_t *>(k_codes); p.v_codes = static_cast<uint8_t *>(v_codes);
+    p.k_meta = static_cast<unsigned *>(k_meta); p.v_meta = static_cast<unsigned *>(v_meta);
+    p.max_len = max_len; p.T = T; p.B = B; p.G = G; p.D = D;
+    return launch_q4_store(p, io_dtype, static_cast<hipStream_t>(stream)) == hipSuccess ? GDN2_OK : GDN2_ERR_LAUNCH;
+}
+
+int gdn2_kv_cache_q4_load(const void *k_codes, const void *k_meta, const void *v_codes, const void *v_meta,
+                          const int64_t *start, int64_t start_stride, void *k, void *v, int io_dtype, int B, int64_t T,
+                          int G, int D, int64_t max_len, void *stream)
+{
+    if (!valid_dtype(io_dtype) || T < 0 || start_stride < 0) return GDN2_ERR_INVALID;
+    const int st = check_q4_cache(k_codes, k_meta, v_codes, v_meta, B, G, D, max_len);
+    if (st != GDN2_OK) return st;
+    if (B == 0 || T == 0) return GDN2_OK;
+    if (!k || !v || ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15)) return GDN2_ERR_INVALID;
+    if (T > (1 << 30) || (static_cast<double>(B) * T * G * (D / 8)) / 128.0 > 2147483000.0) return GDN2_ERR_UNSUPPORTED;
+    Q4LoadParams p = {};
+    p.k = k; p.v = v;
+    p.start = start; p.start_stride = start_stride;
+    p.k_codes = static_cast<const uint8_t *>(k_codes); p.v_codes = static_cast<const uint8_t *>(v_codes);
+    p.k_meta = static_cast<const unsigned *>(k_meta); p.v_meta = static_cast<const unsigned *>(v_meta);
+    p.max_len = max_len; p.T = T; p.B = B; p.G = G; p.D = D;
+    return launch_q4_load(p, io_dtype, static_cast<hipStream_t>(stream)) == hipSuccess ? GDN2_OK : GDN2_ERR_LAUNCH;
+}
+
 static int fill_logprob_args(LogprobParams &p, const void *x, int64_t inner, int64_t outer_stride, int64_t row_stride,
                              int io_dtype, int64_t rows, int64_t n, const int64_t *targets, int64_t ignore)
 {

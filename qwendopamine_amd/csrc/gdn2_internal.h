@@ -356,6 +356,54 @@ int logprob_parts(int64_t rows, int64_t n, int io_dtype);
 hipError_t launch_logprobs(LogprobParams p, int io_dtype, hipStream_t stream);
 hipError_t launch_logprobs_bwd(const LogprobParams &p, int io_dtype, hipStream_t stream);
 
+// Single-token attention over a cache of 4-bit codes.  Caches: codes
+// [B, G, max_len, D / 2] bytes (even channels in the low nibbles), meta
+// [B, G, max_len, D / 64] words (scale bf16 low, minimum bf16 high).  qkv and
+// out as AttnDecodeParams; sequence b's token is at pos[pos_stride * b].
+struct AttnQ4Params {
+    const void *qkv;
+    const float *cos, *sin;
+    int rope_pairs;
+    int64_t rope_stride;
+    const int64_t *pos;
+    int64_t pos_stride;  // 0: one position for all
+    uint8_t *k_codes, *v_codes;
+    unsigned *k_meta, *v_meta;
+    void *out;
+    int64_t max_len;
+    int B, G, qpk, D;
+    float scale;
+    int splits;   // workgroups per (sequence, KV group)
+    float *part;  // attn_q4_workspace_floats, with more than one
+};
+bool attn_q4_supported(int io_dtype, int qpk, int D);
+int attn_q4_splits(int B, int G, int64_t max_len);
+size_t attn_q4_workspace_floats(int B, int G, int qpk, int D, int64_t max_len);
+hipError_t launch_attn_q4(const AttnQ4Params &p, int io_dtype, hipStream_t stream);
+
+// k, v [B, T, G, D] by strides into positions start[b] .. of the cache, and back.
+struct Q4StoreParams {
+    const void *k, *v;
+    int64_t ks[3], vs[3];
+    const int64_t *start;  // NULL: 0
+    int64_t start_stride;
+    uint8_t *k_codes, *v_codes;
+    unsigned *k_meta, *v_meta;
+    int64_t max_len, T;
+    int B, G, D;
+};
+struct Q4LoadParams {
+    void *k, *v;  // [B, T, G, D], contiguous
+    const int64_t *start;
+    int64_t start_stride;
+    const uint8_t *k_codes, *v_codes;
+    const unsigned *k_meta, *v_meta;
+    int64_t max_len, T;
+    int B, G, D;
+};
+hipError_t launch_q4_store(const Q4StoreParams &p, int io_dtype, hipStream_t stream);
+hipError_t launch_q4_load(const Q4LoadParams &p, int io_dtype, hipStream_t stream);
+
 // Backward of the short convolution on a prefill call (no cache).
 struct ConvBwdParams {
     const void *x;      // [B, T, D] input rows: row (b, t) at x + (b * T + t) * ldx

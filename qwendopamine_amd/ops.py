@@ -51,6 +51,11 @@ __all__ = [
     "attention_decode",
     "attention",
     "AttentionFunction",
+    "KVCacheQ4",
+    "kv_cache_q4",
+    "kv_cache_q4_store",
+    "kv_cache_q4_load",
+    "attention_decode_q4",
     "token_logprobs",
     "TokenLogprobs",
     "TokenLogprobsFunction",
@@ -1639,6 +1644,173 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float | 
     kv_len = None if kv_lengths is None else kv_lengths.detach().to(torch.int64).contiguous()
     cu_dev, cu_host = _cu(cu_seqlens, q.device, Tq)
     return AttentionFunction.apply(q, k, v, scale, bool(causal), kv_len, cu_dev, cu_host)
+
+
+class KVCacheQ4(NamedTuple):
+    """A key / value cache held in 4 bits: per position and group of 64 channels, 64 codes 0 .. 15
+    and a scale and minimum.  ``k`` / ``v`` uint8 ``[B, G, L, D / 2]`` (channel ``2 i`` in the low, ``2 i + 1``
+    in the high nibble of byte ``i``), ``k_meta`` / ``v_meta`` bfloat16 ``[B, G, L, D / 64, 2]`` (scale,
+    minimum); a code stands for ``scale * code + minimum``.  A quarter of a 16-bit cache, and the
+    groups' 4 bytes."""
+
+    k: torch.Tensor
+    k_meta: torch.Tensor
+    v: torch.Tensor
+    v_meta: torch.Tensor
+
+
+def kv_cache_q4(batch: int, groups: int, max_length: int, head_dim: int, device=None) -> KVCacheQ4:
+    """An empty :class:`KVCacheQ4` (every position stands for zeros)."""
+    if head_dim % 64 != 0 or head_dim < 64:
+        raise NotImplementedError(f"kv_cache_q4: heads of a multiple of 64 channels, got {head_dim}")
+
+    def codes():
+        return torch.zeros(batch, groups, max_length, head_dim // 2, dtype=torch.uint8, device=device)
+
+    def meta():
+        return torch.zeros(batch, groups, max_length, head_dim // 64, 2, dtype=torch.bfloat16, device=device)
+
+    return KVCacheQ4(codes(), meta(), codes(), meta())
+
+
+def _check_q4(name: str, cache: KVCacheQ4) -> tuple[int, int, int, int]:
+    """``(B, G, L, D)`` of a 4-bit cache the kernels can index."""
+    k, km, v, vm = cache
+    if k.dim() != 4 or k.shape[2] < 1 or k.shape[3] < 32 or k.shape[3] % 32 != 0:
+        raise ValueError(f"{name}: cache codes must be [B, G, L, D / 2] with D a multiple of 64; got {tuple(k.shape)}")
+    B, G, L, half = k.shape
+    if v.shape != k.shape or km.shape != (B, G, L, half // 32, 2) or vm.shape != km.shape:
+        raise ValueError(f"{name}: cache tensors do not agree: {[tuple(t.shape) for t in cache]}")
+    if k.dtype != torch.uint8 or v.dtype != torch.uint8 or km.dtype != torch.bfloat16 or vm.dtype != torch.bfloat16:
+        raise ValueError(f"{name}: a 4-bit cache is uint8 codes and bfloat16 scales")
+    for t in cache:
+        if not t.is_contiguous() or t.device != k.device:
+            raise ValueError(f"{name}: cache tensors must be contiguous, on one device")
+    return B, G, L, 2 * half
+
+
+def _positions(name: str, what: str, pos: torch.Tensor | None, B: int, device) -> tuple[torch.Tensor | None, int]:
+    """Device positions (one for all, or one per sequence) and their stride."""
+    if pos is None:
+        return None, 0
+    if pos.dtype != torch.int64 or pos.dim() > 1 or pos.numel() not in (1, B):
+        raise ValueError(f"{name}: {what} must be one int64 position, or {B}; got {tuple(pos.shape)} {pos.dtype}")
+    _require_gpu(name, pos)
+    if pos.device != device:
+        raise ValueError(f"{name}: tensors on {device} and {pos.device}")
+    return pos, 0 if pos.numel() == 1 else pos.stride(0)
+
+
+@torch.compiler.disable
+def kv_cache_q4_store(cache: KVCacheQ4, k: torch.Tensor, v: torch.Tensor, start: torch.Tensor | None = None) -> None:
+    """Stores ``k``, ``v`` ``[B, T, G, D]`` (bf16, fp16 or float32; any strides) in the 4-bit cache at
+    positions ``start ..`` of each sequence (device int64, one or ``[B]``; 0 without).  Positions
+    outside the cache are not stored; the others of the cache stay as they are.
+
+    Per group of 64 channels, in float32 with every operation rounded by itself: the minimum
+    in bf16, ``scale = (max - minimum) / 15`` in bf16, ``code = rint((x - minimum) * (1 / scale))`` within
+    0 .. 15.  A group with a value that is not finite stands for NaN."""
+    name = "kv_cache_q4_store"
+    B, G, L, D = _check_q4(name, cache)
+    if k.dim() != 4 or k.shape != v.shape or k.shape[0] != B or k.shape[2:] != (G, D) or k.dtype != v.dtype:
+        raise ValueError(f"{name}: k and v must be [{B}, T, {G}, {D}] of one dtype; got {tuple(k.shape)} {k.dtype}, "
+                         f"{tuple(v.shape)} {v.dtype}")
+    dt = nat.dtype_code(k.dtype)
+    _require_gpu(name, k, v, *cache)
+    if k.device != cache.k.device or v.device != k.device:
+        raise ValueError(f"{name}: tensors on {k.device}, {v.device} and {cache.k.device}")
+    pos, stride = _positions(name, "start", start, B, k.device)
+    k, v = _head_rows(k.detach()), _head_rows(v.detach())
+    strides = (ctypes.c_int64 * 6)(*k.stride()[:3], *v.stride()[:3])
+    with _on_device(k.device):
+        st = nat.load().gdn2_kv_cache_q4_store(
+            nat.ptr(k), nat.ptr(v), ctypes.addressof(strides), dt, nat.ptr(pos), stride, nat.ptr(cache.k),
+            nat.ptr(cache.k_meta), nat.ptr(cache.v), nat.ptr(cache.v_meta), B, k.shape[1], G, D, L,
+            nat.stream_handle(k.device))
+    nat.check(st, name)
+
+
+@torch.compiler.disable
+def kv_cache_q4_load(cache: KVCacheQ4, start: torch.Tensor | None, count: int,
+                     dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
+    """What positions ``start .. start + count - 1`` of each sequence stand for (``start`` as in
+    :func:`kv_cache_q4_store`), as ``k``, ``v`` ``[B, count, G, D]`` rounded once to ``dtype``; positions
+    outside the cache are zeros.  What :func:`attention` reads of earlier tokens when a prompt
+    comes in pieces."""
+    name = "kv_cache_q4_load"
+    B, G, L, D = _check_q4(name, cache)
+    if count < 0:
+        raise ValueError(f"{name}: count must not be negative, got {count}")
+    dt = nat.dtype_code(dtype)
+    _require_gpu(name, *cache)
+    dev = cache.k.device
+    pos, stride = _positions(name, "start", start, B, dev)
+    k, v = (torch.empty(B, count, G, D, dtype=dtype, device=dev) for _ in range(2))
+    with _on_device(dev):
+        st = nat.load().gdn2_kv_cache_q4_load(
+            nat.ptr(cache.k), nat.ptr(cache.k_meta), nat.ptr(cache.v), nat.ptr(cache.v_meta), nat.ptr(pos), stride,
+            nat.ptr(k), nat.ptr(v), dt, B, count, G, D, L, nat.stream_handle(dev))
+    nat.check(st, name)
+    return k, v
+
+
+def attention_decode_q4_supported(qkv: torch.Tensor, qpk: int, head_dim: int) -> bool:
+    """Whether ``attention_decode_q4`` takes this dtype, head size and query heads per group."""
+    return qkv.is_cuda and qkv.dtype in (torch.bfloat16, torch.float16) and 1 <= qpk <= 16 and head_dim in (64, 128)
+
+
+@torch.compiler.disable
+def attention_decode_q4(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, input_pos: torch.Tensor,
+                        cache: KVCacheQ4, n_head: int) -> torch.Tensor:
+    """:func:`attention_decode` over a :class:`KVCacheQ4`: RoPE of the token's q heads and k, the store
+    of its k and v as codes at the sequence's position, and softmax attention over positions
+    0 .. position as the cache then holds them.
+
+    ``qkv`` ``[B, 1, G * (qpk + 2) * D]`` (bf16 or fp16, ``D`` 64 or 128, ``qpk = n_head / G`` up to 16),
+    ``input_pos`` device int64, one position for all sequences or ``[B]``; ``cos`` / ``sin`` the whole
+    tables ``[R >= L, rot / 2]`` (fp32, contiguous), whose row of the position the kernel reads, or with
+    a single position the token's row ``[1, rot / 2]``.  A position outside the cache leaves that
+    sequence's cache alone and gives zeros.  Returns ``[B, n_head, D]``.  Products, scores and sums
+    are as exact as with float32 probabilities.  Inference only.
+    """
+    name = "attention_decode_q4"
+    B, G, L, D = _check_q4(name, cache)
+    if n_head < 1 or n_head % G != 0 or qkv.numel() != B * (n_head + 2 * G) * D:
+        raise ValueError(f"{name}: qkv, cache and n_head do not agree")
+    qpk = n_head // G
+    if qkv.dtype not in (torch.bfloat16, torch.float16) or D not in (64, 128) or qpk > 16:
+        raise NotImplementedError(f"{name}: bfloat16 / float16, heads of 64 or 128 channels, up to 16 query heads per "
+                                  f"group; got {qkv.dtype}, {D}, {qpk}")
+    if input_pos is None:
+        raise ValueError(f"{name}: input_pos is needed")
+    _require_gpu(name, qkv, cos, sin, *cache)
+    dev = cache.k.device
+    for t in (qkv, cos, sin):
+        if t.device != dev:
+            raise ValueError(f"{name}: tensors on {t.device} and {dev}")
+    pos, pos_stride = _positions(name, "input_pos", input_pos, B, dev)
+    pairs = cos.shape[-1]
+    if 2 * pairs > D or sin.shape != cos.shape:
+        raise ValueError(f"{name}: the rotation has more than D / 2 pairs, or cos and sin differ in shape")
+    rope_stride = 0
+    if cos.dim() == 2 and cos.shape[0] >= L and (cos.shape[0] > 1 or pos.numel() > 1):
+        rope_stride = pairs
+    elif cos.numel() != pairs or (pos.numel() > 1 and B > 1):
+        raise ValueError(f"{name}: rotation tables need at least {L} rows (or one row, with a single position)")
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or not (cos.is_contiguous() and sin.is_contiguous()):
+        raise ValueError(f"{name}: rotation tables must be contiguous fp32")
+    qc = qkv.contiguous()
+    out = torch.empty(B, n_head, D, dtype=qkv.dtype, device=dev)
+    lib = nat.load()
+    ws_bytes = lib.gdn2_attn_decode_q4_workspace_size(B, G, qpk, D, L)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+    with _on_device(dev):
+        st = lib.gdn2_attn_decode_q4(
+            nat.ptr(qc), nat.ptr(cos), nat.ptr(sin), pairs, rope_stride, nat.ptr(pos), pos_stride, nat.ptr(cache.k),
+            nat.ptr(cache.k_meta), nat.ptr(cache.v), nat.ptr(cache.v_meta), nat.ptr(out), nat.dtype_code(qkv.dtype), B,
+            G, qpk, D, L, float(D) ** -0.5, nat.ptr(ws), ws_bytes, nat.stream_handle(dev))
+    nat.check(st, name)
+    return out
 
 
 class TokenLogprobs(NamedTuple):

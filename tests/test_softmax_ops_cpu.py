@@ -124,3 +124,79 @@ def test_token_logprobs_entry_point_checks(lib, want, over):
     a.update(over)
     assert lib.gdn2_token_logprobs_fwd(a["x"], a["inner"], a["so"], a["sr"], a["dt"], a["rows"], a["n"], a["t"], -100,
                                        a["logp"], 4096, None, a["top"], None, None, None, 0, None) == want
+
+
+def _cache(B=2, G=2, L=10, D=64):
+    return ops.kv_cache_q4(B, G, L, D)
+
+
+def test_kv_cache_q4_shapes():
+    c = ops.kv_cache_q4(2, 3, 5, 128)
+    assert c.k.shape == (2, 3, 5, 64) and c.k_meta.shape == (2, 3, 5, 2, 2) and c.v.dtype == torch.uint8
+    with pytest.raises(NotImplementedError):
+        ops.kv_cache_q4(1, 1, 1, 80)
+
+
+@pytest.mark.parametrize("err,cache,kv,start", [
+    (ValueError, _cache(), torch.zeros(3, 4, 2, 64), None),
+    (ValueError, _cache(), torch.zeros(2, 4, 2, 128), None),
+    (ValueError, _cache()._replace(k=torch.zeros(2, 2, 9, 32, dtype=torch.uint8)), torch.zeros(2, 4, 2, 64), None),
+    (ValueError, _cache()._replace(k=torch.zeros(2, 2, 10, 32)), torch.zeros(2, 4, 2, 64), None),
+    (ValueError, _cache()._replace(v_meta=torch.zeros(2, 2, 10, 1, 2)), torch.zeros(2, 4, 2, 64), None),
+    (ValueError, ops.KVCacheQ4(*(t.transpose(0, 1) for t in _cache())), torch.zeros(2, 4, 2, 64), None),
+    (NotImplementedError, _cache(), torch.zeros(2, 4, 2, 64, dtype=torch.float64), None),
+    (RuntimeError, _cache(), torch.zeros(2, 4, 2, 64), None),
+])
+def test_kv_cache_q4_store_refuses(err, cache, kv, start):
+    with pytest.raises(err):
+        ops.kv_cache_q4_store(cache, kv, kv, start)
+
+
+@pytest.mark.parametrize("err,over", [
+    (ValueError, dict(n_head=3)),
+    (ValueError, dict(n_head=0)),
+    (ValueError, dict(qkv=torch.zeros(2, 1, 100, dtype=BF))),
+    (ValueError, dict(pos=None)),
+    (NotImplementedError, dict(qkv=torch.zeros(2, 1, 8 * 64))),
+    (NotImplementedError, dict(qkv=torch.zeros(2, 1, 38 * 64, dtype=BF), n_head=34)),
+    (RuntimeError, dict()),
+])
+def test_attention_decode_q4_refuses(err, over):
+    a = dict(qkv=torch.zeros(2, 1, 8 * 64, dtype=BF), cos=torch.zeros(10, 32), pos=torch.tensor([1]), n_head=4)
+    a.update(over)
+    with pytest.raises(err):
+        ops.attention_decode_q4(a["qkv"], a["cos"], a["cos"], a["pos"], _cache(), a["n_head"])
+
+
+def test_positions_are_checked():
+    for bad in (torch.zeros(3, dtype=torch.int64), torch.zeros(2, dtype=torch.int32), torch.zeros(2, 1, dtype=torch.int64)):
+        with pytest.raises(ValueError):
+            ops._positions("x", "start", bad, 2, torch.device("cpu"))
+    with pytest.raises(RuntimeError):
+        ops._positions("x", "start", torch.zeros(2, dtype=torch.int64), 2, torch.device("cpu"))
+
+
+@pytest.mark.parametrize("want,over", [
+    (nat.ERR_INVALID, dict(dt=9)),
+    (nat.ERR_INVALID, dict(qpk=0)),
+    (nat.ERR_INVALID, dict(L=0)),
+    (nat.ERR_INVALID, dict(pairs=33)),
+    (nat.ERR_INVALID, dict(cos=None)),
+    (nat.ERR_INVALID, dict(rs=8)),
+    (nat.ERR_INVALID, dict(kc=4104)),
+    (nat.ERR_INVALID, dict(km=4098)),
+    (nat.ERR_INVALID, dict(pos=None)),
+    (nat.ERR_UNSUPPORTED, dict(dt=nat.DTYPE_F32)),
+    (nat.ERR_UNSUPPORTED, dict(qpk=17)),
+    (nat.ERR_UNSUPPORTED, dict(D=192)),
+    (nat.ERR_UNSUPPORTED, dict(D=96)),
+    (nat.ERR_UNSUPPORTED, dict(L=1 << 31)),
+    (nat.ERR_WORKSPACE, dict(L=100000)),
+    (nat.OK, dict(B=0)),
+])
+def test_attention_decode_q4_entry_point_checks(lib, want, over):
+    a = dict(cos=4096, pairs=32, rs=32, pos=4096, kc=4096, km=4096, dt=nat.DTYPE_BF16, B=1, G=1, qpk=1, D=64, L=10)
+    a.update(over)
+    assert lib.gdn2_attn_decode_q4(4096, a["cos"], a["cos"], a["pairs"], a["rs"], a["pos"], 0, a["kc"], a["km"], a["kc"],
+                                   a["km"], 4096, a["dt"], a["B"], a["G"], a["qpk"], a["D"], a["L"], 1.0, None, 0,
+                                   None) == want
