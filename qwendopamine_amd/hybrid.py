@@ -16,6 +16,7 @@ What differs from the reference host, deliberately:
 * **Attention KV caches** are kept in the model dtype (the reference allocates them
   in the default dtype, ``model.py:421-424``), at a fixed ``max_seq_length``; decode
   masks the unused tail.
+  ``setup_caches(..., kv_bits=4)`` holds them in 4 bits instead (``ops.KVCacheQ4``).
 * **Decode as one HIP graph.** ``GreedyDecoder`` captures a whole decode step
   (embedding, 24 layers, LM head, argmax, position update) once and replays it;
   the gdn2 caches are refreshed in place at the end of every step, so replays
@@ -24,6 +25,9 @@ What differs from the reference host, deliberately:
   RMSNorm that reads its result (``ops.add_rms_norm``), and SwiGLU's ``silu(a) * b``
   is one pass (``ops.silu_mul``); both round as the torch ops they replace, and the
   logits are bit-identical to the unfused host's.
+* **Training and scoring.** ``HybridConfig.attention = "hip"`` trains (and prefills) the
+  attention layers on ``ops.attention``; ``HybridDecoder.token_logprobs`` and ``loss`` take the
+  logits through ``ops.token_logprobs`` instead of a log-softmax in memory.
 """
 
 from __future__ import annotations
@@ -69,8 +73,14 @@ class HybridConfig:
     allow_neg_eigval: bool = False
     backend: str = "auto"
     fp32_decay: bool = True
+    # Multi-token attention: "sdpa" (torch's flash or memory-efficient kernels) or "hip"
+    # (``ops.attention``: grouped heads in place, its own backward; bf16 / fp16 heads of 64 or
+    # 128 channels on the GPU, else as "sdpa").
+    attention: str = "sdpa"
 
     def __post_init__(self) -> None:
+        if self.attention not in ("sdpa", "hip"):
+            raise ValueError(f"attention must be 'sdpa' or 'hip', got {self.attention!r}")
         if self.padded_vocab_size is None:
             self.padded_vocab_size = self.vocab_size
 
@@ -181,9 +191,10 @@ class CausalSelfAttention(nn.Module):
     """Grouped-query attention with RoPE and a static KV cache (reference ``model.py:89-173``):
     fused ``attn`` projection laid out ``[groups, q_per_kv + 2, head_size]``, output ``proj``.
 
-    The cache is ``[B, groups, max_seq_length, head_size]`` per tensor. A multi-token
-    cached call is a prefill from position 0: it attends within its own tokens
-    (causal SDPA, flash or memory-efficient kernels only) and stores k, v. A single-token
+    The cache is ``[B, groups, max_seq_length, head_size]`` per tensor, or an ``ops.KVCacheQ4``
+    (inference only). A multi-token cached call is a prefill from position 0: it attends
+    within its own tokens (causal SDPA, flash or memory-efficient kernels only, or
+    ``ops.attention``: ``HybridConfig.attention``) and stores k, v. A single-token
     call attends over the cache up to its position; its products are issued with
     contiguous right operands."""
 
@@ -197,7 +208,7 @@ class CausalSelfAttention(nn.Module):
         self.attn = nn.Linear(config.n_embd, (self.n_head + 2 * self.n_query_groups) * self.head_size,
                               bias=config.bias)
         self.proj = nn.Linear(self.n_head * self.head_size, config.n_embd, bias=config.bias)
-        self.kv_cache: tuple[torch.Tensor, torch.Tensor] | None = None
+        self.kv_cache: tuple[torch.Tensor, torch.Tensor] | ops.KVCacheQ4 | None = None
 
     def forward(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
                 input_pos: torch.Tensor | None = None, mask: torch.Tensor | None = None) -> torch.Tensor:
@@ -208,6 +219,13 @@ class CausalSelfAttention(nn.Module):
         """``forward`` from the fused ``attn`` projection's output ``[B, T, (n_head + 2 G) D]``."""
         b, t, _ = qkv.shape
         G, qpk, D = self.n_query_groups, self.n_head // self.n_query_groups, self.head_size
+        q4 = input_pos is not None and isinstance(self.kv_cache, ops.KVCacheQ4)
+        if q4 and t == 1:
+            if not _inference(qkv):
+                raise NotImplementedError("a 4-bit cache is decoded without gradients")
+            # One launch (and a merge for long caches), as below.
+            o = ops.attention_decode_q4(qkv, cos, sin, input_pos, self.kv_cache, self.n_head)
+            return ops.linear(o.reshape(b, 1, self.n_head * D), self.proj.weight, self.proj.bias)
         if (t == 1 and input_pos is not None and self.kv_cache is not None and _inference(qkv)
                 and ops.attention_decode_supported(qkv, qpk, D)):
             # RoPE, the cache store and the attention of the token in one HIP launch.
@@ -219,7 +237,7 @@ class CausalSelfAttention(nn.Module):
             # this one the projection output).  Select the rows of input_pos and build the
             # causal mask over the cache here.
             cos, sin = cos.index_select(0, input_pos), sin.index_select(0, input_pos)
-            if mask is None and self.kv_cache is not None:
+            if mask is None and self.kv_cache is not None and not q4:
                 L = self.kv_cache[0].shape[2]
                 mask = (torch.arange(L, device=qkv.device)[None, :] <= input_pos[:, None]).reshape(1, 1, t, L)
         qkv = qkv.view(b, t, G, qpk + 2, D)
@@ -230,12 +248,17 @@ class CausalSelfAttention(nn.Module):
         if input_pos is not None:
             if self.kv_cache is None:
                 raise RuntimeError("KV cache not set up: call HybridDecoder.setup_caches first")
-            ck, cv = self.kv_cache
-            ck.index_copy_(2, input_pos, k.transpose(1, 2))
-            cv.index_copy_(2, input_pos, v.transpose(1, 2))
-            if t == 1:
-                return ops.linear(self._decode(q, ck, cv, mask).reshape(b, 1, self.n_head * D), self.proj.weight,
-                                  self.proj.bias)
+            if q4:
+                ops.kv_cache_q4_store(self.kv_cache, k, v, input_pos[:1])  # consecutive positions
+            else:
+                ck, cv = self.kv_cache
+                ck.index_copy_(2, input_pos, k.transpose(1, 2))
+                cv.index_copy_(2, input_pos, v.transpose(1, 2))
+                if t == 1:
+                    return ops.linear(self._decode(q, ck, cv, mask).reshape(b, 1, self.n_head * D), self.proj.weight,
+                                      self.proj.bias)
+        if self.config.attention == "hip" and ops.attention_supported(q, D):
+            return self.proj(ops.attention(q, k, v).reshape(b, t, self.n_head * D))
         q, k, v = (z.transpose(1, 2) for z in (q, k, v))
         if qpk > 1:
             k, v = k.repeat_interleave(qpk, dim=1), v.repeat_interleave(qpk, dim=1)
@@ -403,16 +426,24 @@ class HybridDecoder(nn.Module):
             at = blk.attn
             w = at.attn.weight
             G, qpk, D = at.n_query_groups, at.n_head // at.n_query_groups, at.head_size
+            if isinstance(at.kv_cache, ops.KVCacheQ4):
+                continue  # attention_decode_q4 reads the tables' row too
             if at.kv_cache is None or not _inference(w) or not ops.attention_decode_supported(w, qpk, D):
                 return False
         return True
 
-    def setup_caches(self, batch: int, max_seq_length: int) -> None:
+    def setup_caches(self, batch: int, max_seq_length: int, kv_bits: int = 16) -> None:
         """Allocate the attention KV caches ``[batch, groups, max_seq_length, head_size]``
         and the causal mask, and drop every gdn2 cache (the next cached forward is a
-        prefill)."""
+        prefill).  ``kv_bits=4``: the KV caches in 4 bits (``ops.KVCacheQ4``; a bf16 or fp16
+        model on the GPU, heads of 64 or 128 channels, inference)."""
         p = self.lm_head.weight
         c = self.config
+        if kv_bits not in (4, 16):
+            raise ValueError(f"kv_bits must be 4 or 16 (the model's dtype), got {kv_bits}")
+        if kv_bits == 4 and not ops.attention_decode_q4_supported(p, c.n_head // c.n_query_groups, c.head_size):
+            raise NotImplementedError("a 4-bit cache needs a bf16 or fp16 model on the GPU, heads of 64 or 128 "
+                                      "channels and at most 16 query heads per group")
         self.max_seq_length = max_seq_length
         self.mask_cache = torch.tril(torch.ones(max_seq_length, max_seq_length, dtype=torch.bool,
                                                 device=p.device))[None, None]
@@ -421,6 +452,9 @@ class HybridDecoder(nn.Module):
             blk.gdn2_cache = None
             if not blk.use_gdn2:
                 shape = (batch, c.n_query_groups, max_seq_length, c.head_size)
+                if kv_bits == 4:
+                    blk.attn.kv_cache = ops.kv_cache_q4(*shape, device=p.device)
+                    continue
                 blk.attn.kv_cache = (torch.zeros(shape, dtype=p.dtype, device=p.device),
                                      torch.zeros(shape, dtype=p.dtype, device=p.device))
 
@@ -463,6 +497,22 @@ class HybridDecoder(nn.Module):
             x = x[:, -1:]
         return self.lm_head(self.ln_f(x))
 
+    def token_logprobs(self, idx: torch.Tensor, targets: torch.Tensor | None = None, top_k: int = 0,
+                       ignore_index: int = -100) -> ops.TokenLogprobs:
+        """``ops.token_logprobs`` of ``targets [B, T]`` over this model's logits of ``idx [B, T]``; without
+        ``targets`` of each next token of ``idx`` (``[B, T - 1]``)."""
+        logits = self(idx)
+        if targets is None:
+            logits, targets = logits[:, :-1], idx[:, 1:]
+        return ops.token_logprobs(logits, targets, top_k=top_k, ignore_index=ignore_index)
+
+    def loss(self, idx: torch.Tensor, targets: torch.Tensor | None = None, ignore_index: int = -100) -> torch.Tensor:
+        """Mean negative log probability of the targets that are not ignored (0 where all are);
+        arguments as :meth:`token_logprobs`."""
+        r = self.token_logprobs(idx, targets, ignore_index=ignore_index)
+        n = ((idx[:, 1:] if targets is None else targets) != ignore_index).sum()
+        return -r.logprobs.sum() / n.clamp_min(1)
+
 
 class GreedyDecoder:
     """Prefill, then greedy decode with the step captured once as a HIP graph.
@@ -470,12 +520,23 @@ class GreedyDecoder:
     ``generate(prompt, n)`` returns the ``n`` generated token ids ``[B, n]``. The
     captured step reads the previous token and position from static device tensors,
     writes the next token and advances the position, so the host only replays it.
+
+    ``kv_bits=4`` decodes from 4-bit KV caches (``HybridDecoder.setup_caches``).  With
+    ``keep_logprobs=n``, ``logprobs`` holds the last step's ``ops.TokenLogprobs`` (of the token it
+    chose, with ``n`` alternatives; overwritten by the next step), and ``generate`` leaves every
+    step's in ``sequence_logprobs`` (``[B, n_tokens, ...]``).
     """
 
-    def __init__(self, model: HybridDecoder, use_graph: bool = True, keep_logits: bool = False) -> None:
+    def __init__(self, model: HybridDecoder, use_graph: bool = True, keep_logits: bool = False,
+                 kv_bits: int = 16, keep_logprobs: int | None = None) -> None:
         self.model = model
         self.use_graph = use_graph
         self.keep_logits = keep_logits
+        self.kv_bits = kv_bits
+        self.keep_logprobs = keep_logprobs
+        self.logprobs: ops.TokenLogprobs | None = None
+        self._replayed_logprobs: ops.TokenLogprobs | None = None
+        self.sequence_logprobs: ops.TokenLogprobs | None = None
         self.graph: torch.cuda.CUDAGraph | None = None
         self.logits: torch.Tensor | None = None  # last step's fp32 logits [B, vocab] (keep_logits)
 
@@ -483,13 +544,15 @@ class GreedyDecoder:
     def prefill(self, prompt: torch.Tensor, max_new_tokens: int) -> torch.Tensor:
         B, T = prompt.shape
         dev = prompt.device
-        self.model.setup_caches(B, T + max_new_tokens)
+        self.model.setup_caches(B, T + max_new_tokens, self.kv_bits)
         self.graph = None
         logits = self.model(prompt, input_pos=torch.arange(T, device=dev), last_only=True)[:, -1]
         self.tok = logits.argmax(-1, keepdim=True)
         self.pos = torch.full((1,), T, dtype=torch.long, device=dev)
         if self.keep_logits:
             self.logits = logits.float()
+        if self.keep_logprobs is not None:
+            self.logprobs = ops.token_logprobs(logits, self.tok[:, 0], top_k=self.keep_logprobs)
         return self.tok
 
     def _step(self) -> None:
@@ -498,6 +561,8 @@ class GreedyDecoder:
         self.pos.add_(1)
         if self.keep_logits:
             self.logits.copy_(logits)
+        if self.keep_logprobs is not None:
+            self.logprobs = ops.token_logprobs(logits, self.tok[:, 0], top_k=self.keep_logprobs)
 
     @torch.no_grad()
     def step(self) -> torch.Tensor:
@@ -514,18 +579,28 @@ class GreedyDecoder:
             with torch.cuda.stream(side):
                 self._step()
             torch.cuda.current_stream().wait_stream(side)
+            done = self.logprobs
             self.graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(self.graph):
                 self._step()
+            # The captured step has not run yet: its results are the replays'.
+            self._replayed_logprobs, self.logprobs = self.logprobs, done
             return self.tok
         self.graph.replay()
+        self.logprobs = self._replayed_logprobs
         return self.tok
 
     @torch.no_grad()
     def generate(self, prompt: torch.Tensor, max_new_tokens: int) -> torch.Tensor:
-        out = [self.prefill(prompt, max_new_tokens).clone()]
-        for _ in range(max_new_tokens - 1):
-            out.append(self.step().clone())
+        out, lps = [self.prefill(prompt, max_new_tokens).clone()], []
+        for i in range(max_new_tokens):
+            if i > 0:
+                out.append(self.step().clone())
+            if self.keep_logprobs is not None:
+                lps.append([None if x is None else x.clone() for x in self.logprobs])
+        if self.keep_logprobs is not None:
+            self.sequence_logprobs = ops.TokenLogprobs(
+                *(None if x[0] is None else torch.stack(x, dim=1) for x in zip(*lps)))
         return torch.cat(out, dim=1)
 
 

@@ -200,3 +200,21 @@ def test_attention_decode_q4_entry_point_checks(lib, want, over):
     assert lib.gdn2_attn_decode_q4(4096, a["cos"], a["cos"], a["pairs"], a["rs"], a["pos"], 0, a["kc"], a["km"], a["kc"],
                                    a["km"], 4096, a["dt"], a["B"], a["G"], a["qpk"], a["D"], a["L"], 1.0, None, 0,
                                    None) == want
+
+
+def test_hybrid_options_are_checked():
+    from qwendopamine_amd.hybrid import HybridConfig, HybridDecoder
+
+    with pytest.raises(ValueError):
+        HybridConfig(attention="other")
+    cfg = HybridConfig(n_layer=1, n_embd=64, n_head=1, n_query_groups=1, intermediate_size=64, vocab_size=10,
+                       gdn2_layers=[], block_size=16, attention="hip")
+    m = HybridDecoder(cfg).eval()
+    with pytest.raises(ValueError):
+        m.setup_caches(1, 8, kv_bits=8)
+    with pytest.raises(NotImplementedError):
+        m.setup_caches(1, 8, kv_bits=4)  # on the CPU
+    idx = torch.zeros(1, 5, dtype=torch.int64)
+    assert m(idx).shape == (1, 5, 10)  # on the CPU "hip" is torch's attention
+    with pytest.raises(RuntimeError):
+        m.loss(idx)
