@@ -418,7 +418,8 @@ int gdn2_attn_fwd(const void *q, const void *k, const void *v, const int64_t *st
                   int io_dtype, const int64_t *kv_lengths, const int64_t *cu_seqlens,
                   const int64_t *cu_seqlens_host, int num_seqs, int B, int Tq, int Tk, int H, int G, int D,
                   float scale, int causal, void *stream);
-size_t gdn2_attn_bwd_workspace_size(int B, int Tq, int H, int G);
+size_t gdn2_attn_bwd_workspace_size(const int64_t *cu_seqlens_host, int num_seqs, int B, int Tq, int Tk, int H, int G,
+                                    int D, int causal);
 int gdn2_attn_bwd(const void *q, const void *k, const void *v, const int64_t *strides, const void *o,
                   const void *o_lo, const float *lse, const void *dout, void *dq, void *dk, void *dv, int io_dtype,
                   const int64_t *kv_lengths, const int64_t *cu_seqlens, const int64_t *cu_seqlens_host,

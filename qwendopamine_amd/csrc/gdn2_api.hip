@@ -608,27 +608,50 @@ int gdn2_token_logprobs_bwd(const void *x, int64_t inner_rows, int64_t outer_str
     return launch_logprobs_bwd(p, io_dtype, static_cast<hipStream_t>(stream)) == hipSuccess ? GDN2_OK : GDN2_ERR_LAUNCH;
 }
 
+// The sizes gdn2_attn_fwd, gdn2_attn_bwd and its workspace depend on, checked.
+static int fill_attn_sizes(AttnTrainParams &p, const int64_t *cu_host, int num_seqs, int B, int Tq, int Tk, int H,
+                           int G, int D, int causal)
+{
+    if (B < 0 || Tq < 0 || Tk < 0 || H < 1 || G < 1 || D < 1 || H % G != 0) return GDN2_ERR_INVALID;
+    if (Tq > (1 << 30) || Tk > (1 << 30) || B > (1 << 30) || H > (1 << 20) || D > (1 << 20) || num_seqs > (1 << 30))
+        return GDN2_ERR_UNSUPPORTED;
+    p.max_q = Tq;
+    p.k_tiles = static_cast<int64_t>(B) * ((Tk + 127) / 128);
+    if (cu_host) {
+        if (B != 1 || Tq != Tk || num_seqs < 0) return GDN2_ERR_INVALID;
+        if (cu_host[0] != 0 || cu_host[num_seqs] != Tq) return GDN2_ERR_INVALID;
+        p.max_q = 0;
+        p.k_tiles = 0;
+        for (int i = 0; i < num_seqs; ++i) {
+            const int64_t n = cu_host[i + 1] - cu_host[i];
+            if (n < 0 || n > Tq) return GDN2_ERR_INVALID;
+            if (n > p.max_q) p.max_q = static_cast<int>(n);
+            p.k_tiles += (n + 127) / 128;
+        }
+    }
+    p.nseq = cu_host ? num_seqs : B;
+    p.B = B; p.Tq = Tq; p.Tk = Tk; p.H = H; p.G = G; p.D = D;
+    p.causal = causal != 0;
+    p.splits = attn_bwd_splits(p);
+    // One launch of at most 2^31 - 1 workgroups, the smallest of them 32 rows.
+    const double longest = p.max_q > Tk ? p.max_q : Tk;
+    if ((longest / 32 + 1) * p.nseq * H * p.splits > 2147483000.0 || static_cast<double>(B) * Tq * H > 17179869184.0 ||
+        static_cast<double>(B) * (H + G) > 500000000.0 || static_cast<double>(B) * Tk * G * D > 500000000000.0)
+        return GDN2_ERR_UNSUPPORTED;
+    return GDN2_OK;
+}
+
 // Shared by gdn2_attn_fwd and gdn2_attn_bwd: checks, and the parameters both take.
 static int fill_attn_args(AttnTrainParams &p, const void *q, const void *k, const void *v, const int64_t *strides,
                           int io_dtype, const int64_t *kv_lengths, const int64_t *cu, const int64_t *cu_host,
                           int num_seqs, int B, int Tq, int Tk, int H, int G, int D, float scale, int causal)
 {
-    if (!valid_dtype(io_dtype) || B < 0 || Tq < 0 || Tk < 0 || H < 1 || G < 1 || D < 1 || H % G != 0)
+    if (!valid_dtype(io_dtype) || !strides || (cu == nullptr) != (cu_host == nullptr) || (cu && kv_lengths))
         return GDN2_ERR_INVALID;
-    if (!strides || (cu == nullptr) != (cu_host == nullptr)) return GDN2_ERR_INVALID;
+    const int st = fill_attn_sizes(p, cu_host, num_seqs, B, Tq, Tk, H, G, D, causal);
+    if (st != GDN2_OK) return st;
     if (!attn_train_supported(io_dtype, D)) return GDN2_ERR_UNSUPPORTED;
     if (!(scale > 0.0f) || scale > 1e30f) return GDN2_ERR_UNSUPPORTED;
-    p.max_q = Tq;
-    if (cu) {
-        if (B != 1 || Tq != Tk || kv_lengths || num_seqs < 0) return GDN2_ERR_INVALID;
-        if (cu_host[0] != 0 || cu_host[num_seqs] != Tq) return GDN2_ERR_INVALID;
-        p.max_q = 0;
-        for (int i = 0; i < num_seqs; ++i) {
-            const int64_t n = cu_host[i + 1] - cu_host[i];
-            if (n < 0 || n > Tq) return GDN2_ERR_INVALID;
-            if (n > p.max_q) p.max_q = static_cast<int>(n);
-        }
-    }
     if ((B > 0 && Tq > 0 && !q) || (B > 0 && Tk > 0 && (!k || !v))) return GDN2_ERR_INVALID;
     if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15)
         return GDN2_ERR_INVALID;
@@ -637,17 +660,9 @@ static int fill_attn_args(AttnTrainParams &p, const void *q, const void *k, cons
         if (strides[i] < 0 || (size[i] > 1 && strides[i] % 8 != 0)) return GDN2_ERR_INVALID;
         (i < 3 ? p.qs : i < 6 ? p.ks : p.vs)[i % 3] = strides[i];
     }
-    p.nseq = cu ? num_seqs : B;
-    // One launch of at most 2^31 - 1 workgroups, the smallest of them 32 rows.
-    const int64_t longest = p.max_q > Tk ? p.max_q : Tk;
-    if (Tq > (1 << 30) || Tk > (1 << 30) || (longest / 32 + 1) * static_cast<int64_t>(p.nseq) * H > 2147483647LL ||
-        static_cast<int64_t>(B) * Tq * H > (static_cast<int64_t>(1) << 34))
-        return GDN2_ERR_UNSUPPORTED;
     p.q = q; p.k = k; p.v = v;
     p.kv_len = kv_lengths;
     p.cu = cu;
-    p.B = B; p.Tq = Tq; p.Tk = Tk; p.H = H; p.G = G; p.D = D;
-    p.causal = causal != 0;
     p.scale = scale;
     return GDN2_OK;
 }
@@ -669,10 +684,12 @@ int gdn2_attn_fwd(const void *q, const void *k, const void *v, const int64_t *st
     return launch_attn_fwd(p, io_dtype, static_cast<hipStream_t>(stream)) == hipSuccess ? GDN2_OK : GDN2_ERR_LAUNCH;
 }
 
-size_t gdn2_attn_bwd_workspace_size(int B, int Tq, int H, int G)
+size_t gdn2_attn_bwd_workspace_size(const int64_t *cu_seqlens_host, int num_seqs, int B, int Tq, int Tk, int H, int G,
+                                    int D, int causal)
 {
-    if (B < 0 || Tq < 0 || H < 1 || G < 1) return 0;
-    return attn_bwd_workspace_bytes(B, Tq, H, G);
+    AttnTrainParams p = {};
+    if (fill_attn_sizes(p, cu_seqlens_host, num_seqs, B, Tq, Tk, H, G, D, causal) != GDN2_OK) return 0;
+    return attn_bwd_workspace_bytes(p);
 }
 
 int gdn2_attn_bwd(const void *q, const void *k, const void *v, const int64_t *strides, const void *o,
@@ -690,18 +707,14 @@ int gdn2_attn_bwd(const void *q, const void *k, const void *v, const int64_t *st
     if ((reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(o_lo) | reinterpret_cast<uintptr_t>(dout) | reinterpret_cast<uintptr_t>(dq) |
          reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv)) & 15)
         return GDN2_ERR_INVALID;
-    if (!workspace || workspace_bytes < attn_bwd_workspace_bytes(B, Tq, H, G) ||
-        (reinterpret_cast<uintptr_t>(workspace) & 15))
+    if (!workspace || workspace_bytes < attn_bwd_workspace_bytes(p) || (reinterpret_cast<uintptr_t>(workspace) & 15))
         return GDN2_ERR_WORKSPACE;
     p.o = const_cast<void *>(o);
     p.o_lo = const_cast<void *>(o_lo);
     p.lse = const_cast<float *>(lse);
     p.dout = dout;
     p.dq = dq; p.dk = dk; p.dv = dv;
-    p.delta = static_cast<float *>(workspace);
-    p.mx_do = reinterpret_cast<unsigned *>(static_cast<char *>(workspace) +
-                                           ((static_cast<size_t>(B) * H * Tq * sizeof(float) + 15) & ~static_cast<size_t>(15)));
-    p.mx_v = p.mx_do + static_cast<size_t>(B) * H;
+    attn_bwd_workspace(p, workspace);
     return launch_attn_bwd(p, io_dtype, static_cast<hipStream_t>(stream)) == hipSuccess ? GDN2_OK : GDN2_ERR_LAUNCH;
 }
 

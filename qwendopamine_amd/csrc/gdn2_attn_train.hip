@@ -96,14 +96,14 @@ __device__ __forceinline__ int swz(int row)
     return (((row & 3) << 1) | ((row >> 2) & 1) | (row & 8)) & (D / 8 - 1);
 }
 
-// One tile, row0 .. row0 + kTile - 1 of nrows rows ts elements apart, requested
+// One tile, row0 .. row0 + ROWS - 1 of nrows rows ts elements apart, requested
 // into LDS.  Rows past the end repeat the last row (never out of bounds, never
 // another sequence's row); the scores of such rows are hidden.
-template <int D, int NW>
+template <int D, int NW, int ROWS = kTile>
 __device__ __forceinline__ void stage(const uint16_t *base, int64_t ts, int row0, int nrows, uint16_t *lds, int wave,
                                       int lane)
 {
-    constexpr int P = D / 8, R = 64 / P, IT = kTile / R;  // pieces per row, rows per request, requests
+    constexpr int P = D / 8, R = 64 / P, IT = ROWS / R;  // pieces per row, rows per request, requests
 #pragma unroll
     for (int it = 0; it < (IT + NW - 1) / NW; ++it) {
         const int c = it * NW + wave;
@@ -116,31 +116,52 @@ __device__ __forceinline__ void stage(const uint16_t *base, int64_t ts, int row0
     }
 }
 
-// A operand, rows r0 + (l & 31), contraction step s of the row (16 channels).
+// A lane's byte offset within a tile for row reads (row l & 31, its half of the
+// 16 channels of step 0) and for column reads (rows 4 h + 0..3 of 16, channel
+// l & 31 of 32).  A row's pitch is a power of two, so that the permutation of
+// any step and channel block is one XOR of the offset with a constant.
 template <int D>
-__device__ __forceinline__ uint4 row_frag(const uint16_t *lds, int r0, int s, int lane)
+__device__ __forceinline__ int row_base(int lane)
 {
-    const int row = r0 + (lane & 31);
-    return *reinterpret_cast<const uint4 *>(lds + row * D + (((2 * s + (lane >> 5)) ^ swz<D>(row)) * 8));
+    return (lane & 31) * (2 * D) + (((lane >> 5) ^ swz<D>(lane & 31)) * 16);
+}
+template <int D>
+__device__ __forceinline__ int col_base(int lane)
+{
+    const int i = lane & 15, grp = (lane >> 4) & 1, r = 4 * (lane >> 5) + (i >> 2);
+    return r * (2 * D) + (((grp * 2 + ((i & 3) >> 1)) ^ swz<D>(r)) * 16) + (i & 1) * 8;
+}
+
+// A operand, rows r0 + (l & 31) of the tile, contraction step s of the row (16
+// channels); `at` is row_base plus the tile's place in smem.
+template <int D>
+__device__ __forceinline__ uint4 row_frag(const char *smem, int at, int r0, int s)
+{
+    return *reinterpret_cast<const uint4 *>(smem + r0 * (2 * D) + (at ^ (32 * s)));
 }
 
 // A operand of the transposed tile: channels 32 dt + (l & 31), contraction
-// over rows r0 + {4 h + 0..3, 8 + 4 h + 0..3}.
+// over rows r0 + {4 h + 0..3, 8 + 4 h + 0..3}; `at` is col_base plus the tile's place.
 template <int D>
-__device__ __forceinline__ uint4 col_frag(const uint16_t *lds, int r0, int dt, int lane)
+__device__ __forceinline__ uint4 col_frag(const char *smem, int at, int r0, int dt)
 {
     typedef short s4 __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) s4 *lds_s4;
-    const int i = lane & 15, grp = (lane >> 4) & 1, h = lane >> 5;
     uint2 r[2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        const int row = r0 + 8 * u + 4 * h + (i >> 2);
-        const int piece = (dt * 4 + grp * 2 + ((i & 3) >> 1)) ^ swz<D>(8 * u + 4 * h + (i >> 2));
+    for (int u = 0; u < 2; ++u)
         r[u] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                             (lds_s4)(lds + row * D + piece * 8 + (i & 1) * 4)));
-    }
+                                             (lds_s4)(smem + (r0 + 8 * u) * (2 * D) +
+                                                      (at ^ ((64 * dt) ^ ((128 * u) & (2 * D - 1)))))));
     return make_uint4(r[0].x, r[0].y, r[1].x, r[1].y);
+}
+
+// Keeps the compiler from forming every step's address before the loop, where
+// they would hold registers throughout.
+__device__ __forceinline__ int opaque(int x)
+{
+    asm volatile("" : "+v"(x));
+    return x;
 }
 
 // What a workgroup works on: head h of sequence s, its rows and their extent.
@@ -209,10 +230,13 @@ template <PrecKind PK, int D, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(AttnTrainParams p)
 {
     constexpr int KS = D / 16, DT = D / 32, BM = 32 * NW;
-    __shared__ __align__(16) uint16_t sk[2][kTile * D];
-    __shared__ __align__(16) uint16_t sv[2][kTile * D];
+    constexpr int kBytes = kTile * D * 2;
+    __shared__ __align__(256) char smem[4 * kBytes];  // two tiles of k, two of v
+    auto tile_k = [&](int t) __attribute__((always_inline)) { return reinterpret_cast<uint16_t *>(smem + (t & 1) * kBytes); };
+    auto tile_v = [&](int t) __attribute__((always_inline)) { return reinterpret_cast<uint16_t *>(smem + (2 + (t & 1)) * kBytes); };
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, h = lane >> 5;
+    const int rb = row_base<D>(lane), cb = col_base<D>(lane);
     const Where w = where_q(p);
     const int m0 = w.tile * BM;
     if (m0 >= w.nq) return;
@@ -244,25 +268,25 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(AttnTrainParams p)
 
     const int nt = kend > 0 ? (kend + kTile - 1) / kTile : 0;
     if (nt > 0) {
-        stage<D, NW>(kb, p.ks[1], 0, w.nk, sk[0], wave, lane);
-        stage<D, NW>(vb, p.vs[1], 0, w.nk, sv[0], wave, lane);
+        stage<D, NW>(kb, p.ks[1], 0, w.nk, tile_k(0), wave, lane);
+        stage<D, NW>(vb, p.vs[1], 0, w.nk, tile_v(0), wave, lane);
     }
     for (int t = 0; t < nt; ++t) {
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();  // tile t has landed, and every wave is done with tile t - 1
         if (t + 1 < nt) {
-            stage<D, NW>(kb, p.ks[1], (t + 1) * kTile, w.nk, sk[(t + 1) & 1], wave, lane);
-            stage<D, NW>(vb, p.vs[1], (t + 1) * kTile, w.nk, sv[(t + 1) & 1], wave, lane);
+            stage<D, NW>(kb, p.ks[1], (t + 1) * kTile, w.nk, tile_k(t + 1), wave, lane);
+            stage<D, NW>(vb, p.vs[1], (t + 1) * kTile, w.nk, tile_v(t + 1), wave, lane);
         }
         const int j0 = t * kTile;
         if (j0 >= wend) continue;
-        const uint16_t *kt = sk[t & 1], *vt = sv[t & 1];
+        const int kr = opaque(rb + (t & 1) * kBytes), vc = opaque(cb + (2 + (t & 1)) * kBytes);
         f32x16 s[2];
 #pragma unroll
         for (int a = 0; a < 2; ++a) {
             s[a] = zero16();
 #pragma unroll
-            for (int st = 0; st < KS; ++st) s[a] = mma32<PK>(s[a], row_frag<D>(kt, 32 * a, st, lane), qf[st]);
+            for (int st = 0; st < KS; ++st) s[a] = mma32<PK>(s[a], row_frag<D>(smem, kr, 32 * a, st), qf[st]);
         }
         if (j0 + kTile > wlim) {
             hide<true>(s[0], j0, h, lim);
@@ -300,7 +324,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(AttnTrainParams p)
             for (int u = 0; u < 2; ++u) {
                 const uint4 pf = pack8<PK>(s[a], u);
 #pragma unroll
-                for (int d = 0; d < DT; ++d) acc[d] = mma32<PK>(acc[d], col_frag<D>(vt, 32 * a + 16 * u, d, lane), pf);
+                for (int d = 0; d < DT; ++d) acc[d] = mma32<PK>(acc[d], col_frag<D>(smem, vc, 32 * a + 16 * u, d), pf);
             }
     }
     l = half_add(l);
@@ -333,54 +357,33 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(AttnTrainParams p)
 
 // ---------------------------------------------------------------- backward
 
-// D = dO . O per query (fp32), one 16-byte piece per lane.  fp16 also leaves
-// the largest squared row norm of dO per (row of the batch, head), from which
-// and from V's the kernels below scale dS into fp16's range (norm_max_kernel).
-template <PrecKind PK, int D>
-__global__ __launch_bounds__(256) void attn_delta_kernel(AttnTrainParams p)
-{
-    constexpr int P = D / 8;
-    const int64_t row = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / P;  // (b * Tq + t) * H + h
-    const int piece = threadIdx.x % P;
-    const int64_t rows = static_cast<int64_t>(p.B) * p.Tq * p.H;
-    if (row >= rows) return;  // whole groups of P lanes
-    const int hh = static_cast<int>(row % p.H);
-    const int64_t bt = row / p.H;
-    const int b = static_cast<int>(bt / p.Tq), t = static_cast<int>(bt % p.Tq);
-    typename Prec<PK>::frag fo, fl, fd;
-    fo.u = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.o) + row * D + piece * 8);
-    fl.u = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.o_lo) + row * D + piece * 8);
-    fd.u = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.dout) + row * D + piece * 8);
-    float xo[8], xl[8], xd[8];
-    unpack_frag<PK>(fo, xo);
-    unpack_frag<PK>(fl, xl);
-    unpack_frag<PK>(fd, xd);
-    float s = 0.0f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) s = fmaf(xo[e] + xl[e], xd[e], s);
-#pragma unroll
-    for (int k = 1; k < P; k <<= 1) s += __shfl_xor(s, k, 64);
-    if (piece == 0) p.delta[(static_cast<int64_t>(b) * p.H + hh) * p.Tq + t] = s;
-}
-
-// fp16 only: the largest squared row norm of x [B, T, heads, D] per (b, head)
-// into mx [B][heads] (cleared before), by integer maxima of the float bits
-// (non-negative floats order as integers, so the order of arrival does not
-// matter).  Rows that are not finite, or past len[b], do not count.
-constexpr int kNormParts = 4;  // workgroups per (b, head)
+// fp16 only: the largest squared row norms of dO per (batch row, head) and of V per
+// (batch row, group), from which the kernels below scale dS into fp16's range;
+// kNormParts workgroups each, [B][heads][kNormParts].  Rows that are not finite,
+// or past the row's length, do not count.
+constexpr int kNormParts = 4;
 template <int D>
-__global__ __launch_bounds__(256) void norm_max_kernel(const uint16_t *x, int64_t sb, int64_t st, int64_t sh, int T,
-                                                       const int64_t *len, int heads, unsigned *mx)
+__global__ __launch_bounds__(256) void norm_max_kernel(AttnTrainParams p)
 {
     constexpr int P = D / 8, R = 256 / P;
-    const int bh = blockIdx.x % (gridDim.x / kNormParts), part = blockIdx.x / (gridDim.x / kNormParts);
-    const int b = bh / heads, hh = bh - b * heads;
-    if (len && len[b] < T) T = static_cast<int>(len[b] < 0 ? 0 : len[b]);
+    __shared__ float s_best[4];
+    const int ndo = p.B * p.H;
+    const int part = blockIdx.x % kNormParts;
+    int bh = blockIdx.x / kNormParts;
+    const bool is_v = bh >= ndo;
+    if (is_v) bh -= ndo;
+    const int heads = is_v ? p.G : p.H, b = bh / heads, hh = bh - b * heads;
+    const int64_t HD = static_cast<int64_t>(p.H) * D;
+    const uint16_t *x = is_v ? static_cast<const uint16_t *>(p.v) + b * p.vs[0] + hh * p.vs[2]
+                             : static_cast<const uint16_t *>(p.dout) + b * p.Tq * HD + hh * D;
+    const int64_t st = is_v ? p.vs[1] : HD;
+    int T = is_v ? p.Tk : p.Tq;
+    if (is_v && p.kv_len && p.kv_len[b] < T) T = static_cast<int>(p.kv_len[b] < 0 ? 0 : p.kv_len[b]);
     const int piece = threadIdx.x % P;
     float best = 0.0f;
     for (int t = part * R + threadIdx.x / P; t < T; t += kNormParts * R) {
         typename Prec<PrecKind::F16>::frag f;
-        f.u = *reinterpret_cast<const uint4 *>(x + b * sb + t * st + hh * sh + piece * 8);
+        f.u = *reinterpret_cast<const uint4 *>(x + t * st + piece * 8);
         float v[8];
         unpack_frag<PrecKind::F16>(f, v);
         float s = 0.0f;
@@ -392,13 +395,11 @@ __global__ __launch_bounds__(256) void norm_max_kernel(const uint16_t *x, int64_
     }
 #pragma unroll
     for (int k = 32; k > 0; k >>= 1) best = fmaxf(best, __shfl_xor(best, k, 64));
-    if ((threadIdx.x & 63) == 0) atomicMax(mx + bh, __float_as_uint(best));
-}
-
-__global__ __launch_bounds__(256) void clear_kernel(unsigned *x, int n)
-{
-    const int i = blockIdx.x * 256 + threadIdx.x;
-    if (i < n) x[i] = 0u;
+    if ((threadIdx.x & 63) == 0) s_best[threadIdx.x >> 6] = best;
+    __syncthreads();
+    if (threadIdx.x == 0)
+        (is_v ? p.mx_v : p.mx_do)[bh * kNormParts + part] =
+            fmaxf(fmaxf(s_best[0], s_best[1]), fmaxf(s_best[2], s_best[3]));
 }
 
 // fp16: P is held scaled by 2^kP16 (P = 1 / T of long rows stays a normal
@@ -410,7 +411,12 @@ template <PrecKind PK>
 __device__ __forceinline__ float ds_scale(const AttnTrainParams &p, const Where &w)
 {
     if constexpr (PK != PrecKind::F16) return 1.0f;
-    const float a = __uint_as_float(p.mx_do[w.bq * p.H + w.h]), b = __uint_as_float(p.mx_v[w.bk * p.G + w.g]);
+    float a = 0.0f, b = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kNormParts; ++i) {
+        a = fmaxf(a, p.mx_do[(w.bq * p.H + w.h) * kNormParts + i]);
+        b = fmaxf(b, p.mx_v[(w.bk * p.G + w.g) * kNormParts + i]);
+    }
     const float bound = 2.0f * sqrtf(a) * sqrtf(b);
     if (!(bound > 0.0f)) return 1.0f;
     int e = 13 - ilogbf(bound);
@@ -418,15 +424,19 @@ __device__ __forceinline__ float ds_scale(const AttnTrainParams &p, const Where 
     return ldexpf(1.0f, e);
 }
 
-// dQ: queries resident, one pass over the keys.
+// dQ: queries resident, one pass over the keys.  Also forms D = dO . (O + what its
+// rounding left out) per query, which the kernel below reads.
 template <PrecKind PK, int D, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void attn_dq_kernel(AttnTrainParams p)
 {
     constexpr int KS = D / 16, DT = D / 32, BM = 32 * NW;
-    __shared__ __align__(16) uint16_t sk[2][kTile * D];
-    __shared__ __align__(16) uint16_t sv[2][kTile * D];
+    constexpr int kBytes = kTile * D * 2;
+    __shared__ __align__(256) char smem[4 * kBytes];  // two tiles of k, two of v
+    auto tile_k = [&](int t) __attribute__((always_inline)) { return reinterpret_cast<uint16_t *>(smem + (t & 1) * kBytes); };
+    auto tile_v = [&](int t) __attribute__((always_inline)) { return reinterpret_cast<uint16_t *>(smem + (2 + (t & 1)) * kBytes); };
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, h = lane >> 5;
+    const int rb = row_base<D>(lane), cb = col_base<D>(lane);
     const Where w = where_q(p);
     const int m0 = w.tile * BM;
     if (m0 >= w.nq) return;
@@ -445,7 +455,24 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dq_kernel(AttnTrainParams p)
         df[s] = *reinterpret_cast<const uint4 *>(dr + 16 * s + 8 * h);
     }
     const float sc = ds_scale<PK>(p, w);
-    const float lse = p.lse[srow], dl = p.delta[srow] * sc;
+    float dl = 0.0f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+        typename Prec<PK>::frag fd, fo, fl;
+        fd.u = df[s];
+        fo.u = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.o) + orow + 16 * s + 8 * h);
+        fl.u = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.o_lo) + orow + 16 * s + 8 * h);
+        float xd[8], xo[8], xl[8];
+        unpack_frag<PK>(fd, xd);
+        unpack_frag<PK>(fo, xo);
+        unpack_frag<PK>(fl, xl);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dl = fmaf(xo[e] + xl[e], xd[e], dl);
+    }
+    dl = half_add(dl);
+    if (h == 0 && qi < w.nq) p.delta[srow] = dl;
+    dl *= sc;
+    const float lse = p.lse[srow];
 
     int kend = w.nk;
     if (p.causal) {
@@ -463,26 +490,27 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dq_kernel(AttnTrainParams p)
     for (int d = 0; d < DT; ++d) acc[d] = zero16();
     const int nt = kend > 0 ? (kend + kTile - 1) / kTile : 0;
     if (nt > 0) {
-        stage<D, NW>(kb, p.ks[1], 0, w.nk, sk[0], wave, lane);
-        stage<D, NW>(vb, p.vs[1], 0, w.nk, sv[0], wave, lane);
+        stage<D, NW>(kb, p.ks[1], 0, w.nk, tile_k(0), wave, lane);
+        stage<D, NW>(vb, p.vs[1], 0, w.nk, tile_v(0), wave, lane);
     }
     for (int t = 0; t < nt; ++t) {
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
         if (t + 1 < nt) {
-            stage<D, NW>(kb, p.ks[1], (t + 1) * kTile, w.nk, sk[(t + 1) & 1], wave, lane);
-            stage<D, NW>(vb, p.vs[1], (t + 1) * kTile, w.nk, sv[(t + 1) & 1], wave, lane);
+            stage<D, NW>(kb, p.ks[1], (t + 1) * kTile, w.nk, tile_k(t + 1), wave, lane);
+            stage<D, NW>(vb, p.vs[1], (t + 1) * kTile, w.nk, tile_v(t + 1), wave, lane);
         }
         const int j0 = t * kTile;
         if (j0 >= wend) continue;
-        const uint16_t *kt = sk[t & 1], *vt = sv[t & 1];
+        const int kr = opaque(rb + (t & 1) * kBytes), vr = opaque(rb + (2 + (t & 1)) * kBytes);
+        const int kc = opaque(cb + (t & 1) * kBytes);
 #pragma unroll
         for (int a = 0; a < 2; ++a) {
             f32x16 s = zero16(), dp = zero16();
 #pragma unroll
-            for (int st = 0; st < KS; ++st) s = mma32<PK>(s, row_frag<D>(kt, 32 * a, st, lane), qf[st]);
+            for (int st = 0; st < KS; ++st) s = mma32<PK>(s, row_frag<D>(smem, kr, 32 * a, st), qf[st]);
 #pragma unroll
-            for (int st = 0; st < KS; ++st) dp = mma32<PK>(dp, row_frag<D>(vt, 32 * a, st, lane), df[st]);
+            for (int st = 0; st < KS; ++st) dp = mma32<PK>(dp, row_frag<D>(smem, vr, 32 * a, st), df[st]);
             if (j0 + kTile > wlim) hide<true>(s, j0 + 32 * a, h, lim);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -493,7 +521,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dq_kernel(AttnTrainParams p)
             for (int u = 0; u < 2; ++u) {
                 const uint4 pf = pack8<PK>(s, u);
 #pragma unroll
-                for (int d = 0; d < DT; ++d) acc[d] = mma32<PK>(acc[d], col_frag<D>(kt, 32 * a + 16 * u, d, lane), pf);
+                for (int d = 0; d < DT; ++d) acc[d] = mma32<PK>(acc[d], col_frag<D>(smem, kc, 32 * a + 16 * u, d), pf);
             }
         }
     }
@@ -508,20 +536,31 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dq_kernel(AttnTrainParams p)
                                                              acc[d][4 * i + 2] * f, acc[d][4 * i + 3] * f));
 }
 
-// dK, dV: keys resident, one pass over the queries of every head of the group.
-template <PrecKind PK, int D, int NW>
-__global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : 1) void attn_dkv_kernel(AttnTrainParams p)
+// dK, dV: keys resident, one pass over the queries of every head of the group,
+// or, where that leaves too few or too uneven workgroups (attn_bwd_splits), over
+// one of p.splits equal shares of it, whose fp32 sums attn_dkv_sum_kernel adds.
+template <PrecKind PK, int D, int NW, int BQ>
+__global__ __launch_bounds__(64 * NW, 2) void attn_dkv_kernel(AttnTrainParams p)
 {
     constexpr int KS = D / 16, DT = D / 32, BN = 32 * NW;
-    __shared__ __align__(16) uint16_t sq[2][kTile * D];
-    __shared__ __align__(16) uint16_t sd[2][kTile * D];
-    __shared__ __align__(16) float sl[2][2][kTile];  // L and scaled D of the tile's queries
+    constexpr int kBytes = BQ * D * 2;
+    // D = 128: V's fragments are read from LDS, K's stay in registers.  Both in
+    // registers is 64 beside 128 of accumulators and 32 of S and dP, and the
+    // kernel spilled 59 (B2 T8192 H16 G4, this kernel alone: 3172 us against 1777).
+    constexpr bool kVLds = D == 128;
+    // Two tiles of q, two of dout, V's rows, and per tile L and scaled D of its queries.
+    constexpr int kOffV = 4 * kBytes, kOffL = kOffV + (kVLds ? BN * D * 2 : 0);
+    __shared__ __align__(256) char smem[kOffL + 4 * BQ * 4];
+    float *const sl = reinterpret_cast<float *>(smem + kOffL);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, h = lane >> 5;
+    const int rb = row_base<D>(lane), cb = col_base<D>(lane);
     Where w;
     const int nbg = p.nseq * p.G, qpk = p.H / p.G;
-    w.tile = blockIdx.x / nbg;
-    const int jg = blockIdx.x - w.tile * nbg;
+    const int ts = blockIdx.x / nbg;
+    w.tile = ts / p.splits;
+    const int share = ts - w.tile * p.splits;
+    const int jg = blockIdx.x - ts * nbg;
     w.s = jg / p.G;
     w.g = jg - w.s * p.G;
     w.h = w.g * qpk;
@@ -532,12 +571,13 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : 1) void attn_dkv_kernel(Attn
     const int kj = n0 + 32 * wave + n;  // this lane's key
     const int kc = kj < w.nk ? kj : (w.nk > 0 ? w.nk - 1 : 0);
     const uint16_t *kr = static_cast<const uint16_t *>(p.k) + w.bk * p.ks[0] + (w.k0 + kc) * p.ks[1] + w.g * p.ks[2];
-    const uint16_t *vr = static_cast<const uint16_t *>(p.v) + w.bk * p.vs[0] + (w.k0 + kc) * p.vs[1] + w.g * p.vs[2];
-    uint4 kf[KS], vf[KS];
+    const uint16_t *vb = static_cast<const uint16_t *>(p.v) + w.bk * p.vs[0] + w.k0 * p.vs[1] + w.g * p.vs[2];
+    const uint16_t *vr = vb + kc * p.vs[1];
+    uint4 kf[KS], vf[kVLds ? 1 : KS];
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
         kf[s] = *reinterpret_cast<const uint4 *>(kr + 16 * s + 8 * h);
-        vf[s] = *reinterpret_cast<const uint4 *>(vr + 16 * s + 8 * h);
+        if constexpr (!kVLds) vf[s] = *reinterpret_cast<const uint4 *>(vr + 16 * s + 8 * h);
     }
     // First query that sees this lane's key, any of the wave's, all of the wave's.
     const int big = 0x7fffffff;
@@ -547,8 +587,8 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : 1) void attn_dkv_kernel(Attn
     const int wall = wk0 + 31 >= w.nk ? big : (p.causal ? wk0 + 31 - w.shift : 0);
     int gfirst = n0 >= w.nk ? big : (p.causal ? n0 - w.shift : 0);
     gfirst = gfirst < 0 ? 0 : gfirst;
-    const int t0 = gfirst / kTile;
-    const int nt = gfirst >= w.nq ? 0 : (w.nq + kTile - 1) / kTile - t0;
+    const int t0 = gfirst / BQ;
+    const int nt = gfirst >= w.nq ? 0 : (w.nq + BQ - 1) / BQ - t0;
     const float c = p.scale * kLog2e;
     const float p16 = PK == PrecKind::F16 ? kP16 : 0.0f;
 
@@ -570,44 +610,50 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : 1) void attn_dkv_kernel(Attn
     }
     const float ds_mul = PK == PrecKind::F16 ? sc * ldexpf(1.0f, -14) : 1.0f;
 
-    const int steps = nt * qpk;
+    // Step x: head x / nt of the group, query tile t0 + x % nt; this share's are x0 .. x0 + steps - 1.
+    const int x0 = static_cast<int>(static_cast<int64_t>(nt) * qpk * share / p.splits);
+    const int steps = static_cast<int>(static_cast<int64_t>(nt) * qpk * (share + 1) / p.splits) - x0;
     const uint16_t *qb = static_cast<const uint16_t *>(p.q) + w.bq * p.qs[0] + w.q0 * p.qs[1];
     const uint16_t *db = static_cast<const uint16_t *>(p.dout) + (w.bq * static_cast<int64_t>(p.Tq) + w.q0) * p.H * D;
     const int64_t sb = static_cast<int64_t>(w.bq) * p.H * p.Tq + w.q0;
-    // Step x: head x / nt of the group, query tile t0 + x % nt.
-    int rh = 0, rt = 0;  // of the step requested next
+    int rh = nt > 0 ? x0 / nt : 0, rt = nt > 0 ? x0 - rh * nt : 0;  // of the step requested next
+    int ct = rt;                                                    // query tile of the current step
     auto request = [&](int buf) __attribute__((always_inline)) {
-        const int hh = w.h + rh, row0 = (t0 + rt) * kTile;
-        stage<D, NW>(qb + hh * p.qs[2], p.qs[1], row0, w.nq, sq[buf], wave, lane);
-        stage<D, NW>(db + hh * D, static_cast<int64_t>(p.H) * D, row0, w.nq, sd[buf], wave, lane);
-        if (tid < 2 * kTile) {
-            const int r = row0 + (tid & (kTile - 1));
-            const float *src = (tid < kTile ? p.lse : p.delta) + sb + static_cast<int64_t>(hh) * p.Tq;
+        const int hh = w.h + rh, row0 = (t0 + rt) * BQ;
+        stage<D, NW, BQ>(qb + hh * p.qs[2], p.qs[1], row0, w.nq, reinterpret_cast<uint16_t *>(smem + buf * kBytes), wave, lane);
+        stage<D, NW, BQ>(db + hh * D, static_cast<int64_t>(p.H) * D, row0, w.nq,
+                     reinterpret_cast<uint16_t *>(smem + (2 + buf) * kBytes), wave, lane);
+        if (tid < 2 * BQ) {
+            const int r = row0 + (tid & (BQ - 1));
+            const float *src = (tid < BQ ? p.lse : p.delta) + sb + static_cast<int64_t>(hh) * p.Tq;
             // Queries past the end: L = +inf hides them.
-            const float x = r < w.nq ? src[r] : (tid < kTile ? INFINITY : 0.0f);
-            sl[buf][tid < kTile ? 0 : 1][tid & (kTile - 1)] = tid < kTile ? x - p16 : x * ds_mul;
+            const float x = r < w.nq ? src[r] : (tid < BQ ? INFINITY : 0.0f);
+            sl[buf * 2 * BQ + tid] = tid < BQ ? x - p16 : x * ds_mul;
         }
         if (++rt == nt) {
             rt = 0;
             ++rh;
         }
     };
-    if (steps > 0) request(0);
-    int ct = 0;  // query tile of the current step
+    if (steps > 0) {
+        request(0);
+        if constexpr (kVLds) stage<D, NW, BN>(vb, p.vs[1], n0, w.nk, reinterpret_cast<uint16_t *>(smem + kOffV), wave, lane);
+    }
     for (int x = 0; x < steps; ++x) {
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
         if (x + 1 < steps) request((x + 1) & 1);
-        const int i0 = (t0 + ct) * kTile;
+        const int i0 = (t0 + ct) * BQ;
         if (++ct == nt) ct = 0;
-        if (i0 + kTile <= wfirst) continue;
-        const uint16_t *qt = sq[x & 1], *dt = sd[x & 1];
-        const float *lt = sl[x & 1][0], *et = sl[x & 1][1];
+        if (i0 + BQ <= wfirst) continue;
+        const int qr = opaque(rb + (x & 1) * kBytes), dr = opaque(rb + (2 + (x & 1)) * kBytes);
+        const int qc = opaque(cb + (x & 1) * kBytes), dc = opaque(cb + (2 + (x & 1)) * kBytes);
+        const float *lt = sl + (x & 1) * 2 * BQ, *et = lt + BQ;
 #pragma unroll
-        for (int a = 0; a < 2; ++a) {
+        for (int a = 0; a < BQ / 32; ++a) {
             f32x16 s = zero16(), dp = zero16();
 #pragma unroll
-            for (int st = 0; st < KS; ++st) s = mma32<PK>(s, row_frag<D>(qt, 32 * a, st, lane), kf[st]);
+            for (int st = 0; st < KS; ++st) s = mma32<PK>(s, row_frag<D>(smem, qr, 32 * a, st), kf[st]);
             if (i0 < wall) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
@@ -616,7 +662,14 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : 1) void attn_dkv_kernel(Attn
                 }
             }
 #pragma unroll
-            for (int st = 0; st < KS; ++st) dp = mma32<PK>(dp, row_frag<D>(dt, 32 * a, st, lane), vf[st]);
+            for (int st = 0; st < KS; ++st) {
+                uint4 bv;
+                if constexpr (kVLds)
+                    bv = row_frag<D>(smem, rb + kOffV, 32 * wave, st);
+                else
+                    bv = vf[st];
+                dp = mma32<PK>(dp, row_frag<D>(smem, dr, 32 * a, st), bv);
+            }
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
                 const float4 lv = *reinterpret_cast<const float4 *>(lt + 32 * a + 8 * b + 4 * h);
@@ -628,7 +681,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : 1) void attn_dkv_kernel(Attn
             for (int u = 0; u < 2; ++u) {
                 const uint4 pf = pack8<PK>(s, u);
 #pragma unroll
-                for (int d = 0; d < DT; ++d) dv[d] = mma32<PK>(dv[d], col_frag<D>(dt, 32 * a + 16 * u, d, lane), pf);
+                for (int d = 0; d < DT; ++d) dv[d] = mma32<PK>(dv[d], col_frag<D>(smem, dc, 32 * a + 16 * u, d), pf);
             }
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
@@ -642,13 +695,27 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : 1) void attn_dkv_kernel(Attn
             for (int u = 0; u < 2; ++u) {
                 const uint4 pf = pack8<PK>(s, u);
 #pragma unroll
-                for (int d = 0; d < DT; ++d) dk[d] = mma32<PK>(dk[d], col_frag<D>(qt, 32 * a + 16 * u, d, lane), pf);
+                for (int d = 0; d < DT; ++d) dk[d] = mma32<PK>(dk[d], col_frag<D>(smem, qc, 32 * a + 16 * u, d), pf);
             }
         }
     }
     if (kj >= kall) return;
     const float fk = p.scale / sc, fv = PK == PrecKind::F16 ? ldexpf(1.0f, -14) : 1.0f;
     const int64_t krow = ((w.bk * static_cast<int64_t>(p.Tk) + w.k0 + kj) * p.G + w.g) * D;
+    if (p.splits > 1) {
+        const int64_t all = static_cast<int64_t>(p.B) * p.Tk * p.G * D;
+        float *pk = p.part + 2 * share * all + krow, *pv = pk + all;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                *reinterpret_cast<float4 *>(pk + 32 * d + 8 * i + 4 * h) = make_float4(
+                    dk[d][4 * i] * fk, dk[d][4 * i + 1] * fk, dk[d][4 * i + 2] * fk, dk[d][4 * i + 3] * fk);
+                *reinterpret_cast<float4 *>(pv + 32 * d + 8 * i + 4 * h) = make_float4(
+                    dv[d][4 * i] * fv, dv[d][4 * i + 1] * fv, dv[d][4 * i + 2] * fv, dv[d][4 * i + 3] * fv);
+            }
+        return;
+    }
     uint16_t *ok = static_cast<uint16_t *>(p.dk) + krow, *ov = static_cast<uint16_t *>(p.dv) + krow;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -661,55 +728,67 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : 1) void attn_dkv_kernel(Attn
         }
 }
 
+// Sums of the shares, in their order; thread: 4 channels of dk or of dv.
+template <PrecKind PK>
+__global__ __launch_bounds__(256) void attn_dkv_sum_kernel(AttnTrainParams p)
+{
+    const int64_t all = static_cast<int64_t>(p.B) * p.Tk * p.G * p.D;
+    int64_t e = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
+    if (e >= 2 * all) return;
+    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int s = 0; s < p.splits; ++s) {
+        const float4 y = *reinterpret_cast<const float4 *>(p.part + 2 * s * all + e);
+        x.x += y.x;
+        x.y += y.y;
+        x.z += y.z;
+        x.w += y.w;
+    }
+    uint16_t *out = static_cast<uint16_t *>(e < all ? p.dk : p.dv) + (e < all ? e : e - all);
+    st_q4<PK>(out, pack4<PK>(x.x, x.y, x.z, x.w));
+}
+
+// Four waves per workgroup, two workgroups per CU: against eight waves and one, the
+// same time on long rows and less on short ones, whose few workgroups fill the card
+// more evenly (forward, B1 T4096 H16 D64: 72 us against 87; packed, 9 sequences of
+// 7013 tokens, H16 D128: 78 against 97; B2 T8192 H16 D128: 556 against 574).
+constexpr int kWaves = 4;
+
 template <PrecKind PK, int D>
 hipError_t fwd_d(AttnTrainParams p, hipStream_t s)
 {
-    constexpr int NW = 8;
-    p.tiles = (p.max_q + 32 * NW - 1) / (32 * NW);
-    hipLaunchKernelGGL((attn_fwd_kernel<PK, D, NW>), dim3(static_cast<unsigned>(p.tiles) * p.nseq * p.H), dim3(64 * NW),
-                       0, s, p);
+    p.tiles = (p.max_q + 32 * kWaves - 1) / (32 * kWaves);
+    hipLaunchKernelGGL((attn_fwd_kernel<PK, D, kWaves>), dim3(static_cast<unsigned>(p.tiles) * p.nseq * p.H),
+                       dim3(64 * kWaves), 0, s, p);
     return hipGetLastError();
 }
 
 template <PrecKind PK, int D>
 hipError_t bwd_d(AttnTrainParams p, hipStream_t s)
 {
-    constexpr int NW = 8;
     hipError_t e;
-    if (p.Tq > 0) {
-        const int64_t rows = static_cast<int64_t>(p.B) * p.Tq * p.H;
-        hipLaunchKernelGGL((attn_delta_kernel<PK, D>), dim3(static_cast<unsigned>((rows * (D / 8) + 255) / 256)),
-                           dim3(256), 0, s, p);
+    if constexpr (PK == PrecKind::F16) {
+        hipLaunchKernelGGL((norm_max_kernel<D>), dim3(kNormParts * p.B * (p.H + p.G)), dim3(256), 0, s, p);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
-    if constexpr (PK == PrecKind::F16) {
-        const int n = p.B * (p.H + p.G);
-        hipLaunchKernelGGL(clear_kernel, dim3((n + 255) / 256), dim3(256), 0, s, p.mx_do, n);
+    if (p.Tq > 0 && p.max_q > 0) {
+        p.tiles = (p.max_q + 32 * kWaves - 1) / (32 * kWaves);
+        hipLaunchKernelGGL((attn_dq_kernel<PK, D, kWaves>), dim3(static_cast<unsigned>(p.tiles) * p.nseq * p.H),
+                           dim3(64 * kWaves), 0, s, p);
         if ((e = hipGetLastError()) != hipSuccess) return e;
-        const int64_t HD = static_cast<int64_t>(p.H) * D;
-        if (p.Tq > 0) {
-            hipLaunchKernelGGL((norm_max_kernel<D>), dim3(kNormParts * p.B * p.H), dim3(256), 0, s,
-                               static_cast<const uint16_t *>(p.dout), p.Tq * HD, HD, static_cast<int64_t>(D), p.Tq,
-                               static_cast<const int64_t *>(nullptr), p.H, p.mx_do);
-            if ((e = hipGetLastError()) != hipSuccess) return e;
-        }
-        if (p.Tk > 0) {
-            hipLaunchKernelGGL((norm_max_kernel<D>), dim3(kNormParts * p.B * p.G), dim3(256), 0, s,
-                               static_cast<const uint16_t *>(p.v), p.vs[0], p.vs[1], p.vs[2], p.Tk, p.kv_len, p.G,
-                               p.mx_v);
-            if ((e = hipGetLastError()) != hipSuccess) return e;
-        }
     }
     if (p.Tk > 0) {
-        const int tiles = ((p.cu ? p.max_q : p.Tk) + 32 * NW - 1) / (32 * NW);
-        hipLaunchKernelGGL((attn_dkv_kernel<PK, D, NW>), dim3(static_cast<unsigned>(tiles) * p.nseq * p.G),
-                           dim3(64 * NW), 0, s, p);
+        // Query rows per tile: at D = 128 half of the other's, so that two
+        // workgroups' tiles and V rows fit a CU's LDS.
+        constexpr int BQ = D == 64 ? 64 : 32;
+        const int tiles = ((p.cu ? p.max_q : p.Tk) + 32 * kWaves - 1) / (32 * kWaves);
+        hipLaunchKernelGGL((attn_dkv_kernel<PK, D, kWaves, BQ>),
+                           dim3(static_cast<unsigned>(tiles) * p.nseq * p.G * p.splits), dim3(64 * kWaves), 0, s, p);
         if ((e = hipGetLastError()) != hipSuccess) return e;
-    }
-    if (p.Tq > 0) {
-        p.tiles = (p.max_q + 32 * NW - 1) / (32 * NW);
-        hipLaunchKernelGGL((attn_dq_kernel<PK, D, NW>), dim3(static_cast<unsigned>(p.tiles) * p.nseq * p.H),
-                           dim3(64 * NW), 0, s, p);
+        if (p.splits > 1) {
+            const int64_t threads = static_cast<int64_t>(p.B) * p.Tk * p.G * D / 2;
+            hipLaunchKernelGGL((attn_dkv_sum_kernel<PK>), dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256),
+                               0, s, p);
+        }
     }
     return hipGetLastError();
 }
@@ -721,10 +800,42 @@ bool attn_train_supported(int io_dtype, int D)
     return (io_dtype == GDN2_DTYPE_BF16 || io_dtype == GDN2_DTYPE_F16) && (D == 64 || D == 128);
 }
 
-size_t attn_bwd_workspace_bytes(int B, int Tq, int H, int G)
+// Shares of a key tile's queries in attn_dkv_kernel.  Two workgroups fit a CU: 512
+// fill the card, and causal ones, of unequal length, even out over two rounds with
+// the longest first.  Fewer are split, as long as a share keeps 16 query tiles of 64 (a
+// shorter one is over before its start and its sums' traffic are paid).  Backward in
+// us with 1 / 2 / 4 / 8 shares: B2 T8192 H16 G4 D128 causal (512 workgroups)
+// 2314 / 1812 / 1814 / 1913; packed 7013 tokens, H16 G4 D128 (240) 310 / 217 / 184 / 223;
+// B1 T4096 H16 G2 D64 (64) 795 / 456 / 288 / 213; B4 T2048 H16 D64 (1024)
+// 162 / 207 / 274 / 421; B8 T509 H8 D64, not causal (256, 8 tiles each) 53 / 59 / 63 / 80.
+int attn_bwd_splits(const AttnTrainParams &p)
 {
-    const size_t delta = (static_cast<size_t>(B) * H * Tq * sizeof(float) + 15) & ~static_cast<size_t>(15);
-    return delta + static_cast<size_t>(B) * (H + G) * sizeof(unsigned);
+    const int64_t wgs = p.k_tiles * p.G, want = p.causal ? 1024 : 512;
+    const int64_t steps = static_cast<int64_t>(p.H / p.G) * ((p.max_q + 63) / 64);
+    int64_t s = wgs > 0 ? (want + wgs / 2) / wgs : 1;
+    s = s < steps / 16 ? s : steps / 16;
+    return static_cast<int>(s < 1 ? 1 : (s > 16 ? 16 : s));
+}
+
+static size_t up16(size_t x) { return (x + 15) & ~static_cast<size_t>(15); }
+
+// D per query, fp16's norms, the shares' sums.
+size_t attn_bwd_workspace_bytes(const AttnTrainParams &p)
+{
+    const size_t part = p.splits > 1 ? static_cast<size_t>(p.splits) * 2 * p.B * p.Tk * p.G * p.D * sizeof(float) : 0;
+    return up16(static_cast<size_t>(p.B) * p.H * p.Tq * sizeof(float)) +
+           up16(static_cast<size_t>(p.B) * (p.H + p.G) * kNormParts * sizeof(float)) + part;
+}
+
+void attn_bwd_workspace(AttnTrainParams &p, void *workspace)
+{
+    char *w = static_cast<char *>(workspace);
+    p.delta = reinterpret_cast<float *>(w);
+    w += up16(static_cast<size_t>(p.B) * p.H * p.Tq * sizeof(float));
+    p.mx_do = reinterpret_cast<float *>(w);
+    p.mx_v = p.mx_do + static_cast<size_t>(p.B) * p.H * kNormParts;
+    w += up16(static_cast<size_t>(p.B) * (p.H + p.G) * kNormParts * sizeof(float));
+    p.part = reinterpret_cast<float *>(w);
 }
 
 hipError_t launch_attn_fwd(const AttnTrainParams &p, int io_dtype, hipStream_t s)

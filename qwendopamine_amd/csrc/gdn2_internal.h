@@ -317,18 +317,23 @@ struct AttnTrainParams {
     const void *dout;
     void *dq, *dk, *dv;
     float *delta;
-    unsigned *mx_do, *mx_v;  // fp16: squared row norm maxima [B][H], [B][G]
+    float *mx_do, *mx_v;     // fp16: squared row norm maxima [B][H][], [B][G][]
+    float *part;             // dk and dv of each share [splits][2][B, Tk, G, D], with more than one
+    int splits;              // shares of a key tile's queries (attn_bwd_splits)
     const int64_t *kv_len;   // [B] or NULL
     const int64_t *cu;       // [nseq + 1] or NULL
     int nseq;                // B without cu
     int max_q;               // longest sequence's queries
+    int64_t k_tiles;         // tiles of 128 keys over all sequences (one head)
     int tiles;               // set by the launcher
     int B, Tq, Tk, H, G, D;
     int causal;
     float scale;
 };
 bool attn_train_supported(int io_dtype, int D);
-size_t attn_bwd_workspace_bytes(int B, int Tq, int H, int G);
+int attn_bwd_splits(const AttnTrainParams &p);
+size_t attn_bwd_workspace_bytes(const AttnTrainParams &p);
+void attn_bwd_workspace(AttnTrainParams &p, void *workspace);
 hipError_t launch_attn_fwd(const AttnTrainParams &p, int io_dtype, hipStream_t stream);
 hipError_t launch_attn_bwd(const AttnTrainParams &p, int io_dtype, hipStream_t stream);
 

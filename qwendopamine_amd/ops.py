@@ -1574,7 +1574,8 @@ class AttentionFunction(torch.autograd.Function):
         strides = (ctypes.c_int64 * 9)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
         n = 0 if cu_host is None else cu_host.numel() - 1
         lib = nat.load()
-        ws = torch.empty(max(lib.gdn2_attn_bwd_workspace_size(B, Tq, H, G), 16), dtype=torch.uint8, device=q.device)
+        nbytes = lib.gdn2_attn_bwd_workspace_size(nat.ptr(cu_host), n, B, Tq, Tk, H, G, D, int(ctx.causal))
+        ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=q.device)
         with _on_device(q.device):
             st = lib.gdn2_attn_bwd(
                 nat.ptr(q), nat.ptr(k), nat.ptr(v), ctypes.addressof(strides), nat.ptr(o), nat.ptr(o_lo),

@@ -91,6 +91,23 @@ def test_attention_padded_rows(gpu_device, dt, D, causal):
     assert (got["o"][0] == 0).all() and (got["dq"][0] == 0).all() and (got["dk"][0] == 0).all()
 
 
+@pytest.mark.parametrize("D,dt", [(64, FP), (128, BF), (128, FP)])
+@pytest.mark.parametrize("rows", ["whole", "padded", "packed"])
+def test_attention_shares_of_many_heads(gpu_device, rows, D, dt):
+    """Eight query heads per group over few key tiles: dK and dV are summed in shares."""
+    print(f"[case] attention shares {rows} {dt} D{D}", flush=True)
+    T = 400
+    x = _inputs(gpu_device, 2 if rows == "padded" else 1, T, T, 8, 1, D, dt, seed=17)
+    if rows == "padded":
+        _check(_run(*x, causal=False, kv_lengths=torch.tensor([130, 400], device=gpu_device)), *x, causal=False,
+               kv_lengths=[130, 400])
+    elif rows == "packed":
+        cu = [0, 3, 70, 71, 400]
+        _check(_run(*x, cu_seqlens=torch.tensor(cu)), *x, cu=cu)
+    else:
+        _check(_run(*x), *x)
+
+
 def test_attention_lengths_are_clamped(gpu_device):
     x = _inputs(gpu_device, 2, 50, 50, 2, 2, 64, BF, seed=6)
     a = _run(*x, causal=False, kv_lengths=torch.tensor([-7, 10 ** 12], device=gpu_device))
