@@ -9,18 +9,23 @@
 // attention sees is scale * code + min.
 //
 // Codes enter the matrix products without being converted: a nibble n shifted into
-// the top of a 16-bit float's mantissa under the exponent of 1 is 1 + n / 16,
+// the top of a 16-bit float's mantissa under the exponent of 16 is 16 + n,
 // exact, two elements per shift and and-or.  The offsets leave through fp32 sums:
-//   q . k = sum_groups 16 scale (q . (1 + n/16) - sum q) + min sum q     (accumulators start at -sum q)
-//   o_d   = sum_j P'_j (1 + n_jd/16) + sum_j (p_j min_j - P'_j),  P'_j = 16 p_j scale_j
+//   q . k = sum_groups scale (q . (16 + n) - 16 sum q) + min sum q     (accumulators start at -16 sum q)
+//   o_d   = sum_j P'_j (16 + n_jd) + sum_j p_j min_j - 16 sum_j P'_j,  P'_j = p_j scale_j
 // P' is split into two bf16 numbers (16 significant bits) and both halves are
-// multiplied: one alone would leave an error of half a bf16 step of 1 + n/16,
+// multiplied: one alone would leave an error of half a bf16 step of 16 + n,
 // several times that of the values themselves.
 //
-// v_mfma_f32_16x16x32 throughout: a wave takes 32 positions a step, the group's
-// query heads are the 16 columns.  Scores come out with 4 positions of one
-// head per lane and tile, which is the B operand of the value product.  Bound
-// by the read of the codes: D / 2 + 4 D / 64 bytes per position, k and v each.
+// v_mfma_f32_16x16x32 throughout, positions as rows, query heads as the 16 columns:
+// scores come out with 4 positions of one head per lane and 16-position tile,
+// which is the B operand of the value product.  With few heads per group the
+// columns repeat them kSub = 16 / heads times, and column block u keeps only the
+// scores of tile u: the work per score (scales, exponential, splitting P') is then
+// done once and not kSub times over, and each column carries its own softmax
+// state (4 heads per group, D = 128: 427 -> 257 vector instructions per 32
+// positions).  Zeros in the other blocks keep a tile's P' to its columns.
+// Bound by the read of the codes: D / 2 + 4 D / 64 bytes per position, k and v each.
 #include "gdn2_common.h"
 #include "gdn2_internal.h"
 #include "gdn2_mfma.h"
@@ -29,7 +34,7 @@ namespace gdn2 {
 namespace {
 
 constexpr int kQ4Waves = 4;
-constexpr int kStep = 32;  // positions per wave and step
+constexpr int kQ4MaxSplits = 256;
 constexpr float kNoMax = -3.0e38f;
 constexpr float kLazy = 8.0f;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -38,29 +43,41 @@ struct __attribute__((aligned(4))) U4 {
     unsigned x[4];
 };
 
-// 8 codes of a word as A operand: register r holds nibbles r and r + 4, each as 1 + n / 16.
+// Mask and exponent of "nibble n -> 16 + n", kept in registers (one scalar, one
+// vector) so that v_and_or_b32 can take both: as literals they need two instructions.
+struct Magic {
+    unsigned mask, one;
+};
 template <PrecKind PK>
-__device__ __forceinline__ uint4 codes_frag(unsigned w)
+__device__ __forceinline__ Magic magic()
 {
-    if constexpr (PK == PrecKind::BF16) {
-        constexpr unsigned M = 0x00780078u, E = 0x3f803f80u;
-        return make_uint4(((w << 3) & M) | E, ((w >> 1) & M) | E, ((w >> 5) & M) | E, ((w >> 9) & M) | E);
-    } else {
-        constexpr unsigned M = 0x03c003c0u, E = 0x3c003c00u;
-        return make_uint4(((w << 6) & M) | E, ((w << 2) & M) | E, ((w >> 2) & M) | E, ((w >> 6) & M) | E);
-    }
+    Magic m = PK == PrecKind::BF16 ? Magic{0x00780078u, 0x41804180u} : Magic{0x03c003c0u, 0x4c004c00u};
+    asm volatile("" : "+s"(m.mask));
+    asm volatile("" : "+v"(m.one));
+    return m;
 }
 
-// Nibble c of both halves of a word (two positions, one channel) as two bf16 1 + n / 16.
-template <int C>
-__device__ __forceinline__ unsigned pair_frag(unsigned w)
+// 8 codes of a word as A operand: register r holds nibbles r and r + 4, each as 16 + n.
+template <PrecKind PK>
+__device__ __forceinline__ uint4 codes_frag(unsigned w, Magic m)
 {
-    constexpr unsigned M = 0x00780078u, E = 0x3f803f80u;
-    constexpr int s = 3 - 4 * C;
-    if constexpr (s >= 0)
-        return ((w << s) & M) | E;
+    if constexpr (PK == PrecKind::BF16)
+        return make_uint4(((w << 3) & m.mask) | m.one, ((w >> 1) & m.mask) | m.one, ((w >> 5) & m.mask) | m.one,
+                          ((w >> 9) & m.mask) | m.one);
     else
-        return ((w >> -s) & M) | E;
+        return make_uint4(((w << 6) & m.mask) | m.one, ((w << 2) & m.mask) | m.one, ((w >> 2) & m.mask) | m.one,
+                          ((w >> 6) & m.mask) | m.one);
+}
+
+// Nibble C of both halves of four words (two positions each, one channel) as bf16 16 + n.
+template <int C>
+__device__ __forceinline__ uint4 pair_frag(const unsigned (&w)[4], Magic m)
+{
+    constexpr int s = 3 - 4 * C;
+    unsigned r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = ((s >= 0 ? w[i] << (s >= 0 ? s : 0) : w[i] >> (s >= 0 ? 0 : -s)) & m.mask) | m.one;
+    return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
 template <PrecKind PK>
@@ -125,10 +142,34 @@ __device__ __forceinline__ unsigned code_of(float x, unsigned meta, float inv)
     return n >= 15.0f ? 15u : (n > 0.0f ? static_cast<unsigned>(n) : 0u);  // NaN: 0
 }
 
-template <typename T, PrecKind PK, int D>
-__global__ __launch_bounds__(64 * kQ4Waves) void attn_q4_kernel(AttnQ4Params p)
+// Positions per workgroup: whole rounds of its waves, the longest sequence over p.splits.
+__device__ __forceinline__ int q4_share(const AttnQ4Params &p, int len, int lane)
 {
-    constexpr int NG = D / 64, RB = D / 2;  // groups, bytes of a row of codes
+    int longest = len;
+    if (p.splits > 1 && p.pos_stride != 0) {
+        for (int b = lane; b < p.B; b += 64) {
+            const int64_t x = p.pos[p.pos_stride * b];
+            if (x >= 0 && x < p.max_len) longest = longest > x + 1 ? longest : static_cast<int>(x) + 1;
+        }
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_xor(longest, o, 64);
+            longest = longest > y ? longest : y;
+        }
+    }
+    const int rounds = (longest + p.round - 1) / p.round;
+    return (rounds + p.splits - 1) / p.splits * p.round;
+}
+
+// kSub column blocks (1, 2 or 4).
+template <typename T, PrecKind PK, int D, int kSub>
+__global__ __launch_bounds__(64 * kQ4Waves, 2) void attn_q4_kernel(AttnQ4Params p)
+{
+    constexpr int NG = D / 64, RB = D / 2;           // groups, bytes of a row of codes
+    constexpr int kTiles = kSub < 2 ? 2 : kSub;      // 16-position tiles per step
+    constexpr int kStep = 16 * kTiles, kRound = kStep * kQ4Waves;
+    constexpr int kOwn = kTiles / kSub;              // tiles whose scores a lane keeps
+    constexpr int kHeads = 16 / kSub;                // heads per column block
     __shared__ __align__(16) float s_o[kQ4Waves][16][D];
     __shared__ float s_m[kQ4Waves][16], s_l[kQ4Waves][16];
     __shared__ __align__(16) uint16_t s_q[16][D];
@@ -141,23 +182,16 @@ __global__ __launch_bounds__(64 * kQ4Waves) void attn_q4_kernel(AttnQ4Params p)
     float *part = p.part + (static_cast<int64_t>(bg) * p.splits + blockIdx.y) * qpk * (D + 2);
     const bool inside = pos >= 0 && pos < p.max_len;
     const int len = inside ? static_cast<int>(pos) + 1 : 0;
-    // This workgroup's positions: whole steps of its waves.
-    constexpr int kRound = kStep * kQ4Waves;
-    const int rounds = (len + kRound - 1) / kRound;
-    const int per = (rounds + p.splits - 1) / p.splits * kRound;
+    // This workgroup's positions: share blockIdx.y of those of the longest
+    // sequence, so that all workgroups that have any have equally many.
+    const int per = q4_share(p, len, lane);
+    const int sub = n / kHeads;  // this column's block
     const int lo = static_cast<int>(blockIdx.y) * per;
     const int hi = lo + per < len ? lo + per : len;
     if (lo >= hi) {
-        // Nothing here: an empty partial state, or (outside the caches) zeros.
-        for (int e = tid; e < qpk * D; e += 64 * kQ4Waves) {
-            if (p.splits == 1) {
-                io<T>::st(out, e, 0.0f);
-            } else {
-                const int h = e / D, d = e - h * D;
-                part[h * (D + 2) + d] = 0.0f;
-                if (d < 2) part[h * (D + 2) + D + d] = d == 0 ? kNoMax : 0.0f;
-            }
-        }
+        // Nothing here (the merge does not read this share); outside the caches: zeros.
+        if (p.splits == 1)
+            for (int e = tid; e < qpk * D; e += 64 * kQ4Waves) io<T>::st(out, e, 0.0f);
         return;
     }
     const T *x = static_cast<const T *>(p.qkv) + static_cast<int64_t>(bg) * (qpk + 2) * D;
@@ -165,6 +199,85 @@ __global__ __launch_bounds__(64 * kQ4Waves) void attn_q4_kernel(AttnQ4Params p)
     uint8_t *kc = p.k_codes + row0 * RB, *vc = p.v_codes + row0 * RB;
     unsigned *km = p.k_meta + row0 * NG, *vm = p.v_meta + row0 * NG;
     const float *cs = p.cos + p.rope_stride * pos, *sn = p.sin + p.rope_stride * pos;
+
+    // ---- a step's requests: codes and (scale, minimum) of 32 positions ----
+    struct Step {
+        uint2 k[kTiles][NG];
+        unsigned v[4 * kTiles][NG], mk[kOwn][4 * NG], mv[kOwn][4 * NG];
+    };
+    const int64_t row = lo + wave * kStep;
+    const uint8_t *kp = kc + (row + n) * RB + 8 * kg;
+    const uint8_t *vp = vc + (row + 4 * kg) * RB + 2 * n;
+    const unsigned *kmp = km + (row + 16 * kOwn * sub + 4 * kg) * NG;
+    const unsigned *vmp = vm + (row + 16 * kOwn * sub + 4 * kg) * NG;
+    // The step at the pointers, which then move to the wave's next.
+    auto request = [&](Step &st) __attribute__((always_inline)) {
+#pragma unroll
+        for (int a = 0; a < kTiles; ++a)
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                st.k[a][g] = *reinterpret_cast<const uint2 *>(kp + 16 * a * RB + 32 * g);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    st.v[4 * a + i][g] = *reinterpret_cast<const uint16_t *>(vp + (16 * a + i) * RB + 32 * g);
+            }
+#pragma unroll
+        for (int a = 0; a < kOwn; ++a)
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                const U4 uk = *reinterpret_cast<const U4 *>(kmp + 16 * a * NG + 4 * g);
+                const U4 uv = *reinterpret_cast<const U4 *>(vmp + 16 * a * NG + 4 * g);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    st.mk[a][4 * g + i] = uk.x[i];
+                    st.mv[a][4 * g + i] = uv.x[i];
+                }
+            }
+        kp += kRound * RB;
+        vp += kRound * RB;
+        kmp += kRound * NG;
+        vmp += kRound * NG;
+    };
+    // A last step of fewer positions, from j0: those past the end read the last
+    // one, and their values count for nothing whatever lies there.
+    auto request_part = [&](Step &st, int j0) {
+#pragma unroll
+        for (int a = 0; a < kTiles; ++a) {
+            int j = j0 + 16 * a + n;
+            j = j < hi ? j : hi - 1;
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+                st.k[a][g] = *reinterpret_cast<const uint2 *>(kc + static_cast<int64_t>(j) * RB + 32 * g + 8 * kg);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                int jv = j0 + 16 * a + 4 * kg + i;
+                jv = jv < hi ? jv : hi - 1;
+#pragma unroll
+                for (int g = 0; g < NG; ++g)
+                    st.v[4 * a + i][g] =
+                        *reinterpret_cast<const uint16_t *>(vc + static_cast<int64_t>(jv) * RB + 32 * g + 2 * n);
+            }
+        }
+#pragma unroll
+        for (int a = 0; a < kOwn; ++a)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int jm = j0 + 16 * (kOwn * sub + a) + 4 * kg + i;
+                const bool in = jm < hi;
+                const int64_t at = in ? jm : hi - 1;
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    st.mk[a][i * NG + g] = km[at * NG + g];
+                    st.mv[a][i * NG + g] = in ? vm[at * NG + g] : 0u;
+                }
+            }
+    };
+    const int jw = lo + wave * kStep;                                       // the wave's first position
+    const int whole = hi - jw >= kStep ? (hi - jw - kStep) / kRound + 1 : 0;  // its whole steps
+    Step cur;
+    // The first step is requested before the token is worked on, unless the token is in it.
+    const bool early = whole > 0 && jw + kStep < len;
+    if (early) request(cur);
 
     // ---- the token: q rotated into LDS; the workgroup that holds its position
     // rotates k, turns k and v into codes and stores them ----
@@ -214,13 +327,13 @@ __global__ __launch_bounds__(64 * kQ4Waves) void attn_q4_kernel(AttnQ4Params p)
 
     // ---- q as B operand: MFMA (g, w) takes channels 64 g + 16 kg + 8 w + {0, 4, 1, 5, 2, 6, 3, 7} ----
     uint4 qf[NG][2];
-    float qs[NG];
+    float qs[NG], q16[NG];
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
         float sum = 0.0f;
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-            const uint16_t *s = &s_q[n][64 * g + 16 * kg + 8 * w];
+            const uint16_t *s = &s_q[n % kHeads][64 * g + 16 * kg + 8 * w];
             unsigned r[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -230,86 +343,58 @@ __global__ __launch_bounds__(64 * kQ4Waves) void attn_q4_kernel(AttnQ4Params p)
             qf[g][w] = make_uint4(r[0], r[1], r[2], r[3]);
         }
         qs[g] = rows_sum(sum);
+        q16[g] = -16.0f * qs[g];
     }
     const float c = p.scale * kLog2e;
+    const Magic mg_k = magic<PK>(), mg_v = magic<PrecKind::BF16>();
 
-    float m = kNoMax, l = 0.0f, corr[NG];
+    float m = kNoMax, l = 0.0f, cm[NG], cp[NG];  // sums of p, of p min and of P'
     f32x4 acc[NG][4];
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-        corr[g] = 0.0f;
+        cm[g] = cp[g] = 0.0f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[g][i] = zero4();
     }
-    for (int j0 = lo + wave * kStep; j0 < hi; j0 += kRound) {
-        // Requests of the step.  Positions past the end read the last one.
-        uint2 kw[2][NG];
-        unsigned vw[8][NG], mk[2][4 * NG], mv[2][4 * NG];
-        const bool full = j0 + kStep <= hi;
+    // ---- one step; PART: the last one, of which positions from hi on are hidden ----
+    auto step = [&](const Step &st, int j0, auto part_c) __attribute__((always_inline)) {
+        constexpr bool PART = decltype(part_c)::value;
+        // Scores: 4 per tile that the lane keeps, positions j0 + 16 tile + 4 kg + i.
+        float s[4 * kOwn];
 #pragma unroll
-        for (int a = 0; a < 2; ++a) {
-            int j = j0 + 16 * a + n;
-            j = j < hi ? j : hi - 1;
+        for (int i = 0; i < 4 * kOwn; ++i) s[i] = 0.0f;
 #pragma unroll
-            for (int g = 0; g < NG; ++g)
-                kw[a][g] = *reinterpret_cast<const uint2 *>(kc + static_cast<int64_t>(j) * RB + 32 * g + 8 * kg);
-            const int jm = j0 + 16 * a + 4 * kg;
-            if (full) {
+        for (int g = 0; g < NG; ++g) {
+            f32x4 t[kTiles];
 #pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    const U4 uk = *reinterpret_cast<const U4 *>(km + static_cast<int64_t>(jm) * NG + 4 * g);
-                    const U4 uv = *reinterpret_cast<const U4 *>(vm + static_cast<int64_t>(jm) * NG + 4 * g);
+            for (int a = 0; a < kTiles; ++a) {
+                t[a] = f32x4{q16[g], q16[g], q16[g], q16[g]};
+                t[a] = mma16<PK>(t[a], codes_frag<PK>(st.k[a][g].x, mg_k), qf[g][0]);
+                t[a] = mma16<PK>(t[a], codes_frag<PK>(st.k[a][g].y, mg_k), qf[g][1]);
+            }
+            if constexpr (kSub > 1) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        mk[a][4 * g + i] = uk.x[i];
-                        mv[a][4 * g + i] = uv.x[i];
-                    }
-                }
-            } else {
+                for (int a = 1; a < kTiles; ++a)
 #pragma unroll
-                for (int i = 0; i < 4 * NG; ++i) {
-                    const bool in = jm + i / NG < hi;
-                    const int64_t at = static_cast<int64_t>(in ? jm + i / NG : hi - 1) * NG + i % NG;
-                    mk[a][i] = km[at];
-                    mv[a][i] = in ? vm[at] : 0u;  // hidden: P' and p min are 0 whatever lies there
-                }
+                    for (int i = 0; i < 4; ++i) t[0][i] = sub == a ? t[a][i] : t[0][i];
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                int jv = jm + i;
-                jv = jv < hi ? jv : hi - 1;
-#pragma unroll
-                for (int g = 0; g < NG; ++g)
-                    vw[4 * a + i][g] = *reinterpret_cast<const uint16_t *>(vc + static_cast<int64_t>(jv) * RB + 32 * g + 2 * n);
-            }
-        }
-        // Scores: 8 per lane, position j0 + 16 a + 4 kg + i of head n.
-        float s[8];
-#pragma unroll
-        for (int a = 0; a < 2; ++a) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[4 * a + i] = 0.0f;
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                f32x4 t = {-qs[g], -qs[g], -qs[g], -qs[g]};
-                t = mma16<PK>(t, codes_frag<PK>(kw[a][g].x), qf[g][0]);
-                t = mma16<PK>(t, codes_frag<PK>(kw[a][g].y), qf[g][1]);
+            for (int a = 0; a < kOwn; ++a)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const unsigned u = mk[a][i * NG + g];
-                    const float sc16 = 16.0f * __uint_as_float(u << 16), mn = __uint_as_float(u & 0xffff0000u);
-                    s[4 * a + i] = fmaf(sc16, t[i], fmaf(mn, qs[g], s[4 * a + i]));
+                    const unsigned u = st.mk[a][i * NG + g];
+                    const float sc = __uint_as_float(u << 16), mn = __uint_as_float(u & 0xffff0000u);
+                    s[4 * a + i] = fmaf(sc, t[a][i], fmaf(mn, qs[g], s[4 * a + i]));
                 }
-            }
         }
-        if (!full) {
+        if constexpr (PART) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                s[i] = j0 + 16 * (i >> 2) + 4 * kg + (i & 3) < hi ? s[i] : -INFINITY;
+            for (int i = 0; i < 4 * kOwn; ++i)
+                s[i] = j0 + 16 * (kOwn * sub + (i >> 2)) + 4 * kg + (i & 3) < hi ? s[i] : -INFINITY;
         }
         float mx = s[0];
 #pragma unroll
-        for (int i = 1; i < 8; ++i) mx = fmaxf(mx, s[i]);
+        for (int i = 1; i < 4 * kOwn; ++i) mx = fmaxf(mx, s[i]);
         mx = rows_max(mx) * c;
         if (__any(mx > m + kLazy)) {
             const float mn = fmaxf(m, mx);
@@ -318,60 +403,87 @@ __global__ __launch_bounds__(64 * kQ4Waves) void attn_q4_kernel(AttnQ4Params p)
             l *= r;
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                corr[g] *= r;
+                cm[g] *= r;
+                cp[g] *= r;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[g][i] *= r;
             }
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 4 * kOwn; ++i) {
             s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -m));
             l += s[i];
         }
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-            float ph[8], pl[8];
+            unsigned ph[2 * kOwn], pl[2 * kOwn];  // both halves of P', two positions per register
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const unsigned u = mv[i >> 2][(i & 3) * NG + g];
-                const float t = s[i] * (16.0f * __uint_as_float(u << 16));
-                corr[g] += fmaf(s[i], __uint_as_float(u & 0xffff0000u), -t);
-                ph[i] = t;
+            for (int i = 0; i < 2 * kOwn; ++i) {
+                float t[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int x = 2 * i + e;
+                    const unsigned u = st.mv[x >> 2][(x & 3) * NG + g];
+                    t[e] = s[x] * __uint_as_float(u << 16);
+                    cp[g] += t[e];
+                    cm[g] = fmaf(s[x], __uint_as_float(u & 0xffff0000u), cm[g]);
+                }
+                ph[i] = f32x2_to_bf16x2_bits(t[0], t[1]);
+                pl[i] = f32x2_to_bf16x2_bits(t[0] - __uint_as_float(ph[i] << 16),
+                                             t[1] - __uint_as_float(ph[i] & 0xffff0000u));
             }
-            uint4 bh, bl;
-            unsigned *h4 = &bh.x, *l4 = &bl.x;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                h4[i] = f32x2_to_bf16x2_bits(ph[2 * i], ph[2 * i + 1]);
-                pl[2 * i] = ph[2 * i] - __uint_as_float(h4[i] << 16);
-                pl[2 * i + 1] = ph[2 * i + 1] - __uint_as_float(h4[i] & 0xffff0000u);
-                l4[i] = f32x2_to_bf16x2_bits(pl[2 * i], pl[2 * i + 1]);
+            for (int cc = 0; cc < kTiles / 2; ++cc) {  // 32 positions: tiles 2 cc and 2 cc + 1
+                uint4 bh, bl;
+                if constexpr (kSub == 1) {
+                    bh = make_uint4(ph[0], ph[1], ph[2], ph[3]);
+                    bl = make_uint4(pl[0], pl[1], pl[2], pl[3]);
+                } else {
+                    const bool e0 = sub == 2 * cc, e1 = sub == 2 * cc + 1;
+                    bh = make_uint4(e0 ? ph[0] : 0u, e0 ? ph[1] : 0u, e1 ? ph[0] : 0u, e1 ? ph[1] : 0u);
+                    bl = make_uint4(e0 ? pl[0] : 0u, e0 ? pl[1] : 0u, e1 ? pl[0] : 0u, e1 ? pl[1] : 0u);
+                }
+                unsigned vp2[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    vp2[i] = st.v[8 * cc + 2 * i][g] | (st.v[8 * cc + 2 * i + 1][g] << 16);
+                const uint4 a0 = pair_frag<0>(vp2, mg_v), a1 = pair_frag<1>(vp2, mg_v);
+                const uint4 a2 = pair_frag<2>(vp2, mg_v), a3 = pair_frag<3>(vp2, mg_v);
+                acc[g][0] = mma16<PrecKind::BF16>(mma16<PrecKind::BF16>(acc[g][0], a0, bh), a0, bl);
+                acc[g][1] = mma16<PrecKind::BF16>(mma16<PrecKind::BF16>(acc[g][1], a1, bh), a1, bl);
+                acc[g][2] = mma16<PrecKind::BF16>(mma16<PrecKind::BF16>(acc[g][2], a2, bh), a2, bl);
+                acc[g][3] = mma16<PrecKind::BF16>(mma16<PrecKind::BF16>(acc[g][3], a3, bh), a3, bl);
             }
-            unsigned vp[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) vp[i] = vw[2 * i][g] | (vw[2 * i + 1][g] << 16);
-            const uint4 a0 = make_uint4(pair_frag<0>(vp[0]), pair_frag<0>(vp[1]), pair_frag<0>(vp[2]), pair_frag<0>(vp[3]));
-            const uint4 a1 = make_uint4(pair_frag<1>(vp[0]), pair_frag<1>(vp[1]), pair_frag<1>(vp[2]), pair_frag<1>(vp[3]));
-            const uint4 a2 = make_uint4(pair_frag<2>(vp[0]), pair_frag<2>(vp[1]), pair_frag<2>(vp[2]), pair_frag<2>(vp[3]));
-            const uint4 a3 = make_uint4(pair_frag<3>(vp[0]), pair_frag<3>(vp[1]), pair_frag<3>(vp[2]), pair_frag<3>(vp[3]));
-            acc[g][0] = mma16<PrecKind::BF16>(mma16<PrecKind::BF16>(acc[g][0], a0, bh), a0, bl);
-            acc[g][1] = mma16<PrecKind::BF16>(mma16<PrecKind::BF16>(acc[g][1], a1, bh), a1, bl);
-            acc[g][2] = mma16<PrecKind::BF16>(mma16<PrecKind::BF16>(acc[g][2], a2, bh), a2, bl);
-            acc[g][3] = mma16<PrecKind::BF16>(mma16<PrecKind::BF16>(acc[g][3], a3, bh), a3, bl);
         }
+    };
+    // Two register sets in turn: the next step's requests are in flight during this one.
+    if (!early && whole > 0) request(cur);
+    Step alt;
+    int it = 0;
+    for (; it + 2 <= whole; it += 2) {
+        request(alt);
+        step(cur, 0, std::false_type{});
+        if (it + 2 < whole) request(cur);
+        step(alt, 0, std::false_type{});
+    }
+    if (it < whole) step(cur, 0, std::false_type{});
+    const int j_end = jw + whole * kRound;
+    if (j_end < hi) {
+        request_part(cur, j_end);
+        step(cur, j_end, std::true_type{});
     }
     // ---- the waves' states meet in LDS ----
     l = rows_sum(l);
 #pragma unroll
-    for (int g = 0; g < NG; ++g) corr[g] = rows_sum(corr[g]);
-    if (n < qpk) {
+    for (int g = 0; g < NG; ++g) cm[g] = rows_sum(fmaf(-16.0f, cp[g], cm[g]));
+    if (n % kHeads < qpk) {
 #pragma unroll
         for (int g = 0; g < NG; ++g)
 #pragma unroll
             for (int i = 0; i < 4; ++i)  // row 4 kg + i of product cc is channel 64 g + 4 (4 kg + i) + cc
                 *reinterpret_cast<float4 *>(&s_o[wave][n][64 * g + 16 * kg + 4 * i]) =
-                    make_float4(acc[g][0][i] + corr[g], acc[g][1][i] + corr[g], acc[g][2][i] + corr[g],
-                                acc[g][3][i] + corr[g]);
+                    make_float4(acc[g][0][i] + cm[g], acc[g][1][i] + cm[g], acc[g][2][i] + cm[g],
+                                acc[g][3][i] + cm[g]);
         if (kg == 0) {
             s_m[wave][n] = m;
             s_l[wave][n] = l;
@@ -382,13 +494,14 @@ __global__ __launch_bounds__(64 * kQ4Waves) void attn_q4_kernel(AttnQ4Params p)
         const int h = e / D, d = e - h * D;
         float mx = kNoMax;
 #pragma unroll
-        for (int w = 0; w < kQ4Waves; ++w) mx = fmaxf(mx, s_m[w][h]);
+        for (int w = 0; w < kQ4Waves * kSub; ++w) mx = fmaxf(mx, s_m[w / kSub][w % kSub * kHeads + h]);
         float num = 0.0f, den = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kQ4Waves; ++w) {
-            const float r = __builtin_amdgcn_exp2f(s_m[w][h] - mx);
-            num = fmaf(s_o[w][h][d], r, num);
-            den = fmaf(s_l[w][h], r, den);
+        for (int w = 0; w < kQ4Waves * kSub; ++w) {
+            const int col = w % kSub * kHeads + h;
+            const float r = __builtin_amdgcn_exp2f(s_m[w / kSub][col] - mx);
+            num = fmaf(s_o[w / kSub][col][d], r, num);
+            den = fmaf(s_l[w / kSub][col], r, den);
         }
         if (p.splits == 1) {
             io<T>::st(out, e, num / den);
@@ -402,22 +515,45 @@ __global__ __launch_bounds__(64 * kQ4Waves) void attn_q4_kernel(AttnQ4Params p)
     }
 }
 
-// The splits' partial states of one (sequence, head) per workgroup of D threads.
+// The shares' partial states of one (sequence, head) per workgroup: weights first
+// (a thread each), then the values, 256 / D threads per channel.
 template <typename T, int D>
-__global__ __launch_bounds__(D) void attn_q4_merge_kernel(AttnQ4Params p)
+__global__ __launch_bounds__(256) void attn_q4_merge_kernel(AttnQ4Params p)
 {
-    const int d = threadIdx.x, h = static_cast<int>(blockIdx.x % p.qpk);
+    constexpr int N = 256 / D;
+    __shared__ float s_w[kQ4MaxSplits], s_red[4], s_den[4], s_num[N][D];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int h = static_cast<int>(blockIdx.x % p.qpk);
     const int64_t bg = blockIdx.x / p.qpk;
+    const int64_t pos = p.pos[p.pos_stride * (bg / p.G)];
+    const int len = pos >= 0 && pos < p.max_len ? static_cast<int>(pos) + 1 : 0;
+    const int per = q4_share(p, len, lane);
+    const int used = len > 0 ? (len + per - 1) / per : 0;  // shares that hold anything
     const float *part = p.part + (bg * p.splits * p.qpk + h) * (D + 2);
     const int64_t stride = static_cast<int64_t>(p.qpk) * (D + 2);
-    float mx = kNoMax;
-    for (int s = 0; s < p.splits; ++s) mx = fmaxf(mx, part[s * stride + D]);
-    float num = 0.0f, den = 0.0f;
-    for (int s = 0; s < p.splits; ++s) {
-        const float r = __builtin_amdgcn_exp2f(part[s * stride + D] - mx);
-        num = fmaf(part[s * stride + d], r, num);
-        den = fmaf(part[s * stride + D + 1], r, den);
-    }
+    const float mx = tid < used ? part[tid * stride + D] : kNoMax;
+    float den = tid < used ? part[tid * stride + D + 1] : 0.0f;
+    float m = mx;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    if (lane == 0) s_red[wave] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+    const float w = __builtin_amdgcn_exp2f(mx - m);
+    s_w[tid] = w;
+    den = wave_sum(den * w);
+    if (lane == 0) s_den[wave] = den;
+    __syncthreads();
+    const int d = tid % D, g = tid / D;
+    float num = 0.0f;
+#pragma unroll 8
+    for (int s = g; s < used; s += N) num = fmaf(part[s * stride + d], s_w[s], num);
+    s_num[g][d] = num;
+    __syncthreads();
+    if (tid >= D) return;
+    den = (s_den[0] + s_den[1]) + (s_den[2] + s_den[3]);
+#pragma unroll
+    for (int i = 1; i < N; ++i) num += s_num[i][d];
     // No position at all (outside the caches): zeros.
     io<T>::st(static_cast<T *>(p.out), static_cast<int64_t>(blockIdx.x) * D + d, den == 0.0f ? 0.0f : num / den);
 }
@@ -526,25 +662,41 @@ __global__ __launch_bounds__(256) void q4_load_kernel(Q4LoadParams p)
 }
 
 template <typename T, PrecKind PK, int D>
-hipError_t decode_d(const AttnQ4Params &p, hipStream_t s)
+hipError_t decode_d(AttnQ4Params p, hipStream_t s)
 {
-    hipLaunchKernelGGL((attn_q4_kernel<T, PK, D>), dim3(static_cast<unsigned>(p.B * p.G), p.splits),
-                       dim3(64 * kQ4Waves), 0, s, p);
+    const dim3 grid(static_cast<unsigned>(p.B * p.G), p.splits), block(64 * kQ4Waves);
+    p.round = (p.qpk <= 4 ? 64 : 32) * kQ4Waves;
+    if (p.qpk <= 4)
+        hipLaunchKernelGGL((attn_q4_kernel<T, PK, D, 4>), grid, block, 0, s, p);
+    else if (p.qpk <= 8)
+        hipLaunchKernelGGL((attn_q4_kernel<T, PK, D, 2>), grid, block, 0, s, p);
+    else
+        hipLaunchKernelGGL((attn_q4_kernel<T, PK, D, 1>), grid, block, 0, s, p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits == 1) return e;
-    hipLaunchKernelGGL((attn_q4_merge_kernel<T, D>), dim3(static_cast<unsigned>(p.B * p.G * p.qpk)), dim3(D), 0, s, p);
+    hipLaunchKernelGGL((attn_q4_merge_kernel<T, D>), dim3(static_cast<unsigned>(p.B * p.G * p.qpk)), dim3(256), 0, s,
+                       p);
     return hipGetLastError();
 }
 
 }  // namespace
 
+// Workgroups per (sequence, KV group): 512 in all (two per CU), more where a share
+// would exceed 4096 positions of a full cache, so that sequences of unequal lengths
+// even out; but shares of 512 positions or more, of 1024 where the sequences alone
+// occupy half the card (a merge costs about 4 us).  us a call with 256 / 512 / 1024 /
+// 2048 / 4096 workgroups wanted: 32 sequences of up to 32768, 8 groups of 4 heads, D128
+// 198 / 171 / 156 / 137 / 146; 8 x 7373 positions, 16 groups, D64 21.4 / 20.2 / 22.0 / 25.0 / 24.8;
+// 64 x 922 positions, 4 groups of 4, D128 13.2 / 18.8 / 18.6 / 18.6 / 18.7.
 int attn_q4_splits(int B, int G, int64_t max_len)
 {
-    // Enough workgroups for every CU, of at least two rounds of their waves.
-    const int64_t most = (max_len + 2 * kStep * kQ4Waves - 1) / (2 * kStep * kQ4Waves);
-    int64_t s = (1024 + static_cast<int64_t>(B) * G - 1) / (static_cast<int64_t>(B) * G);
+    const int64_t bg = static_cast<int64_t>(B) * G;
+    const int64_t least = bg < 128 ? 512 : 1024, most = (max_len + least - 1) / least;
+    int64_t s = (512 + bg - 1) / bg;
+    const int64_t by_share = (max_len + 4095) / 4096;
+    s = s > by_share ? s : by_share;
     s = s < most ? s : most;
-    return static_cast<int>(s < 1 ? 1 : (s > 256 ? 256 : s));
+    return static_cast<int>(s < 1 ? 1 : (s > kQ4MaxSplits ? kQ4MaxSplits : s));
 }
 
 size_t attn_q4_workspace_floats(int B, int G, int qpk, int D, int64_t max_len)

@@ -379,6 +379,7 @@ struct AttnQ4Params {
     int B, G, qpk, D;
     float scale;
     int splits;   // workgroups per (sequence, KV group)
+    int round;    // positions that a workgroup's waves take at a time (set by the launcher)
     float *part;  // attn_q4_workspace_floats, with more than one
 };
 bool attn_q4_supported(int io_dtype, int qpk, int D);
