@@ -121,11 +121,14 @@ struct Top {
     u64 *list;
     int n, k;
     float last;   // with n >= k after keep_best: the k-th best value
+    bool sorted;  // nothing was appended since keep_best
 };
 
 // Keeps the k best of the list, in order.
 __device__ __forceinline__ void keep_best(Top &t, int lane)
 {
+    if (t.sorted) return;
+    t.sorted = true;
     wave_fence();
     u64 own[kCand / 64];
     int rank[kCand / 64];
@@ -160,21 +163,21 @@ __device__ __forceinline__ void push(Top &t, bool have, u64 key, int lane)
     if (t.n + 64 > kCand) keep_best(t, lane);
     if (have) t.list[t.n + __popcll(mask & ((1ull << lane) - 1))] = key;
     t.n += __popcll(mask);
+    t.sorted = false;
 }
 
-// The k-th largest of the lanes' values (NaN as the largest).
-__device__ __forceinline__ float kth_of_lanes(float v, int k)
+// A lower bound of the k-th largest of the lanes' ordered values (key_of's high
+// word), its upper 16 bits found bit by bit by counting lanes: a filter, which may let a
+// few more elements through than the exact value would.
+__device__ __forceinline__ unsigned kth_bound(unsigned mine, int k)
 {
-    const unsigned mine = static_cast<unsigned>(key_of(v, 0) >> 32);
-    const int lane = threadIdx.x & 63;
-    int rank = 0;
-#pragma unroll 8
-    for (int j = 0; j < 64; ++j) {
-        const unsigned x = __builtin_amdgcn_readlane(mine, j);
-        rank += x > mine || (x == mine && j < lane);
+    unsigned t = 0;
+#pragma unroll
+    for (int bit = 31; bit >= 16; --bit) {
+        const unsigned trial = t | (1u << bit);
+        if (__popcll(__ballot(mine >= trial)) >= k) t = trial;
     }
-    const int src = __ffsll(__ballot(rank == k - 1)) - 1;
-    return __shfl(v, src, 64);
+    return t;
 }
 
 __device__ __forceinline__ int64_t row_offset(const LogprobParams &p, int64_t row)
@@ -235,7 +238,7 @@ __global__ __launch_bounds__(64) void logp_part_kernel(LogprobParams p)
     const int64_t c_hi = c_lo + p.pieces_per_part < pieces ? c_lo + p.pieces_per_part : pieces;
     const T *xa = x + head;  // 16-byte aligned
     Stat a = {-INFINITY, 0.0f, 0.0f};
-    Top top = {s_list, 0, p.top, -INFINITY};
+    Top top = {s_list, 0, p.top, -INFINITY, true};
     // The row's ragged ends, one element per lane: what precedes the first
     // piece belongs to the first part and comes first, what follows the last
     // piece to the last part and comes last (the lists below rely on it: later
@@ -252,83 +255,67 @@ __global__ __launch_bounds__(64) void logp_part_kernel(LogprobParams p)
     };
     if (part == 0 && head > 0) ragged(lane < head ? lane : -1);
     bool first = true;
-    for (int64_t c0 = c_lo; c0 < c_hi; c0 += 64 * kU) {
+    // One chunk from piece c0 on; FULL: all 64 kU pieces are there, else the
+    // missing ones are skipped (a lane's pieces by its own count, whole rows of 64 by branch).
+    auto chunk = [&](int64_t c0, auto full_c) __attribute__((always_inline)) {
+        constexpr bool FULL = decltype(full_c)::value;
         uint4 raw[kU];
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
             const int64_t c = c0 + 64 * u + lane;
-            raw[u] = *reinterpret_cast<const uint4 *>(xa + (c < c_hi ? c : c_hi - 1) * EPP);
+            if (FULL || c0 + 64 * u < c_hi) raw[u] = *reinterpret_cast<const uint4 *>(xa + (FULL || c < c_hi ? c : c_hi - 1) * EPP);
         }
-        const bool full = c0 + 64 * kU <= c_hi;
-        // Chunk maximum of this lane (NaN and repeated pieces do no harm in it).
-        float mx = -INFINITY;
+        // Runs f(element, its number in the chunk) over the lane's elements.
+        auto each = [&](auto f) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < kU; ++u) {
-            float f[EPP];
-            Piece<T>::widen(raw[u], f);
+            for (int u = 0; u < kU; ++u) {
+                if (!FULL && c0 + 64 * u >= c_hi) break;
+                float v[EPP];
+                Piece<T>::widen(raw[u], v);
+                if (FULL || c0 + 64 * u + lane < c_hi)
 #pragma unroll
-            for (int e = 0; e < EPP; ++e) mx = fmaxf(mx, f[e]);
-        }
+                    for (int e = 0; e < EPP; ++e) f(v[e], u * EPP + e);
+            }
+        };
+        float mx = -INFINITY;  // of this lane, NaN left out
+        bool nan = false;
+        each([&](float v, int) __attribute__((always_inline)) {
+            mx = fmaxf(mx, v);
+            if constexpr (TOP) nan |= v != v;
+        });
         // +inf stays out of the reference (its terms are NaN, as the formula's).
         rebase(a, fmaxf(a.m, mx < INFINITY ? mx : -INFINITY));
         if (a.m == -INFINITY) {
             // Nothing finite yet: -inf adds nothing, +inf and NaN make the row NaN.
-#pragma unroll
-            for (int u = 0; u < kU; ++u) {
-                float f[EPP];
-                Piece<T>::widen(raw[u], f);
-                if (full || c0 + 64 * u + lane < c_hi)
-#pragma unroll
-                    for (int e = 0; e < EPP; ++e)
-                        if (f[e] != -INFINITY) a.s = a.u = __uint_as_float(0x7fc00000u);
-            }
+            each([&](float v, int) __attribute__((always_inline)) {
+                if (v != -INFINITY) a.s = a.u = __uint_as_float(0x7fc00000u);
+            });
         } else {
             float s0 = 0.0f, u0 = 0.0f;
-#pragma unroll
-            for (int u = 0; u < kU; ++u) {
-                float f[EPP];
-                Piece<T>::widen(raw[u], f);
-                if (full || c0 + 64 * u + lane < c_hi) {
-#pragma unroll
-                    for (int e = 0; e < EPP; ++e) {
-                        const float t = (f[e] - a.m) * kL2e;
-                        const float ex = __builtin_amdgcn_exp2f(t);
-                        s0 += ex;
-                        u0 = fmaf(fmaxf(t, -1000.0f), ex, u0);  // t = -inf: 0, not inf * 0; t = NaN: ex is NaN
-                    }
-                }
-            }
+            each([&](float v, int) __attribute__((always_inline)) {
+                const float t = (v - a.m) * kL2e;
+                const float ex = __builtin_amdgcn_exp2f(t);
+                s0 += ex;
+                u0 = fmaf(fmaxf(t, -1000.0f), ex, u0);  // t = -inf: 0, not inf * 0; t = NaN: ex is NaN
+            });
             a.s += s0;
             a.u += u0;
         }
         if constexpr (TOP) {
             // Which of the chunk's elements may be among the k best: in the
-            // first chunk those that reach the k-th largest lane maximum,
-            // later those beyond the list's last (an equal one comes after it).
-            float lane_mx = -INFINITY;
-#pragma unroll
-            for (int u = 0; u < kU; ++u) {
-                float f[EPP];
-                Piece<T>::widen(raw[u], f);
-                if (full || c0 + 64 * u + lane < c_hi)
-#pragma unroll
-                    for (int e = 0; e < EPP; ++e) lane_mx = f[e] > lane_mx || f[e] != f[e] ? f[e] : lane_mx;
-            }
-            // (A NaN in lane_mx stays: nothing compares above it.)
-            const float thr = first ? kth_of_lanes(lane_mx, p.top) : top.last;
+            // first chunk those that reach (a bound of) the k-th largest lane
+            // maximum, later those beyond the list's last (an equal one comes after it).
+            const float lane_mx = nan ? __uint_as_float(0x7fc00000u) : mx;
+            float thr = top.last;
+            if (first)
+                thr = key_value(static_cast<u64>(kth_bound(static_cast<unsigned>(key_of(lane_mx, 0) >> 32), p.top)) << 32);
             const bool strict = !first;
             const bool any = strict ? !(lane_mx <= thr) : !(lane_mx < thr);
             if (__ballot(any)) {
                 u64 mask = 0;
-#pragma unroll
-                for (int u = 0; u < kU; ++u) {
-                    float f[EPP];
-                    Piece<T>::widen(raw[u], f);
-                    const bool in = full || c0 + 64 * u + lane < c_hi;
-#pragma unroll
-                    for (int e = 0; e < EPP; ++e)
-                        if (in && (strict ? !(f[e] <= thr) : !(f[e] < thr))) mask |= 1ull << (u * EPP + e);
-                }
+                each([&](float v, int i) __attribute__((always_inline)) {
+                    if (strict ? !(v <= thr) : !(v < thr)) mask |= 1ull << i;
+                });
                 if (!any) mask = 0;
                 while (__ballot(mask != 0)) {
                     const bool have = mask != 0;
@@ -344,7 +331,10 @@ __global__ __launch_bounds__(64) void logp_part_kernel(LogprobParams p)
             }
             first = top.n < p.top;
         }
-    }
+    };
+    int64_t c0 = c_lo;
+    for (; c0 + 64 * kU <= c_hi; c0 += 64 * kU) chunk(c0, std::true_type{});
+    if (c0 < c_hi) chunk(c0, std::false_type{});
     if (part == p.parts - 1 && tail0 < p.n) ragged(tail0 + lane < p.n ? tail0 + lane : -1);
     a = wave_merge(a);
     if constexpr (TOP) keep_best(top, lane);
@@ -372,7 +362,7 @@ __global__ __launch_bounds__(64) void logp_merge_kernel(LogprobParams p)
         a = merge(a, Stat{st.x, st.y, st.z});
     }
     a = wave_merge(a);
-    Top top = {s_list, 0, p.top, -INFINITY};
+    Top top = {s_list, 0, p.top, -INFINITY, true};
     if constexpr (TOP) {
         const u64 *src = p.part_top + row * p.parts * p.top;
         const int n = p.parts * p.top;
@@ -381,18 +371,7 @@ __global__ __launch_bounds__(64) void logp_merge_kernel(LogprobParams p)
             const u64 key = src[i];
             best = key > best ? key : best;
         }
-        // k-th largest of the lanes' largest, by counting whole keys.
-        int rank = 0;
-#pragma unroll 8
-        for (int j = 0; j < 64; ++j) {
-            const unsigned hi = __builtin_amdgcn_readlane(static_cast<unsigned>(best >> 32), j);
-            const unsigned lo = __builtin_amdgcn_readlane(static_cast<unsigned>(best), j);
-            const u64 x = (static_cast<u64>(hi) << 32) | lo;
-            rank += x > best || (x == best && j < lane);
-        }
-        const int src_lane = __ffsll(__ballot(rank == p.top - 1)) - 1;
-        const u64 thr = (static_cast<u64>(__shfl(static_cast<unsigned>(best >> 32), src_lane, 64)) << 32) |
-                        __shfl(static_cast<unsigned>(best), src_lane, 64);
+        const u64 thr = static_cast<u64>(kth_bound(static_cast<unsigned>(best >> 32), p.top)) << 32;
         for (int i0 = 0; i0 < n; i0 += 64) {
             const u64 key = i0 + lane < n ? src[i0 + lane] : 0;
             push(top, key != 0 && key >= thr, key, lane);
