@@ -347,10 +347,16 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(AttnTrainParams p)
             if (p.o_lo) {
                 // What the rounding left out, for D = dO . O: without it D is
                 // off by half a step of O, which shows in dS where few keys
-                // carry the weight and dP - D cancels.
+                // carry the weight and dP - D cancels.  What is below the sums'
+                // own error is left out: O of a single key is then exactly its V.
                 float z[4];
                 unpack4<PK>(r, z);
-                st_q4<PK>(ol + 32 * d + 8 * i + 4 * h, pack4<PK>(y[0] - z[0], y[1] - z[1], y[2] - z[2], y[3] - z[3]));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    z[e] = y[e] - z[e];
+                    z[e] = fabsf(z[e]) > 0x1p-18f * fabsf(y[e]) ? z[e] : 0.0f;
+                }
+                st_q4<PK>(ol + 32 * d + 8 * i + 4 * h, pack4<PK>(z[0], z[1], z[2], z[3]));
             }
         }
 }
@@ -455,21 +461,26 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dq_kernel(AttnTrainParams p)
         df[s] = *reinterpret_cast<const uint4 *>(dr + 16 * s + 8 * h);
     }
     const float sc = ds_scale<PK>(p, w);
+    // D = dO . O as the diagonal of a product of the same shape, operands and order as
+    // dP: where a query sees a single key, O is that key's V and D is dP to the
+    // bit, so that its dS is the formula's zero and not the difference of two sums.
     float dl = 0.0f;
+    {
+        f32x16 t = zero16(), tl = zero16();
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-        typename Prec<PK>::frag fd, fo, fl;
-        fd.u = df[s];
-        fo.u = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.o) + orow + 16 * s + 8 * h);
-        fl.u = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.o_lo) + orow + 16 * s + 8 * h);
-        float xd[8], xo[8], xl[8];
-        unpack_frag<PK>(fd, xd);
-        unpack_frag<PK>(fo, xo);
-        unpack_frag<PK>(fl, xl);
+        for (int s = 0; s < KS; ++s) {
+            const uint4 fo = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.o) + orow + 16 * s + 8 * h);
+            const uint4 fl = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.o_lo) + orow + 16 * s + 8 * h);
+            t = mma32<PK>(t, fo, df[s]);
+            tl = mma32<PK>(tl, fl, df[s]);
+        }
+        // Row n of column n: element 4 (n / 8) + n % 4 of half (n / 4) % 2.
+        const int at = (n >> 3) * 4 + (n & 3);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) dl = fmaf(xo[e] + xl[e], xd[e], dl);
+        for (int i = 0; i < 16; ++i) dl = at == i ? t[i] + tl[i] : dl;
+        dl = ((n >> 2) & 1) == h ? dl : 0.0f;
+        dl = half_add(dl);
     }
-    dl = half_add(dl);
     if (h == 0 && qi < w.nq) p.delta[srow] = dl;
     dl *= sc;
     const float lse = p.lse[srow];

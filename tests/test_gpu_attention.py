@@ -206,6 +206,17 @@ def test_attention_nonfinite_spreads_as_the_formula_says(gpu_device):
     assert torch.isfinite(o[0, :70, 1]).all()  # a hidden infinite key leaves the queries before it alone
 
 
+@pytest.mark.parametrize("D,dt", [(64, BF), (128, FP)])
+def test_attention_single_key_rows_have_no_score_gradient(gpu_device, D, dt):
+    """Where a query sees one key, P = 1 whatever the score: o is that key's v and dq exactly zero."""
+    x = _inputs(gpu_device, 3, 300, 300, 4, 2, D, dt, seed=18, mag=3.0)
+    got = _run(*x, causal=False, kv_lengths=torch.tensor([1, 1, 1], device=gpu_device))
+    assert torch.equal(got["o"], x[2][:, :1].repeat_interleave(2, 2).expand(3, 300, 4, D))
+    assert (got["dq"] == 0).all() and (got["dk"] == 0).all()
+    got = _run(*x)
+    assert (got["dq"][:, 0] == 0).all() and (got["dq"][:, 1] != 0).any()
+
+
 def test_attention_gradient_against_differences(gpu_device):
     """<gradient, d> against central differences of the float64 loss along random directions."""
     q, k, v, do = _inputs(gpu_device, 1, 45, 45, 2, 1, 64, FP, seed=15)
