@@ -1523,6 +1523,8 @@ def _on_device(device: torch.device):
 def _head_rows(x: torch.Tensor) -> torch.Tensor:
     """``x [B, T, heads, D]`` as the attention kernels read it: in place where its channels are
     contiguous and every row starts on 16 bytes, else a contiguous copy."""
+    if x.is_contiguous() and x.data_ptr() % 16 == 0:
+        return x
     per = 16 // x.element_size()
     if x.stride(3) == 1 and x.data_ptr() % 16 == 0 and all(
             x.stride(i) % per == 0 for i in range(3) if x.shape[i] > 1):
@@ -1536,6 +1538,28 @@ def attention_supported(q: torch.Tensor, head_dim: int) -> bool:
     return q.is_cuda and q.dtype in (torch.bfloat16, torch.float16) and head_dim in (64, 128)
 
 
+_I64x6, _I64x9 = ctypes.c_int64 * 6, ctypes.c_int64 * 9
+
+
+def _attention_fwd(q, k, v, scale: float, causal: bool, kv_len, cu_dev, cu_host, keep: bool):
+    """``(o, o_lo, lse)`` of readable q, k, v (:func:`_head_rows`); ``o_lo`` only with ``keep``."""
+    B, Tq, H, D = q.shape
+    Tk, G = k.shape[1], k.shape[2]
+    dev = q.device
+    o = torch.empty((B, Tq, H, D), dtype=q.dtype, device=dev)
+    o_lo = torch.empty_like(o) if keep else None
+    lse = torch.empty((B, H, Tq), dtype=torch.float32, device=dev)
+    strides = _I64x9(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
+    n = 0 if cu_host is None else cu_host.numel() - 1
+    with _on_device(dev):
+        st = nat.load().gdn2_attn_fwd(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), ctypes.addressof(strides), o.data_ptr(), nat.ptr(o_lo),
+            lse.data_ptr(), nat.dtype_code(q.dtype), nat.ptr(kv_len), nat.ptr(cu_dev), nat.ptr(cu_host), n, B, Tq, Tk, H,
+            G, D, scale, causal, nat.stream_handle(dev))
+    nat.check(st, "attention")
+    return o, o_lo, lse
+
+
 class AttentionFunction(torch.autograd.Function):
     """:func:`attention` with the HIP forward and backward (``gdn2_attn_fwd`` / ``gdn2_attn_bwd``):
     the output (with what its rounding left out) and the softmax's log sums are kept, the
@@ -1544,19 +1568,7 @@ class AttentionFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, scale: float, causal: bool, kv_len, cu_dev, cu_host):
         q, k, v = _head_rows(q), _head_rows(k), _head_rows(v)
-        B, Tq, H, D = q.shape
-        Tk, G = k.shape[1], k.shape[2]
-        o = torch.empty(B, Tq, H, D, dtype=q.dtype, device=q.device)
-        o_lo = torch.empty_like(o) if any(ctx.needs_input_grad) else None
-        lse = torch.empty(B, H, Tq, dtype=torch.float32, device=q.device)
-        strides = (ctypes.c_int64 * 9)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
-        n = 0 if cu_host is None else cu_host.numel() - 1
-        with _on_device(q.device):
-            st = nat.load().gdn2_attn_fwd(
-                nat.ptr(q), nat.ptr(k), nat.ptr(v), ctypes.addressof(strides), nat.ptr(o), nat.ptr(o_lo),
-                nat.ptr(lse), nat.dtype_code(q.dtype), nat.ptr(kv_len), nat.ptr(cu_dev), nat.ptr(cu_host), n, B, Tq, Tk, H, G, D,
-                scale, int(causal), nat.stream_handle(q.device))
-        nat.check(st, "attention")
+        o, o_lo, lse = _attention_fwd(q, k, v, scale, causal, kv_len, cu_dev, cu_host, any(ctx.needs_input_grad))
         ctx.save_for_backward(q, k, v, o, o_lo, lse, kv_len, cu_dev)
         ctx.scale, ctx.causal, ctx.cu_host = scale, causal, cu_host
         return o
@@ -1565,23 +1577,25 @@ class AttentionFunction(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, do):
         q, k, v, o, o_lo, lse, kv_len, cu_dev = ctx.saved_tensors
-        cu_host = ctx.cu_host
+        cu_host, causal = ctx.cu_host, ctx.causal
         B, Tq, H, D = q.shape
         Tk, G = k.shape[1], k.shape[2]
-        do = _io(do, q.dtype)
-        dq = torch.empty(B, Tq, H, D, dtype=q.dtype, device=q.device)
-        dk, dv = (torch.empty(B, Tk, G, D, dtype=q.dtype, device=q.device) for _ in range(2))
-        strides = (ctypes.c_int64 * 9)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
+        dt, dev = q.dtype, q.device
+        do = _io(do, dt)
+        dq = torch.empty((B, Tq, H, D), dtype=dt, device=dev)
+        dk = torch.empty((B, Tk, G, D), dtype=dt, device=dev)
+        dv = torch.empty((B, Tk, G, D), dtype=dt, device=dev)
+        strides = _I64x9(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
         n = 0 if cu_host is None else cu_host.numel() - 1
         lib = nat.load()
-        nbytes = lib.gdn2_attn_bwd_workspace_size(nat.ptr(cu_host), n, B, Tq, Tk, H, G, D, int(ctx.causal))
-        ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=q.device)
-        with _on_device(q.device):
+        nbytes = lib.gdn2_attn_bwd_workspace_size(nat.ptr(cu_host), n, B, Tq, Tk, H, G, D, causal)
+        ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
+        with _on_device(dev):
             st = lib.gdn2_attn_bwd(
-                nat.ptr(q), nat.ptr(k), nat.ptr(v), ctypes.addressof(strides), nat.ptr(o), nat.ptr(o_lo),
-                nat.ptr(lse), nat.ptr(do), nat.ptr(dq), nat.ptr(dk), nat.ptr(dv), nat.dtype_code(q.dtype), nat.ptr(kv_len), nat.ptr(cu_dev),
-                nat.ptr(cu_host), n, B, Tq, Tk, H, G, D, ctx.scale, int(ctx.causal), nat.ptr(ws), ws.numel(),
-                nat.stream_handle(q.device))
+                q.data_ptr(), k.data_ptr(), v.data_ptr(), ctypes.addressof(strides), o.data_ptr(), o_lo.data_ptr(),
+                lse.data_ptr(), do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), nat.dtype_code(dt),
+                nat.ptr(kv_len), nat.ptr(cu_dev), nat.ptr(cu_host), n, B, Tq, Tk, H, G, D, ctx.scale, causal,
+                ws.data_ptr(), nbytes, nat.stream_handle(dev))
         nat.check(st, "attention backward")
         return dq, dk, dv, None, None, None, None, None
 
@@ -1644,7 +1658,10 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float | 
             raise ValueError(f"{name}: tensors on {q.device} and {t.device}")
     kv_len = None if kv_lengths is None else kv_lengths.detach().to(torch.int64).contiguous()
     cu_dev, cu_host = _cu(cu_seqlens, q.device, Tq)
-    return AttentionFunction.apply(q, k, v, scale, bool(causal), kv_len, cu_dev, cu_host)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return AttentionFunction.apply(q, k, v, scale, int(causal), kv_len, cu_dev, cu_host)
+    return _attention_fwd(_head_rows(q), _head_rows(k), _head_rows(v), scale, int(causal), kv_len, cu_dev, cu_host,
+                          False)[0]
 
 
 class KVCacheQ4(NamedTuple):
@@ -1722,7 +1739,7 @@ def kv_cache_q4_store(cache: KVCacheQ4, k: torch.Tensor, v: torch.Tensor, start:
         raise ValueError(f"{name}: tensors on {k.device}, {v.device} and {cache.k.device}")
     pos, stride = _positions(name, "start", start, B, k.device)
     k, v = _head_rows(k.detach()), _head_rows(v.detach())
-    strides = (ctypes.c_int64 * 6)(*k.stride()[:3], *v.stride()[:3])
+    strides = _I64x6(*k.stride()[:3], *v.stride()[:3])
     with _on_device(k.device):
         st = nat.load().gdn2_kv_cache_q4_store(
             nat.ptr(k), nat.ptr(v), ctypes.addressof(strides), dt, nat.ptr(pos), stride, nat.ptr(cache.k),
@@ -1837,26 +1854,35 @@ def _logit_rows(x: torch.Tensor) -> tuple[torch.Tensor, int, int, int, int]:
     return x, max(rows, 1), 0, x.stride(0) if x.dim() == 2 else x.shape[-1], rows
 
 
+def _token_logprobs_fwd(logits, targets, top_k: int, ignore_index: int, keep: bool):
+    """``(logp, entropy, top_logp, top_ids, x, lse)``: ``x`` the logits as read, ``lse`` only with ``keep``."""
+    x, inner, so, sr, rows = _logit_rows(logits)
+    V, dev, shape = x.shape[-1], x.device, targets.shape
+    logp = torch.empty(shape, dtype=torch.float32, device=dev)
+    ent = torch.empty(shape, dtype=torch.float32, device=dev)
+    lse = torch.empty((rows, 2), dtype=torch.float32, device=dev) if keep else None
+    top_lp = torch.empty((*shape, top_k), dtype=torch.float32, device=dev) if top_k else None
+    top_ids = torch.empty((*shape, top_k), dtype=torch.int64, device=dev) if top_k else None
+    lib, dt = nat.load(), nat.dtype_code(x.dtype)
+    nbytes = lib.gdn2_token_logprobs_workspace_size(rows, V, top_k, dt)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    with _on_device(dev):
+        st = lib.gdn2_token_logprobs_fwd(
+            x.data_ptr(), inner, so, sr, dt, rows, V, targets.data_ptr(), ignore_index, logp.data_ptr(),
+            ent.data_ptr(), nat.ptr(lse), top_k, nat.ptr(top_lp), nat.ptr(top_ids), nat.ptr(ws), nbytes,
+            nat.stream_handle(dev))
+    nat.check(st, "token_logprobs")
+    return logp, ent, top_lp, top_ids, x, lse
+
+
 class TokenLogprobsFunction(torch.autograd.Function):
     """:func:`token_logprobs` with the HIP forward and backward (``gdn2_token_logprobs_fwd`` /
     ``gdn2_token_logprobs_bwd``): each row's maximum and log sum are kept, nothing of its size."""
 
     @staticmethod
     def forward(ctx, logits, targets, top_k: int, ignore_index: int):
-        x, inner, so, sr, rows = _logit_rows(logits)
-        V, dev, shape = x.shape[-1], x.device, tuple(targets.shape)
-        logp, ent = (torch.empty(shape, dtype=torch.float32, device=dev) for _ in range(2))
-        lse = torch.empty(rows, 2, dtype=torch.float32, device=dev) if ctx.needs_input_grad[0] else None
-        top_lp = torch.empty(*shape, top_k, dtype=torch.float32, device=dev) if top_k else None
-        top_ids = torch.empty(*shape, top_k, dtype=torch.int64, device=dev) if top_k else None
-        lib, dt = nat.load(), nat.dtype_code(x.dtype)
-        nbytes = lib.gdn2_token_logprobs_workspace_size(rows, V, top_k, dt)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        with _on_device(dev):
-            st = lib.gdn2_token_logprobs_fwd(
-                nat.ptr(x), inner, so, sr, dt, rows, V, nat.ptr(targets), ignore_index, nat.ptr(logp), nat.ptr(ent),
-                nat.ptr(lse), top_k, nat.ptr(top_lp), nat.ptr(top_ids), nat.ptr(ws), nbytes, nat.stream_handle(dev))
-        nat.check(st, "token_logprobs")
+        logp, ent, top_lp, top_ids, x, lse = _token_logprobs_fwd(logits, targets, top_k, ignore_index,
+                                                                 ctx.needs_input_grad[0])
         ctx.save_for_backward(x, targets, ent, lse)
         ctx.shape, ctx.ignore_index = logits.shape, ignore_index
         ctx.set_materialize_grads(False)
@@ -1915,7 +1941,10 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0,
     _require_gpu(name, logits, targets)
     if targets.device != logits.device:
         raise ValueError(f"{name}: tensors on {logits.device} and {targets.device}")
-    return TokenLogprobs(*TokenLogprobsFunction.apply(logits, targets.contiguous(), int(top_k), int(ignore_index)))
+    args = logits, targets.contiguous(), int(top_k), int(ignore_index)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return TokenLogprobs(*TokenLogprobsFunction.apply(*args))
+    return TokenLogprobs(*_token_logprobs_fwd(*args, False)[:4])
 
 
 def _rows2d(name: str, x: torch.Tensor, dt: torch.dtype, width: int) -> int:
