@@ -412,12 +412,16 @@ int gdn2_token_logprobs_bwd(const void *x, int64_t inner_rows, int64_t outer_str
  * over the query heads of a group, from o, o_lo and lse of the forward and dout
  * [B, Tq, H, D] contiguous; the probabilities are recomputed.  Every output has
  * the same bits in every run.  bf16 / fp16, D in {64, 128}, scale > 0; else
- * GDN2_ERR_UNSUPPORTED.
+ * GDN2_ERR_UNSUPPORTED.  workspace: gdn2_attn_fwd_workspace_size() (0 unless few
+ * queries face many keys; then it may be NULL) and gdn2_attn_bwd_workspace_size()
+ * bytes, 16-byte aligned, of which concurrent calls need one each.
  */
 int gdn2_attn_fwd(const void *q, const void *k, const void *v, const int64_t *strides, void *o, void *o_lo, float *lse,
                   int io_dtype, const int64_t *kv_lengths, const int64_t *cu_seqlens,
                   const int64_t *cu_seqlens_host, int num_seqs, int B, int Tq, int Tk, int H, int G, int D,
-                  float scale, int causal, void *stream);
+                  float scale, int causal, void *workspace, size_t workspace_bytes, void *stream);
+size_t gdn2_attn_fwd_workspace_size(const int64_t *cu_seqlens_host, int num_seqs, int B, int Tq, int Tk, int H, int G,
+                                    int D, int causal);
 size_t gdn2_attn_bwd_workspace_size(const int64_t *cu_seqlens_host, int num_seqs, int B, int Tq, int Tk, int H, int G,
                                     int D, int causal);
 int gdn2_attn_bwd(const void *q, const void *k, const void *v, const int64_t *strides, const void *o,

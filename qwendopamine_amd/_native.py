@@ -93,8 +93,9 @@ SIGNATURES: dict[str, tuple] = {
     "gdn2_token_logprobs_fwd": (_i, [_vp, _i64, _i64, _i64, _i, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _i, _vp, _vp, _vp,
                                      _sz, _vp]),
     "gdn2_token_logprobs_bwd": (_i, [_vp, _i64, _i64, _i64, _i, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "gdn2_attn_fwd_workspace_size": (_sz, [_vp, _i, _i, _i, _i, _i, _i, _i, _i]),
     "gdn2_attn_fwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _f, _i,
-                           _vp]),
+                           _vp, _sz, _vp]),
     "gdn2_attn_bwd_workspace_size": (_sz, [_vp, _i, _i, _i, _i, _i, _i, _i, _i]),
     "gdn2_attn_bwd": (
         _i,

@@ -616,6 +616,7 @@ static int fill_attn_sizes(AttnTrainParams &p, const int64_t *cu_host, int num_s
     if (Tq > (1 << 30) || Tk > (1 << 30) || B > (1 << 30) || H > (1 << 20) || D > (1 << 20) || num_seqs > (1 << 30))
         return GDN2_ERR_UNSUPPORTED;
     p.max_q = Tq;
+    p.q_tiles = static_cast<int64_t>(B) * ((Tq + 127) / 128);
     p.k_tiles = static_cast<int64_t>(B) * ((Tk + 127) / 128);
     if (cu_host) {
         if (B != 1 || Tq != Tk || num_seqs < 0) return GDN2_ERR_INVALID;
@@ -628,14 +629,17 @@ static int fill_attn_sizes(AttnTrainParams &p, const int64_t *cu_host, int num_s
             if (n > p.max_q) p.max_q = static_cast<int>(n);
             p.k_tiles += (n + 127) / 128;
         }
+        p.q_tiles = p.k_tiles;
     }
     p.nseq = cu_host ? num_seqs : B;
     p.B = B; p.Tq = Tq; p.Tk = Tk; p.H = H; p.G = G; p.D = D;
     p.causal = causal != 0;
     p.splits = attn_bwd_splits(p);
+    p.splits_f = p.splits_q = attn_key_shares(p);
     // One launch of at most 2^31 - 1 workgroups, the smallest of them 32 rows.
     const double longest = p.max_q > Tk ? p.max_q : Tk;
-    if ((longest / 32 + 1) * p.nseq * H * p.splits > 2147483000.0 || static_cast<double>(B) * Tq * H > 17179869184.0 ||
+    if ((longest / 32 + 1) * p.nseq * H * p.splits > 2147483000.0 ||
+        (longest / 32 + 1) * p.nseq * H * p.splits_f > 2147483000.0 || static_cast<double>(B) * Tq * H > 17179869184.0 ||
         static_cast<double>(B) * (H + G) > 500000000.0 || static_cast<double>(B) * Tk * G * D > 500000000000.0)
         return GDN2_ERR_UNSUPPORTED;
     return GDN2_OK;
@@ -670,7 +674,7 @@ static int fill_attn_args(AttnTrainParams &p, const void *q, const void *k, cons
 int gdn2_attn_fwd(const void *q, const void *k, const void *v, const int64_t *strides, void *o, void *o_lo, float *lse,
                   int io_dtype, const int64_t *kv_lengths, const int64_t *cu_seqlens,
                   const int64_t *cu_seqlens_host, int num_seqs, int B, int Tq, int Tk, int H, int G, int D,
-                  float scale, int causal, void *stream)
+                  float scale, int causal, void *workspace, size_t workspace_bytes, void *stream)
 {
     AttnTrainParams p = {};
     const int st = fill_attn_args(p, q, k, v, strides, io_dtype, kv_lengths, cu_seqlens, cu_seqlens_host, num_seqs, B,
@@ -678,10 +682,22 @@ int gdn2_attn_fwd(const void *q, const void *k, const void *v, const int64_t *st
     if (st != GDN2_OK) return st;
     if (B == 0 || Tq == 0 || p.nseq == 0) return GDN2_OK;
     if (!o || !lse || ((reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(o_lo)) & 15)) return GDN2_ERR_INVALID;
+    const size_t need = attn_fwd_workspace_bytes(p);
+    if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15)))
+        return GDN2_ERR_WORKSPACE;
     p.o = o;
     p.o_lo = o_lo;
     p.lse = lse;
+    attn_fwd_workspace(p, workspace);
     return launch_attn_fwd(p, io_dtype, static_cast<hipStream_t>(stream)) == hipSuccess ? GDN2_OK : GDN2_ERR_LAUNCH;
+}
+
+size_t gdn2_attn_fwd_workspace_size(const int64_t *cu_seqlens_host, int num_seqs, int B, int Tq, int Tk, int H, int G,
+                                    int D, int causal)
+{
+    AttnTrainParams p = {};
+    if (fill_attn_sizes(p, cu_seqlens_host, num_seqs, B, Tq, Tk, H, G, D, causal) != GDN2_OK) return 0;
+    return attn_fwd_workspace_bytes(p);
 }
 
 size_t gdn2_attn_bwd_workspace_size(const int64_t *cu_seqlens_host, int num_seqs, int B, int Tq, int Tk, int H, int G,

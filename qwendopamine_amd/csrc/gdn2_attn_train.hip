@@ -171,6 +171,7 @@ struct Where {
     int bq, bk;      // batch row of q and k
     int nq, nk;      // queries, visible keys
     int shift;       // causal: query i sees keys j <= i + shift
+    int share;       // which share of the streamed side
 };
 
 __device__ __forceinline__ void where_rows(const AttnTrainParams &p, Where &w)
@@ -195,12 +196,14 @@ __device__ __forceinline__ void where_rows(const AttnTrainParams &p, Where &w)
 }
 
 // Query-resident kernels: heads of a group next to each other in the order of
-// workgroups modulo 8 (the XCDs), long causal tiles first.
-__device__ __forceinline__ Where where_q(const AttnTrainParams &p)
+// workgroups modulo 8 (the XCDs), long causal tiles first; w.share of `shares` of the keys.
+__device__ __forceinline__ Where where_q(const AttnTrainParams &p, int shares)
 {
     Where w;
     const int nbh = p.nseq * p.H;
-    const int t = blockIdx.x / nbh, j = blockIdx.x - t * nbh;
+    const int ts = blockIdx.x / nbh, j = blockIdx.x - ts * nbh;
+    const int t = ts / shares;
+    w.share = ts - t * shares;
     w.s = j / p.H;
     const int jh = j - w.s * p.H;
     w.g = jh % p.G;
@@ -226,6 +229,33 @@ __device__ __forceinline__ void hide(f32x16 &s, int j0, int h, int limit)
 
 // ---------------------------------------------------------------- forward
 
+// L in base 2.  A query that sees no key: +inf, which makes its recomputed P zero.
+__device__ __forceinline__ float log_sum(float m, float l)
+{
+    return l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
+}
+
+// Four channels of O, and, for D = dO . O, what their rounding left out: without it D is
+// off by half a step of O, which shows in dS where few keys carry the weight
+// and dP - D cancels.  What is below the sums' own error is dropped: O of a
+// single key is then exactly its V.
+template <PrecKind PK>
+__device__ __forceinline__ void store_o(uint16_t *o, uint16_t *ol, float a, float b, float c, float d)
+{
+    const Q4<PK> r = pack4<PK>(a, b, c, d);
+    st_q4<PK>(o, r);
+    if (!ol) return;
+    const float y[4] = {a, b, c, d};
+    float z[4];
+    unpack4<PK>(r, z);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        z[e] = y[e] - z[e];
+        z[e] = fabsf(z[e]) > 0x1p-18f * fabsf(y[e]) ? z[e] : 0.0f;
+    }
+    st_q4<PK>(ol, pack4<PK>(z[0], z[1], z[2], z[3]));
+}
+
 template <PrecKind PK, int D, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(AttnTrainParams p)
 {
@@ -237,7 +267,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(AttnTrainParams p)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, h = lane >> 5;
     const int rb = row_base<D>(lane), cb = col_base<D>(lane);
-    const Where w = where_q(p);
+    const Where w = where_q(p, p.splits_f);
     const int m0 = w.tile * BM;
     if (m0 >= w.nq) return;
     const int qi = m0 + 32 * wave + n;  // this lane's query
@@ -266,12 +296,14 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(AttnTrainParams p)
 #pragma unroll
     for (int d = 0; d < DT; ++d) acc[d] = zero16();
 
-    const int nt = kend > 0 ? (kend + kTile - 1) / kTile : 0;
-    if (nt > 0) {
-        stage<D, NW>(kb, p.ks[1], 0, w.nk, tile_k(0), wave, lane);
-        stage<D, NW>(vb, p.vs[1], 0, w.nk, tile_v(0), wave, lane);
+    const int all = kend > 0 ? (kend + kTile - 1) / kTile : 0;
+    const int first = static_cast<int>(static_cast<int64_t>(all) * w.share / p.splits_f);
+    const int nt = static_cast<int>(static_cast<int64_t>(all) * (w.share + 1) / p.splits_f);
+    if (first < nt) {
+        stage<D, NW>(kb, p.ks[1], first * kTile, w.nk, tile_k(first), wave, lane);
+        stage<D, NW>(vb, p.vs[1], first * kTile, w.nk, tile_v(first), wave, lane);
     }
-    for (int t = 0; t < nt; ++t) {
+    for (int t = first; t < nt; ++t) {
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();  // tile t has landed, and every wave is done with tile t - 1
         if (t + 1 < nt) {
@@ -329,36 +361,65 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(AttnTrainParams p)
     }
     l = half_add(l);
     if (qi >= w.nq) return;
-    // A query that sees no key: zeros, and L = +inf, which makes its recomputed P zero.
+    const int64_t orow = (w.bq * static_cast<int64_t>(p.Tq) + w.q0 + qi) * p.H + w.h;
+    if (p.splits_f > 1) {
+        // This share's state; attn_fwd_join_kernel puts the shares together.
+        const int64_t at = w.share * (static_cast<int64_t>(p.B) * p.Tq * p.H) + orow;
+        if (h == 0) *reinterpret_cast<float2 *>(p.part_ml + 2 * at) = make_float2(m, l);
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<float4 *>(p.part + at * D + 32 * d + 8 * i + 4 * h) =
+                    make_float4(acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]);
+        return;
+    }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    if (h == 0)
-        p.lse[(static_cast<int64_t>(w.bq) * p.H + w.h) * p.Tq + w.q0 + qi] =
-            l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
-    const int64_t row = ((w.bq * static_cast<int64_t>(p.Tq) + w.q0 + qi) * p.H + w.h) * D;
-    uint16_t *o = static_cast<uint16_t *>(p.o) + row, *ol = static_cast<uint16_t *>(p.o_lo) + row;
+    if (h == 0) p.lse[(static_cast<int64_t>(w.bq) * p.H + w.h) * p.Tq + w.q0 + qi] = log_sum(m, l);
+    uint16_t *o = static_cast<uint16_t *>(p.o) + orow * D;
+    uint16_t *ol = p.o_lo ? static_cast<uint16_t *>(p.o_lo) + orow * D : nullptr;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float y[4] = {acc[d][4 * i] * inv, acc[d][4 * i + 1] * inv, acc[d][4 * i + 2] * inv,
-                                acc[d][4 * i + 3] * inv};
-            const Q4<PK> r = pack4<PK>(y[0], y[1], y[2], y[3]);
-            st_q4<PK>(o + 32 * d + 8 * i + 4 * h, r);
-            if (p.o_lo) {
-                // What the rounding left out, for D = dO . O: without it D is
-                // off by half a step of O, which shows in dS where few keys
-                // carry the weight and dP - D cancels.  What is below the sums'
-                // own error is left out: O of a single key is then exactly its V.
-                float z[4];
-                unpack4<PK>(r, z);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    z[e] = y[e] - z[e];
-                    z[e] = fabsf(z[e]) > 0x1p-18f * fabsf(y[e]) ? z[e] : 0.0f;
-                }
-                st_q4<PK>(ol + 32 * d + 8 * i + 4 * h, pack4<PK>(z[0], z[1], z[2], z[3]));
-            }
+            const int e = 32 * d + 8 * i + 4 * h;
+            store_o<PK>(o + e, ol ? ol + e : nullptr, acc[d][4 * i] * inv, acc[d][4 * i + 1] * inv,
+                        acc[d][4 * i + 2] * inv, acc[d][4 * i + 3] * inv);
         }
+}
+
+// The shares of a query's keys, in their order; thread: 4 channels of a row.
+template <PrecKind PK>
+__global__ __launch_bounds__(256) void attn_fwd_join_kernel(AttnTrainParams p)
+{
+    const int64_t rows = static_cast<int64_t>(p.B) * p.Tq * p.H;
+    const int64_t e = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
+    const int64_t row = e / p.D;
+    if (row >= rows) return;
+    float m = kNoMax;
+    for (int s = 0; s < p.splits_f; ++s) m = fmaxf(m, p.part_ml[2 * (s * rows + row)]);
+    float l = 0.0f;
+    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int s = 0; s < p.splits_f; ++s) {
+        const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + 2 * (s * rows + row));
+        const float4 y = *reinterpret_cast<const float4 *>(p.part + s * rows * p.D + e);
+        const float r = __builtin_amdgcn_exp2f(ml.x - m);
+        l = fmaf(ml.y, r, l);
+        x.x = fmaf(y.x, r, x.x);
+        x.y = fmaf(y.y, r, x.y);
+        x.z = fmaf(y.z, r, x.z);
+        x.w = fmaf(y.w, r, x.w);
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    if (e == row * p.D) {
+        const int64_t bt = row / p.H;
+        const int hh = static_cast<int>(row - bt * p.H);
+        const int64_t b = bt / p.Tq;
+        p.lse[(b * p.H + hh) * p.Tq + (bt - b * p.Tq)] = log_sum(m, l);
+    }
+    store_o<PK>(static_cast<uint16_t *>(p.o) + e, p.o_lo ? static_cast<uint16_t *>(p.o_lo) + e : nullptr, x.x * inv,
+                x.y * inv, x.z * inv, x.w * inv);
 }
 
 // ---------------------------------------------------------------- backward
@@ -443,7 +504,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dq_kernel(AttnTrainParams p)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, h = lane >> 5;
     const int rb = row_base<D>(lane), cb = col_base<D>(lane);
-    const Where w = where_q(p);
+    const Where w = where_q(p, p.splits_q);
     const int m0 = w.tile * BM;
     if (m0 >= w.nq) return;
     const int qi = m0 + 32 * wave + n;
@@ -481,7 +542,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dq_kernel(AttnTrainParams p)
         dl = ((n >> 2) & 1) == h ? dl : 0.0f;
         dl = half_add(dl);
     }
-    if (h == 0 && qi < w.nq) p.delta[srow] = dl;
+    if (h == 0 && qi < w.nq && w.share == 0) p.delta[srow] = dl;
     dl *= sc;
     const float lse = p.lse[srow];
 
@@ -499,12 +560,14 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dq_kernel(AttnTrainParams p)
     f32x16 acc[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d) acc[d] = zero16();
-    const int nt = kend > 0 ? (kend + kTile - 1) / kTile : 0;
-    if (nt > 0) {
-        stage<D, NW>(kb, p.ks[1], 0, w.nk, tile_k(0), wave, lane);
-        stage<D, NW>(vb, p.vs[1], 0, w.nk, tile_v(0), wave, lane);
+    const int all = kend > 0 ? (kend + kTile - 1) / kTile : 0;
+    const int first = static_cast<int>(static_cast<int64_t>(all) * w.share / p.splits_q);
+    const int nt = static_cast<int>(static_cast<int64_t>(all) * (w.share + 1) / p.splits_q);
+    if (first < nt) {
+        stage<D, NW>(kb, p.ks[1], first * kTile, w.nk, tile_k(first), wave, lane);
+        stage<D, NW>(vb, p.vs[1], first * kTile, w.nk, tile_v(first), wave, lane);
     }
-    for (int t = 0; t < nt; ++t) {
+    for (int t = first; t < nt; ++t) {
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
         if (t + 1 < nt) {
@@ -538,6 +601,16 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dq_kernel(AttnTrainParams p)
     }
     if (qi >= w.nq) return;
     const float f = p.scale / sc;
+    if (p.splits_q > 1) {
+        float *part = p.part_q + w.share * (static_cast<int64_t>(p.B) * p.Tq * p.H * D) + orow;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<float4 *>(part + 32 * d + 8 * i + 4 * h) =
+                    make_float4(acc[d][4 * i] * f, acc[d][4 * i + 1] * f, acc[d][4 * i + 2] * f, acc[d][4 * i + 3] * f);
+        return;
+    }
     uint16_t *dq = static_cast<uint16_t *>(p.dq) + orow;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -549,7 +622,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dq_kernel(AttnTrainParams p)
 
 // dK, dV: keys resident, one pass over the queries of every head of the group,
 // or, where that leaves too few or too uneven workgroups (attn_bwd_splits), over
-// one of p.splits equal shares of it, whose fp32 sums attn_dkv_sum_kernel adds.
+// one of p.splits equal shares of it, whose fp32 sums attn_sum_kernel adds.
 template <PrecKind PK, int D, int NW, int BQ>
 __global__ __launch_bounds__(64 * NW, 2) void attn_dkv_kernel(AttnTrainParams p)
 {
@@ -739,23 +812,31 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dkv_kernel(AttnTrainParams p)
         }
 }
 
-// Sums of the shares, in their order; thread: 4 channels of dk or of dv.
+// Sums of n shares of `all` values each, stride apart, in their order, rounded; thread: 4 values.
 template <PrecKind PK>
-__global__ __launch_bounds__(256) void attn_dkv_sum_kernel(AttnTrainParams p)
+__global__ __launch_bounds__(256) void attn_sum_kernel(const float *part, int64_t stride, int n, uint16_t *out,
+                                                       int64_t all)
 {
-    const int64_t all = static_cast<int64_t>(p.B) * p.Tk * p.G * p.D;
-    int64_t e = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
-    if (e >= 2 * all) return;
+    const int64_t e = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
+    if (e >= all) return;
     float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int s = 0; s < p.splits; ++s) {
-        const float4 y = *reinterpret_cast<const float4 *>(p.part + 2 * s * all + e);
+#pragma unroll 4
+    for (int s = 0; s < n; ++s) {
+        const float4 y = *reinterpret_cast<const float4 *>(part + s * stride + e);
         x.x += y.x;
         x.y += y.y;
         x.z += y.z;
         x.w += y.w;
     }
-    uint16_t *out = static_cast<uint16_t *>(e < all ? p.dk : p.dv) + (e < all ? e : e - all);
-    st_q4<PK>(out, pack4<PK>(x.x, x.y, x.z, x.w));
+    st_q4<PK>(out + e, pack4<PK>(x.x, x.y, x.z, x.w));
+}
+
+template <PrecKind PK>
+hipError_t sum_shares(const float *part, int64_t stride, int n, void *out, int64_t all, hipStream_t s)
+{
+    hipLaunchKernelGGL((attn_sum_kernel<PK>), dim3(static_cast<unsigned>((all / 4 + 255) / 256)), dim3(256), 0, s, part,
+                       stride, n, static_cast<uint16_t *>(out), all);
+    return hipGetLastError();
 }
 
 // Four waves per workgroup, two workgroups per CU: against eight waves and one, the
@@ -768,8 +849,13 @@ template <PrecKind PK, int D>
 hipError_t fwd_d(AttnTrainParams p, hipStream_t s)
 {
     p.tiles = (p.max_q + 32 * kWaves - 1) / (32 * kWaves);
-    hipLaunchKernelGGL((attn_fwd_kernel<PK, D, kWaves>), dim3(static_cast<unsigned>(p.tiles) * p.nseq * p.H),
-                       dim3(64 * kWaves), 0, s, p);
+    hipLaunchKernelGGL((attn_fwd_kernel<PK, D, kWaves>),
+                       dim3(static_cast<unsigned>(p.tiles) * p.nseq * p.H * p.splits_f), dim3(64 * kWaves), 0, s, p);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || p.splits_f == 1) return e;
+    const int64_t threads = static_cast<int64_t>(p.B) * p.Tq * p.H * (D / 4);
+    hipLaunchKernelGGL((attn_fwd_join_kernel<PK>), dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0, s,
+                       p);
     return hipGetLastError();
 }
 
@@ -783,9 +869,11 @@ hipError_t bwd_d(AttnTrainParams p, hipStream_t s)
     }
     if (p.Tq > 0 && p.max_q > 0) {
         p.tiles = (p.max_q + 32 * kWaves - 1) / (32 * kWaves);
-        hipLaunchKernelGGL((attn_dq_kernel<PK, D, kWaves>), dim3(static_cast<unsigned>(p.tiles) * p.nseq * p.H),
-                           dim3(64 * kWaves), 0, s, p);
+        hipLaunchKernelGGL((attn_dq_kernel<PK, D, kWaves>),
+                           dim3(static_cast<unsigned>(p.tiles) * p.nseq * p.H * p.splits_q), dim3(64 * kWaves), 0, s, p);
         if ((e = hipGetLastError()) != hipSuccess) return e;
+        const int64_t all = static_cast<int64_t>(p.B) * p.Tq * p.H * D;
+        if (p.splits_q > 1 && (e = sum_shares<PK>(p.part_q, all, p.splits_q, p.dq, all, s)) != hipSuccess) return e;
     }
     if (p.Tk > 0) {
         // Query rows per tile: at D = 128 half of the other's, so that two
@@ -795,11 +883,12 @@ hipError_t bwd_d(AttnTrainParams p, hipStream_t s)
         hipLaunchKernelGGL((attn_dkv_kernel<PK, D, kWaves, BQ>),
                            dim3(static_cast<unsigned>(tiles) * p.nseq * p.G * p.splits), dim3(64 * kWaves), 0, s, p);
         if ((e = hipGetLastError()) != hipSuccess) return e;
+        const int64_t all = static_cast<int64_t>(p.B) * p.Tk * p.G * D;
         if (p.splits > 1) {
-            const int64_t threads = static_cast<int64_t>(p.B) * p.Tk * p.G * D / 2;
-            hipLaunchKernelGGL((attn_dkv_sum_kernel<PK>), dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256),
-                               0, s, p);
+            if ((e = sum_shares<PK>(p.part, 2 * all, p.splits, p.dk, all, s)) != hipSuccess) return e;
+            e = sum_shares<PK>(p.part + all, 2 * all, p.splits, p.dv, all, s);
         }
+        return e;
     }
     return hipGetLastError();
 }
@@ -828,25 +917,55 @@ int attn_bwd_splits(const AttnTrainParams &p)
     return static_cast<int>(s < 1 ? 1 : (s > 16 ? 16 : s));
 }
 
-static size_t up16(size_t x) { return (x + 15) & ~static_cast<size_t>(15); }
-
-// D per query, fp16's norms, the shares' sums.
-size_t attn_bwd_workspace_bytes(const AttnTrainParams &p)
+// Shares of the keys in the query-resident kernels, where few queries face many
+// keys: up to 512 workgroups, of at least 8 key tiles each.
+int attn_key_shares(const AttnTrainParams &p)
 {
-    const size_t part = p.splits > 1 ? static_cast<size_t>(p.splits) * 2 * p.B * p.Tk * p.G * p.D * sizeof(float) : 0;
-    return up16(static_cast<size_t>(p.B) * p.H * p.Tq * sizeof(float)) +
-           up16(static_cast<size_t>(p.B) * (p.H + p.G) * kNormParts * sizeof(float)) + part;
+    const int64_t wgs = p.q_tiles * p.H, tiles = (p.Tk + kTile - 1) / kTile;
+    if (wgs == 0 || wgs >= 256) return 1;
+    int64_t s = 512 / wgs;
+    s = s < tiles / 8 ? s : tiles / 8;
+    return static_cast<int>(s < 1 ? 1 : (s > 64 ? 64 : s));
 }
 
-void attn_bwd_workspace(AttnTrainParams &p, void *workspace)
+static size_t up16(size_t x) { return (x + 15) & ~static_cast<size_t>(15); }
+
+// The shares' values, maxima and sums.
+size_t attn_fwd_workspace_bytes(const AttnTrainParams &p)
+{
+    const size_t rows = static_cast<size_t>(p.B) * p.Tq * p.H;
+    return p.splits_f > 1 ? p.splits_f * rows * (p.D + 2) * sizeof(float) : 0;
+}
+
+void attn_fwd_workspace(AttnTrainParams &p, void *workspace)
+{
+    p.part = static_cast<float *>(workspace);
+    p.part_ml = p.part + static_cast<size_t>(p.splits_f) * p.B * p.Tq * p.H * p.D;
+}
+
+// D per query, fp16's norms, the shares' sums of dk and dv and of dq.
+size_t attn_bwd_workspace_bytes(const AttnTrainParams &p)
+{
+    AttnTrainParams q = p;
+    return attn_bwd_workspace(q, nullptr);
+}
+
+size_t attn_bwd_workspace(AttnTrainParams &p, void *workspace)
 {
     char *w = static_cast<char *>(workspace);
-    p.delta = reinterpret_cast<float *>(w);
-    w += up16(static_cast<size_t>(p.B) * p.H * p.Tq * sizeof(float));
-    p.mx_do = reinterpret_cast<float *>(w);
-    p.mx_v = p.mx_do + static_cast<size_t>(p.B) * p.H * kNormParts;
-    w += up16(static_cast<size_t>(p.B) * (p.H + p.G) * kNormParts * sizeof(float));
-    p.part = reinterpret_cast<float *>(w);
+    size_t at = 0;
+    auto take = [&](size_t floats) {
+        float *x = reinterpret_cast<float *>(w + at);
+        at += up16(floats * sizeof(float));
+        return x;
+    };
+    const size_t q = static_cast<size_t>(p.B) * p.Tq * p.H, k = static_cast<size_t>(p.B) * p.Tk * p.G;
+    p.delta = take(q);
+    p.mx_do = take(static_cast<size_t>(p.B) * p.H * kNormParts);
+    p.mx_v = take(static_cast<size_t>(p.B) * p.G * kNormParts);
+    p.part = take(p.splits > 1 ? p.splits * 2 * k * p.D : 0);
+    p.part_q = take(p.splits_q > 1 ? p.splits_q * q * p.D : 0);
+    return at;
 }
 
 hipError_t launch_attn_fwd(const AttnTrainParams &p, int io_dtype, hipStream_t s)

@@ -318,13 +318,17 @@ struct AttnTrainParams {
     void *dq, *dk, *dv;
     float *delta;
     float *mx_do, *mx_v;     // fp16: squared row norm maxima [B][H][], [B][G][]
-    float *part;             // dk and dv of each share [splits][2][B, Tk, G, D], with more than one
-    int splits;              // shares of a key tile's queries (attn_bwd_splits)
+    // Shares, and with more than one their fp32 results: of a key tile's queries
+    // (part: dk and dv [splits][2][B, Tk, G, D]), of a query tile's keys in the forward
+    // (part: values [splits_f][B, Tq, H, D], part_ml: maxima and sums [..][B, Tq, H][2])
+    // and for dq (part_q [splits_q][B, Tq, H, D]).
+    int splits, splits_f, splits_q;
+    float *part, *part_ml, *part_q;
     const int64_t *kv_len;   // [B] or NULL
     const int64_t *cu;       // [nseq + 1] or NULL
     int nseq;                // B without cu
     int max_q;               // longest sequence's queries
-    int64_t k_tiles;         // tiles of 128 keys over all sequences (one head)
+    int64_t q_tiles, k_tiles;  // tiles of 128 queries, keys, over all sequences (one head)
     int tiles;               // set by the launcher
     int B, Tq, Tk, H, G, D;
     int causal;
@@ -333,7 +337,10 @@ struct AttnTrainParams {
 bool attn_train_supported(int io_dtype, int D);
 int attn_bwd_splits(const AttnTrainParams &p);
 size_t attn_bwd_workspace_bytes(const AttnTrainParams &p);
-void attn_bwd_workspace(AttnTrainParams &p, void *workspace);
+size_t attn_bwd_workspace(AttnTrainParams &p, void *workspace);
+int attn_key_shares(const AttnTrainParams &p);
+size_t attn_fwd_workspace_bytes(const AttnTrainParams &p);
+void attn_fwd_workspace(AttnTrainParams &p, void *workspace);
 hipError_t launch_attn_fwd(const AttnTrainParams &p, int io_dtype, hipStream_t stream);
 hipError_t launch_attn_bwd(const AttnTrainParams &p, int io_dtype, hipStream_t stream);
 

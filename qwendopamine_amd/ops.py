@@ -1551,11 +1551,14 @@ def _attention_fwd(q, k, v, scale: float, causal: bool, kv_len, cu_dev, cu_host,
     lse = torch.empty((B, H, Tq), dtype=torch.float32, device=dev)
     strides = _I64x9(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
     n = 0 if cu_host is None else cu_host.numel() - 1
+    lib = nat.load()
+    nbytes = lib.gdn2_attn_fwd_workspace_size(nat.ptr(cu_host), n, B, Tq, Tk, H, G, D, causal)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     with _on_device(dev):
-        st = nat.load().gdn2_attn_fwd(
+        st = lib.gdn2_attn_fwd(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), ctypes.addressof(strides), o.data_ptr(), nat.ptr(o_lo),
             lse.data_ptr(), nat.dtype_code(q.dtype), nat.ptr(kv_len), nat.ptr(cu_dev), nat.ptr(cu_host), n, B, Tq, Tk, H,
-            G, D, scale, causal, nat.stream_handle(dev))
+            G, D, scale, causal, nat.ptr(ws), nbytes, nat.stream_handle(dev))
     nat.check(st, "attention")
     return o, o_lo, lse
 

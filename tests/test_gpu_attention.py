@@ -61,6 +61,9 @@ def _check(got, q, k, v, do, scale=None, causal=True, kv_lengths=None, cu=None):
     (2, 300, 511, 8, 2, 128, BF, False),
     (1, 1023, 1023, 4, 1, 64, BF, True),
     (1, 777, 1200, 6, 3, 128, FP, True),
+    (1, 1, 2100, 4, 2, 64, FP, True),      # few queries over many keys: the keys are shared out
+    (2, 5, 1500, 8, 2, 128, BF, True),
+    (1, 150, 1111, 2, 1, 64, BF, False),
 ])
 def test_attention_matches_float64(gpu_device, B, Tq, Tk, H, G, D, dt, causal):
     print(f"[case] attention B{B} Tq{Tq} Tk{Tk} H{H} G{G} D{D} {dt} causal={causal}", flush=True)
@@ -125,6 +128,15 @@ def test_attention_packed(gpu_device, cu, causal):
     _check(got, *x, causal=causal, cu=cu)
     on_device = _run(*x, causal=causal, cu_seqlens=torch.tensor(cu, device=gpu_device, dtype=torch.int32))
     assert all(torch.equal(got[n], on_device[n]) for n in got)
+
+
+def test_attention_shared_keys_of_padded_rows(gpu_device):
+    """Key shares past a row's length hold nothing; a row of no keys gives zeros."""
+    lens = [0, 1, 700, 1600]
+    x = _inputs(gpu_device, 4, 3, 1600, 2, 2, 64, BF, seed=19)
+    got = _run(*x, causal=False, kv_lengths=torch.tensor(lens, device=gpu_device))
+    _check(got, *x, causal=False, kv_lengths=lens)
+    assert (got["o"][0] == 0).all() and (got["dq"][0] == 0).all()
 
 
 def test_attention_nothing_to_see(gpu_device):

@@ -58,7 +58,7 @@ def _attn_call(lib, **over):
     return lib.gdn2_attn_fwd(a["ptr"], a["ptr"], a["ptr"], st and ctypes.addressof(st), a["o"], None, a["lse"],
                              a["dt"], a["kv"],
                              a["cu"], host and ctypes.addressof(host), a["n"], a["B"], a["Tq"], a["Tk"], a["H"], a["G"],
-                             a["D"], a["scale"], 1, None)
+                             a["D"], a["scale"], 1, None, 0, None)
 
 
 @pytest.mark.parametrize("want,over", [
@@ -80,6 +80,7 @@ def _attn_call(lib, **over):
     (nat.ERR_UNSUPPORTED, dict(scale=0.0)),
     (nat.ERR_UNSUPPORTED, dict(scale=float("nan"))),
     (nat.ERR_UNSUPPORTED, dict(B=1 << 30, Tq=1 << 20)),
+    (nat.ERR_WORKSPACE, dict(Tk=100000)),
     (nat.OK, dict(B=0)),
     (nat.OK, dict(Tq=0)),
 ])
