@@ -195,6 +195,18 @@ __device__ __forceinline__ void where_rows(const AttnTrainParams &p, Where &w)
     }
 }
 
+// Order of causal tiles, longest first, as workgroups of equal place in successive
+// rounds over the 256 CUs share a CU: every other round runs backwards, so that
+// a CU's tiles add up to about the same length (`row`: workgroups per tile).
+__device__ __forceinline__ int snake(int t, int tiles, int row)
+{
+    const int m = row < 256 ? 256 / row : 1;  // tiles per round
+    const int c = t / m, base = c * m;
+    if ((c & 1) == 0) return t;
+    const int last = base + m < tiles ? base + m - 1 : tiles - 1;
+    return base + last - t;
+}
+
 // Query-resident kernels: heads of a group next to each other in the order of
 // workgroups modulo 8 (the XCDs), long causal tiles first; w.share of `shares` of the keys.
 __device__ __forceinline__ Where where_q(const AttnTrainParams &p, int shares)
@@ -208,7 +220,7 @@ __device__ __forceinline__ Where where_q(const AttnTrainParams &p, int shares)
     const int jh = j - w.s * p.H;
     w.g = jh % p.G;
     w.h = w.g * (p.H / p.G) + jh / p.G;
-    w.tile = p.tiles - 1 - t;
+    w.tile = p.tiles - 1 - snake(t, p.tiles, nbh * shares);
     where_rows(p, w);
     return w;
 }
