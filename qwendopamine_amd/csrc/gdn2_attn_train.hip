@@ -33,8 +33,8 @@ namespace {
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr float kLog2e = 1.4426950408889634f;
-// Reference maximum before any key has been seen: finite, so that the
-// exponent of a hidden score (-inf) is -inf and never inf - inf.
+// Reference of a share of the keys that holds none a query sees: finite, below
+// every score, so that differences of references are never inf - inf.
 constexpr float kNoMax = -3.0e38f;
 // The running maximum moves only when a score exceeds it by 2^kLazy: until
 // then the probabilities are at most 2^kLazy, exact in the same number of
@@ -96,23 +96,47 @@ __device__ __forceinline__ int swz(int row)
     return (((row & 3) << 1) | ((row >> 2) & 1) | (row & 8)) & (D / 8 - 1);
 }
 
-// One tile, row0 .. row0 + ROWS - 1 of nrows rows ts elements apart, requested
-// into LDS.  Rows past the end repeat the last row (never out of bounds, never
-// another sequence's row); the scores of such rows are hidden.
-template <int D, int NW, int ROWS = kTile>
-__device__ __forceinline__ void stage(const uint16_t *base, int64_t ts, int row0, int nrows, uint16_t *lds, int wave,
-                                      int lane)
+// A streamed matrix: rows ts bytes apart, and this lane's place in a request (its
+// row of the first R and its 16-byte piece; later requests of a tile are whole
+// multiples of 16 rows on, where the permutation repeats, so that a tile's
+// requests differ in their scalar base alone).
+struct Stream {
+    const char *base;
+    int64_t ts;
+    unsigned lane_off;
+};
+template <int D, int NW>
+__device__ __forceinline__ Stream stream_of(const uint16_t *base, int64_t ts, int wave, int lane)
 {
-    constexpr int P = D / 8, R = 64 / P, IT = ROWS / R;  // pieces per row, rows per request, requests
+    constexpr int P = D / 8, R = 64 / P;  // pieces per row, rows per request
+    static_assert(NW * R % 16 == 0, "the permutation repeats from one of a wave's requests to its next");
+    const int r = wave * R + lane / P;
+    return {reinterpret_cast<const char *>(base), 2 * ts,
+            static_cast<unsigned>(r * static_cast<int>(2 * ts) + ((lane % P) ^ swz<D>(r)) * 16)};
+}
+
+// One tile, row0 .. row0 + ROWS - 1 of nrows rows, requested into LDS.  Rows past the
+// end repeat the last row (never out of bounds, never another sequence's row);
+// the scores of such rows are hidden.
+template <int D, int NW, int ROWS = kTile>
+__device__ __forceinline__ void stage(const Stream &x, int row0, int nrows, char *lds, int wave, int lane)
+{
+    constexpr int P = D / 8, R = 64 / P, IT = ROWS / R;  // requests per tile
+    static_assert(IT % NW == 0, "every wave issues as many requests");
+    const char *tile = x.base + row0 * x.ts;
+    if (row0 + ROWS <= nrows) {
 #pragma unroll
-    for (int it = 0; it < (IT + NW - 1) / NW; ++it) {
-        const int c = it * NW + wave;
-        if (IT % NW != 0 && c >= IT) break;
-        const int r = c * R + lane / P;
-        const int piece = (lane % P) ^ swz<D>(r);
-        const int gr = row0 + r < nrows ? row0 + r : nrows - 1;
-        __builtin_amdgcn_global_load_lds(reinterpret_cast<const char *>(base + gr * ts + piece * 8), lds + c * R * D, 16,
-                                         0, 0);
+        for (int it = 0; it < IT / NW; ++it)
+            __builtin_amdgcn_global_load_lds(reinterpret_cast<const char *>(tile + it * (NW * R) * x.ts + x.lane_off),
+                                             lds + (it * NW + wave) * 1024, 16, 0, 0);
+    } else {
+#pragma unroll
+        for (int it = 0; it < IT / NW; ++it) {
+            const int r = (it * NW + wave) * R + lane / P;
+            const int rc = row0 + r < nrows ? r : nrows - 1 - row0;
+            __builtin_amdgcn_global_load_lds(reinterpret_cast<const char *>(tile + rc * x.ts + ((lane % P) ^ swz<D>(r)) * 16),
+                                             lds + (it * NW + wave) * 1024, 16, 0, 0);
+        }
     }
 }
 
@@ -274,8 +298,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(AttnTrainParams p)
     constexpr int KS = D / 16, DT = D / 32, BM = 32 * NW;
     constexpr int kBytes = kTile * D * 2;
     __shared__ __align__(256) char smem[4 * kBytes];  // two tiles of k, two of v
-    auto tile_k = [&](int t) __attribute__((always_inline)) { return reinterpret_cast<uint16_t *>(smem + (t & 1) * kBytes); };
-    auto tile_v = [&](int t) __attribute__((always_inline)) { return reinterpret_cast<uint16_t *>(smem + (2 + (t & 1)) * kBytes); };
+    auto tile_k = [&](int t) __attribute__((always_inline)) { return smem + (t & 1) * kBytes; };
+    auto tile_v = [&](int t) __attribute__((always_inline)) { return smem + (2 + (t & 1)) * kBytes; };
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, h = lane >> 5;
     const int rb = row_base<D>(lane), cb = col_base<D>(lane);
@@ -286,6 +310,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(AttnTrainParams p)
     const int qc = qi < w.nq ? qi : w.nq - 1;
     const uint16_t *kb = static_cast<const uint16_t *>(p.k) + w.bk * p.ks[0] + w.k0 * p.ks[1] + w.g * p.ks[2];
     const uint16_t *vb = static_cast<const uint16_t *>(p.v) + w.bk * p.vs[0] + w.k0 * p.vs[1] + w.g * p.vs[2];
+    const Stream ks = stream_of<D, NW>(kb, p.ks[1], wave, lane), vs = stream_of<D, NW>(vb, p.vs[1], wave, lane);
     const uint16_t *qr = static_cast<const uint16_t *>(p.q) + w.bq * p.qs[0] + (w.q0 + qc) * p.qs[1] + w.h * p.qs[2];
     uint4 qf[KS];
 #pragma unroll
@@ -303,7 +328,9 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(AttnTrainParams p)
     const int wend = p.causal && wmax + w.shift + 1 < w.nk ? wmax + w.shift + 1 : w.nk;  // none sees more
     const float c = p.scale * kLog2e;
 
-    float m = kNoMax, l = 0.0f;
+    // Reference of the exponents (the running maximum, within kLazy) and their sum.
+    float m = 0.0f, l = 0.0f;
+    bool fresh = true;  // no visible key yet
     f32x16 acc[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d) acc[d] = zero16();
@@ -312,15 +339,15 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(AttnTrainParams p)
     const int first = static_cast<int>(static_cast<int64_t>(all) * w.share / p.splits_f);
     const int nt = static_cast<int>(static_cast<int64_t>(all) * (w.share + 1) / p.splits_f);
     if (first < nt) {
-        stage<D, NW>(kb, p.ks[1], first * kTile, w.nk, tile_k(first), wave, lane);
-        stage<D, NW>(vb, p.vs[1], first * kTile, w.nk, tile_v(first), wave, lane);
+        stage<D, NW>(ks, first * kTile, w.nk, tile_k(first), wave, lane);
+        stage<D, NW>(vs, first * kTile, w.nk, tile_v(first), wave, lane);
     }
     for (int t = first; t < nt; ++t) {
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();  // tile t has landed, and every wave is done with tile t - 1
         if (t + 1 < nt) {
-            stage<D, NW>(kb, p.ks[1], (t + 1) * kTile, w.nk, tile_k(t + 1), wave, lane);
-            stage<D, NW>(vb, p.vs[1], (t + 1) * kTile, w.nk, tile_v(t + 1), wave, lane);
+            stage<D, NW>(ks, (t + 1) * kTile, w.nk, tile_k(t + 1), wave, lane);
+            stage<D, NW>(vs, (t + 1) * kTile, w.nk, tile_v(t + 1), wave, lane);
         }
         const int j0 = t * kTile;
         if (j0 >= wend) continue;
@@ -336,26 +363,41 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(AttnTrainParams p)
             hide<true>(s[0], j0, h, lim);
             hide<true>(s[1], j0 + 32, h, lim);
         }
-        float mx = s[0][0];
+        // Exponents relative to the reference so far, and their maximum (taken
+        // from them and not from the scores: fmaxf of a product's result costs a
+        // second instruction, to quiet a NaN it might hold).
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, fmaxf(s[0][i], s[1][i]));
-        mx = half_max(mx) * c;
-        if (__any(mx > m + kLazy)) {
-            const float mn = fmaxf(m, mx);
-            const float r = __builtin_amdgcn_exp2f(m - mn);
-            m = mn;
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[a][i] = fmaf(s[a][i], c, -m);
+                mx[i & 3] = fmaxf(mx[i & 3], s[a][i]);
+            }
+        const float top = half_max(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+        if (__any(top > (fresh ? -INFINITY : kLazy))) {
+            // The first visible key sets the reference, later ones raise it.
+            const bool set = fresh && top > -INFINITY;
+            const float d = set ? top : fmaxf(top, 0.0f);
+            const float r = fresh ? 1.0f : __builtin_amdgcn_exp2f(-d);  // nothing to rescale yet
+            m += d;
+            fresh = fresh && !set;
             l *= r;
 #pragma unroll
-            for (int d = 0; d < DT; ++d)
+            for (int e = 0; e < DT; ++e)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) acc[d][i] *= r;
+                for (int i = 0; i < 16; ++i) acc[e][i] *= r;
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[a][i] -= d;
         }
         float sum = 0.0f;
 #pragma unroll
         for (int a = 0; a < 2; ++a)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                s[a][i] = __builtin_amdgcn_exp2f(fmaf(s[a][i], c, -m));
+                s[a][i] = __builtin_amdgcn_exp2f(s[a][i]);
                 sum += s[a][i];
             }
         l += sum;
@@ -372,6 +414,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(AttnTrainParams p)
             }
     }
     l = half_add(l);
+    m = fresh ? kNoMax : m;
     if (qi >= w.nq) return;
     const int64_t orow = (w.bq * static_cast<int64_t>(p.Tq) + w.q0 + qi) * p.H + w.h;
     if (p.splits_f > 1) {
@@ -511,8 +554,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dq_kernel(AttnTrainParams p)
     constexpr int KS = D / 16, DT = D / 32, BM = 32 * NW;
     constexpr int kBytes = kTile * D * 2;
     __shared__ __align__(256) char smem[4 * kBytes];  // two tiles of k, two of v
-    auto tile_k = [&](int t) __attribute__((always_inline)) { return reinterpret_cast<uint16_t *>(smem + (t & 1) * kBytes); };
-    auto tile_v = [&](int t) __attribute__((always_inline)) { return reinterpret_cast<uint16_t *>(smem + (2 + (t & 1)) * kBytes); };
+    auto tile_k = [&](int t) __attribute__((always_inline)) { return smem + (t & 1) * kBytes; };
+    auto tile_v = [&](int t) __attribute__((always_inline)) { return smem + (2 + (t & 1)) * kBytes; };
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, h = lane >> 5;
     const int rb = row_base<D>(lane), cb = col_base<D>(lane);
@@ -523,6 +566,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dq_kernel(AttnTrainParams p)
     const int qc = qi < w.nq ? qi : w.nq - 1;
     const uint16_t *kb = static_cast<const uint16_t *>(p.k) + w.bk * p.ks[0] + w.k0 * p.ks[1] + w.g * p.ks[2];
     const uint16_t *vb = static_cast<const uint16_t *>(p.v) + w.bk * p.vs[0] + w.k0 * p.vs[1] + w.g * p.vs[2];
+    const Stream ks = stream_of<D, NW>(kb, p.ks[1], wave, lane), vs = stream_of<D, NW>(vb, p.vs[1], wave, lane);
     const uint16_t *qr = static_cast<const uint16_t *>(p.q) + w.bq * p.qs[0] + (w.q0 + qc) * p.qs[1] + w.h * p.qs[2];
     const int64_t orow = ((w.bq * static_cast<int64_t>(p.Tq) + w.q0 + qc) * p.H + w.h) * D;
     const uint16_t *dr = static_cast<const uint16_t *>(p.dout) + orow;
@@ -576,15 +620,15 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dq_kernel(AttnTrainParams p)
     const int first = static_cast<int>(static_cast<int64_t>(all) * w.share / p.splits_q);
     const int nt = static_cast<int>(static_cast<int64_t>(all) * (w.share + 1) / p.splits_q);
     if (first < nt) {
-        stage<D, NW>(kb, p.ks[1], first * kTile, w.nk, tile_k(first), wave, lane);
-        stage<D, NW>(vb, p.vs[1], first * kTile, w.nk, tile_v(first), wave, lane);
+        stage<D, NW>(ks, first * kTile, w.nk, tile_k(first), wave, lane);
+        stage<D, NW>(vs, first * kTile, w.nk, tile_v(first), wave, lane);
     }
     for (int t = first; t < nt; ++t) {
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
         if (t + 1 < nt) {
-            stage<D, NW>(kb, p.ks[1], (t + 1) * kTile, w.nk, tile_k(t + 1), wave, lane);
-            stage<D, NW>(vb, p.vs[1], (t + 1) * kTile, w.nk, tile_v(t + 1), wave, lane);
+            stage<D, NW>(ks, (t + 1) * kTile, w.nk, tile_k(t + 1), wave, lane);
+            stage<D, NW>(vs, (t + 1) * kTile, w.nk, tile_v(t + 1), wave, lane);
         }
         const int j0 = t * kTile;
         if (j0 >= wend) continue;
@@ -711,14 +755,18 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dkv_kernel(AttnTrainParams p)
     const int steps = static_cast<int>(static_cast<int64_t>(nt) * qpk * (share + 1) / p.splits) - x0;
     const uint16_t *qb = static_cast<const uint16_t *>(p.q) + w.bq * p.qs[0] + w.q0 * p.qs[1];
     const uint16_t *db = static_cast<const uint16_t *>(p.dout) + (w.bq * static_cast<int64_t>(p.Tq) + w.q0) * p.H * D;
+    const Stream qs = stream_of<D, NW>(qb, p.qs[1], wave, lane);
+    const Stream ds = stream_of<D, NW>(db, static_cast<int64_t>(p.H) * D, wave, lane);
     const int64_t sb = static_cast<int64_t>(w.bq) * p.H * p.Tq + w.q0;
     int rh = nt > 0 ? x0 / nt : 0, rt = nt > 0 ? x0 - rh * nt : 0;  // of the step requested next
     int ct = rt;                                                    // query tile of the current step
     auto request = [&](int buf) __attribute__((always_inline)) {
         const int hh = w.h + rh, row0 = (t0 + rt) * BQ;
-        stage<D, NW, BQ>(qb + hh * p.qs[2], p.qs[1], row0, w.nq, reinterpret_cast<uint16_t *>(smem + buf * kBytes), wave, lane);
-        stage<D, NW, BQ>(db + hh * D, static_cast<int64_t>(p.H) * D, row0, w.nq,
-                     reinterpret_cast<uint16_t *>(smem + (2 + buf) * kBytes), wave, lane);
+        Stream qh = qs, dh = ds;
+        qh.base += 2 * hh * p.qs[2];
+        dh.base += 2 * hh * D;
+        stage<D, NW, BQ>(qh, row0, w.nq, smem + buf * kBytes, wave, lane);
+        stage<D, NW, BQ>(dh, row0, w.nq, smem + (2 + buf) * kBytes, wave, lane);
         if (tid < 2 * BQ) {
             const int r = row0 + (tid & (BQ - 1));
             const float *src = (tid < BQ ? p.lse : p.delta) + sb + static_cast<int64_t>(hh) * p.Tq;
@@ -733,7 +781,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dkv_kernel(AttnTrainParams p)
     };
     if (steps > 0) {
         request(0);
-        if constexpr (kVLds) stage<D, NW, BN>(vb, p.vs[1], n0, w.nk, reinterpret_cast<uint16_t *>(smem + kOffV), wave, lane);
+        if constexpr (kVLds)
+            stage<D, NW, BN>(stream_of<D, NW>(vb, p.vs[1], wave, lane), n0, w.nk, smem + kOffV, wave, lane);
     }
     for (int x = 0; x < steps; ++x) {
         __builtin_amdgcn_s_waitcnt(0);

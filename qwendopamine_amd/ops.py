@@ -1526,7 +1526,7 @@ def _head_rows(x: torch.Tensor) -> torch.Tensor:
     if x.is_contiguous() and x.data_ptr() % 16 == 0:
         return x
     per = 16 // x.element_size()
-    if x.stride(3) == 1 and x.data_ptr() % 16 == 0 and all(
+    if x.stride(3) == 1 and x.data_ptr() % 16 == 0 and x.stride(1) <= 1 << 25 and all(
             x.stride(i) % per == 0 for i in range(3) if x.shape[i] > 1):
         return x
     x = x.contiguous()
