@@ -457,6 +457,12 @@ static int check_q4_cache(const void *kc, const void *km, const void *vc, const 
     return GDN2_OK;
 }
 
+// One launch of at most 2^31 - 1 workgroups (of 128 tokens of one head's group each).
+static bool q4_launchable(int B, int64_t T, int G, int D)
+{
+    return T <= (1 << 30) && 2.0 * ((T + 127) / 128) * (D / 64) * G * B < 2147483000.0;
+}
+
 size_t gdn2_attn_decode_q4_workspace_size(int B, int G, int qpk, int D, int64_t max_len)
 {
     if (B < 1 || G < 1 || qpk < 1 || D < 1 || max_len < 1) return 0;
@@ -503,8 +509,7 @@ int gdn2_kv_cache_q4_store(const void *k, const void *v, const int64_t *strides,
     if (st != GDN2_OK) return st;
     if (B == 0 || T == 0) return GDN2_OK;
     if (!k || !v || ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15)) return GDN2_ERR_INVALID;
-    if (T > (1 << 30) || ((T + 7) / 8) * (D / 64) * static_cast<int64_t>(G) * B > 2147483647LL)
-        return GDN2_ERR_UNSUPPORTED;
+    if (!q4_launchable(B, T, G, D)) return GDN2_ERR_UNSUPPORTED;
     Q4StoreParams p = {};
     const int64_t size[6] = {B, T, G, B, T, G};
     const int per = io_dtype == GDN2_DTYPE_F32 ? 4 : 8;
@@ -529,7 +534,7 @@ int gdn2_kv_cache_q4_load(const void *k_codes, const void *k_meta, const void *v
     if (st != GDN2_OK) return st;
     if (B == 0 || T == 0) return GDN2_OK;
     if (!k || !v || ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15)) return GDN2_ERR_INVALID;
-    if (T > (1 << 30) || (static_cast<double>(B) * T * G * (D / 8)) / 128.0 > 2147483000.0) return GDN2_ERR_UNSUPPORTED;
+    if (!q4_launchable(B, T, G, D)) return GDN2_ERR_UNSUPPORTED;
     Q4LoadParams p = {};
     p.k = k; p.v = v;
     p.start = start; p.start_stride = start_stride;

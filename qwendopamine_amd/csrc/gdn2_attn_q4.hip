@@ -558,32 +558,41 @@ __global__ __launch_bounds__(256) void attn_q4_merge_kernel(AttnQ4Params p)
     io<T>::st(static_cast<T *>(p.out), static_cast<int64_t>(blockIdx.x) * D + d, den == 0.0f ? 0.0f : num / den);
 }
 
-// Whole prompts into the cache: 8 lanes per group of 64 channels, one 16-byte
-// piece each; the lanes of a wave take 8 consecutive tokens of one group, whose
-// codes are consecutive in the cache.
-template <typename T>
-__global__ __launch_bounds__(256) void q4_store_kernel(Q4StoreParams p)
+// ---- whole prompts in and out of the cache.  8 lanes per group of 64 channels, 8
+// channels each; a wave takes 8 consecutive tokens at a time, whose codes are consecutive
+// in the cache, and kQ4Tiles such tiles with all of their reads requested first.  A
+// workgroup works on one (k or v, sequence, head, group).
+constexpr int kQ4Tiles = 4;
+constexpr int kQ4BlockTokens = 8 * kQ4Tiles * 4;
+
+struct Q4Place {
+    bool is_k;
+    int b, g, grp;
+    int64_t t0;  // this lane's first token; its others 8 on each
+    int e;       // its 8 channels
+};
+
+__device__ __forceinline__ Q4Place q4_place(int64_t T, int B, int G, int NG)
 {
-    const int NG = p.D / 64;
-    const int64_t tiles = (p.T + 7) / 8;
-    const int64_t wv = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63, e = lane & 7;
-    // (which of k, v; batch; head; group; tile of 8 tokens), tiles fastest
-    const int64_t per = tiles * NG * p.G * p.B;
-    if (wv >= 2 * per) return;
-    const bool is_k = wv < per;
-    int64_t r = is_k ? wv : wv - per;
-    const int64_t tile = r % tiles;
-    r /= tiles;
-    const int grp = static_cast<int>(r % NG);
+    const unsigned blocks = static_cast<unsigned>((T + kQ4BlockTokens - 1) / kQ4BlockTokens);
+    unsigned r = blockIdx.x / blocks;
+    const unsigned blk = blockIdx.x - r * blocks;
+    Q4Place x;
+    x.grp = static_cast<int>(r % NG);
     r /= NG;
-    const int g = static_cast<int>(r % p.G), b = static_cast<int>(r / p.G);
-    const int64_t t = tile * 8 + (lane >> 3);
-    const int64_t pos = (p.start ? p.start[p.start_stride * b] : 0) + t;
-    const bool in = t < p.T && pos >= 0 && pos < p.max_len;  // positions outside the cache are not stored
-    const int64_t *st = is_k ? p.ks : p.vs;
-    const T *x = static_cast<const T *>(is_k ? p.k : p.v) + b * st[0] + (t < p.T ? t : 0) * st[1] + g * st[2] + grp * 64 + e * 8;
-    float v[8];
+    x.g = static_cast<int>(r % G);
+    r /= G;
+    x.b = static_cast<int>(r % B);
+    x.is_k = r / B == 0;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    x.t0 = static_cast<int64_t>(blk) * kQ4BlockTokens + wave * (8 * kQ4Tiles) + (lane >> 3);
+    x.e = lane & 7;
+    return x;
+}
+
+template <typename T>
+__device__ __forceinline__ void load8(const T *x, float (&v)[8])
+{
     if constexpr (sizeof(T) == 4) {
         const float4 a = reinterpret_cast<const float4 *>(x)[0], c = reinterpret_cast<const float4 *>(x)[1];
         v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
@@ -594,30 +603,53 @@ __global__ __launch_bounds__(256) void q4_store_kernel(Q4StoreParams p)
         f.u = *reinterpret_cast<const uint4 *>(x);
         unpack_frag<PK>(f, v);
     }
-    float mn = v[0], mx = v[0];
-    bool finite = true;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void q4_store_kernel(Q4StoreParams p)
+{
+    const int NG = p.D / 64, lane = threadIdx.x & 63;
+    const Q4Place at = q4_place(p.T, p.B, p.G, NG);
+    const int64_t *st = at.is_k ? p.ks : p.vs;
+    const T *x = static_cast<const T *>(at.is_k ? p.k : p.v) + at.b * st[0] + at.g * st[2] + at.grp * 64 + at.e * 8;
+    const int64_t first = p.start ? p.start[p.start_stride * at.b] : 0;
+    const int64_t row0 = (static_cast<int64_t>(at.b) * p.G + at.g) * p.max_len;
+    unsigned *codes = reinterpret_cast<unsigned *>((at.is_k ? p.k_codes : p.v_codes) + at.grp * 32);
+    unsigned *meta_out = (at.is_k ? p.k_meta : p.v_meta) + at.grp;
+    float v[kQ4Tiles][8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        mn = fminf(mn, v[i]);
-        mx = fmaxf(mx, v[i]);
-        finite = finite && fabsf(v[i]) < INFINITY;
+    for (int u = 0; u < kQ4Tiles; ++u) {
+        const int64_t t = at.t0 + 8 * u;
+        load8(x + (t < p.T ? t : 0) * st[1], v[u]);
     }
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
-        mn = fminf(mn, __shfl_xor(mn, o, 64));
-        mx = fmaxf(mx, __shfl_xor(mx, o, 64));
-    }
-    finite = ((__ballot(!finite) >> (lane & ~7)) & 0xff) == 0;
-    const unsigned meta = group_meta(mn, mx, finite);
-    const float inv = inv_scale(meta);
-    unsigned w = 0;
+    for (int u = 0; u < kQ4Tiles; ++u) {
+        float mn = v[u][0], mx = v[u][0];
+        bool finite = true;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w |= code_of(v[i], meta, inv) << (4 * i);
-    if (!finite) w = 0;
-    if (!in) return;
-    const int64_t row = (static_cast<int64_t>(b) * p.G + g) * p.max_len + pos;
-    reinterpret_cast<unsigned *>((is_k ? p.k_codes : p.v_codes) + row * (p.D / 2) + grp * 32)[e] = w;
-    if (e == 0) (is_k ? p.k_meta : p.v_meta)[row * NG + grp] = meta;
+        for (int i = 0; i < 8; ++i) {
+            mn = fminf(mn, v[u][i]);
+            mx = fmaxf(mx, v[u][i]);
+            finite = finite && fabsf(v[u][i]) < INFINITY;
+        }
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) {
+            mn = fminf(mn, __shfl_xor(mn, o, 64));
+            mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+        }
+        finite = ((__ballot(!finite) >> (lane & ~7)) & 0xff) == 0;
+        const unsigned meta = group_meta(mn, mx, finite);
+        const float inv = inv_scale(meta);
+        unsigned w = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w |= code_of(v[u][i], meta, inv) << (4 * i);
+        if (!finite) w = 0;
+        const int64_t t = at.t0 + 8 * u, pos = first + t;
+        if (t < p.T && pos >= 0 && pos < p.max_len) {  // positions outside the cache are not stored
+            codes[(row0 + pos) * (p.D / 8) + at.e] = w;
+            if (at.e == 0) meta_out[(row0 + pos) * NG] = meta;
+        }
+    }
 }
 
 // What positions start .. start + T - 1 stand for, [B, T, G, D] in T (zeros
@@ -626,39 +658,44 @@ __global__ __launch_bounds__(256) void q4_store_kernel(Q4StoreParams p)
 template <typename T>
 __global__ __launch_bounds__(256) void q4_load_kernel(Q4LoadParams p)
 {
-    const int W = p.D / 8, NG = p.D / 64;
-    const int64_t per = static_cast<int64_t>(p.B) * p.T * p.G * W;
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    if (i >= 2 * per) return;
-    const bool is_k = i < per;
-    const int64_t o = is_k ? i : i - per;
-    int64_t r = o;
-    const int w = static_cast<int>(r % W);
-    r /= W;
-    const int g = static_cast<int>(r % p.G);
-    r /= p.G;
-    const int64_t t = r % p.T;
-    const int b = static_cast<int>(r / p.T);
-    const int64_t pos = (p.start ? p.start[p.start_stride * b] : 0) + t;
-    float v[8];
+    const int NG = p.D / 64;
+    const Q4Place at = q4_place(p.T, p.B, p.G, NG);
+    const int64_t first = p.start ? p.start[p.start_stride * at.b] : 0;
+    const int64_t row0 = (static_cast<int64_t>(at.b) * p.G + at.g) * p.max_len;
+    const unsigned *codes = reinterpret_cast<const unsigned *>((at.is_k ? p.k_codes : p.v_codes) + at.grp * 32);
+    const unsigned *metas = (at.is_k ? p.k_meta : p.v_meta) + at.grp;
+    unsigned w[kQ4Tiles], m[kQ4Tiles];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-    if (pos >= 0 && pos < p.max_len) {
-        const int64_t row = (static_cast<int64_t>(b) * p.G + g) * p.max_len + pos;
-        const unsigned u = reinterpret_cast<const unsigned *>((is_k ? p.k_codes : p.v_codes) + row * (p.D / 2))[w];
-        const unsigned meta = (is_k ? p.k_meta : p.v_meta)[row * NG + w / 8];
-        const float sc = __uint_as_float(meta << 16), mn = __uint_as_float(meta & 0xffff0000u);
+    for (int u = 0; u < kQ4Tiles; ++u) {
+        const int64_t t = at.t0 + 8 * u, pos = first + t;
+        const bool in = t < p.T && pos >= 0 && pos < p.max_len;
+        const int64_t row = row0 + (in ? pos : 0);
+        const unsigned cw = codes[row * (p.D / 8) + at.e], cm = metas[row * NG];
+        w[u] = in ? cw : 0u;
+        m[u] = in ? cm : 0u;
+    }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = fmaf(static_cast<float>((u >> (4 * e)) & 15u), sc, mn);
+    for (int u = 0; u < kQ4Tiles; ++u) {
+        const int64_t t = at.t0 + 8 * u;
+        if (t >= p.T) break;
+        const float sc = __uint_as_float(m[u] << 16), mn = __uint_as_float(m[u] & 0xffff0000u);
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = fmaf(static_cast<float>((w[u] >> (4 * i)) & 15u), sc, mn);
+        T *y = static_cast<T *>(at.is_k ? p.k : p.v) + ((at.b * p.T + t) * p.G + at.g) * p.D + at.grp * 64 + at.e * 8;
+        if constexpr (sizeof(T) == 4) {
+            reinterpret_cast<float4 *>(y)[0] = make_float4(v[0], v[1], v[2], v[3]);
+            reinterpret_cast<float4 *>(y)[1] = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+            constexpr PrecKind PK = std::is_same<T, bf16_t>::value ? PrecKind::BF16 : PrecKind::F16;
+            *reinterpret_cast<uint4 *>(y) = pack_frag<PK>(v).u;
+        }
     }
-    T *y = static_cast<T *>(is_k ? p.k : p.v) + o * 8;
-    if constexpr (sizeof(T) == 4) {
-        reinterpret_cast<float4 *>(y)[0] = make_float4(v[0], v[1], v[2], v[3]);
-        reinterpret_cast<float4 *>(y)[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-        constexpr PrecKind PK = std::is_same<T, bf16_t>::value ? PrecKind::BF16 : PrecKind::F16;
-        *reinterpret_cast<uint4 *>(y) = pack_frag<PK>(v).u;
-    }
+}
+
+unsigned q4_blocks(int64_t T, int B, int G, int D)
+{
+    return static_cast<unsigned>(2 * ((T + kQ4BlockTokens - 1) / kQ4BlockTokens) * (D / 64) * G * B);
 }
 
 template <typename T, PrecKind PK, int D>
@@ -719,8 +756,7 @@ hipError_t launch_attn_q4(const AttnQ4Params &p, int io_dtype, hipStream_t s)
 
 hipError_t launch_q4_store(const Q4StoreParams &p, int io_dtype, hipStream_t s)
 {
-    const int64_t waves = 2 * ((p.T + 7) / 8) * (p.D / 64) * p.G * p.B;
-    const dim3 grid(static_cast<unsigned>((waves + 3) / 4));
+    const dim3 grid(q4_blocks(p.T, p.B, p.G, p.D));
     switch (io_dtype) {
     case GDN2_DTYPE_F32: hipLaunchKernelGGL((q4_store_kernel<float>), grid, dim3(256), 0, s, p); break;
     case GDN2_DTYPE_BF16: hipLaunchKernelGGL((q4_store_kernel<bf16_t>), grid, dim3(256), 0, s, p); break;
@@ -731,8 +767,7 @@ hipError_t launch_q4_store(const Q4StoreParams &p, int io_dtype, hipStream_t s)
 
 hipError_t launch_q4_load(const Q4LoadParams &p, int io_dtype, hipStream_t s)
 {
-    const int64_t threads = 2 * static_cast<int64_t>(p.B) * p.T * p.G * (p.D / 8);
-    const dim3 grid(static_cast<unsigned>((threads + 255) / 256));
+    const dim3 grid(q4_blocks(p.T, p.B, p.G, p.D));
     switch (io_dtype) {
     case GDN2_DTYPE_F32: hipLaunchKernelGGL((q4_load_kernel<float>), grid, dim3(256), 0, s, p); break;
     case GDN2_DTYPE_BF16: hipLaunchKernelGGL((q4_load_kernel<bf16_t>), grid, dim3(256), 0, s, p); break;
