@@ -407,7 +407,7 @@ int gdn2_token_logprobs_bwd(const void *x, int64_t inner_rows, int64_t outer_str
  * copy; B = 1, Tq = Tk, no kv_lengths) sequences are packed along the tokens,
  * each attending within itself.  A query that sees no key gets zeros (and
  * lse = +inf), and gradients of zero.  Keys outside a row's length or sequence
- * are not read; a hidden key inside it must be finite (0 * inf is NaN).
+ * are not read; a hidden key inside it and dout must be finite (0 * inf is NaN).
  * gdn2_attn_bwd writes dq (like o) and dk, dv [B, Tk, G, D] contiguous, summed
  * over the query heads of a group, from o, o_lo and lse of the forward and dout
  * [B, Tq, H, D] contiguous; the probabilities are recomputed.  Every output has

@@ -249,6 +249,8 @@ class CausalSelfAttention(nn.Module):
             if self.kv_cache is None:
                 raise RuntimeError("KV cache not set up: call HybridDecoder.setup_caches first")
             if q4:
+                if t > self.kv_cache.k.shape[2]:
+                    raise ValueError(f"a prompt of {t} tokens does not fit a cache of {self.kv_cache.k.shape[2]}")
                 ops.kv_cache_q4_store(self.kv_cache, k, v, input_pos[:1])  # consecutive positions
             else:
                 ck, cv = self.kv_cache

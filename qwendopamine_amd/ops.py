@@ -1621,12 +1621,12 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float | 
     * ``kv_lengths`` (int32 / int64 ``[B]`` on the device): ``j < kv_lengths[b]``; keys from there on
       are not read, and their gradients are zero;
     * ``cu_seqlens`` (``[N + 1]`` offsets, one row, ``Tq = Tk``, without ``kv_lengths``): both belong to
-      the same packed sequence.  The offsets are checked on the host: pass them as a CPU tensor
-      to avoid a device synchronisation (a captured graph needs that).
+      the same packed sequence.  The offsets are checked on the host (a CPU tensor saves the device
+      synchronisation) and copied to the device, so a packed call cannot be captured into a graph.
 
     A query that sees no key gives zeros and passes no gradient.  A key hidden from some queries of
-    its row by ``causal`` must be finite (0 times infinity is NaN, as in any attention by
-    products).  Scores, softmax statistics and sums are float32; the probabilities, and in the
+    its row by ``causal`` must be finite, and so must the upstream gradients (0 times infinity is
+    NaN, as in any attention by products).  Scores, softmax statistics and sums are float32; the probabilities, and in the
     backward their gradients, are rounded to the io dtype for the products.  The gradients have
     the same bits in every run.  In a HIP graph, capture the forward and backward together with no
     eager autograd graph of the same leaves alive, as torch asks of any captured backward.
@@ -1929,6 +1929,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0,
     ``[0, V)`` gives NaN.  A row with a NaN or +inf, or of -inf alone, gives NaN, as ``log_softmax``
     does; single -inf logits have probability 0 and pass no gradient.  Sums are float32, the
     gradient is rounded once to the logits' dtype; everything has the same bits in every run.
+    In a HIP graph, capture the forward and backward together with no eager autograd graph of the
+    same leaves alive, as torch asks of any captured backward.
     """
     name = "token_logprobs"
     if logits.dim() < 1 or logits.shape[-1] < 1:

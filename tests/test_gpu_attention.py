@@ -299,6 +299,35 @@ def test_attention_captured_training_replays(gpu_device):
             assert all(torch.equal(a, b) for a, b in zip(out, want.values()))
 
 
+def test_attention_captured_with_lengths(gpu_device):
+    """Padded rows replayed with other lengths (int32), key shares included."""
+    from qwendopamine_amd import ops
+
+    q, k, v, _ = (x.detach() for x in _inputs(gpu_device, 2, 4, 2000, 2, 1, 64, BF, seed=25))
+    kv = torch.tensor([2000, 10], device=gpu_device, dtype=torch.int32)
+    ops.attention(q, k, v, causal=False, kv_lengths=kv)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        o = ops.attention(q, k, v, causal=False, kv_lengths=kv)
+    for lens in ([5, 1999], [0, 700], [2000, 2000]):
+        kv.copy_(torch.tensor(lens, device=gpu_device, dtype=torch.int32))
+        g.replay()
+        assert torch.equal(o, ops.attention(q, k, v, causal=False, kv_lengths=kv))
+
+
+def test_attention_on_a_side_stream(gpu_device):
+    """Inputs made on another stream, after it has been waited for; results used there."""
+    x = _inputs(gpu_device, 1, 90, 90, 2, 2, 64, FP, seed=26)
+    want = _run(*x)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = _run(*(t.detach().clone().requires_grad_(i < 3) for i, t in enumerate(x)))
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(want[n], got[n]) for n in want)
+
+
 def test_attention_refuses_a_second_derivative(gpu_device):
     from qwendopamine_amd import ops
 

@@ -121,6 +121,8 @@ def decode_check(qkv, cos, sin, pos, cache, n_head, out, before):
     (1, 3, 7, 64, 4099, [4098]),
     (1, 1, 8, 128, 20000, [19990]),
     (5, 2, 4, 64, 77, [-1, 5, 77, 10 ** 10, -10 ** 10]),   # outside: zeros, the cache left alone
+    (4, 1, 2, 128, 3000, [2999, -5, 3000, 700]),           # the same, with shares
+    (2, 1, 12, 64, 5000, [4999, 1]),                       # more than eight heads, ragged shares
 ])
 def test_decode_matches_float64(gpu_device, B, G, qpk, D, L, P, dt):
     from qwendopamine_amd import ops

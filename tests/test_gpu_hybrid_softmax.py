@@ -153,6 +153,9 @@ def test_four_bit_layer_is_the_operator(gpu_device):
             o = ops.attention_decode_q4(ops.linear(y, at.attn.weight), cos, sin, pos, want, 4)
             assert torch.equal(got, ops.linear(o.reshape(2, 1, 256), at.proj.weight))
             assert all(torch.equal(a, b) for a, b in zip(at.kv_cache, want))
+    m.setup_caches(2, 20, kv_bits=4)
+    with torch.no_grad(), pytest.raises(ValueError):
+        at(x, cos[:33], sin[:33], torch.arange(33, device=gpu_device))  # a prompt longer than the cache
     m.setup_caches(2, 50, kv_bits=4)
     with pytest.raises(NotImplementedError):
         at(x[:, :1], cos[:1], sin[:1], torch.tensor([0], device=gpu_device))  # gradients through a 4-bit step
