@@ -641,10 +641,9 @@ static int fill_attn_sizes(AttnTrainParams &p, const int64_t *cu_host, int num_s
     p.causal = causal != 0;
     p.splits = attn_bwd_splits(p);
     p.splits_f = p.splits_q = attn_key_shares(p);
-    // One launch of at most 2^31 - 1 workgroups, the smallest of them 32 rows.
-    const double longest = p.max_q > Tk ? p.max_q : Tk;
-    if ((longest / 32 + 1) * p.nseq * H * p.splits > 2147483000.0 ||
-        (longest / 32 + 1) * p.nseq * H * p.splits_f > 2147483000.0 || static_cast<double>(B) * Tq * H > 17179869184.0 ||
+    // One launch of at most 2^31 - 1 workgroups (packed rows: up to 8 times their tiles).
+    const double tiles = static_cast<double>(p.q_tiles > p.k_tiles ? p.q_tiles : p.k_tiles) * H * (cu_host ? 8 : 1);
+    if (tiles * p.splits > 2147483000.0 || tiles * p.splits_f > 2147483000.0 || static_cast<double>(B) * Tq * H > 17179869184.0 ||
         static_cast<double>(B) * (H + G) > 500000000.0 || static_cast<double>(B) * Tk * G * D > 500000000000.0)
         return GDN2_ERR_UNSUPPORTED;
     return GDN2_OK;

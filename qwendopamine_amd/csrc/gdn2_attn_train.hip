@@ -231,20 +231,123 @@ __device__ __forceinline__ int snake(int t, int tiles, int row)
     return base + last - t;
 }
 
+template <int CTRL>
+__device__ __forceinline__ int dpp_add(int x)
+{
+    return x + __builtin_amdgcn_update_dpp(0, x, CTRL, 0xf, 0xf, true);
+}
+// The sum over the wave's lanes, in a scalar register.
+__device__ __forceinline__ int lanes_sum(int x)
+{
+    x = dpp_add<0xb1>(x);   // quad_perm [1, 0, 3, 2]
+    x = dpp_add<0x4e>(x);   // quad_perm [2, 3, 0, 1]
+    x = dpp_add<0x141>(x);  // row_half_mirror: the quads hold equal values
+    x = dpp_add<0x140>(x);  // row_mirror
+    return __builtin_amdgcn_readlane(x, 0) + __builtin_amdgcn_readlane(x, 16) + __builtin_amdgcn_readlane(x, 32) +
+           __builtin_amdgcn_readlane(x, 48);
+}
+
+// Packed sequences of very unequal lengths (packed_ranked): tile t of all their tiles,
+// in an order that starts with long work: by the tile's number in its sequence
+// (`level`, causal work grows with it; from the end for key tiles), the highest
+// first; past kRanked sequences, where a lane would hold too many lengths, in the
+// order of the sequences.  The launch then holds no more workgroups than there are tiles.
+constexpr int kRanked = 256;
+struct Packed {
+    int s, level, tiles;  // sequence, and its number of tiles; s < 0: none
+};
+__device__ __forceinline__ int seq_tiles(const int64_t *cu, int nseq, int s)
+{
+    const int64_t n = s < nseq ? cu[s + 1] - cu[s] : 0;
+    return n > 0 ? static_cast<int>((n + 127) >> 7) : 0;
+}
+__device__ __forceinline__ Packed packed_tile(const int64_t *cu, int nseq, int longest, int t)
+{
+    const int lane = threadIdx.x & 63;
+    if (nseq <= kRanked) {
+        constexpr int U = kRanked / 64;
+        int n[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) n[u] = 64 * u < nseq ? seq_tiles(cu, nseq, 64 * u + lane) : 0;
+        auto at_least = [&](int x) {  // tiles of level x and above
+            int c = 0;
+#pragma unroll
+            for (int u = 0; u < U; ++u) c += n[u] > x ? n[u] - x : 0;
+            return lanes_sum(c);
+        };
+        int lo = 0, hi = longest;  // the highest level with more than t tiles at or above it
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (at_least(mid) > t) lo = mid;
+            else hi = mid;
+        }
+        int r = t - at_least(lo + 1);  // the r-th of the sequences that have this level
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint64_t have = __ballot(n[u] > lo);
+            const int c = __popcll(have);
+            if (r >= 0 && r < c) {
+                const int before = __popcll(have & ((1ull << lane) - 1));
+                const int l = __ffsll(static_cast<unsigned long long>(__ballot(n[u] > lo && before == r))) - 1;
+                return {64 * u + l, lo, __builtin_amdgcn_readlane(n[u], l)};
+            }
+            r -= c;
+        }
+        return {-1, 0, 0};
+    }
+    // Each lane's range of sequences first, then 64 sequences at a time within it.
+    auto before = [&](int x) {  // sum over the lanes below
+        int y = x;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int z = __shfl_up(y, d);
+            y += lane >= d ? z : 0;
+        }
+        return y - x;
+    };
+    const int each = (nseq + 63) / 64;
+    int c = 0;
+    for (int i = 0; i < each; ++i) c += seq_tiles(cu, nseq, lane * each + i);
+    int b = before(c);
+    uint64_t hit = __ballot(t >= b && t - b < c);
+    if (!hit) return {-1, 0, 0};
+    int l = __ffsll(static_cast<unsigned long long>(hit)) - 1;
+    t -= __builtin_amdgcn_readlane(b, l);
+    for (int s0 = l * each, end = s0 + each; s0 < end; s0 += 64) {
+        c = s0 + lane < end ? seq_tiles(cu, nseq, s0 + lane) : 0;
+        b = before(c);
+        hit = __ballot(t >= b && t - b < c);
+        if (hit) {
+            l = __ffsll(static_cast<unsigned long long>(hit)) - 1;
+            const int tiles = __builtin_amdgcn_readlane(c, l);
+            return {s0 + l, tiles - 1 - (t - __builtin_amdgcn_readlane(b, l)), tiles};
+        }
+        t -= lanes_sum(c);
+    }
+    return {-1, 0, 0};
+}
+
 // Query-resident kernels: heads of a group next to each other in the order of
 // workgroups modulo 8 (the XCDs), long causal tiles first; w.share of `shares` of the keys.
 __device__ __forceinline__ Where where_q(const AttnTrainParams &p, int shares)
 {
     Where w;
-    const int nbh = p.nseq * p.H;
+    const int nbh = (p.ranked ? 1 : p.nseq) * p.H;
     const int ts = blockIdx.x / nbh, j = blockIdx.x - ts * nbh;
-    const int t = ts / shares;
+    const int tiles = p.ranked ? static_cast<int>(p.q_tiles) : p.tiles;
+    int t = ts / shares;
     w.share = ts - t * shares;
     w.s = j / p.H;
     const int jh = j - w.s * p.H;
     w.g = jh % p.G;
     w.h = w.g * (p.H / p.G) + jh / p.G;
-    w.tile = p.tiles - 1 - snake(t, p.tiles, nbh * shares);
+    t = snake(t, tiles, nbh * shares);
+    w.tile = tiles - 1 - t;
+    if (p.ranked) {
+        const Packed x = packed_tile(p.cu, p.nseq, p.tiles, t);
+        w.s = x.s < 0 ? 0 : x.s;
+        w.tile = x.s < 0 ? p.tiles : x.level;
+    }
     where_rows(p, w);
     return w;
 }
@@ -696,13 +799,18 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dkv_kernel(AttnTrainParams p)
     const int n = lane & 31, h = lane >> 5;
     const int rb = row_base<D>(lane), cb = col_base<D>(lane);
     Where w;
-    const int nbg = p.nseq * p.G, qpk = p.H / p.G;
+    const int nbg = (p.ranked ? 1 : p.nseq) * p.G, qpk = p.H / p.G;
     const int ts = blockIdx.x / nbg;
     w.tile = ts / p.splits;
     const int share = ts - w.tile * p.splits;
     const int jg = blockIdx.x - ts * nbg;
     w.s = jg / p.G;
     w.g = jg - w.s * p.G;
+    if (p.ranked) {
+        const Packed x = packed_tile(p.cu, p.nseq, p.tiles, w.tile);
+        w.s = x.s < 0 ? 0 : x.s;
+        w.tile = x.s < 0 ? p.tiles : x.tiles - 1 - x.level;
+    }
     w.h = w.g * qpk;
     where_rows(p, w);
     const int n0 = w.tile * BN;
@@ -905,13 +1013,30 @@ hipError_t sum_shares(const float *part, int64_t stride, int n, void *out, int64
 // more evenly (forward, B1 T4096 H16 D64: 72 us against 87; packed, 9 sequences of
 // 7013 tokens, H16 D128: 78 against 97; B2 T8192 H16 D128: 556 against 574).
 constexpr int kWaves = 4;
+static_assert(32 * kWaves == 128, "q_tiles, k_tiles and packed_tile count tiles of 128 rows");
+
+// Tiles of one head, each sequence having as many as the longest, or looked up.  A
+// workgroup without a tile ends after 0.7 ns of the card's time, a lookup costs it 2
+// (hundreds of sequences) to 6 (thousands).  H16 G4 D128, forward and backward, looked
+// up against not: one document of 16384 tokens among 400 of 20 .. 200 (51000 against 900
+// tiles) 7030 us against 8102; 1000 of 20 .. 100 (1000, all of them there; H16 G16 D64)
+// 1146 against 794; 9 of 259 .. 1348 (99 against 62) 327 against 324.
+bool packed_ranked(const AttnTrainParams &p)
+{
+    return p.cu && static_cast<int64_t>(p.nseq) * ((p.max_q + 127) / 128) > 8 * p.q_tiles;
+}
+int64_t grid_tiles(const AttnTrainParams &p, int64_t all)
+{
+    return p.cu && !p.ranked ? static_cast<int64_t>(p.nseq) * p.tiles : all;
+}
 
 template <PrecKind PK, int D>
 hipError_t fwd_d(AttnTrainParams p, hipStream_t s)
 {
     p.tiles = (p.max_q + 32 * kWaves - 1) / (32 * kWaves);
+    p.ranked = packed_ranked(p);
     hipLaunchKernelGGL((attn_fwd_kernel<PK, D, kWaves>),
-                       dim3(static_cast<unsigned>(p.tiles) * p.nseq * p.H * p.splits_f), dim3(64 * kWaves), 0, s, p);
+                       dim3(static_cast<unsigned>(grid_tiles(p, p.q_tiles)) * p.H * p.splits_f), dim3(64 * kWaves), 0, s, p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits_f == 1) return e;
     const int64_t threads = static_cast<int64_t>(p.B) * p.Tq * p.H * (D / 4);
@@ -928,10 +1053,11 @@ hipError_t bwd_d(AttnTrainParams p, hipStream_t s)
         hipLaunchKernelGGL((norm_max_kernel<D>), dim3(kNormParts * p.B * (p.H + p.G)), dim3(256), 0, s, p);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
+    p.tiles = (p.max_q + 32 * kWaves - 1) / (32 * kWaves);
+    p.ranked = packed_ranked(p);
     if (p.Tq > 0 && p.max_q > 0) {
-        p.tiles = (p.max_q + 32 * kWaves - 1) / (32 * kWaves);
         hipLaunchKernelGGL((attn_dq_kernel<PK, D, kWaves>),
-                           dim3(static_cast<unsigned>(p.tiles) * p.nseq * p.H * p.splits_q), dim3(64 * kWaves), 0, s, p);
+                           dim3(static_cast<unsigned>(grid_tiles(p, p.q_tiles)) * p.H * p.splits_q), dim3(64 * kWaves), 0, s, p);
         if ((e = hipGetLastError()) != hipSuccess) return e;
         const int64_t all = static_cast<int64_t>(p.B) * p.Tq * p.H * D;
         if (p.splits_q > 1 && (e = sum_shares<PK>(p.part_q, all, p.splits_q, p.dq, all, s)) != hipSuccess) return e;
@@ -940,9 +1066,8 @@ hipError_t bwd_d(AttnTrainParams p, hipStream_t s)
         // Query rows per tile: at D = 128 half of the other's, so that two
         // workgroups' tiles and V rows fit a CU's LDS.
         constexpr int BQ = D == 64 ? 64 : 32;
-        const int tiles = ((p.cu ? p.max_q : p.Tk) + 32 * kWaves - 1) / (32 * kWaves);
         hipLaunchKernelGGL((attn_dkv_kernel<PK, D, kWaves, BQ>),
-                           dim3(static_cast<unsigned>(tiles) * p.nseq * p.G * p.splits), dim3(64 * kWaves), 0, s, p);
+                           dim3(static_cast<unsigned>(grid_tiles(p, p.k_tiles)) * p.G * p.splits), dim3(64 * kWaves), 0, s, p);
         if ((e = hipGetLastError()) != hipSuccess) return e;
         const int64_t all = static_cast<int64_t>(p.B) * p.Tk * p.G * D;
         if (p.splits > 1) {

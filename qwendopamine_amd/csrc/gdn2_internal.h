@@ -329,7 +329,9 @@ struct AttnTrainParams {
     int nseq;                // B without cu
     int max_q;               // longest sequence's queries
     int64_t q_tiles, k_tiles;  // tiles of 128 queries, keys, over all sequences (one head)
-    int tiles;               // set by the launcher
+    // Set by the launcher: tiles of the longest sequence, and whether a workgroup of
+    // packed sequences looks its tile up (rows of unequal lengths).
+    int tiles, ranked;
     int B, Tq, Tk, H, G, D;
     int causal;
     float scale;

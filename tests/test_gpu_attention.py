@@ -130,6 +130,19 @@ def test_attention_packed(gpu_device, cu, causal):
     assert all(torch.equal(got[n], on_device[n]) for n in got)
 
 
+@pytest.mark.parametrize("n,longest", [(70, 1500), (256, 300), (256, 2000), (257, 2000), (4200, 2600)])
+def test_attention_many_packed_sequences(gpu_device, n, longest):
+    """Empty, single-token and short sequences around one long one: each tile is found once."""
+    print(f"[case] attention {n} packed sequences", flush=True)
+    lens = [(i * 7) % 3 if n > 1000 else (i * i * 13) % 140 if i % 4 else 0 for i in range(n)]
+    lens[n // 2] = longest
+    cu = [0]
+    for x in lens:
+        cu.append(cu[-1] + x)
+    x = _inputs(gpu_device, 1, cu[-1], cu[-1], 2, 1, 64, BF, seed=n)
+    _check(_run(*x, cu_seqlens=torch.tensor(cu)), *x, cu=cu)
+
+
 def test_attention_shared_keys_of_padded_rows(gpu_device):
     """Key shares past a row's length hold nothing; a row of no keys gives zeros."""
     lens = [0, 1, 700, 1600]
