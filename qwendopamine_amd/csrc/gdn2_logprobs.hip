@@ -364,17 +364,29 @@ __global__ __launch_bounds__(64) void logp_merge_kernel(LogprobParams p)
     a = wave_merge(a);
     Top top = {s_list, 0, p.top, -INFINITY, true};
     if constexpr (TOP) {
+        // kB keys per lane at a time, requested together; the bound from the first of
+        // them (the k-th largest of some is at most that of all) filters every one.
+        constexpr int kB = 16;
         const u64 *src = p.part_top + row * p.parts * p.top;
         const int n = p.parts * p.top;
-        u64 best = 0;  // the lane's largest
-        for (int i = lane; i < n; i += 64) {
-            const u64 key = src[i];
-            best = key > best ? key : best;
-        }
-        const u64 thr = static_cast<u64>(kth_bound(static_cast<unsigned>(best >> 32), p.top)) << 32;
-        for (int i0 = 0; i0 < n; i0 += 64) {
-            const u64 key = i0 + lane < n ? src[i0 + lane] : 0;
-            push(top, key != 0 && key >= thr, key, lane);
+        u64 thr = 1;  // 0 is no element
+        for (int i0 = 0; i0 < n; i0 += 64 * kB) {
+            u64 key[kB];
+#pragma unroll
+            for (int b = 0; b < kB; ++b) {
+                const int i = i0 + 64 * b + lane;
+                key[b] = src[i < n ? i : n - 1];
+                if (i >= n) key[b] = 0;
+            }
+            if (i0 == 0) {
+                u64 best = 0;  // the lane's largest
+#pragma unroll
+                for (int b = 0; b < kB; ++b) best = key[b] > best ? key[b] : best;
+                const u64 t = static_cast<u64>(kth_bound(static_cast<unsigned>(best >> 32), p.top)) << 32;
+                thr = t > thr ? t : thr;
+            }
+#pragma unroll
+            for (int b = 0; b < kB; ++b) push(top, key[b] >= thr, key[b], lane);
         }
         keep_best(top, lane);
     }
