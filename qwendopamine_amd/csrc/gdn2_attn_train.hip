@@ -117,27 +117,38 @@ __device__ __forceinline__ Stream stream_of(const uint16_t *base, int64_t ts, in
 
 // One tile, row0 .. row0 + ROWS - 1 of nrows rows, requested into LDS.  Rows past the
 // end repeat the last row (never out of bounds, never another sequence's row);
-// the scores of such rows are hidden.
+// the scores of such rows are hidden.  Buffer requests: they take a tile's scalar base,
+// a lane's offset and a request's scalar one as they are, and unlike flat ones leave
+// the counts of outstanding LDS reads exact.
 template <int D, int NW, int ROWS = kTile>
 __device__ __forceinline__ void stage(const Stream &x, int row0, int nrows, char *lds, int wave, int lane)
 {
     constexpr int P = D / 8, R = 64 / P, IT = ROWS / R;  // requests per tile
     static_assert(IT % NW == 0, "every wave issues as many requests");
-    const char *tile = x.base + row0 * x.ts;
+#ifdef __HIP_DEVICE_COMPILE__  // the host's pass does not know the builtins' types
+    typedef __attribute__((address_space(3))) char *lds_ptr;
+    const uint64_t at = reinterpret_cast<uint64_t>(x.base + row0 * x.ts);
+    const uint64_t tile = static_cast<uint64_t>(__builtin_amdgcn_readfirstlane(static_cast<unsigned>(at >> 32))) << 32 |
+                          static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<unsigned>(at)));
+    // Raw buffer, 32-bit elements, offsets up to 2^32 (63 rows of at most 2^26 bytes).
+    const __amdgpu_buffer_rsrc_t rsrc =
+        __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void *>(tile), 0, 0xffffffffu, 0x00020000);
+    const unsigned ts = static_cast<unsigned>(x.ts);
     if (row0 + ROWS <= nrows) {
 #pragma unroll
         for (int it = 0; it < IT / NW; ++it)
-            __builtin_amdgcn_global_load_lds(reinterpret_cast<const char *>(tile + it * (NW * R) * x.ts + x.lane_off),
-                                             lds + (it * NW + wave) * 1024, 16, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr)(lds + (it * NW + wave) * 1024), 16, x.lane_off,
+                                                     it * (NW * R) * ts, 0, 0);
     } else {
 #pragma unroll
         for (int it = 0; it < IT / NW; ++it) {
             const int r = (it * NW + wave) * R + lane / P;
             const int rc = row0 + r < nrows ? r : nrows - 1 - row0;
-            __builtin_amdgcn_global_load_lds(reinterpret_cast<const char *>(tile + rc * x.ts + ((lane % P) ^ swz<D>(r)) * 16),
-                                             lds + (it * NW + wave) * 1024, 16, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr)(lds + (it * NW + wave) * 1024), 16,
+                                                     rc * ts + ((lane % P) ^ swz<D>(r)) * 16, 0, 0, 0);
         }
     }
+#endif
 }
 
 // A lane's byte offset within a tile for row reads (row l & 31, its half of the
@@ -400,9 +411,10 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(AttnTrainParams p)
 {
     constexpr int KS = D / 16, DT = D / 32, BM = 32 * NW;
     constexpr int kBytes = kTile * D * 2;
-    __shared__ __align__(256) char smem[4 * kBytes];  // two tiles of k, two of v
-    auto tile_k = [&](int t) __attribute__((always_inline)) { return smem + (t & 1) * kBytes; };
-    auto tile_v = [&](int t) __attribute__((always_inline)) { return smem + (2 + (t & 1)) * kBytes; };
+    // Two tiles of k and of v, each an array of its own: reads of one and requests into
+    // another are then known not to meet.  In one array the compiler waited for
+    // the request of the next tile before the first read of this one.
+    __shared__ __align__(256) char sk0[kBytes], sk1[kBytes], sv0[kBytes], sv1[kBytes];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, h = lane >> 5;
     const int rb = row_base<D>(lane), cb = col_base<D>(lane);
@@ -442,25 +454,27 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(AttnTrainParams p)
     const int first = static_cast<int>(static_cast<int64_t>(all) * w.share / p.splits_f);
     const int nt = static_cast<int>(static_cast<int64_t>(all) * (w.share + 1) / p.splits_f);
     if (first < nt) {
-        stage<D, NW>(ks, first * kTile, w.nk, tile_k(first), wave, lane);
-        stage<D, NW>(vs, first * kTile, w.nk, tile_v(first), wave, lane);
+        stage<D, NW>(ks, first * kTile, w.nk, sk0, wave, lane);
+        stage<D, NW>(vs, first * kTile, w.nk, sv0, wave, lane);
     }
-    for (int t = first; t < nt; ++t) {
+    auto step = [&](int t, auto buf) __attribute__((always_inline)) {
+        constexpr bool kOdd = decltype(buf)::value;
+        const char *const tk = kOdd ? sk1 : sk0, *const tv = kOdd ? sv1 : sv0;
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();  // tile t has landed, and every wave is done with tile t - 1
         if (t + 1 < nt) {
-            stage<D, NW>(ks, (t + 1) * kTile, w.nk, tile_k(t + 1), wave, lane);
-            stage<D, NW>(vs, (t + 1) * kTile, w.nk, tile_v(t + 1), wave, lane);
+            stage<D, NW>(ks, (t + 1) * kTile, w.nk, kOdd ? sk0 : sk1, wave, lane);
+            stage<D, NW>(vs, (t + 1) * kTile, w.nk, kOdd ? sv0 : sv1, wave, lane);
         }
         const int j0 = t * kTile;
-        if (j0 >= wend) continue;
-        const int kr = opaque(rb + (t & 1) * kBytes), vc = opaque(cb + (2 + (t & 1)) * kBytes);
+        if (j0 >= wend) return;
+        const int kr = opaque(rb), vc = opaque(cb);
         f32x16 s[2];
 #pragma unroll
         for (int a = 0; a < 2; ++a) {
             s[a] = zero16();
 #pragma unroll
-            for (int st = 0; st < KS; ++st) s[a] = mma32<PK>(s[a], row_frag<D>(smem, kr, 32 * a, st), qf[st]);
+            for (int st = 0; st < KS; ++st) s[a] = mma32<PK>(s[a], row_frag<D>(tk, kr, 32 * a, st), qf[st]);
         }
         if (j0 + kTile > wlim) {
             hide<true>(s[0], j0, h, lim);
@@ -513,8 +527,12 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(AttnTrainParams p)
             for (int u = 0; u < 2; ++u) {
                 const uint4 pf = pack8<PK>(s[a], u);
 #pragma unroll
-                for (int d = 0; d < DT; ++d) acc[d] = mma32<PK>(acc[d], col_frag<D>(smem, vc, 32 * a + 16 * u, d), pf);
+                for (int d = 0; d < DT; ++d) acc[d] = mma32<PK>(acc[d], col_frag<D>(tv, vc, 32 * a + 16 * u, d), pf);
             }
+    };
+    for (int t = first; t < nt; t += 2) {
+        step(t, std::false_type{});
+        if (t + 1 < nt) step(t + 1, std::true_type{});
     }
     l = half_add(l);
     m = fresh ? kNoMax : m;
@@ -656,9 +674,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dq_kernel(AttnTrainParams p)
 {
     constexpr int KS = D / 16, DT = D / 32, BM = 32 * NW;
     constexpr int kBytes = kTile * D * 2;
-    __shared__ __align__(256) char smem[4 * kBytes];  // two tiles of k, two of v
-    auto tile_k = [&](int t) __attribute__((always_inline)) { return smem + (t & 1) * kBytes; };
-    auto tile_v = [&](int t) __attribute__((always_inline)) { return smem + (2 + (t & 1)) * kBytes; };
+    __shared__ __align__(256) char sk0[kBytes], sk1[kBytes], sv0[kBytes], sv1[kBytes];  // as in the forward
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, h = lane >> 5;
     const int rb = row_base<D>(lane), cb = col_base<D>(lane);
@@ -723,27 +739,28 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dq_kernel(AttnTrainParams p)
     const int first = static_cast<int>(static_cast<int64_t>(all) * w.share / p.splits_q);
     const int nt = static_cast<int>(static_cast<int64_t>(all) * (w.share + 1) / p.splits_q);
     if (first < nt) {
-        stage<D, NW>(ks, first * kTile, w.nk, tile_k(first), wave, lane);
-        stage<D, NW>(vs, first * kTile, w.nk, tile_v(first), wave, lane);
+        stage<D, NW>(ks, first * kTile, w.nk, sk0, wave, lane);
+        stage<D, NW>(vs, first * kTile, w.nk, sv0, wave, lane);
     }
-    for (int t = first; t < nt; ++t) {
+    auto step = [&](int t, auto buf) __attribute__((always_inline)) {
+        constexpr bool kOdd = decltype(buf)::value;
+        const char *const tk = kOdd ? sk1 : sk0, *const tv = kOdd ? sv1 : sv0;
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
         if (t + 1 < nt) {
-            stage<D, NW>(ks, (t + 1) * kTile, w.nk, tile_k(t + 1), wave, lane);
-            stage<D, NW>(vs, (t + 1) * kTile, w.nk, tile_v(t + 1), wave, lane);
+            stage<D, NW>(ks, (t + 1) * kTile, w.nk, kOdd ? sk0 : sk1, wave, lane);
+            stage<D, NW>(vs, (t + 1) * kTile, w.nk, kOdd ? sv0 : sv1, wave, lane);
         }
         const int j0 = t * kTile;
-        if (j0 >= wend) continue;
-        const int kr = opaque(rb + (t & 1) * kBytes), vr = opaque(rb + (2 + (t & 1)) * kBytes);
-        const int kc = opaque(cb + (t & 1) * kBytes);
+        if (j0 >= wend) return;
+        const int rr = opaque(rb), kc = opaque(cb);
 #pragma unroll
         for (int a = 0; a < 2; ++a) {
             f32x16 s = zero16(), dp = zero16();
 #pragma unroll
-            for (int st = 0; st < KS; ++st) s = mma32<PK>(s, row_frag<D>(smem, kr, 32 * a, st), qf[st]);
+            for (int st = 0; st < KS; ++st) s = mma32<PK>(s, row_frag<D>(tk, rr, 32 * a, st), qf[st]);
 #pragma unroll
-            for (int st = 0; st < KS; ++st) dp = mma32<PK>(dp, row_frag<D>(smem, vr, 32 * a, st), df[st]);
+            for (int st = 0; st < KS; ++st) dp = mma32<PK>(dp, row_frag<D>(tv, rr, 32 * a, st), df[st]);
             if (j0 + kTile > wlim) hide<true>(s, j0 + 32 * a, h, lim);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -754,9 +771,13 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dq_kernel(AttnTrainParams p)
             for (int u = 0; u < 2; ++u) {
                 const uint4 pf = pack8<PK>(s, u);
 #pragma unroll
-                for (int d = 0; d < DT; ++d) acc[d] = mma32<PK>(acc[d], col_frag<D>(smem, kc, 32 * a + 16 * u, d), pf);
+                for (int d = 0; d < DT; ++d) acc[d] = mma32<PK>(acc[d], col_frag<D>(tk, kc, 32 * a + 16 * u, d), pf);
             }
         }
+    };
+    for (int t = first; t < nt; t += 2) {
+        step(t, std::false_type{});
+        if (t + 1 < nt) step(t + 1, std::true_type{});
     }
     if (qi >= w.nq) return;
     const float f = p.scale / sc;
@@ -791,10 +812,10 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dkv_kernel(AttnTrainParams p)
     // registers is 64 beside 128 of accumulators and 32 of S and dP, and the
     // kernel spilled 59 (B2 T8192 H16 G4, this kernel alone: 3172 us against 1777).
     constexpr bool kVLds = D == 128;
-    // Two tiles of q, two of dout, V's rows, and per tile L and scaled D of its queries.
-    constexpr int kOffV = 4 * kBytes, kOffL = kOffV + (kVLds ? BN * D * 2 : 0);
-    __shared__ __align__(256) char smem[kOffL + 4 * BQ * 4];
-    float *const sl = reinterpret_cast<float *>(smem + kOffL);
+    // Two tiles of q and of dout, V's rows, and per tile L and scaled D of its queries
+    // (arrays of their own, as in the forward).
+    __shared__ __align__(256) char sq0[kBytes], sq1[kBytes], sd0[kBytes], sd1[kBytes], sv[kVLds ? BN * D * 2 : 16];
+    __shared__ __align__(16) float sl0[2 * BQ], sl1[2 * BQ];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, h = lane >> 5;
     const int rb = row_base<D>(lane), cb = col_base<D>(lane);
@@ -868,19 +889,25 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dkv_kernel(AttnTrainParams p)
     const int64_t sb = static_cast<int64_t>(w.bq) * p.H * p.Tq + w.q0;
     int rh = nt > 0 ? x0 / nt : 0, rt = nt > 0 ? x0 - rh * nt : 0;  // of the step requested next
     int ct = rt;                                                    // query tile of the current step
-    auto request = [&](int buf) __attribute__((always_inline)) {
+    // L and D of the queries of a step travel through a register (`next`), stored after
+    // the products of the step before: stored at once, the store would wait for
+    // every tile request ahead of it.
+    float next = 0.0f;
+    auto keep = [&](float *sl) __attribute__((always_inline)) {
+        if (tid < 2 * BQ) sl[tid] = tid < BQ ? next - p16 : next * ds_mul;
+    };
+    auto request = [&](char *tq, char *td) __attribute__((always_inline)) {
         const int hh = w.h + rh, row0 = (t0 + rt) * BQ;
         Stream qh = qs, dh = ds;
         qh.base += 2 * hh * p.qs[2];
         dh.base += 2 * hh * D;
-        stage<D, NW, BQ>(qh, row0, w.nq, smem + buf * kBytes, wave, lane);
-        stage<D, NW, BQ>(dh, row0, w.nq, smem + (2 + buf) * kBytes, wave, lane);
+        stage<D, NW, BQ>(qh, row0, w.nq, tq, wave, lane);
+        stage<D, NW, BQ>(dh, row0, w.nq, td, wave, lane);
         if (tid < 2 * BQ) {
             const int r = row0 + (tid & (BQ - 1));
             const float *src = (tid < BQ ? p.lse : p.delta) + sb + static_cast<int64_t>(hh) * p.Tq;
             // Queries past the end: L = +inf hides them.
-            const float x = r < w.nq ? src[r] : (tid < BQ ? INFINITY : 0.0f);
-            sl[buf * 2 * BQ + tid] = tid < BQ ? x - p16 : x * ds_mul;
+            next = r < w.nq ? src[r] : (tid < BQ ? INFINITY : 0.0f);
         }
         if (++rt == nt) {
             rt = 0;
@@ -888,25 +915,27 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dkv_kernel(AttnTrainParams p)
         }
     };
     if (steps > 0) {
-        request(0);
+        request(sq0, sd0);
         if constexpr (kVLds)
-            stage<D, NW, BN>(stream_of<D, NW>(vb, p.vs[1], wave, lane), n0, w.nk, smem + kOffV, wave, lane);
+            stage<D, NW, BN>(stream_of<D, NW>(vb, p.vs[1], wave, lane), n0, w.nk, sv, wave, lane);
     }
-    for (int x = 0; x < steps; ++x) {
+    auto step = [&](int x, auto buf) __attribute__((always_inline)) {
+        constexpr bool kOdd = decltype(buf)::value;
+        const char *const tq = kOdd ? sq1 : sq0, *const td = kOdd ? sd1 : sd0;
+        keep(kOdd ? sl1 : sl0);
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
-        if (x + 1 < steps) request((x + 1) & 1);
+        if (x + 1 < steps) request(kOdd ? sq0 : sq1, kOdd ? sd0 : sd1);
         const int i0 = (t0 + ct) * BQ;
         if (++ct == nt) ct = 0;
-        if (i0 + BQ <= wfirst) continue;
-        const int qr = opaque(rb + (x & 1) * kBytes), dr = opaque(rb + (2 + (x & 1)) * kBytes);
-        const int qc = opaque(cb + (x & 1) * kBytes), dc = opaque(cb + (2 + (x & 1)) * kBytes);
-        const float *lt = sl + (x & 1) * 2 * BQ, *et = lt + BQ;
+        if (i0 + BQ <= wfirst) return;
+        const int rr = opaque(rb), cc = opaque(cb);
+        const float *const lt = kOdd ? sl1 : sl0, *const et = lt + BQ;
 #pragma unroll
         for (int a = 0; a < BQ / 32; ++a) {
             f32x16 s = zero16(), dp = zero16();
 #pragma unroll
-            for (int st = 0; st < KS; ++st) s = mma32<PK>(s, row_frag<D>(smem, qr, 32 * a, st), kf[st]);
+            for (int st = 0; st < KS; ++st) s = mma32<PK>(s, row_frag<D>(tq, rr, 32 * a, st), kf[st]);
             if (i0 < wall) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
@@ -918,10 +947,10 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dkv_kernel(AttnTrainParams p)
             for (int st = 0; st < KS; ++st) {
                 uint4 bv;
                 if constexpr (kVLds)
-                    bv = row_frag<D>(smem, rb + kOffV, 32 * wave, st);
+                    bv = row_frag<D>(sv, rr, 32 * wave, st);
                 else
                     bv = vf[st];
-                dp = mma32<PK>(dp, row_frag<D>(smem, dr, 32 * a, st), bv);
+                dp = mma32<PK>(dp, row_frag<D>(td, rr, 32 * a, st), bv);
             }
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
@@ -934,7 +963,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dkv_kernel(AttnTrainParams p)
             for (int u = 0; u < 2; ++u) {
                 const uint4 pf = pack8<PK>(s, u);
 #pragma unroll
-                for (int d = 0; d < DT; ++d) dv[d] = mma32<PK>(dv[d], col_frag<D>(smem, dc, 32 * a + 16 * u, d), pf);
+                for (int d = 0; d < DT; ++d) dv[d] = mma32<PK>(dv[d], col_frag<D>(td, cc, 32 * a + 16 * u, d), pf);
             }
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
@@ -948,9 +977,13 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dkv_kernel(AttnTrainParams p)
             for (int u = 0; u < 2; ++u) {
                 const uint4 pf = pack8<PK>(s, u);
 #pragma unroll
-                for (int d = 0; d < DT; ++d) dk[d] = mma32<PK>(dk[d], col_frag<D>(smem, qc, 32 * a + 16 * u, d), pf);
+                for (int d = 0; d < DT; ++d) dk[d] = mma32<PK>(dk[d], col_frag<D>(tq, cc, 32 * a + 16 * u, d), pf);
             }
         }
+    };
+    for (int x = 0; x < steps; x += 2) {
+        step(x, std::false_type{});
+        if (x + 1 < steps) step(x + 1, std::true_type{});
     }
     if (kj >= kall) return;
     const float fk = p.scale / sc, fv = PK == PrecKind::F16 ? ldexpf(1.0f, -14) : 1.0f;
