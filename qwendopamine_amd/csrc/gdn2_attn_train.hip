@@ -898,7 +898,14 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dkv_kernel(AttnTrainParams p)
     }
     const float ds_mul = PK == PrecKind::F16 ? sc * ldexpf(1.0f, -14) : 1.0f;
 
-    // Step x: head x / nt of the group, query tile t0 + x % nt; this share's are x0 .. x0 + steps - 1.
+    // Steps: the first nm query tiles of each head of the group, which not every key of the
+    // workgroup's sees whole, then the others of each head; this share's are x0 .. x0 + steps - 1.
+    // At D = 64 all are taken as the first kind: the second loop costs more than it saves there
+    // (forward and backward, with it and without: B4 T2048 H16 D64 216 and 205 us, B2 T8192 H16
+    // G4 D128 2279 and 2309).
+    const int gall = n0 + BN > w.nk ? big : (p.causal ? n0 + BN - 1 - w.shift : 0);
+    int nm = gall >= w.nq ? nt : (gall + BQ - 1) / BQ - t0;
+    nm = D == 64 ? nt : (nm < 0 ? 0 : nm);
     const int x0 = static_cast<int>(static_cast<int64_t>(nt) * qpk * share / p.splits);
     const int steps = static_cast<int>(static_cast<int64_t>(nt) * qpk * (share + 1) / p.splits) - x0;
     const uint16_t *qb = static_cast<const uint16_t *>(p.q) + w.bq * p.qs[0] + w.q0 * p.qs[1];
@@ -906,8 +913,11 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dkv_kernel(AttnTrainParams p)
     const Stream qs = stream_of<D, NW>(qb, p.qs[1], wave, lane);
     const Stream ds = stream_of<D, NW>(db, static_cast<int64_t>(p.H) * D, wave, lane);
     const int64_t sb = static_cast<int64_t>(w.bq) * p.H * p.Tq + w.q0;
-    int rh = nt > 0 ? x0 / nt : 0, rt = nt > 0 ? x0 - rh * nt : 0;  // of the step requested next
-    int ct = rt;                                                    // query tile of the current step
+    const int masked = nm * qpk - x0;  // steps of the first kind left to this share
+    int lo = masked > 0 ? 0 : nm, hi = masked > 0 ? nm : nt;  // tiles of the kind
+    const int y0 = masked > 0 ? x0 : -masked;
+    int rh = hi > lo ? y0 / (hi - lo) : 0, rt = hi > lo ? lo + y0 - rh * (hi - lo) : 0;  // of the step requested next
+    int ci = 0, ni = 0;  // first query of the current step, and of the one requested last
     // L and D of the queries of a step travel through a register (`next`), stored after
     // the products of the step before: stored at once, the store would wait for
     // every tile request ahead of it.
@@ -917,6 +927,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dkv_kernel(AttnTrainParams p)
     };
     auto request = [&](char *tq, char *td) __attribute__((always_inline)) {
         const int hh = w.h + rh, row0 = (t0 + rt) * BQ;
+        ni = row0;
         Stream qh = qs, dh = ds;
         qh.base += 2 * hh * p.qs[2];
         dh.base += 2 * hh * D;
@@ -928,9 +939,13 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dkv_kernel(AttnTrainParams p)
             // Queries past the end: L = +inf hides them.
             next = r < w.nq ? src[r] : (tid < BQ ? INFINITY : 0.0f);
         }
-        if (++rt == nt) {
-            rt = 0;
-            ++rh;
+        if (++rt == hi) {
+            if (++rh == qpk) {
+                rh = 0;
+                lo = nm;
+                hi = nt;
+            }
+            rt = lo;
         }
     };
     if (steps > 0) {
@@ -938,16 +953,16 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dkv_kernel(AttnTrainParams p)
         if constexpr (kVLds)
             stage<D, NW, BN>(stream_of<D, NW>(vb, p.vs[1], wave, lane), n0, w.nk, sv, wave, lane);
     }
-    auto step = [&](int x, auto buf) __attribute__((always_inline)) {
-        constexpr bool kOdd = decltype(buf)::value;
+    auto step = [&](int x, auto buf, auto hidden) __attribute__((always_inline)) {
+        constexpr bool kOdd = decltype(buf)::value, kHide = decltype(hidden)::value;
         const char *const tq = kOdd ? sq1 : sq0, *const td = kOdd ? sd1 : sd0;
         keep(kOdd ? sl1 : sl0);
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
+        ci = ni;
         if (x + 1 < steps) request(kOdd ? sq0 : sq1, kOdd ? sd0 : sd1);
-        const int i0 = (t0 + ct) * BQ;
-        if (++ct == nt) ct = 0;
-        if (i0 + BQ <= wfirst) return;
+        const int i0 = ci;
+        if (kHide && i0 + BQ <= wfirst) return;
         const int rr = opaque(rb), cc = opaque(cb);
         const float *const lt = kOdd ? sl1 : sl0, *const et = lt + BQ;
 #pragma unroll
@@ -955,7 +970,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dkv_kernel(AttnTrainParams p)
             f32x16 s = zero16(), dp = zero16();
 #pragma unroll
             for (int st = 0; st < KS; ++st) s = mma32<PK>(s, row_frag<D>(tq, rr, 32 * a, st), kf[st]);
-            if (i0 < wall) {
+            if (kHide && i0 < wall) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const int qi = i0 + 32 * a + 8 * (i >> 2) + 4 * h + (i & 3);
@@ -1000,10 +1015,16 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dkv_kernel(AttnTrainParams p)
             }
         }
     };
-    for (int x = 0; x < steps; x += 2) {
-        step(x, std::false_type{});
-        if (x + 1 < steps) step(x + 1, std::true_type{});
+    int x = 0;
+    for (; x < steps && x < masked; x += 2) {
+        step(x, std::false_type{}, std::true_type{});
+        if (x + 1 < steps) step(x + 1, std::true_type{}, std::true_type{});
     }
+    if constexpr (D == 128)
+        for (; x < steps; x += 2) {
+            step(x, std::false_type{}, std::false_type{});
+            if (x + 1 < steps) step(x + 1, std::true_type{}, std::false_type{});
+        }
     if (kj >= kall) return;
     const float fk = p.scale / sc, fv = PK == PrecKind::F16 ? ldexpf(1.0f, -14) : 1.0f;
     const int64_t krow = ((w.bk * static_cast<int64_t>(p.Tk) + w.k0 + kj) * p.G + w.g) * D;
