@@ -86,14 +86,17 @@ __device__ __forceinline__ float half_add(float x)
     return __uint_as_float(s[0]) + __uint_as_float(s[1]);
 }
 
-// LDS tile [rows][D]: a row's 16-byte pieces are permuted by XOR with
-// swz(row), which differs in its upper bits over 4 consecutive rows (a column
-// read touches 4 rows x 2 pieces) and in all of its bits over 8 (a row read
-// touches 8 rows x 1 piece per LDS cycle).
+// LDS tile [rows][D]: a row's 16-byte pieces are permuted by XOR with swz(row).  64
+// banks serve 256 bytes per clock: of a row read 16 lanes (the same piece of 16
+// rows, which must land on 16 places; at D = 64 two rows share the banks, so 8 of each
+// parity), of a column read 32 (4 pieces of 4 rows: at D = 128 the rows must
+// differ in the upper two bits, at D = 64 each two of a parity in the uppermost).  A
+// wave's row read then takes 4.8 clocks, a column read 2.9 (8.2 and 4.2 with a
+// conflict in each pair of lanes; all waves of a CU reading).
 template <int D>
 __device__ __forceinline__ int swz(int row)
 {
-    return (((row & 3) << 1) | ((row >> 2) & 1) | (row & 8)) & (D / 8 - 1);
+    return D == 64 ? ((row << 1) & 4) | ((row >> 2) & 3) : ((row << 2) & 12) | ((row >> 2) & 3);
 }
 
 // A streamed matrix: rows ts bytes apart, and this lane's place in a request (its
@@ -168,17 +171,17 @@ __device__ __forceinline__ int col_base(int lane)
 }
 
 // A operand, rows r0 + (l & 31) of the tile, contraction step s of the row (16
-// channels); `at` is row_base plus the tile's place in smem.
+// channels); `at` is row_base.
 template <int D>
-__device__ __forceinline__ uint4 row_frag(const char *smem, int at, int r0, int s)
+__device__ __forceinline__ uint4 row_frag(const char *tile, int at, int r0, int s)
 {
-    return *reinterpret_cast<const uint4 *>(smem + r0 * (2 * D) + (at ^ (32 * s)));
+    return *reinterpret_cast<const uint4 *>(tile + r0 * (2 * D) + (at ^ (32 * s)));
 }
 
 // A operand of the transposed tile: channels 32 dt + (l & 31), contraction
-// over rows r0 + {4 h + 0..3, 8 + 4 h + 0..3}; `at` is col_base plus the tile's place.
+// over rows r0 + {4 h + 0..3, 8 + 4 h + 0..3}; `at` is col_base.
 template <int D>
-__device__ __forceinline__ uint4 col_frag(const char *smem, int at, int r0, int dt)
+__device__ __forceinline__ uint4 col_frag(const char *tile, int at, int r0, int dt)
 {
     typedef short s4 __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) s4 *lds_s4;
@@ -186,8 +189,7 @@ __device__ __forceinline__ uint4 col_frag(const char *smem, int at, int r0, int 
 #pragma unroll
     for (int u = 0; u < 2; ++u)
         r[u] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                             (lds_s4)(smem + (r0 + 8 * u) * (2 * D) +
-                                                      (at ^ ((64 * dt) ^ ((128 * u) & (2 * D - 1)))))));
+                                             (lds_s4)(tile + (r0 + 8 * u) * (2 * D) + (at ^ (64 * dt + 32 * u)))));
     return make_uint4(r[0].x, r[0].y, r[1].x, r[1].y);
 }
 
@@ -407,7 +409,7 @@ __device__ __forceinline__ void store_o(uint16_t *o, uint16_t *ol, float a, floa
 }
 
 template <PrecKind PK, int D, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(AttnTrainParams p)
+__global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void attn_fwd_kernel(AttnTrainParams p)
 {
     constexpr int KS = D / 16, DT = D / 32, BM = 32 * NW;
     constexpr int kBytes = kTile * D * 2;
@@ -678,7 +680,7 @@ __device__ __forceinline__ float ds_scale(const AttnTrainParams &p, const Where 
 // dQ: queries resident, one pass over the keys.  Also forms D = dO . (O + what its
 // rounding left out) per query, which the kernel below reads.
 template <PrecKind PK, int D, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void attn_dq_kernel(AttnTrainParams p)
+__global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void attn_dq_kernel(AttnTrainParams p)
 {
     constexpr int KS = D / 16, DT = D / 32, BM = 32 * NW;
     constexpr int kBytes = kTile * D * 2;
@@ -786,8 +788,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dq_kernel(AttnTrainParams p)
         }
     };
     // Pairs of tiles that every query of the workgroup sees, then the others.  At D = 64 one loop
-    // for all: its 126 registers leave room for four waves per SIMD, which count for more
-    // than the masks' branches (B4 T2048 H16: 67 us against 72 with both loops).
+    // for all: within 128 registers four waves fit a SIMD, which count for more than the
+    // masks' branches (B4 T2048 H16: 67 us against 72 with both loops and three waves).
     int t = first;
     if constexpr (D == 128)
         for (; (t + 2) * kTile <= glim; t += 2) {
@@ -1089,8 +1091,8 @@ hipError_t sum_shares(const float *part, int64_t stride, int n, void *out, void 
 
 // Four waves per workgroup, two workgroups per CU: against eight waves and one, the
 // same time on long rows and less on short ones, whose few workgroups fill the card
-// more evenly (forward, B1 T4096 H16 D64: 72 us against 87; packed, 9 sequences of
-// 7013 tokens, H16 D128: 78 against 97; B2 T8192 H16 D128: 556 against 574).
+// more evenly (forward, with the first tiles: B1 T4096 H16 D64 72 us against 87; packed, 9
+// sequences of 7013 tokens, H16 D128 78 against 97; B2 T8192 H16 D128 556 against 574).
 constexpr int kWaves = 4;
 static_assert(32 * kWaves == 128, "q_tiles, k_tiles and packed_tile count tiles of 128 rows");
 
@@ -1166,7 +1168,7 @@ bool attn_train_supported(int io_dtype, int D)
 // fill the card, and causal ones, of unequal length, even out over two rounds with
 // the longest first.  Fewer are split, as long as a share keeps 16 query tiles of 64 (a
 // shorter one is over before its start and its sums' traffic are paid).  Backward in
-// us with 1 / 2 / 4 / 8 shares: B2 T8192 H16 G4 D128 causal (512 workgroups)
+// us, with the first tiles, with 1 / 2 / 4 / 8 shares: B2 T8192 H16 G4 D128 causal (512 workgroups)
 // 2314 / 1812 / 1814 / 1913; packed 7013 tokens, H16 G4 D128 (240) 310 / 217 / 184 / 223;
 // B1 T4096 H16 G2 D64 (64) 795 / 456 / 288 / 213; B4 T2048 H16 D64 (1024)
 // 162 / 207 / 274 / 421; B8 T509 H8 D64, not causal (256, 8 tiles each) 53 / 59 / 63 / 80.
