@@ -322,7 +322,7 @@ int gdn2_attn_decode(const void *qkv, const float *cos, const float *sin, int ro
  * gdn2_attn_decode over caches held in 4 bits (the same reference path; the
  * cache format is this library's).  A position's 64-channel group is held as 64
  * codes 0 .. 15 and two bf16 numbers:
- *   minimum = bf16(min x), scale = bf16(max((max x - minimum) / 15, 0)),
+ *   minimum = bf16(min x), scale = bf16(max((max x - minimum) * (1 / 15), 0)),
  *   code = clamp(rint((x - minimum) * (1 / scale)), 0, 15)   (0 if scale is 0)
  * in fp32, every operation rounded by itself; it stands for scale * code +
  * minimum.  A group with a value that is not finite gets NaN for both.

@@ -4,8 +4,9 @@
 // whole prompts.
 //
 // A group of 64 channels shares a minimum and a scale (bf16 each):
-//   min = bf16(min x), scale = bf16((max x - min) / 15), code = rint((x - min) / scale) in 0 .. 15,
-// in fp32 with 1 / scale rounded once, so a code is the same on every path.  What
+//   min = bf16(min x), scale = bf16((max x - min) (1 / 15)), code = rint((x - min) (1 / scale)) in 0 .. 15,
+// in fp32 with both reciprocals rounded once (as torch divides by a number on the
+// GPU), so a code is the same on every path.  What
 // attention sees is scale * code + min.
 //
 // Codes enter the matrix products without being converted: a nibble n shifted into
@@ -126,7 +127,7 @@ __device__ __forceinline__ unsigned group_meta(float lo, float hi, bool finite)
 #pragma clang fp contract(off)
     if (!finite) return 0x7fc07fc0u;
     const unsigned mn = f32_to_bf16_bits(lo);
-    const float sc = fmaxf((hi - __uint_as_float(mn << 16)) / 15.0f, 0.0f);
+    const float sc = fmaxf((hi - __uint_as_float(mn << 16)) * (1.0f / 15.0f), 0.0f);
     return f32_to_bf16_bits(sc) | (mn << 16);
 }
 __device__ __forceinline__ float inv_scale(unsigned meta)
@@ -161,7 +162,8 @@ __device__ __forceinline__ int q4_share(const AttnQ4Params &p, int len, int lane
     return (rounds + p.splits - 1) / p.splits * p.round;
 }
 
-// kSub column blocks (1, 2 or 4).
+// kSub column blocks (1, 2 or 4).  B32 of unequal positions up to 32768, H32 G8 D128: 135 us,
+// 4.5 TB/s of codes, scales and minima (a large copy: 4.8); B4 at 2074 of 2304, H16 D64: 7.8 us.
 template <typename T, PrecKind PK, int D, int kSub>
 __global__ __launch_bounds__(64 * kQ4Waves, 2) void attn_q4_kernel(AttnQ4Params p)
 {
@@ -516,7 +518,7 @@ __global__ __launch_bounds__(64 * kQ4Waves, 2) void attn_q4_kernel(AttnQ4Params 
 }
 
 // The shares' partial states of one (sequence, head) per workgroup: weights first
-// (a thread each), then the values, 256 / D threads per channel.
+// (a thread each), then the values, 256 / D threads per channel.  4 to 6 us, its latency.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void attn_q4_merge_kernel(AttnQ4Params p)
 {
@@ -605,6 +607,8 @@ __device__ __forceinline__ void load8(const T *x, float (&v)[8])
     }
 }
 
+// Codes, scales and minima of positions start .. start + T - 1.  B4 T2048 G16 D64 bf16
+// (k and v): 15.1 us, 2.8 TB/s.
 template <typename T>
 __global__ __launch_bounds__(256) void q4_store_kernel(Q4StoreParams p)
 {
@@ -654,7 +658,7 @@ __global__ __launch_bounds__(256) void q4_store_kernel(Q4StoreParams p)
 
 // What positions start .. start + T - 1 stand for, [B, T, G, D] in T (zeros
 // outside the cache).  scale * code has 12 significant bits, so the sum is
-// rounded once with or without fusing.
+// rounded once with or without fusing.  B4 T2048 G16 D64: 9.8 us, 4.4 TB/s.
 template <typename T>
 __global__ __launch_bounds__(256) void q4_load_kernel(Q4LoadParams p)
 {

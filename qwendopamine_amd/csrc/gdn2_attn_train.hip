@@ -408,6 +408,12 @@ __device__ __forceinline__ void store_o(uint16_t *o, uint16_t *ol, float a, floa
     st_q4<PK>(ol, pack4<PK>(z[0], z[1], z[2], z[3]));
 }
 
+// One pass over the keys with the running maximum and sum.  D = 128 is bound by the
+// matrix units (B2 T8192 H16 G4 causal: 516 us, 1065 TFLOP/s; a large library product
+// reaches 1121), D = 64 by vector arithmetic, as a score costs a scaling, a maximum, an
+// exponential of four issue slots, a sum and half a conversion whatever D is (B4
+// T2048 H16 causal: 47 us, 732 TFLOP/s, vector units busy 72% of the time, matrix
+// units 40%).  Few queries over many keys: B1 Tq1 Tk16384 H32 G8 D128, keys in shares, 45 us.
 template <PrecKind PK, int D, int NW>
 __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void attn_fwd_kernel(AttnTrainParams p)
 {
@@ -574,7 +580,9 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void attn_fwd_kernel(Attn
         }
 }
 
-// The shares of a query's keys, in their order; thread: 4 channels of a row.
+// The shares of a query's keys, in their order; thread: 4 channels of a row.  Bound by
+// its launch: it follows at most 512 workgroups' partial results (B1 Tq64 Tk8192 H8
+// D64: 19 us with the kernel above).
 template <PrecKind PK>
 __global__ __launch_bounds__(256) void attn_fwd_join_kernel(AttnTrainParams p)
 {
@@ -678,7 +686,9 @@ __device__ __forceinline__ float ds_scale(const AttnTrainParams &p, const Where 
 }
 
 // dQ: queries resident, one pass over the keys.  Also forms D = dO . (O + what its
-// rounding left out) per query, which the kernel below reads.
+// rounding left out) per query, which the kernel below reads.  Three products a tile:
+// B2 T8192 H16 G4 D128 causal 730 us, 1130 TFLOP/s, the matrix units' rate; B4 T2048
+// H16 D64 66 us, 780 TFLOP/s, vector units busy 57% and matrix units 48%.
 template <PrecKind PK, int D, int NW>
 __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void attn_dq_kernel(AttnTrainParams p)
 {
@@ -823,7 +833,11 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void attn_dq_kernel(AttnT
 
 // dK, dV: keys resident, one pass over the queries of every head of the group,
 // or, where that leaves too few or too uneven workgroups (attn_bwd_splits), over
-// one of p.splits equal shares of it, whose fp32 sums attn_sum_kernel adds.
+// one of p.splits equal shares of it, whose fp32 sums attn_sum_kernel adds.  Four
+// products a tile: B2 T8192 H16 G4 D128 causal 1050 us, 1047 TFLOP/s; B4 T2048 H16 D64
+// 90 us, 764 TFLOP/s, vector and matrix units each busy 43%, two waves per SIMD that wait
+// for each other's products in turn (three, within 168 registers: 84 us, but less
+// even over short rows, B8 T509 H8 63 us for 60 forward and backward).
 template <PrecKind PK, int D, int NW, int BQ>
 __global__ __launch_bounds__(64 * NW, 2) void attn_dkv_kernel(AttnTrainParams p)
 {

@@ -1729,7 +1729,7 @@ def kv_cache_q4_store(cache: KVCacheQ4, k: torch.Tensor, v: torch.Tensor, start:
     outside the cache are not stored; the others of the cache stay as they are.
 
     Per group of 64 channels, in float32 with every operation rounded by itself: the minimum
-    in bf16, ``scale = (max - minimum) / 15`` in bf16, ``code = rint((x - minimum) * (1 / scale))`` within
+    in bf16, ``scale = (max - minimum) * (1 / 15)`` in bf16, ``code = rint((x - minimum) * (1 / scale))`` within
     0 .. 15.  A group with a value that is not finite stands for NaN."""
     name = "kv_cache_q4_store"
     B, G, L, D = _check_q4(name, cache)

@@ -21,7 +21,8 @@ def quantise(x):
     g = x.cpu().float().unflatten(-1, (-1, 64))
     ok = g.isfinite().all(-1, keepdim=True)
     lo = g.amin(-1, keepdim=True).bfloat16()
-    sc = ((g.amax(-1, keepdim=True) - lo.float()) / 15.0).clamp_min(0).bfloat16()
+    fifteenth = torch.tensor(1.0 / 15.0, dtype=F32)
+    sc = ((g.amax(-1, keepdim=True) - lo.float()) * fifteenth).clamp_min(0).bfloat16()
     inv = torch.where(sc.float() > 0, 1.0 / sc.float(), 0.0)
     n = torch.where(ok, ((g - lo.float()) * inv).round().clamp(0, 15), 0.0)
     nan = torch.tensor(float("nan"), dtype=BF)
