@@ -71,6 +71,21 @@ __device__ __forceinline__ uint4 pack8(const f32x16 &x, int t)
     return make_uint4(lo.u.x, lo.u.y, hi.u.x, hi.u.y);
 }
 
+// What pack8 left out of the same elements, rounded in its turn.
+template <PrecKind PK>
+__device__ __forceinline__ uint4 rest8(const f32x16 &x, int t, uint4 hi)
+{
+    Q4<PK> a, b;
+    a.u = make_uint2(hi.x, hi.y);
+    b.u = make_uint2(hi.z, hi.w);
+    float f[4], g[4];
+    unpack4<PK>(a, f);
+    unpack4<PK>(b, g);
+    a = pack4<PK>(x[8 * t] - f[0], x[8 * t + 1] - f[1], x[8 * t + 2] - f[2], x[8 * t + 3] - f[3]);
+    b = pack4<PK>(x[8 * t + 4] - g[0], x[8 * t + 5] - g[1], x[8 * t + 6] - g[2], x[8 * t + 7] - g[3]);
+    return make_uint4(a.u.x, a.u.y, b.u.x, b.u.y);
+}
+
 // The other half's value (lane l ^ 32) combined with this lane's.
 __device__ __forceinline__ float half_max(float x)
 {
@@ -191,6 +206,26 @@ __device__ __forceinline__ uint4 col_frag(const char *tile, int at, int r0, int 
         r[u] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                                              (lds_s4)(tile + (r0 + 8 * u) * (2 * D) + (at ^ (64 * dt + 32 * u)))));
     return make_uint4(r[0].x, r[0].y, r[1].x, r[1].y);
+}
+
+// acc[d] += (columns 32 d .. of the tile)^T X for rows r0 + 16 t .. of it, X the elements 8 t ..
+// 8 t + 7 of x.  X is rounded to the operand type: a relative error of half a step
+// each, as large as the rounding of the result.  Of FINE calls (attn_fine) also what
+// that left out is multiplied.
+template <PrecKind PK, int D, bool FINE>
+__device__ __forceinline__ void add_columns(f32x16 (&acc)[D / 32], const char *tile, int at, int r0, const f32x16 &x)
+{
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const uint4 hi = pack8<PK>(x, t);
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) acc[d] = mma32<PK>(acc[d], col_frag<D>(tile, at, r0 + 16 * t, d), hi);
+        if constexpr (FINE) {
+            const uint4 lo = rest8<PK>(x, t, hi);
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d) acc[d] = mma32<PK>(acc[d], col_frag<D>(tile, at, r0 + 16 * t, d), lo);
+        }
+    }
 }
 
 // Keeps the compiler from forming every step's address before the loop, where
@@ -414,7 +449,7 @@ __device__ __forceinline__ void store_o(uint16_t *o, uint16_t *ol, float a, floa
 // exponential of four issue slots, a sum and half a conversion whatever D is (B4
 // T2048 H16 causal: 47 us, 732 TFLOP/s, vector units busy 72% of the time, matrix
 // units 40%).  Few queries over many keys: B1 Tq1 Tk16384 H32 G8 D128, keys in shares, 45 us.
-template <PrecKind PK, int D, int NW>
+template <PrecKind PK, int D, int NW, bool FINE>
 __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void attn_fwd_kernel(AttnTrainParams p)
 {
     constexpr int KS = D / 16, DT = D / 32, BM = 32 * NW;
@@ -528,17 +563,9 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void attn_fwd_kernel(Attn
                 sum += s[a][i];
             }
         l += sum;
-        // The probabilities are rounded to the operand type for this product
-        // (their sum l is not): a relative error of half a step each, as large
-        // as the rounding of V itself and averaged over the keys.
+        // The probabilities are rounded for this product, their sum l is not.
 #pragma unroll
-        for (int a = 0; a < 2; ++a)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const uint4 pf = pack8<PK>(s[a], u);
-#pragma unroll
-                for (int d = 0; d < DT; ++d) acc[d] = mma32<PK>(acc[d], col_frag<D>(tv, vc, 32 * a + 16 * u, d), pf);
-            }
+        for (int a = 0; a < 2; ++a) add_columns<PK, D, FINE>(acc, tv, vc, 32 * a, s[a]);
     };
     // Pairs of tiles that every query of the workgroup sees, then the others.
     int t = first;
@@ -689,8 +716,8 @@ __device__ __forceinline__ float ds_scale(const AttnTrainParams &p, const Where 
 // rounding left out) per query, which the kernel below reads.  Three products a tile:
 // B2 T8192 H16 G4 D128 causal 730 us, 1130 TFLOP/s, the matrix units' rate; B4 T2048
 // H16 D64 66 us, 780 TFLOP/s, vector units busy 57% and matrix units 48%.
-template <PrecKind PK, int D, int NW>
-__global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void attn_dq_kernel(AttnTrainParams p)
+template <PrecKind PK, int D, int NW, bool FINE>
+__global__ __launch_bounds__(64 * NW, D == 64 && !FINE ? 4 : 2) void attn_dq_kernel(AttnTrainParams p)
 {
     constexpr int KS = D / 16, DT = D / 32, BM = 32 * NW;
     constexpr int kBytes = kTile * D * 2;
@@ -789,12 +816,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void attn_dq_kernel(AttnT
                 const float pr = __builtin_amdgcn_exp2f(fmaf(s[i], c, -lse));
                 s[i] = pr * fmaf(dp[i], sc, -dl);
             }
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const uint4 pf = pack8<PK>(s, u);
-#pragma unroll
-                for (int d = 0; d < DT; ++d) acc[d] = mma32<PK>(acc[d], col_frag<D>(tk, kc, 32 * a + 16 * u, d), pf);
-            }
+            add_columns<PK, D, FINE>(acc, tk, kc, 32 * a, s);
         }
     };
     // Pairs of tiles that every query of the workgroup sees, then the others.  At D = 64 one loop
@@ -838,7 +860,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void attn_dq_kernel(AttnT
 // 90 us, 764 TFLOP/s, vector and matrix units each busy 43%, two waves per SIMD that wait
 // for each other's products in turn (three, within 168 registers: 84 us, but less
 // even over short rows, B8 T509 H8 63 us for 60 forward and backward).
-template <PrecKind PK, int D, int NW, int BQ>
+template <PrecKind PK, int D, int NW, int BQ, bool FINE>
 __global__ __launch_bounds__(64 * NW, 2) void attn_dkv_kernel(AttnTrainParams p)
 {
     constexpr int KS = D / 16, DT = D / 32, BN = 32 * NW;
@@ -1009,11 +1031,17 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dkv_kernel(AttnTrainParams p)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) s[4 * b + i] = __builtin_amdgcn_exp2f(fmaf(s[4 * b + i], c, -ls[i]));
             }
+            // add_columns, written out: through it the compiler spilled 13 registers here and
+            // not 3 (B2 T8192 H16 G4 D128 forward and backward 2320 us against 2269).
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const uint4 pf = pack8<PK>(s, u);
 #pragma unroll
-                for (int d = 0; d < DT; ++d) dv[d] = mma32<PK>(dv[d], col_frag<D>(td, cc, 32 * a + 16 * u, d), pf);
+                for (int d = 0; d < DT; ++d) {
+                    const uint4 cf = col_frag<D>(td, cc, 32 * a + 16 * u, d);
+                    dv[d] = mma32<PK>(dv[d], cf, pf);
+                    if constexpr (FINE) dv[d] = mma32<PK>(dv[d], cf, rest8<PK>(s, u, pf));
+                }
             }
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
@@ -1027,7 +1055,11 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dkv_kernel(AttnTrainParams p)
             for (int u = 0; u < 2; ++u) {
                 const uint4 pf = pack8<PK>(s, u);
 #pragma unroll
-                for (int d = 0; d < DT; ++d) dk[d] = mma32<PK>(dk[d], col_frag<D>(tq, cc, 32 * a + 16 * u, d), pf);
+                for (int d = 0; d < DT; ++d) {
+                    const uint4 cf = col_frag<D>(tq, cc, 32 * a + 16 * u, d);
+                    dk[d] = mma32<PK>(dk[d], cf, pf);
+                    if constexpr (FINE) dk[d] = mma32<PK>(dk[d], cf, rest8<PK>(s, u, pf));
+                }
             }
         }
     };
@@ -1125,12 +1157,23 @@ int64_t grid_tiles(const AttnTrainParams &p, int64_t all)
     return p.cu && !p.ranked ? static_cast<int64_t>(p.nseq) * p.tiles : all;
 }
 
+// Whether P and dS are multiplied in two parts.  In short sequences few rounded terms make
+// up a gradient, and one of them shows in D values of it: rounded once, the error
+// of dk against 64 bits is 2.8 times that of rounding the exact result at 2 tokens, 1.6 at
+// 8, 1.5 at 64 and below 1.5 past 128; in two parts it is the same as that.  The products
+// they add are cheap there: forward and backward in two parts and in one, B64 T64 H8 D64
+// 27.2 and 26.2 us, B256 T128 H16 D64 366 and 359, B64 T128 H16 G4 D128 124 and 121.
+bool attn_fine(const AttnTrainParams &p)
+{
+    return p.max_q <= 128 && (p.cu || p.Tk <= 128);
+}
+
 template <PrecKind PK, int D>
 hipError_t fwd_d(AttnTrainParams p, hipStream_t s)
 {
     p.tiles = (p.max_q + 32 * kWaves - 1) / (32 * kWaves);
     p.ranked = packed_ranked(p);
-    hipLaunchKernelGGL((attn_fwd_kernel<PK, D, kWaves>),
+    hipLaunchKernelGGL((attn_fine(p) ? attn_fwd_kernel<PK, D, kWaves, true> : attn_fwd_kernel<PK, D, kWaves, false>),
                        dim3(static_cast<unsigned>(grid_tiles(p, p.q_tiles)) * p.H * p.splits_f), dim3(64 * kWaves), 0, s, p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits_f == 1) return e;
@@ -1151,7 +1194,7 @@ hipError_t bwd_d(AttnTrainParams p, hipStream_t s)
     p.tiles = (p.max_q + 32 * kWaves - 1) / (32 * kWaves);
     p.ranked = packed_ranked(p);
     if (p.Tq > 0 && p.max_q > 0) {
-        hipLaunchKernelGGL((attn_dq_kernel<PK, D, kWaves>),
+        hipLaunchKernelGGL((attn_fine(p) ? attn_dq_kernel<PK, D, kWaves, true> : attn_dq_kernel<PK, D, kWaves, false>),
                            dim3(static_cast<unsigned>(grid_tiles(p, p.q_tiles)) * p.H * p.splits_q), dim3(64 * kWaves), 0, s, p);
         if ((e = hipGetLastError()) != hipSuccess) return e;
         const int64_t all = static_cast<int64_t>(p.B) * p.Tq * p.H * D;
@@ -1161,7 +1204,8 @@ hipError_t bwd_d(AttnTrainParams p, hipStream_t s)
         // Query rows per tile: at D = 128 half of the other's, so that two
         // workgroups' tiles and V rows fit a CU's LDS.
         constexpr int BQ = D == 64 ? 64 : 32;
-        hipLaunchKernelGGL((attn_dkv_kernel<PK, D, kWaves, BQ>),
+        hipLaunchKernelGGL((attn_fine(p) ? attn_dkv_kernel<PK, D, kWaves, BQ, true>
+                                         : attn_dkv_kernel<PK, D, kWaves, BQ, false>),
                            dim3(static_cast<unsigned>(grid_tiles(p, p.k_tiles)) * p.G * p.splits), dim3(64 * kWaves), 0, s, p);
         if ((e = hipGetLastError()) != hipSuccess) return e;
         const int64_t all = static_cast<int64_t>(p.B) * p.Tk * p.G * D;

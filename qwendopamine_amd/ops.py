@@ -1626,9 +1626,10 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float | 
 
     A query that sees no key gives zeros and passes no gradient.  A key hidden from some queries of
     its row by ``causal`` must be finite, and so must the upstream gradients (0 times infinity is
-    NaN, as in any attention by products).  Scores, softmax statistics and sums are float32; the probabilities, and in the
-    backward their gradients, are rounded to the io dtype for the products.  The gradients have
-    the same bits in every run.  In a HIP graph, capture the forward and backward together with no
+    NaN, as in any attention by products).  Scores, softmax statistics and sums are float32; the
+    probabilities, and in the backward their gradients, are rounded to the io dtype for the
+    products (sequences of up to 128 tokens: multiplied in two parts, with twice the bits).  The
+    gradients have the same bits in every run.  In a HIP graph, capture the forward and backward together with no
     eager autograd graph of the same leaves alive, as torch asks of any captured backward.
     """
     name = "attention"

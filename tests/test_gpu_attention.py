@@ -143,6 +143,23 @@ def test_attention_many_packed_sequences(gpu_device, n, longest):
     _check(_run(*x, cu_seqlens=torch.tensor(cu)), *x, cu=cu)
 
 
+@pytest.mark.parametrize("dt", [BF, FP])
+@pytest.mark.parametrize("T,packed", [(2, False), (5, False), (64, False), (128, False), (128, True)])
+def test_attention_short_sequences_are_as_exact_as_their_rounding(gpu_device, T, packed, dt):
+    """Up to 128 tokens P and dS are multiplied in two parts: 2 x 8 (bf16) significant bits leave
+    2^-17 of a term, against the 2^-9 of the result's rounding, whose root mean square is thus
+    all but the whole error; 1.05 leaves room for results that round the other way."""
+    print(f"[case] attention short T{T} packed={packed} {dt}", flush=True)
+    n = 3
+    shape = (1, n * T) if packed else (n, T)
+    x = _inputs(gpu_device, shape[0], shape[1], shape[1], 4, 2, 64, dt, seed=T)
+    cu = [T * i for i in range(n + 1)] if packed else None
+    got = _run(*x, **(dict(cu_seqlens=torch.tensor(cu)) if packed else {}))
+    for name, e in reference(*x, 0.125, True, cu=cu)[0].items():
+        off, rounding = (got[name].detach().double().cpu() - e).norm(), (e.to(dt).double() - e).norm()
+        assert off <= 1.05 * rounding, (name, float(off / rounding))
+
+
 def test_attention_shared_keys_of_padded_rows(gpu_device):
     """Key shares past a row's length hold nothing; a row of no keys gives zeros."""
     lens = [0, 1, 700, 1600]
