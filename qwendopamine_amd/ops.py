@@ -1629,8 +1629,9 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float | 
     NaN, as in any attention by products).  Scores, softmax statistics and sums are float32; the
     probabilities, and in the backward their gradients, are rounded to the io dtype for the
     products (sequences of up to 128 tokens: multiplied in two parts, with twice the bits).  The
-    gradients have the same bits in every run.  In a HIP graph, capture the forward and backward together with no
-    eager autograd graph of the same leaves alive, as torch asks of any captured backward.
+    gradients have the same bits in every run.  In a HIP graph, capture the forward and backward
+    together with no eager autograd graph of the same leaves alive, as torch asks of any captured
+    backward.
     """
     name = "attention"
     if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape:
