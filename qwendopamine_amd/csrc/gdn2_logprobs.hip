@@ -205,7 +205,7 @@ __device__ __forceinline__ void finish_row(const LogprobParams &p, int64_t row, 
     if (lane == 0) {
         const int64_t t = p.targets[row];
         float lp = 0.0f;
-        if (t >= 0 && t < p.n)
+        if (t >= 0 && t < p.n && t != p.ignore)
             lp = (io<T>::ld(static_cast<const T *>(p.x) + row_offset(p, row), t) - a.m) - ln_s;
         else if (t != p.ignore)
             lp = __uint_as_float(0x7fc00000u);
@@ -408,7 +408,7 @@ __global__ __launch_bounds__(256) void logp_bwd_kernel(LogprobParams p)
     const T *x = static_cast<const T *>(p.x) + row_offset(p, row);
     T *dx = static_cast<T *>(p.dx) + row * p.n;
     const int64_t t = p.targets[row];
-    const bool known = t >= 0 && t < p.n;
+    const bool known = t >= 0 && t < p.n && t != p.ignore;
     float gl = known && p.dlogp ? p.dlogp[row] : 0.0f;
     if (!known && t != p.ignore && p.dlogp) gl = __uint_as_float(0x7fc00000u);
     const float ge = p.dent ? p.dent[row] : 0.0f;

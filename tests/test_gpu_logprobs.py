@@ -22,7 +22,7 @@ def _ref(x, t, dlogp, dent, ignore=-100):
     p = lp.exp()
     plp = torch.where(p == 0, 0.0, p * lp)
     h = -plp.sum(-1)
-    known = (t >= 0) & (t < V)
+    known = (t >= 0) & (t < V) & (t != ignore)
     one = torch.nn.functional.one_hot(t.clamp(0, V - 1), V).double() * known[..., None]
     logp = torch.where(known, (one * torch.where(one > 0, lp, 0.0)).sum(-1), torch.where(t == ignore, 0.0, float("nan")))
     gl = torch.where(known, dlogp.cpu().double(), 0.0)[..., None]
@@ -160,6 +160,18 @@ def test_logprobs_targets(gpu_device):
         x[0] = float("nan")
     r, dx = _run(x, t, 0, gl, torch.zeros_like(ge))
     assert (dx[0] == 0).all()
+
+
+@pytest.mark.parametrize("V", [777, 40000])  # rows of one part, and of several
+def test_logprobs_ignored_token_of_the_vocabulary(gpu_device, V):
+    """``ignore_index`` may be a token, as a padding id is."""
+    x, t, gl, ge = _case(gpu_device, 6, V, BF)
+    t[:] = torch.tensor([0, 5, 0, V - 1, 1, 0])
+    r, dx = _run(x, t, 3, gl, ge, ignore_index=0)
+    assert (r.logprobs[t == 0] == 0).all() and (r.logprobs[t != 0] < 0).all()
+    _check(x, t, r, dx, gl, ge, 0)
+    _, dx = _run(x, t, 0, gl, ignore_index=0)
+    assert (dx[t == 0] == 0).all() and (dx[t != 0] != 0).any(-1).all()
 
 
 def test_logprobs_one_gradient_or_none(gpu_device):
