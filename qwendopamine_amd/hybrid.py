@@ -595,7 +595,7 @@ class GreedyDecoder:
     @torch.no_grad()
     def generate(self, prompt: torch.Tensor, max_new_tokens: int) -> torch.Tensor:
         out, lps = [self.prefill(prompt, max_new_tokens).clone()], []
-        for i in range(max_new_tokens):
+        for i in range(max(max_new_tokens, 1)):  # the prompt gives the first token
             if i > 0:
                 out.append(self.step().clone())
             if self.keep_logprobs is not None:

@@ -76,6 +76,9 @@ def test_loss_ignores_targets_and_repeats(gpu_device):
     targets[:] = -100
     v, g = _grads(m, idx, lambda m, i: m.loss(i, targets))
     assert v == 0 and all((x == 0).all() for x in g.values())
+    targets.random_(0, 3)
+    v, r = m.loss(idx, targets, ignore_index=1), m.token_logprobs(idx, targets).logprobs
+    assert float(v) == pytest.approx(-float(r[targets != 1].mean()), rel=1e-5)
 
 
 def test_scoring(gpu_device):
@@ -124,6 +127,8 @@ def test_decoder_without_alternatives_or_logprobs(gpu_device):
     b = GreedyDecoder(m)
     assert torch.equal(ta, b.generate(prompt, 5)) and b.sequence_logprobs is None
     assert a.sequence_logprobs.logprobs.shape == (1, 5) and a.sequence_logprobs.top_ids is None
+    # The prompt gives a token whatever the number asked for.
+    assert torch.equal(a.generate(prompt, 0), ta[:, :1]) and a.sequence_logprobs.logprobs.shape == (1, 1)
 
 
 def test_four_bit_layer_is_the_operator(gpu_device):
