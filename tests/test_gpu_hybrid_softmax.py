@@ -77,7 +77,8 @@ def test_loss_ignores_targets_and_repeats(gpu_device):
     v, g = _grads(m, idx, lambda m, i: m.loss(i, targets))
     assert v == 0 and all((x == 0).all() for x in g.values())
     targets.random_(0, 3)
-    v, r = m.loss(idx, targets, ignore_index=1), m.token_logprobs(idx, targets).logprobs
+    with torch.no_grad():
+        v, r = m.loss(idx, targets, ignore_index=1), m.token_logprobs(idx, targets).logprobs
     assert float(v) == pytest.approx(-float(r[targets != 1].mean()), rel=1e-5)
 
 
