@@ -267,6 +267,14 @@ __device__ __forceinline__ void where_rows(const AttnTrainParams &p, Where &w)
     }
 }
 
+// Asks the scheduler to alternate LDS reads and matrix products in a block (D = 128, where
+// the products bound it: forward 516 -> 507 us, forward and backward 2250 -> 2196, B2
+// T8192 H16 G4; at D = 64 the backward lost 3%).
+__device__ __forceinline__ void mix_reads()
+{
+    __builtin_amdgcn_iglp_opt(0);
+}
+
 // Order of causal tiles, longest first, as workgroups of equal place in successive
 // rounds over the 256 CUs share a CU: every other round runs backwards, so that
 // a CU's tiles add up to about the same length (`row`: workgroups per tile).
@@ -514,6 +522,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void attn_fwd_kernel(Attn
         const int j0 = t * kTile;
         if (kHide && j0 >= wend) return;
         const int kr = opaque(rb), vc = opaque(cb);
+        if constexpr (D == 128) mix_reads();
         f32x16 s[2];
 #pragma unroll
         for (int a = 0; a < 2; ++a) {
@@ -803,6 +812,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 && !FINE ? 4 : 2) void attn_dq_ker
         const int j0 = t * kTile;
         if (kHide && j0 >= wend) return;
         const int rr = opaque(rb), kc = opaque(cb);
+        if constexpr (D == 128) mix_reads();
 #pragma unroll
         for (int a = 0; a < 2; ++a) {
             f32x16 s = zero16(), dp = zero16();
@@ -1002,6 +1012,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dkv_kernel(AttnTrainParams p)
         const int i0 = ci;
         if (kHide && i0 + BQ <= wfirst) return;
         const int rr = opaque(rb), cc = opaque(cb);
+        if constexpr (D == 128) mix_reads();
         const float *const lt = kOdd ? sl1 : sl0, *const et = lt + BQ;
 #pragma unroll
         for (int a = 0; a < BQ / 32; ++a) {
