@@ -621,29 +621,35 @@ static int fill_attn_sizes(AttnTrainParams &p, const int64_t *cu_host, int num_s
     if (Tq > (1 << 30) || Tk > (1 << 30) || B > (1 << 30) || H > (1 << 20) || D > (1 << 20) || num_seqs > (1 << 30))
         return GDN2_ERR_UNSUPPORTED;
     p.max_q = Tq;
-    p.q_tiles = static_cast<int64_t>(B) * ((Tq + 127) / 128);
+    const int64_t qpk = H / G;
+    if (Tq * qpk > (1 << 30)) return GDN2_ERR_UNSUPPORTED;  // a group's rows are counted in 32 bits
+    while ((static_cast<int64_t>(1) << p.qpk_s) < qpk) ++p.qpk_s;
+    p.qpk_m = static_cast<unsigned>(((static_cast<int64_t>(1) << (31 + p.qpk_s)) + qpk - 1) / qpk);
+    p.q_tiles = B * ((Tq * qpk + 127) / 128);
     p.k_tiles = static_cast<int64_t>(B) * ((Tk + 127) / 128);
     if (cu_host) {
         if (B != 1 || Tq != Tk || num_seqs < 0) return GDN2_ERR_INVALID;
         if (cu_host[0] != 0 || cu_host[num_seqs] != Tq) return GDN2_ERR_INVALID;
         p.max_q = 0;
-        p.k_tiles = 0;
+        p.q_tiles = p.k_tiles = 0;
         for (int i = 0; i < num_seqs; ++i) {
             const int64_t n = cu_host[i + 1] - cu_host[i];
             if (n < 0 || n > Tq) return GDN2_ERR_INVALID;
             if (n > p.max_q) p.max_q = static_cast<int>(n);
+            p.q_tiles += (n * qpk + 127) / 128;
             p.k_tiles += (n + 127) / 128;
         }
-        p.q_tiles = p.k_tiles;
     }
     p.nseq = cu_host ? num_seqs : B;
     p.B = B; p.Tq = Tq; p.Tk = Tk; p.H = H; p.G = G; p.D = D;
     p.causal = causal != 0;
     p.splits = attn_bwd_splits(p);
     p.splits_f = p.splits_q = attn_key_shares(p);
-    // One launch of at most 2^31 - 1 workgroups (packed rows: up to 8 times their tiles).
-    const double tiles = static_cast<double>(p.q_tiles > p.k_tiles ? p.q_tiles : p.k_tiles) * H * (cu_host ? 8 : 1);
-    if (tiles * p.splits > 2147483000.0 || tiles * p.splits_f > 2147483000.0 || static_cast<double>(B) * Tq * H > 17179869184.0 ||
+    // One launch of at most 2^31 - 1 workgroups (packed rows: up to 8 times their tiles; an
+    // eighth more where the last deal of groups is short).
+    const double most = cu_host ? 1.9e9 / 8 : 1.9e9;
+    if (static_cast<double>(p.q_tiles) * G * p.splits_f > most || static_cast<double>(p.k_tiles) * G * p.splits > most ||
+        static_cast<double>(B) * Tq * H > 17179869184.0 ||
         static_cast<double>(B) * (H + G) > 500000000.0 || static_cast<double>(B) * Tk * G * D > 500000000000.0)
         return GDN2_ERR_UNSUPPORTED;
     return GDN2_OK;

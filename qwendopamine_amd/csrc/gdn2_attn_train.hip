@@ -236,9 +236,9 @@ __device__ __forceinline__ int opaque(int x)
     return x;
 }
 
-// What a workgroup works on: head h of sequence s, its rows and their extent.
+// What a workgroup works on: a tile of group g of sequence s, and the sequence's extent.
 struct Where {
-    int s, h, g, tile;
+    int s, g, tile;
     int64_t q0, k0;  // first query / key token within the batch row
     int bq, bk;      // batch row of q and k
     int nq, nk;      // queries, visible keys
@@ -275,16 +275,34 @@ __device__ __forceinline__ void mix_reads()
     __builtin_amdgcn_iglp_opt(0);
 }
 
-// Order of causal tiles, longest first, as workgroups of equal place in successive
-// rounds over the 256 CUs share a CU: every other round runs backwards, so that
-// a CU's tiles add up to about the same length (`row`: workgroups per tile).
-__device__ __forceinline__ int snake(int t, int tiles, int row)
+// Which of `groups` (a sequence's heads that share keys) and of a group's `tiles`, the
+// longest first, workgroup b takes.  Those of equal place in successive rounds over the
+// 256 CUs share a CU, so every other round runs backwards: a CU's tiles then add up to
+// about the same length.
+//   dealt (many rounds): workgroups go to the 8 XCDs in turn, each with an L2 of its own; the
+//     groups are dealt out to them, and an XCD does one group's tiles after the other's,
+//     whose keys it then holds (200 packed documents, 62381 tokens, H16 G4 D128 forward:
+//     257 us, against 296 the other way).  A last deal may be short (group >= groups).
+//   else: all groups' first tiles (of `row` workgroups each), then their second, which mixes
+//     long and short ones better (B4 T2048 H16 D64, one round: 48 us against 54).
+struct Turn {
+    int group, tile;
+};
+__device__ __forceinline__ int backwards(int x, int round, int all)
 {
-    const int m = row < 256 ? 256 / row : 1;  // tiles per round
-    const int c = t / m, base = c * m;
-    if ((c & 1) == 0) return t;
-    const int last = base + m < tiles ? base + m - 1 : tiles - 1;
-    return base + last - t;
+    const int r = x / round, base = r * round;
+    const int last = base + round < all ? base + round - 1 : all - 1;
+    return r & 1 ? base + last - x : x;
+}
+__device__ __forceinline__ Turn turn_of(bool dealt, int b, int groups, int tiles, int row)
+{
+    if (dealt) {
+        const int x = backwards(b >> 3, 32, (groups + 7) / 8 * tiles), g = x / tiles;
+        return {g * 8 + (b & 7), x - g * tiles};
+    }
+    const int x = b / groups, m = groups * row < 256 ? 256 / (groups * row) : 1;  // tiles per round
+    const int t = x / row;
+    return {b - x * groups, backwards(t, m, tiles / row) * row + x - t * row};
 }
 
 template <int CTRL>
@@ -312,19 +330,20 @@ constexpr int kRanked = 256;
 struct Packed {
     int s, level, tiles;  // sequence, and its number of tiles; s < 0: none
 };
-__device__ __forceinline__ int seq_tiles(const int64_t *cu, int nseq, int s)
+__device__ __forceinline__ int seq_tiles(const int64_t *cu, int nseq, int rows, int s)
 {
-    const int64_t n = s < nseq ? cu[s + 1] - cu[s] : 0;
+    const int64_t n = s < nseq ? (cu[s + 1] - cu[s]) * rows : 0;
     return n > 0 ? static_cast<int>((n + 127) >> 7) : 0;
 }
-__device__ __forceinline__ Packed packed_tile(const int64_t *cu, int nseq, int longest, int t)
+// rows: of a token (its query heads in the query-resident kernels, 1 in the other).
+__device__ __forceinline__ Packed packed_tile(const int64_t *cu, int nseq, int rows, int longest, int t)
 {
     const int lane = threadIdx.x & 63;
     if (nseq <= kRanked) {
         constexpr int U = kRanked / 64;
         int n[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) n[u] = 64 * u < nseq ? seq_tiles(cu, nseq, 64 * u + lane) : 0;
+        for (int u = 0; u < U; ++u) n[u] = 64 * u < nseq ? seq_tiles(cu, nseq, rows, 64 * u + lane) : 0;
         auto at_least = [&](int x) {  // tiles of level x and above
             int c = 0;
 #pragma unroll
@@ -363,14 +382,14 @@ __device__ __forceinline__ Packed packed_tile(const int64_t *cu, int nseq, int l
     };
     const int each = (nseq + 63) / 64;
     int c = 0;
-    for (int i = 0; i < each; ++i) c += seq_tiles(cu, nseq, lane * each + i);
+    for (int i = 0; i < each; ++i) c += seq_tiles(cu, nseq, rows, lane * each + i);
     int b = before(c);
     uint64_t hit = __ballot(t >= b && t - b < c);
     if (!hit) return {-1, 0, 0};
     int l = __ffsll(static_cast<unsigned long long>(hit)) - 1;
     t -= __builtin_amdgcn_readlane(b, l);
     for (int s0 = l * each, end = s0 + each; s0 < end; s0 += 64) {
-        c = s0 + lane < end ? seq_tiles(cu, nseq, s0 + lane) : 0;
+        c = s0 + lane < end ? seq_tiles(cu, nseq, rows, s0 + lane) : 0;
         b = before(c);
         hit = __ballot(t >= b && t - b < c);
         if (hit) {
@@ -383,29 +402,49 @@ __device__ __forceinline__ Packed packed_tile(const int64_t *cu, int nseq, int l
     return {-1, 0, 0};
 }
 
-// Query-resident kernels: heads of a group next to each other in the order of
-// workgroups modulo 8 (the XCDs), long causal tiles first; w.share of `shares` of the keys.
+// Query-resident kernels: a group's rows are its queries' heads, row x the head x % qpk of
+// query x / qpk, so that a tile of keys serves every head that reads it (few queries of
+// many heads fill a tile, and causal tiles of 128 rows span 128 / qpk queries: B1 Tq1
+// Tk16384 H32 G8 D128 ROWSON us against ROWSOFF with a workgroup per head).  Long causal
+// tiles first; w.share of `shares` of the keys; w.nq rows.
 __device__ __forceinline__ Where where_q(const AttnTrainParams &p, int shares)
 {
     Where w;
-    const int nbh = (p.ranked ? 1 : p.nseq) * p.H;
-    const int ts = blockIdx.x / nbh, j = blockIdx.x - ts * nbh;
+    const int nbg = (p.ranked ? 1 : p.nseq) * p.G;
     const int tiles = p.ranked ? static_cast<int>(p.q_tiles) : p.tiles;
-    int t = ts / shares;
-    w.share = ts - t * shares;
-    w.s = j / p.H;
-    const int jh = j - w.s * p.H;
-    w.g = jh % p.G;
-    w.h = w.g * (p.H / p.G) + jh / p.G;
-    t = snake(t, tiles, nbh * shares);
+    const Turn u = turn_of(p.dealt, blockIdx.x, nbg, tiles * shares, shares);
+    const int t = u.tile / shares;
+    w.share = u.tile - t * shares;
+    w.s = u.group / p.G;
+    w.g = u.group - w.s * p.G;
     w.tile = tiles - 1 - t;
-    if (p.ranked) {
-        const Packed x = packed_tile(p.cu, p.nseq, p.tiles, t);
+    if (u.group >= nbg) {
+        w.s = 0;
+        w.tile = p.tiles;  // past every sequence's rows
+    } else if (p.ranked) {
+        const Packed x = packed_tile(p.cu, p.nseq, p.H / p.G, p.tiles, t);
         w.s = x.s < 0 ? 0 : x.s;
         w.tile = x.s < 0 ? p.tiles : x.level;
     }
     where_rows(p, w);
     return w;
+}
+
+// A lane's row of a query-resident kernel: its query and head; rows past the end repeat the last.
+struct Row {
+    int q, h;
+};
+// x / qpk, 0 <= x < 2^31: x times m = 2^(31 + s) / qpk rounded up, 2^s >= qpk; the
+// rounding adds less than x 2^s / 2^(31 + s) < 1 / qpk (by division these six of a
+// workgroup took 0.2 us).
+__device__ __forceinline__ int query_of(const AttnTrainParams &p, int x)
+{
+    return static_cast<int>((static_cast<uint64_t>(static_cast<unsigned>(x)) * p.qpk_m) >> (31 + p.qpk_s));
+}
+__device__ __forceinline__ Row row_of(const AttnTrainParams &p, int x, int rows, int g, int qpk)
+{
+    const int c = x < rows ? x : rows - 1, q = query_of(p, c);
+    return {q, g * qpk + (c - q * qpk)};
 }
 
 // exp2 of a tile's scaled scores relative to ref, hidden keys to 0.  keys of
@@ -435,20 +474,17 @@ __device__ __forceinline__ float log_sum(float m, float l)
 // and dP - D cancels.  What is below the sums' own error is dropped: O of a
 // single key is then exactly its V.
 template <PrecKind PK>
-__device__ __forceinline__ void store_o(uint16_t *o, uint16_t *ol, float a, float b, float c, float d)
+__device__ __forceinline__ Q4<PK> left_out(float a, float b, float c, float d)
 {
-    const Q4<PK> r = pack4<PK>(a, b, c, d);
-    st_q4<PK>(o, r);
-    if (!ol) return;
     const float y[4] = {a, b, c, d};
     float z[4];
-    unpack4<PK>(r, z);
+    unpack4<PK>(pack4<PK>(a, b, c, d), z);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         z[e] = y[e] - z[e];
         z[e] = fabsf(z[e]) > 0x1p-18f * fabsf(y[e]) ? z[e] : 0.0f;
     }
-    st_q4<PK>(ol, pack4<PK>(z[0], z[1], z[2], z[3]));
+    return pack4<PK>(z[0], z[1], z[2], z[3]);
 }
 
 // One pass over the keys with the running maximum and sum.  D = 128 is bound by the
@@ -471,13 +507,14 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void attn_fwd_kernel(Attn
     const int rb = row_base<D>(lane), cb = col_base<D>(lane);
     const Where w = where_q(p, p.splits_f);
     const int m0 = w.tile * BM;
-    if (m0 >= w.nq) return;
-    const int qi = m0 + 32 * wave + n;  // this lane's query
-    const int qc = qi < w.nq ? qi : w.nq - 1;
+    const int qpk = p.H / p.G, rows = w.nq * qpk;
+    if (m0 >= rows) return;
+    const int x = m0 + 32 * wave + n;  // this lane's row
+    const Row row = row_of(p, x, rows, w.g, qpk);
     const uint16_t *kb = static_cast<const uint16_t *>(p.k) + w.bk * p.ks[0] + w.k0 * p.ks[1] + w.g * p.ks[2];
     const uint16_t *vb = static_cast<const uint16_t *>(p.v) + w.bk * p.vs[0] + w.k0 * p.vs[1] + w.g * p.vs[2];
     const Stream ks = stream_of<D, NW>(kb, p.ks[1], wave, lane), vs = stream_of<D, NW>(vb, p.vs[1], wave, lane);
-    const uint16_t *qr = static_cast<const uint16_t *>(p.q) + w.bq * p.qs[0] + (w.q0 + qc) * p.qs[1] + w.h * p.qs[2];
+    const uint16_t *qr = static_cast<const uint16_t *>(p.q) + w.bq * p.qs[0] + (w.q0 + row.q) * p.qs[1] + row.h * p.qs[2];
     uint4 qf[KS];
 #pragma unroll
     for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const uint4 *>(qr + 16 * s + 8 * h);
@@ -485,11 +522,11 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void attn_fwd_kernel(Attn
     // Keys of the workgroup, of this wave and of this lane.
     int kend = w.nk;
     if (p.causal) {
-        const int last = (m0 + BM < w.nq ? m0 + BM : w.nq) + w.shift;
+        const int last = query_of(p, (m0 + BM < rows ? m0 + BM : rows) - 1) + 1 + w.shift;
         kend = last < kend ? last : kend;
     }
-    const int lim = p.causal && qi + w.shift + 1 < w.nk ? qi + w.shift + 1 : w.nk;
-    const int wmin = m0 + 32 * wave, wmax = wmin + 31;
+    const int lim = p.causal && row.q + w.shift + 1 < w.nk ? row.q + w.shift + 1 : w.nk;
+    const int wmin = query_of(p, m0 + 32 * wave), wmax = query_of(p, m0 + 32 * wave + 31);
     const int wlim = p.causal && wmin + w.shift + 1 < w.nk ? wmin + w.shift + 1 : w.nk;  // all of the wave see these
     const int wend = p.causal && wmax + w.shift + 1 < w.nk ? wmax + w.shift + 1 : w.nk;  // none sees more
     const float c = p.scale * kLog2e;
@@ -504,7 +541,8 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void attn_fwd_kernel(Attn
     const int all = kend > 0 ? (kend + kTile - 1) / kTile : 0;
     const int first = static_cast<int>(static_cast<int64_t>(all) * w.share / p.splits_f);
     const int nt = static_cast<int>(static_cast<int64_t>(all) * (w.share + 1) / p.splits_f);
-    int glim = p.causal && m0 + w.shift + 1 < w.nk ? m0 + w.shift + 1 : w.nk;  // all of the workgroup see these
+    const int gmin = query_of(p, m0);
+    int glim = p.causal && gmin + w.shift + 1 < w.nk ? gmin + w.shift + 1 : w.nk;  // all of the workgroup see these
     glim = glim < nt * kTile ? glim : nt * kTile;
     if (first < nt) {
         stage<D, NW>(ks, first * kTile, w.nk, sk0, wave, lane);
@@ -588,10 +626,10 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void attn_fwd_kernel(Attn
     }
     l = half_add(l);
     m = fresh ? kNoMax : m;
-    if (qi >= w.nq) return;
-    const int64_t orow = (w.bq * static_cast<int64_t>(p.Tq) + w.q0 + qi) * p.H + w.h;
     if (p.splits_f > 1) {
+        if (x >= rows) return;
         // This share's state; attn_fwd_join_kernel puts the shares together.
+        const int64_t orow = (w.bq * static_cast<int64_t>(p.Tq) + w.q0 + row.q) * p.H + row.h;
         const int64_t at = w.share * (static_cast<int64_t>(p.B) * p.Tq * p.H) + orow;
         if (h == 0) *reinterpret_cast<float2 *>(p.part_ml + 2 * at) = make_float2(m, l);
 #pragma unroll
@@ -603,17 +641,45 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void attn_fwd_kernel(Attn
         return;
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    if (h == 0) p.lse[(static_cast<int64_t>(w.bq) * p.H + w.h) * p.Tq + w.q0 + qi] = log_sum(m, l);
-    uint16_t *o = static_cast<uint16_t *>(p.o) + orow * D;
-    uint16_t *ol = p.o_lo ? static_cast<uint16_t *>(p.o_lo) + orow * D : nullptr;
+    if (h == 0 && x < rows)
+        p.lse[(static_cast<int64_t>(w.bq) * p.H + row.h) * p.Tq + w.q0 + row.q] = log_sum(m, l);
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int e = 32 * d + 8 * i + 4 * h;
-            store_o<PK>(o + e, ol ? ol + e : nullptr, acc[d][4 * i] * inv, acc[d][4 * i + 1] * inv,
-                        acc[d][4 * i + 2] * inv, acc[d][4 * i + 3] * inv);
+        for (int i = 0; i < 16; ++i) acc[d][i] *= inv;
+    // Whole rows are written, through LDS (this wave's 32 rows): eight bytes a row at a time
+    // left lines half written when others took their place in the L2.
+    __syncthreads();  // the tiles are done with
+    char *const so = (wave < 2 ? sk0 : sv0) + (wave & 1) * (32 * 2 * D);
+    constexpr int P = D / 8;
+    auto write = [&](uint16_t *out) __attribute__((always_inline)) {
+#pragma unroll
+        for (int it = 0; it < P / 2; ++it) {
+            const int r = it * (64 / P) + lane / P, xr = m0 + 32 * wave + r;
+            const uint4 v = *reinterpret_cast<const uint4 *>(so + r * (2 * D) + ((lane ^ r) & (P - 1)) * 16);
+            if (xr < rows) {
+                const Row to = row_of(p, xr, rows, w.g, qpk);
+                const int64_t at = ((w.bq * static_cast<int64_t>(p.Tq) + w.q0 + to.q) * p.H + to.h) * D;
+                *reinterpret_cast<uint4 *>(out + at + (lane % P) * 8) = v;
+            }
         }
+    };
+    auto place = [&](int d, int i) __attribute__((always_inline)) {
+        return reinterpret_cast<uint2 *>(so + n * (2 * D) + (((4 * d + i) ^ n) & (P - 1)) * 16 + 8 * h);
+    };
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            *place(d, i) = pack4<PK>(acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]).u;
+    write(static_cast<uint16_t *>(p.o));
+    if (!p.o_lo) return;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            *place(d, i) = left_out<PK>(acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]).u;
+    write(static_cast<uint16_t *>(p.o_lo));
 }
 
 // The shares of a query's keys, in their order; thread: 4 channels of a row.  Bound by
@@ -648,8 +714,9 @@ __global__ __launch_bounds__(256) void attn_fwd_join_kernel(AttnTrainParams p)
         const int64_t b = bt / p.Tq;
         p.lse[(b * p.H + hh) * p.Tq + (bt - b * p.Tq)] = log_sum(m, l);
     }
-    store_o<PK>(static_cast<uint16_t *>(p.o) + e, p.o_lo ? static_cast<uint16_t *>(p.o_lo) + e : nullptr, x.x * inv,
-                x.y * inv, x.z * inv, x.w * inv);
+    const float y[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
+    st_q4<PK>(static_cast<uint16_t *>(p.o) + e, pack4<PK>(y[0], y[1], y[2], y[3]));
+    if (p.o_lo) st_q4<PK>(static_cast<uint16_t *>(p.o_lo) + e, left_out<PK>(y[0], y[1], y[2], y[3]));
 }
 
 // ---------------------------------------------------------------- backward
@@ -705,13 +772,13 @@ __global__ __launch_bounds__(256) void norm_max_kernel(AttnTrainParams p)
 constexpr float kP16 = 14.0f;
 
 template <PrecKind PK>
-__device__ __forceinline__ float ds_scale(const AttnTrainParams &p, const Where &w)
+__device__ __forceinline__ float ds_scale(const AttnTrainParams &p, const Where &w, int head)
 {
     if constexpr (PK != PrecKind::F16) return 1.0f;
     float a = 0.0f, b = 0.0f;
 #pragma unroll
     for (int i = 0; i < kNormParts; ++i) {
-        a = fmaxf(a, p.mx_do[(w.bq * p.H + w.h) * kNormParts + i]);
+        a = fmaxf(a, p.mx_do[(w.bq * p.H + head) * kNormParts + i]);
         b = fmaxf(b, p.mx_v[(w.bk * p.G + w.g) * kNormParts + i]);
     }
     const float bound = 2.0f * sqrtf(a) * sqrtf(b);
@@ -736,23 +803,24 @@ __global__ __launch_bounds__(64 * NW, D == 64 && !FINE ? 4 : 2) void attn_dq_ker
     const int rb = row_base<D>(lane), cb = col_base<D>(lane);
     const Where w = where_q(p, p.splits_q);
     const int m0 = w.tile * BM;
-    if (m0 >= w.nq) return;
-    const int qi = m0 + 32 * wave + n;
-    const int qc = qi < w.nq ? qi : w.nq - 1;
+    const int qpk = p.H / p.G, rows = w.nq * qpk;
+    if (m0 >= rows) return;
+    const int x = m0 + 32 * wave + n;
+    const Row row = row_of(p, x, rows, w.g, qpk);
     const uint16_t *kb = static_cast<const uint16_t *>(p.k) + w.bk * p.ks[0] + w.k0 * p.ks[1] + w.g * p.ks[2];
     const uint16_t *vb = static_cast<const uint16_t *>(p.v) + w.bk * p.vs[0] + w.k0 * p.vs[1] + w.g * p.vs[2];
     const Stream ks = stream_of<D, NW>(kb, p.ks[1], wave, lane), vs = stream_of<D, NW>(vb, p.vs[1], wave, lane);
-    const uint16_t *qr = static_cast<const uint16_t *>(p.q) + w.bq * p.qs[0] + (w.q0 + qc) * p.qs[1] + w.h * p.qs[2];
-    const int64_t orow = ((w.bq * static_cast<int64_t>(p.Tq) + w.q0 + qc) * p.H + w.h) * D;
+    const uint16_t *qr = static_cast<const uint16_t *>(p.q) + w.bq * p.qs[0] + (w.q0 + row.q) * p.qs[1] + row.h * p.qs[2];
+    const int64_t orow = ((w.bq * static_cast<int64_t>(p.Tq) + w.q0 + row.q) * p.H + row.h) * D;
     const uint16_t *dr = static_cast<const uint16_t *>(p.dout) + orow;
-    const int64_t srow = (static_cast<int64_t>(w.bq) * p.H + w.h) * p.Tq + w.q0 + qc;
+    const int64_t srow = (static_cast<int64_t>(w.bq) * p.H + row.h) * p.Tq + w.q0 + row.q;
     uint4 qf[KS], df[KS];
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
         qf[s] = *reinterpret_cast<const uint4 *>(qr + 16 * s + 8 * h);
         df[s] = *reinterpret_cast<const uint4 *>(dr + 16 * s + 8 * h);
     }
-    const float sc = ds_scale<PK>(p, w);
+    const float sc = ds_scale<PK>(p, w, row.h);
     // D = dO . O as the diagonal of a product of the same shape, operands and order as
     // dP: where a query sees a single key, O is that key's V and D is dP to the
     // bit, so that its dS is the formula's zero and not the difference of two sums.
@@ -773,17 +841,17 @@ __global__ __launch_bounds__(64 * NW, D == 64 && !FINE ? 4 : 2) void attn_dq_ker
         dl = ((n >> 2) & 1) == h ? dl : 0.0f;
         dl = half_add(dl);
     }
-    if (h == 0 && qi < w.nq && w.share == 0) p.delta[srow] = dl;
+    if (h == 0 && x < rows && w.share == 0) p.delta[srow] = dl;
     dl *= sc;
     const float lse = p.lse[srow];
 
     int kend = w.nk;
     if (p.causal) {
-        const int last = (m0 + BM < w.nq ? m0 + BM : w.nq) + w.shift;
+        const int last = query_of(p, (m0 + BM < rows ? m0 + BM : rows) - 1) + 1 + w.shift;
         kend = last < kend ? last : kend;
     }
-    const int lim = p.causal && qi + w.shift + 1 < w.nk ? qi + w.shift + 1 : w.nk;
-    const int wmin = m0 + 32 * wave, wmax = wmin + 31;
+    const int lim = p.causal && row.q + w.shift + 1 < w.nk ? row.q + w.shift + 1 : w.nk;
+    const int wmin = query_of(p, m0 + 32 * wave), wmax = query_of(p, m0 + 32 * wave + 31);
     const int wlim = p.causal && wmin + w.shift + 1 < w.nk ? wmin + w.shift + 1 : w.nk;
     const int wend = p.causal && wmax + w.shift + 1 < w.nk ? wmax + w.shift + 1 : w.nk;
     const float c = p.scale * kLog2e;
@@ -794,7 +862,8 @@ __global__ __launch_bounds__(64 * NW, D == 64 && !FINE ? 4 : 2) void attn_dq_ker
     const int all = kend > 0 ? (kend + kTile - 1) / kTile : 0;
     const int first = static_cast<int>(static_cast<int64_t>(all) * w.share / p.splits_q);
     const int nt = static_cast<int>(static_cast<int64_t>(all) * (w.share + 1) / p.splits_q);
-    int glim = p.causal && m0 + w.shift + 1 < w.nk ? m0 + w.shift + 1 : w.nk;  // all of the workgroup see these
+    const int gmin = query_of(p, m0);
+    int glim = p.causal && gmin + w.shift + 1 < w.nk ? gmin + w.shift + 1 : w.nk;  // all of the workgroup see these
     glim = glim < nt * kTile ? glim : nt * kTile;
     if (first < nt) {
         stage<D, NW>(ks, first * kTile, w.nk, sk0, wave, lane);
@@ -842,7 +911,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 && !FINE ? 4 : 2) void attn_dq_ker
         step(t, std::false_type{}, std::true_type{});
         if (t + 1 < nt) step(t + 1, std::true_type{}, std::true_type{});
     }
-    if (qi >= w.nq) return;
+    if (x >= rows) return;
     const float f = p.scale / sc;
     if (p.splits_q > 1) {
         float *part = p.part_q + w.share * (static_cast<int64_t>(p.B) * p.Tq * p.H * D) + orow;
@@ -888,18 +957,24 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dkv_kernel(AttnTrainParams p)
     const int rb = row_base<D>(lane), cb = col_base<D>(lane);
     Where w;
     const int nbg = (p.ranked ? 1 : p.nseq) * p.G, qpk = p.H / p.G;
-    const int ts = blockIdx.x / nbg;
+    // Dealt as in turn_of, or all groups' first tiles first, both the longest (causal) ones first.
+    int ts = blockIdx.x / nbg, jg = blockIdx.x - ts * nbg;
+    if (p.dealt) {
+        const int per = static_cast<int>(p.ranked ? p.k_tiles : p.tiles) * p.splits, x = blockIdx.x >> 3, g = x / per;
+        ts = x - g * per;
+        jg = g * 8 + (blockIdx.x & 7);
+        if (jg >= nbg) return;
+    }
     w.tile = ts / p.splits;
     const int share = ts - w.tile * p.splits;
-    const int jg = blockIdx.x - ts * nbg;
     w.s = jg / p.G;
     w.g = jg - w.s * p.G;
     if (p.ranked) {
-        const Packed x = packed_tile(p.cu, p.nseq, p.tiles, w.tile);
+        const Packed x = packed_tile(p.cu, p.nseq, 1, p.tiles, w.tile);
         w.s = x.s < 0 ? 0 : x.s;
         w.tile = x.s < 0 ? p.tiles : x.tiles - 1 - x.level;
     }
-    w.h = w.g * qpk;
+    const int head0 = w.g * qpk;  // the group's first query head
     where_rows(p, w);
     const int n0 = w.tile * BN;
     const int kall = p.cu ? w.nk : p.Tk;  // rows that dk and dv have (hidden ones get zeros)
@@ -937,12 +1012,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dkv_kernel(AttnTrainParams p)
     // fp16: one scale for every head of the group, the smallest of theirs.
     float sc = 1.0f;
     if constexpr (PK == PrecKind::F16) {
-        sc = ds_scale<PK>(p, w);
-        for (int r = 1; r < qpk; ++r) {
-            Where o = w;
-            o.h = w.h + r;
-            sc = fminf(sc, ds_scale<PK>(p, o));
-        }
+        sc = ds_scale<PK>(p, w, head0);
+        for (int r = 1; r < qpk; ++r) sc = fminf(sc, ds_scale<PK>(p, w, head0 + r));
     }
     const float ds_mul = PK == PrecKind::F16 ? sc * ldexpf(1.0f, -14) : 1.0f;
 
@@ -974,7 +1045,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dkv_kernel(AttnTrainParams p)
         if (tid < 2 * BQ) sl[tid] = tid < BQ ? next - p16 : next * ds_mul;
     };
     auto request = [&](char *tq, char *td) __attribute__((always_inline)) {
-        const int hh = w.h + rh, row0 = (t0 + rt) * BQ;
+        const int hh = head0 + rh, row0 = (t0 + rt) * BQ;
         ni = row0;
         Stream qh = qs, dh = ds;
         qh.base += 2 * hh * p.qs[2];
@@ -1159,13 +1230,18 @@ static_assert(32 * kWaves == 128, "q_tiles, k_tiles and packed_tile count tiles 
 // up against not: one document of 16384 tokens among 400 of 20 .. 200 (51000 against 900
 // tiles) 7030 us against 8102; 1000 of 20 .. 100 (1000, all of them there; H16 G16 D64)
 // 1146 against 794; 9 of 259 .. 1348 (99 against 62) 327 against 324.
-bool packed_ranked(const AttnTrainParams &p)
+// Sets that, the tiles, and `dealt` (turn_of), for a launch over `all` tiles of a group (a
+// token being `rows` of their rows) in `shares`; returns its workgroups.  Dealt from 4096
+// workgroups (four to eight rounds), of enough groups that a short last deal does not count.
+unsigned set_grid(AttnTrainParams &p, int64_t all, int64_t rows, int shares)
 {
-    return p.cu && static_cast<int64_t>(p.nseq) * ((p.max_q + 127) / 128) > 8 * p.q_tiles;
-}
-int64_t grid_tiles(const AttnTrainParams &p, int64_t all)
-{
-    return p.cu && !p.ranked ? static_cast<int64_t>(p.nseq) * p.tiles : all;
+    p.tiles = static_cast<int>(p.cu ? (p.max_q * rows + 127) / 128 : all / p.nseq);
+    const int64_t even = static_cast<int64_t>(p.nseq) * p.tiles;
+    p.ranked = p.cu && even > 8 * all;
+    const int64_t groups = static_cast<int64_t>(p.ranked ? 1 : p.nseq) * p.G;
+    const int64_t tiles = (p.ranked ? all : p.tiles) * shares;
+    p.dealt = tiles * groups >= 4096 && (groups % 8 == 0 || groups >= 64);
+    return static_cast<unsigned>((p.dealt ? (groups + 7) / 8 * 8 : groups) * tiles);
 }
 
 // Whether P and dS are multiplied in two parts.  In short sequences few rounded terms make
@@ -1182,10 +1258,9 @@ bool attn_fine(const AttnTrainParams &p)
 template <PrecKind PK, int D>
 hipError_t fwd_d(AttnTrainParams p, hipStream_t s)
 {
-    p.tiles = (p.max_q + 32 * kWaves - 1) / (32 * kWaves);
-    p.ranked = packed_ranked(p);
+    const unsigned grid = set_grid(p, p.q_tiles, p.H / p.G, p.splits_f);
     hipLaunchKernelGGL((attn_fine(p) ? attn_fwd_kernel<PK, D, kWaves, true> : attn_fwd_kernel<PK, D, kWaves, false>),
-                       dim3(static_cast<unsigned>(grid_tiles(p, p.q_tiles)) * p.H * p.splits_f), dim3(64 * kWaves), 0, s, p);
+                       dim3(grid), dim3(64 * kWaves), 0, s, p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits_f == 1) return e;
     const int64_t threads = static_cast<int64_t>(p.B) * p.Tq * p.H * (D / 4);
@@ -1202,11 +1277,10 @@ hipError_t bwd_d(AttnTrainParams p, hipStream_t s)
         hipLaunchKernelGGL((norm_max_kernel<D>), dim3(kNormParts * p.B * (p.H + p.G)), dim3(256), 0, s, p);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
-    p.tiles = (p.max_q + 32 * kWaves - 1) / (32 * kWaves);
-    p.ranked = packed_ranked(p);
     if (p.Tq > 0 && p.max_q > 0) {
+        const unsigned grid = set_grid(p, p.q_tiles, p.H / p.G, p.splits_q);
         hipLaunchKernelGGL((attn_fine(p) ? attn_dq_kernel<PK, D, kWaves, true> : attn_dq_kernel<PK, D, kWaves, false>),
-                           dim3(static_cast<unsigned>(grid_tiles(p, p.q_tiles)) * p.H * p.splits_q), dim3(64 * kWaves), 0, s, p);
+                           dim3(grid), dim3(64 * kWaves), 0, s, p);
         if ((e = hipGetLastError()) != hipSuccess) return e;
         const int64_t all = static_cast<int64_t>(p.B) * p.Tq * p.H * D;
         if (p.splits_q > 1 && (e = sum_shares<PK>(p.part_q, all, p.splits_q, p.dq, nullptr, all, s)) != hipSuccess) return e;
@@ -1215,9 +1289,10 @@ hipError_t bwd_d(AttnTrainParams p, hipStream_t s)
         // Query rows per tile: at D = 128 half of the other's, so that two
         // workgroups' tiles and V rows fit a CU's LDS.
         constexpr int BQ = D == 64 ? 64 : 32;
+        const unsigned grid = set_grid(p, p.k_tiles, 1, p.splits);
         hipLaunchKernelGGL((attn_fine(p) ? attn_dkv_kernel<PK, D, kWaves, BQ, true>
                                          : attn_dkv_kernel<PK, D, kWaves, BQ, false>),
-                           dim3(static_cast<unsigned>(grid_tiles(p, p.k_tiles)) * p.G * p.splits), dim3(64 * kWaves), 0, s, p);
+                           dim3(grid), dim3(64 * kWaves), 0, s, p);
         if ((e = hipGetLastError()) != hipSuccess) return e;
         const int64_t all = static_cast<int64_t>(p.B) * p.Tk * p.G * D;
         if (p.splits > 1) e = sum_shares<PK>(p.part, 2 * all, p.splits, p.dk, p.dv, all, s);
@@ -1254,7 +1329,7 @@ int attn_bwd_splits(const AttnTrainParams &p)
 // keys: up to 512 workgroups, of at least 8 key tiles each.
 int attn_key_shares(const AttnTrainParams &p)
 {
-    const int64_t wgs = p.q_tiles * p.H, tiles = (p.Tk + kTile - 1) / kTile;
+    const int64_t wgs = p.q_tiles * p.G, tiles = (p.Tk + kTile - 1) / kTile;
     if (wgs == 0 || wgs >= 256) return 1;
     int64_t s = 512 / wgs;
     s = s < tiles / 8 ? s : tiles / 8;

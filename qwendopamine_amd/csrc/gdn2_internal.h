@@ -328,10 +328,12 @@ struct AttnTrainParams {
     const int64_t *cu;       // [nseq + 1] or NULL
     int nseq;                // B without cu
     int max_q;               // longest sequence's queries
-    int64_t q_tiles, k_tiles;  // tiles of 128 queries, keys, over all sequences (one head)
-    // Set by the launcher: tiles of the longest sequence, and whether a workgroup of
-    // packed sequences looks its tile up (rows of unequal lengths).
-    int tiles, ranked;
+    // Over all sequences, of one group: tiles of 128 rows (a query's heads each one), of 128 keys.
+    int64_t q_tiles, k_tiles;
+    // Set by the launcher: tiles of the longest sequence, whether a workgroup of packed
+    // sequences looks its tile up (rows of unequal lengths), and the order of workgroups.
+    int tiles, ranked, dealt;
+    unsigned qpk_m, qpk_s;  // for the division by H / G
     int B, Tq, Tk, H, G, D;
     int causal;
     float scale;
