@@ -279,7 +279,7 @@ __device__ __forceinline__ void mix_reads()
 // longest first, workgroup b takes.  Those of equal place in successive rounds over the
 // 256 CUs share a CU, so every other round runs backwards: a CU's tiles then add up to
 // about the same length.
-//   dealt (many rounds): workgroups go to the 8 XCDs in turn, each with an L2 of its own; the
+//   dealt (many rounds, set_grid): workgroups go to the 8 XCDs in turn, each with an L2 of its own; the
 //     groups are dealt out to them, and an XCD does one group's tiles after the other's,
 //     whose keys it then holds (200 packed documents, 62381 tokens, H16 G4 D128 forward:
 //     257 us, against 296 the other way).  A last deal may be short (group >= groups).
@@ -405,7 +405,7 @@ __device__ __forceinline__ Packed packed_tile(const int64_t *cu, int nseq, int r
 // Query-resident kernels: a group's rows are its queries' heads, row x the head x % qpk of
 // query x / qpk, so that a tile of keys serves every head that reads it (few queries of
 // many heads fill a tile, and causal tiles of 128 rows span 128 / qpk queries: B1 Tq1
-// Tk16384 H32 G8 D128 ROWSON us against ROWSOFF with a workgroup per head).  Long causal
+// Tk16384 H32 G8 D128 29 us against 43 with a workgroup per head).  Long causal
 // tiles first; w.share of `shares` of the keys; w.nq rows.
 __device__ __forceinline__ Where where_q(const AttnTrainParams &p, int shares)
 {
@@ -461,6 +461,36 @@ __device__ __forceinline__ void hide(f32x16 &s, int j0, int h, int limit)
     }
 }
 
+// A wave's 32 results of D channels, 16-bit, into rows of memory by way of 32 rows of LDS:
+// written from the accumulators eight bytes a row at a time, lines were left half
+// written when others took their place in the L2 (B64 T64 H16 G4 D128 forward, 512
+// workgroups 128 KB apart: 33 us, and 14 as whole rows).  make(a, b, c, d): four
+// channels' bits; to(r): the first element of row r, or -1.
+template <int D, typename Make>
+__device__ __forceinline__ void put_rows(char *so, int lane, const f32x16 (&x)[D / 32], Make make)
+{
+    constexpr int P = D / 8;
+    const int n = lane & 31, h = lane >> 5;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<uint2 *>(so + n * (2 * D) + (((4 * d + i) ^ n) & (P - 1)) * 16 + 8 * h) =
+                make(x[d][4 * i], x[d][4 * i + 1], x[d][4 * i + 2], x[d][4 * i + 3]).u;
+}
+template <int D, typename To>
+__device__ __forceinline__ void write_rows(const char *so, int lane, uint16_t *out, To to)
+{
+    constexpr int P = D / 8;
+#pragma unroll
+    for (int it = 0; it < P / 2; ++it) {
+        const int r = it * (64 / P) + lane / P;
+        const uint4 v = *reinterpret_cast<const uint4 *>(so + r * (2 * D) + ((lane ^ r) & (P - 1)) * 16);
+        const int64_t at = to(r);
+        if (at >= 0) *reinterpret_cast<uint4 *>(out + at + (lane % P) * 8) = v;
+    }
+}
+
 // ---------------------------------------------------------------- forward
 
 // L in base 2.  A query that sees no key: +inf, which makes its recomputed P zero.
@@ -488,11 +518,11 @@ __device__ __forceinline__ Q4<PK> left_out(float a, float b, float c, float d)
 }
 
 // One pass over the keys with the running maximum and sum.  D = 128 is bound by the
-// matrix units (B2 T8192 H16 G4 causal: 516 us, 1065 TFLOP/s; a large library product
+// matrix units (B2 T8192 H16 G4 causal: 503 us, 1094 TFLOP/s; a large library product
 // reaches 1121), D = 64 by vector arithmetic, as a score costs a scaling, a maximum, an
 // exponential of four issue slots, a sum and half a conversion whatever D is (B4
 // T2048 H16 causal: 47 us, 732 TFLOP/s, vector units busy 72% of the time, matrix
-// units 40%).  Few queries over many keys: B1 Tq1 Tk16384 H32 G8 D128, keys in shares, 45 us.
+// units 40%).  Few queries over many keys: B1 Tq1 Tk16384 H32 G8 D128, keys in shares, 29 us.
 template <PrecKind PK, int D, int NW, bool FINE>
 __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void attn_fwd_kernel(AttnTrainParams p)
 {
@@ -643,43 +673,22 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void attn_fwd_kernel(Attn
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     if (h == 0 && x < rows)
         p.lse[(static_cast<int64_t>(w.bq) * p.H + row.h) * p.Tq + w.q0 + row.q] = log_sum(m, l);
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[d][i] *= inv;
-    // Whole rows are written, through LDS (this wave's 32 rows): eight bytes a row at a time
-    // left lines half written when others took their place in the L2.
     __syncthreads();  // the tiles are done with
-    char *const so = (wave < 2 ? sk0 : sv0) + (wave & 1) * (32 * 2 * D);
-    constexpr int P = D / 8;
-    auto write = [&](uint16_t *out) __attribute__((always_inline)) {
-#pragma unroll
-        for (int it = 0; it < P / 2; ++it) {
-            const int r = it * (64 / P) + lane / P, xr = m0 + 32 * wave + r;
-            const uint4 v = *reinterpret_cast<const uint4 *>(so + r * (2 * D) + ((lane ^ r) & (P - 1)) * 16);
-            if (xr < rows) {
-                const Row to = row_of(p, xr, rows, w.g, qpk);
-                const int64_t at = ((w.bq * static_cast<int64_t>(p.Tq) + w.q0 + to.q) * p.H + to.h) * D;
-                *reinterpret_cast<uint4 *>(out + at + (lane % P) * 8) = v;
-            }
-        }
+    char *const so = wave == 0 ? sk0 : wave == 1 ? sk1 : wave == 2 ? sv0 : sv1;
+    auto to = [&](int r) __attribute__((always_inline)) {
+        const int xr = m0 + 32 * wave + r;
+        const Row at = row_of(p, xr, rows, w.g, qpk);
+        return xr < rows ? ((w.bq * static_cast<int64_t>(p.Tq) + w.q0 + at.q) * p.H + at.h) * D : int64_t{-1};
     };
-    auto place = [&](int d, int i) __attribute__((always_inline)) {
-        return reinterpret_cast<uint2 *>(so + n * (2 * D) + (((4 * d + i) ^ n) & (P - 1)) * 16 + 8 * h);
-    };
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            *place(d, i) = pack4<PK>(acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]).u;
-    write(static_cast<uint16_t *>(p.o));
+    put_rows<D>(so, lane, acc, [&](float a, float b, float c, float d) __attribute__((always_inline)) {
+        return pack4<PK>(a * inv, b * inv, c * inv, d * inv);
+    });
+    write_rows<D>(so, lane, static_cast<uint16_t *>(p.o), to);
     if (!p.o_lo) return;
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            *place(d, i) = left_out<PK>(acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]).u;
-    write(static_cast<uint16_t *>(p.o_lo));
+    put_rows<D>(so, lane, acc, [&](float a, float b, float c, float d) __attribute__((always_inline)) {
+        return left_out<PK>(a * inv, b * inv, c * inv, d * inv);
+    });
+    write_rows<D>(so, lane, static_cast<uint16_t *>(p.o_lo), to);
 }
 
 // The shares of a query's keys, in their order; thread: 4 channels of a row.  Bound by
@@ -791,7 +800,7 @@ __device__ __forceinline__ float ds_scale(const AttnTrainParams &p, const Where 
 // dQ: queries resident, one pass over the keys.  Also forms D = dO . (O + what its
 // rounding left out) per query, which the kernel below reads.  Three products a tile:
 // B2 T8192 H16 G4 D128 causal 730 us, 1130 TFLOP/s, the matrix units' rate; B4 T2048
-// H16 D64 66 us, 780 TFLOP/s, vector units busy 57% and matrix units 48%.
+// H16 D64 64 us, 805 TFLOP/s, vector units busy 57% and matrix units 48%.
 template <PrecKind PK, int D, int NW, bool FINE>
 __global__ __launch_bounds__(64 * NW, D == 64 && !FINE ? 4 : 2) void attn_dq_kernel(AttnTrainParams p)
 {
@@ -911,9 +920,9 @@ __global__ __launch_bounds__(64 * NW, D == 64 && !FINE ? 4 : 2) void attn_dq_ker
         step(t, std::false_type{}, std::true_type{});
         if (t + 1 < nt) step(t + 1, std::true_type{}, std::true_type{});
     }
-    if (x >= rows) return;
     const float f = p.scale / sc;
     if (p.splits_q > 1) {
+        if (x >= rows) return;
         float *part = p.part_q + w.share * (static_cast<int64_t>(p.B) * p.Tq * p.H * D) + orow;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
@@ -923,19 +932,22 @@ __global__ __launch_bounds__(64 * NW, D == 64 && !FINE ? 4 : 2) void attn_dq_ker
                     make_float4(acc[d][4 * i] * f, acc[d][4 * i + 1] * f, acc[d][4 * i + 2] * f, acc[d][4 * i + 3] * f);
         return;
     }
-    uint16_t *dq = static_cast<uint16_t *>(p.dq) + orow;
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            st_q4<PK>(dq + 32 * d + 8 * i + 4 * h, pack4<PK>(acc[d][4 * i] * f, acc[d][4 * i + 1] * f,
-                                                             acc[d][4 * i + 2] * f, acc[d][4 * i + 3] * f));
+    __syncthreads();  // the tiles are done with
+    char *const so = wave == 0 ? sk0 : wave == 1 ? sk1 : wave == 2 ? sv0 : sv1;
+    put_rows<D>(so, lane, acc, [&](float a, float b, float c, float d) __attribute__((always_inline)) {
+        return pack4<PK>(a * f, b * f, c * f, d * f);
+    });
+    write_rows<D>(so, lane, static_cast<uint16_t *>(p.dq), [&](int r) __attribute__((always_inline)) {
+        const int xr = m0 + 32 * wave + r;
+        const Row at = row_of(p, xr, rows, w.g, qpk);
+        return xr < rows ? ((w.bq * static_cast<int64_t>(p.Tq) + w.q0 + at.q) * p.H + at.h) * D : int64_t{-1};
+    });
 }
 
 // dK, dV: keys resident, one pass over the queries of every head of the group,
 // or, where that leaves too few or too uneven workgroups (attn_bwd_splits), over
 // one of p.splits equal shares of it, whose fp32 sums attn_sum_kernel adds.  Four
-// products a tile: B2 T8192 H16 G4 D128 causal 1050 us, 1047 TFLOP/s; B4 T2048 H16 D64
+// products a tile: B2 T8192 H16 G4 D128 causal 1000 us, 1100 TFLOP/s; B4 T2048 H16 D64
 // 90 us, 764 TFLOP/s, vector and matrix units each busy 43%, two waves per SIMD that wait
 // for each other's products in turn (three, within 168 registers: 84 us, but less
 // even over short rows, B8 T509 H8 63 us for 60 forward and backward).
@@ -1155,10 +1167,10 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dkv_kernel(AttnTrainParams p)
             step(x, std::false_type{}, std::false_type{});
             if (x + 1 < steps) step(x + 1, std::true_type{}, std::false_type{});
         }
-    if (kj >= kall) return;
     const float fk = p.scale / sc, fv = PK == PrecKind::F16 ? ldexpf(1.0f, -14) : 1.0f;
     const int64_t krow = ((w.bk * static_cast<int64_t>(p.Tk) + w.k0 + kj) * p.G + w.g) * D;
     if (p.splits > 1) {
+        if (kj >= kall) return;
         const int64_t all = static_cast<int64_t>(p.B) * p.Tk * p.G * D;
         float *pk = p.part + 2 * share * all + krow, *pv = pk + all;
 #pragma unroll
@@ -1172,16 +1184,20 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dkv_kernel(AttnTrainParams p)
             }
         return;
     }
-    uint16_t *ok = static_cast<uint16_t *>(p.dk) + krow, *ov = static_cast<uint16_t *>(p.dv) + krow;
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            st_q4<PK>(ok + 32 * d + 8 * i + 4 * h, pack4<PK>(dk[d][4 * i] * fk, dk[d][4 * i + 1] * fk,
-                                                             dk[d][4 * i + 2] * fk, dk[d][4 * i + 3] * fk));
-            st_q4<PK>(ov + 32 * d + 8 * i + 4 * h, pack4<PK>(dv[d][4 * i] * fv, dv[d][4 * i + 1] * fv,
-                                                             dv[d][4 * i + 2] * fv, dv[d][4 * i + 3] * fv));
-        }
+    __syncthreads();  // the tiles are done with
+    char *const so = wave == 0 ? sq0 : wave == 1 ? sq1 : wave == 2 ? sd0 : sd1;
+    auto to = [&](int r) __attribute__((always_inline)) {
+        const int kr = n0 + 32 * wave + r;
+        return kr < kall ? ((w.bk * static_cast<int64_t>(p.Tk) + w.k0 + kr) * p.G + w.g) * D : int64_t{-1};
+    };
+    put_rows<D>(so, lane, dk, [&](float a, float b, float c, float d) __attribute__((always_inline)) {
+        return pack4<PK>(a * fk, b * fk, c * fk, d * fk);
+    });
+    write_rows<D>(so, lane, static_cast<uint16_t *>(p.dk), to);
+    put_rows<D>(so, lane, dv, [&](float a, float b, float c, float d) __attribute__((always_inline)) {
+        return pack4<PK>(a * fv, b * fv, c * fv, d * fv);
+    });
+    write_rows<D>(so, lane, static_cast<uint16_t *>(p.dv), to);
 }
 
 // Sums of n shares of `all` values each, stride apart, in their order, rounded; thread: 4
@@ -1248,8 +1264,9 @@ unsigned set_grid(AttnTrainParams &p, int64_t all, int64_t rows, int shares)
 // up a gradient, and one of them shows in D values of it: rounded once, the error
 // of dk against 64 bits is 2.8 times that of rounding the exact result at 2 tokens, 1.6 at
 // 8, 1.5 at 64 and below 1.5 past 128; in two parts it is the same as that.  The products
-// they add are cheap there: forward and backward in two parts and in one, B64 T64 H8 D64
-// 27.2 and 26.2 us, B256 T128 H16 D64 366 and 359, B64 T128 H16 G4 D128 124 and 121.
+// they add are cheap there (when they came: forward and backward in two parts and in one, B64
+// T64 H8 D64 27.2 and 26.2 us, B256 T128 H16 D64 366 and 359, B64 T128 H16 G4 D128 124
+// and 121).
 bool attn_fine(const AttnTrainParams &p)
 {
     return p.max_q <= 128 && (p.cu || p.Tk <= 128);
