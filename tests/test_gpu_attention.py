@@ -160,6 +160,32 @@ def test_attention_short_sequences_are_as_exact_as_their_rounding(gpu_device, T,
         assert off <= 1.05 * rounding, (name, float(off / rounding))
 
 
+@pytest.mark.parametrize("lens,H,G", [
+    ([(7 * i) % 60 + 1 for i in range(700)] + [140], 6, 3),          # groups not a multiple of the eight XCDs
+    ([(5 * i) % 20 for i in range(600)] + [2000], 8, 8),             # and tiles looked up
+])
+def test_attention_many_rounds_of_packed_sequences(gpu_device, lens, H, G):
+    """Over 4096 workgroups: groups are dealt out, the last deal short."""
+    print(f"[case] attention {len(lens)} packed sequences, H{H} G{G}", flush=True)
+    cu = [0]
+    for x in lens:
+        cu.append(cu[-1] + x)
+    x = _inputs(gpu_device, 1, cu[-1], cu[-1], H, G, 64, BF, seed=H)
+    _check(_run(*x, cu_seqlens=torch.tensor(cu)), *x, cu=cu)
+
+
+@pytest.mark.parametrize("B,Tq,Tk,H,G,D,causal", [
+    (130, 33, 33, 32, 32, 64, True),     # many rounds
+    (70, 20, 50, 120, 60, 64, False),    # more keys than queries
+    (3, 5, 700, 32, 2, 128, True),       # sixteen heads of a query in a tile, the keys shared out
+    (2, 77, 77, 21, 3, 128, True),       # seven heads: queries across tiles
+])
+def test_attention_rows_of_a_group(gpu_device, B, Tq, Tk, H, G, D, causal):
+    print(f"[case] attention rows B{B} Tq{Tq} Tk{Tk} H{H} G{G} D{D}", flush=True)
+    x = _inputs(gpu_device, B, Tq, Tk, H, G, D, BF, seed=B)
+    _check(_run(*x, causal=causal), *x, causal=causal)
+
+
 def test_attention_shared_keys_of_padded_rows(gpu_device):
     """Key shares past a row's length hold nothing; a row of no keys gives zeros."""
     lens = [0, 1, 700, 1600]
