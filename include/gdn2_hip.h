@@ -411,8 +411,8 @@ int gdn2_token_logprobs_bwd(const void *x, int64_t inner_rows, int64_t outer_str
  * gdn2_attn_bwd writes dq (like o) and dk, dv [B, Tk, G, D] contiguous, summed
  * over the query heads of a group, from o, o_lo and lse of the forward and dout
  * [B, Tq, H, D] contiguous; the probabilities are recomputed.  Every output has
- * the same bits in every run.  bf16 / fp16, D in {64, 128}, scale > 0; else
- * GDN2_ERR_UNSUPPORTED.  workspace: gdn2_attn_fwd_workspace_size() (0 unless few
+ * the same bits in every run.  bf16 / fp16, D in {64, 128}, scale > 0, Tq H / G up
+ * to 2^30; else GDN2_ERR_UNSUPPORTED.  workspace: gdn2_attn_fwd_workspace_size() (0 unless few
  * queries face many keys; then it may be NULL) and gdn2_attn_bwd_workspace_size()
  * bytes, 16-byte aligned, of which concurrent calls need one each.
  */

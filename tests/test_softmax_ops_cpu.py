@@ -80,6 +80,7 @@ def _attn_call(lib, **over):
     (nat.ERR_UNSUPPORTED, dict(scale=0.0)),
     (nat.ERR_UNSUPPORTED, dict(scale=float("nan"))),
     (nat.ERR_UNSUPPORTED, dict(B=1 << 30, Tq=1 << 20)),
+    (nat.ERR_UNSUPPORTED, dict(Tq=1 << 24, H=128, G=1)),  # 2^31 rows of one group
     (nat.ERR_WORKSPACE, dict(Tk=100000)),
     (nat.OK, dict(B=0)),
     (nat.OK, dict(Tq=0)),
