@@ -521,7 +521,7 @@ __device__ __forceinline__ Q4<PK> left_out(float a, float b, float c, float d)
 // matrix units (B2 T8192 H16 G4 causal: 503 us, 1094 TFLOP/s; a large library product
 // reaches 1121), D = 64 by vector arithmetic, as a score costs a scaling, a maximum, an
 // exponential of four issue slots, a sum and half a conversion whatever D is (B4
-// T2048 H16 causal: 47 us, 732 TFLOP/s, vector units busy 72% of the time, matrix
+// T2048 H16 causal: 47 us, 732 TFLOP/s, vector units busy 77% of the time, matrix
 // units 40%).  Few queries over many keys: B1 Tq1 Tk16384 H32 G8 D128, keys in shares, 29 us.
 template <PrecKind PK, int D, int NW, bool FINE>
 __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void attn_fwd_kernel(AttnTrainParams p)
@@ -799,8 +799,8 @@ __device__ __forceinline__ float ds_scale(const AttnTrainParams &p, const Where 
 
 // dQ: queries resident, one pass over the keys.  Also forms D = dO . (O + what its
 // rounding left out) per query, which the kernel below reads.  Three products a tile:
-// B2 T8192 H16 G4 D128 causal 730 us, 1130 TFLOP/s, the matrix units' rate; B4 T2048
-// H16 D64 64 us, 805 TFLOP/s, vector units busy 57% and matrix units 48%.
+// B2 T8192 H16 G4 D128 causal 710 us, 1160 TFLOP/s, the matrix units' rate; B4 T2048
+// H16 D64 63 us, 815 TFLOP/s, vector units busy 60% and matrix units 49%.
 template <PrecKind PK, int D, int NW, bool FINE>
 __global__ __launch_bounds__(64 * NW, D == 64 && !FINE ? 4 : 2) void attn_dq_kernel(AttnTrainParams p)
 {
@@ -948,9 +948,9 @@ __global__ __launch_bounds__(64 * NW, D == 64 && !FINE ? 4 : 2) void attn_dq_ker
 // or, where that leaves too few or too uneven workgroups (attn_bwd_splits), over
 // one of p.splits equal shares of it, whose fp32 sums attn_sum_kernel adds.  Four
 // products a tile: B2 T8192 H16 G4 D128 causal 1000 us, 1100 TFLOP/s; B4 T2048 H16 D64
-// 90 us, 764 TFLOP/s, vector and matrix units each busy 43%, two waves per SIMD that wait
-// for each other's products in turn (three, within 168 registers: 84 us, but less
-// even over short rows, B8 T509 H8 63 us for 60 forward and backward).
+// 85 us, 808 TFLOP/s, vector and matrix units each busy 46%, two waves per SIMD that wait
+// for each other's products in turn (three, within 168 registers, gained 4 us, but
+// lost 3 over short rows, B8 T509 H8, forward and backward 60).
 template <PrecKind PK, int D, int NW, int BQ, bool FINE>
 __global__ __launch_bounds__(64 * NW, 2) void attn_dkv_kernel(AttnTrainParams p)
 {
