@@ -1333,6 +1333,8 @@ bool attn_train_supported(int io_dtype, int D)
 // 2314 / 1812 / 1814 / 1913; packed 7013 tokens, H16 G4 D128 (240) 310 / 217 / 184 / 223;
 // B1 T4096 H16 G2 D64 (64) 795 / 456 / 288 / 213; B4 T2048 H16 D64 (1024)
 // 162 / 207 / 274 / 421; B8 T509 H8 D64, not causal (256, 8 tiles each) 53 / 59 / 63 / 80.
+// With the present ones, for 1024 and 512 causal workgroups, forward and backward: B2
+// T8192 2211 and 2524, packed 296 and 312.
 int attn_bwd_splits(const AttnTrainParams &p)
 {
     const int64_t wgs = p.k_tiles * p.G, want = p.causal ? 1024 : 512;
