@@ -137,11 +137,13 @@ def _cu(cu_seqlens, device, total_tokens: int):
     """Device and host int64 copies of ``cu_seqlens``, validated on the host.
 
     The kernels index tokens through these offsets, so they must start at 0,
-    be non-decreasing and end at the packed length.
+    be non-decreasing and end at the packed length.  Never the caller's own storage: a
+    backward takes its launch sizes from the host copy, and the caller may write the
+    buffer again before it.
     """
     if cu_seqlens is None:
         return None, None
-    cu_host = torch.as_tensor(cu_seqlens).detach().to("cpu", torch.int64).contiguous()
+    cu_host = torch.as_tensor(cu_seqlens).detach().to("cpu", torch.int64, copy=True).contiguous()
     if cu_host.dim() != 1 or cu_host.numel() < 1:
         raise ValueError("cu_seqlens must be a 1-D tensor of N+1 offsets")
     if int(cu_host[0]) != 0 or int(cu_host[-1]) != total_tokens or bool((cu_host[1:] < cu_host[:-1]).any()):

@@ -391,3 +391,19 @@ def test_attention_refuses_a_second_derivative(gpu_device):
     (dq,) = torch.autograd.grad(ops.attention(q, k, v), q, do, create_graph=True)
     with pytest.raises(RuntimeError):
         dq.sum().backward()
+
+
+@pytest.mark.parametrize("first,then", [([0, 400, 400, 400, 400], [0, 100, 200, 300, 400]),
+                                        ([0, 3, 70, 400], [0, 400, 400, 400])])
+def test_attention_packed_offsets_written_again_before_the_backward(gpu_device, first, then):
+    """The caller's offsets buffer holds another partition by the time of the backward: gradients of
+    the one that the forward took."""
+    from qwendopamine_amd import ops
+
+    x = _inputs(gpu_device, 1, 400, 400, 4, 2, 64, BF, seed=31)
+    want = _run(*x, cu_seqlens=torch.tensor(first))
+    cu = torch.tensor(first)
+    o = ops.attention(*x[:3], cu_seqlens=cu)
+    cu.copy_(torch.tensor(then))
+    got = torch.autograd.grad(o, x[:3], x[3])
+    assert torch.equal(o, want["o"]) and all(torch.equal(a, want[n]) for a, n in zip(got, ("dq", "dk", "dv")))

@@ -220,3 +220,18 @@ def test_hybrid_options_are_checked():
     assert m(idx).shape == (1, 5, 10)  # on the CPU "hip" is torch's attention
     with pytest.raises(RuntimeError):
         m.loss(idx)
+
+
+@pytest.mark.parametrize("make", [
+    lambda: torch.tensor([0, 5, 70, 400]),
+    lambda: torch.tensor([0, 5, 70, 400], dtype=torch.int32),
+    lambda: torch.tensor([[0, 1], [5, 1], [70, 1], [400, 1]])[:, 0],
+])
+def test_packed_offsets_are_copied(make):
+    """A backward pass takes its sizes from the host's offsets: they may not change with the
+    caller's buffer, which a data loader writes again before the backward."""
+    cu = make()
+    dev, host = ops._cu(cu, torch.device("cpu"), 400)
+    cu[1], cu[2] = 399, 399
+    assert host.tolist() == [0, 5, 70, 400] and dev.tolist() == [0, 5, 70, 400]
+    assert host.dtype == torch.int64 and host.is_contiguous()
