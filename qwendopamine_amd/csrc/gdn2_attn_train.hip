@@ -477,6 +477,7 @@ __device__ __forceinline__ void put_rows(char *so, int lane, const f32x16 (&x)[D
         for (int i = 0; i < 4; ++i)
             *reinterpret_cast<uint2 *>(so + n * (2 * D) + (((4 * d + i) ^ n) & (P - 1)) * 16 + 8 * h) =
                 make(x[d][4 * i], x[d][4 * i + 1], x[d][4 * i + 2], x[d][4 * i + 3]).u;
+    wave_fence();  // write_rows reads what other lanes stored
 }
 template <int D, typename To>
 __device__ __forceinline__ void write_rows(const char *so, int lane, uint16_t *out, To to)
@@ -489,6 +490,7 @@ __device__ __forceinline__ void write_rows(const char *so, int lane, uint16_t *o
         const int64_t at = to(r);
         if (at >= 0) *reinterpret_cast<uint4 *>(out + at + (lane % P) * 8) = v;
     }
+    wave_fence();  // the next put_rows overwrites what other lanes read
 }
 
 // ---------------------------------------------------------------- forward

@@ -73,6 +73,14 @@ struct io<f16_t> {
     }
 };
 
+// What the wave's lanes stored (LDS) before it is seen by its loads after it: lanes that hand
+// each other values within a wave need no barrier, but the compiler has to keep the order.
+__device__ __forceinline__ void wave_fence()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 __device__ __forceinline__ float wave_sum(float x)
 {
 #pragma unroll

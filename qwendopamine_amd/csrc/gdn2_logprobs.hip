@@ -110,12 +110,6 @@ __device__ __forceinline__ Stat wave_merge(Stat a)
     return a;
 }
 
-__device__ __forceinline__ void wave_fence()
-{
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
-
 // The wave's candidate list: n entries of `list` (LDS, this wave's own).
 struct Top {
     u64 *list;
