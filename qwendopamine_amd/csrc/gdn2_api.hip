@@ -672,11 +672,11 @@ static int fill_attn_args(AttnTrainParams &p, const void *q, const void *k, cons
     const int size[9] = {B, Tq, H, B, Tk, G, B, Tk, G};
     for (int i = 0; i < 9; ++i) {
         if (strides[i] < 0 || (size[i] > 1 && strides[i] % 8 != 0)) return GDN2_ERR_INVALID;
-        // A token's offset within 16 of them is 32 bits in the kernels.
-        if (i % 3 == 1 && size[i] > 1 && strides[i] > (1 << 25)) return GDN2_ERR_UNSUPPORTED;
+        // A token's offset within a tile of them is 32 bits in the kernels.
+        if (i % 3 == 1 && size[i] > 1 && strides[i] > kMaxTokenStride) return GDN2_ERR_UNSUPPORTED;
         (i < 3 ? p.qs : i < 6 ? p.ks : p.vs)[i % 3] = size[i] > 1 ? strides[i] : 0;
     }
-    if (static_cast<int64_t>(H) * D > (1 << 25)) return GDN2_ERR_UNSUPPORTED;
+    if (static_cast<int64_t>(H) * D > kMaxTokenStride) return GDN2_ERR_UNSUPPORTED;  // of dout
     p.q = q; p.k = k; p.v = v;
     p.kv_len = kv_lengths;
     p.cu = cu;

@@ -143,12 +143,13 @@ __device__ __forceinline__ void stage(const Stream &x, int row0, int nrows, char
 {
     constexpr int P = D / 8, R = 64 / P, IT = ROWS / R;  // requests per tile
     static_assert(IT % NW == 0, "every wave issues as many requests");
+    static_assert((ROWS - 1) * (2 * kMaxTokenStride) + 2 * D <= 0xffffffffLL, "offsets within a tile are 32 bits");
 #ifdef __HIP_DEVICE_COMPILE__  // the host's pass does not know the builtins' types
     typedef __attribute__((address_space(3))) char *lds_ptr;
     const uint64_t at = reinterpret_cast<uint64_t>(x.base + row0 * x.ts);
     const uint64_t tile = static_cast<uint64_t>(__builtin_amdgcn_readfirstlane(static_cast<unsigned>(at >> 32))) << 32 |
                           static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<unsigned>(at)));
-    // Raw buffer, 32-bit elements, offsets up to 2^32 (63 rows of at most 2^26 bytes).
+    // Raw buffer, 32-bit elements, offsets below 2^32.
     const __amdgpu_buffer_rsrc_t rsrc =
         __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void *>(tile), 0, 0xffffffffu, 0x00020000);
     const unsigned ts = static_cast<unsigned>(x.ts);
@@ -1083,8 +1084,14 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dkv_kernel(AttnTrainParams p)
     };
     if (steps > 0) {
         request(sq0, sd0);
-        if constexpr (kVLds)
-            stage<D, NW, BN>(stream_of<D, NW>(vb, p.vs[1], wave, lane), n0, w.nk, sv, wave, lane);
+        if constexpr (kVLds) {
+            // A tile of kTile rows at a time, each from a base of its own; of one past the
+            // last key (whose rows are hidden) that key.
+            const Stream vt = stream_of<D, NW>(vb, p.vs[1], wave, lane);
+#pragma unroll
+            for (int r = 0; r < BN; r += kTile)
+                stage<D, NW>(vt, n0 + r < w.nk ? n0 + r : w.nk - 1, w.nk, sv + r * D * 2, wave, lane);
+        }
     }
     auto step = [&](int x, auto buf, auto hidden) __attribute__((always_inline)) {
         constexpr bool kOdd = decltype(buf)::value, kHide = decltype(hidden)::value;

@@ -309,6 +309,7 @@ hipError_t launch_attn_decode(const AttnDecodeParams &p, int io_dtype, hipStream
 // contiguous; lse, delta [B, H, Tq] (lse: base-2 log of the softmax sum).
 // Query i sees key j < kv_len[b] (or Tk), with causal only j <= i + Tk - Tq; or,
 // with cu (B = 1, Tq = Tk), the keys of its own packed sequence, causal within it.
+constexpr int64_t kMaxTokenStride = 1 << 25;  // elements: a tile's offsets are 32 bits of bytes
 struct AttnTrainParams {
     const void *q, *k, *v;
     int64_t qs[3], ks[3], vs[3];

@@ -407,3 +407,22 @@ def test_attention_packed_offsets_written_again_before_the_backward(gpu_device, 
     cu.copy_(torch.tensor(then))
     got = torch.autograd.grad(o, x[:3], x[3])
     assert torch.equal(o, want["o"]) and all(torch.equal(a, want[n]) for a, n in zip(got, ("dq", "dk", "dv")))
+
+
+@pytest.mark.parametrize("T,D", [(128, 128), (150, 128), (200, 128), (150, 64)])
+def test_attention_tokens_at_the_largest_stride(gpu_device, T, D):
+    """q, k and v as columns of rows of 2^25 elements: offsets within a tile reach 2^32 bytes.  The
+    same bits as contiguous ones."""
+    print(f"[case] attention token stride 2^25, T{T} D{D}", flush=True)
+    x = _inputs(gpu_device, 1, T, T, 4, 2, D, BF, seed=T)
+    want = _run(*x)
+    rows = torch.empty((T - 1) * 2 ** 25 + 8 * D, dtype=BF, device=gpu_device)
+    at, far = 0, []
+    for z in x[:3]:
+        h = z.shape[2]
+        y = rows.as_strided((1, T, h, D), (T * 2 ** 25, 2 ** 25, D, 1), at)
+        y.copy_(z.detach())
+        far.append(y.requires_grad_(True))
+        at += h * D
+    got = _run(*far, x[3])
+    assert all(torch.equal(want[n], got[n]) for n in want)

@@ -1,14 +1,16 @@
-"""Rows that lanes hand each other through LDS: what the compiler is given has to order the stores
-before the loads.  Read from the unoptimised IR of this repository's own source, where every device
-function is still one of its own."""
+"""What the attention kernels hand the compiler, where a wrong result would depend on sizes or on
+luck: rows that lanes exchange through LDS are fenced, and offsets of 32 bits do not wrap.  Read from
+the unoptimised IR of this repository's own source, where every device function is still one of its own."""
 
 from __future__ import annotations
 
+import ctypes
 import re
 import subprocess
 
 import pytest
 
+from qwendopamine_amd import _native as nat
 from qwendopamine_amd import build
 
 
@@ -38,3 +40,25 @@ def test_rows_exchanged_through_lds_are_fenced(tmp_path):
         at = body.rfind("wave_fence")
         assert at >= 0, f"{name} has no fence"
         assert not re.search(r"^\s*(%\S+ = load|store) ", body[at:], re.M), f"{name} touches memory after its fence"
+
+
+def test_staged_tiles_fit_their_offsets(tmp_path):
+    """A tile's rows are addressed from its first by 32 bits of bytes: ``stage<D, waves, rows>`` at the
+    largest token stride that the entry points take."""
+    tiles = {tuple(map(int, m)) for n in _functions("gdn2_attn_train.hip", tmp_path)
+             for m in re.findall(r"5stageILi(\d+)ELi(\d+)ELi(\d+)EE", n)}
+    assert {d for d, _, _ in tiles} == {64, 128}
+    for d, _, rows in tiles:
+        assert (rows - 1) * 2 * 2 ** 25 + 2 * d <= 2 ** 32 - 1, f"{rows} rows of 2^26 bytes"
+
+
+@pytest.mark.parametrize("over,want", [(0, nat.ERR_WORKSPACE), (8, nat.ERR_UNSUPPORTED)])
+@pytest.mark.parametrize("i", [1, 4, 7])
+def test_largest_token_stride(i, over, want):
+    """2^25 elements are taken (the call then ends for its missing workspace, before any launch)."""
+    st = [256, 256, 64] * 3
+    st[i] = 2 ** 25 + over
+    st = (ctypes.c_int64 * 9)(*st)
+    got = nat.load().gdn2_attn_fwd(4096, 4096, 4096, ctypes.addressof(st), 4096, None, 4096,
+                                   nat.DTYPE_BF16, None, None, None, 0, 1, 4, 100000, 4, 2, 64, 1.0, 1, None, 0, None)
+    assert got == want
