@@ -337,7 +337,9 @@ int gdn2_attn_decode(const void *qkv, const float *cos, const float *sin, int ro
  * position, and every q head attends positions 0 .. pos as the cache then holds
  * them, its own included.  A position outside [0, max_len) leaves its
  * sequence's caches alone and writes zeros.  bf16 / fp16, D in {64, 128}, qpk in
- * 1 .. 16; else GDN2_ERR_UNSUPPORTED.  workspace: gdn2_attn_decode_q4_workspace_size()
+ * 1 .. 16, fewer than 2^24 sequences times groups (as many workgroups as a launch takes; times qpk
+ * too where the workspace is not 0; 2^23 of 128 tokens of 64 channels in a store or load); else
+ * GDN2_ERR_UNSUPPORTED.  workspace: gdn2_attn_decode_q4_workspace_size()
  * bytes, 16-byte aligned (may be 0), of which concurrent calls need one each.
  *
  * gdn2_kv_cache_q4_store stores k, v [B, T, G, D] (io_dtype f32 / bf16 / fp16;
@@ -377,7 +379,8 @@ int gdn2_kv_cache_q4_load(const void *k_codes, const void *k_meta, const void *v
  * A row with a NaN or +inf, or of -inf alone, gives NaN (as log_softmax).
  * gdn2_token_logprobs_bwd writes dx [rows][n] (contiguous, io_dtype) from dlogp and
  * dentropy (fp32 [rows]; either may be NULL), x, lse and entropy; a row to which no gradient
- * arrives gets zeros.  Deterministic.
+ * arrives gets zeros.  Deterministic.  Up to 2^27 rows, n up to 2^30; else
+ * GDN2_ERR_UNSUPPORTED.
  */
 size_t gdn2_token_logprobs_workspace_size(int64_t rows, int64_t n, int top_k, int io_dtype);
 int gdn2_token_logprobs_fwd(const void *x, int64_t inner_rows, int64_t outer_stride, int64_t row_stride, int io_dtype,
@@ -412,7 +415,9 @@ int gdn2_token_logprobs_bwd(const void *x, int64_t inner_rows, int64_t outer_str
  * over the query heads of a group, from o, o_lo and lse of the forward and dout
  * [B, Tq, H, D] contiguous; the probabilities are recomputed.  Every output has
  * the same bits in every run.  bf16 / fp16, D in {64, 128}, scale > 0, Tq H / G up
- * to 2^30; else GDN2_ERR_UNSUPPORTED.  workspace: gdn2_attn_fwd_workspace_size() (0 unless few
+ * to 2^30, and no more tiles of 128 rows (over rows or sequences, groups and shares) than
+ * one launch's 2^24 workgroups, in a forward with o_lo those of the gradient's launches too;
+ * else GDN2_ERR_UNSUPPORTED.  workspace: gdn2_attn_fwd_workspace_size() (0 unless few
  * queries face many keys; then it may be NULL) and gdn2_attn_bwd_workspace_size()
  * bytes, 16-byte aligned, of which concurrent calls need one each.
  */

@@ -450,17 +450,18 @@ static int check_q4_cache(const void *kc, const void *km, const void *vc, const 
 {
     if (B < 0 || G < 1 || D < 1 || max_len < 1) return GDN2_ERR_INVALID;
     if (D % 64 != 0 || D > 1024) return GDN2_ERR_UNSUPPORTED;
-    if (max_len > (1 << 30) || static_cast<int64_t>(B) * G > 2147483647LL) return GDN2_ERR_UNSUPPORTED;
+    if (max_len > (1 << 30) || static_cast<int64_t>(B) * G > max_workgroups(256)) return GDN2_ERR_UNSUPPORTED;
     if (B > 0 && (!kc || !km || !vc || !vm)) return GDN2_ERR_INVALID;
     if ((reinterpret_cast<uintptr_t>(kc) | reinterpret_cast<uintptr_t>(vc)) & 15) return GDN2_ERR_INVALID;
     if ((reinterpret_cast<uintptr_t>(km) | reinterpret_cast<uintptr_t>(vm)) & 3) return GDN2_ERR_INVALID;
     return GDN2_OK;
 }
 
-// One launch of at most 2^31 - 1 workgroups (of 128 tokens of one head's group each).
+// One launch (workgroups of 128 tokens of one head's group each).
 static bool q4_launchable(int B, int64_t T, int G, int D)
 {
-    return T <= (1 << 30) && 2.0 * ((T + 127) / 128) * (D / 64) * G * B < 2147483000.0;
+    return T <= (1 << 30) &&
+           2.0 * ((T + 127) / 128) * (D / 64) * G * B <= static_cast<double>(max_workgroups(256));
 }
 
 size_t gdn2_attn_decode_q4_workspace_size(int B, int G, int qpk, int D, int64_t max_len)
@@ -480,9 +481,10 @@ int gdn2_attn_decode_q4(const void *qkv, const float *cos, const float *sin, int
     if (rope_pairs < 0 || 2 * rope_pairs > D || (rope_pairs > 0 && (!cos || !sin))) return GDN2_ERR_INVALID;
     if (rope_row_stride < 0 || (rope_row_stride > 0 && rope_row_stride < rope_pairs)) return GDN2_ERR_INVALID;
     if (!attn_q4_supported(io_dtype, qpk, D) || !(scale > 0.0f) || scale > 1e30f) return GDN2_ERR_UNSUPPORTED;
-    if (static_cast<int64_t>(B) * G * qpk > 2147483647LL) return GDN2_ERR_UNSUPPORTED;
     if (B == 0) return GDN2_OK;
     if (!qkv || !pos || !out) return GDN2_ERR_INVALID;
+    const int splits = attn_q4_splits(B, G, max_len);
+    if (splits > 1 && static_cast<int64_t>(B) * G * qpk > max_workgroups(256)) return GDN2_ERR_UNSUPPORTED;  // the merge
     AttnQ4Params p = {};
     p.qkv = qkv; p.cos = cos; p.sin = sin;
     p.rope_pairs = rope_pairs;
@@ -492,7 +494,7 @@ int gdn2_attn_decode_q4(const void *qkv, const float *cos, const float *sin, int
     p.k_meta = static_cast<unsigned *>(k_meta); p.v_meta = static_cast<unsigned *>(v_meta);
     p.out = out;
     p.max_len = max_len; p.B = B; p.G = G; p.qpk = qpk; p.D = D; p.scale = scale;
-    p.splits = attn_q4_splits(B, G, max_len);
+    p.splits = splits;
     p.part = static_cast<float *>(workspace);
     if (p.splits > 1 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) ||
                          workspace_bytes < gdn2_attn_decode_q4_workspace_size(B, G, qpk, D, max_len)))
@@ -551,7 +553,7 @@ static int fill_logprob_args(LogprobParams &p, const void *x, int64_t inner, int
         return GDN2_ERR_INVALID;
     if (rows > 0 && (!x || !targets)) return GDN2_ERR_INVALID;
     if (reinterpret_cast<uintptr_t>(x) % (io_dtype == GDN2_DTYPE_F32 ? 4 : 2) != 0) return GDN2_ERR_INVALID;
-    // One launch of rows * parts workgroups; indices of a row in 32 bits.
+    // Indices of a row, and of a row's parts, in 32 bits.
     if (rows > (1 << 27) || n > (1 << 30)) return GDN2_ERR_UNSUPPORTED;
     p.x = x;
     p.inner = inner; p.outer_stride = outer_stride; p.row_stride = row_stride;
@@ -605,7 +607,6 @@ int gdn2_token_logprobs_bwd(const void *x, int64_t inner_rows, int64_t outer_str
     if (rows == 0) return GDN2_OK;
     if (!entropy || !lse || !dx || reinterpret_cast<uintptr_t>(dx) % (io_dtype == GDN2_DTYPE_F32 ? 4 : 2) != 0)
         return GDN2_ERR_INVALID;
-    if ((n / 8192 + 1) * rows > 2147483647LL) return GDN2_ERR_UNSUPPORTED;
     p.entropy = const_cast<float *>(entropy);
     p.lse = const_cast<float *>(lse);
     p.dlogp = dlogp; p.dent = dentropy;
@@ -613,9 +614,11 @@ int gdn2_token_logprobs_bwd(const void *x, int64_t inner_rows, int64_t outer_str
     return launch_logprobs_bwd(p, io_dtype, static_cast<hipStream_t>(stream)) == hipSuccess ? GDN2_OK : GDN2_ERR_LAUNCH;
 }
 
-// The sizes gdn2_attn_fwd, gdn2_attn_bwd and its workspace depend on, checked.
+// The sizes gdn2_attn_fwd, gdn2_attn_bwd and its workspace depend on, checked.  `backward`: also what
+// the gradient's launches take (of a forward that keeps what they read as well, so that none
+// succeeds whose gradient is refused).
 static int fill_attn_sizes(AttnTrainParams &p, const int64_t *cu_host, int num_seqs, int B, int Tq, int Tk, int H,
-                           int G, int D, int causal)
+                           int G, int D, int causal, bool backward)
 {
     if (B < 0 || Tq < 0 || Tk < 0 || H < 1 || G < 1 || D < 1 || H % G != 0) return GDN2_ERR_INVALID;
     if (Tq > (1 << 30) || Tk > (1 << 30) || B > (1 << 30) || H > (1 << 20) || D > (1 << 20) || num_seqs > (1 << 30))
@@ -645,11 +648,7 @@ static int fill_attn_sizes(AttnTrainParams &p, const int64_t *cu_host, int num_s
     p.causal = causal != 0;
     p.splits = attn_bwd_splits(p);
     p.splits_f = p.splits_q = attn_key_shares(p);
-    // One launch of at most 2^31 - 1 workgroups (packed rows: up to 8 times their tiles; an
-    // eighth more where the last deal of groups is short).
-    const double most = cu_host ? 1.9e9 / 8 : 1.9e9;
-    if (static_cast<double>(p.q_tiles) * G * p.splits_f > most || static_cast<double>(p.k_tiles) * G * p.splits > most ||
-        static_cast<double>(B) * Tq * H > 17179869184.0 ||
+    if (!attn_launchable(p, backward) || static_cast<double>(B) * Tq * H > 17179869184.0 ||
         static_cast<double>(B) * (H + G) > 500000000.0 || static_cast<double>(B) * Tk * G * D > 500000000000.0)
         return GDN2_ERR_UNSUPPORTED;
     return GDN2_OK;
@@ -658,11 +657,12 @@ static int fill_attn_sizes(AttnTrainParams &p, const int64_t *cu_host, int num_s
 // Shared by gdn2_attn_fwd and gdn2_attn_bwd: checks, and the parameters both take.
 static int fill_attn_args(AttnTrainParams &p, const void *q, const void *k, const void *v, const int64_t *strides,
                           int io_dtype, const int64_t *kv_lengths, const int64_t *cu, const int64_t *cu_host,
-                          int num_seqs, int B, int Tq, int Tk, int H, int G, int D, float scale, int causal)
+                          int num_seqs, int B, int Tq, int Tk, int H, int G, int D, float scale, int causal,
+                          bool backward)
 {
     if (!valid_dtype(io_dtype) || !strides || (cu == nullptr) != (cu_host == nullptr) || (cu && kv_lengths))
         return GDN2_ERR_INVALID;
-    const int st = fill_attn_sizes(p, cu_host, num_seqs, B, Tq, Tk, H, G, D, causal);
+    const int st = fill_attn_sizes(p, cu_host, num_seqs, B, Tq, Tk, H, G, D, causal, backward);
     if (st != GDN2_OK) return st;
     if (!attn_train_supported(io_dtype, D)) return GDN2_ERR_UNSUPPORTED;
     if (!(scale > 0.0f) || scale > 1e30f) return GDN2_ERR_UNSUPPORTED;
@@ -691,7 +691,7 @@ int gdn2_attn_fwd(const void *q, const void *k, const void *v, const int64_t *st
 {
     AttnTrainParams p = {};
     const int st = fill_attn_args(p, q, k, v, strides, io_dtype, kv_lengths, cu_seqlens, cu_seqlens_host, num_seqs, B,
-                                  Tq, Tk, H, G, D, scale, causal);
+                                  Tq, Tk, H, G, D, scale, causal, o_lo != nullptr);
     if (st != GDN2_OK) return st;
     if (B == 0 || Tq == 0 || p.nseq == 0) return GDN2_OK;
     if (!o || !lse || ((reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(o_lo)) & 15)) return GDN2_ERR_INVALID;
@@ -709,7 +709,7 @@ size_t gdn2_attn_fwd_workspace_size(const int64_t *cu_seqlens_host, int num_seqs
                                     int D, int causal)
 {
     AttnTrainParams p = {};
-    if (fill_attn_sizes(p, cu_seqlens_host, num_seqs, B, Tq, Tk, H, G, D, causal) != GDN2_OK) return 0;
+    if (fill_attn_sizes(p, cu_seqlens_host, num_seqs, B, Tq, Tk, H, G, D, causal, false) != GDN2_OK) return 0;
     return attn_fwd_workspace_bytes(p);
 }
 
@@ -717,7 +717,7 @@ size_t gdn2_attn_bwd_workspace_size(const int64_t *cu_seqlens_host, int num_seqs
                                     int D, int causal)
 {
     AttnTrainParams p = {};
-    if (fill_attn_sizes(p, cu_seqlens_host, num_seqs, B, Tq, Tk, H, G, D, causal) != GDN2_OK) return 0;
+    if (fill_attn_sizes(p, cu_seqlens_host, num_seqs, B, Tq, Tk, H, G, D, causal, true) != GDN2_OK) return 0;
     return attn_bwd_workspace_bytes(p);
 }
 
@@ -729,7 +729,7 @@ int gdn2_attn_bwd(const void *q, const void *k, const void *v, const int64_t *st
 {
     AttnTrainParams p = {};
     const int st = fill_attn_args(p, q, k, v, strides, io_dtype, kv_lengths, cu_seqlens, cu_seqlens_host, num_seqs, B,
-                                  Tq, Tk, H, G, D, scale, causal);
+                                  Tq, Tk, H, G, D, scale, causal, true);
     if (st != GDN2_OK) return st;
     if (B == 0 || p.nseq == 0 || (Tq == 0 && Tk == 0)) return GDN2_OK;
     if ((Tq > 0 && (!o || !o_lo || !lse || !dout || !dq)) || (Tk > 0 && (!dk || !dv))) return GDN2_ERR_INVALID;

@@ -736,16 +736,18 @@ __global__ __launch_bounds__(256) void attn_fwd_join_kernel(AttnTrainParams p)
 // fp16 only: the largest squared row norms of dO per (batch row, head) and of V per
 // (batch row, group), from which the kernels below scale dS into fp16's range;
 // kNormParts workgroups each, [B][heads][kNormParts].  Rows that are not finite,
-// or past the row's length, do not count.
+// or past the row's length, do not count.  `first`: of the launch's workgroups, where
+// there are more than one launch takes.
 constexpr int kNormParts = 4;
 template <int D>
-__global__ __launch_bounds__(256) void norm_max_kernel(AttnTrainParams p)
+__global__ __launch_bounds__(256) void norm_max_kernel(AttnTrainParams p, unsigned first)
 {
     constexpr int P = D / 8, R = 256 / P;
     __shared__ float s_best[4];
     const int ndo = p.B * p.H;
-    const int part = blockIdx.x % kNormParts;
-    int bh = blockIdx.x / kNormParts;
+    const unsigned wg = first + blockIdx.x;
+    const int part = static_cast<int>(wg % kNormParts);
+    int bh = static_cast<int>(wg / kNormParts);
     const bool is_v = bh >= ndo;
     if (is_v) bh -= ndo;
     const int heads = is_v ? p.G : p.H, b = bh / heads, hh = bh - b * heads;
@@ -1258,7 +1260,7 @@ static_assert(32 * kWaves == 128, "q_tiles, k_tiles and packed_tile count tiles 
 // Sets that, the tiles, and `dealt` (turn_of), for a launch over `all` tiles of a group (a
 // token being `rows` of their rows) in `shares`; returns its workgroups.  Dealt from 4096
 // workgroups (four to eight rounds), of enough groups that a short last deal does not count.
-unsigned set_grid(AttnTrainParams &p, int64_t all, int64_t rows, int shares)
+int64_t set_grid(AttnTrainParams &p, int64_t all, int64_t rows, int shares)
 {
     p.tiles = static_cast<int>(p.cu ? (p.max_q * rows + 127) / 128 : all / p.nseq);
     const int64_t even = static_cast<int64_t>(p.nseq) * p.tiles;
@@ -1266,7 +1268,7 @@ unsigned set_grid(AttnTrainParams &p, int64_t all, int64_t rows, int shares)
     const int64_t groups = static_cast<int64_t>(p.ranked ? 1 : p.nseq) * p.G;
     const int64_t tiles = (p.ranked ? all : p.tiles) * shares;
     p.dealt = tiles * groups >= 4096 && (groups % 8 == 0 || groups >= 64);
-    return static_cast<unsigned>((p.dealt ? (groups + 7) / 8 * 8 : groups) * tiles);
+    return (p.dealt ? (groups + 7) / 8 * 8 : groups) * tiles;
 }
 
 // Whether P and dS are multiplied in two parts.  In short sequences few rounded terms make
@@ -1284,7 +1286,7 @@ bool attn_fine(const AttnTrainParams &p)
 template <PrecKind PK, int D>
 hipError_t fwd_d(AttnTrainParams p, hipStream_t s)
 {
-    const unsigned grid = set_grid(p, p.q_tiles, p.H / p.G, p.splits_f);
+    const unsigned grid = static_cast<unsigned>(set_grid(p, p.q_tiles, p.H / p.G, p.splits_f));
     hipLaunchKernelGGL((attn_fine(p) ? attn_fwd_kernel<PK, D, kWaves, true> : attn_fwd_kernel<PK, D, kWaves, false>),
                        dim3(grid), dim3(64 * kWaves), 0, s, p);
     const hipError_t e = hipGetLastError();
@@ -1300,11 +1302,15 @@ hipError_t bwd_d(AttnTrainParams p, hipStream_t s)
 {
     hipError_t e;
     if constexpr (PK == PrecKind::F16) {
-        hipLaunchKernelGGL((norm_max_kernel<D>), dim3(kNormParts * p.B * (p.H + p.G)), dim3(256), 0, s, p);
-        if ((e = hipGetLastError()) != hipSuccess) return e;
+        const int64_t all = static_cast<int64_t>(kNormParts) * p.B * (p.H + p.G), most = max_workgroups(256);
+        for (int64_t first = 0; first < all; first += most) {
+            hipLaunchKernelGGL((norm_max_kernel<D>), dim3(static_cast<unsigned>(all - first < most ? all - first : most)),
+                               dim3(256), 0, s, p, static_cast<unsigned>(first));
+            if ((e = hipGetLastError()) != hipSuccess) return e;
+        }
     }
     if (p.Tq > 0 && p.max_q > 0) {
-        const unsigned grid = set_grid(p, p.q_tiles, p.H / p.G, p.splits_q);
+        const unsigned grid = static_cast<unsigned>(set_grid(p, p.q_tiles, p.H / p.G, p.splits_q));
         hipLaunchKernelGGL((attn_fine(p) ? attn_dq_kernel<PK, D, kWaves, true> : attn_dq_kernel<PK, D, kWaves, false>),
                            dim3(grid), dim3(64 * kWaves), 0, s, p);
         if ((e = hipGetLastError()) != hipSuccess) return e;
@@ -1315,7 +1321,7 @@ hipError_t bwd_d(AttnTrainParams p, hipStream_t s)
         // Query rows per tile: at D = 128 half of the other's, so that two
         // workgroups' tiles and V rows fit a CU's LDS.
         constexpr int BQ = D == 64 ? 64 : 32;
-        const unsigned grid = set_grid(p, p.k_tiles, 1, p.splits);
+        const unsigned grid = static_cast<unsigned>(set_grid(p, p.k_tiles, 1, p.splits));
         hipLaunchKernelGGL((attn_fine(p) ? attn_dkv_kernel<PK, D, kWaves, BQ, true>
                                          : attn_dkv_kernel<PK, D, kWaves, BQ, false>),
                            dim3(grid), dim3(64 * kWaves), 0, s, p);
@@ -1332,6 +1338,20 @@ hipError_t bwd_d(AttnTrainParams p, hipStream_t s)
 bool attn_train_supported(int io_dtype, int D)
 {
     return (io_dtype == GDN2_DTYPE_BF16 || io_dtype == GDN2_DTYPE_F16) && (D == 64 || D == 128);
+}
+
+// The joins and sums of shares are small: shares are made of few workgroups.
+bool attn_launchable(const AttnTrainParams &p, bool backward)
+{
+    AttnTrainParams q = p;
+    const int64_t most = max_workgroups(64 * kWaves);
+    // Before the exact count: every tile takes a workgroup, and the products below fit 64 bits.
+    if (static_cast<double>(p.q_tiles) * p.G * p.splits_f > static_cast<double>(most) ||
+        (backward && static_cast<double>(p.k_tiles) * p.G * p.splits > static_cast<double>(most)))
+        return false;
+    if (p.nseq == 0) return true;
+    return (p.q_tiles == 0 || set_grid(q, p.q_tiles, p.H / p.G, p.splits_f) <= most) &&
+           (!backward || p.k_tiles == 0 || set_grid(q, p.k_tiles, 1, p.splits) <= most);
 }
 
 // Shares of a key tile's queries in attn_dkv_kernel.  Two workgroups fit a CU: 512

@@ -309,6 +309,9 @@ hipError_t launch_attn_decode(const AttnDecodeParams &p, int io_dtype, hipStream
 // contiguous; lse, delta [B, H, Tq] (lse: base-2 log of the softmax sum).
 // Query i sees key j < kv_len[b] (or Tk), with causal only j <= i + Tk - Tq; or,
 // with cu (B = 1, Tq = Tk), the keys of its own packed sequence, causal within it.
+// Workgroups of one launch: HIP takes fewer than 2^32 threads along an axis of the grid.
+constexpr int64_t max_workgroups(int threads) { return 0xffffffffLL / threads; }
+
 constexpr int64_t kMaxTokenStride = 1 << 25;  // elements: a tile's offsets are 32 bits of bytes
 struct AttnTrainParams {
     const void *q, *k, *v;
@@ -346,6 +349,8 @@ size_t attn_bwd_workspace(AttnTrainParams &p, void *workspace);
 int attn_key_shares(const AttnTrainParams &p);
 size_t attn_fwd_workspace_bytes(const AttnTrainParams &p);
 void attn_fwd_workspace(AttnTrainParams &p, void *workspace);
+// Whether each kernel of the forward (with `backward` also of the gradient) is one launch.
+bool attn_launchable(const AttnTrainParams &p, bool backward);
 hipError_t launch_attn_fwd(const AttnTrainParams &p, int io_dtype, hipStream_t stream);
 hipError_t launch_attn_bwd(const AttnTrainParams &p, int io_dtype, hipStream_t stream);
 
@@ -364,6 +369,7 @@ struct LogprobParams {
     int64_t *top_ids;
     const float *dlogp, *dent;  // backward: [rows] or NULL
     void *dx;                   // [rows][n], contiguous
+    int64_t row0;               // first row of a launch, set by the launchers
     int parts;                  // per row (logprob_parts; the backward sets its own)
     int64_t pieces_per_part;    // set by the launchers
     float *part_stat;           // [rows][parts][4]

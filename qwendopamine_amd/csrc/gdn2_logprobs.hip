@@ -226,8 +226,9 @@ __global__ __launch_bounds__(64) void logp_part_kernel(LogprobParams p)
     constexpr int EPP = Piece<T>::N;
     __shared__ u64 s_list[TOP ? kCand : 1];
     const int lane = threadIdx.x;
-    const int64_t row = blockIdx.x / p.parts;
-    const int part = static_cast<int>(blockIdx.x - row * p.parts);
+    const unsigned r = blockIdx.x / p.parts;
+    const int64_t row = p.row0 + r;
+    const int part = static_cast<int>(blockIdx.x - r * p.parts);
     const T *x = static_cast<const T *>(p.x) + row_offset(p, row);
     const int head = head_of(x, p.n);
     const int64_t pieces = (p.n - head) / EPP;
@@ -352,7 +353,7 @@ __global__ __launch_bounds__(64) void logp_merge_kernel(LogprobParams p)
 {
     __shared__ u64 s_list[TOP ? kCand : 1];
     const int lane = threadIdx.x;
-    const int64_t row = blockIdx.x;
+    const int64_t row = p.row0 + blockIdx.x;
     Stat a = {-INFINITY, 0.0f, 0.0f};
     for (int i = lane; i < p.parts; i += 64) {
         const float4 st = *reinterpret_cast<const float4 *>(p.part_stat + (row * p.parts + i) * 4);
@@ -397,8 +398,9 @@ template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void logp_bwd_kernel(LogprobParams p)
 {
     constexpr int EPP = Piece<T>::N;
-    const int64_t row = blockIdx.x / p.parts;
-    const int64_t part = blockIdx.x - row * p.parts;
+    const unsigned r = blockIdx.x / p.parts;
+    const int64_t row = p.row0 + r;
+    const int64_t part = blockIdx.x - r * p.parts;
     const T *x = static_cast<const T *>(p.x) + row_offset(p, row);
     T *dx = static_cast<T *>(p.dx) + row * p.n;
     const int64_t t = p.targets[row];
@@ -478,23 +480,38 @@ __global__ __launch_bounds__(256) void logp_bwd_kernel(LogprobParams p)
     }
 }
 
-template <typename T>
-void fwd_launch(const LogprobParams &p, hipStream_t s)
+// launch(p, rows) over all rows, as many at a time as one launch of `threads` per part takes.
+template <typename Launch>
+hipError_t by_rows(LogprobParams p, int threads, Launch launch)
 {
-    const dim3 grid(static_cast<unsigned>(p.rows * p.parts));
-    if (p.top > 0)
-        hipLaunchKernelGGL((logp_part_kernel<T, true>), grid, dim3(64), 0, s, p);
-    else
-        hipLaunchKernelGGL((logp_part_kernel<T, false>), grid, dim3(64), 0, s, p);
-    if (p.parts == 1) return;
-    if (p.top > 0)
-        hipLaunchKernelGGL((logp_merge_kernel<T, true>), dim3(static_cast<unsigned>(p.rows)), dim3(64), 0, s, p);
-    else
-        hipLaunchKernelGGL((logp_merge_kernel<T, false>), dim3(static_cast<unsigned>(p.rows)), dim3(64), 0, s, p);
+    const int64_t most = max_workgroups(threads) / p.parts;
+    for (p.row0 = 0; p.row0 < p.rows; p.row0 += most) {
+        launch(p, p.rows - p.row0 < most ? p.rows - p.row0 : most);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 template <typename T>
-void bwd_launch(LogprobParams p, hipStream_t s)
+hipError_t fwd_launch(const LogprobParams &all, hipStream_t s)
+{
+    return by_rows(all, 64, [&](const LogprobParams &p, int64_t rows) {
+        const dim3 grid(static_cast<unsigned>(rows * p.parts)), merges(static_cast<unsigned>(rows));
+        if (p.top > 0)
+            hipLaunchKernelGGL((logp_part_kernel<T, true>), grid, dim3(64), 0, s, p);
+        else
+            hipLaunchKernelGGL((logp_part_kernel<T, false>), grid, dim3(64), 0, s, p);
+        if (p.parts == 1) return;
+        if (p.top > 0)
+            hipLaunchKernelGGL((logp_merge_kernel<T, true>), merges, dim3(64), 0, s, p);
+        else
+            hipLaunchKernelGGL((logp_merge_kernel<T, false>), merges, dim3(64), 0, s, p);
+    });
+}
+
+template <typename T>
+hipError_t bwd_launch(LogprobParams p, hipStream_t s)
 {
     constexpr int EPP = Piece<T>::N;
     // Whole rows of x at the same offsets from 16-byte boundaries as dx's.
@@ -505,11 +522,13 @@ void bwd_launch(LogprobParams p, hipStream_t s)
     const int64_t pieces = (p.n + EPP - 1) / EPP;
     p.pieces_per_part = 2048;
     p.parts = static_cast<int>((pieces + p.pieces_per_part - 1) / p.pieces_per_part);
-    const dim3 grid(static_cast<unsigned>(p.rows * p.parts));
-    if (vec)
-        hipLaunchKernelGGL((logp_bwd_kernel<T, true>), grid, dim3(256), 0, s, p);
-    else
-        hipLaunchKernelGGL((logp_bwd_kernel<T, false>), grid, dim3(256), 0, s, p);
+    return by_rows(p, 256, [&](const LogprobParams &p, int64_t rows) {
+        const dim3 grid(static_cast<unsigned>(rows * p.parts));
+        if (vec)
+            hipLaunchKernelGGL((logp_bwd_kernel<T, true>), grid, dim3(256), 0, s, p);
+        else
+            hipLaunchKernelGGL((logp_bwd_kernel<T, false>), grid, dim3(256), 0, s, p);
+    });
 }
 
 }  // namespace
@@ -532,21 +551,19 @@ hipError_t launch_logprobs(LogprobParams p, int io_dtype, hipStream_t s)
     p.pieces_per_part = (chunks + p.parts - 1) / p.parts * (64 * kU);
     if (p.pieces_per_part == 0) p.pieces_per_part = 64 * kU;
     switch (io_dtype) {
-    case GDN2_DTYPE_F32: fwd_launch<float>(p, s); break;
-    case GDN2_DTYPE_BF16: fwd_launch<bf16_t>(p, s); break;
-    default: fwd_launch<f16_t>(p, s); break;
+    case GDN2_DTYPE_F32: return fwd_launch<float>(p, s);
+    case GDN2_DTYPE_BF16: return fwd_launch<bf16_t>(p, s);
+    default: return fwd_launch<f16_t>(p, s);
     }
-    return hipGetLastError();
 }
 
 hipError_t launch_logprobs_bwd(const LogprobParams &p, int io_dtype, hipStream_t s)
 {
     switch (io_dtype) {
-    case GDN2_DTYPE_F32: bwd_launch<float>(p, s); break;
-    case GDN2_DTYPE_BF16: bwd_launch<bf16_t>(p, s); break;
-    default: bwd_launch<f16_t>(p, s); break;
+    case GDN2_DTYPE_F32: return bwd_launch<float>(p, s);
+    case GDN2_DTYPE_BF16: return bwd_launch<bf16_t>(p, s);
+    default: return bwd_launch<f16_t>(p, s);
     }
-    return hipGetLastError();
 }
 
 }  // namespace gdn2

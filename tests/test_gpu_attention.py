@@ -426,3 +426,16 @@ def test_attention_tokens_at_the_largest_stride(gpu_device, T, D):
         at += h * D
     got = _run(*far, x[3])
     assert all(torch.equal(want[n], got[n]) for n in want)
+
+
+def test_attention_float16_gradients_of_many_rows(gpu_device):
+    """65536 rows of one token, 32 heads: the norms that scale fp16's dS take more than one launch.  A
+    query that sees one key: o is its v, dv its dout, dq and dk zero."""
+    print("[case] attention fp16 B65536 T1 H32 D64", flush=True)
+    B, H, D = 65536, 32, 64
+    gen = torch.Generator(gpu_device).manual_seed(3)
+    q, k, v, do = (torch.randn(B, 1, H, D, generator=gen, device=gpu_device, dtype=FP) for _ in range(4))
+    x = [z.requires_grad_(True) for z in (q, k, v)]
+    got = _run(*x, do)
+    assert torch.equal(got["o"], v) and torch.equal(got["dv"], do)
+    assert not got["dq"].any() and not got["dk"].any()

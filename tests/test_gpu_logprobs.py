@@ -248,3 +248,31 @@ def test_logprobs_captured_and_repeated(gpu_device):
         g.replay()
         want, dwant = _run(new[0], new[1], 20, gl, ge)
         assert all(torch.equal(a, b) for a, b in zip(r, want)) and torch.equal(dx, dwant)
+
+
+@pytest.mark.parametrize("rows,V,top", [(2 ** 24 + 5, 4, 0), (2 ** 26 + 3, 2, 1)])
+def test_logprobs_more_rows_than_a_launch(gpu_device, rows, V, top):
+    """Past 2^24 rows the backward, past 2^26 the forward takes more than one launch.  Logits of 0, 1, 2
+    and 3, so that float32 results of few values are known for all rows at once."""
+    from qwendopamine_amd import ops
+
+    print(f"[case] logprobs {rows}x{V}", flush=True)
+    r = torch.arange(rows, device=gpu_device)
+    hot = (r * 7 + r // 1000) % V
+    x = torch.nn.functional.one_hot(hot, V).to(BF) * ((r % 4)[:, None]).to(BF)
+    x.requires_grad_(True)
+    t = (r // 3) % V
+    out = ops.token_logprobs(x, t, top_k=top)
+    gl = ((r % 5) - 2).float()
+    (dx,) = torch.autograd.grad(out.logprobs, x, gl)
+    for lo in range(0, rows, 2 ** 24):
+        s = slice(lo, min(rows, lo + 2 ** 24))
+        lp = x[s].detach().double().log_softmax(-1)
+        one = torch.nn.functional.one_hot(t[s], V).double()
+        want = (one - lp.exp()) * gl[s, None].double()
+        assert float((out.logprobs[s].detach().double() - (lp * one).sum(-1)).abs().max()) <= 2e-6 * 5
+        # Rounded once to bf16, whose half step is 2^-9 of a value's power of two.
+        assert bool(((dx[s].double() - want).abs() <= 2.0 ** -8 * want.abs() + 1e-5).all())
+        if top:
+            first = torch.where((r[s] % 4) == 0, 0, hot[s])
+            assert torch.equal(out.top_ids[s, 0], first)

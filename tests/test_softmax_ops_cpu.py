@@ -235,3 +235,45 @@ def test_packed_offsets_are_copied(make):
     cu[1], cu[2] = 399, 399
     assert host.tolist() == [0, 5, 70, 400] and dev.tolist() == [0, 5, 70, 400]
     assert host.dtype == torch.int64 and host.is_contiguous()
+
+
+# A launch holds fewer than 2^32 threads: sizes beyond are refused before any (or take several).
+
+@pytest.mark.parametrize("over", [
+    dict(B=1 << 20, Tq=1, Tk=1, H=32, G=32),                                   # a workgroup per row and head
+    dict(B=1 << 24, Tq=1, Tk=1, H=1, G=1),
+    dict(cu=4096, cu_host=tuple(range((1 << 20) + 1)), n=1 << 20, Tq=1 << 20, Tk=1 << 20, H=32, G=32),
+])
+def test_attention_refuses_more_than_a_launch(lib, over):
+    assert _attn_call(lib, **over) == nat.ERR_UNSUPPORTED
+
+
+def test_attention_forward_for_a_gradient_is_refused_with_it(lib):
+    """Few queries over the long keys of very many rows: their forward is one launch, the gradient of
+    the keys is not.  A forward that keeps what the gradient reads is refused as it is (the calls end
+    for what they lack, before any launch)."""
+    B, Tk, st = 1 << 23, 257, (ctypes.c_int64 * 9)(*(256, 256, 64) * 3)
+
+    def call(o, o_lo):
+        return lib.gdn2_attn_fwd(4096, 4096, 4096, ctypes.addressof(st), o, o_lo, 4096, nat.DTYPE_BF16, None, None, None,
+                                 0, B, 1, Tk, 1, 1, 64, 1.0, 1, None, 0, None)
+
+    assert call(None, None) == nat.ERR_INVALID  # sizes accepted, no output given
+    assert call(None, 4096) == nat.ERR_UNSUPPORTED
+    size = lib.gdn2_attn_bwd_workspace_size
+    assert size(None, 0, B, 1, Tk, 1, 1, 64, 1) == 0 and size(None, 0, 1 << 10, 1, Tk, 1, 1, 64, 1) > 0
+
+
+def test_four_bit_cache_refuses_more_than_a_launch(lib):
+    def decode(B, G, qpk=1, L=10):
+        return lib.gdn2_attn_decode_q4(4096, 4096, 4096, 32, 32, 4096, 0, 4096, 4096, 4096, 4096, 4096, nat.DTYPE_BF16, B,
+                                       G, qpk, 64, L, 1.0, None, 0, None)
+
+    assert decode(1 << 20, 32) == nat.ERR_UNSUPPORTED
+    assert decode(1 << 16, 32, 16, 5000) == nat.ERR_UNSUPPORTED  # shares: a merge per query head
+    st = (ctypes.c_int64 * 6)(*(256, 256, 64) * 2)
+    store = (4096, 4096, ctypes.addressof(st), nat.DTYPE_BF16, None, 0, 4096, 4096, 4096, 4096)
+    load = (4096, 4096, 4096, 4096, None, 0, 4096, 4096, nat.DTYPE_BF16)
+    for f, head in ((lib.gdn2_kv_cache_q4_store, store), (lib.gdn2_kv_cache_q4_load, load)):
+        assert f(*head, 1 << 19, 1, 32, 64, 10, None) == nat.ERR_UNSUPPORTED
+        assert f(*head, 4, 1 << 29, 1, 64, 10, None) == nat.ERR_UNSUPPORTED
