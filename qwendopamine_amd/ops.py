@@ -28,6 +28,7 @@ import ctypes
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.forward_ad import unpack_dual
 
 from . import _native as nat
 
@@ -1522,6 +1523,13 @@ def _on_device(device: torch.device):
     return torch.cuda.device(device)
 
 
+def _differentiated(*xs: torch.Tensor) -> bool:
+    """Whether a derivative is asked for: a gradient, or a forward-mode tangent, which the autograd
+    functions refuse (called past them, an operator would drop it and pass for constant)."""
+    return (torch.is_grad_enabled() and any(x.requires_grad for x in xs)) or any(
+        unpack_dual(x).tangent is not None for x in xs)
+
+
 def _head_rows(x: torch.Tensor) -> torch.Tensor:
     """``x [B, T, heads, D]`` as the attention kernels read it: in place where its channels are
     contiguous and every row starts on 16 bytes, else a contiguous copy."""
@@ -1633,7 +1641,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float | 
     products (sequences of up to 128 tokens: multiplied in two parts, with twice the bits).  The
     gradients have the same bits in every run.  In a HIP graph, capture the forward and backward
     together with no eager autograd graph of the same leaves alive, as torch asks of any captured
-    backward.
+    backward.  Second derivatives and forward-mode tangents are refused.
     """
     name = "attention"
     if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape:
@@ -1665,7 +1673,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float | 
             raise ValueError(f"{name}: tensors on {q.device} and {t.device}")
     kv_len = None if kv_lengths is None else kv_lengths.detach().to(torch.int64).contiguous()
     cu_dev, cu_host = _cu(cu_seqlens, q.device, Tq)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if _differentiated(q, k, v):
         return AttentionFunction.apply(q, k, v, scale, int(causal), kv_len, cu_dev, cu_host)
     return _attention_fwd(_head_rows(q), _head_rows(k), _head_rows(v), scale, int(causal), kv_len, cu_dev, cu_host,
                           False)[0]
@@ -1934,7 +1942,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0,
     does; single -inf logits have probability 0 and pass no gradient.  Sums are float32, the
     gradient is rounded once to the logits' dtype; everything has the same bits in every run.
     In a HIP graph, capture the forward and backward together with no eager autograd graph of the
-    same leaves alive, as torch asks of any captured backward.
+    same leaves alive, as torch asks of any captured backward.  Second derivatives and forward-mode
+    tangents are refused.
     """
     name = "token_logprobs"
     if logits.dim() < 1 or logits.shape[-1] < 1:
@@ -1951,7 +1960,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0,
     if targets.device != logits.device:
         raise ValueError(f"{name}: tensors on {logits.device} and {targets.device}")
     args = logits, targets.contiguous(), int(top_k), int(ignore_index)
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if _differentiated(logits):
         return TokenLogprobs(*TokenLogprobsFunction.apply(*args))
     return TokenLogprobs(*_token_logprobs_fwd(*args, False)[:4])
 

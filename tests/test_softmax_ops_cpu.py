@@ -277,3 +277,26 @@ def test_four_bit_cache_refuses_more_than_a_launch(lib):
     for f, head in ((lib.gdn2_kv_cache_q4_store, store), (lib.gdn2_kv_cache_q4_load, load)):
         assert f(*head, 1 << 19, 1, 32, 64, 10, None) == nat.ERR_UNSUPPORTED
         assert f(*head, 4, 1 << 29, 1, 64, 10, None) == nat.ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_tangents_are_refused(monkeypatch, grad):
+    """A tangent on any input, with and without gradients, never yields a result without one.  The
+    launches are stood in for."""
+    from torch.autograd import forward_ad
+
+    monkeypatch.setattr(ops, "_require_gpu", lambda *a: None)
+    monkeypatch.setattr(ops, "_attention_fwd", lambda q, *a: (torch.zeros_like(q),) * 3)
+    monkeypatch.setattr(ops, "_token_logprobs_fwd",
+                        lambda x, t, *a: (torch.zeros(t.shape), torch.zeros(t.shape), None, None, x, None))
+    logits, targets = torch.zeros(3, 5), torch.zeros(3, dtype=torch.int64)
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        for i in range(3):
+            x = list(_qkv())
+            x[i] = forward_ad.make_dual(x[i], torch.ones_like(x[i]))
+            with pytest.raises(NotImplementedError):
+                ops.attention(*x)
+        with pytest.raises(NotImplementedError):
+            ops.token_logprobs(forward_ad.make_dual(logits, torch.ones_like(logits)), targets)
+        # Without a tangent nothing changes within the level.
+        assert ops.attention(*_qkv()).shape == (2, 5, 4, 64) and ops.token_logprobs(logits, targets).logprobs.shape == (3,)
