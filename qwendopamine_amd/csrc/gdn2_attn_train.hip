@@ -36,10 +36,20 @@ constexpr float kLog2e = 1.4426950408889634f;
 // Reference of a share of the keys that holds none a query sees: finite, below
 // every score, so that differences of references are never inf - inf.
 constexpr float kNoMax = -3.0e38f;
-// The running maximum moves only when a score exceeds it by 2^kLazy: until
-// then the probabilities are at most 2^kLazy, exact in the same number of
-// bits, and the accumulators need no rescaling.
-constexpr float kLazy = 8.0f;
+// The reference of the exponents lies `down` below the running maximum, and moves only when
+// a score exceeds the maximum it was set by by `lazy`: until then the probabilities
+// are at most 2^(down + lazy), exact in the same number of bits, and the accumulators need
+// no rescaling.  bf16 has the exponents of fp32 and keeps a probability's 8 bits anywhere.
+// fp16 is normal from 2^-14 on only: with the largest probability held at 2^13 .. 2^15,
+// 2^-27 of it still has 11 bits, and what is below is off by at most 2^-38 of it (at
+// down = 0 a row lost every key under 2^-25 of its largest, while the sum counted them).
+// Its smaller `lazy` costs 0.5% (fp16 forward, against down 0 and lazy 8: B2 T8192 H16 G4 D128
+// causal 571 and 575 us, B4 T2048 H16 D64 54.2 and 54.4).
+template <PrecKind PK>
+struct Ref {
+    static constexpr float down = PK == PrecKind::F16 ? 13.0f : 0.0f, lazy = PK == PrecKind::F16 ? 2.0f : 8.0f;
+    static constexpr float undo = PK == PrecKind::F16 ? 0x1p-13f : 1.0f;  // 2^-down
+};
 constexpr int kTile = 64;  // rows of the streamed side per LDS tile
 
 template <PrecKind PK>
@@ -211,8 +221,9 @@ __device__ __forceinline__ uint4 col_frag(const char *tile, int at, int r0, int 
 
 // acc[d] += (columns 32 d .. of the tile)^T X for rows r0 + 16 t .. of it, X the elements 8 t ..
 // 8 t + 7 of x.  X is rounded to the operand type: a relative error of half a step
-// each, as large as the rounding of the result.  Of FINE calls (attn_fine) also what
-// that left out is multiplied.
+// each (fp16: of what Ref and ds_scale keep normal), as large as the rounding of the result, so
+// that results are off by 1.4 to 1.5 times that rounding.  Of FINE calls (attn_fine) also
+// what that left out is multiplied.
 template <PrecKind PK, int D, bool FINE>
 __device__ __forceinline__ void add_columns(f32x16 (&acc)[D / 32], const char *tile, int at, int r0, const f32x16 &x)
 {
@@ -496,10 +507,12 @@ __device__ __forceinline__ void write_rows(const char *so, int lane, uint16_t *o
 
 // ---------------------------------------------------------------- forward
 
-// L in base 2.  A query that sees no key: +inf, which makes its recomputed P zero.
+// L in base 2 from the reference and the sum.  A query that sees no key: +inf, which makes its
+// recomputed P zero.
+template <PrecKind PK>
 __device__ __forceinline__ float log_sum(float m, float l)
 {
-    return l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
+    return l == 0.0f ? INFINITY : (m + Ref<PK>::down) + __builtin_amdgcn_logf(l * Ref<PK>::undo);
 }
 
 // Four channels of O, and, for D = dO . O, what their rounding left out: without it D is
@@ -564,7 +577,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void attn_fwd_kernel(Attn
     const int wend = p.causal && wmax + w.shift + 1 < w.nk ? wmax + w.shift + 1 : w.nk;  // none sees more
     const float c = p.scale * kLog2e;
 
-    // Reference of the exponents (the running maximum, within kLazy) and their sum.
+    // Reference of the exponents (Ref) and their sum.
     float m = 0.0f, l = 0.0f;
     bool fresh = true;  // no visible key yet
     f32x16 acc[DT];
@@ -617,10 +630,11 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void attn_fwd_kernel(Attn
                 mx[i & 3] = fmaxf(mx[i & 3], s[a][i]);
             }
         const float top = half_max(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
-        if (__any(top > (fresh ? -INFINITY : kLazy))) {
+        constexpr float kDown = Ref<PK>::down;
+        if (__any(top > (fresh ? -INFINITY : kDown + Ref<PK>::lazy))) {
             // The first visible key sets the reference, later ones raise it.
             const bool set = fresh && top > -INFINITY;
-            const float d = set ? top : fmaxf(top, 0.0f);
+            const float d = set ? top - kDown : fmaxf(top - kDown, 0.0f);
             const float r = fresh ? 1.0f : __builtin_amdgcn_exp2f(-d);  // nothing to rescale yet
             m += d;
             fresh = fresh && !set;
@@ -675,7 +689,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void attn_fwd_kernel(Attn
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     if (h == 0 && x < rows)
-        p.lse[(static_cast<int64_t>(w.bq) * p.H + row.h) * p.Tq + w.q0 + row.q] = log_sum(m, l);
+        p.lse[(static_cast<int64_t>(w.bq) * p.H + row.h) * p.Tq + w.q0 + row.q] = log_sum<PK>(m, l);
     __syncthreads();  // the tiles are done with
     char *const so = wave == 0 ? sk0 : wave == 1 ? sk1 : wave == 2 ? sv0 : sv1;
     auto to = [&](int r) __attribute__((always_inline)) {
@@ -724,7 +738,7 @@ __global__ __launch_bounds__(256) void attn_fwd_join_kernel(AttnTrainParams p)
         const int64_t bt = row / p.H;
         const int hh = static_cast<int>(row - bt * p.H);
         const int64_t b = bt / p.Tq;
-        p.lse[(b * p.H + hh) * p.Tq + (bt - b * p.Tq)] = log_sum(m, l);
+        p.lse[(b * p.H + hh) * p.Tq + (bt - b * p.Tq)] = log_sum<PK>(m, l);
     }
     const float y[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
     st_q4<PK>(static_cast<uint16_t *>(p.o) + e, pack4<PK>(y[0], y[1], y[2], y[3]));

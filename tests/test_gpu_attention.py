@@ -439,3 +439,33 @@ def test_attention_float16_gradients_of_many_rows(gpu_device):
     got = _run(*x, do)
     assert torch.equal(got["o"], v) and torch.equal(got["dv"], do)
     assert not got["dq"].any() and not got["dk"].any()
+
+
+@pytest.mark.parametrize("dt", [FP, BF])
+@pytest.mark.parametrize("bits", [20.0, 25.5, 30.0])
+@pytest.mark.parametrize("D,at", [(64, 0), (64, 9000), (128, 0)])
+def test_attention_faint_keys_count_together(gpu_device, D, at, bits, dt):
+    """One key of value 0 with all but the whole weight, 16383 others of 2^-bits of it each and values
+    about 1000: the output is what the others add up to.  A probability is rounded by half a step ``u``
+    of itself; fp16 holds it normal down to 2^-27 of the row's largest and to 2^-38 of that
+    below; ``slack`` as in the reference, scores of up to 21."""
+    from qwendopamine_amd import ops
+
+    Tq, Tk, H = 2048, 16384, 16  # enough queries that the keys are not shared out
+    print(f"[case] attention faint keys 2^-{bits} D{D} strong key {at} {dt}", flush=True)
+    gen = torch.Generator(gpu_device).manual_seed(40)
+    q, k = torch.zeros(1, 1, 1, D, device=gpu_device), torch.zeros(1, Tk, 1, D, device=gpu_device)
+    q[..., 3], k[0, at, 0, 3] = 4.0, bits * 0.6931472 / 4
+    v = 1000 * (0.5 + torch.rand(1, Tk, 1, D, generator=gen, device=gpu_device))
+    v[0, at] = 0
+    q, k, v = q.to(dt), k.to(dt), v.to(dt)
+    o = ops.attention(q.expand(1, Tq, H, D), k.expand(1, Tk, H, D), v.expand(1, Tk, H, D), scale=1.0, causal=False)
+    S = k[0, :, 0].double() @ q[0, 0, 0].double()
+    P = torch.softmax(S, 0)
+    want = P @ v[0, :, 0].double()
+    u = torch.finfo(dt).eps / 2
+    slack = 4 * D * 2.0 ** -24 * float(S.max()) + 2.0 ** -20
+    bound = (2 * u + slack) * want * 1.01 + (Tk * 2.0 ** -38 * 1500 if dt == FP else 0.0)
+    e = (o[0].double() - want).abs()
+    print(f"  value {float(want[0]):.3e}, error / bound {float((e / bound).max()):.2f}", flush=True)
+    assert bool((e <= bound).all())
