@@ -371,7 +371,7 @@ int gdn2_kv_cache_q4_load(const void *k_codes, const void *k_meta, const void *v
  *            elements after x (any element alignment)
  *   targets  int64 [rows]: logp[r] = x[r][t] - logsumexp(x[r]); a target equal to
  *            ignore_index gives 0 and passes no gradient, any other outside
- *            [0, n) gives NaN
+ *            [0, n) gives NaN, and a gradient of NaN unless its dlogp is 0
  *   logp, entropy  fp32 [rows], entropy = -sum p ln p
  *   lse      fp32 [rows][2], what the backward needs of the sums; NULL without one
  *   top_logp fp32, top_ids int64 [rows][top_k], 0 <= top_k <= 32, top_k <= n: in

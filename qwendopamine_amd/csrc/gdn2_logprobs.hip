@@ -405,8 +405,8 @@ __global__ __launch_bounds__(256) void logp_bwd_kernel(LogprobParams p)
     T *dx = static_cast<T *>(p.dx) + row * p.n;
     const int64_t t = p.targets[row];
     const bool known = t >= 0 && t < p.n && t != p.ignore;
-    float gl = known && p.dlogp ? p.dlogp[row] : 0.0f;
-    if (!known && t != p.ignore && p.dlogp) gl = __uint_as_float(0x7fc00000u);
+    float gl = t != p.ignore && p.dlogp ? p.dlogp[row] : 0.0f;
+    if (!known && gl != 0.0f) gl = __uint_as_float(0x7fc00000u);  // of a NaN; where none arrives, none passes
     const float ge = p.dent ? p.dent[row] : 0.0f;
     const float m = p.lse[2 * row], ln_s = p.lse[2 * row + 1], h = ge == 0.0f ? 0.0f : p.entropy[row];
     const bool nothing = gl == 0.0f && ge == 0.0f;  // no gradient arrives: zeros, whatever the logits

@@ -276,3 +276,21 @@ def test_logprobs_more_rows_than_a_launch(gpu_device, rows, V, top):
         if top:
             first = torch.where((r[s] % 4) == 0, 0, hot[s])
             assert torch.equal(out.top_ids[s, 0], first)
+
+
+@pytest.mark.parametrize("V", [777, 40000])
+def test_logprobs_unknown_target_that_nothing_asks_for(gpu_device, V):
+    """A target outside the vocabulary whose log probability is selected away (padding of -1): no
+    gradient arrives at its row, and none passes; the entropy's still does."""
+    from qwendopamine_amd import ops
+
+    x, t, gl, ge = _case(gpu_device, 5, V, BF, seed=12)
+    t[1], t[3] = -1, V
+    wanted = (t >= 0) & (t < V)
+    r = ops.token_logprobs(x, t)
+    (dx,) = torch.autograd.grad((torch.where(wanted, r.logprobs, 0.0) * gl).sum(), x)
+    want = _run(x, torch.where(wanted, t, -100), 0, torch.where(wanted, gl, 0.0))[1]
+    assert torch.equal(dx, want) and not dx[~wanted].any() and dx[wanted].any(-1).all()
+    z = torch.where(wanted, gl, 0.0)
+    dx = _run(x, t, 0, z, ge)[1]
+    assert torch.equal(dx, _run(x, torch.where(wanted, t, -100), 0, z, ge)[1]) and dx.isfinite().all()
