@@ -202,7 +202,7 @@ __global__ __launch_bounds__(64 * kQ4Waves, 2) void attn_q4_kernel(AttnQ4Params 
     unsigned *km = p.k_meta + row0 * NG, *vm = p.v_meta + row0 * NG;
     const float *cs = p.cos + p.rope_stride * pos, *sn = p.sin + p.rope_stride * pos;
 
-    // ---- a step's requests: codes and (scale, minimum) of 32 positions ----
+    // ---- a step's requests: codes of kStep positions, (scale, minimum) of the lane's share of them ----
     struct Step {
         uint2 k[kTiles][NG];
         unsigned v[4 * kTiles][NG], mk[kOwn][4 * NG], mv[kOwn][4 * NG];

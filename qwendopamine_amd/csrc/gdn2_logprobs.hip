@@ -393,7 +393,8 @@ __global__ __launch_bounds__(64) void logp_merge_kernel(LogprobParams p)
 
 // Gradient: one workgroup per (row, share of it).  VEC: rows of x and dx start
 // at the same offset from a 16-byte boundary.  Reads the logits again and writes as much:
-// 8192 x 32000 bf16 180 us, 5.8 TB/s; 1000 x 151936 float32 206 us, 5.9 TB/s.
+// 8192 x 32000 bf16 180 us, 5.8 TB/s; 1000 x 151936 float32 206 us, 5.9 TB/s.  Without VEC,
+// an element at a time: 8192 x 50257 bf16 752 us, and 301 with it.
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void logp_bwd_kernel(LogprobParams p)
 {

@@ -1939,7 +1939,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0,
 
     A target equal to ``ignore_index`` gives 0 and passes no gradient; any other target outside
     ``[0, V)`` gives NaN (selected away, as by ``torch.where``, it passes none either).  A row with a NaN or +inf, or of -inf alone, gives NaN, as ``log_softmax``
-    does; single -inf logits have probability 0 and pass no gradient.  Sums are float32, the
+    does; single -inf logits have probability 0 and pass no gradient but the target's own.  Sums are float32, the
     gradient is rounded once to the logits' dtype; everything has the same bits in every run.
     In a HIP graph, capture the forward and backward together with no eager autograd graph of the
     same leaves alive, as torch asks of any captured backward.  Second derivatives and forward-mode
