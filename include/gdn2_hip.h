@@ -362,6 +362,80 @@ int gdn2_kv_cache_q4_load(const void *k_codes, const void *k_meta, const void *v
                           int G, int D, int64_t max_len, void *stream);
 
 /*
+ * Norms of queries and keys for each head with the rotation of positions, in one pass over a
+ * fused projection (the host's attention layers, reference gdn2_gpt/model.py:40-61, 89-173;
+ * the norms have no counterpart there).  qkv: rows of G (R + 2) D channels, a group's R query heads,
+ * its key, its value (batch and token strides in elements, multiples of 16 bytes).  wq, wk [D]
+ * (io dtype or float32; both NULL: no norm): n = x rsqrt(mean x^2 + eps) w.  The first 2 pairs
+ * channels of n are rotated pair by pair (2 i, 2 i + 1) by row pos of cos, sin [table_rows][pairs]
+ * (float32); pos at b pos_stride_b + t pos_stride_t (NULL: t).  Writes q [B, T, G R, D]
+ * and k [B, T, G, D] in io_dtype (f32, bf16, fp16), rounded once; a token whose position lies
+ * outside the tables gives zeros.  D a multiple of 8 up to 256.
+ * _bwd: from dq, dk, dv the gradient dqkv [B, T, G (R + 2) D] (contiguous; dv copied) and
+ * those of the weights (their dtype), summed in a fixed order; no gradient passes through a
+ * token whose position lies outside.  workspace (only with weights): _workspace_size() bytes,
+ * of which concurrent calls need one each.
+ */
+int gdn2_qkv_norm_rope_fwd(const void *qkv, int64_t stride_b, int64_t stride_t, int io_dtype, const void *wq,
+                           const void *wk, int w_dtype, float eps, const float *cos, const float *sin, int pairs,
+                           int64_t table_rows, const int64_t *pos, int64_t pos_stride_b, int64_t pos_stride_t, void *q,
+                           void *k, int B, int64_t T, int G, int R, int D, void *stream);
+size_t gdn2_qkv_norm_rope_bwd_workspace_size(int B, int64_t T, int G, int R, int D);
+int gdn2_qkv_norm_rope_bwd(const void *qkv, int64_t stride_b, int64_t stride_t, int io_dtype, const void *wq,
+                           const void *wk, int w_dtype, float eps, const float *cos, const float *sin, int pairs,
+                           int64_t table_rows, const int64_t *pos, int64_t pos_stride_b, int64_t pos_stride_t,
+                           const void *dq, const void *dk, const void *dv, void *dqkv, void *dwq, void *dwk, int B,
+                           int64_t T, int G, int R, int D, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * A paged key / value cache (no counterpart in the reference): pages [pages][G][page_size][D]
+ * of keys and of values in io_dtype, page_size a multiple of 16, and table [B] rows of table_cols
+ * page numbers (int32, rows table_stride apart): position j of sequence b is row j % page_size of
+ * page table[b][j / page_size].  A number outside 0 .. pages - 1 is no page.
+ *
+ * gdn2_kv_cache_paged_append: gdn2_qkv_norm_rope_fwd of the tokens t < lengths[b] (NULL: all T) of
+ * each sequence at positions pos[pos_stride * b] + t; q is written, k and the value go to their
+ * pages.  A token that is not there or whose position lies outside the tables or the
+ * sequence's row of the page table gives zeros and is not stored; where the table has no page
+ * nothing is stored.
+ *
+ * gdn2_attn_paged: q [B, T, G R, D] (batch, token and head strides in elements, multiples of 8)
+ * over positions 0 .. pos + t of its sequence; out [B, T, G R, D].  Positions without a page are not
+ * seen; a token that is not there, or outside the page table, or that sees nothing, gives zeros.
+ * io_dtype bf16 / fp16, D 64 or 128.  workspace: gdn2_attn_paged_workspace_size() bytes (positions =
+ * page_size table_cols; may be 0), 16-byte aligned, of which concurrent calls need one each.
+ */
+int gdn2_kv_cache_paged_append(const void *qkv, int64_t stride_b, int64_t stride_t, int io_dtype, const void *wq,
+                               const void *wk, int w_dtype, float eps, const float *cos, const float *sin, int pairs,
+                               int64_t table_rows, const int64_t *pos, int64_t pos_stride, const int64_t *lengths, void *q,
+                               void *k_pages, void *v_pages, int64_t pages, int page_size, const int *table,
+                               int64_t table_stride, int table_cols, int B, int64_t T, int G, int R, int D, void *stream);
+size_t gdn2_attn_paged_workspace_size(int B, int64_t T, int G, int R, int D, int64_t positions);
+int gdn2_attn_paged(const void *q, const int64_t *strides, int io_dtype, const void *k_pages, const void *v_pages,
+                    int64_t pages, int page_size, const int *table, int64_t table_stride, int table_cols,
+                    const int64_t *pos, int64_t pos_stride, const int64_t *lengths, void *out, int B, int64_t T, int G,
+                    int R, int D, float scale, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * A token of each row of logits x [rows][n] (row r at (r / inner) outer_stride + (r % inner)
+ * row_stride, any alignment; f32, bf16, fp16; n up to 2^20), drawn with the random number u[r] of
+ * [0, 1): of the weights w_j = exp((x_j - max x) / temperature) those are kept that are at least
+ * min_p, of these the top_k largest (equal logits: the lower index first; 0: all), of these, in
+ * that order, the shortest run whose sum reaches top_p of their sum (1: all); the token is
+ * the lowest index whose running sum of kept weights exceeds u times their total.  A setting is given
+ * for each row (device, [rows]) or, with a NULL pointer, for all.  temperature 0: the largest
+ * logit (the lowest index of equal ones).  A row whose largest logit is NaN or infinite gives its
+ * index (NaN above all).  Whole numbers of 2^-42 are summed, in no order that matters.
+ * workspace: gdn2_sample_tokens_workspace_size() bytes, 16-byte aligned, of which concurrent
+ * calls need one each.
+ */
+size_t gdn2_sample_tokens_workspace_size(int64_t rows, int64_t n);
+int gdn2_sample_tokens(const void *x, int64_t inner, int64_t outer_stride, int64_t row_stride, int io_dtype, int64_t rows,
+                       int64_t n, const float *u, const float *temperature, float temperature_all, const int *top_k,
+                       int top_k_all, const float *top_p, float top_p_all, const float *min_p, float min_p_all,
+                       int64_t *out, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
  * Log probabilities of given tokens over the LM head's logits (the logits of
  * reference src/qwendopamine/models/gdn2_gpt/model.py:304-380, GPT.forward),
  * the rows' entropies and their top_k most probable tokens, and the gradient:

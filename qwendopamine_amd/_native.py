@@ -89,6 +89,27 @@ SIGNATURES: dict[str, tuple] = {
     ),
     "gdn2_kv_cache_q4_store": (_i, [_vp, _vp, _vp, _i, _vp, _i64, _vp, _vp, _vp, _vp, _i, _i64, _i, _i, _i64, _vp]),
     "gdn2_kv_cache_q4_load": (_i, [_vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _i, _i, _i64, _i, _i, _i64, _vp]),
+    "gdn2_qkv_norm_rope_fwd": (_i, [_vp, _i64, _i64, _i, _vp, _vp, _i, _f, _vp, _vp, _i, _i64, _vp, _i64, _i64, _vp, _vp,
+                                    _i, _i64, _i, _i, _i, _vp]),
+    "gdn2_qkv_norm_rope_bwd_workspace_size": (_sz, [_i, _i64, _i, _i, _i]),
+    "gdn2_qkv_norm_rope_bwd": (
+        _i,
+        [_vp, _i64, _i64, _i, _vp, _vp, _i, _f, _vp, _vp, _i, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp,
+         _i, _i64, _i, _i, _i, _vp, _sz, _vp],
+    ),
+    "gdn2_kv_cache_paged_append": (
+        _i,
+        [_vp, _i64, _i64, _i, _vp, _vp, _i, _f, _vp, _vp, _i, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i, _vp, _i64,
+         _i, _i, _i64, _i, _i, _i, _vp],
+    ),
+    "gdn2_attn_paged_workspace_size": (_sz, [_i, _i64, _i, _i, _i, _i64]),
+    "gdn2_attn_paged": (
+        _i,
+        [_vp, _vp, _i, _vp, _vp, _i64, _i, _vp, _i64, _i, _vp, _i64, _vp, _vp, _i, _i64, _i, _i, _i, _f, _vp, _sz, _vp],
+    ),
+    "gdn2_sample_tokens_workspace_size": (_sz, [_i64, _i64]),
+    "gdn2_sample_tokens": (_i, [_vp, _i64, _i64, _i64, _i, _i64, _i64, _vp, _vp, _f, _vp, _i, _vp, _f, _vp, _f, _vp, _vp,
+                                _sz, _vp]),
     "gdn2_token_logprobs_workspace_size": (_sz, [_i64, _i64, _i, _i]),
     "gdn2_token_logprobs_fwd": (_i, [_vp, _i64, _i64, _i64, _i, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _i, _vp, _vp, _vp,
                                      _sz, _vp]),

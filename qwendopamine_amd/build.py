@@ -19,7 +19,8 @@ INCLUDE = PKG.parent / "include"
 LIB_NAME = "libgdn2_hip.so"
 SOURCES = ["gdn2_api.hip", "gdn2_recurrent.hip", "gdn2_chunk_fwd.hip", "gdn2_chunk_bwd.hip", "gdn2_chunk_wide.hip", "gdn2_gate.hip",
            "gdn2_prologue.hip", "gdn2_prologue_bwd.hip", "gdn2_noalloc.hip", "gdn2_skinny.hip",
-           "gdn2_attn.hip", "gdn2_attn_train.hip", "gdn2_attn_q4.hip", "gdn2_logprobs.hip"]
+           "gdn2_attn.hip", "gdn2_attn_train.hip", "gdn2_attn_q4.hip", "gdn2_logprobs.hip",
+           "gdn2_qkv_rope.hip", "gdn2_attn_paged.hip", "gdn2_sample.hip"]
 ARCH = os.environ.get("GDN2_OFFLOAD_ARCH", "gfx950")
 
 HIPCC_FLAGS = [

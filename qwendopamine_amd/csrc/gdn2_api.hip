@@ -546,6 +546,202 @@ int gdn2_kv_cache_q4_load(const void *k_codes, const void *k_meta, const void *v
     return launch_q4_load(p, io_dtype, static_cast<hipStream_t>(stream)) == hipSuccess ? GDN2_OK : GDN2_ERR_LAUNCH;
 }
 
+// What the passes over a fused projection share: its rows, the norm's weights and the angles.
+static int check_qkv_rope(QkvRopeParams &p, const void *qkv, int64_t stride_b, int64_t stride_t, int io_dtype,
+                          const void *wq, const void *wk, int w_dtype, float eps, const float *cos, const float *sin,
+                          int pairs, int64_t table_rows, int B, int64_t T, int G, int R, int D)
+{
+    if (!valid_dtype(io_dtype) || B < 0 || T < 0 || G < 1 || R < 1 || D < 1) return GDN2_ERR_INVALID;
+    if (D % 8 != 0 || D > 256) return GDN2_ERR_UNSUPPORTED;
+    if (static_cast<int64_t>(G) * (R + 2) > 65535) return GDN2_ERR_UNSUPPORTED;
+    if ((wq != nullptr) != (wk != nullptr)) return GDN2_ERR_INVALID;
+    if (wq && w_dtype != io_dtype && w_dtype != GDN2_DTYPE_F32) return GDN2_ERR_INVALID;
+    if (pairs < 0 || 2 * pairs > D || table_rows < 0 || table_rows > 2147483647LL) return GDN2_ERR_INVALID;
+    if (B == 0 || T == 0) return GDN2_OK;
+    const int per = io_dtype == GDN2_DTYPE_F32 ? 4 : 8;
+    if (!qkv || (pairs > 0 && table_rows > 0 && (!cos || !sin))) return GDN2_ERR_INVALID;
+    if (stride_b < 0 || stride_t < 0 || (B > 1 && stride_b % per != 0) || (T > 1 && stride_t % per != 0))
+        return GDN2_ERR_INVALID;
+    if ((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(wq) | reinterpret_cast<uintptr_t>(wk)) & 15)
+        return GDN2_ERR_INVALID;
+    if ((reinterpret_cast<uintptr_t>(cos) | reinterpret_cast<uintptr_t>(sin)) & 3) return GDN2_ERR_INVALID;
+    if (T > 2147483647LL || static_cast<double>(B) * T * qkv_rope_units(G * (R + 2), D) / 4 + 1 >
+                                static_cast<double>(max_workgroups(256)))
+        return GDN2_ERR_UNSUPPORTED;
+    p.qkv = qkv; p.stride_b = stride_b; p.stride_t = stride_t;
+    p.wq = wq; p.wk = wk; p.w_f32 = w_dtype == GDN2_DTYPE_F32; p.eps = eps;
+    p.cos = cos; p.sin = sin; p.pairs = pairs; p.table_rows = table_rows;
+    p.B = B; p.T = static_cast<int>(T); p.G = G; p.R = R; p.D = D;
+    return GDN2_OK;
+}
+
+static bool aligned16(const void *a, const void *b, const void *c)
+{
+    return ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(c)) & 15) == 0;
+}
+
+int gdn2_qkv_norm_rope_fwd(const void *qkv, int64_t stride_b, int64_t stride_t, int io_dtype, const void *wq,
+                           const void *wk, int w_dtype, float eps, const float *cos, const float *sin, int pairs,
+                           int64_t table_rows, const int64_t *pos, int64_t pos_stride_b, int64_t pos_stride_t, void *q,
+                           void *k, int B, int64_t T, int G, int R, int D, void *stream)
+{
+    QkvRopeParams p = {};
+    const int st = check_qkv_rope(p, qkv, stride_b, stride_t, io_dtype, wq, wk, w_dtype, eps, cos, sin, pairs, table_rows,
+                                  B, T, G, R, D);
+    if (st != GDN2_OK) return st;
+    if (B == 0 || T == 0) return GDN2_OK;
+    if (!q || !k || !aligned16(q, k, nullptr) || pos_stride_b < 0 || pos_stride_t < 0) return GDN2_ERR_INVALID;
+    p.pos = pos; p.pos_b = pos_stride_b; p.pos_t = pos_stride_t;
+    p.q = q; p.k = k;
+    return launch_qkv_rope_fwd(p, io_dtype, static_cast<hipStream_t>(stream)) == hipSuccess ? GDN2_OK : GDN2_ERR_LAUNCH;
+}
+
+size_t gdn2_qkv_norm_rope_bwd_workspace_size(int B, int64_t T, int G, int R, int D)
+{
+    if (B < 1 || T < 1 || G < 1 || R < 1 || D < 1 || D > 256) return 0;
+    return static_cast<size_t>(qkv_rope_bwd_blocks(static_cast<int64_t>(B) * T * qkv_rope_units(G * (R + 2), D))) * 2 * D *
+           sizeof(float);
+}
+
+int gdn2_qkv_norm_rope_bwd(const void *qkv, int64_t stride_b, int64_t stride_t, int io_dtype, const void *wq,
+                           const void *wk, int w_dtype, float eps, const float *cos, const float *sin, int pairs,
+                           int64_t table_rows, const int64_t *pos, int64_t pos_stride_b, int64_t pos_stride_t,
+                           const void *dq, const void *dk, const void *dv, void *dqkv, void *dwq, void *dwk, int B,
+                           int64_t T, int G, int R, int D, void *workspace, size_t workspace_bytes, void *stream)
+{
+    QkvRopeParams p = {};
+    const int st = check_qkv_rope(p, qkv, stride_b, stride_t, io_dtype, wq, wk, w_dtype, eps, cos, sin, pairs, table_rows,
+                                  B, T, G, R, D);
+    if (st != GDN2_OK) return st;
+    if (B == 0 || T == 0) return GDN2_OK;
+    if (!dq || !dk || !dv || !dqkv || !aligned16(dq, dk, dv) || !aligned16(dqkv, nullptr, nullptr) || pos_stride_b < 0 ||
+        pos_stride_t < 0)
+        return GDN2_ERR_INVALID;
+    if (wq && (!dwq || !dwk)) return GDN2_ERR_INVALID;
+    if (wq && (!workspace || workspace_bytes < gdn2_qkv_norm_rope_bwd_workspace_size(B, T, G, R, D) ||
+               (reinterpret_cast<uintptr_t>(workspace) & 15)))
+        return GDN2_ERR_WORKSPACE;
+    p.pos = pos; p.pos_b = pos_stride_b; p.pos_t = pos_stride_t;
+    p.q = const_cast<void *>(dq); p.k = const_cast<void *>(dk); p.v = const_cast<void *>(dv);
+    p.dqkv = dqkv; p.dwq = dwq; p.dwk = dwk;
+    p.part = static_cast<float *>(workspace);
+    return launch_qkv_rope_bwd(p, io_dtype, static_cast<hipStream_t>(stream)) == hipSuccess ? GDN2_OK : GDN2_ERR_LAUNCH;
+}
+
+// A paged cache: pages [pages][G][page_size][D] of keys and of values, and the table.
+static int check_paged(const void *k_pages, const void *v_pages, int64_t pages, int page_size, const int *table,
+                       int64_t table_stride, int table_cols, int B, int G, int D)
+{
+    if (pages < 1 || page_size < 1 || table_cols < 1 || table_stride < 0 || B < 0 || G < 1 || D < 1)
+        return GDN2_ERR_INVALID;
+    if (page_size % 16 != 0) return GDN2_ERR_UNSUPPORTED;
+    if (static_cast<int64_t>(page_size) * table_cols > (1 << 30)) return GDN2_ERR_UNSUPPORTED;
+    if (static_cast<double>(pages) * G * page_size > 4.0e9) return GDN2_ERR_UNSUPPORTED;  // rows are counted in 32 bits
+    if (B > 0 && (!k_pages || !v_pages || !table)) return GDN2_ERR_INVALID;
+    if (!aligned16(k_pages, v_pages, nullptr) || (reinterpret_cast<uintptr_t>(table) & 3)) return GDN2_ERR_INVALID;
+    return GDN2_OK;
+}
+
+int gdn2_kv_cache_paged_append(const void *qkv, int64_t stride_b, int64_t stride_t, int io_dtype, const void *wq,
+                               const void *wk, int w_dtype, float eps, const float *cos, const float *sin, int pairs,
+                               int64_t table_rows, const int64_t *pos, int64_t pos_stride, const int64_t *lengths, void *q,
+                               void *k_pages, void *v_pages, int64_t pages, int page_size, const int *table,
+                               int64_t table_stride, int table_cols, int B, int64_t T, int G, int R, int D, void *stream)
+{
+    QkvRopeParams p = {};
+    int st = check_qkv_rope(p, qkv, stride_b, stride_t, io_dtype, wq, wk, w_dtype, eps, cos, sin, pairs, table_rows, B, T,
+                            G, R, D);
+    if (st != GDN2_OK) return st;
+    st = check_paged(k_pages, v_pages, pages, page_size, table, table_stride, table_cols, B, G, D);
+    if (st != GDN2_OK) return st;
+    if (B == 0 || T == 0) return GDN2_OK;
+    if (!q || !pos || pos_stride < 0 || !aligned16(q, nullptr, nullptr)) return GDN2_ERR_INVALID;
+    p.pos = pos; p.pos_b = pos_stride; p.pos_t = 0; p.pos_add_t = 1;
+    p.lengths = lengths;
+    p.q = q; p.k = k_pages; p.v = v_pages;
+    p.table = table; p.table_stride = table_stride; p.table_cols = table_cols;
+    p.pages = pages; p.page = page_size;
+    return launch_qkv_rope_fwd(p, io_dtype, static_cast<hipStream_t>(stream)) == hipSuccess ? GDN2_OK : GDN2_ERR_LAUNCH;
+}
+
+size_t gdn2_attn_paged_workspace_size(int B, int64_t T, int G, int R, int D, int64_t positions)
+{
+    if (B < 1 || T < 1 || G < 1 || R < 1 || D < 1 || positions < 1) return 0;
+    const int s = attn_paged_splits(B, G, T * R, positions);
+    return s == 1 ? 0 : static_cast<size_t>(B) * T * G * R * s * (D + 2) * sizeof(float);
+}
+
+int gdn2_attn_paged(const void *q, const int64_t *strides, int io_dtype, const void *k_pages, const void *v_pages,
+                    int64_t pages, int page_size, const int *table, int64_t table_stride, int table_cols,
+                    const int64_t *pos, int64_t pos_stride, const int64_t *lengths, void *out, int B, int64_t T, int G,
+                    int R, int D, float scale, void *workspace, size_t workspace_bytes, void *stream)
+{
+    if (!valid_dtype(io_dtype) || T < 0 || R < 1 || pos_stride < 0 || !strides) return GDN2_ERR_INVALID;
+    const int st = check_paged(k_pages, v_pages, pages, page_size, table, table_stride, table_cols, B, G, D);
+    if (st != GDN2_OK) return st;
+    if (!attn_paged_supported(io_dtype, D) || !(scale > 0.0f) || scale > 1e30f) return GDN2_ERR_UNSUPPORTED;
+    if (B == 0 || T == 0) return GDN2_OK;
+    if (!q || !pos || !out || !aligned16(q, out, nullptr)) return GDN2_ERR_INVALID;
+    const int64_t size[3] = {B, T, static_cast<int64_t>(G) * R};
+    AttnPagedParams p = {};
+    for (int i = 0; i < 3; ++i) {
+        if (strides[i] < 0 || (size[i] > 1 && strides[i] % 8 != 0)) return GDN2_ERR_INVALID;
+        p.qs[i] = strides[i];
+    }
+    // Rows of a group in 31 bits, and what is launched within HIP's limits.
+    if (static_cast<double>(T) * R > 1073741824.0 || static_cast<double>(B) * G * R * T > static_cast<double>(max_workgroups(256)) ||
+        static_cast<int64_t>(B) * G > 65535 * 16)
+        return GDN2_ERR_UNSUPPORTED;
+    p.q = q; p.k = k_pages; p.v = v_pages;
+    p.table = table; p.table_stride = table_stride; p.pages = pages; p.page = page_size;
+    p.cap = page_size * table_cols;
+    p.pos = pos; p.pos_stride = pos_stride; p.lengths = lengths;
+    p.out = out; p.B = B; p.T = static_cast<int>(T); p.G = G; p.R = R; p.D = D; p.scale = scale;
+    p.rows = attn_paged_rows(T * R);
+    p.tiles = static_cast<int>((T * R + p.rows - 1) / p.rows);
+    p.splits = attn_paged_splits(B, G, T * R, p.cap);
+    p.part = static_cast<float *>(workspace);
+    if (p.splits > 1 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) ||
+                         workspace_bytes < gdn2_attn_paged_workspace_size(B, T, G, R, D, p.cap)))
+        return GDN2_ERR_WORKSPACE;
+    return launch_attn_paged(p, io_dtype, static_cast<hipStream_t>(stream)) == hipSuccess ? GDN2_OK : GDN2_ERR_LAUNCH;
+}
+
+size_t gdn2_sample_tokens_workspace_size(int64_t rows, int64_t n)
+{
+    return rows < 1 || n < 1 ? 0 : static_cast<size_t>(rows) * sample_row_bytes(n);
+}
+
+int gdn2_sample_tokens(const void *x, int64_t inner, int64_t outer_stride, int64_t row_stride, int io_dtype, int64_t rows,
+                       int64_t n, const float *u, const float *temperature, float temperature_all, const int *top_k,
+                       int top_k_all, const float *top_p, float top_p_all, const float *min_p, float min_p_all,
+                       int64_t *out, void *workspace, size_t workspace_bytes, void *stream)
+{
+    if (!valid_dtype(io_dtype) || rows < 0 || n < 1 || inner < 1 || outer_stride < 0 || row_stride < 0)
+        return GDN2_ERR_INVALID;
+    if (n > kSampleMax) return GDN2_ERR_UNSUPPORTED;
+    if (!temperature && !(temperature_all >= 0.0f && temperature_all <= 3.0e38f)) return GDN2_ERR_INVALID;
+    if (!top_p && !(top_p_all > 0.0f && top_p_all <= 1.0f)) return GDN2_ERR_INVALID;
+    if (!min_p && !(min_p_all >= 0.0f && min_p_all <= 1.0f)) return GDN2_ERR_INVALID;
+    if (!top_k && top_k_all < 0) return GDN2_ERR_INVALID;
+    if (rows == 0) return GDN2_OK;
+    const uintptr_t size = io_dtype == GDN2_DTYPE_F32 ? 4 : 2;
+    if (!x || !u || !out || (reinterpret_cast<uintptr_t>(x) & (size - 1))) return GDN2_ERR_INVALID;
+    if (rows > max_workgroups(kSampleFinishThreads) || rows * kSampleParts > max_workgroups(256)) return GDN2_ERR_UNSUPPORTED;
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) ||
+        workspace_bytes < gdn2_sample_tokens_workspace_size(rows, n))
+        return GDN2_ERR_WORKSPACE;
+    SampleParams p = {};
+    p.x = x; p.inner = inner; p.outer_stride = outer_stride; p.row_stride = row_stride; p.rows = rows;
+    p.n = static_cast<int>(n);
+    p.u = u; p.out = out;
+    p.temperature = temperature; p.temperature_all = temperature_all;
+    p.top_k = top_k; p.top_k_all = top_k_all;
+    p.top_p = top_p; p.top_p_all = top_p_all;
+    p.min_p = min_p; p.min_p_all = min_p_all;
+    return launch_sample(p, workspace, io_dtype, static_cast<hipStream_t>(stream)) == hipSuccess ? GDN2_OK : GDN2_ERR_LAUNCH;
+}
+
 static int fill_logprob_args(LogprobParams &p, const void *x, int64_t inner, int64_t outer_stride, int64_t row_stride,
                              int io_dtype, int64_t rows, int64_t n, const int64_t *targets, int64_t ignore)
 {

@@ -1,0 +1,524 @@
+// Softmax attention over a paged key / value cache, gfx950: from one token of each
+// sequence to pieces of prompts, every sequence at its own position.
+//
+//   o_t = sum_j p_tj v_j / sum_j p_tj,  p_tj = exp(scale q_t . k_j),  j <= pos + t
+//   k_j, v_j: row j mod S of page table[b][j / S], pages [P][G][S][D]
+//
+// v_mfma_f32_16x16x32, positions as rows and the rows of a group (its query heads of
+// every token) as columns, 16 C of them: a lane's 16 bytes of a key row are the A
+// operand as they lie in memory, so keys go from memory to the matrix units
+// without passing through LDS, and the scores come out with four positions of one
+// column per lane, which is the B operand of the value product.  Its A operand
+// has positions along the contraction: a lane takes CH = D / 16 channels of four
+// rows and pairs them by byte permutes.  Waves take 32 positions at a time in
+// turn, each with a running reference and sum of its own, and meet in LDS; long
+// contexts are split into shares that a second launch joins.  A wave looks the
+// pages of its next 32 steps up at once (a lane each), so that no key waits for
+// a page number.  One token a sequence is bound by the read of its keys and values.
+#include "gdn2_common.h"
+#include "gdn2_internal.h"
+#include "gdn2_mfma.h"
+
+namespace gdn2 {
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kStep = 32;               // positions of a wave's step: two tiles of 16
+constexpr int kRound = kStep * kWaves;  // positions that a workgroup's waves take at a time
+constexpr int kMaxSplits = 256;
+constexpr float kNoMax = -3.0e38f;  // no key yet: below every score, and differences stay finite
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr unsigned kNoPage = 0xffffffffu;
+
+// The reference of the exponents lies `down` under the running maximum and moves when
+// a score exceeds that maximum by `lazy`: fp16 probabilities are held in 2^13 ..
+// 2^15, where 2^-27 of the largest still has 11 bits (bf16 has fp32's exponents).
+template <PrecKind PK>
+struct Ref {
+    static constexpr float down = PK == PrecKind::F16 ? 13.0f : 0.0f, lazy = PK == PrecKind::F16 ? 2.0f : 8.0f;
+};
+
+template <PrecKind PK>
+__device__ __forceinline__ f32x4 mma16(f32x4 acc, uint4 a, uint4 b)
+{
+    typename Prec<PK>::frag fa, fb;
+    fa.u = a;
+    fb.u = b;
+    return Prec<PK>::mma(acc, fa, fb);
+}
+
+// Over the four lanes of a column.
+__device__ __forceinline__ float col_max(float x)
+{
+    unsigned u = __float_as_uint(x);
+    auto s = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    x = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+    u = __float_as_uint(x);
+    s = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+__device__ __forceinline__ float col_sum(float x)
+{
+    unsigned u = __float_as_uint(x);
+    auto s = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    x = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+    u = __float_as_uint(x);
+    s = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+
+template <PrecKind PK>
+__device__ __forceinline__ unsigned pack2(float a, float b)
+{
+    if constexpr (PK == PrecKind::BF16)
+        return f32x2_to_bf16x2_bits(a, b);
+    else
+        return Prec<PK>::from_f32(a) | static_cast<unsigned>(Prec<PK>::from_f32(b)) << 16;
+}
+
+// What a workgroup works on: rows m0 .. of group g of sequence b, tokens t0 .. t1 - 1 of
+// which are there, and their positions.
+struct Where {
+    int b, g, m0;
+    int t0, t1;  // t1 <= t0: none
+    int pos;     // position of token 0
+    int n;       // keys that some row sees
+};
+
+// Tokens of sequence b that are there and inside the cache.
+__device__ __forceinline__ int tokens_of(const AttnPagedParams &p, int b, int &pos)
+{
+    const int64_t at = p.pos[p.pos_stride * b], cap = p.cap;
+    int64_t t = p.T;
+    if (p.lengths) {
+        const int64_t l = p.lengths[b];
+        t = l < t ? l : t;
+    }
+    if (at < 0 || at >= cap) {
+        pos = 0;
+        return 0;
+    }
+    pos = static_cast<int>(at);
+    return static_cast<int>(t < cap - at ? t : cap - at);
+}
+
+__device__ __forceinline__ Where where(const AttnPagedParams &p, int rows, int bg, int tile)
+{
+    Where w;
+    w.b = bg / p.G;
+    w.g = bg - w.b * p.G;
+    w.m0 = tile * rows;
+    const int there = tokens_of(p, w.b, w.pos);
+    const int all = p.T * p.R, last = (w.m0 + rows < all ? w.m0 + rows : all) - 1;
+    w.t0 = w.m0 / p.R;
+    const int t1 = last / p.R + 1;
+    w.t1 = t1 < there ? t1 : there;
+    w.n = w.t1 > w.t0 ? w.pos + w.t1 : 0;
+    return w;
+}
+
+// Positions of a share: whole rounds, the longest sequence's keys over p.splits, so that all
+// shares that hold any are equally long.
+__device__ __forceinline__ int share_of(const AttnPagedParams &p, int lane)
+{
+    int longest = 1;
+    for (int b = lane; b < p.B; b += 64) {
+        int pos;
+        const int t = tokens_of(p, b, pos);
+        longest = t > 0 && pos + t > longest ? pos + t : longest;
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_xor(longest, o, 64);
+        longest = longest > y ? longest : y;
+    }
+    const int rounds = (longest + kRound - 1) / kRound;
+    return (rounds + p.splits - 1) / p.splits * kRound;
+}
+
+// A row's place in a [B, T, H, ...] tensor's rows.
+__device__ __forceinline__ int64_t out_row(const AttnPagedParams &p, const Where &w, int x)
+{
+    const int t = x / p.R;
+    return (static_cast<int64_t>(w.b) * p.T + t) * (p.G * p.R) + w.g * p.R + (x - t * p.R);
+}
+
+// C column tiles.
+template <typename T, PrecKind PK, int D, int C>
+__global__ __launch_bounds__(64 * kWaves, C == 4 ? 1 : 2) void attn_paged_kernel(AttnPagedParams p)
+{
+    constexpr int KS = D / 32, CH = D / 16, VW = CH / 2;  // contraction steps, channels and dwords of a lane's value row
+    constexpr int kRows = 16 * C;
+    __shared__ __align__(16) float s_o[kWaves][16][D];
+    __shared__ float s_m[kWaves][C][16], s_l[kWaves][C][16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 15, kg = lane >> 4;
+    // A group's tiles of rows read the same keys: all on one XCD (workgroups go to the 8 in turn).
+    int bg = blockIdx.x, tile = 0;
+    if (p.tiles > 1) {
+        const int k = blockIdx.x >> 3;
+        bg = k / p.tiles * 8 + (blockIdx.x & 7);
+        tile = p.tiles - 1 - k % p.tiles;  // the longest first
+        if (bg >= p.B * p.G) return;
+    }
+    const Where w = where(p, kRows, bg, tile);
+    const int all = p.T * p.R;
+    T *out = static_cast<T *>(p.out);
+    const int per = p.splits > 1 ? share_of(p, lane) : (w.n + kRound - 1) / kRound * kRound;
+    const int lo = static_cast<int>(blockIdx.y) * per;
+    const int hi = lo + per < w.n ? lo + per : w.n;
+    if (lo >= hi) {
+        // Nothing here (the join does not read this share); no key at all: zeros.
+        if (p.splits == 1)
+            for (int e = tid; e < kRows * D; e += 64 * kWaves) {
+                const int x = w.m0 + e / D;
+                if (x < all) io<T>::st(out, out_row(p, w, x) * D + e % D, 0.0f);
+            }
+        return;
+    }
+
+    // ---- this lane's columns: query rows as B operands, and the keys they see ----
+    uint4 qf[C][KS];
+    int lim[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        int x = w.m0 + 16 * c + n;
+        const int end = w.t1 * p.R;
+        x = x < end ? x : end - 1;  // rows past the end repeat the last one
+        const int t = x / p.R;
+        lim[c] = w.pos + t + 1;
+        const T *q = static_cast<const T *>(p.q) + w.b * p.qs[0] + t * p.qs[1] + (w.g * p.R + (x - t * p.R)) * p.qs[2];
+#pragma unroll
+        for (int s = 0; s < KS; ++s) qf[c][s] = *reinterpret_cast<const uint4 *>(q + 32 * s + 8 * kg);
+    }
+    const int seen = w.pos + w.t0 + 1;  // every row sees these
+
+    // ---- pages: lane 2 i + a holds the row of the cache where tile a of the wave's step i begins ----
+    const int steps = hi - lo > wave * kStep ? (hi - lo - wave * kStep + kRound - 1) / kRound : 0;
+    const int *table = p.table + w.b * p.table_stride;
+    auto look_up = [&](int base) __attribute__((always_inline)) {
+        const int j = lo + ((base + (lane >> 1)) * kWaves + wave) * kStep + (lane & 1) * 16;
+        unsigned r = kNoPage;
+        if (j < hi) {
+            const int col = j / p.page;
+            const int64_t pg = table[col];
+            if (pg >= 0 && pg < p.pages) r = static_cast<unsigned>((pg * p.G + w.g) * p.page + (j - col * p.page));
+        }
+        return r;
+    };
+
+    struct Step {
+        uint4 k[2][KS];
+        unsigned v[2][4][VW];
+    };
+    const char *kb = static_cast<const char *>(p.k), *vb = static_cast<const char *>(p.v);
+    const unsigned k_off = n * (2 * D) + kg * 16, v_off = 4 * kg * (2 * D) + n * (2 * CH);
+    auto load_v = [&](unsigned (&v)[VW], const char *at) __attribute__((always_inline)) {
+        if constexpr (VW == 2) {
+            const uint2 u = *reinterpret_cast<const uint2 *>(at);
+            v[0] = u.x;
+            v[1] = u.y;
+        } else {
+            const uint4 u = *reinterpret_cast<const uint4 *>(at);
+            v[0] = u.x;
+            v[1] = u.y;
+            v[2] = u.z;
+            v[3] = u.w;
+        }
+    };
+    // Positions j0 .. j0 + 31 from rows r0 and r1; those past the last key read that one again.  A
+    // tile without a page reads row 0 of the cache, and is hidden.
+    auto request = [&](Step &st, int j0, unsigned r0, unsigned r1) __attribute__((always_inline)) {
+        r0 = r0 == kNoPage ? 0 : r0;
+        if (j0 + kStep <= w.n) {
+            r1 = r1 == kNoPage ? 0 : r1;
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                const int64_t at = static_cast<int64_t>(a ? r1 : r0) * (2 * D);
+#pragma unroll
+                for (int s = 0; s < KS; ++s) st.k[a][s] = *reinterpret_cast<const uint4 *>(kb + at + k_off + 64 * s);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) load_v(st.v[a][i], vb + at + v_off + i * (2 * D));
+            }
+        } else {
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                const int last = w.n - 1 - (j0 + 16 * a);  // < 0: the tile is past the end, and reads the other's last row
+                const unsigned r = a && last >= 0 ? (r1 == kNoPage ? 0 : r1) : r0;
+                const int top = last >= 0 ? last : w.n - 1 - j0;
+                const int64_t at = static_cast<int64_t>(r) * (2 * D);
+                const int rk = n < top ? n : top;
+                const char *k = kb + at + rk * (2 * D) + kg * 16;
+#pragma unroll
+                for (int s = 0; s < KS; ++s) st.k[a][s] = *reinterpret_cast<const uint4 *>(k + 64 * s);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int rv = 4 * kg + i < top ? 4 * kg + i : top;
+                    load_v(st.v[a][i], vb + at + rv * (2 * D) + n * (2 * CH));
+                }
+            }
+        }
+    };
+
+    const float scale = p.scale * kLog2e;
+    float m[C], l[C];
+    f32x4 acc[C][CH];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        m[c] = kNoMax;
+        l[c] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < CH; ++e) acc[c][e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    auto step = [&](Step &st, int j0, bool bad0, bool bad1) __attribute__((always_inline)) {
+        const bool hide = bad0 || bad1 || j0 + kStep > seen;
+        if (bad0 || bad1) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < VW; ++e) {
+                    st.v[0][i][e] = bad0 ? 0u : st.v[0][i][e];
+                    st.v[1][i][e] = bad1 ? 0u : st.v[1][i][e];
+                }
+        }
+        uint4 ph[C], pl[C];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            f32x4 t[2];
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                t[a] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int s = 0; s < KS; ++s) t[a] = mma16<PK>(t[a], st.k[a][s], qf[c][s]);
+            }
+            float s[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[i] = t[i >> 2][i & 3];
+            if (hide) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int j = j0 + 16 * (i >> 2) + 4 * kg + (i & 3);
+                    s[i] = j < lim[c] && !(i < 4 ? bad0 : bad1) ? s[i] : -INFINITY;
+                }
+            }
+            float mx = s[0];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) mx = fmaxf(mx, s[i]);
+            mx = col_max(mx) * scale;
+            if (__any(mx > m[c] + (Ref<PK>::down + Ref<PK>::lazy))) {
+                const float mn = fmaxf(m[c], mx - Ref<PK>::down);
+                const float r = __builtin_amdgcn_exp2f(m[c] - mn);
+                m[c] = mn;
+                l[c] *= r;
+#pragma unroll
+                for (int e = 0; e < CH; ++e)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[c][e][i] *= r;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], scale, -m[c]));
+                l[c] += s[i];
+            }
+            // Probabilities in two parts: rounded once they would cost half a step of the
+            // result; the products are cheap beside the read.
+            unsigned h[4], lw[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                h[i] = pack2<PK>(s[2 * i], s[2 * i + 1]);
+                lw[i] = pack2<PK>(s[2 * i] - Prec<PK>::to_f32(static_cast<uint16_t>(h[i] & 0xffffu)),
+                                  s[2 * i + 1] - Prec<PK>::to_f32(static_cast<uint16_t>(h[i] >> 16)));
+            }
+            ph[c] = make_uint4(h[0], h[1], h[2], h[3]);
+            pl[c] = make_uint4(lw[0], lw[1], lw[2], lw[3]);
+        }
+#pragma unroll
+        for (int e = 0; e < CH; ++e) {
+            const unsigned sel = e & 1 ? 0x07060302u : 0x05040100u;
+            const uint4 a = make_uint4(__builtin_amdgcn_perm(st.v[0][1][e / 2], st.v[0][0][e / 2], sel),
+                                       __builtin_amdgcn_perm(st.v[0][3][e / 2], st.v[0][2][e / 2], sel),
+                                       __builtin_amdgcn_perm(st.v[1][1][e / 2], st.v[1][0][e / 2], sel),
+                                       __builtin_amdgcn_perm(st.v[1][3][e / 2], st.v[1][2][e / 2], sel));
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                acc[c][e] = mma16<PK>(acc[c][e], a, ph[c]);
+                acc[c][e] = mma16<PK>(acc[c][e], a, pl[c]);
+            }
+        }
+    };
+
+    // ---- the steps, the next one's keys and values in flight during each ----
+    Step cur, alt;
+    unsigned next = look_up(0);
+    for (int base = 0; base < steps; base += 32) {
+        const unsigned rows = next;
+        if (base + 32 < steps) next = look_up(base + 32);
+        const int cnt = steps - base < 32 ? steps - base : 32;
+        const int jw = lo + (base * kWaves + wave) * kStep;
+        auto row = [&](int i) __attribute__((always_inline)) {
+            return static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(rows), i));
+        };
+        auto get = [&](Step &st, int i) __attribute__((always_inline)) {
+            request(st, jw + i * kRound, row(2 * i), row(2 * i + 1));
+        };
+        auto run = [&](Step &st, int i) __attribute__((always_inline)) {
+            const int j0 = jw + i * kRound;
+            // A tile past the last key has no page either, and is hidden by its positions; it
+            // read the one before it.
+            const bool bad = row(2 * i) == kNoPage;
+            step(st, j0, bad, row(2 * i + 1) == kNoPage && (bad || j0 + 16 < hi));
+        };
+        get(cur, 0);
+        for (int i = 0; i < cnt; i += 2) {
+            if (i + 1 < cnt) get(alt, i + 1);
+            run(cur, i);
+            if (i + 1 < cnt) {
+                if (i + 2 < cnt) get(cur, i + 2);
+                run(alt, i + 1);
+            }
+        }
+    }
+
+    // ---- the waves' states meet in LDS, a column tile at a time ----
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        l[c] = col_sum(l[c]);
+        if (kg == 0) {
+            s_m[wave][c][n] = m[c];
+            s_l[wave][c][n] = l[c];
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        if (c > 0) __syncthreads();  // the last tile's sums are read
+#pragma unroll
+        for (int i = 0; i < 4; ++i)  // row 4 kg + i of product e is channel CH (4 kg + i) + e
+#pragma unroll
+            for (int e = 0; e < CH; e += 4)
+                *reinterpret_cast<float4 *>(&s_o[wave][n][CH * (4 * kg + i) + e]) =
+                    make_float4(acc[c][e][i], acc[c][e + 1][i], acc[c][e + 2][i], acc[c][e + 3][i]);
+        __syncthreads();
+        for (int e = tid; e < 16 * D; e += 64 * kWaves) {
+            const int h = e / D, d = e - h * D, x = w.m0 + 16 * c + h;
+            if (x >= all) continue;
+            float mx = kNoMax;
+#pragma unroll
+            for (int v = 0; v < kWaves; ++v) mx = fmaxf(mx, s_m[v][c][h]);
+            float num = 0.0f, den = 0.0f;
+#pragma unroll
+            for (int v = 0; v < kWaves; ++v) {
+                const float r = __builtin_amdgcn_exp2f(s_m[v][c][h] - mx);
+                num = fmaf(s_o[v][h][d], r, num);
+                den = fmaf(s_l[v][c][h], r, den);
+            }
+            const int64_t row = out_row(p, w, x);
+            if (p.splits == 1) {
+                // Padding, and rows whose every key is without a page: zeros.
+                io<T>::st(out, row * D + d, x < w.t1 * p.R && den != 0.0f ? num / den : 0.0f);
+            } else {
+                float *part = p.part + (row * p.splits + blockIdx.y) * (D + 2);
+                part[d] = num;
+                if (d == 0) {
+                    part[D] = mx;
+                    part[D + 1] = den;
+                }
+            }
+        }
+    }
+}
+
+// The shares' states of one row: weights first (a thread each), then the values, 256 / D threads
+// per channel.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void attn_paged_join_kernel(AttnPagedParams p)
+{
+    constexpr int N = 256 / D;
+    __shared__ float s_w[kMaxSplits], s_red[4], s_den[4], s_num[N][D];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int H = p.G * p.R;
+    const int64_t row = blockIdx.x;
+    const int h = static_cast<int>(row % H), t = static_cast<int>(row / H % p.T);
+    const int g = h / p.R, x = t * p.R + (h - g * p.R);
+    const Where w = where(p, p.rows, static_cast<int>(row / H / p.T) * p.G + g, x / p.rows);
+    const int per = share_of(p, lane);
+    const int used = t < w.t1 ? (w.n + per - 1) / per : 0;
+    const float *part = p.part + row * p.splits * (D + 2);
+    const float mx = tid < used ? part[tid * (D + 2) + D] : kNoMax;
+    float den = tid < used ? part[tid * (D + 2) + D + 1] : 0.0f;
+    float m = mx;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    if (lane == 0) s_red[wave] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+    const float r = __builtin_amdgcn_exp2f(mx - m);
+    s_w[tid] = r;
+    den = wave_sum(den * r);
+    if (lane == 0) s_den[wave] = den;
+    __syncthreads();
+    const int d = tid % D, k = tid / D;
+    float num = 0.0f;
+#pragma unroll 8
+    for (int s = k; s < used; s += N) num = fmaf(part[s * (D + 2) + d], s_w[s], num);
+    s_num[k][d] = num;
+    __syncthreads();
+    if (tid >= D) return;
+    den = (s_den[0] + s_den[1]) + (s_den[2] + s_den[3]);
+#pragma unroll
+    for (int i = 1; i < N; ++i) num += s_num[i][d];
+    io<T>::st(static_cast<T *>(p.out), row * D + d, den == 0.0f ? 0.0f : num / den);
+}
+
+template <typename T, PrecKind PK, int D, int C>
+hipError_t paged_c(AttnPagedParams &p, hipStream_t s)
+{
+    const int bg = p.B * p.G;
+    const unsigned x = p.tiles > 1 ? static_cast<unsigned>((bg + 7) / 8) * 8u * p.tiles : bg;
+    hipLaunchKernelGGL((attn_paged_kernel<T, PK, D, C>), dim3(x, p.splits), dim3(64 * kWaves), 0, s, p);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || p.splits == 1) return e;
+    hipLaunchKernelGGL((attn_paged_join_kernel<T, D>), dim3(static_cast<unsigned>(bg) * p.T * p.R), dim3(256), 0, s, p);
+    return hipGetLastError();
+}
+
+template <typename T, PrecKind PK, int D>
+hipError_t paged_d(AttnPagedParams &p, hipStream_t s)
+{
+    switch (p.rows) {
+    case 16: return paged_c<T, PK, D, 1>(p, s);
+    case 32: return paged_c<T, PK, D, 2>(p, s);
+    default: return paged_c<T, PK, D, 4>(p, s);
+    }
+}
+
+}  // namespace
+
+// Rows of a workgroup: 16 columns for each matrix product, more where a group has more rows.
+int attn_paged_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+
+// Shares of the keys: enough workgroups for two on every CU, no share under 512 positions.
+int attn_paged_splits(int B, int G, int64_t rows, int64_t cap)
+{
+    const int per = attn_paged_rows(rows);
+    const int64_t wg = static_cast<int64_t>(B) * G * ((rows + per - 1) / per);
+    const int64_t least = wg < 128 ? 512 : 1024, most = (cap + least - 1) / least;
+    int64_t s = (512 + wg - 1) / wg;
+    const int64_t by_share = wg < 2048 ? (cap + 4095) / 4096 : 1;
+    s = s > by_share ? s : by_share;
+    s = s < most ? s : most;
+    return static_cast<int>(s < 1 ? 1 : (s > kMaxSplits ? kMaxSplits : s));
+}
+
+bool attn_paged_supported(int io_dtype, int D)
+{
+    return (io_dtype == GDN2_DTYPE_BF16 || io_dtype == GDN2_DTYPE_F16) && (D == 64 || D == 128);
+}
+
+hipError_t launch_attn_paged(AttnPagedParams p, int io_dtype, hipStream_t s)
+{
+    if (io_dtype == GDN2_DTYPE_BF16)
+        return p.D == 64 ? paged_d<bf16_t, PrecKind::BF16, 64>(p, s) : paged_d<bf16_t, PrecKind::BF16, 128>(p, s);
+    return p.D == 64 ? paged_d<f16_t, PrecKind::F16, 64>(p, s) : paged_d<f16_t, PrecKind::F16, 128>(p, s);
+}
+
+}  // namespace gdn2

@@ -428,6 +428,92 @@ struct Q4LoadParams {
 hipError_t launch_q4_store(const Q4StoreParams &p, int io_dtype, hipStream_t stream);
 hipError_t launch_q4_load(const Q4LoadParams &p, int io_dtype, hipStream_t stream);
 
+// Norms of q and k with the rotation, of a fused projection [B, T, G (R + 2) D] by strides; into
+// q [B, T, G R, D] and k [B, T, G, D], or (table) q and pages.
+struct QkvRopeParams {
+    const void *qkv;
+    int64_t stride_b, stride_t;
+    const void *wq, *wk;  // [D], NULL: no norm
+    int w_f32;            // weights (and their gradients) in float32, else the io dtype
+    float eps;
+    const float *cos, *sin;  // [table_rows][pairs]
+    int pairs;
+    int64_t table_rows;
+    const int64_t *pos;  // position of token (b, t) at b pos_b + t pos_t; NULL: t
+    int64_t pos_b, pos_t;
+    int pos_add_t;           // pos is that of a sequence's first token
+    const int64_t *lengths;  // tokens of a sequence that are there (NULL: all)
+    void *q, *k, *v;         // outputs (pages with table); backward: the gradients dq, dk, dv
+    const int *table;        // [B][table_cols], rows table_stride apart
+    int64_t table_stride, pages;
+    int table_cols, page;
+    int B, T, G, R, D;
+    void *dqkv, *dwq, *dwk;  // backward: [B, T, G (R + 2) D] contiguous, [D]
+    float *part;             // [qkv_rope_bwd_blocks][2][D]
+    // Set by the launcher: rows of a group and their reciprocal, units of a token and of
+    // all, 16-byte aligned tables.
+    int per;
+    unsigned per_m;
+    int units;
+    int64_t all_units;
+    int wide_tables;
+};
+int qkv_rope_lanes(int D);
+int qkv_rope_units(int rows, int D);
+int qkv_rope_bwd_blocks(int64_t units);
+hipError_t launch_qkv_rope_fwd(QkvRopeParams p, int io_dtype, hipStream_t stream);
+hipError_t launch_qkv_rope_bwd(QkvRopeParams p, int io_dtype, hipStream_t stream);
+
+// Attention of q [B, T, G R, D] (by strides) over pages [pages][G][page][D].
+struct AttnPagedParams {
+    const void *q;
+    int64_t qs[3];
+    const void *k, *v;
+    const int *table;  // [B][table_cols], rows table_stride apart
+    int64_t table_stride, pages;
+    int page, cap;       // rows of a page, positions of a sequence's row of the table
+    const int64_t *pos;  // position of each sequence's first token
+    int64_t pos_stride;
+    const int64_t *lengths;
+    void *out;  // [B, T, G R, D]
+    int B, T, G, R, D;
+    float scale;
+    int rows, tiles;  // rows of a workgroup, tiles of a group's T R rows
+    int splits;
+    float *part;  // with more than one: [B T G R][splits][D + 2]
+};
+int attn_paged_rows(int64_t rows);
+int attn_paged_splits(int B, int G, int64_t rows, int64_t cap);
+bool attn_paged_supported(int io_dtype, int D);
+hipError_t launch_attn_paged(AttnPagedParams p, int io_dtype, hipStream_t stream);
+
+// A token of each row of logits (rows by two strides, as the log probabilities') by the random
+// number u; settings for each row, or (NULL) for all.
+constexpr int kSampleBins = 512;   // bins of a row's weights
+constexpr int kSampleList = 8192;  // elements of a row's border bins that are listed
+constexpr int kSampleFinishThreads = 1024;
+constexpr int kSampleParts = 64;   // parts of a row at most
+constexpr int kSampleMax = 1 << 20;  // longest row: sums of 2^42 stay under 2^63, indices under 24 bits
+struct SampleParams {
+    const void *x;
+    int64_t inner, outer_stride, row_stride, rows;
+    int n;
+    const float *u, *temperature, *top_p, *min_p;
+    const int *top_k;
+    float temperature_all, top_p_all, min_p_all;
+    int top_k_all;
+    int64_t *out;
+    // The workspace (set by the launcher): of each row [bins][sum, count], the list, the parts'
+    // largest keys and kept sums, their least logits, and the number of listed elements.
+    unsigned long long *hist, *list, *part_key, *part_sum;
+    float *part_low;
+    unsigned *listed;
+    int parts, part_pieces, list_len;
+};
+int sample_parts(int64_t rows, int64_t n);
+size_t sample_row_bytes(int64_t n);
+hipError_t launch_sample(SampleParams p, void *workspace, int io_dtype, hipStream_t stream);
+
 // Backward of the short convolution on a prefill call (no cache).
 struct ConvBwdParams {
     const void *x;      // [B, T, D] input rows: row (b, t) at x + (b * T + t) * ldx

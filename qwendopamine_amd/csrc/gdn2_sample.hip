@@ -1,0 +1,766 @@
+// One token of each row of logits, drawn with a given random number under a temperature,
+// top-k, top-p and min-p, gfx950.
+//
+//   w_j = exp((x_j - max x) / T);  kept: w_j >= min_p; of those the k largest (equal logits: the
+//   lower index); of those, in that order, the shortest run whose sum reaches top_p of their
+//   sum;  token: the lowest index whose running sum of kept weights exceeds u times their total
+//
+// Weights are whole numbers, round(2^42 w): their sums do not depend on an order, so that
+// atomics and any split of a row give the same bits, and two passes that form the same
+// sum agree on every border.  An exponential in float64 costs no more issue slots than one
+// in float32 would save here.  Nothing is sorted.  Every filter keeps a run of the order
+// (logit, lower index), so all that is looked for is its last element:
+//   sample_max     each part's largest element and least logit
+//   sample_hist    counts and sums of the kept by bins that are even in log w
+//   sample_gather  the bins that the borders of top-k and top-p fall into: their elements are
+//                  listed, and what lies above them is summed for each part
+//   sample_finish  the borders themselves, by the digits of the listed elements' keys (of
+//                  the row's, if a bin holds more than the list: equal logits), the total,
+//                  the part that holds u times it, and the element within it
+// The logits are read once from memory and twice more from the caches behind the L2.
+#include "gdn2_common.h"
+#include "gdn2_internal.h"
+
+namespace gdn2 {
+namespace {
+
+typedef unsigned long long u64;
+
+constexpr int kFrac = 42;             // bits of a weight below 1
+constexpr float kFloor = -43.0f;      // log2 of weights that round to nothing
+constexpr int kThreads = 256;         // of the passes over parts
+constexpr int kFinish = kSampleFinishThreads;
+constexpr int kOwn = kSampleList / kFinish;
+constexpr double kLog2e = 1.4426950408889634074;
+
+// 2^y in units of 2^-42, y <= 0: 2^f by its series, |f| <= 1/2 (the first term left out is under
+// 6e-15 of it), rounded by the addition of 2^52.
+__device__ __forceinline__ u64 weight_of(double y)
+{
+    constexpr double c[12] = {1.0, 6.931471805599453094e-1, 2.402265069591007123e-1, 5.550410866482157995e-2,
+                              9.618129107628477162e-3, 1.333355814642844343e-3, 1.540353039338160995e-4,
+                              1.525273380405984028e-5, 1.321548679014430949e-6, 1.017808600923969973e-7,
+                              7.054911620801123329e-9, 4.445538271870811498e-10};
+    const double n = __builtin_rint(y), f = y - n;
+    double p = c[11];
+#pragma unroll
+    for (int i = 10; i >= 0; --i) p = fma(p, f, c[i]);
+    const double v = __builtin_amdgcn_ldexp(p, static_cast<int>(n) + kFrac) + 0x1p52;
+    return static_cast<u64>(__double_as_longlong(v)) & 0xfffffffffffffULL;
+}
+
+// Order of the elements: larger logit first (-0 = 0, NaN above all), of equal ones the lower
+// index.  24 bits of index under 32 of the logit, of 16-bit logits 16.
+template <typename T>
+struct Key {
+    static constexpr int bits = sizeof(T) == 4 ? 56 : 40;
+    static __device__ __forceinline__ u64 of(float v, int i)
+    {
+        const unsigned b = __float_as_uint(v + 0.0f);
+        unsigned k = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+        if (v != v) k = 0xffffffffu;
+        if constexpr (sizeof(T) == 2) {
+            if constexpr (std::is_same<T, f16_t>::value) {
+                const uint16_t h = __builtin_bit_cast(uint16_t, static_cast<_Float16>(v + 0.0f));
+                k = v != v ? 0xffffu : (h & 0x8000u) ? static_cast<uint16_t>(~h) : (h | 0x8000u);
+            } else {
+                k >>= 16;
+            }
+        }
+        return (static_cast<u64>(k) << 24) | (0xffffffu - static_cast<unsigned>(i));
+    }
+    static __device__ __forceinline__ float value(u64 key)
+    {
+        unsigned k = static_cast<unsigned>(key >> 24);
+        if constexpr (std::is_same<T, f16_t>::value) {
+            if (k == 0xffffu) return __uint_as_float(0x7fc00000u);
+            const uint16_t h = static_cast<uint16_t>((k & 0x8000u) ? (k & 0x7fffu) : ~k);
+            return static_cast<float>(__builtin_bit_cast(_Float16, h));
+        }
+        if constexpr (sizeof(T) == 2) k = k << 16 | (k & 0x8000u ? 0u : 0xffffu);
+        if (k == 0xffffffffu || k == 0xffff0000u) return __uint_as_float(0x7fc00000u);
+        return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
+    }
+    static __device__ __forceinline__ int index(u64 key) { return 0xffffff - static_cast<int>(key & 0xffffffu); }
+};
+
+// A row, read by 16-byte pieces of its memory; elements outside the row (the first and last
+// piece's) come as -inf.
+template <typename T>
+struct Logits {
+    static constexpr int N = 16 / static_cast<int>(sizeof(T));
+    const T *x, *xa;
+    int n, off, pieces;
+    __device__ __forceinline__ Logits(const SampleParams &p, int64_t row)
+    {
+        const int64_t b = row / p.inner;
+        x = static_cast<const T *>(p.x) + b * p.outer_stride + (row - b * p.inner) * p.row_stride;
+        n = p.n;
+        off = static_cast<int>(reinterpret_cast<uintptr_t>(x) & 15) / static_cast<int>(sizeof(T));
+        xa = x - off;
+        pieces = (off + n + N - 1) / N;
+    }
+    __device__ __forceinline__ int first(int c) const { return c * N - off; }
+    __device__ __forceinline__ void load(int c, float (&v)[N]) const
+    {
+        const int i0 = first(c);
+        if (i0 >= 0 && i0 + N <= n) {
+            const uint4 u = *reinterpret_cast<const uint4 *>(xa + static_cast<int64_t>(c) * N);
+            const unsigned w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (sizeof(T) == 4) {
+                    v[i] = __uint_as_float(w[i]);
+                } else if constexpr (std::is_same<T, bf16_t>::value) {
+                    v[2 * i] = __uint_as_float(w[i] << 16);
+                    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+                } else {
+                    v[2 * i] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w[i] & 0xffffu)));
+                    v[2 * i + 1] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w[i] >> 16)));
+                }
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[e] = i0 + e >= 0 && i0 + e < n ? io<T>::ld(x, i0 + e) : -INFINITY;
+        }
+    }
+};
+
+__device__ __forceinline__ u64 shfl_xor64(u64 x, int o) { return __shfl_xor(x, o, 64); }
+__device__ __forceinline__ u64 wave_max64(u64 x)
+{
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const u64 y = shfl_xor64(x, o);
+        x = x > y ? x : y;
+    }
+    return x;
+}
+__device__ __forceinline__ u64 wave_sum64(u64 x)
+{
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) x += shfl_xor64(x, o);
+    return x;
+}
+// Sum over the lanes up to and with this one.
+__device__ __forceinline__ u64 wave_scan64(u64 x, int lane)
+{
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const u64 y = __shfl_up(x, o, 64);
+        x += lane >= o ? y : 0;
+    }
+    return x;
+}
+
+// A row's settings and what the first pass found.
+struct RowState {
+    float top;     // largest logit
+    int best;      // its index
+    bool greedy;   // T = 0, or a largest logit that is not finite: the token is `best`
+    double per;    // log2 of the weight of a difference of 1
+    u64 least;     // smallest weight that min-p keeps (at least 1)
+    float scale;   // bins per factor of 2
+    double share;  // top_p; 1 and above: off
+    int k;         // top_k; 0: off
+};
+
+template <typename T>
+__device__ __forceinline__ RowState row_state(const SampleParams &p, int64_t row, int lane)
+{
+    RowState s;
+    const u64 key = wave_max64(lane < p.parts ? p.part_key[row * kSampleParts + lane] : 0);
+    float low = lane < p.parts ? p.part_low[row * kSampleParts + lane] : INFINITY;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) low = fminf(low, __shfl_xor(low, o, 64));
+    s.top = Key<T>::value(key);
+    s.best = Key<T>::index(key);
+    const float t = p.temperature ? p.temperature[row] : p.temperature_all;
+    const float m = p.min_p ? p.min_p[row] : p.min_p_all, share = p.top_p ? p.top_p[row] : p.top_p_all;
+    const int k = p.top_k ? p.top_k[row] : p.top_k_all;
+    s.greedy = !(t > 0.0f) || !(fabsf(s.top) < INFINITY);
+    s.per = kLog2e / static_cast<double>(fmaxf(t, 1e-30f));
+    const double least = m > 0.0f ? ceil(static_cast<double>(fminf(m, 1.0f)) * 0x1p42) : 1.0;
+    s.least = least > 1.0 ? static_cast<u64>(least) : 1;
+    // Bins over the weights that there are: down to 2^-43, the least logit's, or min-p's.
+    float range = fminf(-kFloor, static_cast<float>((static_cast<double>(s.top) - static_cast<double>(low)) * s.per));
+    if (m > 0.0f) range = fminf(range, 1e-3f - 1.0001f * __builtin_amdgcn_logf(fminf(m, 1.0f)));
+    s.scale = range > 0.0f ? kSampleBins / range : 0.0f;
+    s.share = share < 1.0f ? (share > 1e-30f ? static_cast<double>(share) : 1e-30) : 1.0;
+    if (share != share) s.share = 1.0;
+    s.k = k > 0 && k < p.n ? k : 0;
+    return s;
+}
+__device__ __forceinline__ bool filters(const RowState &s) { return s.k > 0 || s.share < 1.0; }
+
+__device__ __forceinline__ double log_weight(const RowState &s, float x)
+{
+    return (static_cast<double>(x) - static_cast<double>(s.top)) * s.per;
+}
+__device__ __forceinline__ int bin_of(const RowState &s, double y)
+{
+    const int b = static_cast<int>(static_cast<float>(-y) * s.scale);
+    return b < kSampleBins ? b : kSampleBins - 1;
+}
+
+// The pieces of a part.
+__device__ __forceinline__ void part_range(const SampleParams &p, int pieces, int part, int &lo, int &hi)
+{
+    lo = part * p.part_pieces;
+    hi = lo + p.part_pieces < pieces ? lo + p.part_pieces : pieces;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void sample_max_kernel(SampleParams p)
+{
+    constexpr int N = Logits<T>::N, U = 4;
+    __shared__ u64 s_key[kThreads / 64];
+    __shared__ float s_low[kThreads / 64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t row = blockIdx.x / p.parts;
+    const int part = static_cast<int>(blockIdx.x - row * p.parts);
+    if (part == 0) {  // what the next passes add to
+        u64 *h = p.hist + row * (2 * kSampleBins);
+        for (int i = tid; i < 2 * kSampleBins; i += kThreads) h[i] = 0;
+        if (tid == 0) p.listed[row] = 0;
+    }
+    const Logits<T> x(p, row);
+    int lo, hi;
+    part_range(p, x.pieces, part, lo, hi);
+    u64 best = 0;
+    float low = INFINITY;
+    for (int c0 = lo + tid; c0 < hi; c0 += U * kThreads) {
+        float v[U][N];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (c0 + u * kThreads < hi) x.load(c0 + u * kThreads, v[u]);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (c0 + u * kThreads >= hi) break;
+            // The piece's first largest (or first NaN), then one comparison of keys.
+            float m = v[u][0];
+            int at = 0;
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const float y = v[u][e];
+                const bool more = e > 0 && (y > m || (y != y && m == m));
+                m = more ? y : m;
+                at = more ? e : at;
+                low = y > -INFINITY ? fminf(low, y) : low;
+            }
+            const int i = x.first(c0 + u * kThreads) + at;
+            if (i >= 0 && i < x.n) {
+                const u64 key = Key<T>::of(m, i);
+                best = best > key ? best : key;
+            } else {
+                // The row's first piece, of -inf alone as far as its maximum goes.
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const int j = x.first(c0 + u * kThreads) + e;
+                    if (j < 0 || j >= x.n) continue;
+                    const u64 key = Key<T>::of(v[u][e], j);
+                    best = best > key ? best : key;
+                }
+            }
+        }
+    }
+    best = wave_max64(best);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) low = fminf(low, __shfl_xor(low, o, 64));
+    if (lane == 0) {
+        s_key[wave] = best;
+        s_low[wave] = low;
+    }
+    __syncthreads();
+    if (tid == 0) {
+#pragma unroll
+        for (int w = 1; w < kThreads / 64; ++w) {
+            best = best > s_key[w] ? best : s_key[w];
+            low = fminf(low, s_low[w]);
+        }
+        p.part_key[row * kSampleParts + part] = best;
+        p.part_low[row * kSampleParts + part] = low;
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void sample_hist_kernel(SampleParams p)
+{
+    constexpr int N = Logits<T>::N, U = 4;
+    __shared__ u64 s_sum[kSampleBins];
+    __shared__ unsigned s_count[kSampleBins];
+    __shared__ u64 s_part[kThreads / 64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t row = blockIdx.x / p.parts;
+    const int part = static_cast<int>(blockIdx.x - row * p.parts);
+    const RowState s = row_state<T>(p, row, lane);
+    if (s.greedy) return;
+    const bool bins = filters(s);
+    if (bins) {
+        for (int i = tid; i < kSampleBins; i += kThreads) {
+            s_sum[i] = 0;
+            s_count[i] = 0;
+        }
+        __syncthreads();
+    }
+    const Logits<T> x(p, row);
+    int lo, hi;
+    part_range(p, x.pieces, part, lo, hi);
+    u64 sum = 0;
+    for (int c0 = lo + tid; c0 < hi; c0 += U * kThreads) {
+        float v[U][N];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (c0 + u * kThreads < hi) x.load(c0 + u * kThreads, v[u]);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (c0 + u * kThreads >= hi) break;
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const double y = log_weight(s, v[u][e]);
+                if (!(y >= static_cast<double>(kFloor))) continue;
+                const u64 w = weight_of(y);
+                if (w < s.least) continue;
+                if (bins) {
+                    const int b = bin_of(s, y);
+                    atomicAdd(&s_sum[b], w);
+                    atomicAdd(&s_count[b], 1u);
+                } else {
+                    sum += w;
+                }
+            }
+        }
+    }
+    if (!bins) {
+        sum = wave_sum64(sum);
+        if (lane == 0) s_part[wave] = sum;
+        __syncthreads();
+        if (tid == 0) p.part_sum[row * kSampleParts + part] = (s_part[0] + s_part[1]) + (s_part[2] + s_part[3]);
+        return;
+    }
+    __syncthreads();
+    u64 *h = p.hist + row * (2 * kSampleBins);
+    for (int i = tid; i < kSampleBins; i += kThreads) {
+        if (s_count[i] == 0) continue;
+        atomicAdd(h + 2 * i, s_sum[i]);
+        atomicAdd(h + 2 * i + 1, static_cast<u64>(s_count[i]));
+    }
+}
+
+// The bins that the borders fall into.
+struct Borders {
+    int sure;          // bins below this one are kept whole
+    int p_lo, p_hi;    // top-p's border lies in these (p_lo > p_hi: off)
+    int k_bin;         // top-k's in this one (-1: off)
+    u64 k_sum, k_count;  // what lies before it
+    u64 p_sum;           // what lies before p_lo
+    u64 total;           // sum of the row (what min-p keeps)
+    __device__ __forceinline__ bool listed(int b) const { return (b >= p_lo && b <= p_hi) || b == k_bin; }
+};
+
+// By one wave, from a row's bins: 8 in turn a lane.
+__device__ __forceinline__ Borders borders_of(const RowState &s, const u64 *hist, int lane)
+{
+    constexpr int E = kSampleBins / 64;
+    u64 sum[E], count[E], own_s = 0, own_c = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const ulonglong2 h = *reinterpret_cast<const ulonglong2 *>(hist + 2 * (lane * E + e));
+        sum[e] = own_s += h.x;
+        count[e] = own_c += h.y;
+    }
+    const u64 base_s = wave_scan64(own_s, lane) - own_s, base_c = wave_scan64(own_c, lane) - own_c;
+    Borders r;
+    r.total = __shfl(base_s + own_s, 63, 64);
+    const u64 all = __shfl(base_c + own_c, 63, 64);
+    // The first lane whose condition holds for some bin, and that bin: bins are in order, so
+    // the least bin over the wave.
+    auto least = [&](int b) {
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_xor(b, o, 64);
+            b = b < y ? b : y;
+        }
+        return b;
+    };
+    auto before = [&](int b, u64 &ps, u64 &pc) {  // sums before bin b
+        u64 a = 0, c = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (lane * E + e == b) {
+                a = base_s + (e ? sum[e - 1] : 0);
+                c = base_c + (e ? count[e - 1] : 0);
+            }
+        ps = wave_sum64(a);
+        pc = wave_sum64(c);
+    };
+    r.k_bin = -1;
+    r.k_sum = r.k_count = 0;
+    u64 lo_sum = r.total, hi_sum = r.total;  // bounds of what top-k leaves
+    int last = kSampleBins - 1;
+    if (s.k > 0 && static_cast<u64>(s.k) < all) {
+        int b = kSampleBins;
+#pragma unroll
+        for (int e = E - 1; e >= 0; --e)
+            if (base_c + count[e] >= static_cast<u64>(s.k)) b = lane * E + e;
+        r.k_bin = last = least(b);
+        before(r.k_bin, r.k_sum, r.k_count);
+        lo_sum = r.k_sum;
+        u64 dummy;
+        hi_sum = r.total;
+        if (r.k_bin + 1 < kSampleBins) before(r.k_bin + 1, hi_sum, dummy);
+    }
+    r.p_lo = kSampleBins;
+    r.p_hi = -1;
+    r.p_sum = 0;
+    r.sure = r.k_bin >= 0 ? r.k_bin : kSampleBins;
+    if (s.share < 1.0) {
+        // An element is kept if what precedes it is less than the share: a whole bin if even
+        // its end is, none of it if its beginning is not.
+        const double low = s.share * static_cast<double>(lo_sum), high = s.share * static_cast<double>(hi_sum);
+        int a = kSampleBins, b = kSampleBins;
+#pragma unroll
+        for (int e = E - 1; e >= 0; --e) {
+            if (!(static_cast<double>(base_s + sum[e]) < low)) a = lane * E + e;
+            if (!(static_cast<double>(base_s + (e ? sum[e - 1] : 0)) < high)) b = lane * E + e;
+        }
+        a = least(a);
+        b = least(b) - 1;
+        r.p_lo = a < last ? a : last;
+        r.p_hi = b < last ? b : last;
+        u64 dummy;
+        before(r.p_lo, r.p_sum, dummy);
+        r.sure = r.p_lo < r.sure ? r.p_lo : r.sure;
+    }
+    return r;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleParams p)
+{
+    constexpr int N = Logits<T>::N, U = 4;
+    __shared__ u64 s_part[kThreads / 64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t row = blockIdx.x / p.parts;
+    const int part = static_cast<int>(blockIdx.x - row * p.parts);
+    const RowState s = row_state<T>(p, row, lane);
+    if (s.greedy || !filters(s)) return;
+    const Borders b = borders_of(s, p.hist + row * (2 * kSampleBins), lane);
+    const int need = b.p_hi > b.k_bin ? b.p_hi : b.k_bin;  // no bin past this one is wanted
+    const int last = need > b.sure - 1 ? need : b.sure - 1;
+    const Logits<T> x(p, row);
+    int lo, hi;
+    part_range(p, x.pieces, part, lo, hi);
+    u64 sum = 0;
+    for (int c0 = lo + tid; c0 < hi; c0 += U * kThreads) {
+        float v[U][N];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (c0 + u * kThreads < hi) x.load(c0 + u * kThreads, v[u]);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (c0 + u * kThreads >= hi) break;
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const double y = log_weight(s, v[u][e]);
+                if (!(y >= static_cast<double>(kFloor))) continue;
+                const int bin = bin_of(s, y);
+                if (bin > last) continue;
+                const u64 w = weight_of(y);
+                if (w < s.least) continue;
+                if (bin < b.sure) {
+                    sum += w;
+                } else if (b.listed(bin)) {
+                    const unsigned at = atomicAdd(p.listed + row, 1u);
+                    if (at < static_cast<unsigned>(p.list_len))
+                        p.list[row * p.list_len + at] = Key<T>::of(v[u][e], x.first(c0 + u * kThreads) + e);
+                }
+            }
+        }
+    }
+    sum = wave_sum64(sum);
+    if (lane == 0) s_part[wave] = sum;
+    __syncthreads();
+    if (tid == 0) p.part_sum[row * kSampleParts + part] = (s_part[0] + s_part[1]) + (s_part[2] + s_part[3]);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kFinish) void sample_finish_kernel(SampleParams p)
+{
+    constexpr int N = Logits<T>::N, kW = kFinish / 64;
+    __shared__ u64 s_sum[256], s_count[256], s_part[kSampleParts], s_wave[kW];
+    __shared__ u64 s_pick[4], s_last;
+    __shared__ int s_found;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t row = blockIdx.x;
+    const RowState s = row_state<T>(p, row, lane);
+    if (s.greedy) {
+        if (tid == 0) p.out[row] = s.best;
+        return;
+    }
+    const Logits<T> x(p, row);
+    if (tid < kSampleParts) s_part[tid] = tid < p.parts ? p.part_sum[row * kSampleParts + tid] : 0;
+    if (tid == 0) s_found = 0;
+    u64 thr = 0;  // the last kept key
+    if (filters(s)) {
+        const Borders b = borders_of(s, p.hist + row * (2 * kSampleBins), lane);
+        const unsigned n = p.listed[row];
+        const bool from_list = n <= static_cast<unsigned>(p.list_len);
+        u64 own[kOwn];
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) {
+            const unsigned at = tid + i * kFinish;
+            own[i] = from_list && at < n ? p.list[row * p.list_len + at] : 0;  // no element's key is 0
+        }
+        // f(key, weight, bin) of the listed bins' elements, from the list or the row.
+        auto each = [&](auto f) __attribute__((always_inline)) {
+            if (from_list) {
+#pragma unroll
+                for (int i = 0; i < kOwn; ++i) {
+                    if (own[i] == 0) continue;
+                    const double y = log_weight(s, Key<T>::value(own[i]));
+                    f(own[i], weight_of(y), bin_of(s, y));
+                }
+            } else {
+                for (int c = tid; c < x.pieces; c += kFinish) {
+                    float v[N];
+                    x.load(c, v);
+#pragma unroll
+                    for (int e = 0; e < N; ++e) {
+                        const double y = log_weight(s, v[e]);
+                        if (!(y >= static_cast<double>(kFloor))) continue;
+                        const int bin = bin_of(s, y);
+                        if (!b.listed(bin)) continue;
+                        const u64 w = weight_of(y);
+                        if (w >= s.least) f(Key<T>::of(v[e], x.first(c) + e), w, bin);
+                    }
+                }
+            }
+        };
+        // The last of the elements in bins lo .. hi with keys from `least` on before which there is
+        // less than the target (`by_sum`: of sum, else of number), `sum0` and `count0` preceding them all.
+        // Digit by digit of the key, from the highest.  `sum0` becomes the sum up to and with it.
+        auto select = [&](bool by_sum, double target, int lo, int hi, u64 least, u64 &sum0, u64 count0) {
+            u64 prefix = 0;
+            for (int shift = Key<T>::bits - 8; shift >= 0; shift -= 8) {
+                __syncthreads();
+                if (tid < 256) s_sum[tid] = s_count[tid] = 0;
+                __syncthreads();
+                each([&](u64 key, u64 w, int bin) __attribute__((always_inline)) {
+                    if (bin < lo || bin > hi || key < least || (key >> shift) >> 8 != prefix) return;
+                    const int d = 255 - static_cast<int>((key >> shift) & 255);
+                    atomicAdd(&s_sum[d], w);
+                    atomicAdd(&s_count[d], 1ull);
+                });
+                __syncthreads();
+                if (wave == 0) {
+                    // Digits from the highest down, four in turn a lane.
+                    u64 a[4], c[4], as = 0, cs = 0;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        a[e] = s_sum[4 * lane + e];
+                        c[e] = s_count[4 * lane + e];
+                        as += a[e];
+                        cs += c[e];
+                    }
+                    u64 bs = sum0 + wave_scan64(as, lane) - as, bc = count0 + wave_scan64(cs, lane) - cs;
+                    int best = -1;
+                    u64 best_s = 0, best_c = 0, best_n = 0;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if (c[e] > 0 && (by_sum ? static_cast<double>(bs) : static_cast<double>(bc)) < target) {
+                            best = 4 * lane + e;
+                            best_s = bs;
+                            best_c = bc;
+                            best_n = c[e];
+                        }
+                        bs += a[e];
+                        bc += c[e];
+                    }
+                    int top = best;
+#pragma unroll
+                    for (int o = 1; o < 64; o <<= 1) {
+                        const int y = __shfl_xor(top, o, 64);
+                        top = top > y ? top : y;
+                    }
+                    if (top >= 0 && best == top) {
+                        s_pick[0] = top;
+                        s_pick[1] = best_s;
+                        s_pick[2] = best_c;
+                        s_pick[3] = best_n;
+                    }
+                    if (top < 0 && lane == 0) s_pick[0] = 256;
+                }
+                __syncthreads();
+                if (s_pick[0] == 256) return ~0ull;  // none
+                prefix = prefix << 8 | (255 - s_pick[0]);
+                sum0 = s_pick[1];
+                count0 = s_pick[2];
+                if (s_pick[3] == 1 || shift == 0) {
+                    // A single element is left: its own key, as others than these elements may share
+                    // the digits so far.
+                    sum0 += s_sum[static_cast<int>(s_pick[0])];
+                    each([&](u64 key, u64, int bin) __attribute__((always_inline)) {
+                        if (bin >= lo && bin <= hi && key >= least && key >> shift == prefix) s_last = key;
+                    });
+                    __syncthreads();
+                    return s_last;
+                }
+            }
+            return prefix;  // not reached: keys differ
+        };
+        u64 total = b.total;
+        if (b.k_bin >= 0) {
+            total = b.k_sum;
+            thr = select(false, static_cast<double>(s.k), b.k_bin, b.k_bin, 0, total, b.k_count);
+        }
+        if (s.share < 1.0) {
+            u64 sum = b.p_sum;
+            const u64 at = select(true, s.share * static_cast<double>(total), b.p_lo, b.p_hi, thr, sum, 0);
+            // No listed element is kept: the border lies at the end of the bins before.
+            if (at == ~0ull) thr = ~0ull;
+            else thr = thr > at ? thr : at;
+        }
+        __syncthreads();
+        // What the list adds to the parts.
+        each([&](u64 key, u64 w, int bin) __attribute__((always_inline)) {
+            if (key >= thr && bin >= b.sure)
+                atomicAdd(&s_part[(Key<T>::index(key) + x.off) / N / p.part_pieces], w);
+        });
+        if (thr == ~0ull) {
+            // Elements of whole bins are told by their bin alone.
+            thr = 0;
+            s_pick[0] = b.sure;
+        } else {
+            s_pick[0] = kSampleBins;
+        }
+    } else {
+        s_pick[0] = kSampleBins;
+    }
+    __syncthreads();
+    const int bins = static_cast<int>(s_pick[0]);
+    // The part that holds u times the total (every wave by itself), and what is left of it there.
+    const u64 own = lane < kSampleParts ? s_part[lane] : 0;
+    const u64 upto = wave_scan64(own, lane), total = __shfl(upto, 63, 64);
+    const float u = p.u[row];
+    const double share = u > 0.0f ? static_cast<double>(u) * static_cast<double>(total) : 0.0;
+    u64 target = share < static_cast<double>(total) ? static_cast<u64>(share) : total;
+    if (target >= total) target = total > 0 ? total - 1 : 0;
+    const u64 past = __ballot(upto > target);
+    const int part = past ? __ffsll(past) - 1 : 0;
+    target -= __shfl(upto - own, part, 64);
+    int lo, hi;
+    part_range(p, x.pieces, part, lo, hi);
+    // The element: running sums of the part's pieces, one a thread.
+    u64 run = 0;
+    for (int c0 = lo; c0 < hi; c0 += kFinish) {
+        const int c = c0 + tid;
+        u64 w[N], mine = 0;
+        if (c < hi) {
+            float v[N];
+            x.load(c, v);
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const double y = log_weight(s, v[e]);
+                w[e] = 0;
+                if (y >= static_cast<double>(kFloor) && Key<T>::of(v[e], x.first(c) + e) >= thr && bin_of(s, y) < bins) {
+                    const u64 a = weight_of(y);
+                    w[e] = a >= s.least ? a : 0;
+                }
+                mine += w[e];
+            }
+        }
+        const u64 in = wave_scan64(mine, lane);
+        if (lane == 63) s_wave[wave] = in;
+        __syncthreads();
+        u64 base = run;
+        for (int i = 0; i < wave; ++i) base += s_wave[i];
+        u64 all = run;
+        for (int i = 0; i < kW; ++i) all += s_wave[i];
+        u64 at = base + in - mine;
+        if (mine > 0 && at <= target && target < base + in) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                if (w[e] > 0 && at <= target && target < at + w[e]) {
+                    p.out[row] = x.first(c) + e;
+                    s_found = 1;
+                }
+                at += w[e];
+            }
+        }
+        run = all;
+        __syncthreads();  // s_wave is read
+        if (run > target) break;
+    }
+    __syncthreads();
+    if (tid == 0 && !s_found) p.out[row] = s.best;
+}
+
+template <typename T>
+hipError_t sample_t(const SampleParams &p, hipStream_t s)
+{
+    const dim3 grid(static_cast<unsigned>(p.rows * p.parts));
+    hipLaunchKernelGGL((sample_max_kernel<T>), grid, dim3(kThreads), 0, s, p);
+    hipError_t e = hipGetLastError();
+    // What the settings given to all rows make needless is not launched.
+    const bool greedy = !p.temperature && !(p.temperature_all > 0.0f);
+    const bool filtered = p.top_k || p.top_p || p.top_k_all > 0 || p.top_p_all < 1.0f;
+    if (e == hipSuccess && !greedy) {
+        hipLaunchKernelGGL((sample_hist_kernel<T>), grid, dim3(kThreads), 0, s, p);
+        e = hipGetLastError();
+        if (e == hipSuccess && filtered) {
+            hipLaunchKernelGGL((sample_gather_kernel<T>), grid, dim3(kThreads), 0, s, p);
+            e = hipGetLastError();
+        }
+    }
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((sample_finish_kernel<T>), dim3(static_cast<unsigned>(p.rows)), dim3(kFinish), 0, s, p);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+// Parts of a row: enough workgroups for the card, none under 2048 elements, at most a wave's lanes.
+int sample_parts(int64_t rows, int64_t n)
+{
+    const int64_t most = (n + 2047) / 2048;
+    int64_t c = (2048 + rows - 1) / rows;
+    c = c < most ? c : most;
+    return static_cast<int>(c < 1 ? 1 : (c > kSampleParts ? kSampleParts : c));
+}
+
+// A row's workspace: bins, list, parts' keys, sums and least logits, the number listed.
+static int sample_list(int64_t n) { return static_cast<int>(n < kSampleList ? n : kSampleList); }
+
+size_t sample_row_bytes(int64_t n)
+{
+    return 2 * kSampleBins * sizeof(u64) + sample_list(n) * sizeof(u64) + kSampleParts * (2 * sizeof(u64) + sizeof(float)) +
+           sizeof(u64);
+}
+
+hipError_t launch_sample(SampleParams p, void *workspace, int io_dtype, hipStream_t s)
+{
+    u64 *w = static_cast<u64 *>(workspace);
+    p.list_len = sample_list(p.n);
+    p.hist = w;
+    w += p.rows * 2 * kSampleBins;
+    p.list = w;
+    w += p.rows * p.list_len;
+    p.part_key = w;
+    w += p.rows * kSampleParts;
+    p.part_sum = w;
+    w += p.rows * kSampleParts;
+    p.part_low = reinterpret_cast<float *>(w);
+    p.listed = reinterpret_cast<unsigned *>(p.part_low + p.rows * kSampleParts);
+    p.parts = sample_parts(p.rows, p.n);
+    const int per = io_dtype == GDN2_DTYPE_F32 ? 4 : 8;
+    const int pieces = (p.n + per - 1) / per + 1;  // of a row at any alignment
+    p.part_pieces = (pieces + p.parts - 1) / p.parts;
+    switch (io_dtype) {
+    case GDN2_DTYPE_F32: return sample_t<float>(p, s);
+    case GDN2_DTYPE_BF16: return sample_t<bf16_t>(p, s);
+    default: return sample_t<f16_t>(p, s);
+    }
+}
+
+}  // namespace gdn2

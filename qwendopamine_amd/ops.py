@@ -57,6 +57,13 @@ __all__ = [
     "kv_cache_q4_store",
     "kv_cache_q4_load",
     "attention_decode_q4",
+    "qkv_norm_rope",
+    "QkvNormRopeFunction",
+    "KVCachePaged",
+    "kv_cache_paged",
+    "kv_cache_paged_append",
+    "attention_paged",
+    "sample_tokens",
     "token_logprobs",
     "TokenLogprobs",
     "TokenLogprobsFunction",
@@ -1548,7 +1555,7 @@ def attention_supported(q: torch.Tensor, head_dim: int) -> bool:
     return q.is_cuda and q.dtype in (torch.bfloat16, torch.float16) and head_dim in (64, 128)
 
 
-_I64x6, _I64x9 = ctypes.c_int64 * 6, ctypes.c_int64 * 9
+_I64x3, _I64x6, _I64x9 = ctypes.c_int64 * 3, ctypes.c_int64 * 6, ctypes.c_int64 * 9
 
 
 def _attention_fwd(q, k, v, scale: float, causal: bool, kv_len, cu_dev, cu_host, keep: bool):
@@ -1846,6 +1853,313 @@ def attention_decode_q4(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
     return out
 
 
+def _qkv_rows(name: str, qkv: torch.Tensor, n_head: int, n_query_groups: int) -> tuple[torch.Tensor, int, int, int, int]:
+    """``(qkv as the kernels read it, B, T, query heads per group, D)`` of a fused projection
+    ``[B, T, (n_head + 2 G) D]``: in place where channels are contiguous and rows start on 16 bytes."""
+    G = n_query_groups
+    if qkv.dim() != 3 or n_head < 1 or G < 1 or n_head % G != 0 or qkv.shape[2] % (n_head + 2 * G) != 0:
+        raise ValueError(f"{name}: qkv must be [B, T, (n_head + 2 G) D] with n_head a multiple of G; got "
+                         f"{tuple(qkv.shape)}, {n_head} heads, {G} groups")
+    B, T, width = qkv.shape
+    D = width // (n_head + 2 * G)
+    nat.dtype_code(qkv.dtype)
+    if D < 8 or D % 8 != 0 or D > 256 or n_head + 2 * G > 65535:
+        raise NotImplementedError(f"{name}: heads of a multiple of 8 channels up to 256, at most 65535 of them; got {D}")
+    per = 16 // qkv.element_size()
+    if qkv.stride(2) != 1 or qkv.data_ptr() % 16 != 0 or any(
+            qkv.stride(i) % per != 0 for i in range(2) if qkv.shape[i] > 1):
+        qkv = qkv.contiguous()
+        qkv = qkv if qkv.data_ptr() % 16 == 0 else qkv.clone()
+    return qkv, B, T, n_head // G, D
+
+
+def _head_weights(name: str, q_weight, k_weight, D: int, dtype: torch.dtype) -> None:
+    if (q_weight is None) != (k_weight is None):
+        raise ValueError(f"{name}: q_weight and k_weight go together")
+    if q_weight is None:
+        return
+    if q_weight.shape != (D,) or k_weight.shape != (D,):
+        raise ValueError(f"{name}: weights must be [{D}]; got {tuple(q_weight.shape)}, {tuple(k_weight.shape)}")
+    if q_weight.dtype != k_weight.dtype or q_weight.dtype not in (dtype, torch.float32):
+        raise ValueError(f"{name}: weights must both be {dtype} or float32; got {q_weight.dtype}, {k_weight.dtype}")
+
+
+def _rope_tables(name: str, cos: torch.Tensor, sin: torch.Tensor, D: int) -> tuple[int, int]:
+    """``(pairs, rows)`` of rotation tables ``[rows, pairs]``."""
+    if cos.dim() != 2 or sin.shape != cos.shape or 2 * cos.shape[1] > D:
+        raise ValueError(f"{name}: cos and sin must be [rows, up to D / 2 pairs]; got {tuple(cos.shape)}, {tuple(sin.shape)}")
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or not (cos.is_contiguous() and sin.is_contiguous()):
+        raise ValueError(f"{name}: rotation tables must be contiguous fp32")
+    if _differentiated(cos, sin):
+        raise ValueError(f"{name}: no gradient passes to the rotation tables")
+    return cos.shape[1], cos.shape[0]
+
+
+def _one_device(name: str, first: torch.Tensor, *others: torch.Tensor | None) -> None:
+    _require_gpu(name, first, *others)
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{name}: tensors on {first.device} and {t.device}")
+
+
+def _aligned(x: torch.Tensor | None) -> torch.Tensor | None:
+    """A weight as the kernels read it: contiguous, on 16 bytes."""
+    if x is None:
+        return None
+    x = x.detach().contiguous()
+    return x if x.data_ptr() % 16 == 0 else x.clone()
+
+
+def _qkv_norm_rope_fwd(qkv, wq, wk, cos, sin, pos, G: int, R: int, D: int, eps: float):
+    B, T, _ = qkv.shape
+    dt, dev = qkv.dtype, qkv.device
+    q = torch.empty((B, T, G * R, D), dtype=dt, device=dev)
+    k = torch.empty((B, T, G, D), dtype=dt, device=dev)
+    w_code = nat.dtype_code(dt if wq is None else wq.dtype)
+    with _on_device(dev):
+        st = nat.load().gdn2_qkv_norm_rope_fwd(
+            qkv.data_ptr(), qkv.stride(0), qkv.stride(1), nat.dtype_code(dt), nat.ptr(wq), nat.ptr(wk), w_code, eps,
+            cos.data_ptr(), sin.data_ptr(), cos.shape[1], cos.shape[0], nat.ptr(pos),
+            0 if pos is None else pos.stride(0), 0 if pos is None else pos.stride(1), q.data_ptr(), k.data_ptr(), B, T,
+            G, R, D, nat.stream_handle(dev))
+    nat.check(st, "qkv_norm_rope")
+    return q, k, qkv.detach().unflatten(-1, (G, R + 2, D))[..., R + 1, :]
+
+
+class QkvNormRopeFunction(torch.autograd.Function):
+    """:func:`qkv_norm_rope` with the HIP forward and backward (``gdn2_qkv_norm_rope_fwd`` /
+    ``gdn2_qkv_norm_rope_bwd``): the projection itself is all that is kept, and only with weights."""
+
+    @staticmethod
+    def forward(ctx, qkv, q_weight, k_weight, cos, sin, pos, n_head: int, G: int, eps: float):
+        qkv, _, _, R, D = _qkv_rows("qkv_norm_rope", qkv, n_head, G)
+        wq, wk = _aligned(q_weight), _aligned(k_weight)
+        ctx.save_for_backward(None if wq is None else qkv, wq, wk, cos, sin, pos)
+        ctx.dims = G, R, D, eps, qkv.shape, qkv.dtype
+        return _qkv_norm_rope_fwd(qkv, wq, wk, cos, sin, pos, G, R, D, eps)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq, dk, dv):
+        qkv, wq, wk, cos, sin, pos = ctx.saved_tensors
+        G, R, D, eps, shape, dt = ctx.dims
+        B, T, _ = shape
+        dq, dk, dv = (_io(x, dt) for x in (dq, dk, dv))
+        dev = dq.device
+        dqkv = torch.empty(shape, dtype=dt, device=dev)
+        x = dqkv if qkv is None else qkv  # without weights the projection is not read
+        dwq, dwk = (None, None) if wq is None else (torch.empty_like(wq), torch.empty_like(wk))
+        if wq is not None and B * T == 0:
+            dwq.zero_()
+            dwk.zero_()
+        lib = nat.load()
+        nbytes = 0 if wq is None else lib.gdn2_qkv_norm_rope_bwd_workspace_size(B, T, G, R, D)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        with _on_device(dev):
+            st = lib.gdn2_qkv_norm_rope_bwd(
+                x.data_ptr(), x.stride(0), x.stride(1), nat.dtype_code(dt), nat.ptr(wq), nat.ptr(wk),
+                nat.dtype_code(dt if wq is None else wq.dtype), eps, cos.data_ptr(), sin.data_ptr(), cos.shape[1],
+                cos.shape[0], nat.ptr(pos), 0 if pos is None else pos.stride(0), 0 if pos is None else pos.stride(1),
+                dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dqkv.data_ptr(), nat.ptr(dwq), nat.ptr(dwk), B, T, G, R, D,
+                nat.ptr(ws), nbytes, nat.stream_handle(dev))
+        nat.check(st, "qkv_norm_rope backward")
+        return dqkv, dwq, dwk, None, None, None, None, None, None
+
+
+@torch.compiler.disable
+def qkv_norm_rope(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, n_head: int, n_query_groups: int,
+                  q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-5,
+                  input_pos: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Queries, keys and values of an attention layer from its fused projection in one pass: the RMS
+    norm of every query and key head (with weights) and the rotation of positions (reference
+    ``apply_rotary_emb`` and the split of ``CausalSelfAttention.forward``, ``gdn2_gpt/model.py:40-61,
+    89-173``; the norms have no counterpart there).  Differentiable in ``qkv`` and the weights.
+
+    ``qkv`` ``[B, T, (n_head + 2 G) D]`` laid out ``[G, n_head / G + 2, D]`` (bf16, fp16 or float32, ``D`` a
+    multiple of 8 up to 256; any strides, read in place where channels are contiguous and rows
+    16-byte aligned), ``q_weight`` / ``k_weight`` ``[D]`` (``qkv``'s dtype or float32; without them no norm),
+    ``cos`` / ``sin`` tables ``[rows, rot / 2]`` (fp32, contiguous) for the first ``rot`` channels, pairs
+    ``(2 i, 2 i + 1)``.  Token ``t`` takes row ``t``, or with ``input_pos`` (device int64, ``[T]`` or ``[B, T]``)
+    that of its position; a position outside the tables gives zeros for q and k and passes no gradient.
+
+    Returns ``q`` ``[B, T, n_head, D]``, ``k`` ``[B, T, G, D]`` and ``v`` ``[B, T, G, D]``, a view of ``qkv``
+    that must not be written to.  Norm and rotation are float32, rounded once (the rotation alone has
+    the bits of the host's torch path).  The weights' gradients are summed in a fixed order: the
+    same bits in every run.  In a HIP graph, capture the forward and backward together with no
+    eager autograd graph of the same leaves alive, as torch asks of any captured backward.  Second
+    derivatives and forward-mode tangents are refused."""
+    name = "qkv_norm_rope"
+    x, B, T, R, D = _qkv_rows(name, qkv, n_head, n_query_groups)
+    _head_weights(name, q_weight, k_weight, D, qkv.dtype)
+    _, rows = _rope_tables(name, cos, sin, D)
+    pos = input_pos
+    if pos is None:
+        if rows < T:
+            raise ValueError(f"{name}: rotation tables of {rows} rows for {T} tokens")
+    else:
+        if pos.dtype != torch.int64 or pos.shape not in ((T,), (B, T)):
+            raise ValueError(f"{name}: input_pos must be int64 [{T}] or [{B}, {T}]; got {tuple(pos.shape)} {pos.dtype}")
+        pos = pos.detach().expand(B, T)
+    _one_device(name, qkv, q_weight, k_weight, cos, sin, pos)
+    weights = [] if q_weight is None else [q_weight, k_weight]
+    if _differentiated(qkv, *weights):
+        return QkvNormRopeFunction.apply(qkv, q_weight, k_weight, cos, sin, pos, n_head, n_query_groups, float(eps))
+    return _qkv_norm_rope_fwd(x, _aligned(q_weight), _aligned(k_weight), cos, sin, pos, n_query_groups, R, D, float(eps))
+
+
+class KVCachePaged(NamedTuple):
+    """A key / value cache in pages: ``k`` / ``v`` ``[P, G, S, D]`` (pages of ``S`` positions, ``S`` a multiple of
+    16) and ``table`` int32 ``[B, N]``, whose entry ``[b, i]`` is the page of positions ``i S .. i S + S - 1`` of
+    sequence ``b``; a number outside ``0 .. P - 1`` (-1, say) is no page.  Sequences may read pages in common;
+    a page that a sequence appends to must be its own."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    table: torch.Tensor
+
+
+def kv_cache_paged(batch: int, groups: int, max_length: int, head_dim: int, page_size: int = 64, pages: int | None = None,
+                   dtype: torch.dtype = torch.bfloat16, device=None) -> KVCachePaged:
+    """A :class:`KVCachePaged` of zeros for ``max_length`` positions a sequence: every sequence with pages
+    of its own, or with ``pages`` that many in all and none given out yet (``table`` -1)."""
+    if page_size < 16 or page_size % 16 != 0:
+        raise NotImplementedError(f"kv_cache_paged: pages of a multiple of 16 positions, got {page_size}")
+    n = (max_length + page_size - 1) // page_size
+    if pages is None:
+        table = torch.arange(batch * n, dtype=torch.int32, device=device).view(batch, n)
+    else:
+        table = torch.full((batch, n), -1, dtype=torch.int32, device=device)
+
+    def make():
+        return torch.zeros(batch * n if pages is None else pages, groups, page_size, head_dim, dtype=dtype, device=device)
+
+    return KVCachePaged(make(), make(), table)
+
+
+def _check_paged(name: str, cache: KVCachePaged) -> tuple[int, int, int, int]:
+    """``(B, G, D, positions of a sequence)`` of a paged cache the kernels can index."""
+    k, v, table = cache
+    if k.dim() != 4 or v.shape != k.shape or min(k.shape) < 1:
+        raise ValueError(f"{name}: pages must be [P, G, S, D]; got {tuple(k.shape)}, {tuple(v.shape)}")
+    P, G, S, D = k.shape
+    if S % 16 != 0:
+        raise NotImplementedError(f"{name}: pages of a multiple of 16 positions, got {S}")
+    if v.dtype != k.dtype or not (k.is_contiguous() and v.is_contiguous()):
+        raise ValueError(f"{name}: pages must be contiguous, of one dtype")
+    if table.dim() != 2 or table.dtype != torch.int32 or table.shape[1] < 1 or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError(f"{name}: the page table must be int32 [B, N] with contiguous rows; got {tuple(table.shape)} "
+                         f"{table.dtype}")
+    if k.data_ptr() % 16 != 0 or v.data_ptr() % 16 != 0:
+        raise ValueError(f"{name}: pages must be 16-byte aligned")
+    return table.shape[0], G, D, S * table.shape[1]
+
+
+def _token_lengths(name: str, lengths: torch.Tensor | None, B: int) -> torch.Tensor | None:
+    if lengths is None:
+        return None
+    if lengths.shape != (B,) or lengths.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{name}: lengths must be {B} int32 / int64 lengths; got {tuple(lengths.shape)} {lengths.dtype}")
+    return lengths.detach().to(torch.int64).contiguous()
+
+
+def _table_stride(table: torch.Tensor) -> int:
+    return table.stride(0) if table.shape[0] > 1 else table.shape[1]
+
+
+@torch.compiler.disable
+def kv_cache_paged_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, input_pos: torch.Tensor,
+                          cache: KVCachePaged, n_head: int, q_weight: torch.Tensor | None = None,
+                          k_weight: torch.Tensor | None = None, eps: float = 1e-5,
+                          lengths: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`qkv_norm_rope` of the next tokens of every sequence with keys and values stored to their
+    pages; returns ``q`` ``[B, T, n_head, D]``.
+
+    ``qkv`` ``[B, T, (n_head + 2 G) D]`` in the cache's dtype (``G`` and ``D`` the cache's), ``input_pos`` device int64,
+    the position of each sequence's first token (one for all, or ``[B]``; the others follow it),
+    ``lengths`` (int32 / int64 ``[B]`` on the device): tokens of each sequence that are there, the rest
+    being padding.  ``cos`` / ``sin`` and the weights as in :func:`qkv_norm_rope`.  A token that is not
+    there, or whose position lies outside the tables or the page table, gives zeros and is not
+    stored; nor is one whose position has no page (its ``q`` is given).  Everything else in the
+    pages stays as it is.  Inference only."""
+    name = "kv_cache_paged_append"
+    B, G, D, _ = _check_paged(name, cache)
+    x, b, T, R, d = _qkv_rows(name, qkv, n_head, G)
+    if b != B or d != D or qkv.dtype != cache.k.dtype:
+        raise ValueError(f"{name}: qkv {tuple(qkv.shape)} {qkv.dtype}, cache and n_head do not agree")
+    _head_weights(name, q_weight, k_weight, D, qkv.dtype)
+    pairs, rows = _rope_tables(name, cos, sin, D)
+    if input_pos is None:
+        raise ValueError(f"{name}: input_pos is needed")
+    n = _token_lengths(name, lengths, B)
+    _one_device(name, qkv, q_weight, k_weight, cos, sin, n, *cache)
+    pos, pos_stride = _positions(name, "input_pos", input_pos, B, qkv.device)
+    x, wq, wk = x.detach(), _aligned(q_weight), _aligned(k_weight)
+    q = torch.empty((B, T, n_head, D), dtype=x.dtype, device=x.device)
+    P, _, S, _ = cache.k.shape
+    with _on_device(x.device):
+        st = nat.load().gdn2_kv_cache_paged_append(
+            x.data_ptr(), x.stride(0), x.stride(1), nat.dtype_code(x.dtype), nat.ptr(wq), nat.ptr(wk),
+            nat.dtype_code(x.dtype if wq is None else wq.dtype), float(eps), cos.data_ptr(), sin.data_ptr(), pairs, rows,
+            pos.data_ptr(), pos_stride, nat.ptr(n), q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), P, S,
+            cache.table.data_ptr(), _table_stride(cache.table), cache.table.shape[1], B, T, G, R, D,
+            nat.stream_handle(x.device))
+    nat.check(st, name)
+    return q
+
+
+def attention_paged_supported(q: torch.Tensor, head_dim: int) -> bool:
+    """Whether :func:`attention_paged` takes this dtype and head size."""
+    return q.is_cuda and q.dtype in (torch.bfloat16, torch.float16) and head_dim in (64, 128)
+
+
+@torch.compiler.disable
+def attention_paged(q: torch.Tensor, cache: KVCachePaged, input_pos: torch.Tensor, lengths: torch.Tensor | None = None,
+                    scale: float | None = None) -> torch.Tensor:
+    """Softmax attention of the last tokens of every sequence over its pages, their own positions
+    included (:func:`kv_cache_paged_append` stores them first): from the single-token path of reference
+    ``CausalSelfAttention.forward`` (``gdn2_gpt/model.py:89-173``) to pieces of long prompts.
+
+    ``q`` ``[B, T, H, D]`` in the cache's dtype (bf16 or fp16, ``D`` 64 or 128, ``H`` a multiple of the cache's
+    ``G``; strides as :func:`attention`), ``input_pos`` and ``lengths`` as in :func:`kv_cache_paged_append`.
+    Token ``t`` of sequence ``b`` sees positions ``0 .. input_pos[b] + t`` that have a page; a token that is not
+    there, lies outside the page table or sees nothing gives zeros.  What lies in a page past a
+    sequence's last token is not read; keys and values hidden from some of a piece's tokens only
+    must be finite.  ``scale`` is ``D**-0.5`` unless given (> 0).  Returns ``[B, T, H, D]``.  Scores and
+    sums are float32, probabilities are multiplied in two parts of the io dtype.  Inference only."""
+    name = "attention_paged"
+    B, G, D, cap = _check_paged(name, cache)
+    if q.dim() != 4 or q.shape[0] != B or q.shape[3] != D or q.shape[2] < 1 or q.shape[2] % G != 0:
+        raise ValueError(f"{name}: q must be [{B}, T, H, {D}] with H a multiple of {G}; got {tuple(q.shape)}")
+    if q.dtype != cache.k.dtype:
+        raise ValueError(f"{name}: q is {q.dtype}, the cache {cache.k.dtype}")
+    if q.dtype not in (torch.bfloat16, torch.float16) or D not in (64, 128):
+        raise NotImplementedError(f"{name}: bfloat16 / float16 heads of 64 or 128 channels; got {q.dtype}, {D}")
+    scale = float(D) ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale <= 1e30:
+        raise NotImplementedError(f"{name}: scale must be positive and at most 1e30, got {scale}")
+    if input_pos is None:
+        raise ValueError(f"{name}: input_pos is needed")
+    n = _token_lengths(name, lengths, B)
+    _one_device(name, q, n, *cache)
+    dev = q.device
+    pos, pos_stride = _positions(name, "input_pos", input_pos, B, dev)
+    q = _head_rows(q.detach())
+    _, T, H, _ = q.shape
+    P, _, S, _ = cache.k.shape
+    out = torch.empty((B, T, H, D), dtype=q.dtype, device=dev)
+    strides = _I64x3(*q.stride()[:3])
+    lib = nat.load()
+    nbytes = lib.gdn2_attn_paged_workspace_size(B, T, G, H // G, D, cap)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    with _on_device(dev):
+        st = lib.gdn2_attn_paged(
+            q.data_ptr(), ctypes.addressof(strides), nat.dtype_code(q.dtype), cache.k.data_ptr(), cache.v.data_ptr(), P, S,
+            cache.table.data_ptr(), _table_stride(cache.table), cache.table.shape[1], pos.data_ptr(), pos_stride,
+            nat.ptr(n), out.data_ptr(), B, T, G, H // G, D, scale, nat.ptr(ws), nbytes, nat.stream_handle(dev))
+    nat.check(st, name)
+    return out
+
+
 class TokenLogprobs(NamedTuple):
     """What :func:`token_logprobs` returns; the last two are None without ``top_k``."""
 
@@ -1963,6 +2277,81 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0,
     if _differentiated(logits):
         return TokenLogprobs(*TokenLogprobsFunction.apply(*args))
     return TokenLogprobs(*_token_logprobs_fwd(*args, False)[:4])
+
+
+def _sample_setting(name: str, what: str, value, shape, dtype: torch.dtype, device) -> tuple[torch.Tensor | None, float]:
+    """A setting as ``(tensor of each row's, 0)`` or ``(None, number for all)``."""
+    if not isinstance(value, torch.Tensor):
+        return None, value
+    if value.shape != shape or value.is_complex() or (dtype == torch.int32 and value.is_floating_point()):
+        raise ValueError(f"{name}: {what} must be a number, or one for each row {tuple(shape)}; got {tuple(value.shape)} "
+                         f"{value.dtype}")
+    _require_gpu(name, value)
+    if value.device != device:
+        raise ValueError(f"{name}: tensors on {device} and {value.device}")
+    if dtype == torch.int32 and value.dtype == torch.int64:
+        value = value.clamp(0, 2**31 - 1)
+    return value.detach().to(dtype).contiguous(), 0
+
+
+@torch.compiler.disable
+def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature: float | torch.Tensor = 1.0,
+                  top_k: int | torch.Tensor = 0, top_p: float | torch.Tensor = 1.0,
+                  min_p: float | torch.Tensor = 0.0) -> torch.Tensor:
+    """A token of each row of logits, drawn with the row's random number of ``[0, 1)`` (the answering step
+    that follows reference ``GPT.forward``, ``gdn2_gpt/model.py:304-380``, beside :func:`argmax_rows`).
+
+    ``logits`` ``[..., V]`` (bf16, fp16 or float32; ``V`` up to 2^20; strides as :func:`token_logprobs`), ``uniforms``
+    float32 ``[...]``; settings are numbers for all rows or tensors ``[...]`` on the device with one for
+    each.  Returns int64 ``[...]``.
+
+    With weights ``w_j = exp((x_j - max x) / temperature)``, those are kept that are at least ``min_p``, of
+    these the ``top_k`` largest (equal logits: the lower index first; 0: all), of these, in that
+    order, the shortest run whose sum reaches ``top_p`` of their sum (1: all).  The token is the lowest
+    index whose running sum of kept weights exceeds ``uniforms`` times their total.  ``temperature``
+    0 takes the largest logit, as :func:`argmax_rows` does; so does every row whose largest logit is
+    NaN (above all) or infinite.  Settings on the device are not checked: one outside its range counts
+    as the range's end (``top_p`` from 0 down: one token), a NaN as the filter left out
+    (``temperature``: as 0).  Settings count in float32.
+
+    Weights are formed in float64 and summed as whole numbers of 2^-42, so that a token does not depend on
+    how a row is divided; weights under 2^-43 are never drawn.  May be captured into a HIP graph."""
+    name = "sample_tokens"
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"{name}: logits must be [..., V] with V >= 1; got {tuple(logits.shape)}")
+    V, shape = logits.shape[-1], logits.shape[:-1]
+    if V > 1 << 20:
+        raise NotImplementedError(f"{name}: at most 2^20 tokens, got {V}")
+    nat.dtype_code(logits.dtype)
+    if uniforms.shape != shape or uniforms.dtype != torch.float32:
+        raise ValueError(f"{name}: uniforms must be float32 {tuple(shape)}; got {tuple(uniforms.shape)} {uniforms.dtype}")
+    if not isinstance(temperature, torch.Tensor) and not 0.0 <= temperature <= 3e38:
+        raise ValueError(f"{name}: temperature must not be negative, got {temperature}")
+    if not isinstance(top_k, torch.Tensor) and (top_k != int(top_k) or top_k < 0):
+        raise ValueError(f"{name}: top_k must be a whole number from 0 on, got {top_k}")
+    if not isinstance(top_p, torch.Tensor) and not 0.0 < top_p <= 1.0:
+        raise ValueError(f"{name}: top_p must be within (0, 1], got {top_p}")
+    if not isinstance(min_p, torch.Tensor) and not 0.0 <= min_p <= 1.0:
+        raise ValueError(f"{name}: min_p must be within [0, 1], got {min_p}")
+    _one_device(name, logits, uniforms)
+    dev = logits.device
+    t, t_all = _sample_setting(name, "temperature", temperature, shape, torch.float32, dev)
+    k, k_all = _sample_setting(name, "top_k", top_k, shape, torch.int32, dev)
+    p, p_all = _sample_setting(name, "top_p", top_p, shape, torch.float32, dev)
+    m, m_all = _sample_setting(name, "min_p", min_p, shape, torch.float32, dev)
+    x, inner, so, sr, rows = _logit_rows(logits.detach())
+    u = uniforms.detach().contiguous()
+    out = torch.empty(shape, dtype=torch.int64, device=dev)
+    lib = nat.load()
+    nbytes = lib.gdn2_sample_tokens_workspace_size(rows, V)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    with _on_device(dev):
+        st = lib.gdn2_sample_tokens(
+            x.data_ptr(), inner, so, sr, nat.dtype_code(x.dtype), rows, V, u.data_ptr(), nat.ptr(t), float(t_all),
+            nat.ptr(k), min(int(k_all), V), nat.ptr(p), float(p_all), nat.ptr(m), float(m_all), out.data_ptr(),
+            nat.ptr(ws), nbytes, nat.stream_handle(dev))
+    nat.check(st, name)
+    return out
 
 
 def _rows2d(name: str, x: torch.Tensor, dt: torch.dtype, width: int) -> int:
