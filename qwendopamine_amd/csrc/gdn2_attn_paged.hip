@@ -18,6 +18,7 @@
 #include "gdn2_common.h"
 #include "gdn2_internal.h"
 #include "gdn2_mfma.h"
+#include "gdn2_attn_tiles.h"
 
 namespace gdn2 {
 namespace {
@@ -26,17 +27,8 @@ constexpr int kWaves = 4;
 constexpr int kStep = 32;               // positions of a wave's step: two tiles of 16
 constexpr int kRound = kStep * kWaves;  // positions that a workgroup's waves take at a time
 constexpr int kMaxSplits = 256;
-constexpr float kNoMax = -3.0e38f;  // no key yet: below every score, and differences stay finite
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr unsigned kNoPage = 0xffffffffu;
-
-// The reference of the exponents lies `down` under the running maximum and moves when
-// a score exceeds that maximum by `lazy`: fp16 probabilities are held in 2^13 ..
-// 2^15, where 2^-27 of the largest still has 11 bits (bf16 has fp32's exponents).
-template <PrecKind PK>
-struct Ref {
-    static constexpr float down = PK == PrecKind::F16 ? 13.0f : 0.0f, lazy = PK == PrecKind::F16 ? 2.0f : 8.0f;
-};
+constexpr int kTileRows = 32 * kWaves;  // rows of a workgroup whose keys lie in LDS
 
 template <PrecKind PK>
 __device__ __forceinline__ f32x4 mma16(f32x4 acc, uint4 a, uint4 b)
@@ -469,6 +461,298 @@ __global__ __launch_bounds__(256) void attn_paged_join_kernel(AttnPagedParams p)
     io<T>::st(static_cast<T *>(p.out), row * D + d, den == 0.0f ? 0.0f : num / den);
 }
 
+// ---- many rows: tiles of 64 positions in LDS, which 128 rows read ----
+
+// A lane's place among the 16 rows of a page's piece, for the request that it makes of them (rows as
+// they lie, their 16-byte pieces permuted as the tile's: swz).
+template <int D>
+struct Place {
+    int row;            // of the piece
+    unsigned piece16;   // byte within the row
+    int sub;            // the request's piece of the tile, it adds kPer * it
+    static constexpr int kP = D / 8, kR = 64 / kP, kIt = kTile / kR / kWaves;  // pieces, rows, requests of a wave
+    static constexpr int kPer = kWaves * kR / 16;
+    __device__ __forceinline__ Place(int wave, int lane)
+    {
+        const int r = wave * kR + lane / kP;
+        row = r & 15;
+        sub = r >> 4;
+        piece16 = ((lane % kP) ^ swz<D>(r)) * 16;
+    }
+};
+
+// Positions row0 .. row0 + 63 requested into LDS: piece a of 16 from the row of the cache that lane
+// i0 + a of `rows` holds.  Positions past the last, n - 1, repeat it; a piece without a page is zeros.
+template <int D>
+__device__ __forceinline__ void stage_pages(const char *pool, unsigned rows, int i0, int row0, int n, bool plain, char *lds,
+                                            const Place<D> &at, int wave, int lane)
+{
+#ifdef __HIP_DEVICE_COMPILE__  // the host's pass does not know the builtins' types
+    constexpr int IT = Place<D>::kIt, PER = Place<D>::kPer;
+    typedef __attribute__((address_space(3))) char *lds_ptr;
+    const int wsub = __builtin_amdgcn_readfirstlane(at.sub);
+    auto load = [&](unsigned row, char *to, unsigned off) __attribute__((always_inline)) {
+        // Raw buffer from this row on, 32-bit elements.
+        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<char *>(pool + static_cast<uint64_t>(row) * (2 * D)), 0, 16 * 2 * D, 0x00020000);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr)to, 16, off, 0, 0, 0);
+    };
+#pragma unroll
+    for (int it = 0; it < IT; ++it) {
+        char *const to = lds + (it * kWaves + wave) * 1024;
+        const int sub = wsub + PER * it;
+        if (plain) {
+            load(static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(rows), i0 + sub)), to,
+                 at.row * (2 * D) + at.piece16);
+        } else {
+            const int last = n - 1 - row0, subc = sub < (last >> 4) ? sub : last >> 4;
+            const unsigned row = static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(rows), i0 + subc));
+            const int r = 16 * sub + at.row < last ? 16 * sub + at.row : last;
+            if (row == kNoPage)
+                *reinterpret_cast<uint4 *>(to + lane * 16) = make_uint4(0, 0, 0, 0);
+            else
+                load(row, to, (r - 16 * subc) * (2 * D) + at.piece16);
+        }
+    }
+#endif
+}
+
+// The products, statistics and layouts of the forward over whole sequences (gdn2_attn_train.hip), keys
+// and values by pages: a wave looks the pages of 16 tiles up at once.  Probabilities are rounded once
+// for their product, as there: off by 1.4 to 1.5 times the rounding of the result.
+template <PrecKind PK, int D>
+__global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void attn_paged_tiles_kernel(AttnPagedParams p)
+{
+    constexpr int KS = D / 16, DT = D / 32, BM = kTileRows;
+    constexpr int kBytes = kTile * D * 2, kAhead = 16;  // tiles whose pages are looked up at once
+    // Arrays of their own, so that reads of one and requests into another are known not to meet.
+    __shared__ __align__(256) char sk0[kBytes], sk1[kBytes], sv0[kBytes], sv1[kBytes];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 31, h = lane >> 5;
+    const int rb = row_base<D>(lane), cb = col_base<D>(lane);
+    const int k = blockIdx.x >> 3, bg = k / p.tiles * 8 + (blockIdx.x & 7);  // a group's tiles on one XCD
+    if (bg >= p.B * p.G) return;
+    const Where w = where(p, BM, bg, p.tiles - 1 - k % p.tiles);  // the longest first
+    const int all = p.T * p.R, end = w.t1 * p.R;  // rows, and those that are there
+    const int per = p.splits > 1 ? share_of(p, lane) : (w.n + kRound - 1) / kRound * kRound;
+    const int lo = static_cast<int>(blockIdx.y) * per, hi = lo + per < w.n ? lo + per : w.n;
+    uint16_t *out = static_cast<uint16_t *>(p.out);
+    if (lo >= hi) {
+        if (p.splits == 1)
+            for (int e = tid; e < BM * (D / 8); e += 64 * kWaves) {
+                const int x = w.m0 + e / (D / 8);
+                if (x < all) *reinterpret_cast<uint4 *>(out + out_row(p, w, x) * D + e % (D / 8) * 8) = make_uint4(0, 0, 0, 0);
+            }
+        return;
+    }
+    const int x = w.m0 + 32 * wave + n, xc = x < end ? x : end - 1;  // this lane's row
+    const int t_of = xc / p.R;
+    const uint16_t *qr = static_cast<const uint16_t *>(p.q) + w.b * p.qs[0] + t_of * p.qs[1] +
+                         (w.g * p.R + (xc - t_of * p.R)) * p.qs[2];
+    uint4 qf[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const uint4 *>(qr + 16 * s + 8 * h);
+    // Keys that this lane sees, all of the wave see, none of the wave sees more than, all of the workgroup see.
+    const int lim = w.pos + t_of + 1;
+    const int wfirst = w.m0 + 32 * wave < end ? w.m0 + 32 * wave : end - 1;
+    const int wlast = wfirst + 31 < end ? wfirst + 31 : end - 1;
+    const int wlim = w.pos + wfirst / p.R + 1, wend = w.pos + wlast / p.R + 1, glim = w.pos + w.t0 + 1;
+    const float c = p.scale * kLog2e;
+
+    const int first = lo / kTile, nt = (hi + kTile - 1) / kTile;
+    const int *table = p.table + w.b * p.table_stride;
+    auto look_up = [&](int tile) __attribute__((always_inline)) {
+        const int j = tile * kTile + lane * 16;
+        unsigned r = kNoPage;
+        if (j < hi) {
+            const int col = j / p.page;
+            const int64_t pg = table[col];
+            if (pg >= 0 && pg < p.pages) r = static_cast<unsigned>((pg * p.G + w.g) * p.page + (j - col * p.page));
+        }
+        return r;
+    };
+    // A bit for each piece of 16 positions that has none.
+    auto missing = [&](unsigned rows, int tile) __attribute__((always_inline)) {
+        return __ballot(rows == kNoPage && tile * kTile + lane * 16 < hi);
+    };
+    unsigned rows = look_up(first), next = look_up(first + kAhead);
+    uint64_t lost = missing(rows, first);
+    const Place<D> at(wave, lane);
+    const char *kp = static_cast<const char *>(p.k), *vp = static_cast<const char *>(p.v);
+    auto stage = [&](int t, char *tk, char *tv) __attribute__((always_inline)) {
+        const int i0 = (t - first) % kAhead * 4;
+        const bool plain = (t + 1) * kTile <= hi && ((lost >> i0) & 15) == 0;
+        stage_pages<D>(kp, rows, i0, t * kTile, hi, plain, tk, at, wave, lane);
+        stage_pages<D>(vp, rows, i0, t * kTile, hi, plain, tv, at, wave, lane);
+    };
+
+    float m = 0.0f, l = 0.0f;
+    bool fresh = true;  // no visible key yet
+    f32x16 acc[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d) acc[d] = zero16();
+    stage(first, sk0, sv0);
+    auto step = [&](int t, int gone, auto buf, auto hidden) __attribute__((always_inline)) {
+        constexpr bool kOdd = decltype(buf)::value, kHide = decltype(hidden)::value;
+        const char *const tk = kOdd ? sk1 : sk0, *const tv = kOdd ? sv1 : sv0;
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();  // tile t has landed, and every wave is done with tile t - 1
+        if (t + 1 < nt) {
+            if (kOdd && (t + 1 - first) % kAhead == 0) {
+                rows = next;
+                lost = missing(rows, t + 1);
+                next = look_up(t + 1 + kAhead);
+            }
+            stage(t + 1, kOdd ? sk0 : sk1, kOdd ? sv0 : sv1);
+        }
+        const int j0 = t * kTile;
+        if (kHide && j0 >= wend) return;
+        const int kr = opaque(rb), vc = opaque(cb);
+        if constexpr (D == 128) mix_reads();
+        f32x16 s[2];
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+            s[a] = zero16();
+#pragma unroll
+            for (int st = 0; st < KS; ++st) s[a] = mma32<PK>(s[a], row_frag<D>(tk, kr, 32 * a, st), qf[st]);
+        }
+        if (kHide && j0 + kTile > wlim) {
+            hide<true>(s[0], j0, h, lim);
+            hide<true>(s[1], j0 + 32, h, lim);
+        }
+        if (kHide && gone) {
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[a][i] = (gone >> (2 * a + (i >> 3))) & 1 ? -INFINITY : s[a][i];
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[a][i] = fmaf(s[a][i], c, -m);
+                mx[i & 3] = fmaxf(mx[i & 3], s[a][i]);
+            }
+        const float top = half_max(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+        constexpr float kDown = Ref<PK>::down;
+        if (__any(top > (fresh ? -INFINITY : kDown + Ref<PK>::lazy))) {
+            // The first visible key sets the reference, later ones raise it.
+            const bool set = fresh && top > -INFINITY;
+            const float d = set ? top - kDown : fmaxf(top - kDown, 0.0f);
+            const float r = fresh ? 1.0f : __builtin_amdgcn_exp2f(-d);  // nothing to rescale yet
+            m += d;
+            fresh = fresh && !set;
+            l *= r;
+#pragma unroll
+            for (int e = 0; e < DT; ++e)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[e][i] *= r;
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[a][i] -= d;
+        }
+        float sum = 0.0f;
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[a][i] = __builtin_amdgcn_exp2f(s[a][i]);
+                sum += s[a][i];
+            }
+        l += sum;
+#pragma unroll
+        for (int a = 0; a < 2; ++a) add_columns<PK, D, false>(acc, tv, vc, 32 * a, s[a]);
+    };
+    for (int t = first; t < nt; t += 2) {
+        // (lost belongs to this pair's tiles: both lie among the 16 that were looked up last.)
+        const int gone = static_cast<int>(lost >> ((t - first) % kAhead * 4)) & 255;
+        if ((t + 2) * kTile <= glim && t + 2 <= nt && gone == 0) {
+            step(t, 0, std::false_type{}, std::false_type{});
+            step(t + 1, 0, std::true_type{}, std::false_type{});
+        } else {
+            step(t, gone & 15, std::false_type{}, std::true_type{});
+            if (t + 1 < nt) step(t + 1, gone >> 4, std::true_type{}, std::true_type{});
+        }
+    }
+    l = half_add(l);
+    m = fresh ? kNoMax : m;
+    if (p.splits > 1) {
+        if (x >= end) return;
+        // This share's state; attn_paged_join_tiles_kernel puts the shares together.
+        const int64_t rows_all = static_cast<int64_t>(p.B) * p.T * (p.G * p.R);
+        const int64_t to = blockIdx.y * rows_all + out_row(p, w, x);
+        if (h == 0) *reinterpret_cast<float2 *>(p.part + p.splits * rows_all * D + 2 * to) = make_float2(m, l);
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<float4 *>(p.part + to * D + 32 * d + 8 * i + 4 * h) =
+                    make_float4(acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]);
+        return;
+    }
+    const bool none = l == 0.0f || x >= end;  // padding, or no key with a page
+    const float inv = 1.0f / l;
+    __syncthreads();  // the tiles are done with
+    char *const so = wave == 0 ? sk0 : wave == 1 ? sk1 : wave == 2 ? sv0 : sv1;
+    put_rows<D>(so, lane, acc, [&](float a, float b, float cc, float d) __attribute__((always_inline)) {
+        return none ? pack4<PK>(0.0f, 0.0f, 0.0f, 0.0f) : pack4<PK>(a * inv, b * inv, cc * inv, d * inv);
+    });
+    write_rows<D>(so, lane, out, [&](int r) __attribute__((always_inline)) {
+        const int xr = w.m0 + 32 * wave + r;
+        return xr < all ? out_row(p, w, xr) * D : int64_t{-1};
+    });
+}
+
+// The shares of a row in their order; thread: 4 channels of a row.
+template <PrecKind PK, int D>
+__global__ __launch_bounds__(256) void attn_paged_join_tiles_kernel(AttnPagedParams p)
+{
+    const int H = p.G * p.R;
+    const int64_t rows = static_cast<int64_t>(p.B) * p.T * H;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * (1024 / D) + threadIdx.x / (D / 4);
+    const int per = share_of(p, threadIdx.x & 63);
+    if (row >= rows) return;
+    const int ch = threadIdx.x % (D / 4) * 4;
+    const unsigned bt = static_cast<unsigned>(row / H), hh = static_cast<unsigned>(row - static_cast<int64_t>(bt) * H);
+    const unsigned b = bt / p.T, t = bt - b * p.T, g = hh / p.R;
+    const Where w = where(p, kTileRows, static_cast<int>(b * p.G + g), static_cast<int>((t * p.R + (hh - g * p.R)) / kTileRows));
+    const int used = static_cast<int>(t) < w.t1 ? (w.n + per - 1) / per : 0;
+    const float2 *ml = reinterpret_cast<const float2 *>(p.part + p.splits * rows * D);
+    float m = kNoMax;
+    for (int s = 0; s < used; ++s) m = fmaxf(m, ml[s * rows + row].x);
+    float l = 0.0f;
+    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int s = 0; s < used; ++s) {
+        const float2 st = ml[s * rows + row];
+        const float4 y = *reinterpret_cast<const float4 *>(p.part + (s * rows + row) * D + ch);
+        const float r = __builtin_amdgcn_exp2f(st.x - m);
+        l = fmaf(st.y, r, l);
+        x.x = fmaf(y.x, r, x.x);
+        x.y = fmaf(y.y, r, x.y);
+        x.z = fmaf(y.z, r, x.z);
+        x.w = fmaf(y.w, r, x.w);
+    }
+    const float inv = 1.0f / l;
+    const Q4<PK> y = l == 0.0f ? pack4<PK>(0.0f, 0.0f, 0.0f, 0.0f) : pack4<PK>(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+    st_q4<PK>(static_cast<uint16_t *>(p.out) + row * D + ch, y);
+}
+
+template <PrecKind PK, int D>
+hipError_t paged_tiles(AttnPagedParams &p, hipStream_t s)
+{
+    const unsigned x = static_cast<unsigned>((p.B * p.G + 7) / 8) * 8u * p.tiles;
+    hipLaunchKernelGGL((attn_paged_tiles_kernel<PK, D>), dim3(x, p.splits), dim3(64 * kWaves), 0, s, p);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || p.splits == 1) return e;
+    const int64_t rows = static_cast<int64_t>(p.B) * p.T * p.G * p.R;
+    hipLaunchKernelGGL((attn_paged_join_tiles_kernel<PK, D>), dim3(static_cast<unsigned>((rows + 1024 / D - 1) / (1024 / D))),
+                       dim3(256), 0, s, p);
+    return hipGetLastError();
+}
+
 template <typename T, PrecKind PK, int D, int C>
 hipError_t paged_c(AttnPagedParams &p, hipStream_t s)
 {
@@ -487,14 +771,15 @@ hipError_t paged_d(AttnPagedParams &p, hipStream_t s)
     switch (p.rows) {
     case 16: return paged_c<T, PK, D, 1>(p, s);
     case 32: return paged_c<T, PK, D, 2>(p, s);
-    default: return paged_c<T, PK, D, 4>(p, s);
+    case 64: return paged_c<T, PK, D, 4>(p, s);
+    default: return paged_tiles<PK, D>(p, s);
     }
 }
 
 }  // namespace
 
 // Rows of a workgroup: 16 columns for each matrix product, more where a group has more rows.
-int attn_paged_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+int attn_paged_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : kTileRows; }
 
 // Shares of the keys: enough workgroups for two on every CU, no share under 512 positions.
 int attn_paged_splits(int B, int G, int64_t rows, int64_t cap)
