@@ -667,8 +667,7 @@ int gdn2_kv_cache_paged_append(const void *qkv, int64_t stride_b, int64_t stride
 size_t gdn2_attn_paged_workspace_size(int B, int64_t T, int G, int R, int D, int64_t positions)
 {
     if (B < 1 || T < 1 || G < 1 || R < 1 || D < 1 || positions < 1) return 0;
-    const int s = attn_paged_splits(B, G, T * R, positions);
-    return s == 1 ? 0 : static_cast<size_t>(B) * T * G * R * s * (D + 2) * sizeof(float);
+    return attn_paged_plan(B, T, G, R, D, positions).floats * sizeof(float);
 }
 
 int gdn2_attn_paged(const void *q, const int64_t *strides, int io_dtype, const void *k_pages, const void *v_pages,
@@ -690,19 +689,18 @@ int gdn2_attn_paged(const void *q, const int64_t *strides, int io_dtype, const v
     }
     // Rows of a group in 31 bits, and what is launched within HIP's limits.
     if (static_cast<double>(T) * R > 1073741824.0 || static_cast<double>(B) * G * R * T > static_cast<double>(max_workgroups(256)) ||
-        static_cast<int64_t>(B) * G > 65535 * 16)
+        G > 65535)
         return GDN2_ERR_UNSUPPORTED;
     p.q = q; p.k = k_pages; p.v = v_pages;
     p.table = table; p.table_stride = table_stride; p.pages = pages; p.page = page_size;
     p.cap = page_size * table_cols;
     p.pos = pos; p.pos_stride = pos_stride; p.lengths = lengths;
     p.out = out; p.B = B; p.T = static_cast<int>(T); p.G = G; p.R = R; p.D = D; p.scale = scale;
-    p.rows = attn_paged_rows(T * R);
-    p.tiles = static_cast<int>((T * R + p.rows - 1) / p.rows);
-    p.splits = attn_paged_splits(B, G, T * R, p.cap);
+    const AttnPagedPlan plan = attn_paged_plan(B, T, G, R, D, p.cap);
+    p.rows = plan.rows; p.tiles = plan.tiles; p.splits = plan.splits; p.workers = plan.workers;
     p.part = static_cast<float *>(workspace);
-    if (p.splits > 1 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) ||
-                         workspace_bytes < gdn2_attn_paged_workspace_size(B, T, G, R, D, p.cap)))
+    if (plan.floats > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) ||
+                            workspace_bytes < plan.floats * sizeof(float)))
         return GDN2_ERR_WORKSPACE;
     return launch_attn_paged(p, io_dtype, static_cast<hipStream_t>(stream)) == hipSuccess ? GDN2_OK : GDN2_ERR_LAUNCH;
 }

@@ -128,6 +128,56 @@ __device__ __forceinline__ int share_of(const AttnPagedParams &p, int lane)
     return (rounds + p.splits - 1) / p.splits * kRound;
 }
 
+// Rounds of sequence b, for a group of few rows (one workgroup holds them all).
+__device__ __forceinline__ int rounds_of(const AttnPagedParams &p, int b)
+{
+    int pos;
+    const int t = tokens_of(p, b, pos);
+    return t > 0 ? (pos + t + kRound - 1) / kRound : 0;
+}
+
+// The sequences' rounds in a row, dealt to p.workers workgroups in equal runs, which may begin and end
+// within a sequence (no run under kLeast): sequences of unequal lengths then keep all of them
+// busy to the end.  Worker w's part of sequence b is slot w + b, as both only grow along the row.
+constexpr int kLeast = 2;
+// By a wave: the rounds before sequence `upto`.
+__device__ __forceinline__ int rounds_before(const AttnPagedParams &p, int upto, int lane)
+{
+    int sum = 0;
+    for (int b = lane; b < upto; b += 64) sum += rounds_of(p, b);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
+    return sum;
+}
+__device__ __forceinline__ int run_of(const AttnPagedParams &p, int total)
+{
+    const int r = (total + p.workers - 1) / p.workers;
+    return r > kLeast ? r : kLeast;
+}
+// The sequence in which round `at` of all lies, and the rounds before it.
+__device__ __forceinline__ int sequence_at(const AttnPagedParams &p, int at, int lane, int &before)
+{
+    int base = 0;
+    for (int b0 = 0; b0 < p.B; b0 += 64) {
+        const int r = b0 + lane < p.B ? rounds_of(p, b0 + lane) : 0;
+        int in = r;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_up(in, o, 64);
+            in += lane >= o ? y : 0;
+        }
+        const uint64_t hit = __ballot(base + in > at);
+        if (hit) {
+            const int l = __ffsll(static_cast<unsigned long long>(hit)) - 1;
+            before = base + __builtin_amdgcn_readlane(in - r, l);
+            return b0 + l;
+        }
+        base += __builtin_amdgcn_readlane(in, 63);
+    }
+    before = base;  // not reached: `at` is less than all
+    return p.B - 1;
+}
+
 // A row's place in a [B, T, H, ...] tensor's rows.
 __device__ __forceinline__ int64_t out_row(const AttnPagedParams &p, const Where &w, int x)
 {
@@ -135,53 +185,62 @@ __device__ __forceinline__ int64_t out_row(const AttnPagedParams &p, const Where
     return (static_cast<int64_t>(w.b) * p.T + t) * (p.G * p.R) + w.g * p.R + (x - t * p.R);
 }
 
-// C column tiles.
-template <typename T, PrecKind PK, int D, int C>
-__global__ __launch_bounds__(64 * kWaves, C == 4 ? 1 : 2) void attn_paged_kernel(AttnPagedParams p)
+// C column tiles hold all the T R rows of a group.  SPREAD: workgroup (worker, group) takes its run of all
+// sequences' rounds, and attn_paged_join_kernel joins the parts; else workgroup (b, group) one sequence.
+template <typename T, PrecKind PK, int D, int C, bool SPREAD>
+__global__ __launch_bounds__(64 * kWaves, 2) void attn_paged_kernel(AttnPagedParams p)
 {
     constexpr int KS = D / 32, CH = D / 16, VW = CH / 2;  // contraction steps, channels and dwords of a lane's value row
     constexpr int kRows = 16 * C;
     __shared__ __align__(16) float s_o[kWaves][16][D];
     __shared__ float s_m[kWaves][C][16], s_l[kWaves][C][16];
+    __shared__ uint4 s_q[C * KS][64];  // the query operands: registers are for keys and values
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, kg = lane >> 4;
-    // A group's tiles of rows read the same keys: all on one XCD (workgroups go to the 8 in turn).
-    int bg = blockIdx.x, tile = 0;
-    if (p.tiles > 1) {
-        const int k = blockIdx.x >> 3;
-        bg = k / p.tiles * 8 + (blockIdx.x & 7);
-        tile = p.tiles - 1 - k % p.tiles;  // the longest first
-        if (bg >= p.B * p.G) return;
-    }
-    const Where w = where(p, kRows, bg, tile);
-    const int all = p.T * p.R;
+    const int g = blockIdx.y, all = p.T * p.R;
     T *out = static_cast<T *>(p.out);
-    const int per = p.splits > 1 ? share_of(p, lane) : (w.n + kRound - 1) / kRound * kRound;
-    const int lo = static_cast<int>(blockIdx.y) * per;
-    const int hi = lo + per < w.n ? lo + per : w.n;
+    int b = blockIdx.x, from = 0, left = 0;  // this part: from round `from` of sequence b, `left` rounds to go in all
+    if constexpr (SPREAD) {
+        const int total = rounds_before(p, p.B, lane), run = run_of(p, total);
+        const int64_t at = static_cast<int64_t>(blockIdx.x) * run;
+        if (at >= total) return;
+        int before;
+        b = __builtin_amdgcn_readfirstlane(sequence_at(p, static_cast<int>(at), lane, before));
+        from = __builtin_amdgcn_readfirstlane(static_cast<int>(at) - before);
+        left = __builtin_amdgcn_readfirstlane(total - at < run ? total - static_cast<int>(at) : run);
+    }
+    for (;;) {
+    Where w = where(p, kRows, b * p.G + g, 0);
+    // In scalar registers, although loaded after stores.
+    w.pos = __builtin_amdgcn_readfirstlane(w.pos);
+    w.t1 = __builtin_amdgcn_readfirstlane(w.t1);
+    w.n = __builtin_amdgcn_readfirstlane(w.n);
+    const int lo = from * kRound;
+    int hi = w.n;
+    if constexpr (SPREAD) hi = (from + left) * kRound < w.n ? (from + left) * kRound : w.n;
     if (lo >= hi) {
-        // Nothing here (the join does not read this share); no key at all: zeros.
-        if (p.splits == 1)
-            for (int e = tid; e < kRows * D; e += 64 * kWaves) {
-                const int x = w.m0 + e / D;
-                if (x < all) io<T>::st(out, out_row(p, w, x) * D + e % D, 0.0f);
-            }
+        if constexpr (SPREAD) {  // a sequence without keys: on to the next
+            ++b;
+            continue;
+        }
+        for (int e = tid; e < all * D; e += 64 * kWaves) io<T>::st(out, out_row(p, w, e / D) * D + e % D, 0.0f);
         return;
     }
 
     // ---- this lane's columns: query rows as B operands, and the keys they see ----
-    uint4 qf[C][KS];
     int lim[C];
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-        int x = w.m0 + 16 * c + n;
+        int x = 16 * c + n;
         const int end = w.t1 * p.R;
         x = x < end ? x : end - 1;  // rows past the end repeat the last one
         const int t = x / p.R;
         lim[c] = w.pos + t + 1;
-        const T *q = static_cast<const T *>(p.q) + w.b * p.qs[0] + t * p.qs[1] + (w.g * p.R + (x - t * p.R)) * p.qs[2];
+        if (c % kWaves == wave) {
+            const T *q = static_cast<const T *>(p.q) + w.b * p.qs[0] + t * p.qs[1] + (g * p.R + (x - t * p.R)) * p.qs[2];
 #pragma unroll
-        for (int s = 0; s < KS; ++s) qf[c][s] = *reinterpret_cast<const uint4 *>(q + 32 * s + 8 * kg);
+            for (int s = 0; s < KS; ++s) s_q[c * KS + s][lane] = *reinterpret_cast<const uint4 *>(q + 32 * s + 8 * kg);
+        }
     }
     const int seen = w.pos + w.t0 + 1;  // every row sees these
 
@@ -274,14 +333,18 @@ __global__ __launch_bounds__(64 * kWaves, C == 4 ? 1 : 2) void attn_paged_kernel
                 }
         }
         uint4 ph[C], pl[C];
+        const int at_q = opaque(lane);  // read anew at each step
 #pragma unroll
         for (int c = 0; c < C; ++c) {
+            uint4 qf[KS];
+#pragma unroll
+            for (int s = 0; s < KS; ++s) qf[s] = s_q[c * KS + s][at_q];
             f32x4 t[2];
 #pragma unroll
             for (int a = 0; a < 2; ++a) {
                 t[a] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int s = 0; s < KS; ++s) t[a] = mma16<PK>(t[a], st.k[a][s], qf[c][s]);
+                for (int s = 0; s < KS; ++s) t[a] = mma16<PK>(t[a], st.k[a][s], qf[s]);
             }
             float s[8];
 #pragma unroll
@@ -342,6 +405,7 @@ __global__ __launch_bounds__(64 * kWaves, C == 4 ? 1 : 2) void attn_paged_kernel
     // ---- the steps, the next one's keys and values in flight during each ----
     Step cur, alt;
     unsigned next = look_up(0);
+    if (steps == 0) __syncthreads();  // as the others below
     for (int base = 0; base < steps; base += 32) {
         const unsigned rows = next;
         if (base + 32 < steps) next = look_up(base + 32);
@@ -361,6 +425,7 @@ __global__ __launch_bounds__(64 * kWaves, C == 4 ? 1 : 2) void attn_paged_kernel
             step(st, j0, bad, row(2 * i + 1) == kNoPage && (bad || j0 + 16 < hi));
         };
         get(cur, 0);
+        if (base == 0) __syncthreads();  // the queries are there
         for (int i = 0; i < cnt; i += 2) {
             if (i + 1 < cnt) get(alt, i + 1);
             run(cur, i);
@@ -403,55 +468,73 @@ __global__ __launch_bounds__(64 * kWaves, C == 4 ? 1 : 2) void attn_paged_kernel
                 num = fmaf(s_o[v][h][d], r, num);
                 den = fmaf(s_l[v][c][h], r, den);
             }
-            const int64_t row = out_row(p, w, x);
-            if (p.splits == 1) {
-                // Padding, and rows whose every key is without a page: zeros.
-                io<T>::st(out, row * D + d, x < w.t1 * p.R && den != 0.0f ? num / den : 0.0f);
-            } else {
-                float *part = p.part + (row * p.splits + blockIdx.y) * (D + 2);
+            if constexpr (SPREAD) {
+                float *part = p.part + ((static_cast<int64_t>(blockIdx.x + b) * p.G + g) * all + x) * (D + 2);
                 part[d] = num;
                 if (d == 0) {
                     part[D] = mx;
                     part[D + 1] = den;
                 }
+            } else {
+                // Padding, and rows whose every key is without a page: zeros.
+                io<T>::st(out, out_row(p, w, x) * D + d, x < w.t1 * p.R && den != 0.0f ? num / den : 0.0f);
             }
         }
     }
+    if constexpr (!SPREAD) return;
+    left -= (hi - lo + kRound - 1) / kRound;
+    if (left <= 0) return;
+    ++b;
+    from = 0;
+    __syncthreads();  // the next part overwrites what was read
+    }
 }
 
-// The shares' states of one row: weights first (a thread each), then the values, 256 / D threads
-// per channel.
+// The parts of one row: weights first (a thread each), then the values, 256 / D threads per channel.
+constexpr int kMaxWorkers = 512;
 template <typename T, int D>
 __global__ __launch_bounds__(256) void attn_paged_join_kernel(AttnPagedParams p)
 {
-    constexpr int N = 256 / D;
-    __shared__ float s_w[kMaxSplits], s_red[4], s_den[4], s_num[N][D];
+    constexpr int N = 256 / D, kEach = kMaxWorkers / 256;
+    __shared__ float s_w[kMaxWorkers], s_red[4], s_den[4], s_num[N][D];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int H = p.G * p.R;
     const int64_t row = blockIdx.x;
-    const int h = static_cast<int>(row % H), t = static_cast<int>(row / H % p.T);
+    const int h = static_cast<int>(row % H), bt = static_cast<int>(row / H), b = bt / p.T, t = bt - b * p.T;
     const int g = h / p.R, x = t * p.R + (h - g * p.R);
-    const Where w = where(p, p.rows, static_cast<int>(row / H / p.T) * p.G + g, x / p.rows);
-    const int per = share_of(p, lane);
-    const int used = t < w.t1 ? (w.n + per - 1) / per : 0;
-    const float *part = p.part + row * p.splits * (D + 2);
-    const float mx = tid < used ? part[tid * (D + 2) + D] : kNoMax;
-    float den = tid < used ? part[tid * (D + 2) + D + 1] : 0.0f;
-    float m = mx;
+    int pos;
+    const int there = tokens_of(p, b, pos);
+    const int total = rounds_before(p, p.B, lane), before = rounds_before(p, b, lane), run = run_of(p, total);
+    const int first = before / run, last = (before + rounds_of(p, b) - 1) / run;  // workers
+    const int used = t < there ? last - first + 1 : 0;
+    const int64_t step = static_cast<int64_t>(p.G) * p.T * p.R * (D + 2);  // from one slot to the next
+    const float *part = p.part + (first + b) * step + (static_cast<int64_t>(g) * p.T * p.R + x) * (D + 2);
+    float mx[kEach], m = kNoMax, den = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        const int s = tid + 256 * i;
+        mx[i] = s < used ? part[s * step + D] : kNoMax;
+        m = fmaxf(m, mx[i]);
+    }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
     if (lane == 0) s_red[wave] = m;
     __syncthreads();
     m = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
-    const float r = __builtin_amdgcn_exp2f(mx - m);
-    s_w[tid] = r;
-    den = wave_sum(den * r);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        const int s = tid + 256 * i;
+        const float r = __builtin_amdgcn_exp2f(mx[i] - m);
+        s_w[s] = r;
+        den = fmaf(s < used ? part[s * step + D + 1] : 0.0f, r, den);
+    }
+    den = wave_sum(den);
     if (lane == 0) s_den[wave] = den;
     __syncthreads();
     const int d = tid % D, k = tid / D;
     float num = 0.0f;
 #pragma unroll 8
-    for (int s = k; s < used; s += N) num = fmaf(part[s * (D + 2) + d], s_w[s], num);
+    for (int s = k; s < used; s += N) num = fmaf(part[s * step + d], s_w[s], num);
     s_num[k][d] = num;
     __syncthreads();
     if (tid >= D) return;
@@ -530,9 +613,10 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void attn_paged_tiles
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, h = lane >> 5;
     const int rb = row_base<D>(lane), cb = col_base<D>(lane);
-    const int k = blockIdx.x >> 3, bg = k / p.tiles * 8 + (blockIdx.x & 7);  // a group's tiles on one XCD
-    if (bg >= p.B * p.G) return;
-    const Where w = where(p, BM, bg, p.tiles - 1 - k % p.tiles);  // the longest first
+    // All groups' last tiles, the longest, then those before.  (A group's tiles dealt to one XCD: the same,
+    // B4 T2048 over 16384 H32 G8 D128 1965 us either way, B1 496 and 543.)
+    const int groups = p.B * p.G, turn = blockIdx.x / groups;
+    const Where w = where(p, BM, static_cast<int>(blockIdx.x) - turn * groups, p.tiles - 1 - turn);
     const int all = p.T * p.R, end = w.t1 * p.R;  // rows, and those that are there
     const int per = p.splits > 1 ? share_of(p, lane) : (w.n + kRound - 1) / kRound * kRound;
     const int lo = static_cast<int>(blockIdx.y) * per, hi = lo + per < w.n ? lo + per : w.n;
@@ -743,7 +827,7 @@ __global__ __launch_bounds__(256) void attn_paged_join_tiles_kernel(AttnPagedPar
 template <PrecKind PK, int D>
 hipError_t paged_tiles(AttnPagedParams &p, hipStream_t s)
 {
-    const unsigned x = static_cast<unsigned>((p.B * p.G + 7) / 8) * 8u * p.tiles;
+    const unsigned x = static_cast<unsigned>(p.B) * p.G * p.tiles;
     hipLaunchKernelGGL((attn_paged_tiles_kernel<PK, D>), dim3(x, p.splits), dim3(64 * kWaves), 0, s, p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits == 1) return e;
@@ -756,42 +840,60 @@ hipError_t paged_tiles(AttnPagedParams &p, hipStream_t s)
 template <typename T, PrecKind PK, int D, int C>
 hipError_t paged_c(AttnPagedParams &p, hipStream_t s)
 {
-    const int bg = p.B * p.G;
-    const unsigned x = p.tiles > 1 ? static_cast<unsigned>((bg + 7) / 8) * 8u * p.tiles : bg;
-    hipLaunchKernelGGL((attn_paged_kernel<T, PK, D, C>), dim3(x, p.splits), dim3(64 * kWaves), 0, s, p);
+    if (p.workers == 0) {
+        hipLaunchKernelGGL((attn_paged_kernel<T, PK, D, C, false>), dim3(p.B, p.G), dim3(64 * kWaves), 0, s, p);
+        return hipGetLastError();
+    }
+    hipLaunchKernelGGL((attn_paged_kernel<T, PK, D, C, true>), dim3(p.workers, p.G), dim3(64 * kWaves), 0, s, p);
     const hipError_t e = hipGetLastError();
-    if (e != hipSuccess || p.splits == 1) return e;
-    hipLaunchKernelGGL((attn_paged_join_kernel<T, D>), dim3(static_cast<unsigned>(bg) * p.T * p.R), dim3(256), 0, s, p);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((attn_paged_join_kernel<T, D>), dim3(static_cast<unsigned>(p.B) * p.G * p.T * p.R), dim3(256), 0, s, p);
     return hipGetLastError();
 }
 
 template <typename T, PrecKind PK, int D>
 hipError_t paged_d(AttnPagedParams &p, hipStream_t s)
 {
-    switch (p.rows) {
-    case 16: return paged_c<T, PK, D, 1>(p, s);
-    case 32: return paged_c<T, PK, D, 2>(p, s);
-    case 64: return paged_c<T, PK, D, 4>(p, s);
-    default: return paged_tiles<PK, D>(p, s);
+    if (p.rows == 16) return paged_c<T, PK, D, 1>(p, s);
+    if constexpr (D == 64) {
+        if (p.rows == 32) return paged_c<T, PK, D, 2>(p, s);
     }
+    return paged_tiles<PK, D>(p, s);
 }
 
 }  // namespace
 
-// Rows of a workgroup: 16 columns for each matrix product, more where a group has more rows.
-int attn_paged_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : kTileRows; }
-
-// Shares of the keys: enough workgroups for two on every CU, no share under 512 positions.
-int attn_paged_splits(int B, int G, int64_t rows, int64_t cap)
+// How a call is divided.  Rows of a workgroup: a group of up to 16 rows (D = 64: 32) has its keys go from memory to the matrix units, more
+// by tiles in LDS (20 rows over 4 x 16384 positions, G8 D128: 54 us, and 107 with two column tiles of registers, which spill; D = 64
+// 20 rows, G16: 57 and 48).
+AttnPagedPlan attn_paged_plan(int B, int64_t T, int G, int R, int D, int64_t cap)
 {
-    const int per = attn_paged_rows(rows);
-    const int64_t wg = static_cast<int64_t>(B) * G * ((rows + per - 1) / per);
-    const int64_t least = wg < 128 ? 512 : 1024, most = (cap + least - 1) / least;
-    int64_t s = (512 + wg - 1) / wg;
-    const int64_t by_share = wg < 2048 ? (cap + 4095) / 4096 : 1;
-    s = s > by_share ? s : by_share;
-    s = s < most ? s : most;
-    return static_cast<int>(s < 1 ? 1 : (s > kMaxSplits ? kMaxSplits : s));
+    AttnPagedPlan a = {};
+    const int64_t rows = T * R;
+    a.rows = rows <= 16 ? 16 : rows <= 32 && D == 64 ? 32 : kTileRows;
+    a.tiles = static_cast<int>((rows + a.rows - 1) / a.rows);
+    a.splits = 1;
+    const int64_t groups = static_cast<int64_t>(B) * G;
+    if (a.rows == kTileRows) {
+        const int64_t wg = groups * a.tiles, most = (cap + 511) / 512;
+        int64_t s = wg >= 512 ? 1 : (640 + wg - 1) / wg;
+        s = s < most ? s : most;
+        a.splits = static_cast<int>(s < 1 ? 1 : (s > kMaxSplits ? kMaxSplits : s));
+        a.floats = a.splits == 1 ? 0 : static_cast<size_t>(a.splits) * groups * rows * (D + 2);
+        return a;
+    }
+    // One workgroup a sequence and group for short contexts (1024 positions, B1 G8 D128: 14 us, 17 by runs), and where there are
+    // many times more than the card holds; else runs, 512 workgroups in all: 32 contexts spread over 32768
+    // positions, G8 D128, 379 us (one a sequence 581), 64 over 4096 125 (152); of equal lengths the
+    // runs lose (32 of 4096: 105, 86), but lengths are not known here.  Fewer where little is to be done.
+    const double rounds = static_cast<double>(B) * ((cap + kRound - 1) / kRound);
+    if (cap > 1024 && groups < 4096 && rounds < 2.0e9) {
+        const int64_t some = (256 + G - 1) / G, many = (512 + G - 1) / G, by_work = static_cast<int64_t>(rounds / 4);
+        const int64_t workers = by_work < some ? some : (by_work < many ? by_work : many);
+        a.workers = static_cast<int>(workers < kMaxWorkers ? workers : kMaxWorkers);
+        a.floats = static_cast<size_t>(a.workers + B) * G * rows * (D + 2);
+    }
+    return a;
 }
 
 bool attn_paged_supported(int io_dtype, int D)

@@ -478,12 +478,17 @@ struct AttnPagedParams {
     void *out;  // [B, T, G R, D]
     int B, T, G, R, D;
     float scale;
-    int rows, tiles;  // rows of a workgroup, tiles of a group's T R rows
-    int splits;
-    float *part;  // with more than one: [B T G R][splits][D + 2]
+    // The plan: rows of a workgroup, tiles of a group's T R rows, and either shares of the keys (many rows:
+    // part [splits][B T G R][D] and their references and sums) or workgroups for each group (few rows; 0: one for each
+    // sequence; part [workers + B][G][T R][D + 2]).
+    int rows, tiles, splits, workers;
+    float *part;
 };
-int attn_paged_rows(int64_t rows);
-int attn_paged_splits(int B, int G, int64_t rows, int64_t cap);
+struct AttnPagedPlan {
+    int rows, tiles, splits, workers;
+    size_t floats;
+};
+AttnPagedPlan attn_paged_plan(int B, int64_t T, int G, int R, int D, int64_t cap);
 bool attn_paged_supported(int io_dtype, int D);
 hipError_t launch_attn_paged(AttnPagedParams p, int io_dtype, hipStream_t stream);
 

@@ -134,7 +134,8 @@ def expected_attention(q, cache, pos, lengths=None, scale=None):
     off by that, by two roundings (two parts: 2^-17 of it in bf16) and by its sums, L / 32 + 64 additions in a
     chain; the result is rounded once.  The exponential is the hardware's, 2 u and u of its argument (at most
     the scores' spread, 150 octaves where a probability still counts).  Half a step of fp16 is 2^-25 under 2^-14.
-    Groups of more than 64 rows: probabilities are rounded once, each is off by half a step of itself."""
+    Groups of more than 16 rows (heads of 64 channels: 32): probabilities are rounded once, each is off by half a
+    step of itself."""
     B, T, H, D = q.shape
     G, S = cache.k.shape[1], cache.k.shape[2]
     scale = D ** -0.5 if scale is None else scale
@@ -162,7 +163,7 @@ def expected_attention(q, cache, pos, lengths=None, scale=None):
             w = torch.softmax(s, -1)
             o = torch.einsum("grj,jgd->grd", w, v)
             off = (D + 4) * u * (torch.einsum("grd,jgd->grj", x.abs(), k.abs()) * scale).amax(-1, keepdim=True)
-            rel = 2 * off + (f.eps / 2 if T * (H // G) > 64 else 2.0 ** -16) + (len(rows) / 32 + 64 + 4 + 150) * u
+            rel = 2 * off + (f.eps / 2 if T * (H // G) > (32 if D == 64 else 16) else 2.0 ** -16) + (len(rows) / 32 + 64 + 4 + 150) * u
             out[b, t] = o.reshape(H, D)
             tol[b, t] = (f.eps / 2 * o.abs().clamp_min(f.tiny) + rel * torch.einsum("grj,jgd->grd", w, v.abs())).reshape(H, D) + 1e-30
     return out.to(q.device), tol.to(q.device)
