@@ -68,6 +68,37 @@ __device__ __forceinline__ unsigned pack2(float a, float b)
         return Prec<PK>::from_f32(a) | static_cast<unsigned>(Prec<PK>::from_f32(b)) << 16;
 }
 
+// Requests from the 16 rows at `tile` (uniform), by the lane's offset: buffer requests take the base in
+// scalar registers, where flat ones hold a 64-bit address a row in vector ones.
+template <int N, int STEP>
+__device__ __forceinline__ void load_rows(uint4 (&x)[N], const char *tile, unsigned off)
+{
+#ifdef __HIP_DEVICE_COMPILE__  // the host's pass does not know the builtins' types
+    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(tile), 0, 0x10000, 0x00020000);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        x[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, off + i * STEP, 0, 0));
+#endif
+}
+template <int N>
+__device__ __forceinline__ void load_row(unsigned (&x)[N], const char *tile, unsigned off)
+{
+#ifdef __HIP_DEVICE_COMPILE__
+    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(tile), 0, 0x10000, 0x00020000);
+    if constexpr (N == 2) {
+        const uint2 u = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rsrc, off, 0, 0));
+        x[0] = u.x;
+        x[1] = u.y;
+    } else {
+        const uint4 u = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, off, 0, 0));
+        x[0] = u.x;
+        x[1] = u.y;
+        x[2] = u.z;
+        x[3] = u.w;
+    }
+#endif
+}
+
 // What a workgroup works on: rows m0 .. of group g of sequence b, tokens t0 .. t1 - 1 of
 // which are there, and their positions.
 struct Where {
@@ -263,50 +294,22 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_paged_kernel(AttnPagedPar
         unsigned v[2][4][VW];
     };
     const char *kb = static_cast<const char *>(p.k), *vb = static_cast<const char *>(p.v);
-    const unsigned k_off = n * (2 * D) + kg * 16, v_off = 4 * kg * (2 * D) + n * (2 * CH);
-    auto load_v = [&](unsigned (&v)[VW], const char *at) __attribute__((always_inline)) {
-        if constexpr (VW == 2) {
-            const uint2 u = *reinterpret_cast<const uint2 *>(at);
-            v[0] = u.x;
-            v[1] = u.y;
-        } else {
-            const uint4 u = *reinterpret_cast<const uint4 *>(at);
-            v[0] = u.x;
-            v[1] = u.y;
-            v[2] = u.z;
-            v[3] = u.w;
-        }
-    };
-    // Positions j0 .. j0 + 31 from rows r0 and r1; those past the last key read that one again.  A
-    // tile without a page reads row 0 of the cache, and is hidden.
+    // Positions j0 .. j0 + 31, a tile of 16 from the row of the cache r0, the other from r1; those past the
+    // last key read that one again.  A tile without a page reads row 0 of the cache, and is hidden.
     auto request = [&](Step &st, int j0, unsigned r0, unsigned r1) __attribute__((always_inline)) {
-        r0 = r0 == kNoPage ? 0 : r0;
-        if (j0 + kStep <= w.n) {
-            r1 = r1 == kNoPage ? 0 : r1;
+        const int end = w.n - 1 - j0;  // the last key, from j0
 #pragma unroll
-            for (int a = 0; a < 2; ++a) {
-                const int64_t at = static_cast<int64_t>(a ? r1 : r0) * (2 * D);
+        for (int a = 0; a < 2; ++a) {
+            const bool past = a && end < 16;  // no key in this tile: the other's
+            const unsigned r = a && !past ? r1 : r0;
+            const int last = end - (a && !past ? 16 : 0), top = last < 15 ? last : 15;
+            const int64_t at = static_cast<int64_t>(r == kNoPage ? 0 : r) * (2 * D);
+            const int rk = n < top ? n : top;
+            load_rows<KS, 64>(st.k[a], kb + at, rk * (2 * D) + kg * 16);
 #pragma unroll
-                for (int s = 0; s < KS; ++s) st.k[a][s] = *reinterpret_cast<const uint4 *>(kb + at + k_off + 64 * s);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) load_v(st.v[a][i], vb + at + v_off + i * (2 * D));
-            }
-        } else {
-#pragma unroll
-            for (int a = 0; a < 2; ++a) {
-                const int last = w.n - 1 - (j0 + 16 * a);  // < 0: the tile is past the end, and reads the other's last row
-                const unsigned r = a && last >= 0 ? (r1 == kNoPage ? 0 : r1) : r0;
-                const int top = last >= 0 ? last : w.n - 1 - j0;
-                const int64_t at = static_cast<int64_t>(r) * (2 * D);
-                const int rk = n < top ? n : top;
-                const char *k = kb + at + rk * (2 * D) + kg * 16;
-#pragma unroll
-                for (int s = 0; s < KS; ++s) st.k[a][s] = *reinterpret_cast<const uint4 *>(k + 64 * s);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int rv = 4 * kg + i < top ? 4 * kg + i : top;
-                    load_v(st.v[a][i], vb + at + rv * (2 * D) + n * (2 * CH));
-                }
+            for (int i = 0; i < 4; ++i) {
+                const int rv = 4 * kg + i < top ? 4 * kg + i : top;
+                load_row<VW>(st.v[a][i], vb + at, rv * (2 * D) + n * (2 * CH));
             }
         }
     };
