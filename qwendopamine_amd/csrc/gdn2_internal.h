@@ -499,6 +499,16 @@ constexpr int kSampleList = 8192;  // elements of a row's border bins that are l
 constexpr int kSampleFinishThreads = 1024;
 constexpr int kSampleParts = 64;   // parts of a row at most
 constexpr int kSampleMax = 1 << 20;  // longest row: sums of 2^42 stay under 2^63, indices under 24 bits
+// The bins that the borders of a row's filters fall into.
+struct SampleBorders {
+    int sure;        // bins below this one are kept whole
+    int p_lo, p_hi;  // top-p's border lies in these (p_lo > p_hi: off)
+    int k_bin;       // top-k's in this one (-1: off)
+    unsigned long long k_sum, k_count;  // what lies before it
+    unsigned long long p_sum;           // what lies before p_lo
+    unsigned long long total;           // sum of the row (what min-p keeps)
+    __host__ __device__ bool listed(int b) const { return (b >= p_lo && b <= p_hi) || b == k_bin; }
+};
 struct SampleParams {
     const void *x;
     int64_t inner, outer_stride, row_stride, rows;
@@ -509,9 +519,10 @@ struct SampleParams {
     int top_k_all;
     int64_t *out;
     // The workspace (set by the launcher): of each row [bins][sum, count], the list, the parts'
-    // largest keys and kept sums, their least logits, and the number of listed elements.
-    unsigned long long *hist, *list, *part_key, *part_sum;
-    float *part_low;
+    // kept sums, their largest and least logits, the borders, and the number of listed elements.
+    unsigned long long *hist, *list, *part_sum;
+    float2 *part_top;
+    SampleBorders *borders;
     unsigned *listed;
     int parts, part_pieces, list_len;
 };

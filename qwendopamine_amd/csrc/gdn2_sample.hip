@@ -10,14 +10,16 @@
 // sum agree on every border.  An exponential in float64 costs no more issue slots than one
 // in float32 would save here.  Nothing is sorted.  Every filter keeps a run of the order
 // (logit, lower index), so all that is looked for is its last element:
-//   sample_max     each part's largest element and least logit
-//   sample_hist    counts and sums of the kept by bins that are even in log w
+//   sample_max     each part's largest and least logit
+//   sample_hist    counts (top-k) and sums (top-p) of the kept by bins that are even in log w
 //   sample_gather  the bins that the borders of top-k and top-p fall into: their elements are
 //                  listed, and what lies above them is summed for each part
-//   sample_finish  the borders themselves, by the digits of the listed elements' keys (of
-//                  the row's, if a bin holds more than the list: equal logits), the total,
-//                  the part that holds u times it, and the element within it
-// The logits are read once from memory and twice more from the caches behind the L2.
+//   sample_finish  the borders themselves, by comparing the listed elements with each other (long lists,
+//                  or the row if it overflows, by the digits of their keys), the total, the part that
+//                  holds u times it, and the element within it
+// The logits are read once from memory and twice more from the caches behind the L2.  The passes
+// are bound by issue slots, of which a weight takes about 25: where an element can be told by its
+// logit alone not to count, none is formed.
 #include "gdn2_common.h"
 #include "gdn2_internal.h"
 
@@ -31,9 +33,10 @@ constexpr float kFloor = -43.0f;      // log2 of weights that round to nothing
 constexpr int kThreads = 256;         // of the passes over parts
 constexpr int kFinish = kSampleFinishThreads;
 constexpr int kOwn = kSampleList / kFinish;
+constexpr int kPairs = 256;  // listed elements that are compared each with each (4 us; by digits 6)
 constexpr double kLog2e = 1.4426950408889634074;
 
-// 2^y in units of 2^-42, y <= 0: 2^f by its series, |f| <= 1/2 (the first term left out is under
+// 2^y in units of 2^-42 (at least 1), kFloor < y <= 0: 2^f by its series, |f| <= 1/2 (the first term left out is under
 // 6e-15 of it), rounded by the addition of 2^52.
 __device__ __forceinline__ u64 weight_of(double y)
 {
@@ -46,8 +49,10 @@ __device__ __forceinline__ u64 weight_of(double y)
 #pragma unroll
     for (int i = 10; i >= 0; --i) p = fma(p, f, c[i]);
     const double v = __builtin_amdgcn_ldexp(p, static_cast<int>(n) + kFrac) + 0x1p52;
-    return static_cast<u64>(__double_as_longlong(v)) & 0xfffffffffffffULL;
+    const u64 w = static_cast<u64>(__double_as_longlong(v)) & 0xfffffffffffffULL;
+    return w > 0 ? w : 1;
 }
+__device__ __forceinline__ bool counts(double y) { return y > static_cast<double>(kFloor); }  // not for NaN
 
 // Order of the elements: larger logit first (-0 = 0, NaN above all), of equal ones the lower
 // index.  24 bits of index under 32 of the logit, of 16-bit logits 16.
@@ -85,7 +90,7 @@ struct Key {
 };
 
 // A row, read by 16-byte pieces of its memory; elements outside the row (the first and last
-// piece's) come as -inf.
+// piece's) come as -inf, or (NEAR) as the row's nearest.
 template <typename T>
 struct Logits {
     static constexpr int N = 16 / static_cast<int>(sizeof(T));
@@ -101,6 +106,7 @@ struct Logits {
         pieces = (off + n + N - 1) / N;
     }
     __device__ __forceinline__ int first(int c) const { return c * N - off; }
+    template <bool NEAR = false>
     __device__ __forceinline__ void load(int c, float (&v)[N]) const
     {
         const int i0 = first(c);
@@ -121,21 +127,36 @@ struct Logits {
             }
         } else {
 #pragma unroll
-            for (int e = 0; e < N; ++e) v[e] = i0 + e >= 0 && i0 + e < n ? io<T>::ld(x, i0 + e) : -INFINITY;
+            for (int e = 0; e < N; ++e) {
+                const int i = i0 + e < 0 ? 0 : i0 + e < n ? i0 + e : n - 1;
+                v[e] = io<T>::ld(x, i);
+                if (!NEAR && i != i0 + e) v[e] = -INFINITY;
+            }
         }
     }
 };
 
 __device__ __forceinline__ u64 shfl_xor64(u64 x, int o) { return __shfl_xor(x, o, 64); }
-__device__ __forceinline__ u64 wave_max64(u64 x)
+// Over the wave's lanes, by DPP within rows of 16 (exchanges through LDS take ten times as long).
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x)
 {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const u64 y = shfl_xor64(x, o);
-        x = x > y ? x : y;
-    }
-    return x;
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
 }
+template <typename F>
+__device__ __forceinline__ float wave_all(float x, F f)
+{
+    x = f(x, dpp<0xb1>(x));   // quad_perm [1, 0, 3, 2]
+    x = f(x, dpp<0x4e>(x));   // quad_perm [2, 3, 0, 1]
+    x = f(x, dpp<0x141>(x));  // row_half_mirror
+    x = f(x, dpp<0x140>(x));  // row_mirror
+    const int i = __float_as_int(x);
+    return f(f(__int_as_float(__builtin_amdgcn_readlane(i, 0)), __int_as_float(__builtin_amdgcn_readlane(i, 16))),
+             f(__int_as_float(__builtin_amdgcn_readlane(i, 32)), __int_as_float(__builtin_amdgcn_readlane(i, 48))));
+}
+// The larger, NaN above all.
+__device__ __forceinline__ float max_nan(float a, float b) { return a != a || a > b ? a : b; }
+__device__ __forceinline__ float min_of(float a, float b) { return fminf(a, b); }
 __device__ __forceinline__ u64 wave_sum64(u64 x)
 {
 #pragma unroll
@@ -156,8 +177,7 @@ __device__ __forceinline__ u64 wave_scan64(u64 x, int lane)
 // A row's settings and what the first pass found.
 struct RowState {
     float top;     // largest logit
-    int best;      // its index
-    bool greedy;   // T = 0, or a largest logit that is not finite: the token is `best`
+    bool greedy;   // T = 0, or a largest logit that is not finite: the token is the first of them
     double per;    // log2 of the weight of a difference of 1
     u64 least;     // smallest weight that min-p keeps (at least 1)
     float scale;   // bins per factor of 2
@@ -165,16 +185,12 @@ struct RowState {
     int k;         // top_k; 0: off
 };
 
-template <typename T>
 __device__ __forceinline__ RowState row_state(const SampleParams &p, int64_t row, int lane)
 {
     RowState s;
-    const u64 key = wave_max64(lane < p.parts ? p.part_key[row * kSampleParts + lane] : 0);
-    float low = lane < p.parts ? p.part_low[row * kSampleParts + lane] : INFINITY;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) low = fminf(low, __shfl_xor(low, o, 64));
-    s.top = Key<T>::value(key);
-    s.best = Key<T>::index(key);
+    const float2 own = lane < p.parts ? p.part_top[row * kSampleParts + lane] : make_float2(-INFINITY, INFINITY);
+    s.top = wave_all(own.x, max_nan);
+    const float low = wave_all(own.y, min_of);
     const float t = p.temperature ? p.temperature[row] : p.temperature_all;
     const float m = p.min_p ? p.min_p[row] : p.min_p_all, share = p.top_p ? p.top_p[row] : p.top_p_all;
     const int k = p.top_k ? p.top_k[row] : p.top_k_all;
@@ -214,8 +230,7 @@ template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_max_kernel(SampleParams p)
 {
     constexpr int N = Logits<T>::N, U = 4;
-    __shared__ u64 s_key[kThreads / 64];
-    __shared__ float s_low[kThreads / 64];
+    __shared__ float s_top[kThreads / 64], s_low[kThreads / 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t row = blockIdx.x / p.parts;
     const int part = static_cast<int>(blockIdx.x - row * p.parts);
@@ -227,59 +242,38 @@ __global__ __launch_bounds__(kThreads) void sample_max_kernel(SampleParams p)
     const Logits<T> x(p, row);
     int lo, hi;
     part_range(p, x.pieces, part, lo, hi);
-    u64 best = 0;
-    float low = INFINITY;
+    float top = -INFINITY, low = INFINITY;
+    bool nan = false;
     for (int c0 = lo + tid; c0 < hi; c0 += U * kThreads) {
         float v[U][N];
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (c0 + u * kThreads < hi) x.load(c0 + u * kThreads, v[u]);
+            if (c0 + u * kThreads < hi) x.template load<true>(c0 + u * kThreads, v[u]);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (c0 + u * kThreads >= hi) break;
-            // The piece's first largest (or first NaN), then one comparison of keys.
-            float m = v[u][0];
-            int at = 0;
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
-                const float y = v[u][e];
-                const bool more = e > 0 && (y > m || (y != y && m == m));
-                m = more ? y : m;
-                at = more ? e : at;
-                low = y > -INFINITY ? fminf(low, y) : low;
-            }
-            const int i = x.first(c0 + u * kThreads) + at;
-            if (i >= 0 && i < x.n) {
-                const u64 key = Key<T>::of(m, i);
-                best = best > key ? best : key;
-            } else {
-                // The row's first piece, of -inf alone as far as its maximum goes.
-#pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    const int j = x.first(c0 + u * kThreads) + e;
-                    if (j < 0 || j >= x.n) continue;
-                    const u64 key = Key<T>::of(v[u][e], j);
-                    best = best > key ? best : key;
-                }
+            for (int e = 0; e < N; e += 2) {  // NaN does not show in a maximum
+                top = fmaxf(fmaxf(v[u][e], v[u][e + 1]), top);
+                low = fminf(fminf(v[u][e], v[u][e + 1]), low);
+                nan |= __builtin_isunordered(v[u][e], v[u][e + 1]);
             }
         }
     }
-    best = wave_max64(best);
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) low = fminf(low, __shfl_xor(low, o, 64));
+    top = wave_all(nan ? __uint_as_float(0x7fc00000u) : top, max_nan);
+    low = wave_all(low, min_of);
     if (lane == 0) {
-        s_key[wave] = best;
+        s_top[wave] = top;
         s_low[wave] = low;
     }
     __syncthreads();
     if (tid == 0) {
 #pragma unroll
         for (int w = 1; w < kThreads / 64; ++w) {
-            best = best > s_key[w] ? best : s_key[w];
+            top = max_nan(top, s_top[w]);
             low = fminf(low, s_low[w]);
         }
-        p.part_key[row * kSampleParts + part] = best;
-        p.part_low[row * kSampleParts + part] = low;
+        p.part_top[row * kSampleParts + part] = make_float2(top, low);
     }
 }
 
@@ -293,9 +287,9 @@ __global__ __launch_bounds__(kThreads) void sample_hist_kernel(SampleParams p)
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t row = blockIdx.x / p.parts;
     const int part = static_cast<int>(blockIdx.x - row * p.parts);
-    const RowState s = row_state<T>(p, row, lane);
+    const RowState s = row_state(p, row, lane);
     if (s.greedy) return;
-    const bool bins = filters(s);
+    const bool bins = filters(s), sums = !bins || s.share < 1.0;
     if (bins) {
         for (int i = tid; i < kSampleBins; i += kThreads) {
             s_sum[i] = 0;
@@ -318,13 +312,16 @@ __global__ __launch_bounds__(kThreads) void sample_hist_kernel(SampleParams p)
 #pragma unroll
             for (int e = 0; e < N; ++e) {
                 const double y = log_weight(s, v[u][e]);
-                if (!(y >= static_cast<double>(kFloor))) continue;
-                const u64 w = weight_of(y);
-                if (w < s.least) continue;
+                if (!counts(y)) continue;
+                u64 w = 0;
+                if (sums || s.least > 1) {
+                    w = weight_of(y);
+                    if (w < s.least) continue;
+                }
                 if (bins) {
                     const int b = bin_of(s, y);
-                    atomicAdd(&s_sum[b], w);
-                    atomicAdd(&s_count[b], 1u);
+                    if (sums) atomicAdd(&s_sum[b], w);
+                    if (s.k > 0) atomicAdd(&s_count[b], 1u);
                 } else {
                     sum += w;
                 }
@@ -341,22 +338,12 @@ __global__ __launch_bounds__(kThreads) void sample_hist_kernel(SampleParams p)
     __syncthreads();
     u64 *h = p.hist + row * (2 * kSampleBins);
     for (int i = tid; i < kSampleBins; i += kThreads) {
-        if (s_count[i] == 0) continue;
-        atomicAdd(h + 2 * i, s_sum[i]);
-        atomicAdd(h + 2 * i + 1, static_cast<u64>(s_count[i]));
+        if (s_sum[i] != 0) atomicAdd(h + 2 * i, s_sum[i]);
+        if (s_count[i] != 0) atomicAdd(h + 2 * i + 1, static_cast<u64>(s_count[i]));
     }
 }
 
-// The bins that the borders fall into.
-struct Borders {
-    int sure;          // bins below this one are kept whole
-    int p_lo, p_hi;    // top-p's border lies in these (p_lo > p_hi: off)
-    int k_bin;         // top-k's in this one (-1: off)
-    u64 k_sum, k_count;  // what lies before it
-    u64 p_sum;           // what lies before p_lo
-    u64 total;           // sum of the row (what min-p keeps)
-    __device__ __forceinline__ bool listed(int b) const { return (b >= p_lo && b <= p_hi) || b == k_bin; }
-};
+using Borders = SampleBorders;
 
 // By one wave, from a row's bins: 8 in turn a lane.
 __device__ __forceinline__ Borders borders_of(const RowState &s, const u64 *hist, int lane)
@@ -435,6 +422,15 @@ __device__ __forceinline__ Borders borders_of(const RowState &s, const u64 *hist
     return r;
 }
 
+// Logits below this lie in bins past `last`: the bin's lower end, and a little less for the roundings.
+__device__ __forceinline__ float cut_of(const RowState &s, int last)
+{
+    if (last >= kSampleBins - 1 || !(s.scale > 0.0f)) return -INFINITY;
+    const double y = -static_cast<double>(last + 1) / static_cast<double>(s.scale) * (1.0 + 1e-5) - 1e-5;
+    const double x = static_cast<double>(s.top) + y / s.per;
+    return static_cast<float>(x - 1e-6 * (x < 0.0 ? -x : x));
+}
+
 template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleParams p)
 {
@@ -443,16 +439,19 @@ __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleParams p)
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t row = blockIdx.x / p.parts;
     const int part = static_cast<int>(blockIdx.x - row * p.parts);
-    const RowState s = row_state<T>(p, row, lane);
+    const RowState s = row_state(p, row, lane);
     if (s.greedy || !filters(s)) return;
     const Borders b = borders_of(s, p.hist + row * (2 * kSampleBins), lane);
+    if (part == 0 && tid == 0) p.borders[row] = b;
     const int need = b.p_hi > b.k_bin ? b.p_hi : b.k_bin;  // no bin past this one is wanted
-    const int last = need > b.sure - 1 ? need : b.sure - 1;
+    const float cut = cut_of(s, need > b.sure - 1 ? need : b.sure - 1);
     const Logits<T> x(p, row);
     int lo, hi;
     part_range(p, x.pieces, part, lo, hi);
     u64 sum = 0;
     for (int c0 = lo + tid; c0 < hi; c0 += U * kThreads) {
+        // Which of the thread's elements may count, then those one after another, of all lanes together.
+        unsigned mask = 0;
         float v[U][N];
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -461,21 +460,34 @@ __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleParams p)
         for (int u = 0; u < U; ++u) {
             if (c0 + u * kThreads >= hi) break;
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
-                const double y = log_weight(s, v[u][e]);
-                if (!(y >= static_cast<double>(kFloor))) continue;
+            for (int e = 0; e < N; ++e) mask |= v[u][e] >= cut && v[u][e] > -INFINITY ? 1u << (u * N + e) : 0u;
+        }
+        while (__ballot(mask != 0)) {
+            const int bit = mask ? __ffs(mask) - 1 : 0;
+            const int i = x.first(c0 + bit / N * kThreads) + bit % N;
+            bool have = false;
+            u64 key = 0;
+            if (mask) {
+                const float a = io<T>::ld(x.x, i);
+                const double y = log_weight(s, a);
                 const int bin = bin_of(s, y);
-                if (bin > last) continue;
-                const u64 w = weight_of(y);
-                if (w < s.least) continue;
-                if (bin < b.sure) {
-                    sum += w;
-                } else if (b.listed(bin)) {
-                    const unsigned at = atomicAdd(p.listed + row, 1u);
-                    if (at < static_cast<unsigned>(p.list_len))
-                        p.list[row * p.list_len + at] = Key<T>::of(v[u][e], x.first(c0 + u * kThreads) + e);
+                if (counts(y) && (bin < b.sure || b.listed(bin))) {
+                    const u64 w = weight_of(y);
+                    if (w >= s.least) {
+                        sum += bin < b.sure ? w : 0;
+                        have = bin >= b.sure;
+                        key = Key<T>::of(a, i);
+                    }
                 }
             }
+            const u64 all = __ballot(have);
+            if (all) {
+                unsigned at = 0;
+                if (lane == 0) at = atomicAdd(p.listed + row, static_cast<unsigned>(__popcll(all)));
+                at = __builtin_amdgcn_readfirstlane(at) + __popcll(all & ((1ull << lane) - 1));
+                if (have && at < static_cast<unsigned>(p.list_len)) p.list[row * p.list_len + at] = key;
+            }
+            mask &= mask - 1;
         }
     }
     sum = wave_sum64(sum);
@@ -489,21 +501,42 @@ __global__ __launch_bounds__(kFinish) void sample_finish_kernel(SampleParams p)
 {
     constexpr int N = Logits<T>::N, kW = kFinish / 64;
     __shared__ u64 s_sum[256], s_count[256], s_part[kSampleParts], s_wave[kW];
-    __shared__ u64 s_pick[4], s_last;
+    __shared__ u64 s_pick[4], s_last, s_least[2], s_total;
+    __shared__ ulonglong2 s_list[kPairs];
     __shared__ int s_found;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t row = blockIdx.x;
-    const RowState s = row_state<T>(p, row, lane);
+    const RowState s = row_state(p, row, lane);
+    const Logits<T> x(p, row);
+    // The first of the largest: the token of a greedy row.
+    auto first_top = [&]() {
+        const float own = lane < p.parts ? p.part_top[row * kSampleParts + lane].x : 0.0f;
+        const u64 have = __ballot(lane < p.parts && (own == s.top || (own != own && s.top != s.top)));
+        int lo, hi;
+        part_range(p, x.pieces, __ffsll(have) - 1, lo, hi);
+        if (tid == 0) s_found = x.n;
+        __syncthreads();
+        for (int c = lo + tid; c < hi; c += kFinish) {
+            float v[N];
+            x.load(c, v);
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const int i = x.first(c) + e;
+                if (i >= 0 && i < x.n && (v[e] == s.top || (v[e] != v[e] && s.top != s.top))) atomicMin(&s_found, i);
+            }
+        }
+        __syncthreads();
+        if (tid == 0) p.out[row] = s_found;
+    };
     if (s.greedy) {
-        if (tid == 0) p.out[row] = s.best;
+        first_top();
         return;
     }
-    const Logits<T> x(p, row);
     if (tid < kSampleParts) s_part[tid] = tid < p.parts ? p.part_sum[row * kSampleParts + tid] : 0;
     if (tid == 0) s_found = 0;
     u64 thr = 0;  // the last kept key
     if (filters(s)) {
-        const Borders b = borders_of(s, p.hist + row * (2 * kSampleBins), lane);
+        const Borders b = p.borders[row];
         const unsigned n = p.listed[row];
         const bool from_list = n <= static_cast<unsigned>(p.list_len);
         u64 own[kOwn];
@@ -528,7 +561,7 @@ __global__ __launch_bounds__(kFinish) void sample_finish_kernel(SampleParams p)
 #pragma unroll
                     for (int e = 0; e < N; ++e) {
                         const double y = log_weight(s, v[e]);
-                        if (!(y >= static_cast<double>(kFloor))) continue;
+                        if (!counts(y)) continue;
                         const int bin = bin_of(s, y);
                         if (!b.listed(bin)) continue;
                         const u64 w = weight_of(y);
@@ -609,17 +642,68 @@ __global__ __launch_bounds__(kFinish) void sample_finish_kernel(SampleParams p)
             }
             return prefix;  // not reached: keys differ
         };
-        u64 total = b.total;
-        if (b.k_bin >= 0) {
-            total = b.k_sum;
-            thr = select(false, static_cast<double>(s.k), b.k_bin, b.k_bin, 0, total, b.k_count);
-        }
-        if (s.share < 1.0) {
-            u64 sum = b.p_sum;
-            const u64 at = select(true, s.share * static_cast<double>(total), b.p_lo, b.p_hi, thr, sum, 0);
-            // No listed element is kept: the border lies at the end of the bins before.
-            if (at == ~0ull) thr = ~0ull;
-            else thr = thr > at ? thr : at;
+        if (n <= static_cast<unsigned>(kPairs)) {
+            // Every element against every other: how many of top-k's bin, and what sum of top-p's, lie before
+            // it; thread (i, q) compares element i with each n2-th of the others.
+            const u64 mine = own[0];
+            u64 w = 0;
+            int bin = 0;
+            if (mine) {
+                const double y = log_weight(s, Key<T>::value(mine));
+                w = weight_of(y);
+                bin = bin_of(s, y);
+            }
+            if (tid == 0) {
+                s_total = b.k_bin >= 0 ? b.k_sum : b.total;
+                s_least[0] = s_least[1] = ~0ull;
+            }
+            if (tid < kPairs) {
+                s_list[tid] = make_ulonglong2(mine, w);
+                s_sum[tid] = s_count[tid] = 0;
+            }
+            __syncthreads();
+            unsigned n2 = 64;
+            while (n2 < n) n2 *= 2;
+            const unsigned i = tid & (n2 - 1);
+            const u64 key = s_list[i].x;
+            u64 before = 0, number = 0;
+            for (unsigned j = tid / n2; j < n; j += kFinish / n2) {
+                const ulonglong2 o = s_list[j];
+                const bool more = o.x > key;
+                before += more ? o.y : 0;
+                number += more ? 1 : 0;
+            }
+            atomicAdd(&s_sum[i], before);
+            atomicAdd(&s_count[i], number);
+            __syncthreads();
+            const bool in_k = mine && bin == b.k_bin, in_p = mine && bin >= b.p_lo && bin <= b.p_hi;
+            before = tid < kPairs ? b.p_sum + s_sum[tid] : 0;
+            number = tid < kPairs ? b.k_count + s_count[tid] : 0;
+            // What was counted of the other border's bins: top-p's lie before top-k's, or are the same.
+            const u64 all = static_cast<u64>(__syncthreads_count(in_p && !in_k));
+            const bool kept_k = mine && (!in_k || number - all < static_cast<u64>(s.k));
+            if (in_k && kept_k) {
+                atomicAdd(&s_total, w);
+                atomicMin(&s_least[0], mine);
+            }
+            __syncthreads();
+            const double most = s.share * static_cast<double>(s_total);
+            if (in_p && kept_k && (s.share >= 1.0 || static_cast<double>(before) < most)) atomicMin(&s_least[1], mine);
+            __syncthreads();
+            if (b.k_bin >= 0) thr = s_least[0];
+            if (s.share < 1.0) thr = s_least[1] == ~0ull ? ~0ull : (thr > s_least[1] ? thr : s_least[1]);
+        } else {
+            u64 total = b.total;
+            if (b.k_bin >= 0) {
+                total = b.k_sum;
+                thr = select(false, static_cast<double>(s.k), b.k_bin, b.k_bin, 0, total, b.k_count);
+            }
+            if (s.share < 1.0) {
+                u64 sum = b.p_sum;
+                const u64 at = select(true, s.share * static_cast<double>(total), b.p_lo, b.p_hi, thr, sum, 0);
+                // No listed element is kept: the border lies at the end of the bins before.
+                thr = at == ~0ull ? ~0ull : (thr > at ? thr : at);
+            }
         }
         __syncthreads();
         // What the list adds to the parts.
@@ -663,7 +747,7 @@ __global__ __launch_bounds__(kFinish) void sample_finish_kernel(SampleParams p)
             for (int e = 0; e < N; ++e) {
                 const double y = log_weight(s, v[e]);
                 w[e] = 0;
-                if (y >= static_cast<double>(kFloor) && Key<T>::of(v[e], x.first(c) + e) >= thr && bin_of(s, y) < bins) {
+                if (counts(y) && Key<T>::of(v[e], x.first(c) + e) >= thr && bin_of(s, y) < bins) {
                     const u64 a = weight_of(y);
                     w[e] = a >= s.least ? a : 0;
                 }
@@ -673,10 +757,13 @@ __global__ __launch_bounds__(kFinish) void sample_finish_kernel(SampleParams p)
         const u64 in = wave_scan64(mine, lane);
         if (lane == 63) s_wave[wave] = in;
         __syncthreads();
-        u64 base = run;
-        for (int i = 0; i < wave; ++i) base += s_wave[i];
-        u64 all = run;
-        for (int i = 0; i < kW; ++i) all += s_wave[i];
+        u64 base = run, all = run;
+#pragma unroll
+        for (int i = 0; i < kW; ++i) {
+            const u64 y = s_wave[i];
+            base += i < wave ? y : 0;
+            all += y;
+        }
         u64 at = base + in - mine;
         if (mine > 0 && at <= target && target < base + in) {
 #pragma unroll
@@ -693,7 +780,9 @@ __global__ __launch_bounds__(kFinish) void sample_finish_kernel(SampleParams p)
         if (run > target) break;
     }
     __syncthreads();
-    if (tid == 0 && !s_found) p.out[row] = s.best;
+    const bool found = s_found;
+    __syncthreads();
+    if (!found) first_top();  // not reached: the parts' sums are the sums of their elements
 }
 
 template <typename T>
@@ -729,13 +818,13 @@ int sample_parts(int64_t rows, int64_t n)
     return static_cast<int>(c < 1 ? 1 : (c > kSampleParts ? kSampleParts : c));
 }
 
-// A row's workspace: bins, list, parts' keys, sums and least logits, the number listed.
 static int sample_list(int64_t n) { return static_cast<int>(n < kSampleList ? n : kSampleList); }
 
+// A row's workspace: bins, list, parts' kept sums and largest and least logits, borders, the number listed.
 size_t sample_row_bytes(int64_t n)
 {
-    return 2 * kSampleBins * sizeof(u64) + sample_list(n) * sizeof(u64) + kSampleParts * (2 * sizeof(u64) + sizeof(float)) +
-           sizeof(u64);
+    return 2 * kSampleBins * sizeof(u64) + sample_list(n) * sizeof(u64) + kSampleParts * (sizeof(u64) + sizeof(float2)) +
+           sizeof(SampleBorders) + sizeof(u64);
 }
 
 hipError_t launch_sample(SampleParams p, void *workspace, int io_dtype, hipStream_t s)
@@ -746,12 +835,12 @@ hipError_t launch_sample(SampleParams p, void *workspace, int io_dtype, hipStrea
     w += p.rows * 2 * kSampleBins;
     p.list = w;
     w += p.rows * p.list_len;
-    p.part_key = w;
-    w += p.rows * kSampleParts;
     p.part_sum = w;
     w += p.rows * kSampleParts;
-    p.part_low = reinterpret_cast<float *>(w);
-    p.listed = reinterpret_cast<unsigned *>(p.part_low + p.rows * kSampleParts);
+    p.borders = reinterpret_cast<SampleBorders *>(w);
+    w = reinterpret_cast<u64 *>(p.borders + p.rows);
+    p.part_top = reinterpret_cast<float2 *>(w);
+    p.listed = reinterpret_cast<unsigned *>(p.part_top + p.rows * kSampleParts);
     p.parts = sample_parts(p.rows, p.n);
     const int per = io_dtype == GDN2_DTYPE_F32 ? 4 : 8;
     const int pieces = (p.n + per - 1) / per + 1;  // of a row at any alignment
