@@ -707,7 +707,7 @@ int gdn2_attn_paged(const void *q, const int64_t *strides, int io_dtype, const v
 
 size_t gdn2_sample_tokens_workspace_size(int64_t rows, int64_t n)
 {
-    return rows < 1 || n < 1 ? 0 : static_cast<size_t>(rows) * sample_row_bytes(n);
+    return rows < 1 || n < 1 ? 0 : sample_workspace(rows, n);
 }
 
 int gdn2_sample_tokens(const void *x, int64_t inner, int64_t outer_stride, int64_t row_stride, int io_dtype, int64_t rows,

@@ -495,7 +495,8 @@ hipError_t launch_attn_paged(AttnPagedParams p, int io_dtype, hipStream_t stream
 // A token of each row of logits (rows by two strides, as the log probabilities') by the random
 // number u; settings for each row, or (NULL) for all.
 constexpr int kSampleBins = 512;   // bins of a row's weights
-constexpr int kSampleList = 8192;  // elements of a row's border bins that are listed
+constexpr int kSampleList = 8192;      // elements of a row's border bins that are taken from lists,
+constexpr int kSamplePartList = 1024;  // and of a part's that are listed
 constexpr int kSampleFinishThreads = 1024;
 constexpr int kSampleParts = 64;   // parts of a row at most
 constexpr int kSampleMax = 1 << 20;  // longest row: sums of 2^42 stay under 2^63, indices under 24 bits
@@ -518,16 +519,16 @@ struct SampleParams {
     float temperature_all, top_p_all, min_p_all;
     int top_k_all;
     int64_t *out;
-    // The workspace (set by the launcher): of each row [bins][sum, count], the list, the parts'
-    // kept sums, their largest and least logits, the borders, and the number of listed elements.
-    unsigned long long *hist, *list, *part_sum;
+    // The workspace (set by the launcher): of each row [bins][sum, count], its parts' lists, kept sums, bins'
+    // sums, largest and least logits and numbers listed, and the borders.
+    unsigned long long *hist, *list, *part_sum, *part_hist;
     float2 *part_top;
     SampleBorders *borders;
-    unsigned *listed;
+    unsigned *part_listed;
     int parts, part_pieces, list_len;
 };
 int sample_parts(int64_t rows, int64_t n);
-size_t sample_row_bytes(int64_t n);
+size_t sample_workspace(int64_t rows, int64_t n);
 hipError_t launch_sample(SampleParams p, void *workspace, int io_dtype, hipStream_t stream);
 
 // Backward of the short convolution on a prefill call (no cache).

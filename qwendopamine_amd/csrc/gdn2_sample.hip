@@ -208,6 +208,9 @@ __device__ __forceinline__ RowState row_state(const SampleParams &p, int64_t row
     return s;
 }
 __device__ __forceinline__ bool filters(const RowState &s) { return s.k > 0 || s.share < 1.0; }
+// Whether the bins hold sums: for top-p's border, and so that what top-k keeps for certain need not be summed again
+// unless it is little.
+__device__ __forceinline__ bool binned_sums(const RowState &s) { return s.share < 1.0 || s.k > 1024; }
 
 __device__ __forceinline__ double log_weight(const RowState &s, float x)
 {
@@ -234,10 +237,9 @@ __global__ __launch_bounds__(kThreads) void sample_max_kernel(SampleParams p)
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t row = blockIdx.x / p.parts;
     const int part = static_cast<int>(blockIdx.x - row * p.parts);
-    if (part == 0) {  // what the next passes add to
+    if (part == 0) {  // what the next pass adds to
         u64 *h = p.hist + row * (2 * kSampleBins);
         for (int i = tid; i < 2 * kSampleBins; i += kThreads) h[i] = 0;
-        if (tid == 0) p.listed[row] = 0;
     }
     const Logits<T> x(p, row);
     int lo, hi;
@@ -289,7 +291,7 @@ __global__ __launch_bounds__(kThreads) void sample_hist_kernel(SampleParams p)
     const int part = static_cast<int>(blockIdx.x - row * p.parts);
     const RowState s = row_state(p, row, lane);
     if (s.greedy) return;
-    const bool bins = filters(s), sums = !bins || s.share < 1.0;
+    const bool bins = filters(s), sums = !bins || binned_sums(s);
     if (bins) {
         for (int i = tid; i < kSampleBins; i += kThreads) {
             s_sum[i] = 0;
@@ -336,8 +338,9 @@ __global__ __launch_bounds__(kThreads) void sample_hist_kernel(SampleParams p)
         return;
     }
     __syncthreads();
-    u64 *h = p.hist + row * (2 * kSampleBins);
+    u64 *h = p.hist + row * (2 * kSampleBins), *own = p.part_hist + (row * p.parts + part) * kSampleBins;
     for (int i = tid; i < kSampleBins; i += kThreads) {
+        if (sums) own[i] = s_sum[i];
         if (s_sum[i] != 0) atomicAdd(h + 2 * i, s_sum[i]);
         if (s_count[i] != 0) atomicAdd(h + 2 * i + 1, static_cast<u64>(s_count[i]));
     }
@@ -422,13 +425,15 @@ __device__ __forceinline__ Borders borders_of(const RowState &s, const u64 *hist
     return r;
 }
 
-// Logits below this lie in bins past `last`: the bin's lower end, and a little less for the roundings.
-__device__ __forceinline__ float cut_of(const RowState &s, int last)
+// The logit where bin b begins, moved by a little more than the roundings: logits above it with SIGN -1, of
+// bins up to b - 1, below it with 1, of bins from b on.
+template <int SIGN>
+__device__ __forceinline__ float edge_of(const RowState &s, int b)
 {
-    if (last >= kSampleBins - 1 || !(s.scale > 0.0f)) return -INFINITY;
-    const double y = -static_cast<double>(last + 1) / static_cast<double>(s.scale) * (1.0 + 1e-5) - 1e-5;
+    if (b >= kSampleBins || !(s.scale > 0.0f)) return SIGN < 0 ? -INFINITY : INFINITY;
+    const double y = -static_cast<double>(b) / static_cast<double>(s.scale) * (1.0 - SIGN * 1e-5) + SIGN * 1e-5;
     const double x = static_cast<double>(s.top) + y / s.per;
-    return static_cast<float>(x - 1e-6 * (x < 0.0 ? -x : x));
+    return static_cast<float>(x + SIGN * 1e-6 * (x < 0.0 ? -x : x));
 }
 
 template <typename T>
@@ -436,6 +441,7 @@ __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleParams p)
 {
     constexpr int N = Logits<T>::N, U = 4;
     __shared__ u64 s_part[kThreads / 64];
+    __shared__ unsigned s_n;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t row = blockIdx.x / p.parts;
     const int part = static_cast<int>(blockIdx.x - row * p.parts);
@@ -443,12 +449,23 @@ __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleParams p)
     if (s.greedy || !filters(s)) return;
     const Borders b = borders_of(s, p.hist + row * (2 * kSampleBins), lane);
     if (part == 0 && tid == 0) p.borders[row] = b;
+    // A list of each part's own (one for the row, and its number added to by every wave, took 40 us of 64 rows of 32000).
+    u64 *list = p.list + (row * p.parts + part) * p.list_len;
+    if (tid == 0) s_n = 0;
+    __syncthreads();
+    // What is kept for certain is summed from the part's own bins, or (few) with the listed bins' elements.
+    const bool binned = binned_sums(s);
     const int need = b.p_hi > b.k_bin ? b.p_hi : b.k_bin;  // no bin past this one is wanted
-    const float cut = cut_of(s, need > b.sure - 1 ? need : b.sure - 1);
+    const float cut = edge_of<-1>(s, (need > b.sure - 1 ? need : b.sure - 1) + 1);
+    const float high = binned ? edge_of<1>(s, b.sure) : INFINITY;
     const Logits<T> x(p, row);
     int lo, hi;
     part_range(p, x.pieces, part, lo, hi);
     u64 sum = 0;
+    if (binned) {
+        const u64 *own = p.part_hist + (row * p.parts + part) * kSampleBins;
+        for (int i = tid; i < b.sure; i += kThreads) sum += own[i];
+    }
     for (int c0 = lo + tid; c0 < hi; c0 += U * kThreads) {
         // Which of the thread's elements may count, then those one after another, of all lanes together.
         unsigned mask = 0;
@@ -460,7 +477,7 @@ __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleParams p)
         for (int u = 0; u < U; ++u) {
             if (c0 + u * kThreads >= hi) break;
 #pragma unroll
-            for (int e = 0; e < N; ++e) mask |= v[u][e] >= cut && v[u][e] > -INFINITY ? 1u << (u * N + e) : 0u;
+            for (int e = 0; e < N; ++e) mask |= v[u][e] >= cut && v[u][e] <= high && v[u][e] > -INFINITY ? 1u << (u * N + e) : 0u;
         }
         while (__ballot(mask != 0)) {
             const int bit = mask ? __ffs(mask) - 1 : 0;
@@ -471,11 +488,11 @@ __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleParams p)
                 const float a = io<T>::ld(x.x, i);
                 const double y = log_weight(s, a);
                 const int bin = bin_of(s, y);
-                if (counts(y) && (bin < b.sure || b.listed(bin))) {
+                if (counts(y) && ((bin < b.sure && !binned) || b.listed(bin))) {
                     const u64 w = weight_of(y);
                     if (w >= s.least) {
                         sum += bin < b.sure ? w : 0;
-                        have = bin >= b.sure;
+                        have = bin >= b.sure;  // listed bins are not below `sure`
                         key = Key<T>::of(a, i);
                     }
                 }
@@ -483,9 +500,9 @@ __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleParams p)
             const u64 all = __ballot(have);
             if (all) {
                 unsigned at = 0;
-                if (lane == 0) at = atomicAdd(p.listed + row, static_cast<unsigned>(__popcll(all)));
+                if (lane == 0) at = atomicAdd(&s_n, static_cast<unsigned>(__popcll(all)));
                 at = __builtin_amdgcn_readfirstlane(at) + __popcll(all & ((1ull << lane) - 1));
-                if (have && at < static_cast<unsigned>(p.list_len)) p.list[row * p.list_len + at] = key;
+                if (have && at < static_cast<unsigned>(p.list_len)) list[at] = key;
             }
             mask &= mask - 1;
         }
@@ -493,7 +510,10 @@ __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleParams p)
     sum = wave_sum64(sum);
     if (lane == 0) s_part[wave] = sum;
     __syncthreads();
-    if (tid == 0) p.part_sum[row * kSampleParts + part] = (s_part[0] + s_part[1]) + (s_part[2] + s_part[3]);
+    if (tid == 0) {
+        p.part_sum[row * kSampleParts + part] = (s_part[0] + s_part[1]) + (s_part[2] + s_part[3]);
+        p.part_listed[row * kSampleParts + part] = s_n;
+    }
 }
 
 template <typename T>
@@ -503,6 +523,7 @@ __global__ __launch_bounds__(kFinish) void sample_finish_kernel(SampleParams p)
     __shared__ u64 s_sum[256], s_count[256], s_part[kSampleParts], s_wave[kW];
     __shared__ u64 s_pick[4], s_last, s_least[2], s_total;
     __shared__ ulonglong2 s_list[kPairs];
+    __shared__ unsigned s_upto[64];
     __shared__ int s_found;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t row = blockIdx.x;
@@ -537,13 +558,25 @@ __global__ __launch_bounds__(kFinish) void sample_finish_kernel(SampleParams p)
     u64 thr = 0;  // the last kept key
     if (filters(s)) {
         const Borders b = p.borders[row];
-        const unsigned n = p.listed[row];
-        const bool from_list = n <= static_cast<unsigned>(p.list_len);
+        // The parts' lists, one after another.
+        const unsigned have = lane < p.parts ? p.part_listed[row * kSampleParts + lane] : 0;
+        const unsigned upto = static_cast<unsigned>(wave_scan64(have, lane)), n = __shfl(upto, 63, 64);
+        const bool from_list = n <= static_cast<unsigned>(kSampleList) &&
+                               !__any(have > static_cast<unsigned>(p.list_len));
+        if (wave == 0) s_upto[lane] = upto;
+        __syncthreads();
         u64 own[kOwn];
 #pragma unroll
         for (int i = 0; i < kOwn; ++i) {
             const unsigned at = tid + i * kFinish;
-            own[i] = from_list && at < n ? p.list[row * p.list_len + at] : 0;  // no element's key is 0
+            own[i] = 0;  // no element's key is 0
+            if (from_list && at < n) {
+                int part = 0;
+#pragma unroll
+                for (int step = 32; step > 0; step >>= 1) part += s_upto[part + step - 1] <= at ? step : 0;
+                const unsigned before = part > 0 ? s_upto[part - 1] : 0;
+                own[i] = p.list[(row * p.parts + part) * p.list_len + (at - before)];
+            }
         }
         // f(key, weight, bin) of the listed bins' elements, from the list or the row.
         auto each = [&](auto f) __attribute__((always_inline)) {
@@ -642,7 +675,7 @@ __global__ __launch_bounds__(kFinish) void sample_finish_kernel(SampleParams p)
             }
             return prefix;  // not reached: keys differ
         };
-        if (n <= static_cast<unsigned>(kPairs)) {
+        if (from_list && n <= static_cast<unsigned>(kPairs)) {
             // Every element against every other: how many of top-k's bin, and what sum of top-p's, lie before
             // it; thread (i, q) compares element i with each n2-th of the others.
             const u64 mine = own[0];
@@ -818,30 +851,33 @@ int sample_parts(int64_t rows, int64_t n)
     return static_cast<int>(c < 1 ? 1 : (c > kSampleParts ? kSampleParts : c));
 }
 
-static int sample_list(int64_t n) { return static_cast<int>(n < kSampleList ? n : kSampleList); }
+static int sample_list(int64_t n) { return static_cast<int>(n < kSamplePartList ? n : kSamplePartList); }
 
-// A row's workspace: bins, list, parts' kept sums and largest and least logits, borders, the number listed.
-size_t sample_row_bytes(int64_t n)
+// A row's workspace: bins; its parts' lists, bins, sums, largest and least logits and numbers listed; borders.
+size_t sample_workspace(int64_t rows, int64_t n)
 {
-    return 2 * kSampleBins * sizeof(u64) + sample_list(n) * sizeof(u64) + kSampleParts * (sizeof(u64) + sizeof(float2)) +
-           sizeof(SampleBorders) + sizeof(u64);
+    const int64_t parts = sample_parts(rows, n);
+    return rows * (2 * kSampleBins * sizeof(u64) + parts * (sample_list(n) + kSampleBins) * sizeof(u64) +
+                   kSampleParts * (sizeof(u64) + sizeof(float2) + sizeof(unsigned)) + sizeof(SampleBorders));
 }
 
 hipError_t launch_sample(SampleParams p, void *workspace, int io_dtype, hipStream_t s)
 {
     u64 *w = static_cast<u64 *>(workspace);
+    p.parts = sample_parts(p.rows, p.n);
     p.list_len = sample_list(p.n);
     p.hist = w;
     w += p.rows * 2 * kSampleBins;
     p.list = w;
-    w += p.rows * p.list_len;
+    w += p.rows * p.parts * p.list_len;
     p.part_sum = w;
     w += p.rows * kSampleParts;
+    p.part_hist = w;
+    w += p.rows * p.parts * kSampleBins;
     p.borders = reinterpret_cast<SampleBorders *>(w);
     w = reinterpret_cast<u64 *>(p.borders + p.rows);
     p.part_top = reinterpret_cast<float2 *>(w);
-    p.listed = reinterpret_cast<unsigned *>(p.part_top + p.rows * kSampleParts);
-    p.parts = sample_parts(p.rows, p.n);
+    p.part_listed = reinterpret_cast<unsigned *>(p.part_top + p.rows * kSampleParts);
     const int per = io_dtype == GDN2_DTYPE_F32 ? 4 : 8;
     const int pieces = (p.n + per - 1) / per + 1;  // of a row at any alignment
     p.part_pieces = (pieces + p.parts - 1) / p.parts;
