@@ -1890,40 +1890,48 @@ def _rope_tables(name: str, cos: torch.Tensor, sin: torch.Tensor, D: int) -> tup
         raise ValueError(f"{name}: cos and sin must be [rows, up to D / 2 pairs]; got {tuple(cos.shape)}, {tuple(sin.shape)}")
     if cos.dtype != torch.float32 or sin.dtype != torch.float32 or not (cos.is_contiguous() and sin.is_contiguous()):
         raise ValueError(f"{name}: rotation tables must be contiguous fp32")
-    if _differentiated(cos, sin):
+    if cos.requires_grad or sin.requires_grad:
         raise ValueError(f"{name}: no gradient passes to the rotation tables")
     return cos.shape[1], cos.shape[0]
 
 
 def _one_device(name: str, first: torch.Tensor, *others: torch.Tensor | None) -> None:
     _require_gpu(name, first, *others)
+    dev = first.device
     for t in others:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"{name}: tensors on {first.device} and {t.device}")
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name}: tensors on {dev} and {t.device}")
 
 
 def _aligned(x: torch.Tensor | None) -> torch.Tensor | None:
     """A weight as the kernels read it: contiguous, on 16 bytes."""
-    if x is None:
-        return None
+    if x is None or (x.is_contiguous() and x.data_ptr() % 16 == 0):
+        return x
     x = x.detach().contiguous()
     return x if x.data_ptr() % 16 == 0 else x.clone()
 
 
 def _qkv_norm_rope_fwd(qkv, wq, wk, cos, sin, pos, G: int, R: int, D: int, eps: float):
+    """``(q, k, v)`` of a readable projection (:func:`_qkv_rows`)."""
     B, T, _ = qkv.shape
+    sb, st, _ = qkv.stride()
     dt, dev = qkv.dtype, qkv.device
-    q = torch.empty((B, T, G * R, D), dtype=dt, device=dev)
-    k = torch.empty((B, T, G, D), dtype=dt, device=dev)
-    w_code = nat.dtype_code(dt if wq is None else wq.dtype)
+    x = qkv.detach()
+    q, k = x.new_empty((B, T, G * R, D)), x.new_empty((B, T, G, D))
+    io = nat.dtype_code(dt)
+    pb, pt = (0, 0) if pos is None else pos.stride()
     with _on_device(dev):
-        st = nat.load().gdn2_qkv_norm_rope_fwd(
-            qkv.data_ptr(), qkv.stride(0), qkv.stride(1), nat.dtype_code(dt), nat.ptr(wq), nat.ptr(wk), w_code, eps,
-            cos.data_ptr(), sin.data_ptr(), cos.shape[1], cos.shape[0], nat.ptr(pos),
-            0 if pos is None else pos.stride(0), 0 if pos is None else pos.stride(1), q.data_ptr(), k.data_ptr(), B, T,
-            G, R, D, nat.stream_handle(dev))
-    nat.check(st, "qkv_norm_rope")
-    return q, k, qkv.detach().unflatten(-1, (G, R + 2, D))[..., R + 1, :]
+        status = nat.load().gdn2_qkv_norm_rope_fwd(
+            x.data_ptr(), sb, st, io, nat.ptr(wq), nat.ptr(wk), io if wq is None else nat.dtype_code(wq.dtype), eps,
+            cos.data_ptr(), sin.data_ptr(), cos.shape[1], cos.shape[0], nat.ptr(pos), pb, pt, q.data_ptr(), k.data_ptr(),
+            B, T, G, R, D, nat.stream_handle(dev))
+    nat.check(status, "qkv_norm_rope")
+    return q, k, x.as_strided((B, T, G, D), (sb, st, (R + 2) * D, 1), x.storage_offset() + (R + 1) * D)
+
+
+def _dense(x: torch.Tensor, dt: torch.dtype) -> torch.Tensor:
+    """:func:`_io` of what mostly needs nothing."""
+    return x if x.dtype == dt and x.is_contiguous() and x.data_ptr() % 16 == 0 else _io(x, dt)
 
 
 class QkvNormRopeFunction(torch.autograd.Function):
@@ -1944,24 +1952,28 @@ class QkvNormRopeFunction(torch.autograd.Function):
         qkv, wq, wk, cos, sin, pos = ctx.saved_tensors
         G, R, D, eps, shape, dt = ctx.dims
         B, T, _ = shape
-        dq, dk, dv = (_io(x, dt) for x in (dq, dk, dv))
+        dq, dk, dv = _dense(dq, dt), _dense(dk, dt), _dense(dv, dt)
         dev = dq.device
-        dqkv = torch.empty(shape, dtype=dt, device=dev)
+        dqkv = dq.new_empty(shape)
         x = dqkv if qkv is None else qkv  # without weights the projection is not read
-        dwq, dwk = (None, None) if wq is None else (torch.empty_like(wq), torch.empty_like(wk))
-        if wq is not None and B * T == 0:
-            dwq.zero_()
-            dwk.zero_()
+        io = nat.dtype_code(dt)
         lib = nat.load()
-        nbytes = 0 if wq is None else lib.gdn2_qkv_norm_rope_bwd_workspace_size(B, T, G, R, D)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        w_code, nbytes, dwq, dwk, ws = io, 0, None, None, None
+        if wq is not None:
+            dwq, dwk = torch.empty_like(wq), torch.empty_like(wk)
+            w_code = nat.dtype_code(wq.dtype)
+            nbytes = lib.gdn2_qkv_norm_rope_bwd_workspace_size(B, T, G, R, D)
+            ws = dq.new_empty(nbytes // dq.element_size())
+            if B * T == 0:
+                dwq.zero_()
+                dwk.zero_()
+        pb, pt = (0, 0) if pos is None else pos.stride()
         with _on_device(dev):
             st = lib.gdn2_qkv_norm_rope_bwd(
-                x.data_ptr(), x.stride(0), x.stride(1), nat.dtype_code(dt), nat.ptr(wq), nat.ptr(wk),
-                nat.dtype_code(dt if wq is None else wq.dtype), eps, cos.data_ptr(), sin.data_ptr(), cos.shape[1],
-                cos.shape[0], nat.ptr(pos), 0 if pos is None else pos.stride(0), 0 if pos is None else pos.stride(1),
-                dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dqkv.data_ptr(), nat.ptr(dwq), nat.ptr(dwk), B, T, G, R, D,
-                nat.ptr(ws), nbytes, nat.stream_handle(dev))
+                x.data_ptr(), x.stride(0), x.stride(1), io, nat.ptr(wq), nat.ptr(wk), w_code, eps, cos.data_ptr(),
+                sin.data_ptr(), cos.shape[1], cos.shape[0], nat.ptr(pos), pb, pt, dq.data_ptr(), dk.data_ptr(),
+                dv.data_ptr(), dqkv.data_ptr(), nat.ptr(dwq), nat.ptr(dwk), B, T, G, R, D, nat.ptr(ws), nbytes,
+                nat.stream_handle(dev))
         nat.check(st, "qkv_norm_rope backward")
         return dqkv, dwq, dwk, None, None, None, None, None, None
 
