@@ -565,7 +565,7 @@ static int check_qkv_rope(QkvRopeParams &p, const void *qkv, int64_t stride_b, i
     if ((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(wq) | reinterpret_cast<uintptr_t>(wk)) & 15)
         return GDN2_ERR_INVALID;
     if ((reinterpret_cast<uintptr_t>(cos) | reinterpret_cast<uintptr_t>(sin)) & 3) return GDN2_ERR_INVALID;
-    if (T > 2147483647LL || static_cast<double>(B) * T * qkv_rope_units(G * (R + 2), D) / 4 + 1 >
+    if (T > 2147483647LL || static_cast<double>(B) * T * qkv_rope_units(G * (R + 2), D, true) / 4 + 1 >
                                 static_cast<double>(max_workgroups(256)))
         return GDN2_ERR_UNSUPPORTED;
     p.qkv = qkv; p.stride_b = stride_b; p.stride_t = stride_t;
@@ -599,7 +599,7 @@ int gdn2_qkv_norm_rope_fwd(const void *qkv, int64_t stride_b, int64_t stride_t, 
 size_t gdn2_qkv_norm_rope_bwd_workspace_size(int B, int64_t T, int G, int R, int D)
 {
     if (B < 1 || T < 1 || G < 1 || R < 1 || D < 1 || D > 256) return 0;
-    return static_cast<size_t>(qkv_rope_bwd_blocks(static_cast<int64_t>(B) * T * qkv_rope_units(G * (R + 2), D))) * 2 * D *
+    return static_cast<size_t>(qkv_rope_bwd_blocks(static_cast<int64_t>(B) * T * qkv_rope_units(G * (R + 2), D, true))) * 2 * D *
            sizeof(float);
 }
 

@@ -459,7 +459,7 @@ struct QkvRopeParams {
     int wide_tables;
 };
 int qkv_rope_lanes(int D);
-int qkv_rope_units(int rows, int D);
+int qkv_rope_units(int rows, int D, bool backward);
 int qkv_rope_bwd_blocks(int64_t units);
 hipError_t launch_qkv_rope_fwd(QkvRopeParams p, int io_dtype, hipStream_t stream);
 hipError_t launch_qkv_rope_bwd(QkvRopeParams p, int io_dtype, hipStream_t stream);

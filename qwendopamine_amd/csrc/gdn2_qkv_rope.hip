@@ -19,7 +19,9 @@
 namespace gdn2 {
 namespace {
 
-constexpr int kRows = 4;  // U: rows in flight per lane
+// U: rows in flight per lane.  The backward holds two tensors' rows and the weights' sums: with 2 it is 30 us at
+// B4 T2048 H16 G16 D64 and 28 at T7013 H16 G4 D128, with 4, at fewer waves, 38 and 36.
+constexpr int kRowsFwd = 4, kRowsBwd = 2;
 
 struct Row8 {
     float x[8];
@@ -145,13 +147,13 @@ __device__ __forceinline__ Row8 weights(const QkvRopeParams &p, const void *w, i
 struct Unit {
     int b, t, row0;
 };
-template <int LPR>
+template <int LPR, int U>
 __device__ __forceinline__ Unit unit_of(const QkvRopeParams &p, int64_t unit)
 {
     const unsigned u = static_cast<unsigned>(unit);
     const unsigned token = u / p.units, b = token / p.T;
     return {static_cast<int>(b), static_cast<int>(token - b * p.T),
-            static_cast<int>(u - token * p.units) * (kRows * (64 / LPR))};
+            static_cast<int>(u - token * p.units) * (U * (64 / LPR))};
 }
 
 // The token's position; -1 where it has none (outside the tables, or padding).
@@ -184,17 +186,17 @@ __global__ __launch_bounds__(256) void qkv_rope_kernel(QkvRopeParams p)
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t unit = static_cast<int64_t>(blockIdx.x) * 4 + wave;
     if (unit >= p.all_units) return;
-    const Unit w = unit_of<LPR>(p, unit);
+    const Unit w = unit_of<LPR, kRowsFwd>(p, unit);
     const int c = lane & (LPR - 1), ch = 8 * c;
     const bool in = ch < p.D;
     const int64_t token = static_cast<int64_t>(w.b) * p.T + w.t;
     const T *x = static_cast<const T *>(p.qkv) + w.b * p.stride_b + w.t * p.stride_t + (in ? ch : 0);
     const int R = p.R, D = p.D;
-    Head hd[kRows];
-    Row8 v[kRows];
-    bool have[kRows];
+    Head hd[kRowsFwd];
+    Row8 v[kRowsFwd];
+    bool have[kRowsFwd];
 #pragma unroll
-    for (int u = 0; u < kRows; ++u) {
+    for (int u = 0; u < kRowsFwd; ++u) {
         const int i = w.row0 + u * (64 / LPR) + lane / LPR;
         have[u] = in && i < p.G * p.per;
         hd[u] = head_of(p, have[u] ? i : 0);
@@ -218,7 +220,7 @@ __global__ __launch_bounds__(256) void qkv_rope_kernel(QkvRopeParams p)
     if (pos < 0) {
         const Row8 zero = {};
 #pragma unroll
-        for (int u = 0; u < kRows; ++u) {
+        for (int u = 0; u < kRowsFwd; ++u) {
             if (!have[u]) continue;
             if (hd[u].slot < R)
                 store8(q + (hd[u].g * R + hd[u].slot) * D, zero);
@@ -234,7 +236,7 @@ __global__ __launch_bounds__(256) void qkv_rope_kernel(QkvRopeParams p)
         wk = weights<T>(p, p.wk, in ? ch : 0);
     }
 #pragma unroll
-    for (int u = 0; u < kRows; ++u) {
+    for (int u = 0; u < kRowsFwd; ++u) {
         const bool is_q = hd[u].slot < R;
         Row8 y = v[u];
         if constexpr (NORM) {
@@ -282,14 +284,14 @@ __global__ __launch_bounds__(256) void qkv_rope_bwd_kernel(QkvRopeParams p)
         wk = weights<T>(p, p.wk, in ? ch : 0);
     }
     for (int64_t unit = static_cast<int64_t>(blockIdx.x) * 4 + wave; unit < p.all_units; unit += 4LL * gridDim.x) {
-        const Unit w = unit_of<LPR>(p, unit);
+        const Unit w = unit_of<LPR, kRowsBwd>(p, unit);
         const int64_t token = static_cast<int64_t>(w.b) * p.T + w.t;
         const T *x = static_cast<const T *>(p.qkv) + w.b * p.stride_b + w.t * p.stride_t + (in ? ch : 0);
-        Head hd[kRows];
-        Row8 dy[kRows], v[kRows];
-        bool have[kRows];
+        Head hd[kRowsBwd];
+        Row8 dy[kRowsBwd], v[kRowsBwd];
+        bool have[kRowsBwd];
 #pragma unroll
-        for (int u = 0; u < kRows; ++u) {
+        for (int u = 0; u < kRowsBwd; ++u) {
             const int i = w.row0 + u * RPW + lane / LPR;
             have[u] = in && i < p.G * p.per;
             hd[u] = head_of(p, have[u] ? i : 0);
@@ -304,7 +306,7 @@ __global__ __launch_bounds__(256) void qkv_rope_bwd_kernel(QkvRopeParams p)
         const Angles a = angles_of(p, pos < 0 ? 0 : pos, c);
         T *dx = static_cast<T *>(p.dqkv) + token * p.G * (R + 2) * D + ch;
 #pragma unroll
-        for (int u = 0; u < kRows; ++u) {
+        for (int u = 0; u < kRowsBwd; ++u) {
             const bool is_v = hd[u].slot > R, is_q = hd[u].slot < R;
             Row8 d = dy[u];
             rotate<true>(d, a);
@@ -427,7 +429,7 @@ hipError_t rope_d(QkvRopeParams &p, int io_dtype, hipStream_t s)
     // Rows of a group: the values are copied into pages, and in the gradient.
     p.per = p.R + (BWD || p.table ? 2 : 1);
     p.per_m = static_cast<unsigned>((0x100000000ULL + p.per - 1) / p.per);
-    p.units = qkv_rope_units(p.G * p.per, p.D);
+    p.units = qkv_rope_units(p.G * p.per, p.D, BWD);
     p.all_units = static_cast<int64_t>(p.B) * p.T * p.units;
     p.wide_tables = ((reinterpret_cast<uintptr_t>(p.cos) | reinterpret_cast<uintptr_t>(p.sin)) & 15) == 0;
     switch (io_dtype) {
@@ -446,9 +448,9 @@ int qkv_rope_lanes(int D)
     return l;
 }
 
-int qkv_rope_units(int rows, int D)
+int qkv_rope_units(int rows, int D, bool backward)
 {
-    const int per = kRows * (64 / qkv_rope_lanes(D));
+    const int per = (backward ? kRowsBwd : kRowsFwd) * (64 / qkv_rope_lanes(D));
     return (rows + per - 1) / per;
 }
 
