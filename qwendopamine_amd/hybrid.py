@@ -26,8 +26,12 @@ What differs from the reference host, deliberately:
   is one pass (``ops.silu_mul``); both round as the torch ops they replace, and the
   logits are bit-identical to the unfused host's.
 * **Training and scoring.** ``HybridConfig.attention = "hip"`` trains (and prefills) the
-  attention layers on ``ops.attention``; ``HybridDecoder.token_logprobs`` and ``loss`` take the
-  logits through ``ops.token_logprobs`` instead of a log-softmax in memory.
+  attention layers on ``ops.attention``, their heads rotated in one pass (``ops.qkv_norm_rope``);
+  ``HybridDecoder.token_logprobs`` and ``loss`` take the logits through ``ops.token_logprobs``
+  instead of a log-softmax in memory.
+* **Query and key norms, paged caches, sampling.** ``HybridConfig.qk_norm`` normalises every query
+  and key head before the rotation; ``setup_caches(..., page_size=n)`` keeps keys and values in
+  pages (``ops.KVCachePaged``); ``SamplingDecoder`` draws its tokens (``ops.sample_tokens``).
 """
 
 from __future__ import annotations
@@ -77,6 +81,9 @@ class HybridConfig:
     # (``ops.attention``: grouped heads in place, its own backward; bf16 / fp16 heads of 64 or
     # 128 channels on the GPU, else as "sdpa").
     attention: str = "sdpa"
+    # An RMS norm of every query and key head before the rotation (``q_norm`` / ``k_norm`` weights of
+    # ``head_size``, shared by a layer's heads); no counterpart in the reference.
+    qk_norm: bool = False
 
     def __post_init__(self) -> None:
         if self.attention not in ("sdpa", "hip"):
@@ -192,7 +199,7 @@ class CausalSelfAttention(nn.Module):
     fused ``attn`` projection laid out ``[groups, q_per_kv + 2, head_size]``, output ``proj``.
 
     The cache is ``[B, groups, max_seq_length, head_size]`` per tensor, or an ``ops.KVCacheQ4``
-    (inference only). A multi-token cached call is a prefill from position 0: it attends
+    or an ``ops.KVCachePaged`` (both inference only). A multi-token cached call is a prefill from position 0: it attends
     within its own tokens (causal SDPA, flash or memory-efficient kernels only, or
     ``ops.attention``: ``HybridConfig.attention``) and stores k, v. A single-token
     call attends over the cache up to its position; its products are issued with
@@ -208,7 +215,28 @@ class CausalSelfAttention(nn.Module):
         self.attn = nn.Linear(config.n_embd, (self.n_head + 2 * self.n_query_groups) * self.head_size,
                               bias=config.bias)
         self.proj = nn.Linear(self.n_head * self.head_size, config.n_embd, bias=config.bias)
-        self.kv_cache: tuple[torch.Tensor, torch.Tensor] | ops.KVCacheQ4 | None = None
+        if config.qk_norm:
+            self.q_norm = RMSNorm(self.head_size, eps=config.norm_eps)
+            self.k_norm = RMSNorm(self.head_size, eps=config.norm_eps)
+        self.kv_cache: tuple[torch.Tensor, torch.Tensor] | ops.KVCacheQ4 | ops.KVCachePaged | None = None
+
+    def _norm_weights(self) -> tuple[torch.Tensor | None, torch.Tensor | None]:
+        return (self.q_norm.weight, self.k_norm.weight) if self.config.qk_norm else (None, None)
+
+    def _heads(self, qkv: torch.Tensor, cos: torch.Tensor,
+               sin: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """q, k (normalised, rotated) and v ``[B, T, heads, D]`` of the fused projection; ``cos`` / ``sin`` the tokens' rows."""
+        b, t, _ = qkv.shape
+        G, qpk, D = self.n_query_groups, self.n_head // self.n_query_groups, self.head_size
+        if ((self.config.qk_norm or self.config.attention == "hip") and qkv.is_cuda and D % 8 == 0 and D <= 256
+                and qkv.dtype in (torch.bfloat16, torch.float16, torch.float32)):
+            # One pass; without norms the bits of the torch operations below.
+            return ops.qkv_norm_rope(qkv, cos, sin, self.n_head, G, *self._norm_weights(), self.config.norm_eps)
+        q, k, v = qkv.view(b, t, G, qpk + 2, D).split((qpk, 1, 1), dim=-2)
+        q, k = q.reshape(b, t, self.n_head, D), k.reshape(b, t, G, D)
+        if self.config.qk_norm:
+            q, k = self.q_norm(q), self.k_norm(k)
+        return apply_rotary_emb(q, cos, sin), apply_rotary_emb(k, cos, sin), v.reshape(b, t, G, D)
 
     def forward(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
                 input_pos: torch.Tensor | None = None, mask: torch.Tensor | None = None) -> torch.Tensor:
@@ -219,6 +247,15 @@ class CausalSelfAttention(nn.Module):
         """``forward`` from the fused ``attn`` projection's output ``[B, T, (n_head + 2 G) D]``."""
         b, t, _ = qkv.shape
         G, qpk, D = self.n_query_groups, self.n_head // self.n_query_groups, self.head_size
+        if input_pos is not None and isinstance(self.kv_cache, ops.KVCachePaged):
+            if not _inference(qkv):
+                raise NotImplementedError("a paged cache is written and read without gradients")
+            # ``cos`` / ``sin`` are whole tables here (``HybridDecoder.forward``); positions are consecutive.
+            start = input_pos[:1]
+            q = ops.kv_cache_paged_append(qkv, cos, sin, start, self.kv_cache, self.n_head, *self._norm_weights(),
+                                          self.config.norm_eps)
+            o = ops.attention_paged(q, self.kv_cache, start)
+            return ops.linear(o.reshape(b, t, self.n_head * D), self.proj.weight, self.proj.bias)
         q4 = input_pos is not None and isinstance(self.kv_cache, ops.KVCacheQ4)
         if q4 and t == 1:
             if not _inference(qkv):
@@ -226,8 +263,8 @@ class CausalSelfAttention(nn.Module):
             # One launch (and a merge for long caches), as below.
             o = ops.attention_decode_q4(qkv, cos, sin, input_pos, self.kv_cache, self.n_head)
             return ops.linear(o.reshape(b, 1, self.n_head * D), self.proj.weight, self.proj.bias)
-        if (t == 1 and input_pos is not None and self.kv_cache is not None and _inference(qkv)
-                and ops.attention_decode_supported(qkv, qpk, D)):
+        if (t == 1 and input_pos is not None and self.kv_cache is not None and not self.config.qk_norm
+                and _inference(qkv) and ops.attention_decode_supported(qkv, qpk, D)):
             # RoPE, the cache store and the attention of the token in one HIP launch.
             o = ops.attention_decode(qkv, cos, sin, input_pos, *self.kv_cache, self.n_head)
             return ops.linear(o.reshape(b, 1, self.n_head * D), self.proj.weight, self.proj.bias)
@@ -240,11 +277,7 @@ class CausalSelfAttention(nn.Module):
             if mask is None and self.kv_cache is not None and not q4:
                 L = self.kv_cache[0].shape[2]
                 mask = (torch.arange(L, device=qkv.device)[None, :] <= input_pos[:, None]).reshape(1, 1, t, L)
-        qkv = qkv.view(b, t, G, qpk + 2, D)
-        q, k, v = qkv.split((qpk, 1, 1), dim=-2)
-        q = apply_rotary_emb(q.reshape(b, t, self.n_head, D), cos, sin)
-        k = apply_rotary_emb(k.reshape(b, t, G, D), cos, sin)
-        v = v.reshape(b, t, G, D)
+        q, k, v = self._heads(qkv, cos, sin)
         if input_pos is not None:
             if self.kv_cache is None:
                 raise RuntimeError("KV cache not set up: call HybridDecoder.setup_caches first")
@@ -428,32 +461,46 @@ class HybridDecoder(nn.Module):
             at = blk.attn
             w = at.attn.weight
             G, qpk, D = at.n_query_groups, at.n_head // at.n_query_groups, at.head_size
-            if isinstance(at.kv_cache, ops.KVCacheQ4):
-                continue  # attention_decode_q4 reads the tables' row too
-            if at.kv_cache is None or not _inference(w) or not ops.attention_decode_supported(w, qpk, D):
+            if isinstance(at.kv_cache, (ops.KVCacheQ4, ops.KVCachePaged)):
+                continue  # their kernels read the tables' row too
+            if at.config.qk_norm or at.kv_cache is None or not _inference(w) or not ops.attention_decode_supported(w, qpk, D):
                 return False
         return True
 
-    def setup_caches(self, batch: int, max_seq_length: int, kv_bits: int = 16) -> None:
+    def setup_caches(self, batch: int, max_seq_length: int, kv_bits: int = 16, page_size: int | None = None) -> None:
         """Allocate the attention KV caches ``[batch, groups, max_seq_length, head_size]``
         and the causal mask, and drop every gdn2 cache (the next cached forward is a
         prefill).  ``kv_bits=4``: the KV caches in 4 bits (``ops.KVCacheQ4``; a bf16 or fp16
-        model on the GPU, heads of 64 or 128 channels, inference)."""
+        model on the GPU, heads of 64 or 128 channels, inference).  ``page_size``: in pages of so
+        many positions (``ops.KVCachePaged``, all layers with one table of pages, every sequence its own;
+        the same models)."""
         p = self.lm_head.weight
         c = self.config
+        if page_size is not None and kv_bits != 16:
+            raise NotImplementedError("a paged cache is kept in the model's dtype (kv_bits=16)")
+        if kv_bits == 4 and c.qk_norm:
+            raise NotImplementedError("the 4-bit cache's decode step does not normalise queries and keys")
         if kv_bits not in (4, 16):
             raise ValueError(f"kv_bits must be 4 or 16 (the model's dtype), got {kv_bits}")
         if kv_bits == 4 and not ops.attention_decode_q4_supported(p, c.n_head // c.n_query_groups, c.head_size):
             raise NotImplementedError("a 4-bit cache needs a bf16 or fp16 model on the GPU, heads of 64 or 128 "
                                       "channels and at most 16 query heads per group")
+        if page_size is not None and not ops.attention_paged_supported(p, c.head_size):
+            raise NotImplementedError("a paged cache needs a bf16 or fp16 model on the GPU and heads of 64 or 128 channels")
         self.max_seq_length = max_seq_length
-        self.mask_cache = torch.tril(torch.ones(max_seq_length, max_seq_length, dtype=torch.bool,
-                                                device=p.device))[None, None]
+        table = None
+        n = 0 if page_size is not None else max_seq_length  # pages need no mask
+        self.mask_cache = torch.tril(torch.ones(n, n, dtype=torch.bool, device=p.device))[None, None]
         self._rope_tables(max_seq_length, p.device)
         for blk in self.h:
             blk.gdn2_cache = None
             if not blk.use_gdn2:
                 shape = (batch, c.n_query_groups, max_seq_length, c.head_size)
+                if page_size is not None:
+                    cache = ops.kv_cache_paged(*shape, page_size=page_size, dtype=p.dtype, device=p.device)
+                    table = cache.table if table is None else table
+                    blk.attn.kv_cache = cache._replace(table=table)
+                    continue
                 if kv_bits == 4:
                     blk.attn.kv_cache = ops.kv_cache_q4(*shape, device=p.device)
                     continue
@@ -475,10 +522,11 @@ class HybridDecoder(nn.Module):
         else:
             if self.mask_cache is None:
                 raise RuntimeError("call setup_caches before a cached forward")
-            if not (t == 1 and self._attention_decode_fused()):
+            paged = any(isinstance(blk.attn.kv_cache, ops.KVCachePaged) for blk in self.h if not blk.use_gdn2)
+            if not paged and not (t == 1 and self._attention_decode_fused()):
                 cos, sin = cos.index_select(0, input_pos), sin.index_select(0, input_pos)
                 mask = self.mask_cache.index_select(2, input_pos)
-            # else: every attention layer takes the fused decode kernel, which reads
+            # else: every attention layer takes the fused decode kernel (or has pages), which reads
             # the rotation tables' row input_pos itself and needs no mask.
         x = self.wte(idx)
         if _inference(x, self.ln_f.weight) and ops.add_rms_norm_supported(x):
@@ -526,15 +574,17 @@ class GreedyDecoder:
     ``kv_bits=4`` decodes from 4-bit KV caches (``HybridDecoder.setup_caches``).  With
     ``keep_logprobs=n``, ``logprobs`` holds the last step's ``ops.TokenLogprobs`` (of the token it
     chose, with ``n`` alternatives; overwritten by the next step), and ``generate`` leaves every
-    step's in ``sequence_logprobs`` (``[B, n_tokens, ...]``).
+    step's in ``sequence_logprobs`` (``[B, n_tokens, ...]``).  ``page_size`` keeps keys and values in
+    pages (``HybridDecoder.setup_caches``).
     """
 
     def __init__(self, model: HybridDecoder, use_graph: bool = True, keep_logits: bool = False,
-                 kv_bits: int = 16, keep_logprobs: int | None = None) -> None:
+                 kv_bits: int = 16, keep_logprobs: int | None = None, page_size: int | None = None) -> None:
         self.model = model
         self.use_graph = use_graph
         self.keep_logits = keep_logits
         self.kv_bits = kv_bits
+        self.page_size = page_size
         self.keep_logprobs = keep_logprobs
         self.logprobs: ops.TokenLogprobs | None = None
         self._replayed_logprobs: ops.TokenLogprobs | None = None
@@ -546,10 +596,10 @@ class GreedyDecoder:
     def prefill(self, prompt: torch.Tensor, max_new_tokens: int) -> torch.Tensor:
         B, T = prompt.shape
         dev = prompt.device
-        self.model.setup_caches(B, T + max_new_tokens, self.kv_bits)
+        self.model.setup_caches(B, T + max_new_tokens, self.kv_bits, self.page_size)
         self.graph = None
         logits = self.model(prompt, input_pos=torch.arange(T, device=dev), last_only=True)[:, -1]
-        self.tok = logits.argmax(-1, keepdim=True)
+        self.tok = self._first(logits)
         self.pos = torch.full((1,), T, dtype=torch.long, device=dev)
         if self.keep_logits:
             self.logits = logits.float()
@@ -557,9 +607,17 @@ class GreedyDecoder:
             self.logprobs = ops.token_logprobs(logits, self.tok[:, 0], top_k=self.keep_logprobs)
         return self.tok
 
+    def _first(self, logits: torch.Tensor) -> torch.Tensor:
+        """The token ``[B, 1]`` that the prompt gives."""
+        return logits.argmax(-1, keepdim=True)
+
+    def _choose(self, logits: torch.Tensor) -> None:
+        """The next token into ``self.tok``."""
+        ops.argmax_rows(logits, out=self.tok)  # one launch (torch's reduction is about 50 µs here)
+
     def _step(self) -> None:
         logits = self.model(self.tok, input_pos=self.pos)[:, -1]
-        ops.argmax_rows(logits, out=self.tok)  # one launch (torch's reduction is about 50 µs here)
+        self._choose(logits)
         self.pos.add_(1)
         if self.keep_logits:
             self.logits.copy_(logits)
@@ -606,6 +664,34 @@ class GreedyDecoder:
         return torch.cat(out, dim=1)
 
 
+class SamplingDecoder(GreedyDecoder):
+    """``GreedyDecoder`` whose tokens are drawn: ``ops.sample_tokens`` with ``temperature``, ``top_k``, ``top_p`` and
+    ``min_p`` (numbers, or tensors ``[B]`` on the device with one for each sequence), from random numbers
+    of ``generator`` (of the model's device; torch's own without one).  They are drawn before each step, into
+    a tensor that the captured step reads, so that a generator's seed gives the same tokens with and
+    without a graph.  ``temperature=0`` decodes greedily."""
+
+    def __init__(self, model: HybridDecoder, temperature: float | torch.Tensor = 1.0, top_k: int | torch.Tensor = 0,
+                 top_p: float | torch.Tensor = 1.0, min_p: float | torch.Tensor = 0.0,
+                 generator: torch.Generator | None = None, **kwargs) -> None:
+        super().__init__(model, **kwargs)
+        self.settings = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        self.generator = generator
+
+    def _first(self, logits: torch.Tensor) -> torch.Tensor:
+        self.uniforms = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
+        self.uniforms.uniform_(generator=self.generator)
+        return ops.sample_tokens(logits, self.uniforms, **self.settings)[:, None]
+
+    def _choose(self, logits: torch.Tensor) -> None:
+        self.tok.copy_(ops.sample_tokens(logits, self.uniforms, **self.settings)[:, None])
+
+    @torch.no_grad()
+    def step(self) -> torch.Tensor:
+        self.uniforms.uniform_(generator=self.generator)
+        return super().step()
+
+
 def count_parameters(config: HybridConfig) -> int:
     """Parameters of ``HybridDecoder(config)`` from the config alone (the closed form of
     reference ``compute_model_params``, ``model.py:433-501``, with the gdn2 mixer's
@@ -618,6 +704,7 @@ def count_parameters(config: HybridConfig) -> int:
     mlp = 3 * d * c.intermediate_size
     norms = 2 * d
     attn = d * (c.n_head + 2 * c.n_query_groups) * c.head_size + c.n_head * c.head_size * d
+    attn += 2 * c.head_size if c.qk_norm else 0
     gdn2 = (d * k_dim * 2 + d * v_dim                                      # q, k, v projections
             + ((2 * k_dim + v_dim) * c.conv_size if c.use_short_conv else 0)
             + d * hv + hv * k_dim                                          # f_proj
@@ -630,4 +717,4 @@ def count_parameters(config: HybridConfig) -> int:
 
 
 __all__ = ["Block", "CausalSelfAttention", "GreedyDecoder", "HybridConfig", "HybridDecoder",
-           "apply_rotary_emb", "build_rope_cache", "count_parameters"]
+           "SamplingDecoder", "apply_rotary_emb", "build_rope_cache", "count_parameters"]

@@ -294,3 +294,36 @@ def test_rope_backward_entry(lib, want, over):
     assert lib.gdn2_qkv_norm_rope_bwd(4096, 512, 512, nat.DTYPE_BF16, 4096, 4096, nat.DTYPE_BF16, 1e-5, 4096, 4096, 32, 9,
                                       None, 0, 0, a["dq"], a["dk"], a["dv"], a["dqkv"], a["dwq"], a["dwk"], 2, a["T"], 2, 2,
                                       64, a["ws"], a["nbytes"], None) == want
+
+
+# ---- the decoder host ----
+
+def test_hybrid_qk_norm_parameters():
+    from qwendopamine_amd.hybrid import HybridConfig, HybridDecoder, count_parameters
+
+    cfg = HybridConfig(n_layer=2, n_embd=64, n_head=2, head_size=32, n_query_groups=1, intermediate_size=64, vocab_size=50,
+                       gdn2_layers=[], qk_norm=True)
+    m = HybridDecoder(cfg)
+    assert sum(p.numel() for p in m.parameters()) == count_parameters(cfg)
+    assert {n.split(".", 2)[2] for n, _ in m.named_parameters() if "attn.q_norm" in n or "attn.k_norm" in n} == {
+        "attn.q_norm.weight", "attn.k_norm.weight"}
+    idx = torch.randint(0, 50, (2, 9), generator=torch.Generator().manual_seed(0))
+    scaled = HybridDecoder(cfg)
+    scaled.load_state_dict(m.state_dict())
+    with torch.no_grad():
+        for blk in scaled.h:  # normalised: the scale of queries and keys does not matter
+            at = blk.attn
+            rows = at.attn.weight.view(at.n_query_groups, at.n_head // at.n_query_groups + 2, at.head_size, -1)
+            rows[:, :-1] *= 8.0
+        assert torch.allclose(m(idx), scaled(idx), rtol=1e-3, atol=1e-3)
+
+
+def test_hybrid_paged_needs_the_gpu():
+    from qwendopamine_amd.hybrid import HybridConfig, HybridDecoder
+
+    m = HybridDecoder(HybridConfig(n_layer=1, n_embd=64, n_head=1, head_size=64, n_query_groups=1, intermediate_size=64,
+                                   vocab_size=50, gdn2_layers=[]))
+    with pytest.raises(NotImplementedError):
+        m.setup_caches(1, 32, page_size=16)
+    with pytest.raises(NotImplementedError):
+        m.setup_caches(1, 32, kv_bits=4, page_size=16)
