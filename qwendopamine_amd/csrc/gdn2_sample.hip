@@ -279,55 +279,108 @@ __global__ __launch_bounds__(kThreads) void sample_max_kernel(SampleParams p)
     }
 }
 
+// bf16 parts of some length: an exponential for each value that occurs instead of each element.  Values of the 16 octaves
+// up to the largest that counts are counted; the few nearer zero, and those of other types, take one each.
+// 256 x 151936: 27 us, one by one 71.
+constexpr int kCounters = 2 * 16 * 128, kCounted = 8192;
+
 template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_hist_kernel(SampleParams p)
 {
     constexpr int N = Logits<T>::N, U = 4;
+    constexpr bool kBf16 = std::is_same<T, bf16_t>::value;
     __shared__ u64 s_sum[kSampleBins];
     __shared__ unsigned s_count[kSampleBins];
+    __shared__ unsigned s_values[kBf16 ? kCounters : 1];
     __shared__ u64 s_part[kThreads / 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t row = blockIdx.x / p.parts;
     const int part = static_cast<int>(blockIdx.x - row * p.parts);
+    const Logits<T> x(p, row);
+    int lo, hi;
+    part_range(p, x.pieces, part, lo, hi);
+    float v[U][N];
+    auto fetch = [&](int c0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (c0 + u * kThreads < hi) x.load(c0 + u * kThreads, v[u]);
+    };
+    fetch(lo + tid);  // in flight while the row's settings are formed
     const RowState s = row_state(p, row, lane);
     if (s.greedy) return;
     const bool bins = filters(s), sums = !bins || binned_sums(s);
+    const bool counted = kBf16 && p.part_pieces * N >= kCounted;
     if (bins) {
         for (int i = tid; i < kSampleBins; i += kThreads) {
             s_sum[i] = 0;
             s_count[i] = 0;
         }
-        __syncthreads();
     }
-    const Logits<T> x(p, row);
-    int lo, hi;
-    part_range(p, x.pieces, part, lo, hi);
+    if (counted)
+        for (int i = tid; i < kCounters; i += kThreads) s_values[i] = 0;
+    if (bins || counted) __syncthreads();
     u64 sum = 0;
-    for (int c0 = lo + tid; c0 < hi; c0 += U * kThreads) {
-        float v[U][N];
+    // `n` elements of logit a.
+    auto add = [&](float a, unsigned n) __attribute__((always_inline)) {
+        const double y = log_weight(s, a);
+        if (!counts(y)) return;
+        u64 w = 0;
+        if (sums || s.least > 1) {
+            w = weight_of(y);
+            if (w < s.least) return;
+        }
+        if (bins) {
+            const int b = bin_of(s, y);
+            if (sums) atomicAdd(&s_sum[b], w * n);
+            if (s.k > 0) atomicAdd(&s_count[b], n);
+        } else {
+            sum += w * n;
+        }
+    };
+    if (counted) {
+        // No logit below `floor` counts; the largest magnitude of those that do.
+        const float floor = static_cast<float>(static_cast<double>(s.top) + 1.01 * static_cast<double>(kFloor) / s.per);
+        const unsigned most = __float_as_uint(fmaxf(fabsf(s.top), fabsf(floor))) >> 23;
+        const unsigned base = (most > 15 ? most - 15 : 0) << 7;
+        for (int c0 = lo + tid; c0 < hi; c0 += U * kThreads) {
+            unsigned mask = 0;
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (c0 + u * kThreads < hi) x.load(c0 + u * kThreads, v[u]);
+            for (int u = 0; u < U; ++u) {
+                if (c0 + u * kThreads >= hi) break;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (c0 + u * kThreads >= hi) break;
-#pragma unroll
-            for (int e = 0; e < N; ++e) {
-                const double y = log_weight(s, v[u][e]);
-                if (!counts(y)) continue;
-                u64 w = 0;
-                if (sums || s.least > 1) {
-                    w = weight_of(y);
-                    if (w < s.least) continue;
-                }
-                if (bins) {
-                    const int b = bin_of(s, y);
-                    if (sums) atomicAdd(&s_sum[b], w);
-                    if (s.k > 0) atomicAdd(&s_count[b], 1u);
-                } else {
-                    sum += w;
+                for (int e = 0; e < N; ++e) {
+                    const unsigned bits = __float_as_uint(v[u][e]) >> 16, at = (bits & 0x7fffu) - base;
+                    if (v[u][e] >= floor) {
+                        if (at < kCounters / 2)
+                            atomicAdd(&s_values[at + (bits >> 15) * (kCounters / 2)], 1u);
+                        else
+                            mask |= v[u][e] > -INFINITY ? 1u << (u * N + e) : 0u;
+                    }
                 }
             }
+            const int at = c0;
+            fetch(c0 + U * kThreads);
+            for (; mask; mask &= mask - 1) {
+                const int bit = __ffs(mask) - 1;
+                add(io<T>::ld(x.x, x.first(at + bit / N * kThreads) + bit % N), 1);
+            }
+        }
+        __syncthreads();
+        for (int i = tid; i < kCounters; i += kThreads) {
+            const unsigned n = s_values[i];
+            if (n == 0) continue;
+            const unsigned mag = (i & (kCounters / 2 - 1)) + base;
+            add(__uint_as_float((mag | (i >= kCounters / 2 ? 0x8000u : 0u)) << 16), n);
+        }
+    } else {
+        for (int c0 = lo + tid; c0 < hi; c0 += U * kThreads) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (c0 + u * kThreads >= hi) break;
+#pragma unroll
+                for (int e = 0; e < N; ++e) add(v[u][e], 1);
+            }
+            fetch(c0 + U * kThreads);
         }
     }
     if (!bins) {
@@ -442,25 +495,39 @@ __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleParams p)
     constexpr int N = Logits<T>::N, U = 4;
     __shared__ u64 s_part[kThreads / 64];
     __shared__ unsigned s_n;
+    __shared__ Borders s_borders;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t row = blockIdx.x / p.parts;
     const int part = static_cast<int>(blockIdx.x - row * p.parts);
+    const Logits<T> x(p, row);
+    int lo, hi;
+    part_range(p, x.pieces, part, lo, hi);
+    float v[U][N];
+    auto fetch = [&](int c0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (c0 + u * kThreads < hi) x.load(c0 + u * kThreads, v[u]);
+    };
+    fetch(lo + tid);  // in flight while the borders are found
     const RowState s = row_state(p, row, lane);
     if (s.greedy || !filters(s)) return;
-    const Borders b = borders_of(s, p.hist + row * (2 * kSampleBins), lane);
-    if (part == 0 && tid == 0) p.borders[row] = b;
+    if (wave == 0) {
+        const Borders found = borders_of(s, p.hist + row * (2 * kSampleBins), lane);
+        if (lane == 0) {
+            s_borders = found;
+            if (part == 0) p.borders[row] = found;
+        }
+    }
     // A list of each part's own (one for the row, and its number added to by every wave, took 40 us of 64 rows of 32000).
     u64 *list = p.list + (row * p.parts + part) * p.list_len;
     if (tid == 0) s_n = 0;
     __syncthreads();
+    const Borders b = s_borders;
     // What is kept for certain is summed from the part's own bins, or (few) with the listed bins' elements.
     const bool binned = binned_sums(s);
     const int need = b.p_hi > b.k_bin ? b.p_hi : b.k_bin;  // no bin past this one is wanted
     const float cut = edge_of<-1>(s, (need > b.sure - 1 ? need : b.sure - 1) + 1);
     const float high = binned ? edge_of<1>(s, b.sure) : INFINITY;
-    const Logits<T> x(p, row);
-    int lo, hi;
-    part_range(p, x.pieces, part, lo, hi);
     u64 sum = 0;
     if (binned) {
         const u64 *own = p.part_hist + (row * p.parts + part) * kSampleBins;
@@ -469,16 +536,13 @@ __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleParams p)
     for (int c0 = lo + tid; c0 < hi; c0 += U * kThreads) {
         // Which of the thread's elements may count, then those one after another, of all lanes together.
         unsigned mask = 0;
-        float v[U][N];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (c0 + u * kThreads < hi) x.load(c0 + u * kThreads, v[u]);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (c0 + u * kThreads >= hi) break;
 #pragma unroll
             for (int e = 0; e < N; ++e) mask |= v[u][e] >= cut && v[u][e] <= high && v[u][e] > -INFINITY ? 1u << (u * N + e) : 0u;
         }
+        fetch(c0 + U * kThreads);
         while (__ballot(mask != 0)) {
             const int bit = mask ? __ffs(mask) - 1 : 0;
             const int i = x.first(c0 + bit / N * kThreads) + bit % N;
