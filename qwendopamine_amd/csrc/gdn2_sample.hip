@@ -669,15 +669,45 @@ __global__ __launch_bounds__(kFinish) void sample_finish_kernel(SampleParams p)
         };
         // The last of the elements in bins lo .. hi with keys from `least` on before which there is
         // less than the target (`by_sum`: of sum, else of number), `sum0` and `count0` preceding them all.
-        // Digit by digit of the key, from the highest.  `sum0` becomes the sum up to and with it.
+        // By 8 bits of the key at a time, from the highest in which the elements differ (where they agree, all would
+        // meet in one counter).  `sum0` becomes the sum up to and with it.
         auto select = [&](bool by_sum, double target, int lo, int hi, u64 least, u64 &sum0, u64 count0) {
-            u64 prefix = 0;
-            for (int shift = Key<T>::bits - 8; shift >= 0; shift -= 8) {
+            u64 low = ~0ull, high = 0;
+            each([&](u64 key, u64, int bin) __attribute__((always_inline)) {
+                if (bin < lo || bin > hi || key < least) return;
+                low = key < low ? key : low;
+                high = key > high ? key : high;
+            });
+            __syncthreads();  // s_least is read
+            if (tid == 0) {
+                s_least[0] = ~0ull;
+                s_least[1] = 0;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const u64 a = shfl_xor64(low, o), b2 = shfl_xor64(high, o);
+                low = a < low ? a : low;
+                high = b2 > high ? b2 : high;
+            }
+            if (lane == 0 && high > 0) {
+                atomicMin(&s_least[0], low);
+                atomicMax(&s_least[1], high);
+            }
+            __syncthreads();
+            low = s_least[0];
+            high = s_least[1];
+            if (high == 0) return ~0ull;  // none
+            int known = low == high ? 8 : 64 - __clzll(static_cast<long long>(low ^ high));  // the bits from here on agree
+            known = known < 8 ? 8 : known;
+            u64 prefix = high >> known;
+            for (;;) {
+                const int shift = known > 8 ? known - 8 : 0;
                 __syncthreads();
                 if (tid < 256) s_sum[tid] = s_count[tid] = 0;
                 __syncthreads();
                 each([&](u64 key, u64 w, int bin) __attribute__((always_inline)) {
-                    if (bin < lo || bin > hi || key < least || (key >> shift) >> 8 != prefix) return;
+                    if (bin < lo || bin > hi || key < least || key >> known != prefix) return;
                     const int d = 255 - static_cast<int>((key >> shift) & 255);
                     atomicAdd(&s_sum[d], w);
                     atomicAdd(&s_count[d], 1ull);
@@ -723,7 +753,9 @@ __global__ __launch_bounds__(kFinish) void sample_finish_kernel(SampleParams p)
                 }
                 __syncthreads();
                 if (s_pick[0] == 256) return ~0ull;  // none
-                prefix = prefix << 8 | (255 - s_pick[0]);
+                // The digit's upper bits are known ones where fewer than 8 were left.
+                prefix = prefix << (known - shift) | ((255 - s_pick[0]) & ((1ull << (known - shift)) - 1));
+                known = shift;
                 sum0 = s_pick[1];
                 count0 = s_pick[2];
                 if (s_pick[3] == 1 || shift == 0) {
@@ -737,7 +769,6 @@ __global__ __launch_bounds__(kFinish) void sample_finish_kernel(SampleParams p)
                     return s_last;
                 }
             }
-            return prefix;  // not reached: keys differ
         };
         if (from_list && n <= static_cast<unsigned>(kPairs)) {
             // Every element against every other: how many of top-k's bin, and what sum of top-p's, lie before

@@ -228,8 +228,8 @@ class CausalSelfAttention(nn.Module):
         """q, k (normalised, rotated) and v ``[B, T, heads, D]`` of the fused projection; ``cos`` / ``sin`` the tokens' rows."""
         b, t, _ = qkv.shape
         G, qpk, D = self.n_query_groups, self.n_head // self.n_query_groups, self.head_size
-        if ((self.config.qk_norm or self.config.attention == "hip") and qkv.is_cuda and D % 8 == 0 and D <= 256
-                and qkv.dtype in (torch.bfloat16, torch.float16, torch.float32)):
+        fits = qkv.is_cuda and D % 8 == 0 and D <= 256 and qkv.dtype in (torch.bfloat16, torch.float16, torch.float32)
+        if (self.config.qk_norm and fits) or (self.config.attention == "hip" and ops.attention_supported(qkv, D)):
             # One pass; without norms the bits of the torch operations below.
             return ops.qkv_norm_rope(qkv, cos, sin, self.n_head, G, *self._norm_weights(), self.config.norm_eps)
         q, k, v = qkv.view(b, t, G, qpk + 2, D).split((qpk, 1, 1), dim=-2)

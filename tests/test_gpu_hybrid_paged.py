@@ -75,6 +75,8 @@ def test_greedy_and_drawn_tokens(gpu_device):
     prompt = _ids(gpu_device, 3, 20)
     greedy = GreedyDecoder(m, page_size=16).generate(prompt, 12)
     assert torch.equal(greedy, GreedyDecoder(m, use_graph=False, page_size=16).generate(prompt, 12))
+    # The contiguous cache, whose decode step has no norms of its own: torch operations around the pass.
+    assert torch.equal(GreedyDecoder(m).generate(prompt, 12), GreedyDecoder(m, use_graph=False).generate(prompt, 12))
 
     def drawn(seed, **kw):
         g = torch.Generator(gpu_device).manual_seed(seed)
