@@ -4,8 +4,8 @@
 //   o_t = sum_j p_tj v_j / sum_j p_tj,  p_tj = exp(scale q_t . k_j),  j <= pos + t
 //   k_j, v_j: row j mod S of page table[b][j / S], pages [P][G][S][D]
 //
-// v_mfma_f32_16x16x32, positions as rows and the rows of a group (its query heads of
-// every token) as columns, 16 C of them: a lane's 16 bytes of a key row are the A
+// Few rows (a group's query heads times the tokens): v_mfma_f32_16x16x32, positions as rows and
+// the rows of the group as columns, 16 C of them: a lane's 16 bytes of a key row are the A
 // operand as they lie in memory, so keys go from memory to the matrix units
 // without passing through LDS, and the scores come out with four positions of one
 // column per lane, which is the B operand of the value product.  Its A operand
@@ -216,6 +216,8 @@ __device__ __forceinline__ int64_t out_row(const AttnPagedParams &p, const Where
     return (static_cast<int64_t>(w.b) * p.T + t) * (p.G * p.R) + w.g * p.R + (x - t * p.R);
 }
 
+// 32 tokens over contexts spread to 32768, H32 G8 D128, pages of 16: 369 us, 5.8 TB/s of keys and values (a large copy 5.1,
+// equal contexts 6.1); 4 over 2074 of 2304, H16 D64: 13 us, four steps' latencies.
 // C column tiles hold all the T R rows of a group.  SPREAD: workgroup (worker, group) takes its run of all
 // sequences' rounds, and attn_paged_join_kernel joins the parts; else workgroup (b, group) one sequence.
 template <typename T, PrecKind PK, int D, int C, bool SPREAD>
@@ -251,7 +253,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_paged_kernel(AttnPagedPar
     if constexpr (SPREAD) hi = (from + left) * kRound < w.n ? (from + left) * kRound : w.n;
     if (lo >= hi) {
         if constexpr (SPREAD) {  // a sequence without keys: on to the next
-            ++b;
+            if (++b >= p.B) return;
             continue;
         }
         for (int e = tid; e < all * D; e += 64 * kWaves) io<T>::st(out, out_row(p, w, e / D) * D + e % D, 0.0f);
@@ -486,8 +488,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_paged_kernel(AttnPagedPar
     }
     if constexpr (!SPREAD) return;
     left -= (hi - lo + kRound - 1) / kRound;
-    if (left <= 0) return;
-    ++b;
+    if (left <= 0 || ++b >= p.B) return;
     from = 0;
     __syncthreads();  // the next part overwrites what was read
     }
@@ -603,6 +604,8 @@ __device__ __forceinline__ void stage_pages(const char *pool, unsigned rows, int
 #endif
 }
 
+// 2048 tokens over 16384, H32 G8 D128 causal: 496 us, 942 TFLOP/s (a large library product 1216); three pieces to 517 over
+// contexts to 9000, H16 G4 D128: 97 us in four shares, whose unequal ends leave CUs idle, and their join 13.
 // The products, statistics and layouts of the forward over whole sequences (gdn2_attn_train.hip), keys
 // and values by pages: a wave looks the pages of 16 tiles up at once.  Probabilities are rounded once
 // for their product, as there: off by 1.4 to 1.5 times the rounding of the result.
@@ -866,9 +869,9 @@ hipError_t paged_d(AttnPagedParams &p, hipStream_t s)
 
 }  // namespace
 
-// How a call is divided.  Rows of a workgroup: a group of up to 16 rows (D = 64: 32) has its keys go from memory to the matrix units, more
-// by tiles in LDS (20 rows over 4 x 16384 positions, G8 D128: 54 us, and 107 with two column tiles of registers, which spill; D = 64
-// 20 rows, G16: 57 and 48).
+// How a call is divided.  Rows of a workgroup: the keys of up to 16 rows (D = 64: 32) go from memory to the
+// matrix units, those of more by tiles in LDS (20 rows over 4 x 16384 positions, G8 D128: 54 us, and 107 with two
+// column tiles in registers, which spill; D = 64 20 rows, G16: 57 and 48).
 AttnPagedPlan attn_paged_plan(int B, int64_t T, int G, int R, int D, int64_t cap)
 {
     AttnPagedPlan a = {};
@@ -885,10 +888,11 @@ AttnPagedPlan attn_paged_plan(int B, int64_t T, int G, int R, int D, int64_t cap
         a.floats = a.splits == 1 ? 0 : static_cast<size_t>(a.splits) * groups * rows * (D + 2);
         return a;
     }
-    // One workgroup a sequence and group for short contexts (1024 positions, B1 G8 D128: 14 us, 17 by runs), and where there are
-    // many times more than the card holds; else runs, 512 workgroups in all: 32 contexts spread over 32768
-    // positions, G8 D128, 379 us (one a sequence 581), 64 over 4096 125 (152); of equal lengths the
-    // runs lose (32 of 4096: 105, 86), but lengths are not known here.  Fewer where little is to be done.
+    // One workgroup a sequence and group for short contexts (1024 positions, B1 G8 D128: 14 us, 17 by runs),
+    // and where there are many times more than the card holds; else runs, 512 workgroups in all: 32
+    // contexts spread over 32768 positions, G8 D128, 379 us (one a sequence 581), 64 over 4096 125 (152); of
+    // equal lengths the runs lose (32 of 4096: 105, 86), but lengths are not known here.  Fewer
+    // workgroups where little is to be done.
     const double rounds = static_cast<double>(B) * ((cap + kRound - 1) / kRound);
     if (cap > 1024 && groups < 4096 && rounds < 2.0e9) {
         const int64_t some = (256 + G - 1) / G, many = (512 + G - 1) / G, by_work = static_cast<int64_t>(rounds / 4);

