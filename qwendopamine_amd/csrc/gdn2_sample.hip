@@ -19,8 +19,8 @@
 //                  holds u times it, and the element within it
 // The logits are read once from memory and twice more from the caches behind the L2.  The passes
 // are bound by issue slots, of which a weight takes about 25: where an element can be told by its
-// logit alone not to count, none is formed.  256 x 151936 bf16, settings of each row: 15, 45, 30 and 32 us;
-// 4 x 151936: 3, 10, 8 and 9, chains of latencies; 64 x 32000 float32, top-p: 5, 12, 8 and 15.
+// logit alone not to count, none is formed.  256 x 151936 bf16, settings of each row: 15, 42, 30 and 32 us;
+// 4 x 151936: 4, 9, 8 and 9, chains of latencies; 64 x 32000 float32, top-p: 5, 10, 9 and 16.
 #include "gdn2_common.h"
 #include "gdn2_internal.h"
 
@@ -282,7 +282,7 @@ __global__ __launch_bounds__(kThreads) void sample_max_kernel(SampleParams p)
 
 // bf16 parts of some length: an exponential for each value that occurs instead of each element.  Values of the 16 octaves
 // up to the largest that counts are counted; the few nearer zero, and those of other types, take one each.
-// 256 x 151936, top-p: 45 us, one by one 71.
+// 256 x 151936, settings of each row: 42 us, one by one 64.
 constexpr int kCounters = 2 * 16 * 128, kCounted = 8192;
 
 template <typename T>
@@ -292,7 +292,7 @@ __global__ __launch_bounds__(kThreads) void sample_hist_kernel(SampleParams p)
     constexpr bool kBf16 = std::is_same<T, bf16_t>::value;
     __shared__ u64 s_sum[kSampleBins];
     __shared__ unsigned s_count[kSampleBins];
-    __shared__ unsigned s_values[kBf16 ? kCounters : 1];
+    __shared__ unsigned s_values[kBf16 ? kCounters + 64 : 1];
     __shared__ u64 s_part[kThreads / 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t row = blockIdx.x / p.parts;
@@ -342,7 +342,7 @@ __global__ __launch_bounds__(kThreads) void sample_hist_kernel(SampleParams p)
         // No logit below `floor` counts; the largest magnitude of those that do.
         const float floor = static_cast<float>(static_cast<double>(s.top) + 1.01 * static_cast<double>(kFloor) / s.per);
         const unsigned most = __float_as_uint(fmaxf(fabsf(s.top), fabsf(floor))) >> 23;
-        const unsigned base = (most > 15 ? most - 15 : 0) << 7;
+        const unsigned base = (most > 15 ? most - 15 : 0) << 7, none = kCounters + lane;
         for (int c0 = lo + tid; c0 < hi; c0 += U * kThreads) {
             unsigned mask = 0;
 #pragma unroll
@@ -350,13 +350,12 @@ __global__ __launch_bounds__(kThreads) void sample_hist_kernel(SampleParams p)
                 if (c0 + u * kThreads >= hi) break;
 #pragma unroll
                 for (int e = 0; e < N; ++e) {
+                    // Counters of no value, one a lane, take the others without a branch.
                     const unsigned bits = __float_as_uint(v[u][e]) >> 16, at = (bits & 0x7fffu) - base;
-                    if (v[u][e] >= floor) {
-                        if (at < kCounters / 2)
-                            atomicAdd(&s_values[at + (bits >> 15) * (kCounters / 2)], 1u);
-                        else
-                            mask |= v[u][e] > -INFINITY ? 1u << (u * N + e) : 0u;
-                    }
+                    const bool inside = at < kCounters / 2;
+                    atomicAdd(&s_values[inside ? at + (bits >> 15) * (kCounters / 2) : none], 1u);
+                    if (__any(!inside))
+                        mask |= !inside && v[u][e] >= floor && v[u][e] > -INFINITY ? 1u << (u * N + e) : 0u;
                 }
             }
             const int at = c0;
@@ -938,10 +937,10 @@ hipError_t sample_t(const SampleParams &p, hipStream_t s)
 
 }  // namespace
 
-// Parts of a row: enough workgroups for the card, none under 2048 elements, at most a wave's lanes.
+// Parts of a row: enough workgroups for the card, none under 4096 elements (4 x 151936: 30 us, of 2048 32), at most a wave's lanes.
 int sample_parts(int64_t rows, int64_t n)
 {
-    const int64_t most = (n + 2047) / 2048;
+    const int64_t most = (n + 4095) / 4096;
     int64_t c = (2048 + rows - 1) / rows;
     c = c < most ? c : most;
     return static_cast<int>(c < 1 ? 1 : (c > kSampleParts ? kSampleParts : c));

@@ -193,6 +193,31 @@ def test_many_rows(gpu_device):
     check(x[:50], u[:50], gpu_device, **kw)
 
 
+@pytest.mark.parametrize("kw", [{}, dict(temperature=0.7, top_p=0.95), dict(top_k=60, top_p=0.8), dict(min_p=0.02), dict(top_k=3000)],
+                         ids=str)
+def test_long_parts(gpu_device, kw):
+    """So many rows that each is a part of its own, long enough for bf16 values to be counted first: the tokens of
+    the same rows a hundred at a time, whose parts are shorter; and the definition's of the odd rows."""
+    rows, V = 2100, 9001
+    x, u = logits(rows, V, BF, 12)
+    x[0] = 0.0
+    x[1, ::2] = -float("inf")
+    x[2, 5:] = torch.finfo(BF).min
+    x[3] = x[3] + 300.0
+    x[4] = x[4] * 1e-4
+    x[5] = x[5] * 1e-30
+    x[6, 17] = float("nan")
+    x[7] = x[7] * 3000.0
+    x[8, 4500:] = -1e4
+    x[9] = -x[9].abs() - 50.0
+    x[10] = -float("inf")
+    got = ops.sample_tokens(x.to(gpu_device), u.to(gpu_device), **kw)
+    few = torch.cat([ops.sample_tokens(x[i:i + 100].to(gpu_device), u[i:i + 100].to(gpu_device), **kw)
+                     for i in range(0, rows, 100)])
+    assert torch.equal(got, few)
+    check(x[:12], u[:12], gpu_device, **kw)
+
+
 def test_largest_row(gpu_device):
     V = 1 << 20
     g = torch.Generator().manual_seed(10)
