@@ -281,6 +281,42 @@ def test_long_contexts(gpu_device, B, T, H, G, D, S, L, dt):
         assert torch.equal(o, ops.attention_paged(q, cache, pos))
 
 
+@pytest.mark.parametrize("T,H,G,D", [(1, 2, 1, 64), (4, 8, 4, 128), (5, 6, 1, 64)])
+def test_many_sequences(gpu_device, T, H, G, D):
+    """More sequences than a wave has lanes, in runs that begin and end within them: empty ones, padding, positions
+    outside, from one position to over a thousand."""
+    B, S, N = 150, 16, 70
+    g = torch.Generator().manual_seed(18)
+    P = 400
+    cache = make_cache(1, G, S, D, P - 3, BF, gpu_device, 19)._replace(
+        table=torch.randint(0, P, (B, N), generator=g).to(torch.int32).to(gpu_device))  # pages in common
+    assert ops.nat.load().gdn2_attn_paged_workspace_size(B, T, G, H // G, D, N * S) > 0
+    q = queries(B, T, H, D, BF, gpu_device, 8)
+    pos = torch.randint(-40, N * S + 40, (B,), generator=g)
+    pos[:9] = torch.tensor([0, N * S - 1, N * S - T, -1, N * S, 127, 128, 255, 1])
+    lengths = torch.randint(-1, T + 2, (B,), generator=g)
+    lengths[70:80] = 0
+    pos, lengths = pos.to(gpu_device), lengths.to(gpu_device)
+    check(ops.attention_paged(q, cache, pos, lengths), expected_attention(q, cache, pos, lengths))
+    none = ops.attention_paged(q, cache, torch.full_like(pos, -1), lengths)
+    assert (none == 0).all()
+
+
+def test_very_many_sequences(gpu_device):
+    """One workgroup for each where there are many times more than the card holds."""
+    B, T, H, G, D, S, N = 4200, 1, 2, 1, 64, 16, 70
+    g = torch.Generator().manual_seed(20)
+    cache = make_cache(1, G, S, D, 97, BF, gpu_device, 23)._replace(
+        table=torch.randint(0, 100, (B, N), generator=g).to(torch.int32).to(gpu_device))
+    assert ops.nat.load().gdn2_attn_paged_workspace_size(B, T, G, H // G, D, N * S) == 0
+    q = queries(B, T, H, D, BF, gpu_device, 9)
+    pos = torch.randint(0, N * S, (B,), generator=g).to(gpu_device)
+    o = ops.attention_paged(q, cache, pos)
+    for at in (0, 2000, 4180):
+        part = slice(at, at + 20)
+        check(o[part], expected_attention(q[part], cache._replace(table=cache.table[part]), pos[part]))
+
+
 def test_sharp_scores(gpu_device):
     """Scores far apart and far from zero: one key carries nearly all, references move late in the walk; and
     probabilities that underflow."""
