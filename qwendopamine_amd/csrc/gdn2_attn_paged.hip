@@ -115,7 +115,7 @@ __device__ __forceinline__ int tokens_of(const AttnPagedParams &p, int b, int &p
     int64_t t = p.T;
     if (p.lengths) {
         const int64_t l = p.lengths[b];
-        t = l < t ? l : t;
+        t = l < 0 ? 0 : l < t ? l : t;
     }
     if (at < 0 || at >= cap) {
         pos = 0;

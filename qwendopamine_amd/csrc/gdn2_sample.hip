@@ -7,8 +7,8 @@
 //
 // Weights are whole numbers, round(2^42 w): their sums do not depend on an order, so that
 // atomics and any split of a row give the same bits, and two passes that form the same
-// sum agree on every border.  An exponential in float64 costs no more issue slots than one
-// in float32 would save here.  Nothing is sorted.  Every filter keeps a run of the order
+// sum agree on every border.  They are formed in float64, as a running sum of a whole vocabulary has borders
+// that float32 would miss (a wrong token in a hundred rows).  Nothing is sorted.  Every filter keeps a run of the order
 // (logit, lower index), so all that is looked for is its last element:
 //   sample_max     each part's largest and least logit
 //   sample_hist    counts (top-k) and sums (top-p) of the kept by bins that are even in log w

@@ -109,6 +109,19 @@ def test_append_missing_pages_and_tables(gpu_device):
         assert torch.equal(a, b), name
 
 
+def test_append_lengths_past_32_bits(gpu_device):
+    B, T, H, G, D, S, N = 4, 3, 2, 2, 64, 16, 2
+    cache = make_cache(B, G, S, D, N, BF, gpu_device, 24)
+    qkv = torch.randn(B, T, (H + 2 * G) * D, generator=torch.Generator().manual_seed(25)).to(BF).to(gpu_device)
+    cos, sin = tables(N * S, 32, gpu_device)
+    lengths = torch.tensor([-2 ** 40 + 2, 2 ** 40, 2, -2 ** 62 + 3], device=gpu_device)
+    pos = torch.tensor([0, 5, 2 ** 33 + 1, 2], device=gpu_device)
+    want = expected_append(qkv, cos, sin, pos, cache, H, None, None, lengths.clamp(0, T))
+    q = ops.kv_cache_paged_append(qkv, cos, sin, pos, cache, H, lengths=lengths)
+    for name, a, b in zip("qkv", (q, cache.k, cache.v), want):
+        assert torch.equal(a, b), name
+
+
 def test_append_layouts(gpu_device):
     """Column ranges, one position for all, a table that is a column range, int32 lengths."""
     B, T, H, G, D, S, N = 2, 5, 4, 2, 64, 16, 3
@@ -296,6 +309,7 @@ def test_many_sequences(gpu_device, T, H, G, D):
     pos[:9] = torch.tensor([0, N * S - 1, N * S - T, -1, N * S, 127, 128, 255, 1])
     lengths = torch.randint(-1, T + 2, (B,), generator=g)
     lengths[70:80] = 0
+    lengths[5], lengths[100], lengths[101] = -2 ** 40 + 3, 2 ** 40 + 1, -2 ** 62 + 1  # past 32 bits
     pos, lengths = pos.to(gpu_device), lengths.to(gpu_device)
     check(ops.attention_paged(q, cache, pos, lengths), expected_attention(q, cache, pos, lengths))
     none = ops.attention_paged(q, cache, torch.full_like(pos, -1), lengths)
