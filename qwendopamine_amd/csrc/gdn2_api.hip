@@ -570,7 +570,9 @@ static int check_qkv_rope(QkvRopeParams &p, const void *qkv, int64_t stride_b, i
         return GDN2_ERR_UNSUPPORTED;
     p.qkv = qkv; p.stride_b = stride_b; p.stride_t = stride_t;
     p.wq = wq; p.wk = wk; p.w_f32 = w_dtype == GDN2_DTYPE_F32; p.eps = eps;
-    p.cos = cos; p.sin = sin; p.pairs = pairs; p.table_rows = table_rows;
+    // Tables of no rows hold no angles: no token has a position, and none is read (the backward reads a row for
+    // tokens without one, too).
+    p.cos = cos; p.sin = sin; p.pairs = table_rows > 0 ? pairs : 0; p.table_rows = table_rows;
     p.B = B; p.T = static_cast<int>(T); p.G = G; p.R = R; p.D = D;
     return GDN2_OK;
 }

@@ -346,3 +346,19 @@ def test_graph_and_stream(gpu_device):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want))
         torch.randn(1000, device=gpu_device).sum()
+
+
+@pytest.mark.parametrize("norm", [True, False])
+def test_tables_without_rows(gpu_device, norm):
+    """No token has a position: q and k are zeros, and no gradient passes but the values'."""
+    B, T, H, G, D = 2, 5, 4, 2, 64
+    qkv, wq, wk, d = inputs(B, T, H, G, D, BF, gpu_device, 30, norm)
+    cos = sin = torch.empty(0, 32, device=gpu_device)
+    pos = torch.tensor([0, 1, -1, 2 ** 40, 4], device=gpu_device)
+    leaves = [x.requires_grad_(True) for x in (qkv, wq, wk) if x is not None]
+    q, k, v = ops.qkv_norm_rope(qkv, cos, sin, H, G, wq, wk, EPS, pos)
+    grads = torch.autograd.grad((q, k, v), leaves, d)
+    rows = grads[0].view(B, T, G, H // G + 2, D)
+    assert (q == 0).all() and (k == 0).all() and torch.equal(v, qkv.view(rows.shape)[..., -1, :])
+    assert (rows[..., :-1, :] == 0).all() and torch.equal(rows[..., -1, :], d[2])
+    assert all((g == 0).all() for g in grads[1:])
