@@ -489,7 +489,8 @@ class HybridDecoder(nn.Module):
             raise NotImplementedError("a paged cache needs a bf16 or fp16 model on the GPU and heads of 64 or 128 channels")
         self.max_seq_length = max_seq_length
         table = None
-        n = 0 if page_size is not None else max_seq_length  # pages need no mask
+        # Attention over pages needs no mask; a model without attention layers selects its rows all the same.
+        n = 0 if page_size is not None and any(not blk.use_gdn2 for blk in self.h) else max_seq_length
         self.mask_cache = torch.tril(torch.ones(n, n, dtype=torch.bool, device=p.device))[None, None]
         self._rope_tables(max_seq_length, p.device)
         for blk in self.h:

@@ -327,3 +327,25 @@ def test_hybrid_paged_needs_the_gpu():
         m.setup_caches(1, 32, page_size=16)
     with pytest.raises(NotImplementedError):
         m.setup_caches(1, 32, kv_bits=4, page_size=16)
+
+
+def _cpu_decoder(monkeypatch, gdn2_layers):
+    """A decoder of two layers whose caches are set up as on the GPU and whose blocks pass their input on."""
+    from qwendopamine_amd import hybrid
+
+    m = hybrid.HybridDecoder(hybrid.HybridConfig(
+        n_layer=2, n_embd=64, n_head=1, head_size=64, n_query_groups=1, intermediate_size=64, vocab_size=50, block_size=32,
+        gdn2_layers=gdn2_layers)).to(BF)
+    monkeypatch.setattr(ops, "attention_paged_supported", lambda q, head_dim: True)
+    monkeypatch.setattr(hybrid.Block, "forward", lambda self, x, *args: x)
+    return m
+
+
+def test_hybrid_pages_without_attention_layers(monkeypatch):
+    """No layer reads the mask, yet its rows are selected: they have to be there."""
+    m = _cpu_decoder(monkeypatch, [0, 1])
+    idx = torch.arange(5)[None]
+    for page_size in (None, 16):
+        m.setup_caches(1, 20, page_size=page_size)
+        assert m(idx, input_pos=torch.arange(5)).shape == (1, 5, 50)
+        assert m(idx, input_pos=torch.arange(15, 20)).shape == (1, 5, 50)
