@@ -487,6 +487,8 @@ class HybridDecoder(nn.Module):
                                       "channels and at most 16 query heads per group")
         if page_size is not None and not ops.attention_paged_supported(p, c.head_size):
             raise NotImplementedError("a paged cache needs a bf16 or fp16 model on the GPU and heads of 64 or 128 channels")
+        if page_size is not None:
+            ops._check_page_size("setup_caches", page_size)  # before anything is replaced
         self.max_seq_length = max_seq_length
         table = None
         # Attention over pages needs no mask; a model without attention layers selects its rows all the same.

@@ -2030,12 +2030,16 @@ class KVCachePaged(NamedTuple):
     table: torch.Tensor
 
 
+def _check_page_size(name: str, page_size: int) -> None:
+    if page_size < 16 or page_size % 16 != 0:
+        raise NotImplementedError(f"{name}: pages of a multiple of 16 positions, got {page_size}")
+
+
 def kv_cache_paged(batch: int, groups: int, max_length: int, head_dim: int, page_size: int = 64, pages: int | None = None,
                    dtype: torch.dtype = torch.bfloat16, device=None) -> KVCachePaged:
     """A :class:`KVCachePaged` of zeros for ``max_length`` positions a sequence: every sequence with pages
     of its own, or with ``pages`` that many in all and none given out yet (``table`` -1)."""
-    if page_size < 16 or page_size % 16 != 0:
-        raise NotImplementedError(f"kv_cache_paged: pages of a multiple of 16 positions, got {page_size}")
+    _check_page_size("kv_cache_paged", page_size)
     n = (max_length + page_size - 1) // page_size
     if pages is None:
         table = torch.arange(batch * n, dtype=torch.int32, device=device).view(batch, n)

@@ -349,3 +349,14 @@ def test_hybrid_pages_without_attention_layers(monkeypatch):
         m.setup_caches(1, 20, page_size=page_size)
         assert m(idx, input_pos=torch.arange(5)).shape == (1, 5, 50)
         assert m(idx, input_pos=torch.arange(15, 20)).shape == (1, 5, 50)
+
+
+def test_hybrid_refused_pages_leave_the_caches(monkeypatch):
+    m = _cpu_decoder(monkeypatch, [0])
+    m.setup_caches(1, 20)
+    before = m.mask_cache, m.max_seq_length, m.h[1].attn.kv_cache
+    m.h[0].gdn2_cache = state = {}
+    for page_size in (8, 24, 0, -16):
+        with pytest.raises(NotImplementedError):
+            m.setup_caches(2, 40, page_size=page_size)
+    assert (m.mask_cache, m.max_seq_length, m.h[1].attn.kv_cache) == before and m.h[0].gdn2_cache is state
