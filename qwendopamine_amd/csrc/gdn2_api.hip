@@ -682,6 +682,13 @@ int gdn2_attn_paged(const void *q, const int64_t *strides, int io_dtype, const v
     if (st != GDN2_OK) return st;
     if (!attn_paged_supported(io_dtype, D) || !(scale > 0.0f) || scale > 1e30f) return GDN2_ERR_UNSUPPORTED;
     if (B == 0 || T == 0) return GDN2_OK;
+    // Rows of a group in 31 bits, and every launch within HIP's limits: a workgroup for each tile and share and then 1024 /
+    // D rows of the join, or (few rows) for each group, and with runs of the keys a row of the join.
+    if (static_cast<double>(T) * R > 1073741824.0 || G > 65535) return GDN2_ERR_UNSUPPORTED;
+    const AttnPagedPlan plan = attn_paged_plan(B, T, G, R, D, static_cast<int64_t>(page_size) * table_cols);
+    const double all_rows = static_cast<double>(B) * G * R * T, groups = static_cast<double>(B) * G;
+    const double join = plan.splits > 1 ? all_rows * D / 1024 + 1 : plan.workers > 0 ? all_rows : 0;
+    if (groups * plan.tiles * plan.splits > max_workgroups(256) || join > max_workgroups(256)) return GDN2_ERR_UNSUPPORTED;
     if (!q || !pos || !out || !aligned16(q, out, nullptr)) return GDN2_ERR_INVALID;
     const int64_t size[3] = {B, T, static_cast<int64_t>(G) * R};
     AttnPagedParams p = {};
@@ -689,16 +696,11 @@ int gdn2_attn_paged(const void *q, const int64_t *strides, int io_dtype, const v
         if (strides[i] < 0 || (size[i] > 1 && strides[i] % 8 != 0)) return GDN2_ERR_INVALID;
         p.qs[i] = strides[i];
     }
-    // Rows of a group in 31 bits, and what is launched within HIP's limits.
-    if (static_cast<double>(T) * R > 1073741824.0 || static_cast<double>(B) * G * R * T > static_cast<double>(max_workgroups(256)) ||
-        G > 65535)
-        return GDN2_ERR_UNSUPPORTED;
     p.q = q; p.k = k_pages; p.v = v_pages;
     p.table = table; p.table_stride = table_stride; p.pages = pages; p.page = page_size;
     p.cap = page_size * table_cols;
     p.pos = pos; p.pos_stride = pos_stride; p.lengths = lengths;
     p.out = out; p.B = B; p.T = static_cast<int>(T); p.G = G; p.R = R; p.D = D; p.scale = scale;
-    const AttnPagedPlan plan = attn_paged_plan(B, T, G, R, D, p.cap);
     p.rows = plan.rows; p.tiles = plan.tiles; p.splits = plan.splits; p.workers = plan.workers;
     p.part = static_cast<float *>(workspace);
     if (plan.floats > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) ||

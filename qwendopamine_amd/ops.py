@@ -2143,7 +2143,8 @@ def attention_paged(q: torch.Tensor, cache: KVCachePaged, input_pos: torch.Tenso
     must be finite.  ``scale`` is ``D**-0.5`` unless given (> 0).  Returns ``[B, T, H, D]``.  Scores and
     sums are float32; probabilities are multiplied in two parts of the io dtype, those of pieces with
     more than 16 rows (tokens times heads per group; heads of 64 channels: 32) rounded once, as in
-    :func:`attention`.  Inference only."""
+    :func:`attention`.  Up to 2^30 rows a group and 2^24 groups, or pieces of 128 rows of them.  Inference
+    only."""
     name = "attention_paged"
     B, G, D, cap = _check_paged(name, cache)
     if q.dim() != 4 or q.shape[0] != B or q.shape[3] != D or q.shape[2] < 1 or q.shape[2] % G != 0:

@@ -479,3 +479,22 @@ def test_two_streams_at_once(gpu_device):
     torch.cuda.synchronize()
     assert all(torch.equal(o, want[i]) for i in range(2) for o in got[i])
     assert math.isfinite(float(want[0].float().sum()))
+
+
+@pytest.mark.parametrize("B,T,H,N", [(512, 520, 64, 34), (1 << 20, 1, 17, 1)])
+def test_calls_of_many_rows(gpu_device, B, T, H, N):
+    """More rows than one launch holds workgroups, in tiles and of few rows a sequence: as in smaller calls, which give
+    every sequence its workgroups by the same rule."""
+    G, D, S = 1, 64, 16
+    assert B * T * H > 2 ** 24
+    g = torch.Generator().manual_seed(70)
+    cache = make_cache(1, G, S, D, 97, BF, gpu_device, 71)._replace(
+        table=torch.randint(0, 100, (B, N), generator=g).to(torch.int32).to(gpu_device))
+    q = queries(1, T, H, D, BF, gpu_device, 72).expand(B, T, H, D)
+    pos = torch.randint(0, N * S - T + 1, (B,), generator=g).to(gpu_device)
+    o = ops.attention_paged(q, cache, pos)
+    for at in range(0, B, B // 4):
+        part = slice(at, at + B // 4)
+        assert torch.equal(o[part], ops.attention_paged(q[part], cache._replace(table=cache.table[part]), pos[part]))
+    part = slice(B - 1, B)
+    check(o[part], expected_attention(q[part], cache._replace(table=cache.table[part]), pos[part]))

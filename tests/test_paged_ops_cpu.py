@@ -249,6 +249,20 @@ def test_attn_paged_entry(lib, want, over):
     assert _paged_call(lib, **over) == want
 
 
+@pytest.mark.parametrize("fits,over", [
+    (True, dict(B=32, T=16384, G=8, R=4, D=128)),             # more rows than HIP's workgroups, in tiles of 128
+    (True, dict(B=32, T=65535 * 128, G=8, R=1)),
+    (False, dict(B=32, T=65536 * 128, G=8, R=1)),
+    (True, dict(B=(1 << 24) - 1, T=1, G=1, R=32)),            # few rows: a workgroup for each group
+    (False, dict(B=1 << 24, T=1, G=1, R=32)),
+    (True, dict(B=1, T=(1 << 30) // 4, G=1, R=4)),
+    (False, dict(B=1, T=(1 << 30) // 4 + 1, G=1, R=4)),
+])
+def test_attn_paged_sizes(lib, fits, over):
+    """What is launched decides, not the rows; a call that fits goes on to its missing queries."""
+    assert _paged_call(lib, q=None, **over) == (nat.ERR_INVALID if fits else nat.ERR_UNSUPPORTED)
+
+
 @pytest.mark.parametrize("want,over", [
     (nat.ERR_INVALID, dict(dt=5)),
     (nat.ERR_INVALID, dict(rows=-1)),
