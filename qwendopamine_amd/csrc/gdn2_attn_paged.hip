@@ -893,12 +893,18 @@ AttnPagedPlan attn_paged_plan(int B, int64_t T, int G, int R, int D, int64_t cap
     // contexts spread over 32768 positions, G8 D128, 379 us (one a sequence 581), 64 over 4096 125 (152); of
     // equal lengths the runs lose (32 of 4096: 105, 86), but lengths are not known here.  Fewer
     // workgroups where little is to be done.
-    const double rounds = static_cast<double>(B) * ((cap + kRound - 1) / kRound);
+    const int64_t per = (cap + kRound - 1) / kRound;
+    const double rounds = static_cast<double>(B) * per;
     if (cap > 1024 && groups < 4096 && rounds < 2.0e9) {
         const int64_t some = (256 + G - 1) / G, many = (512 + G - 1) / G, by_work = static_cast<int64_t>(rounds / 4);
         const int64_t workers = by_work < some ? some : (by_work < many ? by_work : many);
-        a.workers = static_cast<int>(workers < kMaxWorkers ? workers : kMaxWorkers);
-        a.floats = static_cast<size_t>(a.workers + B) * G * rows * (D + 2);
+        const int64_t used = workers < kMaxWorkers ? workers : kMaxWorkers;
+        // A run's end is counted from the start of a sequence, past whose own end it may lie, in 31 bits.
+        const double end = per + rounds / used + kLeast;
+        if ((end < rounds ? end : rounds) * kRound < 2147483648.0) {
+            a.workers = static_cast<int>(used);
+            a.floats = static_cast<size_t>(a.workers + B) * G * rows * (D + 2);
+        }
     }
     return a;
 }

@@ -263,6 +263,20 @@ def test_attn_paged_sizes(lib, fits, over):
     assert _paged_call(lib, q=None, **over) == (nat.ERR_INVALID if fits else nat.ERR_UNSUPPORTED)
 
 
+@pytest.mark.parametrize("runs,B,G,L", [
+    (True, 2, 8, 32768),
+    (False, 2, 8, 1024),
+    (True, 100, 1, 1 << 30),
+    (True, 1, 600, 1 << 30),
+    (False, 2, 2000, 1 << 30),   # one run over both sequences would end at 2^31
+    (False, 7, 512, 1 << 30),
+    (False, 4000, 1, 1 << 30),
+])
+def test_attn_paged_runs_end_within_31_bits(lib, runs, B, G, L):
+    """One token over the longest contexts: a run of several sequences' positions is counted from its first sequence's."""
+    assert (lib.gdn2_attn_paged_workspace_size(B, 1, G, 1, 64, L) > 0) == runs
+
+
 @pytest.mark.parametrize("want,over", [
     (nat.ERR_INVALID, dict(dt=5)),
     (nat.ERR_INVALID, dict(rows=-1)),
