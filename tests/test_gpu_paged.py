@@ -498,3 +498,65 @@ def test_calls_of_many_rows(gpu_device, B, T, H, N):
         assert torch.equal(o[part], ops.attention_paged(q[part], cache._replace(table=cache.table[part]), pos[part]))
     part = slice(B - 1, B)
     check(o[part], expected_attention(q[part], cache._replace(table=cache.table[part]), pos[part]))
+
+
+def check_groups(o, q, cache, pos, groups):
+    """Some groups' heads of every sequence against float64."""
+    R = q.shape[2] // cache.k.shape[1]
+    for g in groups:
+        heads = slice(g * R, (g + 1) * R)
+        check(o[:, :, heads], expected_attention(q[:, :, heads], cache._replace(k=cache.k[:, g:g + 1], v=cache.v[:, g:g + 1]),
+                                                 pos))
+
+
+@pytest.mark.parametrize("dt", [BF, FP], ids=str)
+@pytest.mark.parametrize("G,D,S,T,shares", [(32, 64, 16, 40, 1), (32, 128, 64, 23, 1), (20, 64, 32, 40, 2)])
+def test_tiles_look_pages_up_again(gpu_device, G, D, S, T, shares, dt):
+    """A workgroup's walk over more than the 16 tiles whose pages are looked up at once: pages that are missing on either
+    side of each look-up, or all of one, and last positions there.  Queries are near keys on either side, so that each
+    of these carries a row."""
+    B, L, P = 16, 2560, 200
+    g = torch.Generator().manual_seed(50)
+    cache = make_cache(1, G, S, D, P - 3, dt, gpu_device, 51)._replace(
+        table=torch.randint(0, P, (B, L // S), generator=g).to(torch.int32).to(gpu_device))
+    nbytes = ops.nat.load().gdn2_attn_paged_workspace_size(B, T, G, 1, D, L)
+    assert nbytes == (0 if shares == 1 else 4 * shares * B * T * G * (D + 2))
+    table = cache.table
+    table[0, 1040 // S] = -1
+    table[1, 2100 // S] = P
+    table[2, 1008 // S] = table[2, 1024 // S] = -5
+    table[3, 1024 // S:2048 // S] = -1
+    table[4, :2304 // S] = -1
+    q = queries(B, T, G, D, dt, gpu_device, 52)
+    near = [(996, 1020, 1028, 1044, 1060, 2040, 2056, 2104, 2312)[t % 9] + t // 9 for t in range(T)]
+    some = slice(0, 9)
+    for b in range(9):
+        for t, j in enumerate(near):
+            p = page_of(cache, b, j)
+            if p is not None:
+                q[b, t] = 2 * cache.k[p, :, j % S]
+    pos = torch.full((B,), L - T, device=gpu_device)
+    pos[5], pos[6], pos[7], pos[8] = 1024 - T, 1025 - T, 1024, 2048 + 64 - T
+    o = ops.attention_paged(q, cache, pos)
+    check_groups(o[some], q[some], cache._replace(table=table[some]), pos[some], (0, G - 1))
+
+
+@pytest.mark.parametrize("dt", [BF, FP], ids=str)
+@pytest.mark.parametrize("R,D,T", [(2, 64, 1), (10, 64, 2), (4, 128, 2)])
+def test_runs_look_pages_up_again(gpu_device, R, D, T, dt):
+    """Runs of more than the 32 rounds of 128 positions whose pages are looked up at once, some over two sequences."""
+    B, G, S, L, P = 4, 64, 32, 20000, 80
+    N = L // S
+    g = torch.Generator().manual_seed(60)
+    cache = make_cache(1, G, S, D, P - 3, dt, gpu_device, 61)._replace(
+        table=torch.randint(0, P, (B, N), generator=g).to(torch.int32).to(gpu_device))
+    # 8 workgroups a group for all four sequences' 600 rounds.
+    assert ops.nat.load().gdn2_attn_paged_workspace_size(B, T, G, R, D, N * S) == 4 * (8 + B) * G * T * R * (D + 2)
+    table = cache.table
+    table[0, 4100 // S] = -1
+    table[0, 8192 // S] = P
+    table[1, 4090 // S] = table[1, 9000 // S] = -1
+    table[2, 4096 // S:12000 // S] = -1
+    q = queries(B, T, G * R, D, dt, gpu_device, 62)
+    pos = torch.tensor([N * S - T, 18000, N * S - T - 5, 19111], device=gpu_device)
+    check_groups(ops.attention_paged(q, cache, pos), q, cache, pos, (0, G - 1))
