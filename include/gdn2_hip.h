@@ -419,7 +419,7 @@ int gdn2_attn_paged(const void *q, const int64_t *strides, int io_dtype, const v
 
 /*
  * A token of each row of logits x [rows][n] (row r at (r / inner) outer_stride + (r % inner)
- * row_stride, any alignment; f32, bf16, fp16; n up to 2^20), drawn with the random number u[r] of
+ * row_stride, any alignment; f32, bf16, fp16; n up to 2^20, fewer than 2^22 rows), drawn with the random number u[r] of
  * [0, 1): of the weights w_j = exp((x_j - max x) / temperature) those are kept that are at least
  * min_p, of these the top_k largest (equal logits: the lower index first; 0: all), of these, in
  * that order, the shortest run whose sum reaches top_p of their sum (1: all); the token is

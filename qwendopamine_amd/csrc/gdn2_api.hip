@@ -729,7 +729,9 @@ int gdn2_sample_tokens(const void *x, int64_t inner, int64_t outer_stride, int64
     if (rows == 0) return GDN2_OK;
     const uintptr_t size = io_dtype == GDN2_DTYPE_F32 ? 4 : 2;
     if (!x || !u || !out || (reinterpret_cast<uintptr_t>(x) & (size - 1))) return GDN2_ERR_INVALID;
-    if (rows > max_workgroups(kSampleFinishThreads) || rows * kSampleParts > max_workgroups(256)) return GDN2_ERR_UNSUPPORTED;
+    // A workgroup for each part of a row, and one for the row.
+    if (rows > max_workgroups(kSampleFinishThreads) || rows * sample_parts(rows, n) > max_workgroups(256))
+        return GDN2_ERR_UNSUPPORTED;
     if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) ||
         workspace_bytes < gdn2_sample_tokens_workspace_size(rows, n))
         return GDN2_ERR_WORKSPACE;

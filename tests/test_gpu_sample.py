@@ -274,3 +274,15 @@ def test_refusals_on_the_device(gpu_device):
         ops.sample_tokens(x.to(gpu_device), u.to(gpu_device), top_p=torch.ones(1, device=gpu_device))
     with pytest.raises(ValueError):
         ops.sample_tokens(x.to(gpu_device), u.to(gpu_device), top_k=torch.ones(2, device=gpu_device))
+
+
+def test_many_rows(gpu_device):
+    """More rows than the largest number of parts would leave workgroups for: as in smaller calls."""
+    g = torch.Generator().manual_seed(90)
+    x, u = torch.randn(300001, 7, generator=g), torch.rand(300001, generator=g)
+    xd, ud = x.to(gpu_device), u.to(gpu_device)
+    got = ops.sample_tokens(xd, ud, temperature=0.9, top_k=4, top_p=0.95)
+    parts = [ops.sample_tokens(xd[i:i + 100000], ud[i:i + 100000], temperature=0.9, top_k=4, top_p=0.95)
+             for i in range(0, 300001, 100000)]
+    assert torch.equal(got, torch.cat(parts))
+    assert got[-300:].tolist() == [pick(x[i], u[i], T=0.9, k=4, p=0.95) for i in range(-300, 0)]

@@ -297,6 +297,9 @@ def test_attn_paged_runs_end_within_31_bits(lib, runs, B, G, L):
     (nat.ERR_WORKSPACE, dict(ws=4104)),
     (nat.ERR_WORKSPACE, dict(nbytes=100)),
     (nat.ERR_UNSUPPORTED, dict(rows=1 << 32)),
+    (nat.ERR_UNSUPPORTED, dict(rows=1 << 22)),
+    (nat.ERR_WORKSPACE, dict(rows=(1 << 22) - 1, ws=None)),
+    (nat.ERR_WORKSPACE, dict(rows=300000, n=1 << 20, ws=None)),
     (nat.OK, dict(rows=0)),
 ])
 def test_sample_entry(lib, want, over):
