@@ -2367,7 +2367,8 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature: flo
     with _on_device(dev):
         st = lib.gdn2_sample_tokens(
             x.data_ptr(), inner, so, sr, nat.dtype_code(x.dtype), rows, V, u.data_ptr(), nat.ptr(t), float(t_all),
-            nat.ptr(k), min(int(k_all), V), nat.ptr(p), float(p_all), nat.ptr(m), float(m_all), out.data_ptr(),
+            nat.ptr(k), min(int(k_all), V), nat.ptr(p), max(float(p_all), 2.0 ** -126), nat.ptr(m), float(m_all),
+            out.data_ptr(),
             nat.ptr(ws), nbytes, nat.stream_handle(dev))
     nat.check(st, name)
     return out

@@ -286,3 +286,13 @@ def test_many_rows(gpu_device):
              for i in range(0, 300001, 100000)]
     assert torch.equal(got, torch.cat(parts))
     assert got[-300:].tolist() == [pick(x[i], u[i], T=0.9, k=4, p=0.95) for i in range(-300, 0)]
+
+
+@pytest.mark.parametrize("p", [1e-30, 1e-40, 1e-46, 5e-324])
+def test_shares_under_float32(gpu_device, p):
+    """A share that is 0 in float32 keeps one token, given as a number or for each row."""
+    x, u = logits(9, 300, BF, 91)
+    want = [int((row == row.max()).nonzero()[0]) for row in x]
+    assert ops.sample_tokens(x.to(gpu_device), u.to(gpu_device), top_p=p).tolist() == want
+    each = torch.full((9,), p, device=gpu_device)
+    assert ops.sample_tokens(x.to(gpu_device), u.to(gpu_device), top_p=each).tolist() == want
