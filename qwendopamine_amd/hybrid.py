@@ -248,12 +248,12 @@ class CausalSelfAttention(nn.Module):
         b, t, _ = qkv.shape
         G, qpk, D = self.n_query_groups, self.n_head // self.n_query_groups, self.head_size
         if input_pos is not None and isinstance(self.kv_cache, ops.KVCachePaged):
-            if not _inference(qkv):
+            weights = self._norm_weights()
+            if not _inference(qkv, *weights):
                 raise NotImplementedError("a paged cache is written and read without gradients")
             # ``cos`` / ``sin`` are whole tables here (``HybridDecoder.forward``); positions are consecutive.
             start = input_pos[:1]
-            q = ops.kv_cache_paged_append(qkv, cos, sin, start, self.kv_cache, self.n_head, *self._norm_weights(),
-                                          self.config.norm_eps)
+            q = ops.kv_cache_paged_append(qkv, cos, sin, start, self.kv_cache, self.n_head, *weights, self.config.norm_eps)
             o = ops.attention_paged(q, self.kv_cache, start)
             return ops.linear(o.reshape(b, t, self.n_head * D), self.proj.weight, self.proj.bias)
         q4 = input_pos is not None and isinstance(self.kv_cache, ops.KVCacheQ4)

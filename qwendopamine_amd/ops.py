@@ -1537,6 +1537,12 @@ def _differentiated(*xs: torch.Tensor) -> bool:
         unpack_dual(x).tangent is not None for x in xs)
 
 
+def _no_derivatives(name: str, *xs: torch.Tensor | None) -> None:
+    """Refuses what an operator without a backward would pass for constant."""
+    if _differentiated(*(x for x in xs if x is not None)):
+        raise NotImplementedError(f"{name}: inference only; call it under torch.no_grad() or on detached tensors")
+
+
 def _head_rows(x: torch.Tensor) -> torch.Tensor:
     """``x [B, T, heads, D]`` as the attention kernels read it: in place where its channels are
     contiguous and every row starts on 16 bytes, else a contiguous copy."""
@@ -1890,8 +1896,8 @@ def _rope_tables(name: str, cos: torch.Tensor, sin: torch.Tensor, D: int) -> tup
         raise ValueError(f"{name}: cos and sin must be [rows, up to D / 2 pairs]; got {tuple(cos.shape)}, {tuple(sin.shape)}")
     if cos.dtype != torch.float32 or sin.dtype != torch.float32 or not (cos.is_contiguous() and sin.is_contiguous()):
         raise ValueError(f"{name}: rotation tables must be contiguous fp32")
-    if cos.requires_grad or sin.requires_grad:
-        raise ValueError(f"{name}: no gradient passes to the rotation tables")
+    if cos.requires_grad or sin.requires_grad or any(unpack_dual(x).tangent is not None for x in (cos, sin)):
+        raise ValueError(f"{name}: no derivative passes to the rotation tables")
     return cos.shape[1], cos.shape[0]
 
 
@@ -2096,7 +2102,7 @@ def kv_cache_paged_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tenso
     being padding.  ``cos`` / ``sin`` and the weights as in :func:`qkv_norm_rope`.  A token that is not
     there, or whose position lies outside the tables or the page table, gives zeros and is not
     stored; nor is one whose position has no page (its ``q`` is given).  Everything else in the
-    pages stays as it is.  Inference only."""
+    pages stays as it is.  Inference only: gradients and forward-mode tangents are refused."""
     name = "kv_cache_paged_append"
     B, G, D, _ = _check_paged(name, cache)
     x, b, T, R, d = _qkv_rows(name, qkv, n_head, G)
@@ -2107,6 +2113,7 @@ def kv_cache_paged_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tenso
     if input_pos is None:
         raise ValueError(f"{name}: input_pos is needed")
     n = _token_lengths(name, lengths, B)
+    _no_derivatives(name, qkv, q_weight, k_weight, cache.k, cache.v)
     _one_device(name, qkv, q_weight, k_weight, cos, sin, n, *cache)
     pos, pos_stride = _positions(name, "input_pos", input_pos, B, qkv.device)
     x, wq, wk = x.detach(), _aligned(q_weight), _aligned(k_weight)
@@ -2144,7 +2151,7 @@ def attention_paged(q: torch.Tensor, cache: KVCachePaged, input_pos: torch.Tenso
     sums are float32; probabilities are multiplied in two parts of the io dtype, those of pieces with
     more than 16 rows (tokens times heads per group; heads of 64 channels: 32) rounded once, as in
     :func:`attention`.  Up to 2^30 rows a group and 2^24 groups, or pieces of 128 rows of them.  Inference
-    only."""
+    only: gradients and forward-mode tangents are refused."""
     name = "attention_paged"
     B, G, D, cap = _check_paged(name, cache)
     if q.dim() != 4 or q.shape[0] != B or q.shape[3] != D or q.shape[2] < 1 or q.shape[2] % G != 0:
@@ -2159,6 +2166,7 @@ def attention_paged(q: torch.Tensor, cache: KVCachePaged, input_pos: torch.Tenso
     if input_pos is None:
         raise ValueError(f"{name}: input_pos is needed")
     n = _token_lengths(name, lengths, B)
+    _no_derivatives(name, q, cache.k, cache.v)
     _one_device(name, q, n, *cache)
     dev = q.device
     pos, pos_stride = _positions(name, "input_pos", input_pos, B, dev)

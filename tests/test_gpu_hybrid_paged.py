@@ -118,3 +118,16 @@ def test_refusals(gpu_device):
     m.setup_caches(1, 32, page_size=16)
     with pytest.raises(NotImplementedError):  # gradients
         m(_ids(gpu_device, 1, 5), input_pos=torch.arange(5, device=gpu_device))
+
+
+def test_norms_that_train_are_refused_over_pages(gpu_device):
+    """Over a frozen projection, too: a step through the pages would take their gradients for nothing."""
+    m = _model(BF, gpu_device, layers=(), qk_norm=True).requires_grad_(False)
+    m.setup_caches(1, 32, page_size=16)
+    idx, pos = _ids(gpu_device, 1, 5), torch.arange(5, device=gpu_device)
+    assert m(idx, input_pos=pos).shape == (1, 5, 1000)
+    m.h[1].attn.k_norm.weight.requires_grad_(True)
+    with pytest.raises(NotImplementedError):
+        m(idx, input_pos=pos)
+    with torch.no_grad():
+        assert m(idx, input_pos=pos).shape == (1, 5, 1000)

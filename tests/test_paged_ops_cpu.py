@@ -125,6 +125,49 @@ def test_attention_paged_refuses(err, args, kw):
         ops.attention_paged(*args, **{"input_pos": torch.zeros(1, dtype=torch.int64), **kw})
 
 
+@pytest.mark.parametrize("what", ["qkv", "q_weight", "k_weight", "k", "v"])
+@pytest.mark.parametrize("how", ["gradient", "tangent"])
+def test_append_refuses_derivatives(what, how):
+    """Instead of passing for constant; the check of devices, which CPU tensors do not pass, comes after it."""
+    def call(mark):
+        a = _append()
+        a["cache"] = a["cache"]._replace(**{what: mark(getattr(a["cache"], what))}) if what in "kv" else a["cache"]
+        a.update({} if what in "kv" else {what: mark(a[what])})
+        return ops.kv_cache_paged_append(**a)
+    _derivative(call, how)
+
+
+@pytest.mark.parametrize("what", ["q", "k", "v"])
+@pytest.mark.parametrize("how", ["gradient", "tangent"])
+def test_attention_paged_refuses_derivatives(what, how):
+    def call(mark):
+        q, cache = _q(), _cache()
+        if what == "q":
+            q = mark(q)
+        else:
+            cache = cache._replace(**{what: mark(getattr(cache, what))})
+        return ops.attention_paged(q, cache, torch.zeros(1, dtype=torch.int64))
+    _derivative(call, how)
+
+
+def _derivative(call, how):
+    if how == "gradient":
+        with pytest.raises(NotImplementedError):
+            call(lambda x: x.requires_grad_(True))
+        with torch.no_grad(), pytest.raises(RuntimeError, match="GPU"):
+            call(lambda x: x.requires_grad_(True))
+    else:
+        with torch.autograd.forward_ad.dual_level(), pytest.raises(NotImplementedError):
+            call(lambda x: torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)))
+
+
+def test_tangents_of_rotation_tables_are_refused():
+    with torch.autograd.forward_ad.dual_level():
+        cos = torch.autograd.forward_ad.make_dual(torch.zeros(9, 32), torch.ones(9, 32))
+        with pytest.raises(ValueError):
+            ops.qkv_norm_rope(**_rope(cos=cos))
+
+
 def test_paged_cache_constructor():
     c = ops.kv_cache_paged(3, 2, 100, 64, page_size=32)
     assert c.k.shape == (12, 2, 32, 64) and c.table.shape == (3, 4) and c.table.unique().numel() == 12
