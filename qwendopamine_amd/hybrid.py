@@ -229,7 +229,11 @@ class CausalSelfAttention(nn.Module):
         b, t, _ = qkv.shape
         G, qpk, D = self.n_query_groups, self.n_head // self.n_query_groups, self.head_size
         fits = qkv.is_cuda and D % 8 == 0 and D <= 256 and qkv.dtype in (torch.bfloat16, torch.float16, torch.float32)
-        if (self.config.qk_norm and fits) or (self.config.attention == "hip" and ops.attention_supported(qkv, D)):
+        # A caller's own tables may be of any type, layout and broadcast, and train.
+        plain = cos.shape == sin.shape == (t, cos.shape[-1]) and 2 * cos.shape[-1] <= D and all(
+            x.dtype == torch.float32 and x.is_contiguous() and not x.requires_grad for x in (cos, sin))
+        if plain and ((self.config.qk_norm and fits) or (
+                self.config.attention == "hip" and ops.attention_supported(qkv, D))):
             # One pass; without norms the bits of the torch operations below.
             return ops.qkv_norm_rope(qkv, cos, sin, self.n_head, G, *self._norm_weights(), self.config.norm_eps)
         q, k, v = qkv.view(b, t, G, qpk + 2, D).split((qpk, 1, 1), dim=-2)

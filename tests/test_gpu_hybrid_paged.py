@@ -6,7 +6,8 @@ import pytest
 import torch
 
 from qwendopamine_amd import ops
-from qwendopamine_amd.hybrid import GreedyDecoder, HybridConfig, HybridDecoder, SamplingDecoder
+from qwendopamine_amd.hybrid import (GreedyDecoder, HybridConfig, HybridDecoder, SamplingDecoder, apply_rotary_emb,
+                                     build_rope_cache)
 from tests._helpers import REL_TOL, rel_l2
 
 pytestmark = pytest.mark.gpu
@@ -131,3 +132,38 @@ def test_norms_that_train_are_refused_over_pages(gpu_device):
         m(idx, input_pos=pos)
     with torch.no_grad():
         assert m(idx, input_pos=pos).shape == (1, 5, 1000)
+
+
+@pytest.mark.parametrize("qk_norm", [False, True])
+@pytest.mark.parametrize("how", ["float32", "bfloat16", "float64", "strided", "trained", "one row"])
+def test_attention_layer_takes_tables_of_any_kind(gpu_device, how, qk_norm):
+    """By itself, with a caller's own rotation tables: queries and keys are the torch operations' on those tables."""
+    at = _model(BF, gpu_device, layers=(), qk_norm=qk_norm).h[0].attn
+    T, H, G, D = 9, at.n_head, at.n_query_groups, at.head_size
+    cos, sin = build_rope_cache(T, D, gpu_device)
+    if how in ("bfloat16", "float64"):
+        cos, sin = (x.to(getattr(torch, how)) for x in (cos, sin))
+    elif how == "strided":
+        cos, sin = (x.T.contiguous().T for x in (cos, sin))
+    elif how == "one row":
+        cos, sin = cos[3:4], sin[3:4]
+    elif how == "trained":
+        cos.requires_grad_(True)
+    x = torch.randn(2, T, 256, generator=torch.Generator().manual_seed(3)).to(BF).to(gpu_device)
+    qkv = at.attn(x)
+    q, k, v = at._heads(qkv, cos, sin)
+    wq, wk, wv = qkv.view(2, T, G, H // G + 2, D).split((H // G, 1, 1), dim=-2)
+    wq, wk = wq.reshape(2, T, H, D), wk.reshape(2, T, G, D)
+    if qk_norm:
+        wq, wk = at.q_norm(wq), at.k_norm(wk)
+    assert torch.equal(v, wv.reshape(2, T, G, D))
+    for got, want in ((q, apply_rotary_emb(wq, cos, sin)), (k, apply_rotary_emb(wk, cos, sin))):
+        if how == "float32" and qk_norm:
+            assert rel_l2(got, want) <= REL_TOL[BF]  # torch's norm rounds every operation
+        else:
+            assert torch.equal(got, want)
+    o = at(x, cos, sin)
+    assert o.shape == x.shape and o.isfinite().all()
+    if how == "trained":
+        (g,) = torch.autograd.grad(o.float().sum(), cos)
+        assert g.shape == cos.shape and g.isfinite().all() and (g != 0).any()
