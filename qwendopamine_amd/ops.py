@@ -2021,7 +2021,7 @@ def qkv_norm_rope(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, n_hea
     _one_device(name, qkv, q_weight, k_weight, cos, sin, pos)
     weights = [] if q_weight is None else [q_weight, k_weight]
     if _differentiated(qkv, *weights):
-        return QkvNormRopeFunction.apply(qkv, q_weight, k_weight, cos, sin, pos, n_head, n_query_groups, float(eps))
+        return QkvNormRopeFunction.apply(x, q_weight, k_weight, cos, sin, pos, n_head, n_query_groups, float(eps))
     return _qkv_norm_rope_fwd(x, _aligned(q_weight), _aligned(k_weight), cos, sin, pos, n_query_groups, R, D, float(eps))
 
 

@@ -362,3 +362,31 @@ def test_tables_without_rows(gpu_device, norm):
     assert (q == 0).all() and (k == 0).all() and torch.equal(v, qkv.view(rows.shape)[..., -1, :])
     assert (rows[..., :-1, :] == 0).all() and torch.equal(rows[..., -1, :], d[2])
     assert all((g == 0).all() for g in grads[1:])
+
+
+@pytest.mark.parametrize("how,copies", [("readable", 0), ("unaligned", 1), ("spread", 1)])
+def test_projection_is_copied_once(gpu_device, how, copies):
+    """In training, where it cannot be read in place; its gradient has its layout all the same."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    B, T, H, G, D = 2, 12, 4, 2, 64
+    W = (H + 2 * G) * D
+    qkv, wq, wk, d = inputs(B, T, H, G, D, BF, gpu_device, 31)
+    cos, sin = tables(T, 32, gpu_device)
+    base = torch.zeros(B, T, 2 * W, dtype=BF, device=gpu_device)
+    x = {"readable": base[..., :W], "unaligned": base[..., 3:3 + W], "spread": base[..., ::2]}[how]
+    x = x.copy_(qkv).detach().requires_grad_(True)
+    made = []
+
+    class Count(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            out = func(*args, **(kwargs or {}))
+            if func in (torch.ops.aten.clone.default, torch.ops.aten._to_copy.default, torch.ops.aten.copy_.default):
+                made.append(out.numel())
+            return out
+    with Count():
+        outs = ops.qkv_norm_rope(x, cos, sin, H, G, wq, wk)
+    assert made == [B * T * W] * copies
+    (g,) = torch.autograd.grad(outs, x, d)
+    check(dict(q=outs[0], k=outs[1], dqkv=g),
+          {n: r for n, r in reference(qkv, cos, sin, H, G, wq, wk, None, *d).items() if n in ("q", "k", "dqkv")})
