@@ -252,6 +252,9 @@ class CausalSelfAttention(nn.Module):
         b, t, _ = qkv.shape
         G, qpk, D = self.n_query_groups, self.n_head // self.n_query_groups, self.head_size
         if input_pos is not None and isinstance(self.kv_cache, ops.KVCachePaged):
+            room = self.kv_cache.table.shape[1] * self.kv_cache.k.shape[2]
+            if t > room:
+                raise ValueError(f"a prompt of {t} tokens does not fit a cache of {room}")
             weights = self._norm_weights()
             if not _inference(qkv, *weights):
                 raise NotImplementedError("a paged cache is written and read without gradients")

@@ -434,3 +434,15 @@ def test_hybrid_refused_pages_leave_the_caches(monkeypatch):
         with pytest.raises(NotImplementedError):
             m.setup_caches(2, 40, page_size=page_size)
     assert (m.mask_cache, m.max_seq_length, m.h[1].attn.kv_cache) == before and m.h[0].gdn2_cache is state
+
+
+def test_hybrid_prompt_longer_than_its_pages():
+    """Refused, as over the other caches: its last tokens would have no place and count as padding."""
+    from qwendopamine_amd.hybrid import CausalSelfAttention, HybridConfig
+
+    at = CausalSelfAttention(HybridConfig(n_layer=1, n_embd=64, n_head=1, head_size=64, n_query_groups=1, vocab_size=50), 0)
+    at.kv_cache = ops.kv_cache_paged(1, 1, 40, 64, page_size=16)
+    cos, sin = torch.zeros(64, 32), torch.zeros(64, 32)
+    for t, err in ((49, ValueError), (48, NotImplementedError)):  # (48 fit, and need the GPU)
+        with torch.no_grad(), pytest.raises(err):
+            at.forward_qkv(torch.zeros(1, t, 192), cos, sin, torch.arange(t))
