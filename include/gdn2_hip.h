@@ -402,6 +402,7 @@ int gdn2_qkv_norm_rope_bwd(const void *qkv, int64_t stride_b, int64_t stride_t, 
  * gdn2_attn_paged: q [B, T, G R, D] (batch, token and head strides in elements, multiples of 8)
  * over positions 0 .. pos + t of its sequence; out [B, T, G R, D].  Positions without a page are not
  * seen; a token that is not there, or outside the page table, or that sees nothing, gives zeros.
+ * Keys and values up to a sequence's last token must be finite; what lies past it is not read.
  * io_dtype bf16 / fp16, D 64 or 128; T R up to 2^30, G up to 65535, and fewer than 2^24 workgroups: one for every
  * 128 rows of a group, at least one each.  workspace: gdn2_attn_paged_workspace_size() bytes (positions =
  * page_size table_cols; may be 0), 16-byte aligned, of which concurrent calls need one each.

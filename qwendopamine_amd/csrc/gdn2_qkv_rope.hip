@@ -75,17 +75,6 @@ __device__ __forceinline__ void store8(T *p, const Row8 &r)
     }
 }
 
-// The raw bits of 8 channels, to be copied.
-template <typename T>
-struct Raw8 {
-    uint4 u[sizeof(T) / 2];
-};
-template <typename T>
-__device__ __forceinline__ void copy8(const T *from, T *to)
-{
-    *reinterpret_cast<Raw8<T> *>(to) = *reinterpret_cast<const Raw8<T> *>(from);
-}
-
 // Sum over the LPR lanes of a row.
 template <int LPR>
 __device__ __forceinline__ float row_sum(float x)

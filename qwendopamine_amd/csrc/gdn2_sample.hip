@@ -38,7 +38,7 @@ constexpr int kPairs = 256;  // listed elements that are compared each with each
 constexpr double kLog2e = 1.4426950408889634074;
 
 // 2^y in units of 2^-42 (at least 1), kFloor < y <= 0: 2^f by its series, |f| <= 1/2 (the first term left out is under
-// 6e-15 of it), rounded by the addition of 2^52.
+// 9e-15 of it), rounded by the addition of 2^52.
 __device__ __forceinline__ u64 weight_of(double y)
 {
     constexpr double c[12] = {1.0, 6.931471805599453094e-1, 2.402265069591007123e-1, 5.550410866482157995e-2,
@@ -59,7 +59,6 @@ __device__ __forceinline__ bool counts(double y) { return y > static_cast<double
 // index.  24 bits of index under 32 of the logit, of 16-bit logits 16.
 template <typename T>
 struct Key {
-    static constexpr int bits = sizeof(T) == 4 ? 56 : 40;
     static __device__ __forceinline__ u64 of(float v, int i)
     {
         const unsigned b = __float_as_uint(v + 0.0f);

@@ -2146,12 +2146,13 @@ def attention_paged(q: torch.Tensor, cache: KVCachePaged, input_pos: torch.Tenso
     ``G``; strides as :func:`attention`), ``input_pos`` and ``lengths`` as in :func:`kv_cache_paged_append`.
     Token ``t`` of sequence ``b`` sees positions ``0 .. input_pos[b] + t`` that have a page; a token that is not
     there, lies outside the page table or sees nothing gives zeros.  What lies in a page past a
-    sequence's last token is not read; keys and values hidden from some of a piece's tokens only
-    must be finite.  ``scale`` is ``D**-0.5`` unless given (> 0).  Returns ``[B, T, H, D]``.  Scores and
-    sums are float32; probabilities are multiplied in two parts of the io dtype, those of pieces with
-    more than 16 rows (tokens times heads per group; heads of 64 channels: 32) rounded once, as in
-    :func:`attention`.  Up to 2^30 rows a group and 2^24 groups, or pieces of 128 rows of them.  Inference
-    only: gradients and forward-mode tangents are refused."""
+    sequence's last token is not read; keys and values that any token of a sequence sees must be
+    finite (an infinite value may give NaN, also to tokens that do not see it).  ``scale`` is ``D**-0.5``
+    unless given (> 0).  Returns ``[B, T, H, D]``.  Scores and sums are float32; probabilities are
+    multiplied in two parts of the io dtype, those of pieces with more than 16 rows (tokens times heads
+    per group; heads of 64 channels: 32) rounded once, as in :func:`attention`.  Up to 2^30 rows a group
+    and 2^24 groups, or pieces of 128 rows of them.  Inference only: gradients and forward-mode tangents
+    are refused."""
     name = "attention_paged"
     B, G, D, cap = _check_paged(name, cache)
     if q.dim() != 4 or q.shape[0] != B or q.shape[3] != D or q.shape[2] < 1 or q.shape[2] % G != 0:
