@@ -1530,16 +1530,19 @@ def _on_device(device: torch.device):
     return torch.cuda.device(device)
 
 
-def _differentiated(*xs: torch.Tensor) -> bool:
+def _differentiated(*xs: torch.Tensor | None) -> bool:
     """Whether a derivative is asked for: a gradient, or a forward-mode tangent, which the autograd
     functions refuse (called past them, an operator would drop it and pass for constant)."""
-    return (torch.is_grad_enabled() and any(x.requires_grad for x in xs)) or any(
-        unpack_dual(x).tangent is not None for x in xs)
+    grad = torch.is_grad_enabled()
+    for x in xs:
+        if x is not None and ((grad and x.requires_grad) or unpack_dual(x).tangent is not None):
+            return True
+    return False
 
 
 def _no_derivatives(name: str, *xs: torch.Tensor | None) -> None:
     """Refuses what an operator without a backward would pass for constant."""
-    if _differentiated(*(x for x in xs if x is not None)):
+    if _differentiated(*xs):
         raise NotImplementedError(f"{name}: inference only; call it under torch.no_grad() or on detached tensors")
 
 
