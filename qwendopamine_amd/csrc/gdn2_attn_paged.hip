@@ -216,8 +216,8 @@ __device__ __forceinline__ int64_t out_row(const AttnPagedParams &p, const Where
     return (static_cast<int64_t>(w.b) * p.T + t) * (p.G * p.R) + w.g * p.R + (x - t * p.R);
 }
 
-// 32 tokens over contexts spread to 32768, H32 G8 D128, pages of 16: 369 us, 5.8 TB/s of keys and values (a large copy 5.1,
-// equal contexts 6.1); 4 over 2074 of 2304, H16 D64: 13 us, four steps' latencies.
+// 32 tokens over contexts spread to 32768, H32 G8 D128, pages of 16: 370 us, 5.8 TB/s of keys and values (a large copy 5.2,
+// equal contexts 6.1), and the join 7; 4 over 2074 of 2304, H16 D64: 13 us, four steps' latencies.
 // C column tiles hold all the T R rows of a group.  SPREAD: workgroup (worker, group) takes its run of all
 // sequences' rounds, and attn_paged_join_kernel joins the parts; else workgroup (b, group) one sequence.
 template <typename T, PrecKind PK, int D, int C, bool SPREAD>
@@ -604,8 +604,8 @@ __device__ __forceinline__ void stage_pages(const char *pool, unsigned rows, int
 #endif
 }
 
-// 2048 tokens over 16384, H32 G8 D128 causal: 496 us, 942 TFLOP/s (a large library product 1216); three pieces to 517 over
-// contexts to 9000, H16 G4 D128: 97 us in four shares, whose unequal ends leave CUs idle, and their join 13.
+// 2048 tokens over 16384, H32 G8 D128 causal: 504 us, 930 TFLOP/s (a large library product 1216); three pieces to 517 over
+// contexts to 9000, H16 G4 D128: 78 us in four shares, whose unequal ends leave CUs idle, and their join 11.
 // The products, statistics and layouts of the forward over whole sequences (gdn2_attn_train.hip), keys
 // and values by pages: a wave looks the pages of 16 tiles up at once.  Probabilities are rounded once
 // for their product, as there: off by 1.4 to 1.5 times the rounding of the result.
@@ -890,7 +890,7 @@ AttnPagedPlan attn_paged_plan(int B, int64_t T, int G, int R, int D, int64_t cap
     }
     // One workgroup a sequence and group for short contexts (1024 positions, B1 G8 D128: 14 us, 17 by runs),
     // and where there are many times more than the card holds; else runs, 512 workgroups in all: 32
-    // contexts spread over 32768 positions, G8 D128, 379 us (one a sequence 581), 64 over 4096 125 (152); of
+    // contexts spread over 32768 positions, G8 D128, 377 us (one a sequence 581), 64 over 4096 125 (152); of
     // equal lengths the runs lose (32 of 4096: 105, 86), but lengths are not known here.  Fewer
     // workgroups where little is to be done.
     const int64_t per = (cap + kRound - 1) / kRound;

@@ -12,16 +12,16 @@
 // token, all requested before the first is used, and the token's angles once for
 // all of them.  Nothing is kept for the backward but the projection itself: r costs
 // one mean, and reading it back would cost more than forming it.  Both directions
-// are bound by memory: 16384 tokens H32 G8 D128 without norms 63 us, 5.3 TB/s; B4 T2048 H16 G16 D64 with norms
-// 17 us forward (4.0) and 30 backward (4.5), its weights' sum 4; into pages 22 (3.7).
+// are bound by memory: 16384 tokens H32 G8 D128 without norms 62 us, 5.5 TB/s (float32 150); B4 T2048 H16 G16
+// D64 with norms 16 us forward (4.2 TB/s) and 28 backward (4.8), its weights' sum 4; into pages 22 (3.8).
 #include "gdn2_common.h"
 #include "gdn2_internal.h"
 
 namespace gdn2 {
 namespace {
 
-// U: rows in flight per lane.  The backward holds two tensors' rows and the weights' sums: with 2 it is 30 us at
-// B4 T2048 H16 G16 D64 and 28 at T7013 H16 G4 D128, with 4, at fewer waves, 38 and 36.
+// U: rows in flight per lane.  The backward holds two tensors' rows and the weights' sums: with 2 it is 28 us at
+// B4 T2048 H16 G16 D64 and 26 at T7013 H16 G4 D128, with 4, at fewer waves, 38 and 36.
 constexpr int kRowsFwd = 4, kRowsBwd = 2;
 
 struct Row8 {

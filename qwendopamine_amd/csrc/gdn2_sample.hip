@@ -19,8 +19,8 @@
 //                  holds u times it, and the element within it
 // The logits are read once from memory and twice more from the caches behind the L2.  The passes
 // are bound by issue slots, of which a weight takes about 25: where an element can be told by its
-// logit alone not to count, none is formed.  256 x 151936 bf16, settings of each row: 15, 42, 30 and 32 us;
-// 4 x 151936: 4, 9, 8 and 9, chains of latencies; 64 x 32000 float32, top-p: 5, 10, 9 and 16.
+// logit alone not to count, none is formed.  256 x 151936 bf16, settings of each row: 15, 40, 30 and 31 us (fp16 16,
+// 61, 30 and 30); 4 x 151936: 4, 9, 8 and 9, chains of latencies; 64 x 32000 float32, top-p: 5, 9, 8 and 16.
 #include "gdn2_common.h"
 #include "gdn2_internal.h"
 
@@ -281,7 +281,7 @@ __global__ __launch_bounds__(kThreads) void sample_max_kernel(SampleParams p)
 
 // bf16 parts of some length: an exponential for each value that occurs instead of each element.  Values of the 16 octaves
 // up to the largest that counts are counted; the few nearer zero, and those of other types, take one each.
-// 256 x 151936, settings of each row: 42 us, one by one 64.
+// 256 x 151936, settings of each row: 40 us, one by one 64 (fp16, always one by one: 61).
 constexpr int kCounters = 2 * 16 * 128, kCounted = 8192;
 
 template <typename T>
