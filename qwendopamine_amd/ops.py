@@ -2333,8 +2333,8 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature: flo
     that follows reference ``GPT.forward``, ``gdn2_gpt/model.py:304-380``, beside :func:`argmax_rows`).
 
     ``logits`` ``[..., V]`` (bf16, fp16 or float32; ``V`` up to 2^20, fewer than 2^22 rows; strides as
-    :func:`token_logprobs`), ``uniforms`` float32 ``[...]``; settings are numbers for all rows or tensors ``[...]`` on the device with one for
-    each.  Returns int64 ``[...]``.
+    :func:`token_logprobs`), ``uniforms`` float32 ``[...]``; settings are numbers for all rows or tensors
+    ``[...]`` on the device with one for each.  Returns int64 ``[...]``.
 
     With weights ``w_j = exp((x_j - max x) / temperature)``, those are kept that are at least ``min_p``, of
     these the ``top_k`` largest (equal logits: the lower index first; 0: all), of these, in that

@@ -6,8 +6,8 @@ import pytest
 import torch
 
 from qwendopamine_amd import ops
-from qwendopamine_amd.hybrid import (GreedyDecoder, HybridConfig, HybridDecoder, SamplingDecoder, apply_rotary_emb,
-                                     build_rope_cache)
+from qwendopamine_amd.hybrid import GreedyDecoder, HybridConfig, HybridDecoder, SamplingDecoder
+from qwendopamine_amd.hybrid import apply_rotary_emb, build_rope_cache
 from tests._helpers import REL_TOL, rel_l2
 
 pytestmark = pytest.mark.gpu

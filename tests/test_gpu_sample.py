@@ -276,7 +276,7 @@ def test_refusals_on_the_device(gpu_device):
         ops.sample_tokens(x.to(gpu_device), u.to(gpu_device), top_k=torch.ones(2, device=gpu_device))
 
 
-def test_many_rows(gpu_device):
+def test_rows_past_a_quarter_million(gpu_device):
     """More rows than the largest number of parts would leave workgroups for: as in smaller calls."""
     g = torch.Generator().manual_seed(90)
     x, u = torch.randn(300001, 7, generator=g), torch.rand(300001, generator=g)
@@ -296,3 +296,22 @@ def test_shares_under_float32(gpu_device, p):
     assert ops.sample_tokens(x.to(gpu_device), u.to(gpu_device), top_p=p).tolist() == want
     each = torch.full((9,), p, device=gpu_device)
     assert ops.sample_tokens(x.to(gpu_device), u.to(gpu_device), top_p=each).tolist() == want
+
+
+@pytest.mark.parametrize("kw", [{}, dict(top_p=0.7), dict(top_k=9), dict(top_k=1500, top_p=0.5), dict(min_p=1.0), dict(min_p=0.3)],
+                         ids=str)
+@pytest.mark.parametrize("dt", [BF, FP, F32], ids=str)
+def test_largest_temperatures(gpu_device, kw, dt):
+    """All weights are 1, in the order of the logits; an infinite temperature of a row counts as the largest."""
+    x, u = logits(8, 4000, dt, 92)
+    x[1, ::3] = -float("inf")
+    x[2] = -float("inf")
+    x[3, 1:] = -float("inf")
+    x[4] = torch.finfo(dt).min
+    x[4, 77] = torch.finfo(dt).max / 2
+    want = [pick(x[i], u[i], T=3e38, **{dict(top_k="k", top_p="p", min_p="m")[n]: v for n, v in kw.items()}) for i in range(8)]
+    for t in (3e38, torch.full((8,), 3e38, device=gpu_device), torch.full((8,), float("inf"), device=gpu_device)):
+        got = ops.sample_tokens(x.to(gpu_device), u.to(gpu_device), temperature=t, **kw).tolist()
+        for i in range(8):
+            if i != 4 or not isinstance(t, torch.Tensor) or bool(t[4].isfinite()):  # (there a span of the type's counts)
+                assert got[i] == want[i], i
