@@ -203,7 +203,8 @@ class CausalSelfAttention(nn.Module):
     within its own tokens (causal SDPA, flash or memory-efficient kernels only, or
     ``ops.attention``: ``HybridConfig.attention``) and stores k, v. A single-token
     call attends over the cache up to its position; its products are issued with
-    contiguous right operands."""
+    contiguous right operands. Over pages every call takes whole rotation tables, and its tokens, at
+    consecutive positions, attend to all that the pages hold up to them."""
 
     def __init__(self, config: HybridConfig, layer_idx: int) -> None:
         super().__init__()

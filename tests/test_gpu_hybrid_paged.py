@@ -167,3 +167,22 @@ def test_attention_layer_takes_tables_of_any_kind(gpu_device, how, qk_norm):
     if how == "trained":
         (g,) = torch.autograd.grad(o.float().sum(), cos)
         assert g.shape == cos.shape and g.isfinite().all() and (g != 0).any()
+
+
+def test_prompt_in_pieces(gpu_device):
+    """A prompt in pieces and then single tokens through attention layers over pages (gdn2 layers begin their short
+    convolutions anew in every call of several tokens, as the reference's do): as near the weights in float32 as one
+    bf16 forward over the whole sequence (a quarter more for the roundings' chance)."""
+    m = _model(BF, gpu_device, layers=(), qk_norm=True)
+    full = _model(F32, gpu_device, layers=(), qk_norm=True)
+    full.load_state_dict(m.state_dict())
+    idx = _ids(gpu_device, 2, 70)
+    with torch.no_grad():
+        whole = full(idx)
+        base = rel_l2(m(idx), whole)
+        m.setup_caches(2, 80, page_size=16)
+        out, at = [], 0
+        for n in (30, 1, 25, 13, 1):
+            out.append(m(idx[:, at:at + n], input_pos=torch.arange(at, at + n, device=gpu_device)))
+            at += n
+    assert rel_l2(torch.cat(out, 1), whole) <= 1.25 * base

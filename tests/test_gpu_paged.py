@@ -560,3 +560,88 @@ def test_runs_look_pages_up_again(gpu_device, R, D, T, dt):
     q = queries(B, T, G * R, D, dt, gpu_device, 62)
     pos = torch.tensor([N * S - T, 18000, N * S - T - 5, 19111], device=gpu_device)
     check_groups(ops.attention_paged(q, cache, pos), q, cache, pos, (0, G - 1))
+
+
+@pytest.mark.parametrize("T,H,G,D", [(40, 4, 2, 64), (150, 8, 1, 128), (3, 8, 2, 128)])
+def test_captured_pieces(gpu_device, T, H, G, D):
+    """A padded piece of every sequence captured once (in tiles and their shares, or few rows in runs) and replayed as
+    positions, lengths and page numbers change, with eager work between the replays."""
+    B, S, N = 3, 16, 150
+    g = torch.Generator().manual_seed(80)
+    cos, sin = tables(N * S, D // 2, gpu_device)
+    a, b = (make_cache(B, G, S, D, N, BF, gpu_device, 81) for _ in range(2))
+    assert ops.nat.load().gdn2_attn_paged_workspace_size(B, T, G, H // G, D, N * S) > 0
+    steps = []
+    for i in range(4):
+        n = torch.randint(0, T + 1, (B,), generator=g, dtype=torch.int32)
+        pos = torch.randint(0, N * S - T, (B,), generator=g)
+        table = a.table.clone()
+        if i == 2:
+            table[0, 3], table[1] = -1, table[1].flip(0)
+        steps.append((torch.randn(B, T, (H + 2 * G) * D, generator=g).to(BF).to(gpu_device), pos.to(gpu_device),
+                      n.to(gpu_device), table))
+
+    def run(cache, x, pos, n):
+        q = ops.kv_cache_paged_append(x, cos, sin, pos, cache, H, lengths=n)
+        return ops.attention_paged(q, cache, pos, n)
+    want = [run(a._replace(table=t), x, pos, n).clone() for x, pos, n, t in steps]
+    torch.cuda.synchronize()
+    static = [x.clone() for x in steps[0]]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(b._replace(table=static[3]), *static[:3])
+    for w, step in zip(want, steps):
+        for to, x in zip(static, step):
+            to.copy_(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, w)
+        torch.randn(1000, device=gpu_device).sum()
+    assert torch.equal(a.k, b.k) and torch.equal(a.v, b.v)
+
+
+def test_append_float32_weights_and_tables_of_any_alignment(gpu_device):
+    B, T, H, G, D, S, N = 2, 9, 4, 2, 64, 16, 2
+    g = torch.Generator().manual_seed(85)
+    qkv = torch.randn(B, T, (H + 2 * G) * D, generator=g).to(FP).to(gpu_device)
+    wq, wk = ((1 + 0.2 * torch.randn(D + 1, generator=g)).to(gpu_device)[1:] for _ in range(2))
+    cos, sin = tables(N * S, 32, gpu_device)
+    pos = torch.tensor([20, 3], device=gpu_device)
+    cache = make_cache(B, G, S, D, N, FP, gpu_device, 86)
+    want = expected_append(qkv, cos, sin, pos, cache, H, wq, wk, None)
+    odd = [torch.zeros(N * S * 32 + 1, device=gpu_device)[1:].view(N * S, 32).copy_(x) for x in (cos, sin)]
+    assert odd[0].data_ptr() % 16 != 0
+    q = ops.kv_cache_paged_append(qkv, *odd, pos, cache, H, wq, wk)
+    for name, a, b in zip("qkv", (q, cache.k, cache.v), want):
+        assert torch.equal(a, b), name
+
+
+def test_no_sequences_no_tokens_and_inference_mode(gpu_device):
+    H, G, D, S, N = 4, 2, 64, 16, 3
+    cos, sin = tables(N * S, 32, gpu_device)
+    for B, T in ((0, 3), (2, 0)):
+        cache = make_cache(2, G, S, D, N, BF, gpu_device, 87)
+        cache = cache._replace(table=cache.table[:B])
+        before = cache.k.clone(), cache.v.clone()
+        pos = torch.zeros(1, dtype=torch.int64, device=gpu_device)
+        q = ops.kv_cache_paged_append(torch.zeros(B, T, (H + 2 * G) * D, dtype=BF, device=gpu_device), cos, sin, pos, cache, H)
+        assert q.shape == (B, T, H, D) and ops.attention_paged(q, cache, pos).shape == (B, T, H, D)
+        assert torch.equal(cache.k, before[0]) and torch.equal(cache.v, before[1])
+    cache, pos = make_cache(2, G, S, D, N, BF, gpu_device, 88), torch.tensor([5, 40], device=gpu_device)
+    qkv = torch.randn(2, 3, (H + 2 * G) * D, generator=torch.Generator().manual_seed(89)).to(BF).to(gpu_device)
+    want = expected_append(qkv, cos, sin, pos, cache, H, None, None, None)
+    with torch.inference_mode():
+        q = ops.kv_cache_paged_append(qkv, cos, sin, pos, cache, H)
+        o = ops.attention_paged(q, cache, pos)
+    assert torch.equal(q, want[0]) and torch.equal(cache.k, want[1]) and torch.equal(cache.v, want[2])
+    check(o, expected_attention(q, cache, pos))
+
+
+def test_sequences_of_one_table_row(gpu_device):
+    """Every sequence over the same pages: a table whose rows are one row."""
+    B, T, H, G, D, S, N = 4, 2, 4, 2, 64, 16, 9
+    cache = make_cache(1, G, S, D, N, BF, gpu_device, 90)
+    q, pos = queries(B, T, H, D, BF, gpu_device, 91), torch.tensor([3, 140, 77, 16], device=gpu_device)
+    o = ops.attention_paged(q, cache._replace(table=cache.table.expand(B, N)), pos)
+    assert torch.equal(o, ops.attention_paged(q, cache._replace(table=cache.table.repeat(B, 1)), pos))
+    check(o, expected_attention(q, cache._replace(table=cache.table.repeat(B, 1)), pos))
