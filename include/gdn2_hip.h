@@ -370,7 +370,8 @@ int gdn2_kv_cache_q4_load(const void *k_codes, const void *k_meta, const void *v
  * channels of n are rotated pair by pair (2 i, 2 i + 1) by row pos of cos, sin [table_rows][pairs]
  * (float32); pos at b pos_stride_b + t pos_stride_t (NULL: t).  Writes q [B, T, G R, D]
  * and k [B, T, G, D] in io_dtype (f32, bf16, fp16), rounded once; a token whose position lies
- * outside the tables gives zeros.  D a multiple of 8 up to 256.
+ * outside the tables gives zeros.  D a multiple of 8 up to 256, G (R + 2) up to 65535, and B T ceil(G (R + 2) / n)
+ * under 2^26, where n = 128 / (D / 8 rounded up to a power of two).
  * _bwd: from dq, dk, dv the gradient dqkv [B, T, G (R + 2) D] (contiguous; dv copied) and
  * those of the weights (their dtype), summed in a fixed order; no gradient passes through a
  * token whose position lies outside.  workspace (only with weights): _workspace_size() bytes,

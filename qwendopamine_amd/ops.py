@@ -2008,7 +2008,8 @@ def qkv_norm_rope(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, n_hea
     the bits of the host's torch path).  The weights' gradients are summed in a fixed order: the
     same bits in every run.  In a HIP graph, capture the forward and backward together with no
     eager autograd graph of the same leaves alive, as torch asks of any captured backward.  Second
-    derivatives and forward-mode tangents are refused."""
+    derivatives and forward-mode tangents are refused.  Under 2^26 tokens, and as many times fewer as their
+    heads exceed 1024 channels in all."""
     name = "qkv_norm_rope"
     x, B, T, R, D = _qkv_rows(name, qkv, n_head, n_query_groups)
     _head_weights(name, q_weight, k_weight, D, qkv.dtype)
